@@ -579,6 +579,66 @@ typedef struct strata_hip_gated_add_args {
 
 int strata_hip_gated_add(const strata_hip_gated_add_args* args, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * AdamW over many tensors in one call (the optimizer step that follows the clipping of
+ * the gradients in training, train.py:1163-1170):
+ *   c = min(1, max_norm / (norm + 1e-6)) with norm the 2-norm of all gradients, or 1
+ *   g = c * grad,  m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,  t = ++*step
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v / (1 - beta2^t)) + eps)
+ * Each tensor has its own lr, weight_decay and types: parameter and gradient bf16 or f32; moments f32, or in
+ * 8 bits: exp_avg int8 codes c standing for scale * sign(c) (c / 127)^2, exp_avg_sq uint8
+ * codes for scale * ((c + 1) / 256)^2, one f32 scale for every 256 consecutive elements
+ * (the largest magnitude among them; ceil(n / 256) scales).  master: f32 weights that a bf16
+ * parameter is rounded from (they are read in the parameter's place), or NULL.
+ * max_norm > 0: *norm receives the norm (64-bit sums in an order fixed by the sizes); a
+ * norm that is not finite leaves every tensor and *step as they were.  max_norm <= 0: no
+ * clipping.  Tensors are contiguous and aligned to their elements (16-byte alignment of all
+ * of a tensor's arrays is the fast path); no two arrays that are written may overlap
+ * (STRATA_HIP_EINVAL).  `tensors` is a HOST array, read during the call; step, norm and
+ * workspace (strata_hip_adamw_workspace() doubles) are device memory.
+ * ------------------------------------------------------------------------- */
+typedef struct strata_hip_adamw_tensor {
+  void* param;
+  const void* grad;
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* exp_avg_scale;    /* 8-bit moments only */
+  float* exp_avg_sq_scale;
+  float* master;           /* or NULL */
+  int64_t n;               /* elements */
+  double lr;
+  double weight_decay;
+  int32_t param_dtype;     /* strata_hip_dtype */
+  int32_t grad_dtype;
+  int32_t state_bits;      /* 32 or 8 */
+  int32_t reserved;
+} strata_hip_adamw_tensor;
+
+typedef struct strata_hip_adamw_args {
+  const strata_hip_adamw_tensor* tensors; /* host array of `count` */
+  int64_t count;
+  int64_t* step;     /* steps done so far; counted up */
+  double* norm;      /* out, with max_norm > 0 */
+  double* workspace;
+  double beta1, beta2, eps, max_norm;
+} strata_hip_adamw_args;
+
+int64_t strata_hip_adamw_workspace(const strata_hip_adamw_tensor* tensors, int64_t count);
+int strata_hip_adamw_step(const strata_hip_adamw_args* args, void* stream);
+
+/* out[i] = what code i of an 8-bit moment stands for (see strata_hip_adamw_step), f32;
+ * is_signed: 1 for exp_avg codes, 0 for exp_avg_sq codes.  codes 4-byte, out 16-byte aligned. */
+typedef struct strata_hip_adamw_values_args {
+  const void* codes;
+  const float* scales;
+  float* out;
+  int64_t n;
+  int32_t is_signed;
+  int32_t reserved;
+} strata_hip_adamw_values_args;
+
+int strata_hip_adamw_state_values(const strata_hip_adamw_values_args* args, void* stream);
+
 int strata_hip_abi_version(void);
 
 #ifdef __cplusplus

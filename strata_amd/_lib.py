@@ -330,6 +330,50 @@ class StateUpdateArgs(ctypes.Structure):
     ]
 
 
+class AdamwTensor(ctypes.Structure):
+    _fields_ = [
+        ("param", ctypes.c_void_p),
+        ("grad", ctypes.c_void_p),
+        ("exp_avg", ctypes.c_void_p),
+        ("exp_avg_sq", ctypes.c_void_p),
+        ("exp_avg_scale", ctypes.c_void_p),
+        ("exp_avg_sq_scale", ctypes.c_void_p),
+        ("master", ctypes.c_void_p),
+        ("n", ctypes.c_int64),
+        ("lr", ctypes.c_double),
+        ("weight_decay", ctypes.c_double),
+        ("param_dtype", ctypes.c_int32),
+        ("grad_dtype", ctypes.c_int32),
+        ("state_bits", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class AdamwArgs(ctypes.Structure):
+    _fields_ = [
+        ("tensors", ctypes.POINTER(AdamwTensor)),
+        ("count", ctypes.c_int64),
+        ("step", ctypes.c_void_p),
+        ("norm", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("beta1", ctypes.c_double),
+        ("beta2", ctypes.c_double),
+        ("eps", ctypes.c_double),
+        ("max_norm", ctypes.c_double),
+    ]
+
+
+class AdamwValuesArgs(ctypes.Structure):
+    _fields_ = [
+        ("codes", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("n", ctypes.c_int64),
+        ("is_signed", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
 EXPORTS = {
     "strata_hip_na3d_fwd": ([ctypes.POINTER(Na3dArgs), ctypes.c_void_p], ctypes.c_int),
     "strata_hip_na3d_fwd_rope_q": (
@@ -359,6 +403,9 @@ EXPORTS = {
     "strata_hip_upsample_dw_gelu": ([ctypes.POINTER(UpsampleDwGeluArgs), ctypes.c_void_p], ctypes.c_int),
     "strata_hip_layer_norm_modulate": ([ctypes.POINTER(LayerNormModulateArgs), ctypes.c_void_p], ctypes.c_int),
     "strata_hip_gated_add": ([ctypes.POINTER(GatedAddArgs), ctypes.c_void_p], ctypes.c_int),
+    "strata_hip_adamw_workspace": ([ctypes.POINTER(AdamwTensor), ctypes.c_int64], ctypes.c_int64),
+    "strata_hip_adamw_step": ([ctypes.POINTER(AdamwArgs), ctypes.c_void_p], ctypes.c_int),
+    "strata_hip_adamw_state_values": ([ctypes.POINTER(AdamwValuesArgs), ctypes.c_void_p], ctypes.c_int),
     "strata_hip_last_error": ([], ctypes.c_char_p),
     "strata_hip_abi_version": ([], ctypes.c_int),
 }

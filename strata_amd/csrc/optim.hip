@@ -1,0 +1,574 @@
+// AdamW over many tensors for gfx950, with the clipping of the gradients by their
+// global norm and moments held in 32 or in 8 bits.
+//
+//   c = min(1, max_norm / (|all gradients| + 1e-6)),  g <- c g
+//   m <- b1 m + (1 - b1) g        v <- b2 v + (1 - b2) g^2        t <- t + 1
+//   p <- p (1 - lr decay) - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)
+//
+// 8-bit moments: 256 consecutive elements share one fp32 scale each for m and v, the
+// largest magnitude among them.  A code stands for
+//   m = scale * sign(c) (c / 127)^2, c in -127 .. 127      v = scale * ((c + 1) / 256)^2, c in 0 .. 255
+// and is the nearest one in the root's domain: the quadratic spacing keeps 2 to 3
+// digits of values down to 1e-4 of their block's largest, and v, which divides, is never
+// below 1.5e-5 of it.  Decays and sums run in 64 bits there (v_fma_f64 issues at the
+// rate of v_fma_f32 here), so a code does not depend on how 32-bit sums round: beside a
+// border between two codes one such rounding moves the state by a whole code.  The
+// norm's sum of squares runs in 64 bits too, in an order fixed by the sizes.
+//
+// Bound by memory.  The tensors' addresses travel in the launch's arguments, so nothing
+// is kept between calls; the step count lives on the device, so a captured step counts on.
+#include <algorithm>
+#include <cmath>
+#include <new>
+#include <vector>
+
+#include "common.h"
+
+namespace strata {
+
+constexpr int AW_BLOCK = 256;    // elements per 8-bit scale
+constexpr int AW_CHUNK = 4096;   // elements per workgroup of the step
+constexpr int AW_SUM = 16384;    // elements per workgroup of the sum of squares
+constexpr int AW_HEAD = 8;       // doubles before the partial sums
+constexpr int AW_PER = 48;       // tensors per launch: 80 bytes each in 4 KiB of arguments
+enum { AW_P32 = 1, AW_G32 = 2, AW_Q8 = 4, AW_ALIGNED = 8 };
+
+struct AwTensor {
+  void* p;
+  const void* g;
+  void* m;
+  void* v;
+  float* ms;
+  float* vs;
+  float* master;
+  int64_t n;
+  float lr;
+  float decay;     // 1 - lr * weight_decay
+  uint32_t first;  // the tensor's first workgroup in the launch
+  uint32_t flags;
+};
+struct AwBatch {
+  AwTensor t[AW_PER];
+  int count;
+  float eps;
+  double b1, b2;
+  const double* head;    // what aw_head_kernel left, see there
+};
+struct SumBatch {
+  const void* g[3 * AW_PER];
+  int64_t n[3 * AW_PER];
+  uint32_t first[3 * AW_PER];
+  uint32_t wide[3 * AW_PER];  // 1: fp32, 0: bf16; 2: 16-byte aligned
+  int count;
+  double* part;
+};
+static_assert(sizeof(AwBatch) <= 4096 && sizeof(SumBatch) <= 4096, "kernel arguments");
+
+// Last entry whose first workgroup is at or before `wg`.
+template <typename F>
+__device__ __forceinline__ int find_entry(int count, uint32_t wg, F first) {
+  int lo = 0, hi = count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (first(mid) <= wg) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+// ---- sum of squares: one 64-bit partial per AW_SUM elements ----
+__global__ __launch_bounds__(256) void aw_sum_kernel(SumBatch b) {
+  const uint32_t wg = blockIdx.x;
+  const int e = find_entry(b.count, wg, [&](int i) { return b.first[i]; });
+  const int64_t i0 = (int64_t)(wg - b.first[e]) * AW_SUM, i1 = min(i0 + AW_SUM, b.n[e]);
+  const uint32_t wide = b.wide[e];
+  const int tid = threadIdx.x;
+  double s = 0.;
+  if (wide & 1) {
+    const float* g = (const float*)b.g[e];
+    if ((wide & 2) && i1 - i0 == AW_SUM) {
+#pragma unroll 8
+      for (int k = 0; k < AW_SUM / 1024; ++k) {
+        const f32x4 v = *(const f32x4*)(g + i0 + 1024 * k + 4 * tid);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s = fma((double)v[j], (double)v[j], s);
+      }
+    } else {
+      for (int64_t i = i0 + tid; i < i1; i += 256) s = fma((double)g[i], (double)g[i], s);
+    }
+  } else {
+    const bf16* g = (const bf16*)b.g[e];
+    if ((wide & 2) && i1 - i0 == AW_SUM) {
+#pragma unroll 8
+      for (int k = 0; k < AW_SUM / 2048; ++k) {
+        const u32x4 v = *(const u32x4*)(g + i0 + 2048 * k + 8 * tid);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const double lo = bf16_lo(v[j]), hi = bf16_hi(v[j]);
+          s = fma(lo, lo, s);
+          s = fma(hi, hi, s);
+        }
+      }
+    } else {
+      for (int64_t i = i0 + tid; i < i1; i += 256) {
+        const double x = (float)g[i];
+        s = fma(x, x, s);
+      }
+    }
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
+  __shared__ double red[4];
+  if ((tid & 63) == 0) red[tid >> 6] = s;
+  __syncthreads();
+  if (tid == 0) b.part[wg] = ((red[0] + red[1]) + red[2]) + red[3];
+}
+
+// ---- what every element shares: head[0] the factor c, [1] 1 / (1 - b1^t),
+// [2] 1 / sqrt(1 - b2^t), [3] 1 where the step is left out (a norm that is not finite).
+// One workgroup; the partial sums in a fixed order.
+__global__ __launch_bounds__(1024) void aw_head_kernel(double* head, const double* part, int64_t parts, int64_t* step,
+                                                       double* norm, double max_norm, double b1, double b2) {
+  __shared__ double red[16];
+  const int tid = threadIdx.x;
+  double c = 1.;
+  bool skip = false;
+  if (norm) {
+    double s = 0.;
+    for (int64_t i = tid; i < parts; i += 1024) s += part[i];
+#pragma unroll
+    for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
+    if ((tid & 63) == 0) red[tid >> 6] = s;
+    __syncthreads();
+    if (tid == 0) {
+      for (int k = 1; k < 16; ++k) s += red[k];
+      const double nrm = sqrt(s);
+      *norm = nrm;
+      skip = !(nrm < __builtin_inf());
+      c = fmin(1., max_norm / (nrm + 1e-6));
+    }
+  }
+  if (tid == 0) {
+    const int64_t t = *step + (skip ? 0 : 1);
+    *step = t;
+    head[0] = c;
+    head[1] = 1. / (1. - pow(b1, (double)t));
+    head[2] = 1. / sqrt(1. - pow(b2, (double)t));
+    head[3] = skip ? 1. : 0.;
+  }
+}
+
+// ---- the step ----
+struct AwShared {
+  float c, rate, rbc2, eps, decay, b1, b2, omb1, omb2;
+  double dc, db1, db2, domb1, domb2;
+};
+
+__device__ __forceinline__ float aw_update(const AwShared& s, float p, float m, float v) {
+  const float denom = fmaf(__builtin_sqrtf(v), s.rbc2, s.eps);
+  return fmaf(p, s.decay, -(s.rate * m) / denom);
+}
+
+__device__ __forceinline__ float load1(const void* p, int64_t i, bool wide) {
+  return wide ? ((const float*)p)[i] : (float)((const bf16*)p)[i];
+}
+
+// Four consecutive elements from a 16-byte (fp32) or 8-byte (bf16) run.
+__device__ __forceinline__ f32x4 load4(const void* p, int64_t i, bool wide) {
+  if (wide) return *(const f32x4*)((const float*)p + i);
+  const u32x2 w = *(const u32x2*)((const bf16*)p + i);
+  return (f32x4){bf16_lo(w[0]), bf16_hi(w[0]), bf16_lo(w[1]), bf16_hi(w[1])};
+}
+__device__ __forceinline__ void store4(void* p, int64_t i, bool wide, f32x4 v) {
+  if (wide) *(f32x4*)((float*)p + i) = v;
+  else *(u32x2*)((bf16*)p + i) = (u32x2){pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+}
+
+// 32-bit moments: 256 threads x 4 elements x 4 rounds.
+template <bool P32, bool G32, bool MASTER>
+__device__ __forceinline__ void aw_chunk32(const AwTensor& t, const AwShared& s, int64_t i0, int tid) {
+  float* m = (float*)t.m;
+  float* v = (float*)t.v;
+  auto one = [&](float g, float& mm, float& vv, float pp) {
+    g *= s.c;
+    mm = fmaf(s.omb1, g, s.b1 * mm);
+    vv = fmaf(s.omb2 * g, g, s.b2 * vv);
+    return aw_update(s, pp, mm, vv);
+  };
+  if ((t.flags & AW_ALIGNED) && i0 + AW_CHUNK <= t.n) {
+    f32x4 g[4], mm[4], vv[4], pp[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int64_t i = i0 + 1024 * k + 4 * tid;
+      g[k] = load4(t.g, i, G32);
+      mm[k] = *(const f32x4*)(m + i);
+      vv[k] = *(const f32x4*)(v + i);
+      pp[k] = MASTER ? *(const f32x4*)(t.master + i) : load4(t.p, i, P32);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int64_t i = i0 + 1024 * k + 4 * tid;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float a = mm[k][e], b = vv[k][e];
+        pp[k][e] = one(g[k][e], a, b, pp[k][e]);
+        mm[k][e] = a;
+        vv[k][e] = b;
+      }
+      *(f32x4*)(m + i) = mm[k];
+      *(f32x4*)(v + i) = vv[k];
+      if (MASTER) *(f32x4*)(t.master + i) = pp[k];
+      store4(t.p, i, P32, pp[k]);
+    }
+    return;
+  }
+  const int64_t i1 = min(i0 + AW_CHUNK, t.n);
+  for (int64_t i = i0 + tid; i < i1; i += 256) {
+    float a = m[i], b = v[i];
+    const float p = one(load1(t.g, i, G32), a, b, MASTER ? t.master[i] : load1(t.p, i, P32));
+    m[i] = a;
+    v[i] = b;
+    if (MASTER) t.master[i] = p;
+    if (P32) ((float*)t.p)[i] = p;
+    else ((bf16*)t.p)[i] = (bf16)p;
+  }
+}
+
+__device__ __forceinline__ double aw_value_m(int c, double scale) {
+  const double r = (double)c * (1. / 127.);
+  return (c < 0 ? -(r * r) : r * r) * scale;
+}
+__device__ __forceinline__ double aw_value_v(int c, double scale) {
+  const double r = (double)(c + 1) * (1. / 256.);
+  return r * r * scale;
+}
+// The code nearest to steps * sqrt(x / scale): from 32 bits, then held to its borders
+// (k +- 1/2)^2 scale in 64.
+__device__ __forceinline__ int aw_code(double x, float scale, float inv, float steps, int lo, int hi) {
+  int k = (int)rintf(steps * __builtin_sqrtf((float)x * inv));
+  k = min(max(k, lo), hi);
+  const double q = x * ((double)steps * (double)steps), sc = (double)scale;
+  const double up = (double)k + .5, dn = (double)k - .5;
+  if (k < hi && q > up * up * sc) ++k;
+  else if (k > lo && q < dn * dn * sc) --k;
+  return k;
+}
+
+// The larger of two magnitudes; one that is no number stays (the block's scale then says so).
+__device__ __forceinline__ float aw_max(float a, float b) { return b > a || b != b ? b : a; }
+
+// 8-bit moments: 16 lanes take a block of 256, 16 consecutive elements each.
+template <bool P32, bool G32, bool MASTER>
+__device__ __forceinline__ void aw_chunk8(const AwTensor& t, const AwShared& s, int64_t i0, int tid) {
+  const int64_t i = i0 + 16 * tid;
+  const int64_t blk = i / AW_BLOCK;
+  if (i0 + (tid / 16) * AW_BLOCK >= t.n) return;  // whole groups of 16 lanes leave
+  const int left = (int)min((int64_t)16, t.n - i);  // elements of this lane (0 or less: none)
+  const bool vec = (t.flags & AW_ALIGNED) && left == 16;
+  int8_t* mc = (int8_t*)t.m;
+  uint8_t* vc = (uint8_t*)t.v;
+  float g[16], p[16];
+  int cm[16], cv[16];
+  if (vec) {
+    const u32x4 a = *(const u32x4*)(mc + i), b = *(const u32x4*)(vc + i);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const f32x4 x = load4(t.g, i + 4 * k, G32), y = MASTER ? *(const f32x4*)(t.master + i + 4 * k) : load4(t.p, i + 4 * k, P32);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        g[4 * k + e] = x[e];
+        p[4 * k + e] = y[e];
+        cm[4 * k + e] = (int)(int8_t)(a[k] >> (8 * e));
+        cv[4 * k + e] = (int)((b[k] >> (8 * e)) & 255u);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const bool in = k < left;
+      g[k] = in ? load1(t.g, i + k, G32) : 0.f;
+      p[k] = in ? (MASTER ? t.master[i + k] : load1(t.p, i + k, P32)) : 0.f;
+      cm[k] = in ? mc[i + k] : 0;
+      cv[k] = in ? vc[i + k] : 0;
+    }
+  }
+  const double sm = (double)t.ms[blk], sv = (double)t.vs[blk];
+  double m[16], v[16];
+  float am = 0.f, av = 0.f;
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const double gd = (double)g[k] * s.dc;
+    m[k] = fma(s.domb1, gd, s.db1 * aw_value_m(cm[k], sm));
+    v[k] = fma(s.domb2 * gd, gd, s.db2 * aw_value_v(cv[k], sv));
+    if (k < left) {  // rounding keeps the order: the largest rounded is the largest, rounded
+      am = aw_max(am, fabsf((float)m[k]));
+      av = aw_max(av, (float)v[k]);
+    }
+    p[k] = aw_update(s, p[k], (float)m[k], (float)v[k]);
+  }
+#pragma unroll
+  for (int d = 1; d < 16; d <<= 1) {
+    am = aw_max(am, __shfl_xor(am, d));
+    av = aw_max(av, __shfl_xor(av, d));
+  }
+  const float im = am > 0.f ? 1.f / am : 0.f, iv = av > 0.f ? 1.f / av : 0.f;
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const int c = aw_code(fabs(m[k]), am, im, 127.f, 0, 127);
+    cm[k] = m[k] < 0. ? -c : c;
+    cv[k] = aw_code(v[k], av, iv, 256.f, 1, 256) - 1;
+  }
+  if ((tid & 15) == 0) {
+    t.ms[blk] = am;
+    t.vs[blk] = av;
+  }
+  if (vec) {
+    u32x4 a, b;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      a[k] = b[k] = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        a[k] |= (uint32_t)(cm[4 * k + e] & 255) << (8 * e);
+        b[k] |= (uint32_t)cv[4 * k + e] << (8 * e);
+      }
+      const f32x4 y = {p[4 * k], p[4 * k + 1], p[4 * k + 2], p[4 * k + 3]};
+      if (MASTER) *(f32x4*)(t.master + i + 4 * k) = y;
+      store4(t.p, i + 4 * k, P32, y);
+    }
+    *(u32x4*)(mc + i) = a;
+    *(u32x4*)(vc + i) = b;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      if (k >= left) continue;
+      mc[i + k] = (int8_t)cm[k];
+      vc[i + k] = (uint8_t)cv[k];
+      if (MASTER) t.master[i + k] = p[k];
+      if (P32) ((float*)t.p)[i + k] = p[k];
+      else ((bf16*)t.p)[i + k] = (bf16)p[k];
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void aw_step_kernel(AwBatch b) {
+  const uint32_t wg = blockIdx.x;
+  if (b.head[3] != 0.) return;
+  const int e = find_entry(b.count, wg, [&](int i) { return b.t[i].first; });
+  const AwTensor t = b.t[e];
+  AwShared s;
+  s.dc = b.head[0];
+  s.c = (float)s.dc;
+  s.rate = t.lr * (float)b.head[1];
+  s.rbc2 = (float)b.head[2];
+  s.eps = b.eps;
+  s.decay = t.decay;
+  s.db1 = b.b1;
+  s.db2 = b.b2;
+  s.domb1 = 1. - b.b1;
+  s.domb2 = 1. - b.b2;
+  s.b1 = (float)s.db1;
+  s.b2 = (float)s.db2;
+  s.omb1 = (float)s.domb1;
+  s.omb2 = (float)s.domb2;
+  const int64_t i0 = (int64_t)(wg - t.first) * AW_CHUNK;
+  const int tid = threadIdx.x;
+  const bool q8 = t.flags & AW_Q8, p32 = t.flags & AW_P32, g32 = t.flags & AW_G32;
+  auto go = [&](auto P, auto G, auto M) {
+    constexpr bool p_ = decltype(P)::value, g_ = decltype(G)::value, m_ = decltype(M)::value;
+    if (q8) aw_chunk8<p_, g_, m_>(t, s, i0, tid);
+    else aw_chunk32<p_, g_, m_>(t, s, i0, tid);
+  };
+  if (p32) {
+    if (g32) go(std::true_type{}, std::true_type{}, std::false_type{});
+    else go(std::true_type{}, std::false_type{}, std::false_type{});
+  } else if (t.master) {
+    if (g32) go(std::false_type{}, std::true_type{}, std::true_type{});
+    else go(std::false_type{}, std::false_type{}, std::true_type{});
+  } else {
+    if (g32) go(std::false_type{}, std::true_type{}, std::false_type{});
+    else go(std::false_type{}, std::false_type{}, std::false_type{});
+  }
+}
+
+// ---- the values that 8-bit states stand for ----
+__global__ __launch_bounds__(256) void aw_values_kernel(const uint8_t* __restrict__ codes, const float* __restrict__ scales,
+                                                        float* __restrict__ out, int64_t n, int is_signed) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  const double sc = (double)scales[i / AW_BLOCK];
+  uint32_t w = 0;
+  const int left = (int)min((int64_t)4, n - i);
+  if (left == 4) w = *(const uint32_t*)(codes + i);
+  else
+    for (int e = 0; e < left; ++e) w |= (uint32_t)codes[i + e] << (8 * e);
+  f32x4 o;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int c = (w >> (8 * e)) & 255;
+    o[e] = (float)(is_signed ? aw_value_m((int)(int8_t)c, sc) : aw_value_v(c, sc));
+  }
+  if (left == 4) *(f32x4*)(out + i) = o;
+  else
+    for (int e = 0; e < left; ++e) out[i + e] = o[e];
+}
+
+static int64_t aw_parts(const strata_hip_adamw_tensor* t, int64_t count) {
+  int64_t parts = 0;
+  for (int64_t i = 0; i < count; ++i) parts += t[i].n > 0 ? (t[i].n + AW_SUM - 1) / AW_SUM : 0;
+  return parts;
+}
+
+static int aw_check(const strata_hip_adamw_args* a) {
+  if (!a) return fail(STRATA_HIP_EINVAL, "adamw_step: null args");
+  if (a->count < 0 || (a->count > 0 && !a->tensors)) return fail(STRATA_HIP_EINVAL, "adamw_step: bad tensor list");
+  if (!a->step || !a->workspace || ((uintptr_t)a->step & 7) || ((uintptr_t)a->workspace & 7))
+    return fail(STRATA_HIP_EINVAL, "adamw_step: step and workspace must be given, 8-byte aligned");
+  if (!(a->beta1 >= 0. && a->beta1 < 1. && a->beta2 >= 0. && a->beta2 < 1.))
+    return fail(STRATA_HIP_EINVAL, "adamw_step: betas must lie in [0, 1)");
+  if (!(a->eps >= 0.) || !std::isfinite(a->eps))
+    return fail(STRATA_HIP_EINVAL, "adamw_step: eps must be finite and not negative");
+  if (!std::isfinite(a->max_norm) || (a->max_norm > 0. && (!a->norm || ((uintptr_t)a->norm & 7))))
+    return fail(STRATA_HIP_EINVAL, "adamw_step: max_norm must be finite and norm given with it, 8-byte aligned");
+  std::vector<std::pair<uintptr_t, uintptr_t>> written;
+  written.reserve((size_t)a->count * 6);
+  int64_t chunks = 0;
+  for (int64_t i = 0; i < a->count; ++i) {
+    const strata_hip_adamw_tensor& t = a->tensors[i];
+    if (t.n < 0) return fail(STRATA_HIP_EINVAL, "adamw_step: negative size");
+    if (t.n == 0) continue;
+    if (!std::isfinite(t.lr) || !std::isfinite(t.weight_decay))
+      return fail(STRATA_HIP_EINVAL, "adamw_step: lr and weight_decay must be finite");
+    const bool p32 = t.param_dtype == STRATA_HIP_F32, g32 = t.grad_dtype == STRATA_HIP_F32;
+    if ((!p32 && t.param_dtype != STRATA_HIP_BF16) || (!g32 && t.grad_dtype != STRATA_HIP_BF16))
+      return fail(STRATA_HIP_EINVAL, "adamw_step: parameters and gradients must be bf16 or f32");
+    if (t.state_bits != 32 && t.state_bits != 8) return fail(STRATA_HIP_EINVAL, "adamw_step: state_bits must be 32 or 8");
+    if (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq) return fail(STRATA_HIP_EINVAL, "adamw_step: null tensor");
+    if (t.state_bits == 8 && (!t.exp_avg_scale || !t.exp_avg_sq_scale))
+      return fail(STRATA_HIP_EINVAL, "adamw_step: 8-bit states need their scales");
+    if (p32 && t.master) return fail(STRATA_HIP_EINVAL, "adamw_step: master weights are for bf16 parameters");
+    const uintptr_t ps = p32 ? 4 : 2, gs = g32 ? 4 : 2, ss = t.state_bits / 8;
+    if (((uintptr_t)t.param % ps) || ((uintptr_t)t.grad % gs) || ((uintptr_t)t.exp_avg % ss) || ((uintptr_t)t.exp_avg_sq % ss) ||
+        ((uintptr_t)t.master % 4) || ((uintptr_t)t.exp_avg_scale % 4) || ((uintptr_t)t.exp_avg_sq_scale % 4))
+      return fail(STRATA_HIP_EINVAL, "adamw_step: a tensor is not aligned to its elements");
+    auto add = [&](const void* p, uintptr_t bytes) { written.emplace_back((uintptr_t)p, (uintptr_t)p + bytes); };
+    add(t.param, ps * t.n);
+    add(t.exp_avg, ss * t.n);
+    add(t.exp_avg_sq, ss * t.n);
+    if (t.master) add(t.master, 4 * t.n);
+    if (t.state_bits == 8) {
+      add(t.exp_avg_scale, 4 * ((t.n + AW_BLOCK - 1) / AW_BLOCK));
+      add(t.exp_avg_sq_scale, 4 * ((t.n + AW_BLOCK - 1) / AW_BLOCK));
+    }
+    chunks += (t.n + AW_CHUNK - 1) / AW_CHUNK;
+  }
+  if (chunks > 0x7fffffff) return fail(STRATA_HIP_EUNSUPPORTED, "adamw_step: too many elements for one call");
+  std::sort(written.begin(), written.end());
+  for (size_t i = 1; i < written.size(); ++i)
+    if (written[i].first < written[i - 1].second)
+      return fail(STRATA_HIP_EINVAL, "adamw_step: two of the tensors to update overlap");
+  return STRATA_HIP_OK;
+}
+
+static int aw_launch(const strata_hip_adamw_args* a, hipStream_t st) {
+  if (const int rc = aw_check(a)) return rc;
+  double* part = a->workspace + AW_HEAD;
+  int64_t parts = 0;
+  if (a->max_norm > 0.) {
+    SumBatch b;
+    b.count = 0;
+    uint32_t wgs = 0;
+    auto flush = [&]() -> int {
+      if (!b.count) return STRATA_HIP_OK;
+      b.part = part + parts;
+      hipLaunchKernelGGL(aw_sum_kernel, dim3(wgs), dim3(256), 0, st, b);
+      parts += wgs;
+      b.count = 0;
+      wgs = 0;
+      return check_launch("adamw sum of squares");
+    };
+    for (int64_t i = 0; i < a->count; ++i) {
+      const strata_hip_adamw_tensor& t = a->tensors[i];
+      if (t.n == 0) continue;
+      const int k = b.count++;
+      b.g[k] = t.grad;
+      b.n[k] = t.n;
+      b.first[k] = wgs;
+      b.wide[k] = (t.grad_dtype == STRATA_HIP_F32 ? 1u : 0u) | (((uintptr_t)t.grad & 15) ? 0u : 2u);
+      wgs += (uint32_t)((t.n + AW_SUM - 1) / AW_SUM);
+      if (b.count == 3 * AW_PER)
+        if (const int rc = flush()) return rc;
+    }
+    if (const int rc = flush()) return rc;
+  }
+  hipLaunchKernelGGL(aw_head_kernel, dim3(1), dim3(1024), 0, st, a->workspace, part, parts, a->step,
+                     a->max_norm > 0. ? a->norm : nullptr, a->max_norm, a->beta1, a->beta2);
+  if (const int rc = check_launch("adamw head")) return rc;
+  AwBatch b;
+  b.count = 0;
+  b.eps = (float)a->eps;
+  b.b1 = a->beta1;
+  b.b2 = a->beta2;
+  b.head = a->workspace;
+  uint32_t wgs = 0;
+  auto flush = [&]() -> int {
+    if (!b.count) return STRATA_HIP_OK;
+    hipLaunchKernelGGL(aw_step_kernel, dim3(wgs), dim3(256), 0, st, b);
+    b.count = 0;
+    wgs = 0;
+    return check_launch("adamw step");
+  };
+  for (int64_t i = 0; i < a->count; ++i) {
+    const strata_hip_adamw_tensor& t = a->tensors[i];
+    if (t.n == 0) continue;
+    AwTensor& o = b.t[b.count++];
+    o.p = t.param;
+    o.g = t.grad;
+    o.m = t.exp_avg;
+    o.v = t.exp_avg_sq;
+    o.ms = t.exp_avg_scale;
+    o.vs = t.exp_avg_sq_scale;
+    o.master = t.master;
+    o.n = t.n;
+    o.lr = (float)t.lr;
+    o.decay = (float)(1. - t.lr * t.weight_decay);
+    o.first = wgs;
+    const uintptr_t all = (uintptr_t)t.param | (uintptr_t)t.grad | (uintptr_t)t.exp_avg | (uintptr_t)t.exp_avg_sq | (uintptr_t)t.master;
+    o.flags = (t.param_dtype == STRATA_HIP_F32 ? AW_P32 : 0) | (t.grad_dtype == STRATA_HIP_F32 ? AW_G32 : 0) |
+              (t.state_bits == 8 ? AW_Q8 : 0) | ((all & 15) ? 0 : AW_ALIGNED);
+    wgs += (uint32_t)((t.n + AW_CHUNK - 1) / AW_CHUNK);
+    if (b.count == AW_PER)
+      if (const int rc = flush()) return rc;
+  }
+  return flush();
+}
+
+}  // namespace strata
+
+extern "C" int64_t strata_hip_adamw_workspace(const strata_hip_adamw_tensor* tensors, int64_t count) {
+  if (!tensors || count <= 0) return strata::AW_HEAD;
+  return strata::AW_HEAD + strata::aw_parts(tensors, count);
+}
+
+extern "C" int strata_hip_adamw_step(const strata_hip_adamw_args* a, void* stream) {
+  try {
+    return strata::aw_launch(a, (hipStream_t)stream);
+  } catch (const std::bad_alloc&) {
+    return strata::fail(STRATA_HIP_EUNSUPPORTED, "adamw_step: out of host memory");
+  }
+}
+
+extern "C" int strata_hip_adamw_state_values(const strata_hip_adamw_values_args* a, void* stream) {
+  using namespace strata;
+  if (!a) return fail(STRATA_HIP_EINVAL, "adamw_state_values: null args");
+  if (a->n < 0) return fail(STRATA_HIP_EINVAL, "adamw_state_values: negative size");
+  if (a->n == 0) return STRATA_HIP_OK;
+  if (!a->codes || !a->scales || !a->out) return fail(STRATA_HIP_EINVAL, "adamw_state_values: null pointer");
+  if (((uintptr_t)a->codes & 3) || ((uintptr_t)a->scales & 3) || ((uintptr_t)a->out & 15))
+    return fail(STRATA_HIP_EINVAL, "adamw_state_values: codes must be 4-byte, out 16-byte aligned");
+  const int64_t wgs = (a->n + 1023) / 1024;
+  if (wgs > 0x7fffffff) return fail(STRATA_HIP_EUNSUPPORTED, "adamw_state_values: too many elements for one call");
+  hipLaunchKernelGGL(aw_values_kernel, dim3((unsigned)wgs), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)a->codes,
+                     a->scales, a->out, a->n, a->is_signed);
+  return check_launch("adamw state values");
+}

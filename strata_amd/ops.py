@@ -43,6 +43,8 @@ __all__ = [
     "upsample_dw_gelu",
     "layer_norm_modulate",
     "gated_add",
+    "adamw_step",
+    "adamw_state_values",
 ]
 
 
@@ -1383,3 +1385,114 @@ def _(res, gate, y):
 
 
 gated_add.register_autograd(_no_backward("strata_hip::gated_add"))
+
+
+# ---------------------------------------------------------------------------
+# AdamW over many tensors
+# ---------------------------------------------------------------------------
+STATE_BLOCK = 256  # consecutive elements that share a scale of an 8-bit moment
+
+
+def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequence[Tensor],
+               exp_avg_sqs: Sequence[Tensor], step: Tensor, *, lr: float | Sequence[float] = 1e-3,
+               betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
+               weight_decay: float | Sequence[float] = 0.01, max_norm: Optional[float] = None,
+               masters: Optional[Sequence[Optional[Tensor]]] = None,
+               exp_avg_scales: Optional[Sequence[Optional[Tensor]]] = None,
+               exp_avg_sq_scales: Optional[Sequence[Optional[Tensor]]] = None) -> Optional[Tensor]:
+    """One AdamW step, in place, over many contiguous tensors of one GPU (the optimizer step and
+    the gradient clipping before it, train.py:1163-1170)::
+
+        g = grad * min(1, max_norm / (norm + 1e-6))       (norm: of all gradients together)
+        m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2
+        p = p (1 - lr weight_decay) - lr mh / (sqrt(vh) + eps),  mh = m / (1 - b1^t), vh = v / (1 - b2^t)
+
+    Each parameter and its gradient are bf16 or fp32.  Its moments are fp32 tensors, or int8 / uint8
+    codes with fp32 scales ``[ceil(numel / 256)]`` in ``exp_avg_scales`` / ``exp_avg_sq_scales``
+    (``adamw_state_values`` says what they stand for; zero codes and scales are zero moments).
+    ``masters``: fp32 weights (or None) that a bf16 parameter is rounded from.  ``step`` is an int64
+    tensor ``[1]`` on the GPU, counted up, so that a captured step counts on; ``lr`` and
+    ``weight_decay`` may be one number for every tensor.  With ``max_norm`` the norm is returned
+    (fp64 ``[1]``), and one that is not finite leaves everything as it was, ``step`` too."""
+    name = "adamw_step"
+    n = len(params)
+    lists = [params, grads, exp_avgs, exp_avg_sqs]
+    for opt in (masters, exp_avg_scales, exp_avg_sq_scales):
+        lists.append([None] * n if opt is None else opt)
+    if any(len(x) != n for x in lists):
+        raise ValueError(f"{name}: the lists must have one entry for each of the {n} parameters")
+    lrs = [float(lr)] * n if isinstance(lr, (int, float)) else [float(x) for x in lr]
+    wds = [float(weight_decay)] * n if isinstance(weight_decay, (int, float)) else [float(x) for x in weight_decay]
+    if len(lrs) != n or len(wds) != n:
+        raise ValueError(f"{name}: lr and weight_decay must be numbers or have one entry for each parameter")
+    _require_gpu(name, step, *[t for x in lists for t in x])
+    if step.dtype != torch.int64 or step.numel() != 1:
+        raise ValueError(f"{name}: step must be an int64 tensor [1]")
+    if max_norm is not None and not (0 < max_norm < math.inf):
+        raise ValueError(f"{name}: max_norm must be positive and finite")
+    table = (_lib.AdamwTensor * max(n, 1))()
+    written = [step]
+    for i, (p, g, m, v, w, ms, vs) in enumerate(zip(*lists)):
+        k = p.numel()
+        codes = m.dtype == torch.int8
+        for t, what, dtypes, size in ((p, "params", _ADAMW_FLOATS, k), (g, "grads", _ADAMW_FLOATS, k),
+                                      (m, "exp_avgs", (torch.int8,) if codes else _F32, k),
+                                      (v, "exp_avg_sqs", (torch.uint8,) if codes else _F32, k),
+                                      (w, "masters", _F32, k),
+                                      (ms, "exp_avg_scales", _F32, -(-k // STATE_BLOCK)),
+                                      (vs, "exp_avg_sq_scales", _F32, -(-k // STATE_BLOCK))):
+            if t is None:
+                continue
+            if t.dtype not in dtypes or t.numel() != size or not t.is_contiguous():
+                raise ValueError(f"{name}: {what}[{i}] must be contiguous, of {size} elements and one of {dtypes}, "
+                                 f"got {t.dtype} {tuple(t.shape)}")
+        if codes == (ms is None) or codes == (vs is None):
+            raise ValueError(f"{name}: 8-bit moments come with their scales, fp32 ones without (tensor {i})")
+        if w is not None and p.dtype != torch.bfloat16:
+            raise ValueError(f"{name}: masters[{i}] belongs to a bfloat16 parameter")
+        table[i] = (p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), ms.data_ptr() if codes else None,
+                    vs.data_ptr() if codes else None, w.data_ptr() if w is not None else None, k, lrs[i], wds[i],
+                    _lib.F32 if p.dtype == torch.float32 else _lib.BF16,
+                    _lib.F32 if g.dtype == torch.float32 else _lib.BF16, 8 if codes else 32, 0)
+        written += [t for t in (p, m, v, w, ms, vs) if t is not None]
+    ws = torch.empty(int(_lib.function("strata_hip_adamw_workspace")(table, n)), dtype=torch.float64, device=step.device)
+    norm = torch.empty(1, dtype=torch.float64, device=step.device) if max_norm is not None else None
+    a = _lib.AdamwArgs(table, n, step.data_ptr(), norm.data_ptr() if norm is not None else None, ws.data_ptr(),
+                       float(betas[0]), float(betas[1]), float(eps), float(max_norm or 0.0))
+    _launch("strata_hip_adamw_step", a, step)
+    torch.autograd.graph.increment_version([t for t in written if not t.is_inference()])
+    return norm
+
+
+_ADAMW_FLOATS = (torch.bfloat16, torch.float32)
+_F32 = (torch.float32,)
+
+
+@torch.library.custom_op("strata_hip::adamw_state_values", mutates_args=())
+def adamw_state_values(codes: Tensor, scales: Tensor) -> Tensor:
+    """The fp32 moments that ``adamw_step``'s 8-bit states stand for: ``scale * sign(c) (c / 127)^2``
+    for int8 codes (exp_avg), ``scale * ((c + 1) / 256)^2`` for uint8 codes (exp_avg_sq), one scale
+    for every 256 consecutive elements."""
+    name = "adamw_state_values"
+    _require_gpu(name, codes, scales)
+    if codes.dtype not in (torch.int8, torch.uint8) or scales.dtype != torch.float32:
+        raise ValueError(f"{name}: expected int8 or uint8 codes and float32 scales, got {codes.dtype}, {scales.dtype}")
+    n = codes.numel()
+    if scales.numel() != -(-n // STATE_BLOCK):
+        raise ValueError(f"{name}: {n} codes need {-(-n // STATE_BLOCK)} scales, got {scales.numel()}")
+    c, s = codes.contiguous(), scales.contiguous()
+    if c.data_ptr() % 4:
+        c = c.clone()
+    out = torch.empty(codes.shape, dtype=torch.float32, device=codes.device)
+    if n:
+        a = _lib.AdamwValuesArgs(c.data_ptr(), s.data_ptr(), out.data_ptr(), n, int(codes.dtype == torch.int8), 0)
+        _launch("strata_hip_adamw_state_values", a, codes)
+    return out
+
+
+@adamw_state_values.register_fake
+def _(codes, scales):
+    return torch.empty(codes.shape, dtype=torch.float32, device=codes.device)
+
+
+adamw_state_values.register_autograd(_no_backward("strata_hip::adamw_state_values"))
