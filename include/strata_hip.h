@@ -580,6 +580,128 @@ typedef struct strata_hip_gated_add_args {
 int strata_hip_gated_add(const strata_hip_gated_add_args* args, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Routing of tokens to experts (a sparse form of the block's Mlp,
+ * screamcast/checkpoint_compat.py:243-249; no counterpart in the reference).
+ *   s = softmax of the logits, or sigmoid;  key = s + bias, the logit itself where there is
+ *   neither a bias nor a group; of `groups` equal groups of experts the top_groups with the
+ *   largest sums of their two best keys stay (the lower of two equal groups)
+ *   index[t, i] = the top_k largest keys left in falling order (the lower expert of two equal
+ *   keys), -1 where none is left;  weights[t, i] = scale * s (/ sum of the chosen s), 0 with -1
+ * A logit or bias that is not finite masks its expert (s = 0, never chosen).  Scores and keys
+ * that decide (a bias or groups given) are held in 64 bits.  At most 512 experts, top_k 64.
+ * logits: [tokens, experts], row stride ld; weights, dweights: [tokens, top_k] of the
+ * logits' type; index: int32 [tokens, top_k]; dlogits: [tokens, experts] contiguous.
+ * _bwd: dlogits from dweights and the forward's index (weights is not read).
+ * ------------------------------------------------------------------------- */
+enum strata_hip_score { STRATA_HIP_SCORE_SOFTMAX = 0, STRATA_HIP_SCORE_SIGMOID = 1 };
+
+typedef struct strata_hip_expert_route_args {
+  const void* logits;
+  const float* bias;     /* [experts] or NULL; takes part in the choice, not in the weights */
+  void* weights;
+  int32_t* index;        /* out; in for _bwd */
+  const void* dweights;  /* _bwd only */
+  void* dlogits;         /* _bwd only */
+  int64_t tokens;
+  int64_t ld;
+  int32_t dtype;         /* strata_hip_dtype of logits, weights and their gradients */
+  int32_t experts;
+  int32_t top_k;
+  int32_t score;         /* strata_hip_score */
+  int32_t groups;        /* 1: none */
+  int32_t top_groups;
+  int32_t renormalize;   /* 1: weights divided by the sum of the chosen scores */
+  float scale;
+} strata_hip_expert_route_args;
+
+int strata_hip_expert_route(const strata_hip_expert_route_args* args, void* stream);
+int strata_hip_expert_route_bwd(const strata_hip_expert_route_args* args, void* stream);
+
+/* The order in which the experts' products take the chosen (token, slot) pairs: by expert,
+ * pairs of one expert in their own order.  An index outside [0, experts) drops its pair.
+ * index: [pairs].  Out: row_slot[r] the pair of row r ([pairs], rows past the last one stay
+ * as they were); slot_row[s] the row of pair s or -1; offsets[e] the first row of expert e,
+ * offsets[experts] the number of rows; tiles: [1 + 2 * (pairs / tile + experts)], the
+ * number of row tiles, then (expert, first row) of each: up to `tile` rows of one expert.
+ * workspace: strata_hip_expert_plan_workspace() int32 (NULL when that is 0). */
+typedef struct strata_hip_expert_plan_args {
+  const int32_t* index;
+  int32_t* row_slot;
+  int32_t* slot_row;
+  int32_t* offsets;
+  int32_t* tiles;
+  int32_t* workspace;
+  int64_t pairs;
+  int32_t experts;
+  int32_t tile;
+} strata_hip_expert_plan_args;
+
+int64_t strata_hip_expert_plan_workspace(int64_t pairs, int32_t experts);
+int strata_hip_expert_plan(const strata_hip_expert_plan_args* args, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * The chosen experts' MLPs, the block's Mlp (fc1 -> GELU(tanh) -> fc2,
+ * screamcast/checkpoint_compat.py:243-249) with weights of its own for each expert:
+ *   out[t] = residual[t] + sum over s of weights[t, s] (gelu(x[t] w1_e^T + b1_e) w2_e^T + b2_e)
+ * for the pairs (t, s) that the plan (strata_hip_expert_plan with tile =
+ * strata_hip_expert_tile(tokens * top_k, experts)) gives a row; e is the row's expert.
+ * x: [tokens, dim], row stride ldx; weights: [tokens, top_k]; w1 [experts, hidden, dim],
+ * b1 [experts, hidden] or NULL, w2 [experts, out_dim, hidden], b2 [experts, out_dim] or NULL,
+ * residual [tokens, out_dim] (row stride ldr) or NULL, out [tokens, out_dim]: bf16, contiguous
+ * where no stride is given, fp32 accumulation.  Widths multiples of 8, at most 32768; x and
+ * out under 2 GiB.  Workspaces, rows of the plan's order (rows past the last one stay as they
+ * were): h [pairs, hidden] bf16, y [pairs, out_dim] fp32, dact [pairs, hidden] bf16 or NULL:
+ * gelu' for a backward, which reads h, y and dact again.  x, w, h, y, dact, out, residual
+ * 16-byte aligned, b1, b2 8-byte.  The order of every sum is fixed by the sizes and the plan.
+ * ------------------------------------------------------------------------- */
+typedef struct strata_hip_expert_mlp_args {
+  const void* x;
+  const void* weights;
+  const int32_t* row_slot;
+  const int32_t* slot_row;
+  const int32_t* offsets;
+  const int32_t* tiles;
+  const void* w1;
+  const void* b1;
+  const void* w2;
+  const void* b2;
+  const void* residual;
+  void* out;
+  void* h;
+  void* dact;
+  float* y;
+  int64_t tokens, ldx, ldr;
+  int32_t top_k, experts, dim, hidden, out_dim, tile;
+} strata_hip_expert_mlp_args;
+
+int32_t strata_hip_expert_tile(int64_t pairs, int32_t experts);
+int strata_hip_expert_mlp(const strata_hip_expert_mlp_args* args, void* stream);
+
+/* Gradients of strata_hip_expert_mlp for dout [tokens, out_dim] bf16 contiguous; `fwd` as in the
+ * forward (out and residual are not read; the residual's gradient is dout).  Each of dx
+ * [tokens, dim], dweights [tokens, top_k], dw1, db1, dw2, db2 (the shapes of their weights, bf16)
+ * may be NULL, a weight's only with its bias's; a dropped pair's dweights and an
+ * unused expert's gradients are zero.  Workspaces in bf16: gs [pairs, out_dim] for dw2,
+ * gz [pairs, hidden] and w2t (w2's elements) for dx or dw1, dxs [pairs, dim] and w1t for dx. */
+typedef struct strata_hip_expert_mlp_bwd_args {
+  strata_hip_expert_mlp_args fwd;
+  const void* dout;
+  void* dx;
+  void* dweights;
+  void* dw1;
+  void* db1;
+  void* dw2;
+  void* db2;
+  void* gs;
+  void* gz;
+  void* dxs;
+  void* w1t;
+  void* w2t;
+} strata_hip_expert_mlp_bwd_args;
+
+int strata_hip_expert_mlp_bwd(const strata_hip_expert_mlp_bwd_args* args, void* stream);
+
+/* ---------------------------------------------------------------------------
  * AdamW over many tensors in one call (the optimizer step that follows the clipping of
  * the gradients in training, train.py:1163-1170):
  *   c = min(1, max_norm / (norm + 1e-6)) with norm the 2-norm of all gradients, or 1

@@ -34,6 +34,9 @@ ACT_SIGMOID_GRAD = 5
 RES_ADD = 0
 RES_MUL = 1
 
+SCORE_SOFTMAX = 0
+SCORE_SIGMOID = 1
+
 ROPE_HALF = 0
 ROPE_INTERLEAVED = 1
 
@@ -330,6 +333,53 @@ class StateUpdateArgs(ctypes.Structure):
     ]
 
 
+class ExpertRouteArgs(ctypes.Structure):
+    _fields_ = [
+        ("logits", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("weights", ctypes.c_void_p),
+        ("index", ctypes.c_void_p),
+        ("dweights", ctypes.c_void_p),
+        ("dlogits", ctypes.c_void_p),
+        ("tokens", ctypes.c_int64),
+        ("ld", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("experts", ctypes.c_int32),
+        ("top_k", ctypes.c_int32),
+        ("score", ctypes.c_int32),
+        ("groups", ctypes.c_int32),
+        ("top_groups", ctypes.c_int32),
+        ("renormalize", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+    ]
+
+
+class ExpertPlanArgs(ctypes.Structure):
+    _fields_ = [
+        ("index", ctypes.c_void_p),
+        ("row_slot", ctypes.c_void_p),
+        ("slot_row", ctypes.c_void_p),
+        ("offsets", ctypes.c_void_p),
+        ("tiles", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("pairs", ctypes.c_int64),
+        ("experts", ctypes.c_int32),
+        ("tile", ctypes.c_int32),
+    ]
+
+
+class ExpertMlpArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "weights", "row_slot", "slot_row", "offsets", "tiles", "w1", "b1", "w2",
+                                               "b2", "residual", "out", "h", "dact", "y")] + \
+        [(n, ctypes.c_int64) for n in ("tokens", "ldx", "ldr")] + \
+        [(n, ctypes.c_int32) for n in ("top_k", "experts", "dim", "hidden", "out_dim", "tile")]
+
+
+class ExpertMlpBwdArgs(ctypes.Structure):
+    _fields_ = [("fwd", ExpertMlpArgs)] + \
+        [(n, ctypes.c_void_p) for n in ("dout", "dx", "dweights", "dw1", "db1", "dw2", "db2", "gs", "gz", "dxs", "w1t", "w2t")]
+
+
 class AdamwTensor(ctypes.Structure):
     _fields_ = [
         ("param", ctypes.c_void_p),
@@ -403,6 +453,13 @@ EXPORTS = {
     "strata_hip_upsample_dw_gelu": ([ctypes.POINTER(UpsampleDwGeluArgs), ctypes.c_void_p], ctypes.c_int),
     "strata_hip_layer_norm_modulate": ([ctypes.POINTER(LayerNormModulateArgs), ctypes.c_void_p], ctypes.c_int),
     "strata_hip_gated_add": ([ctypes.POINTER(GatedAddArgs), ctypes.c_void_p], ctypes.c_int),
+    "strata_hip_expert_route": ([ctypes.POINTER(ExpertRouteArgs), ctypes.c_void_p], ctypes.c_int),
+    "strata_hip_expert_route_bwd": ([ctypes.POINTER(ExpertRouteArgs), ctypes.c_void_p], ctypes.c_int),
+    "strata_hip_expert_plan": ([ctypes.POINTER(ExpertPlanArgs), ctypes.c_void_p], ctypes.c_int),
+    "strata_hip_expert_plan_workspace": ([ctypes.c_int64, ctypes.c_int32], ctypes.c_int64),
+    "strata_hip_expert_tile": ([ctypes.c_int64, ctypes.c_int32], ctypes.c_int32),
+    "strata_hip_expert_mlp": ([ctypes.POINTER(ExpertMlpArgs), ctypes.c_void_p], ctypes.c_int),
+    "strata_hip_expert_mlp_bwd": ([ctypes.POINTER(ExpertMlpBwdArgs), ctypes.c_void_p], ctypes.c_int),
     "strata_hip_adamw_workspace": ([ctypes.POINTER(AdamwTensor), ctypes.c_int64], ctypes.c_int64),
     "strata_hip_adamw_step": ([ctypes.POINTER(AdamwArgs), ctypes.c_void_p], ctypes.c_int),
     "strata_hip_adamw_state_values": ([ctypes.POINTER(AdamwValuesArgs), ctypes.c_void_p], ctypes.c_int),

@@ -43,6 +43,8 @@ __all__ = [
     "upsample_dw_gelu",
     "layer_norm_modulate",
     "gated_add",
+    "expert_route",
+    "expert_mlp",
     "adamw_step",
     "adamw_state_values",
 ]
@@ -1385,6 +1387,309 @@ def _(res, gate, y):
 
 
 gated_add.register_autograd(_no_backward("strata_hip::gated_add"))
+
+
+# ---------------------------------------------------------------------------
+# Routing to experts
+# ---------------------------------------------------------------------------
+SCORES = {"softmax": _lib.SCORE_SOFTMAX, "sigmoid": _lib.SCORE_SIGMOID}
+
+
+def _route_args(name, logits, bias, top_k, score, groups, top_groups, renormalize, scale):
+    _require_gpu(name, logits, bias)
+    if score not in SCORES:
+        raise ValueError(f"{name}: score must be one of {sorted(SCORES)}, got {score!r}")
+    if logits.dim() < 1:
+        raise ValueError(f"{name}: logits must be [..., experts]")
+    E = logits.shape[-1]
+    if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (E,)):
+        raise ValueError(f"{name}: bias must be float32 [{E}], got {bias.dtype} {tuple(bias.shape)}")
+    l2 = logits.reshape(-1, E)
+    if l2.stride(1) != 1:
+        l2 = l2.contiguous()
+    a = _lib.ExpertRouteArgs()
+    a.logits, a.tokens, a.ld = l2.data_ptr(), l2.shape[0], l2.stride(0) if l2.shape[0] > 1 else E
+    b = bias.contiguous() if bias is not None else None
+    a.bias = b.data_ptr() if b is not None else None
+    a.dtype, a.experts, a.top_k, a.score = _dtype_code(name, logits), E, int(top_k), SCORES[score]
+    a.groups, a.top_groups, a.renormalize, a.scale = int(groups), int(top_groups), int(bool(renormalize)), float(scale)
+    return a, (l2, b)
+
+
+@torch.library.custom_op("strata_hip::expert_route", mutates_args=())
+def expert_route(logits: Tensor, top_k: int, score: str = "softmax", bias: Optional[Tensor] = None, groups: int = 1,
+                 top_groups: int = 1, renormalize: bool = True, scale: float = 1.0) -> tuple[Tensor, Tensor]:
+    """``top_k`` experts for each token and their weights, ``(weights, index)`` ``[..., top_k]`` from
+    router logits ``[..., experts]`` (bf16 or fp32; the weights have their type, the index is int32).
+
+    Scores are the ``"softmax"`` of a token's logits or their ``"sigmoid"``.  The experts with the
+    largest score + ``bias`` (fp32 ``[experts]``, for the balance of their load; it takes no part in
+    the weights) are chosen in falling order, the lower one of two that are equal; of ``groups``
+    equal groups only the ``top_groups`` with the largest sums of their two best count.  The weights
+    are ``scale`` times the chosen scores, divided by their sum with ``renormalize``.
+
+    A logit (or bias) that is not finite masks its expert; a token with too few experts left has
+    index -1 and weight 0 in the slots that stay empty.  At most 512 experts and top_k 64.  The
+    backward gives the logits' gradient (none flows to the bias)."""
+    name = "expert_route"
+    a, keep = _route_args(name, logits, bias, top_k, score, groups, top_groups, renormalize, scale)
+    shape = (*logits.shape[:-1], int(top_k))
+    weights = torch.empty(shape, dtype=logits.dtype, device=logits.device)
+    index = torch.empty(shape, dtype=torch.int32, device=logits.device)
+    a.weights, a.index = weights.data_ptr(), index.data_ptr()
+    _launch("strata_hip_expert_route", a, logits)
+    return weights, index
+
+
+@expert_route.register_fake
+def _(logits, top_k, score="softmax", bias=None, groups=1, top_groups=1, renormalize=True, scale=1.0):
+    shape = (*logits.shape[:-1], top_k)
+    return logits.new_empty(shape), logits.new_empty(shape, dtype=torch.int32)
+
+
+@torch.library.custom_op("strata_hip::expert_route_bwd", mutates_args=())
+def expert_route_bwd(dweights: Tensor, logits: Tensor, index: Tensor, top_k: int, score: str, bias: Optional[Tensor],
+                     renormalize: bool, scale: float) -> Tensor:
+    """The gradient at the logits of ``expert_route``, from its index and the weights' gradient."""
+    name = "expert_route_bwd"
+    a, keep = _route_args(name, logits, bias, top_k, score, 1, 1, renormalize, scale)
+    _require_gpu(name, logits, dweights, index)
+    shape = (*logits.shape[:-1], int(top_k))
+    if dweights.dtype != logits.dtype or tuple(dweights.shape) != shape or index.dtype != torch.int32 \
+            or tuple(index.shape) != shape:
+        raise ValueError(f"{name}: dweights must be {logits.dtype} and index int32, {shape}")
+    d, i = dweights.contiguous(), index.contiguous()
+    out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    a.dweights, a.index, a.dlogits = d.data_ptr(), i.data_ptr(), out.data_ptr()
+    _launch("strata_hip_expert_route_bwd", a, logits)
+    return out
+
+
+@expert_route_bwd.register_fake
+def _(dweights, logits, index, top_k, score, bias, renormalize, scale):
+    return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+
+
+expert_route_bwd.register_autograd(_no_backward("strata_hip::expert_route_bwd"))
+
+
+def _route_setup_context(ctx, inputs, output):
+    logits, ctx.top_k, ctx.score, bias, _, _, ctx.renormalize, ctx.scale = inputs
+    _, index = output
+    ctx.mark_non_differentiable(index)
+    ctx.set_materialize_grads(False)
+    ctx.save_for_backward(logits, bias, index)
+
+
+def _route_backward(ctx, dweights, _dindex):
+    if dweights is None:
+        return (None,) * 8
+    logits, bias, index = ctx.saved_tensors
+    d = expert_route_bwd(dweights, logits, index, ctx.top_k, ctx.score, bias, ctx.renormalize, ctx.scale)
+    return d, None, None, None, None, None, None, None
+
+
+expert_route.register_autograd(_route_backward, setup_context=_route_setup_context)
+
+
+# ---------------------------------------------------------------------------
+# The experts' MLPs
+# ---------------------------------------------------------------------------
+def _expert_check(name, x, weights, index, w1, b1, w2, b2, residual):
+    _require_gpu(name, x, weights, index, w1, b1, w2, b2, residual)
+    for t, nm in ((x, "x"), (weights, "weights"), (w1, "w1"), (b1, "b1"), (w2, "w2"), (b2, "b2"), (residual, "residual")):
+        if t is not None and t.dtype != torch.bfloat16:
+            raise ValueError(f"{name}: {nm} must be bfloat16, got {t.dtype}")
+    if index.dtype != torch.int32:
+        raise ValueError(f"{name}: index must be int32, got {index.dtype}")
+    C = x.shape[-1]
+    if w1.dim() != 3 or w2.dim() != 3 or w1.shape[2] != C or w2.shape[0] != w1.shape[0] or w2.shape[2] != w1.shape[1]:
+        raise ValueError(f"{name}: w1 must be [E, H, {C}] and w2 [E, N, H], got {tuple(w1.shape)}, {tuple(w2.shape)}")
+    E, H, N = w1.shape[0], w1.shape[1], w2.shape[1]
+    if C % 8 or H % 8 or N % 8 or not (C and H and N and E):
+        raise ValueError(f"{name}: widths must be multiples of 8 and at least one expert given, got {C}, {H}, {N}, {E}")
+    if weights.shape != index.shape or weights.shape[:-1] != x.shape[:-1] or weights.shape[-1] < 1:
+        raise ValueError(f"{name}: weights and index must be {tuple(x.shape[:-1])} + (top_k,), got "
+                         f"{tuple(weights.shape)}, {tuple(index.shape)}")
+    for b, nm, n in ((b1, "b1", H), (b2, "b2", N)):
+        if b is not None and tuple(b.shape) != (E, n):
+            raise ValueError(f"{name}: {nm} must be [{E}, {n}], got {tuple(b.shape)}")
+    if residual is not None and tuple(residual.shape) != (*x.shape[:-1], N):
+        raise ValueError(f"{name}: residual must have shape {(*x.shape[:-1], N)}, got {tuple(residual.shape)}")
+
+
+def _dense(t: Optional[Tensor]) -> Optional[Tensor]:
+    """t contiguous and 16-byte aligned (a copy where it is not)."""
+    if t is None:
+        return None
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
+def _dense_rows(t: Tensor, cols: int) -> tuple[int, int, int, Tensor]:
+    """``_row_view`` of t, or of a copy where t starts between 16-byte addresses."""
+    view = _row_view(t, cols)
+    return view if view[1] % 16 == 0 else _row_view(t.clone(memory_format=torch.contiguous_format), cols)
+
+
+def _ptr(t: Optional[Tensor]) -> Optional[int]:
+    return t.data_ptr() if t is not None else None
+
+
+def _expert_plan(index: Tensor, experts: int) -> tuple[Tensor, int]:
+    """The plan of ``strata_hip_expert_plan`` in one int32 tensor, [row_slot | slot_row | offsets |
+    tiles], and the rows of a tile."""
+    i = index.contiguous()
+    n = i.numel()
+    lib = _lib.load()
+    tile = int(lib.strata_hip_expert_tile(n, experts))
+    plan = torch.empty(2 * n + experts + 2 + 2 * (n // tile + experts), dtype=torch.int32, device=index.device)
+    nws = int(lib.strata_hip_expert_plan_workspace(n, experts))
+    ws = torch.empty(nws, dtype=torch.int32, device=index.device) if nws else None
+    p = plan.data_ptr()
+    a = _lib.ExpertPlanArgs(i.data_ptr(), p, p + 4 * n, p + 8 * n, p + 4 * (2 * n + experts + 1), _ptr(ws), n, experts, tile)
+    _launch("strata_hip_expert_plan", a, index)
+    return plan, tile
+
+
+def _expert_args(x, weights, plan, tile, w1, b1, w2, b2, h, dact, y):
+    """The structure of strata_hip_expert_mlp without out and residual, and what it points into."""
+    C, E, H, N, k = x.shape[-1], w1.shape[0], w1.shape[1], w2.shape[1], weights.shape[-1]
+    T, xp, ldx, x2 = _dense_rows(x, C)
+    w, w1, b1, w2, b2 = weights.contiguous(), _dense(w1), _dense(b1), _dense(w2), _dense(b2)
+    n, p = T * k, plan.data_ptr()
+    a = _lib.ExpertMlpArgs(xp, w.data_ptr(), p, p + 4 * n, p + 8 * n, p + 4 * (2 * n + E + 1), w1.data_ptr(), _ptr(b1),
+                           w2.data_ptr(), _ptr(b2), None, None, h.data_ptr(), _ptr(dact), y.data_ptr(), T, ldx, 0, k, E, C, H,
+                           N, tile)
+    return a, (x2, w, w1, b1, w2, b2)
+
+
+def _expert_forward(name, x, weights, index, w1, b1, w2, b2, residual, save: bool):
+    _expert_check(name, x, weights, index, w1, b1, w2, b2, residual)
+    E, H, N = w1.shape[0], w1.shape[1], w2.shape[1]
+    n = index.numel()
+    out = torch.empty((*x.shape[:-1], N), dtype=torch.bfloat16, device=x.device)
+    h = torch.empty((n, H), dtype=torch.bfloat16, device=x.device)
+    dact = torch.empty_like(h) if save else None
+    y = torch.empty((n, N), dtype=torch.float32, device=x.device)
+    plan, tile = _expert_plan(index, E)
+    a, keep = _expert_args(x, weights, plan, tile, w1, b1, w2, b2, h, dact, y)
+    if residual is not None:
+        _, a.residual, a.ldr, r2 = _dense_rows(residual, N)
+    a.out = out.data_ptr()
+    _launch("strata_hip_expert_mlp", a, x)
+    return out, h, dact, y, plan
+
+
+@torch.library.custom_op("strata_hip::expert_mlp_fwd", mutates_args=())
+def expert_mlp_fwd(x: Tensor, weights: Tensor, index: Tensor, w1: Tensor, b1: Optional[Tensor], w2: Tensor,
+                   b2: Optional[Tensor], residual: Optional[Tensor]) -> Tensor:
+    """``expert_mlp`` for inference: nothing is kept for a backward."""
+    return _expert_forward("expert_mlp", x, weights, index, w1, b1, w2, b2, residual, False)[0]
+
+
+@expert_mlp_fwd.register_fake
+def _(x, weights, index, w1, b1, w2, b2, residual):
+    return x.new_empty((*x.shape[:-1], w2.shape[1]))
+
+
+expert_mlp_fwd.register_autograd(_no_backward("strata_hip::expert_mlp_fwd"))
+
+
+@torch.library.custom_op("strata_hip::expert_mlp_train", mutates_args=())
+def expert_mlp_train(x: Tensor, weights: Tensor, index: Tensor, w1: Tensor, b1: Optional[Tensor], w2: Tensor,
+                     b2: Optional[Tensor], residual: Optional[Tensor]) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """``expert_mlp`` under autograd: the output and, for the backward, the hidden activations, the
+    GELU's derivative at them, the experts' outputs and the plan."""
+    return _expert_forward("expert_mlp", x, weights, index, w1, b1, w2, b2, residual, True)
+
+
+@expert_mlp_train.register_fake
+def _(x, weights, index, w1, b1, w2, b2, residual):
+    n, E, H, N = index.numel(), w1.shape[0], w1.shape[1], w2.shape[1]
+    tile = int(_lib.load().strata_hip_expert_tile(n, E))
+    return (x.new_empty((*x.shape[:-1], N)), x.new_empty((n, H)), x.new_empty((n, H)),
+            x.new_empty((n, N), dtype=torch.float32),
+            x.new_empty((2 * n + E + 2 + 2 * (n // tile + E),), dtype=torch.int32))
+
+
+@torch.library.custom_op("strata_hip::expert_mlp_bwd", mutates_args=())
+def expert_mlp_bwd(dout: Tensor, x: Tensor, weights: Tensor, w1: Tensor, b1: Optional[Tensor], w2: Tensor,
+                   b2: Optional[Tensor], h: Tensor, dact: Tensor, y: Tensor, plan: Tensor,
+                   need: Sequence[bool]) -> list[Tensor]:
+    """Gradients of ``expert_mlp_train`` at ``(x, weights, w1, b1, w2, b2)``, an empty tensor where
+    ``need`` asks for none (a bias's comes from its weight's launch)."""
+    E, H, C = w1.shape
+    N, k = w2.shape[1], weights.shape[-1]
+    n = h.shape[0]
+    tile = int(_lib.load().strata_hip_expert_tile(n, E))
+    a, keep = _expert_args(x, weights, plan, tile, w1, b1, w2, b2, h, dact, y)
+    new = lambda *shape: torch.empty(shape, dtype=torch.bfloat16, device=x.device)  # noqa: E731
+    want_x, want_wt = need[0], need[1]
+    want_1, want_2 = need[2] or (need[3] and b1 is not None), need[4] or (need[5] and b2 is not None)
+    hid = want_x or want_1
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_x else None
+    dwt = torch.empty(weights.shape, dtype=weights.dtype, device=x.device) if want_wt else None
+    dw1, db1 = (new(E, H, C), new(E, H) if b1 is not None else None) if want_1 else (None, None)
+    dw2, db2 = (new(E, N, H), new(E, N) if b2 is not None else None) if want_2 else (None, None)
+    g = _dense(dout)
+    gs = new(n, N) if want_2 else None
+    gz, w2t = (new(n, H), new(E, H, N)) if hid else (None, None)
+    dxs, w1t = (new(n, C), new(E, C, H)) if want_x else (None, None)
+    b = _lib.ExpertMlpBwdArgs(a, g.data_ptr(), *(_ptr(t) for t in (dx, dwt, dw1, db1, dw2, db2, gs, gz, dxs, w1t, w2t)))
+    _launch("strata_hip_expert_mlp_bwd", b, x)
+    return [t if t is not None and wanted else new(0) for t, wanted in zip((dx, dwt, dw1, db1, dw2, db2), need)]
+
+
+@expert_mlp_bwd.register_fake
+def _(dout, x, weights, w1, b1, w2, b2, h, dact, y, plan, need):
+    return [torch.empty_like(t) if t is not None and wanted else x.new_empty(0)
+            for t, wanted in zip((x, weights, w1, b1, w2, b2), need)]
+
+
+expert_mlp_bwd.register_autograd(_no_backward("strata_hip::expert_mlp_bwd"))
+
+
+def _expert_setup_context(ctx, inputs, output):
+    x, weights, index, w1, b1, w2, b2, residual = inputs
+    _, h, dact, y, plan = output
+    ctx.has = [True, True, True, b1 is not None, True, b2 is not None]
+    ctx.has_res = residual is not None
+    ctx.mark_non_differentiable(h, dact, y, plan)
+    ctx.set_materialize_grads(False)
+    ctx.save_for_backward(x, weights, w1, b1, w2, b2, h, dact, y, plan)
+
+
+def _expert_backward(ctx, dout, *_unused):
+    if dout is None:
+        return (None,) * 8
+    x, weights, w1, b1, w2, b2, h, dact, y, plan = ctx.saved_tensors
+    n = ctx.needs_input_grad
+    need = [bool(q and has) for q, has in zip((n[0], n[1], n[3], n[4], n[5], n[6]), ctx.has)]
+    grads = expert_mlp_bwd(dout, x, weights, w1, b1, w2, b2, h, dact, y, plan, need) if any(need) else [None] * 6
+    gx, gwt, g1, gb1, g2, gb2 = (g if wanted else None for g, wanted in zip(grads, need))
+    return gx, gwt, None, g1, gb1, g2, gb2, dout if ctx.has_res and n[7] else None
+
+
+expert_mlp_train.register_autograd(_expert_backward, setup_context=_expert_setup_context)
+
+
+def expert_mlp(x: Tensor, weights: Tensor, index: Tensor, w1: Tensor, b1: Optional[Tensor], w2: Tensor,
+               b2: Optional[Tensor], residual: Optional[Tensor] = None) -> Tensor:
+    """The chosen experts' MLPs and their weighted sum, bf16 with fp32 accumulation::
+
+        out[t] = residual[t] + sum over s of weights[t, s] * (gelu_tanh(x[t] @ w1[e].T + b1[e]) @ w2[e].T + b2[e])
+
+    with e = ``index[t, s]``.  x ``[..., C]``, weights (bf16) and index (int32) ``[..., top_k]`` as
+    ``expert_route`` gives them, w1 ``[E, H, C]``, b1 ``[E, H]`` or None, w2 ``[E, N, H]``, b2
+    ``[E, N]`` or None, residual ``[..., N]`` or None; widths multiples of 8, x and the output under
+    2 GiB.  An index outside ``[0, E)`` adds nothing, and the same expert may stand in two slots.
+    No token is dropped for an expert's load.  Differentiable once, in every argument but the
+    index."""
+    ts = (x, weights, w1, b1, w2, b2, residual)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        return expert_mlp_train(x, weights, index, w1, b1, w2, b2, residual)[0]
+    return expert_mlp_fwd(x, weights, index, w1, b1, w2, b2, residual)
 
 
 # ---------------------------------------------------------------------------

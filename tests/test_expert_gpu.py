@@ -1,0 +1,225 @@
+"""The experts' MLPs (``ops.expert_mlp``) against the float64 oracle, every output inside the bound that the
+oracle derives from its operands (oracle/experts.py: bf16 operands, fp32 sums)."""
+
+import math
+
+import pytest
+import torch
+
+from oracle import experts as O
+from strata_amd import ops
+
+from .conftest import rel_l2
+
+pytestmark = pytest.mark.gpu
+NAMES = ("x", "weights", "w1", "b1", "w2", "b2", "residual")
+
+
+def _case(T, E, k, C, H, N, seed, biases=True, residual=True, dropped=0.1, skew=1.0):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s, std=1.0: (torch.randn(*s, generator=g) * std).bfloat16()  # noqa: E731
+    c = dict(x=r(T, C), w1=r(E, H, C, std=C**-0.5), w2=r(E, N, H, std=H**-0.5), b1=r(E, H, std=0.2) if biases else None,
+             b2=r(E, N, std=0.2) if biases else None, residual=r(T, N) if residual else None, dout=r(T, N))
+    c["weights"] = torch.rand(T, k, generator=g).bfloat16()
+    logits = torch.randn(T, E, generator=g) + skew * torch.randn(E, generator=g)
+    idx = torch.stack([logits.argsort(1, descending=True)[:, s % E] for s in range(k)], 1).int()
+    idx[torch.rand(T, k, generator=g) < dropped] = -1
+    c["index"] = idx
+    return c
+
+
+def _to(c, gpu, train):
+    out = {n: t.to(gpu) if t is not None else None for n, t in c.items()}
+    if train:
+        for n in NAMES:
+            if out[n] is not None:
+                out[n].requires_grad_()
+    return out
+
+
+def _call(d):
+    return ops.expert_mlp(d["x"], d["weights"], d["index"], d["w1"], d["b1"], d["w2"], d["b2"], d["residual"])
+
+
+def _inside(got, want, what):
+    value, bound = want
+    diff = (got.detach().cpu().double().view(value.shape) - value).abs()
+    assert torch.isfinite(got).all(), what
+    assert (diff <= bound).all(), (what, float((diff / bound).max()))
+    # the bound adds every rounding up; on the whole they cancel: 4 roundings to bf16 of random sign
+    if value.numel() > 1000:
+        assert rel_l2(got.detach().view(value.shape), value) <= 2 * 2.0**-8, what
+
+
+SHAPES = [
+    # tokens, experts, top_k, dim, hidden, out_dim
+    (1, 1, 1, 8, 8, 8), (1, 8, 2, 64, 128, 64), (3, 4, 3, 72, 40, 24), (64, 2, 1, 64, 64, 64), (65, 3, 2, 136, 72, 200),
+    (130, 5, 2, 64, 264, 64), (200, 24, 3, 104, 56, 96), (300, 2, 2, 128, 256, 128), (513, 3, 1, 264, 136, 520),
+    (700, 4, 2, 96, 640, 96), (40, 64, 4, 32, 48, 32), (1500, 3, 2, 192, 128, 64),
+]
+
+
+@pytest.mark.parametrize("T,E,k,C,H,N", SHAPES)
+def test_forward_and_gradients(gpu, T, E, k, C, H, N):
+    print(f"experts {T} {E} {k} {C} {H} {N}", flush=True)
+    for seed, biases, residual in ((1, True, True), (2, False, False)):
+        c = _case(T, E, k, C, H, N, seed, biases, residual)
+        want = O.mlp_bounds(*(c[n] for n in ("x", "weights", "index", "w1", "b1", "w2", "b2", "residual", "dout")))
+        with torch.no_grad():
+            _inside(_call(_to(c, gpu, False)), want["out"], "inference")
+        d = _to(c, gpu, True)
+        out = _call(d)
+        _inside(out, want["out"], "out")
+        names = [n for n in NAMES if d[n] is not None]
+        grads = torch.autograd.grad(out, [d[n] for n in names], d["dout"])
+        for n, g in zip(names, grads):
+            assert g.shape == d[n].shape and g.dtype == torch.bfloat16
+            _inside(g, want[n], n)
+
+
+def test_nothing_chosen_and_unused_experts(gpu):
+    c = _case(70, 6, 2, 64, 72, 64, 3)
+    c["index"][:] = -1
+    d = _to(c, gpu, True)
+    out = _call(d)
+    assert torch.equal(out, d["residual"])
+    grads = dict(zip(NAMES, torch.autograd.grad(out, [d[n] for n in NAMES], d["dout"])))
+    for n in NAMES[:-1]:
+        assert (grads[n] == 0).all(), n
+    assert torch.equal(grads["residual"], d["dout"])
+    c["index"][:] = torch.tensor([4, 9])  # one expert for all, and one that does not exist
+    d = _to(c, gpu, True)
+    want = O.mlp_bounds(*(c[n] for n in ("x", "weights", "index", "w1", "b1", "w2", "b2", "residual", "dout")))
+    out = _call(d)
+    _inside(out, want["out"], "out")
+    for n, g in zip(NAMES, torch.autograd.grad(out, [d[n] for n in NAMES], d["dout"])):
+        _inside(g, want[n], n)
+    for n in ("w1", "b1", "w2", "b2"):
+        assert (torch.autograd.grad(_call(d), d[n], d["dout"])[0][[0, 1, 2, 3, 5]] == 0).all()
+
+
+def test_no_tokens(gpu):
+    c = _case(0, 3, 2, 16, 24, 16, 4)
+    d = _to(c, gpu, True)
+    out = _call(d)
+    assert tuple(out.shape) == (0, 16)
+    for n, g in zip(NAMES, torch.autograd.grad(out, [d[n] for n in NAMES], d["dout"])):
+        assert g.shape == d[n].shape and (g == 0).all()
+
+
+def test_the_same_expert_twice(gpu):
+    """Two slots of one expert are two rows: as one slot with the weights' sum, both gradients alike."""
+    c = _case(90, 3, 2, 64, 64, 64, 5, dropped=0.0)
+    c["index"][:, 1] = c["index"][:, 0]
+    want = O.mlp_bounds(*(c[n] for n in ("x", "weights", "index", "w1", "b1", "w2", "b2", "residual", "dout")))
+    d = _to(c, gpu, True)
+    out = _call(d)
+    _inside(out, want["out"], "out")
+    for n, g in zip(NAMES, torch.autograd.grad(out, [d[n] for n in NAMES], d["dout"])):
+        _inside(g, want[n], n)
+        if n == "weights":
+            assert torch.equal(g[:, 0], g[:, 1])
+
+
+@pytest.mark.parametrize("which", NAMES)
+def test_one_gradient_alone(gpu, which):
+    c = _case(150, 4, 2, 72, 80, 64, 6)
+    want = O.mlp_bounds(*(c[n] for n in ("x", "weights", "index", "w1", "b1", "w2", "b2", "residual", "dout")))
+    d = _to(c, gpu, False)
+    d[which].requires_grad_()
+    _inside(torch.autograd.grad(_call(d), d[which], d["dout"])[0], want[which], which)
+
+
+def test_layouts(gpu):
+    """Rows inside wider tensors, leading dimensions, weights and biases that are views, an expanded dout."""
+    c = _case(60, 3, 2, 64, 48, 64, 7)
+    want = O.mlp_bounds(*(c[n] for n in ("x", "weights", "index", "w1", "b1", "w2", "b2", "residual", "dout")))["out"]
+    d = _to(c, gpu, False)
+
+    def wide(t, pad):
+        buf = torch.full((*t.shape[:-1], t.shape[-1] + pad), math.nan, dtype=t.dtype, device=gpu)
+        buf[..., : t.shape[-1]] = t
+        return buf[..., : t.shape[-1]]
+
+    v = dict(d, x=wide(d["x"], 16), residual=wide(d["residual"], 8), w1=wide(d["w1"], 24), w2=d["w2"].transpose(1, 2).contiguous().transpose(1, 2),
+             b1=wide(d["b1"], 1), weights=wide(d["weights"], 3))
+    _inside(_call(v), want, "strided")
+    odd = torch.empty(60 * 64 + 1, dtype=torch.bfloat16, device=gpu)[1:].view(60, 64)
+    odd.copy_(d["x"])
+    _inside(_call(dict(d, x=odd, residual=odd)), O.mlp_bounds(*(c[n] for n in NAMES[:2]), c["index"], *(c[n] for n in NAMES[2:6]), c["x"])["out"], "odd first element")
+    lead = {n: (d[n].view(3, 4, 5, -1) if n in ("x", "weights", "index", "residual") else d[n]) for n in d}
+    out = _call(lead)
+    assert tuple(out.shape) == (3, 4, 5, 64)
+    _inside(out, want, "leading")
+    d = _to(c, gpu, True)
+    ones = torch.ones((), device=gpu).bfloat16().expand(60, 64)
+    full = torch.autograd.grad(_call(d), d["w2"], ones.contiguous())[0]
+    assert torch.equal(torch.autograd.grad(_call(d), d["w2"], ones)[0], full)
+
+
+def test_masked_tokens_do_not_reach_others(gpu):
+    """A dropped token's x may hold anything; an infinite one reaches its own row alone."""
+    c = _case(100, 4, 2, 64, 64, 64, 8, dropped=0.0)
+    c["index"][10] = -1
+    d = _to(c, gpu, False)
+    clean = _call(d)
+    x = d["x"].clone()
+    x[10] = math.nan
+    assert torch.equal(_call(dict(d, x=x)), clean)
+    x[20] = math.inf
+    out = _call(dict(d, x=x))
+    keep = [t for t in range(100) if t != 20]
+    assert torch.equal(out[keep], clean[keep]) and not torch.isfinite(out[20]).all()
+
+
+def test_repeats_bit_for_bit_and_order_of_tokens(gpu):
+    c = _case(900, 5, 2, 128, 192, 128, 9)
+    d = _to(c, gpu, True)
+    names = list(NAMES)
+
+    def both():
+        out = _call(d)
+        return [out, *torch.autograd.grad(out, [d[n] for n in names], d["dout"])]
+
+    a, b = both(), both()
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    perm = torch.randperm(900, generator=torch.Generator().manual_seed(1)).to(gpu)
+    with torch.no_grad():  # a token's result does not depend on its place
+        p = {n: (d[n][perm] if n in ("x", "weights", "index", "residual") else d[n]) for n in d}
+        assert torch.equal(_call(p), a[0][perm])
+
+
+def test_another_stream_and_graph(gpu):
+    c = _case(333, 4, 2, 96, 128, 96, 10)
+    d = _to(c, gpu, False)
+    want = _call(d).clone()
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        got = _call(d)
+    s.synchronize()
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = _call(d)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        again = _call(d)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(again, want)
+
+
+def test_refusals(gpu):
+    c = _to(_case(8, 3, 2, 16, 24, 16, 11), gpu, False)
+    for over, msg in ((dict(x=c["x"].float()), "bfloat16"), (dict(index=c["index"].long()), "int32"),
+                      (dict(w1=c["w1"][:, :, :8]), r"\[E, H"), (dict(w2=c["w2"][:2]), r"\[E, N"), (dict(b1=c["b2"]), "b1"),
+                      (dict(weights=c["weights"][:, :1]), "top_k"), (dict(residual=c["residual"][:4]), "residual"),
+                      (dict(x=c["x"][:, :12], w1=c["w1"][:, :, :12]), "multiples"), (dict(x=c["x"].cpu()), "GPU")):
+        with pytest.raises(ValueError, match=msg):
+            _call(dict(c, **over))
+    x = c["x"].clone().requires_grad_()
+    out = _call(dict(c, x=x))
+    (g,) = torch.autograd.grad(out.float().square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="no backward"):
+        g.sum().backward()

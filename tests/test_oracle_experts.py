@@ -1,0 +1,168 @@
+"""The experts' oracle: closed forms, torch's own pieces, and differences (float64, CPU); refusals of
+the operators without a GPU."""
+
+import ctypes
+import math
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from oracle import experts as O
+from strata_amd import _lib, ops
+
+
+def _rand(seed, *shape):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed), dtype=torch.float64)
+
+
+def test_one_expert_is_the_dense_mlp():
+    x, w1, b1, w2, b2 = _rand(0, 5, 8), _rand(1, 1, 12, 8), _rand(2, 1, 12), _rand(3, 1, 8, 12), _rand(4, 1, 8)
+    want = x + F.linear(F.gelu(F.linear(x, w1[0], b1[0]), approximate="tanh"), w2[0], b2[0])
+    idx, one = torch.zeros(5, 1, dtype=torch.int32), torch.ones(5, 1, dtype=torch.float64)
+    assert torch.allclose(O.mlp(x, one, idx, w1, b1, w2, b2, x), want, rtol=1e-12)
+    # the same expert in both slots, weights that sum to one
+    both = torch.tensor([[0.25, 0.75]], dtype=torch.float64).expand(5, 2)
+    assert torch.allclose(O.mlp(x, both, idx.expand(5, 2), w1, b1, w2, b2, x), want, rtol=1e-12)
+    assert torch.equal(O.mlp(x, one, idx - 1, w1, b1, w2, b2, x), x)  # dropped
+
+
+def test_bounds_values_are_the_definition_and_its_gradients():
+    x, w1, b1, w2, b2, res = _rand(0, 7, 8), _rand(1, 3, 8, 8), _rand(2, 3, 8), _rand(3, 3, 16, 8), _rand(4, 3, 16), _rand(5, 7, 16)
+    wt = torch.rand(7, 2, generator=torch.Generator().manual_seed(6), dtype=torch.float64)
+    idx = torch.tensor([[0, 1], [1, 1], [-1, 2], [2, 0], [-1, -1], [0, 7], [1, 2]], dtype=torch.int32)
+    dout = _rand(7, 7, 16)
+    leaves = [t.clone().requires_grad_() for t in (x, wt, w1, b1, w2, b2, res)]
+    out = O.mlp(leaves[0], leaves[1], idx, *leaves[2:])
+    grads = torch.autograd.grad(out, leaves, dout)
+    got = O.mlp_bounds(x, wt, idx, w1, b1, w2, b2, res, dout)
+    assert torch.allclose(got["out"][0], out, rtol=1e-11, atol=1e-12)
+    for n, g in zip(("x", "weights", "w1", "b1", "w2", "b2", "residual"), grads):
+        assert torch.allclose(got[n][0], g, rtol=1e-10, atol=1e-11), n
+    fn = lambda *a: O.mlp(a[0], a[1], idx, *a[2:])  # noqa: E731
+    assert torch.autograd.gradcheck(fn, leaves)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renorm", [False, True])
+def test_route_closed_forms(score, renorm):
+    l = _rand(1, 6, 10)
+    w, i = O.route(l, 3, score, renormalize=renorm, scale=2.0)
+    top = l.topk(3, dim=1)
+    assert torch.equal(i.long(), top.indices)
+    s = torch.softmax(l, 1) if score == "softmax" else torch.sigmoid(l)
+    s = s.gather(1, top.indices)
+    want = 2.0 * (s / s.sum(1, keepdim=True) if renorm else s)
+    assert torch.allclose(w, want, rtol=1e-12)
+    lg = l.clone().requires_grad_()
+    assert torch.allclose(O.route_weights(lg, i, score, renorm, 2.0), want, rtol=1e-12)
+    assert torch.autograd.gradcheck(lambda a: O.route_weights(a, i, score, renorm, 2.0), lg)
+
+
+def test_route_bias_groups_ties_and_masks():
+    l = torch.tensor([[0.0, 1.0, 1.0, 3.0, 2.0, 2.0]], dtype=torch.float64)
+    assert O.route(l, 4)[1].tolist() == [[3, 4, 5, 1]]  # of two equal keys the lower expert
+    bias = torch.tensor([10.0, 0, 0, 0, 0, 0])
+    w, i = O.route(l, 1, "sigmoid", bias, renormalize=False)
+    assert i.tolist() == [[0]] and float(w) == 0.5  # the bias chooses and does not weigh
+    # groups (0, 1), (2, 3), (4, 5): the sums of their two best are s(0)+s(1), s(1)+s(3), s(2)+s(2)
+    assert O.route(l, 2, "sigmoid", None, 3, 1)[1].tolist() == [[4, 5]]
+    assert O.route(l, 2, "softmax", None, 3, 1)[1].tolist() == [[3, 2]]
+    m = l.clone()
+    m[0, 1:] = -math.inf
+    w, i = O.route(m, 3)
+    assert i.tolist() == [[0, -1, -1]] and w.tolist() == [[1.0, 0.0, 0.0]]
+    m[0, 0] = math.nan
+    assert O.route(m, 2)[1].tolist() == [[-1, -1]]
+
+
+# ---------------------------------------------------------------------------
+# Refusals
+# ---------------------------------------------------------------------------
+@pytest.fixture(scope="module")
+def lib():
+    return _lib.load()
+
+
+def _route_args(**over):
+    a = _lib.ExpertRouteArgs()
+    a.logits = a.weights = a.index = a.dweights = a.dlogits = 0x1000
+    a.tokens, a.ld, a.dtype, a.experts, a.top_k, a.score = 4, 8, _lib.BF16, 8, 2, 0
+    a.groups, a.top_groups, a.renormalize, a.scale = 1, 1, 1, 1.0
+    for k, v in over.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("over,code,msg", [
+    (dict(tokens=-1), _lib.EINVAL, "tokens"), (dict(top_k=0), _lib.EINVAL, "top_k"), (dict(dtype=3), _lib.EINVAL, "dtype"),
+    (dict(score=2), _lib.EINVAL, "score"), (dict(experts=513, ld=513), _lib.EUNSUPPORTED, "512"),
+    (dict(experts=512, ld=512, top_k=65), _lib.EUNSUPPORTED, "64"), (dict(groups=3), _lib.EINVAL, "groups"),
+    (dict(groups=4, top_groups=5), _lib.EINVAL, "groups"), (dict(groups=4, top_groups=1, top_k=3), _lib.EINVAL, "exceeds"),
+    (dict(top_k=9), _lib.EINVAL, "exceeds"), (dict(ld=7), _lib.EINVAL, "stride"), (dict(scale=math.inf), _lib.EINVAL, "scale"),
+    (dict(tokens=1 << 31), _lib.EUNSUPPORTED, "pairs"), (dict(index=None), _lib.EINVAL, "null"),
+])
+def test_route_refusals(lib, over, code, msg):
+    a = _route_args(**over)
+    for fn in (lib.strata_hip_expert_route, lib.strata_hip_expert_route_bwd):
+        assert fn(ctypes.byref(a), None) == code and msg in lib.strata_hip_last_error().decode()
+    a = _route_args(tokens=0, logits=None, index=None)
+    assert lib.strata_hip_expert_route(ctypes.byref(a), None) == 0
+
+
+def test_plan_refusals_and_sizes(lib):
+    assert lib.strata_hip_expert_plan_workspace(1024, 8) == 0 and lib.strata_hip_expert_plan_workspace(1025, 8) == 16
+    for over, code in ((dict(pairs=-1), _lib.EINVAL), (dict(experts=0), _lib.EINVAL), (dict(tile=0), _lib.EINVAL),
+                       (dict(experts=513), _lib.EUNSUPPORTED), (dict(offsets=None), _lib.EINVAL),
+                       (dict(row_slot=None), _lib.EINVAL), (dict(pairs=2000, workspace=None), _lib.EINVAL)):
+        a = _lib.ExpertPlanArgs(*[0x1000] * 6, 100, 8, 64)
+        for k, v in over.items():
+            setattr(a, k, v)
+        assert lib.strata_hip_expert_plan(ctypes.byref(a), None) == code, over
+
+
+def _mlp_args(lib, **over):
+    a = _lib.ExpertMlpArgs(*[0x1000] * 15, 16, 64, 64, 2, 8, 64, 128, 64, 0)
+    for k, v in over.items():
+        setattr(a, k, v)
+    if a.tile == 0:
+        a.tile = lib.strata_hip_expert_tile(a.tokens * a.top_k, a.experts)
+    return a
+
+
+@pytest.mark.parametrize("over,code,msg", [
+    (dict(tokens=-1), _lib.EINVAL, "sizes"), (dict(dim=60), _lib.EINVAL, "multiples"), (dict(hidden=4), _lib.EINVAL, "multiples"),
+    (dict(out_dim=0), _lib.EINVAL, "sizes"), (dict(experts=513), _lib.EUNSUPPORTED, "512"), (dict(tile=3), _lib.EINVAL, "tile"),
+    (dict(w1=0x1008), _lib.EINVAL, "aligned"), (dict(b1=0x1004), _lib.EINVAL, "aligned"), (dict(x=None), _lib.EINVAL, "null"),
+    (dict(h=None), _lib.EINVAL, "null"), (dict(ldx=60), _lib.EINVAL, "stride"), (dict(ldx=56), _lib.EINVAL, "stride"),
+    (dict(tokens=1 << 24), _lib.EUNSUPPORTED, "2 GiB"), (dict(x=0x1002), _lib.EINVAL, "aligned"),
+])
+def test_mlp_refusals(lib, over, code, msg):
+    a = _mlp_args(lib, **over)
+    assert lib.strata_hip_expert_mlp(ctypes.byref(a), None) == code and msg in lib.strata_hip_last_error().decode()
+    b = _lib.ExpertMlpBwdArgs(a, *[0x1000] * 12)
+    assert lib.strata_hip_expert_mlp_bwd(ctypes.byref(b), None) == code
+
+
+@pytest.mark.parametrize("over,msg", [
+    (dict(dout=None), "dout"), (dict(gs=None), "gs"), (dict(gz=None), "gz"), (dict(w2t=None), "w2t"), (dict(dxs=None), "dxs"),
+    (dict(dw2=None), "bias gradient"), (dict(dw1=None), "bias gradient"), (dict(dx=0x1008), "aligned"),
+])
+def test_mlp_bwd_refusals(lib, over, msg):
+    b = _lib.ExpertMlpBwdArgs(_mlp_args(lib), *[0x1000] * 12)
+    for k, v in over.items():
+        setattr(b, k, v)
+    assert lib.strata_hip_expert_mlp_bwd(ctypes.byref(b), None) == _lib.EINVAL
+    assert msg in lib.strata_hip_last_error().decode()
+    if "dout" in over:
+        b.fwd.out = None
+        assert lib.strata_hip_expert_mlp(ctypes.byref(b.fwd), None) == _lib.EINVAL
+
+
+def test_ops_refuse_cpu_tensors():
+    with pytest.raises(ValueError, match="GPU"):
+        ops.expert_route(torch.zeros(2, 8), 2)
+    x, w = torch.zeros(2, 8).bfloat16(), torch.zeros(2, 1).bfloat16()
+    w1, w2 = torch.zeros(3, 16, 8).bfloat16(), torch.zeros(3, 8, 16).bfloat16()
+    with pytest.raises(ValueError, match="GPU"):
+        ops.expert_mlp(x, w, torch.zeros(2, 1, dtype=torch.int32), w1, None, w2, None)

@@ -1,0 +1,187 @@
+"""Routing to experts (``ops.expert_route``) and the plan of the chosen pairs against the float64 oracle.
+
+The index has to be equal.  Weights (u = 2^-24): a score's exponent x - top is rounded once (|x| u
+relative in the score), exp and the reciprocal are within 4 u, the sum of a lane's scores and of its
+neighbours' has at most 64 + 6 roundings, the sum of the chosen ones top_k, and quotient, scale and
+product 4: u (span + 80 + top_k) relative, span the largest |logit - top| chosen; then the rounding to
+the logits' type.
+"""
+
+import math
+
+import pytest
+import torch
+
+from oracle import experts as O
+from strata_amd import _lib, ops
+
+pytestmark = pytest.mark.gpu
+U = 2.0**-24
+
+
+def _logits(T, E, dtype, seed, masked=0.0, ties=False):
+    g = torch.Generator().manual_seed(seed)
+    l = torch.randn(T, E, generator=g) * 2
+    if ties:
+        l = torch.round(l)
+    if masked:
+        l[torch.rand(T, E, generator=g) < masked] = -math.inf
+        l[::7] = -math.inf  # rows with nothing left
+        l[1::11, :1] = math.nan
+        l[2::13, -1:] = math.inf
+        l[3::17] = torch.finfo(dtype).min  # the type's lowest value is a logit like others
+    return l.to(dtype)
+
+
+def _check(l, kw, got, gpu_weights_dtype):
+    w, i = got
+    ww, wi = O.route(l, **kw)
+    assert i.dtype == torch.int32 and w.dtype == gpu_weights_dtype
+    assert torch.equal(i.cpu().view(wi.shape), wi)
+    ok = torch.isfinite(l.double())
+    lo = torch.where(ok, l.double(), 0.0)
+    span = (lo.gather(1, wi.clamp_min(0).long()) - torch.where(ok, l.double(), -math.inf).amax(1, keepdim=True).nan_to_num(0, 0, 0)).abs()
+    span = torch.minimum(span.amax(1, keepdim=True), torch.tensor(120.0, dtype=torch.float64))  # beyond, the score is 0
+    half = 2.0**-8 if w.dtype == torch.bfloat16 else U
+    tol = ww * (U * (span + 80 + kw["top_k"]) + half) + 1e-37
+    assert ((w.cpu().double().view(ww.shape) - ww).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,E,k", [(1, 1, 1), (1, 8, 2), (3, 5, 5), (63, 8, 1), (65, 9, 4), (257, 16, 2), (130, 24, 3),
+                                   (31, 33, 7), (200, 64, 8), (33, 65, 6), (17, 128, 8), (40, 200, 5), (9, 300, 64),
+                                   (5, 512, 10)])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_route(gpu, T, E, k, score, dtype):
+    print(f"route {T} {E} {k} {score} {dtype}", flush=True)
+    for seed, masked, ties, renorm in ((0, 0.0, False, True), (1, 0.3, False, False), (2, 0.0, True, False), (3, 0.5, True, True)):
+        l = _logits(T, E, dtype, seed, masked, ties)
+        kw = dict(top_k=k, score=score, renormalize=renorm, scale=1.5)
+        _check(l, kw, ops.expert_route(l.to(gpu), **kw), dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,E,k,groups,top", [(70, 8, 2, 4, 2), (33, 24, 3, 2, 1), (129, 64, 8, 8, 4), (11, 60, 6, 20, 3),
+                                              (40, 96, 4, 4, 4), (7, 192, 8, 8, 3), (5, 512, 16, 64, 8), (3, 6, 1, 6, 1)])
+@pytest.mark.parametrize("with_bias", [False, True])
+def test_route_bias_and_groups(gpu, T, E, k, groups, top, with_bias, dtype):
+    print(f"route {T} {E} {k} groups {groups}/{top} bias {with_bias} {dtype}", flush=True)
+    g = torch.Generator().manual_seed(9)
+    bias = torch.randn(E, generator=g) * 0.3 if with_bias else None
+    if with_bias:
+        bias[E // 2] = math.nan  # masks its expert
+        bias[0] = -5.0
+    for score, masked, ties in (("sigmoid", 0.0, False), ("softmax", 0.3, False), ("sigmoid", 0.2, True)):
+        l = _logits(T, E, dtype, 4, masked, ties)
+        kw = dict(top_k=k, score=score, bias=bias, groups=groups, top_groups=top, renormalize=True, scale=2.5)
+        lm = l.clone()
+        if with_bias:
+            lm[:, E // 2] = -math.inf
+        got = ops.expert_route(l.to(gpu), k, score, bias.to(gpu) if with_bias else None, groups, top, True, 2.5)
+        _check(lm, kw, got, dtype)
+
+
+def test_route_near_ties_are_told_apart(gpu):
+    """Keys s + bias whose difference a 32-bit sum loses: 64 bits choose, in either order."""
+    l = torch.zeros(2, 8)
+    l[:, 1] = 1e-8
+    l[1] = l[1].flip(0)
+    b = torch.zeros(8)
+    for bias in (b, b + 3.0):
+        _, i = ops.expert_route(l.to(gpu), 1, "sigmoid", bias.to(gpu))
+        assert i.flatten().tolist() == [1, 6]
+
+
+def test_route_layouts_and_leading_dims(gpu):
+    """Rows inside a wider tensor, an odd first element, a transposed view, leading dimensions, no tokens."""
+    big = _logits(40, 50, torch.float32, 5)
+    l = big[:, 3:27].clone()
+    want = O.route(l, 4)
+    views = [big.to(gpu)[:, 3:27], l.t().contiguous().to(gpu).t(), l.view(4, 2, 5, 24).to(gpu)]
+    for v in views:
+        w, i = ops.expert_route(v, 4)
+        assert tuple(w.shape) == (*v.shape[:-1], 4)
+        assert torch.equal(i.cpu().view(-1, 4), want[1])
+        assert (w.cpu().double().view(-1, 4) - want[0]).abs().max() <= 100 * U
+    w, i = ops.expert_route(torch.zeros(0, 3, 8, device=gpu), 2)
+    assert tuple(w.shape) == tuple(i.shape) == (0, 3, 2)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renorm", [False, True])
+@pytest.mark.parametrize("T,E,k", [(1, 8, 2), (65, 24, 3), (50, 64, 8), (21, 100, 4), (6, 300, 9)])
+def test_route_gradient(gpu, T, E, k, score, renorm, dtype):
+    """Against the differentiated oracle.  ds has roundings of the scores (as the weights), of a / S
+    and of their difference, whose terms may cancel: u (span + 100 + 2 top_k) of c (|dw| + |a| / S), times s
+    (and 1 - s); the softmax's sum of s ds likewise."""
+    print(f"route gradient {T} {E} {k} {score} {renorm} {dtype}", flush=True)
+    l = _logits(T, E, dtype, 6, 0.2)
+    l[3::17] = 1.0  # the oracle's softmax takes exp of the logits themselves
+    g = torch.Generator().manual_seed(7)
+    dw = torch.randn(T, k, generator=g).to(dtype)
+    x = l.to(gpu).requires_grad_()
+    w, i = ops.expert_route(x, k, score, renormalize=renorm, scale=1.5)
+    (dl,) = torch.autograd.grad(w, x, dw.to(gpu))
+    l64 = torch.where(torch.isfinite(l.double()), l.double(), math.nan).requires_grad_()
+    (want,) = torch.autograd.grad(O.route_weights(l64, i.cpu(), score, renorm, 1.5), l64, dw.double())
+    want = want.nan_to_num(0.0)
+    s, ok = O.scores(l, score)
+    have = i.cpu() >= 0
+    sel = s.gather(1, i.cpu().clamp_min(0).long()) * have
+    S = sel.sum(1, keepdim=True) if renorm else torch.ones(T, 1, dtype=torch.float64)
+    S = torch.where(S > 0, S, 1.0)
+    a = (dw.double().abs() * sel).sum(1, keepdim=True)
+    mag = 1.5 / S * (torch.zeros(T, E, dtype=torch.float64).scatter_add_(1, i.cpu().clamp_min(0).long(), dw.double().abs() * have)
+                     + a / S)
+    mag = s * (mag + (1.5 / S * 2 * a if score == "softmax" else 0))
+    half = 2.0**-8 if dtype == torch.bfloat16 else U
+    tol = U * (30 + 100 + 2 * k) * mag + half * want.abs() + 1e-37
+    assert ((dl.cpu().double() - want).abs() <= tol).all()
+    assert (dl.cpu()[~ok] == 0).all()
+
+
+def test_route_repeats_and_replays(gpu):
+    l = _logits(1000, 64, torch.float32, 8).to(gpu)
+    b = (torch.randn(64, generator=torch.Generator().manual_seed(1)) * 0.1).to(gpu)
+    call = lambda: ops.expert_route(l, 8, "sigmoid", b, 8, 4)  # noqa: E731
+    want = [t.clone() for t in call()]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = call()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        again = call()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) and torch.equal(x, z) for x, y, z in zip(want, got, again))
+
+
+@pytest.mark.parametrize("n,E", [(0, 3), (1, 1), (2, 8), (63, 5), (64, 64), (65, 2), (1000, 100), (1024, 512), (1025, 8),
+                                 (5000, 1), (4097, 300), (70000, 24), (40000, 512)])
+def test_plan(gpu, n, E):
+    """Rows sorted by expert, stable; offsets and tiles; indices that name no expert left out."""
+    print(f"plan {n} {E}", flush=True)
+    g = torch.Generator().manual_seed(n)
+    idx = (torch.rand(n, generator=g) ** 2 * E).int()
+    idx[torch.rand(n, generator=g) < 0.1] = -1
+    if n > 4:
+        idx[3], idx[4] = E, 2**31 - 1
+    plan, tile = ops._expert_plan(idx.to(gpu), E)
+    plan = plan.cpu()
+    row_slot, slot_row, off = plan[:n], plan[n:2 * n], plan[2 * n:2 * n + E + 1]
+    tiles = plan[2 * n + E + 1:]
+    ok = (idx >= 0) & (idx < E)
+    order = torch.where(ok, idx, E).sort(stable=True).indices[: int(ok.sum())]
+    R = order.numel()
+    assert torch.equal(row_slot[:R].long(), order)
+    want = torch.full((n,), -1, dtype=torch.int32)
+    want[order] = torch.arange(R, dtype=torch.int32)
+    assert torch.equal(slot_row, want)
+    count = torch.bincount(idx[ok].long(), minlength=E)
+    assert torch.equal(off.long(), torch.cat([torch.zeros(1, dtype=torch.int64), count.cumsum(0)]))
+    wt = [(e, int(off[e]) + k) for e in range(E) for k in range(0, int(count[e]), tile)]
+    assert int(tiles[0]) == len(wt)
+    assert tiles[1:1 + 2 * len(wt)].view(-1, 2).tolist() == [list(t) for t in wt]
+    assert tile == _lib.load().strata_hip_expert_tile(n, E)
