@@ -619,21 +619,26 @@ int strata_hip_expert_route_bwd(const strata_hip_expert_route_args* args, void* 
 
 /* The order in which the experts' products take the chosen (token, slot) pairs: by expert,
  * pairs of one expert in their own order.  An index outside [0, experts) drops its pair.
- * index: [pairs].  Out: row_slot[r] the pair of row r ([pairs], rows past the last one stay
+ * index: [pairs], pair = token * top_k + slot; weights: bf16 [pairs].  Out: row_token[r] and
+ * row_weight[r], the token and the weight of row r's pair ([pairs], rows past the last one stay
  * as they were); slot_row[s] the row of pair s or -1; offsets[e] the first row of expert e,
  * offsets[experts] the number of rows; tiles: [1 + 2 * (pairs / tile + experts)], the
  * number of row tiles, then (expert, first row) of each: up to `tile` rows of one expert.
  * workspace: strata_hip_expert_plan_workspace() int32 (NULL when that is 0). */
 typedef struct strata_hip_expert_plan_args {
   const int32_t* index;
-  int32_t* row_slot;
+  const void* weights;
+  int32_t* row_token;
+  float* row_weight;
   int32_t* slot_row;
   int32_t* offsets;
   int32_t* tiles;
   int32_t* workspace;
   int64_t pairs;
+  int32_t top_k;
   int32_t experts;
   int32_t tile;
+  int32_t reserved;
 } strata_hip_expert_plan_args;
 
 int64_t strata_hip_expert_plan_workspace(int64_t pairs, int32_t experts);
@@ -644,20 +649,21 @@ int strata_hip_expert_plan(const strata_hip_expert_plan_args* args, void* stream
  * screamcast/checkpoint_compat.py:243-249) with weights of its own for each expert:
  *   out[t] = residual[t] + sum over s of weights[t, s] (gelu(x[t] w1_e^T + b1_e) w2_e^T + b2_e)
  * for the pairs (t, s) that the plan (strata_hip_expert_plan with tile =
- * strata_hip_expert_tile(tokens * top_k, experts)) gives a row; e is the row's expert.
+ * strata_hip_expert_tile()) gives a row; e is the row's expert.
  * x: [tokens, dim], row stride ldx; weights: [tokens, top_k]; w1 [experts, hidden, dim],
  * b1 [experts, hidden] or NULL, w2 [experts, out_dim, hidden], b2 [experts, out_dim] or NULL,
  * residual [tokens, out_dim] (row stride ldr) or NULL, out [tokens, out_dim]: bf16, contiguous
  * where no stride is given, fp32 accumulation.  Widths multiples of 8, at most 32768; x and
  * out under 2 GiB.  Workspaces, rows of the plan's order (rows past the last one stay as they
- * were): h [pairs, hidden] bf16, y [pairs, out_dim] fp32, dact [pairs, hidden] bf16 or NULL:
- * gelu' for a backward, which reads h, y and dact again.  x, w, h, y, dact, out, residual
+ * were): h [pairs, hidden] bf16, y [pairs, out_dim] fp32, dact [pairs, hidden] fp16 or NULL:
+ * gelu' for a backward, which reads h, y and dact again.  A weight under 2^-100 counts as 0.  x, w, h, y, dact, out, residual
  * 16-byte aligned, b1, b2 8-byte.  The order of every sum is fixed by the sizes and the plan.
  * ------------------------------------------------------------------------- */
 typedef struct strata_hip_expert_mlp_args {
   const void* x;
   const void* weights;
-  const int32_t* row_slot;
+  const int32_t* row_token;
+  const float* row_weight;
   const int32_t* slot_row;
   const int32_t* offsets;
   const int32_t* tiles;
@@ -674,15 +680,15 @@ typedef struct strata_hip_expert_mlp_args {
   int32_t top_k, experts, dim, hidden, out_dim, tile;
 } strata_hip_expert_mlp_args;
 
-int32_t strata_hip_expert_tile(int64_t pairs, int32_t experts);
+int32_t strata_hip_expert_tile(int64_t pairs, int32_t experts, int32_t dim, int32_t hidden, int32_t out_dim);
 int strata_hip_expert_mlp(const strata_hip_expert_mlp_args* args, void* stream);
 
 /* Gradients of strata_hip_expert_mlp for dout [tokens, out_dim] bf16 contiguous; `fwd` as in the
  * forward (out and residual are not read; the residual's gradient is dout).  Each of dx
  * [tokens, dim], dweights [tokens, top_k], dw1, db1, dw2, db2 (the shapes of their weights, bf16)
  * may be NULL, a weight's only with its bias's; a dropped pair's dweights and an
- * unused expert's gradients are zero.  Workspaces in bf16: gs [pairs, out_dim] for dw2,
- * gz [pairs, hidden] and w2t (w2's elements) for dx or dw1, dxs [pairs, dim] and w1t for dx. */
+ * unused expert's gradients are zero.  Workspaces: gz [pairs, hidden] bf16 for dx or dw1,
+ * dxs [pairs, dim] fp32 for dx. */
 typedef struct strata_hip_expert_mlp_bwd_args {
   strata_hip_expert_mlp_args fwd;
   const void* dout;
@@ -692,11 +698,8 @@ typedef struct strata_hip_expert_mlp_bwd_args {
   void* db1;
   void* dw2;
   void* db2;
-  void* gs;
   void* gz;
-  void* dxs;
-  void* w1t;
-  void* w2t;
+  float* dxs;
 } strata_hip_expert_mlp_bwd_args;
 
 int strata_hip_expert_mlp_bwd(const strata_hip_expert_mlp_bwd_args* args, void* stream);

@@ -94,8 +94,8 @@ def mlp_bounds(x, weights, index, w1, b1, w2, b2, residual, dout=None) -> dict:
     u = 2^-24, v = 2^-8 (half a step of fp32 and bf16, relative).  A sum of n products in fp32 is off
     by at most n u of the sum of their magnitudes (any order), and its operands' own bounds are
     carried through; GELU and its derivative have slopes of at most 1.13 and 1.3 and are evaluated
-    within 32 u of max(1, |z|); h, gelu', gs, gz, the rows of dx and every output are rounded to
-    bf16 once."""
+    within 32 u of max(1, |z|); h (scaled by its pair's weight), gz and every output are rounded to
+    bf16 once, gelu' to fp16 (v / 8, and 2^-24 below its normal numbers)."""
     u, v = 2.0**-24, 2.0**-8
     x, weights, w1, w2 = (a.double() for a in (x, weights, w1, w2))
     b1 = b1.double() if b1 is not None else None
@@ -139,15 +139,14 @@ def mlp_bounds(x, weights, index, w1, b1, w2, b2, residual, dout=None) -> dict:
         g = g_all[tok]
         dwt[tok, slot] = (g * y).sum(1)
         dwtb[tok, slot] = (g.abs() * ey).sum(1) + (N + 8) * u * (g * y).abs().sum(1)
-        gs = we * g
-        egs = (v + u) * gs.abs()
-        dw2[e] = gs.T @ h
-        dw2b[e] = egs.T @ (h.abs() + eh) + gs.abs().T @ eh + (R + 2) * u * (gs.abs().T @ h.abs())
-        db2[e] = gs.sum(0)
-        db2b[e] = egs.sum(0) + (R + 2) * u * gs.abs().sum(0)
+        hs, ehs = we * h, we.abs() * (eh + u * h.abs())
+        dw2[e] = g.T @ hs
+        dw2b[e] = g.abs().T @ ehs + (R + 2) * u * (g.abs().T @ (hs.abs() + ehs))
+        db2[e] = (we * g).sum(0)
+        db2b[e] = (R + 2) * u * (we * g).abs().sum(0)
         gh, gha = g @ b, g.abs() @ b.abs()
         ed0 = 1.3 * ez + 32 * u * z.abs().clamp_min(1)
-        ed = ed0 + v * (d.abs() + ed0)
+        ed = ed0 + v / 8 * (d.abs() + ed0) + u
         gz = we * gh * d
         egz0 = we.abs() * ((N + 4) * u * gha * (d.abs() + ed) + gh.abs() * ed)
         egz = egz0 + v * (gz.abs() + egz0)
@@ -159,7 +158,7 @@ def mlp_bounds(x, weights, index, w1, b1, w2, b2, residual, dout=None) -> dict:
         er0 = egz @ a.abs() + (H + 2) * u * ((gz.abs() + egz) @ a.abs())
         dx.index_add_(0, tok, r)
         dxm.index_add_(0, tok, r.abs())
-        dxb.index_add_(0, tok, er0 + v * (r.abs() + er0))
+        dxb.index_add_(0, tok, er0)
     half = lambda val, b: b + v * (val.abs() + b) + 1e-40  # noqa: E731  (the last rounding)
     res["out"] = (out, half(out, bad + (k + 2) * u * mag))
     if dout is not None:

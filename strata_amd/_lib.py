@@ -357,19 +357,23 @@ class ExpertRouteArgs(ctypes.Structure):
 class ExpertPlanArgs(ctypes.Structure):
     _fields_ = [
         ("index", ctypes.c_void_p),
-        ("row_slot", ctypes.c_void_p),
+        ("weights", ctypes.c_void_p),
+        ("row_token", ctypes.c_void_p),
+        ("row_weight", ctypes.c_void_p),
         ("slot_row", ctypes.c_void_p),
         ("offsets", ctypes.c_void_p),
         ("tiles", ctypes.c_void_p),
         ("workspace", ctypes.c_void_p),
         ("pairs", ctypes.c_int64),
+        ("top_k", ctypes.c_int32),
         ("experts", ctypes.c_int32),
         ("tile", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
     ]
 
 
 class ExpertMlpArgs(ctypes.Structure):
-    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "weights", "row_slot", "slot_row", "offsets", "tiles", "w1", "b1", "w2",
+    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "weights", "row_token", "row_weight", "slot_row", "offsets", "tiles", "w1", "b1", "w2",
                                                "b2", "residual", "out", "h", "dact", "y")] + \
         [(n, ctypes.c_int64) for n in ("tokens", "ldx", "ldr")] + \
         [(n, ctypes.c_int32) for n in ("top_k", "experts", "dim", "hidden", "out_dim", "tile")]
@@ -377,7 +381,7 @@ class ExpertMlpArgs(ctypes.Structure):
 
 class ExpertMlpBwdArgs(ctypes.Structure):
     _fields_ = [("fwd", ExpertMlpArgs)] + \
-        [(n, ctypes.c_void_p) for n in ("dout", "dx", "dweights", "dw1", "db1", "dw2", "db2", "gs", "gz", "dxs", "w1t", "w2t")]
+        [(n, ctypes.c_void_p) for n in ("dout", "dx", "dweights", "dw1", "db1", "dw2", "db2", "gz", "dxs")]
 
 
 class AdamwTensor(ctypes.Structure):
@@ -457,7 +461,7 @@ EXPORTS = {
     "strata_hip_expert_route_bwd": ([ctypes.POINTER(ExpertRouteArgs), ctypes.c_void_p], ctypes.c_int),
     "strata_hip_expert_plan": ([ctypes.POINTER(ExpertPlanArgs), ctypes.c_void_p], ctypes.c_int),
     "strata_hip_expert_plan_workspace": ([ctypes.c_int64, ctypes.c_int32], ctypes.c_int64),
-    "strata_hip_expert_tile": ([ctypes.c_int64, ctypes.c_int32], ctypes.c_int32),
+    "strata_hip_expert_tile": ([ctypes.c_int64] + [ctypes.c_int32] * 4, ctypes.c_int32),
     "strata_hip_expert_mlp": ([ctypes.POINTER(ExpertMlpArgs), ctypes.c_void_p], ctypes.c_int),
     "strata_hip_expert_mlp_bwd": ([ctypes.POINTER(ExpertMlpBwdArgs), ctypes.c_void_p], ctypes.c_int),
     "strata_hip_adamw_workspace": ([ctypes.POINTER(AdamwTensor), ctypes.c_int64], ctypes.c_int64),

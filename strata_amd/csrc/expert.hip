@@ -2,23 +2,30 @@
 //
 //   out[t] = residual[t] + sum over slots s of w[t, s] (gelu(x[t] W1_e^T + b1_e) W2_e^T + b2_e),  e = index[t, s]
 //
-// Row r of the products is the pair (t, s) = row_slot[r] of the plan; the first product
-// gathers its rows of x as it copies them into LDS, so no sorted copy of x exists.  Forward:
-//   h = gelu(x[t] W1_e^T + b1_e)       bf16 (the second product's operand), with gelu' for a backward
-//   y = h W2_e^T + b2_e                fp32: out is rounded once
-//   out[t] = residual[t] + sum_s w y   in slot order
+// Row r of the products is a pair (t, s) in the plan's order; products over tokens gather
+// their rows as they copy them into LDS, so no sorted copy of x or dout exists.  The pair's
+// weight scales its hidden row before that is rounded to bf16, so the sum over slots needs
+// no weights and dW2 no scaled copy of dout:
+//   h_r = w' gelu(x[t] W1_e^T + b1_e)  bf16, with gelu' in fp16 (its values lie in (-0.13, 1.13)) for a backward
+//   y_r = h_r W2_e^T + w' b2_e         fp32: out is rounded once
+//   out[t] = residual[t] + sum_s y     in slot order
+// w' = w, or 1 where |w| < 2^-100: such a pair adds nothing, but its weight has a gradient.
 // Backward, g = dout:
-//   dw[t, s] = <g[t], y_r>             gs_r = w g[t], bf16 (an operand of dW2)
+//   dw[t, s] = <g[t], y_r> / w'
 //   gz_r = w (g[t] W2_e) gelu'         bf16 (an operand of the next three)
-//   dW2_e = sum_r gs_r^T h_r  db2_e = sum_r gs_r  dW1_e = sum_r gz_r^T x[t]  db1_e = sum_r gz_r
-//   dx[t] = sum_s (gz W1_e)_r          rows in bf16, summed in fp32 in slot order
-// Each intermediate is rounded once, where a matrix instruction needs bf16.  Every sum has
-// an order fixed by the sizes and the plan: results repeat bit for bit.
+//   dW2_e = sum_r g[t]^T h_r  db2_e = sum_r w g[t]  dW1_e = sum_r gz_r^T x[t]  db1_e = sum_r gz_r
+//   dx[t] = sum_s (gz W1_e)_r          fp32 rows, in slot order
+// Each gradient then has one rounding of an operand to bf16 and its own.  The backward's
+// products take the weights along their rows: they are read transposed out of LDS
+// (ds_read_b64_tr_b16), no transposed copy is made.  Every sum has an order fixed by the
+// sizes and the plan: results repeat bit for bit.
 #include <algorithm>
 
 #include "common.h"
 
 namespace strata {
+
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ void gelu_both(float x, float& y, float& d) {
   // x s and its derivative s + x s (1 - s) 2u' with s = sigmoid(2u), u = sqrt(2/pi) (x + 0.044715 x^3)
@@ -29,42 +36,62 @@ __device__ __forceinline__ void gelu_both(float x, float& y, float& d) {
   d = fmaf(y * (1.f - s), 2.f * c * fmaf(3.f * 0.044715f, x * x, 1.f), s);
 }
 
+// Whether a pair's weight counts as nothing, and what its row is scaled by (a weight that
+// is no number scales).
+__device__ __forceinline__ bool no_weight(float w) { return fabsf(w) < 0x1p-100f; }
+__device__ __forceinline__ float row_scale(float w) { return no_weight(w) ? 1.f : w; }
+
 struct ExpertGemm {
   const bf16* x;
-  const int32_t* rows;   // gather: row r of the product is row rows[r] / top_k of x; or null
-  const bf16* w;         // [E, N, K]
+  const bf16* w;         // [E, N, K], WT: [E, K, N]
   const bf16* bias;      // [E, N] or null
-  const bf16* mul;       // HIDDEN_GRAD: gelu', [P, N]
-  const bf16* scale;     // HIDDEN_GRAD: the weight of each pair, by rows[r]
-  const int32_t* slots;  // HIDDEN_GRAD: row_slot
+  const _Float16* mul;   // HIDDEN_GRAD: gelu', [P, N]
   void* out;             // [P, N] bf16, OUT: fp32
-  bf16* out2;            // HIDDEN: gelu' or null
+  _Float16* out2;        // HIDDEN: gelu' or null
+  const int32_t* token;  // row_token and row_weight of the plan
+  const float* weight;
   const int32_t* offsets;
   const int32_t* tiles;
   int64_t ldx;
-  int top_k, N, K, nt;
+  int N, K, nt;
 };
 
-enum { EX_HIDDEN = 0, EX_OUT = 1, EX_HIDDEN_GRAD = 2, EX_INPUT_GRAD = 3 };
+enum { EX_HIDDEN = 0, EX_OUT = 1, EX_HIDDEN_GRAD = 2 };
 
-template <int CH>
-__device__ __forceinline__ int ex_swz(int chunk, int row) {
-  return chunk ^ ((row & 7) ^ ((row >> 3) & 1));
+// Chunks of 16 bytes of an LDS row are stored at their index xor these:
+// K-contiguous rows of 128 bytes, read 16 bytes a lane by 32 rows at one chunk, and
+// (WT) rows of BN columns, read transposed by 8 rows at 4 chunks: each instruction's
+// lanes then spread over all banks.
+__device__ __forceinline__ int ex_swz(int row) { return (row & 7) ^ ((row >> 3) & 1); }
+template <int BN>
+__device__ __forceinline__ int ex_wswz(int row) {
+  return BN == 64 ? ((row >> 1) & 1) << 2 : (row & 3) << 2;
 }
 
-// One BM x BN tile of one expert's product a workgroup: x and w tiles stream into an
-// LDS ring of NST stages of 64 columns, NST - 1 stages ahead of the v_mfma_f32_32x32x16_bf16.
-// The weights are the MFMA's A operand: a lane owns four consecutive columns of one row.
-template <int BM, int BN, int WGM, int WGN, int NST, int MODE>
-__global__ __launch_bounds__(64 * WGM * WGN) void expert_gemm_kernel(ExpertGemm p) {
+struct ExpertTile {
+  int e, row0, rows, n0;
+};
+
+// BM x BN tiles of the experts' products: x and w stream into an LDS ring of NST stages of
+// 64 columns (buffer_load ... lds) ahead of v_mfma_f32_32x32x16_bf16, whose A operand the
+// weights are: a lane owns four consecutive columns of one row.
+// BIG: 256 x 256, one workgroup a CU walks over the tiles; the last step of a tile starts
+// the next one's first stage, whose rows' tokens were loaded a tile ahead.  Otherwise one
+// tile a workgroup and several workgroups a CU.
+template <int BM, int BN, int WGM, int WGN, int NST, int MODE, bool WT>
+__global__ __launch_bounds__(64 * WGM * WGN, 1) void expert_gemm_kernel(ExpertGemm p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  constexpr bool BIG = BM == 256, GATHER = MODE != EX_OUT;
   constexpr int BK = 64, NW = WGM * WGN;
   constexpr int WTM = BM / WGM, WTN = BN / WGN, FM = WTM / 32, FN = WTN / 32;
   constexpr int ROWB = BK * 2, CH = ROWB / 16, RPC = 1024 / ROWB;
   constexpr int XB = BM * ROWB, XCH = XB / 1024, STAGE = XB + BN * ROWB;
-  constexpr int LPW = STAGE / 1024 / NW;
-  constexpr int SLAB = WTM * WTN * 2;
+  constexpr int LPX = XCH / NW, LPW = BN * ROWB / 1024 / NW;  // 1-KiB copies a wave and stage
+  constexpr int WLPR = BN / 8, WRPC = 64 / WLPR;             // WT: lanes a row, rows a copy
+  constexpr int HALVES = BIG ? 2 : 1, HM = FM / HALVES;
+  constexpr int SLAB = HM * 32 * WTN * 2;
   static_assert(WTM % 32 == 0 && WTN % 32 == 0 && XCH % NW == 0 && (STAGE / 1024) % NW == 0, "wave tile / stage layout");
-  static_assert(NW * SLAB <= NST * STAGE, "the epilogue slabs fit the ring");
+  static_assert(NW * SLAB <= (BIG ? STAGE : NST * STAGE) && (!BIG || NST == 2), "the epilogue slabs fit the ring");
   __shared__ __attribute__((aligned(1024))) char lds[NST * STAGE];
 
   const int tid = (int)__builtin_amdgcn_workitem_id_x();
@@ -73,212 +100,324 @@ __global__ __launch_bounds__(64 * WGM * WGN) void expert_gemm_kernel(ExpertGemm 
   const uint32_t lds_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
 
   // The grid is sized for the most tiles that the pairs can make; the plan says how many there are.
-  const int mt = p.tiles[0], total = mt * p.nt, id = (int)__builtin_amdgcn_workgroup_id_x();
-  if (id >= total) return;
-  int tm, n0;
-  {
-    const int wg = xcd_tile_order(total, id);
-    constexpr int GRP = 8;
+  const int mt = p.tiles[0], total = mt * p.nt, wg_id = (int)__builtin_amdgcn_workgroup_id_x();
+  if (wg_id >= total) return;
+  auto tile_at = [&](int t) {
+    const int wg = xcd_tile_order(total, t);
+    constexpr int GRP = BIG ? 4 : 8;  // row panels x every column panel, row panel fastest
     const int gi = wg / (GRP * p.nt), li = wg % (GRP * p.nt), gmn = min(GRP, mt - gi * GRP);
-    tm = gi * GRP + li % gmn;
-    n0 = (li / gmn) * BN;
-  }
-  const int e = p.tiles[1 + 2 * tm], row0 = p.tiles[2 + 2 * tm];
-  const int rows = min(p.offsets[e + 1] - row0, BM);  // rows of this tile
-  const bf16* we = p.w + (int64_t)e * p.N * p.K;
-
-  uint32_t voff[LPW];
-#pragma unroll
-  for (int j = 0; j < LPW; ++j) {
-    const bool isw = j * NW >= XCH;
-    const int c = j * NW + wave - (isw ? XCH : 0), row = RPC * c + lane / CH;
-    const uint32_t chunk = ex_swz<CH>(lane % CH, row) * 16;
-    if (isw) {
-      voff[j] = n0 + row < p.N ? (uint32_t)((uint32_t)row * p.K * 2) + chunk : OOB;
-    } else {
-      int64_t at = row;
-      if (p.rows && row < rows) at = p.rows[row0 + row] / p.top_k;
-      voff[j] = row < rows ? (uint32_t)(at * p.ldx * 2) + chunk : OOB;
-    }
-  }
+    const int tm = gi * GRP + li % gmn;
+    ExpertTile r;
+    r.e = p.tiles[1 + 2 * tm];
+    r.row0 = p.tiles[2 + 2 * tm];
+    r.rows = min(p.offsets[r.e + 1] - r.row0, BM);
+    r.n0 = (li / gmn) * BN;
+    return r;
+  };
   const int nk = (p.K + BK - 1) / BK, ktail = p.K % BK;
-  const char* xk = (const char*)(p.rows ? p.x : p.x + (int64_t)row0 * p.ldx);
-  const char* wk = (const char*)(we + (int64_t)n0 * p.K);
-  auto issue = [&](int kt, int slot) {
-    const u32x4 rx = make_rsrc(xk + (int64_t)kt * BK * 2, OOB), rw = make_rsrc(wk + (int64_t)kt * BK * 2, OOB);
+  // lane offsets of a tile's x rows
+  auto x_offsets = [&](const ExpertTile& t, uint32_t (&vo)[LPX]) {
+#pragma unroll
+    for (int j = 0; j < LPX; ++j) {
+      const int row = RPC * (j * NW + wave) + lane / CH;
+      const uint32_t chunk = ((lane % CH) ^ ex_swz(row)) * 16;
+      int64_t at = row;
+      if (GATHER && row < t.rows) at = p.token[t.row0 + row];
+      vo[j] = row < t.rows ? (uint32_t)(at * p.ldx * 2) + chunk : OOB;
+    }
+  };
+  auto w_offsets = [&](const ExpertTile& t, uint32_t (&vo)[LPW]) {
+#pragma unroll
+    for (int j = 0; j < LPW; ++j) {
+      if (WT) {
+        const int row = WRPC * (j * NW + wave) + lane / WLPR, chunk = (lane % WLPR) ^ ex_wswz<BN>(row);
+        vo[j] = t.n0 + 8 * chunk < p.N ? (uint32_t)((uint32_t)row * p.N * 2) + chunk * 16 : OOB;
+      } else {
+        const int row = RPC * (j * NW + wave) + lane / CH, chunk = (lane % CH) ^ ex_swz(row);
+        vo[j] = t.n0 + row < p.N ? (uint32_t)((uint32_t)row * p.K * 2) + chunk * 16 : OOB;
+      }
+    }
+  };
+  auto issue_x = [&](const ExpertTile& t, const uint32_t (&vo)[LPX], int kt, int slot) {
+    const bf16* base = GATHER ? p.x : p.x + (int64_t)t.row0 * p.ldx;
+    const u32x4 r = make_rsrc((const char*)base + (int64_t)kt * BK * 2, OOB);
     const uint32_t dst = lds_base + slot * STAGE + wave * 1024;
     const bool last = ktail && kt == nk - 1;  // uniform: chunks at or past K read as zero
 #pragma unroll
+    for (int j = 0; j < LPX; ++j) {
+      uint32_t o = vo[j];
+      if (last && ((lane % CH) ^ ex_swz(RPC * (j * NW + wave) + lane / CH)) * 8 >= ktail) o = OOB;
+      dma_row16(r, dst + j * NW * 1024, o);
+    }
+  };
+  auto issue_w = [&](const ExpertTile& t, const uint32_t (&vo)[LPW], int kt, int slot) {
+    const bf16* base = p.w + (int64_t)t.e * p.N * p.K + (WT ? (int64_t)kt * BK * p.N + t.n0 : (int64_t)t.n0 * p.K + kt * BK);
+    const u32x4 r = make_rsrc(base, OOB);
+    const uint32_t dst = lds_base + slot * STAGE + XB + wave * 1024;
+    const bool last = ktail && kt == nk - 1;
+#pragma unroll
     for (int j = 0; j < LPW; ++j) {
-      const bool isw = j * NW >= XCH;
-      uint32_t vo = voff[j];
+      uint32_t o = vo[j];
       if (last) {
-        const int row = RPC * (j * NW + wave - (isw ? XCH : 0)) + lane / CH;
-        if (ex_swz<CH>(lane % CH, row) * 8 >= ktail) vo = OOB;
+        if (WT ? WRPC * (j * NW + wave) + lane / WLPR >= ktail
+               : ((lane % CH) ^ ex_swz(RPC * (j * NW + wave) + lane / CH)) * 8 >= ktail)
+          o = OOB;
       }
-      dma_row16(isw ? rw : rx, dst + j * NW * 1024, vo);
+      dma_row16(r, dst + j * NW * 1024, o);
     }
   };
 
-  // The bias as the accumulators' first C operand (columns 8q + 4hi + e of each 32).
-  const int gn0 = n0 + wn * WTN;
-  f32x16 acc[FN][FM];
-#pragma unroll
-  for (int i = 0; i < FN; ++i)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      u32x2 bb = {0u, 0u};
-      if (MODE <= EX_OUT && p.bias) bb = *(const u32x2*)(p.bias + (int64_t)e * p.N + min(gn0 + 32 * i + 8 * q + 4 * hi, p.N - 4));
-#pragma unroll
-      for (int j = 0; j < FM; ++j) {
-        acc[i][j][4 * q + 0] = bf16_lo(bb[0]);
-        acc[i][j][4 * q + 1] = bf16_hi(bb[0]);
-        acc[i][j][4 * q + 2] = bf16_lo(bb[1]);
-        acc[i][j][4 * q + 3] = bf16_hi(bb[1]);
-      }
-    }
-
-  uint32_t aoff[FN][2], boff[FM][2];  // sub-steps 2, 3 flip bit 2 of the chunk: offset ^ 64
+  // LDS offsets of the fragments: x (and w) for K sub-steps 0, 1 (2, 3 flip bit 2 of the chunk:
+  // offset ^ 64); WT: rows 8 hi + 4 half + (lane & 15) / 4 of columns 32 i + 16 ((lane >> 4) & 1).
+  uint32_t aoff[FN][WT ? 1 : 2], boff[FM][2];
 #pragma unroll
   for (int i = 0; i < FN; ++i) {
-    const int row = wn * WTN + 32 * i + l32;
-    for (int kk = 0; kk < 2; ++kk) aoff[i][kk] = XB + row * ROWB + ex_swz<CH>(2 * kk + hi, row) * 16;
+    if (WT) {
+      const int r4 = (lane & 15) >> 2, c = (wn * WTN + 32 * i) / 8 + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+      aoff[i][0] = XB + (8 * hi + r4) * (BN * 2) + ((c ^ ex_wswz<BN>(r4)) << 4) + 8 * (lane & 1);
+    } else {
+      const int row = wn * WTN + 32 * i + l32;
+      for (int kk = 0; kk < 2; ++kk) aoff[i][WT ? 0 : kk] = XB + row * ROWB + ((2 * kk + hi) ^ ex_swz(row)) * 16;
+    }
   }
 #pragma unroll
   for (int j = 0; j < FM; ++j) {
     const int row = wm * WTM + 32 * j + l32;
-    for (int kk = 0; kk < 2; ++kk) boff[j][kk] = row * ROWB + ex_swz<CH>(2 * kk + hi, row) * 16;
+    for (int kk = 0; kk < 2; ++kk) boff[j][kk] = row * ROWB + ((2 * kk + hi) ^ ex_swz(row)) * 16;
   }
-
+  auto load_frags = [&](const char* st, int kk, bf16x8 (&a)[FN], bf16x8 (&b)[FM]) {
 #pragma unroll
-  for (int s = 0; s < NST - 1; ++s)
-    if (s < nk) issue(s, s);
-  int rd = 0;
-  for (int kt = 0; kt < nk; ++kt) {
-    if (NST > 2 && kt + NST - 2 < nk) wait_vmcnt((NST - 2) * LPW);
-    else wait_vmcnt(0);
-    lds_barrier();  // landed for every wave, and the slot read last step is free
-    const int wr = rd == 0 ? NST - 1 : rd - 1;
-    if (kt + NST - 1 < nk) issue(kt + NST - 1, wr);
-    const char* st = lds + rd * STAGE;
-    rd = rd + 1 == NST ? 0 : rd + 1;
-    bf16x8 af[2][FN], bfr[2][FM];
-    auto load_frags = [&](int kk, int buf) {
-#pragma unroll
-      for (int i = 0; i < FN; ++i) af[buf][i] = *(const bf16x8*)(st + (aoff[i][kk & 1] ^ ((kk >> 1) * 64)));
-#pragma unroll
-      for (int j = 0; j < FM; ++j) bfr[buf][j] = *(const bf16x8*)(st + (boff[j][kk & 1] ^ ((kk >> 1) * 64)));
-    };
-    load_frags(0, 0);
-#pragma unroll
-    for (int kk = 0; kk < BK / 16; ++kk) {
-      const int cb = kk & 1;
-      if (kk + 1 < BK / 16) load_frags(kk + 1, cb ^ 1);
-#pragma unroll
-      for (int i = 0; i < FN; ++i)
-#pragma unroll
-        for (int j = 0; j < FM; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af[cb][i], bfr[cb][j], acc[i][j], 0, 0, 0);
+    for (int i = 0; i < FN; ++i) {
+      if constexpr (WT) {
+        const char* q = st + aoff[i][0] + kk * 16 * (BN * 2);
+        const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, q));
+        const bf16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, q + 4 * (BN * 2)));
+        a[i] = __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7);
+      } else {
+        a[i] = *(const bf16x8*)(st + (aoff[i][kk & 1] ^ ((kk >> 1) * 64)));
+      }
     }
-  }
+#pragma unroll
+    for (int j = 0; j < FM; ++j) b[j] = *(const bf16x8*)(st + (boff[j][kk & 1] ^ ((kk >> 1) * 64)));
+  };
 
-  // ---- epilogue ----
-  const int wr0 = wm * WTM;  // first row of the wave's tile
-  if constexpr (MODE == EX_OUT) {  // fp32, straight from the accumulators
-    float* out = (float*)p.out;
+  f32x16 acc[FN][FM];
+  ExpertTile t = tile_at(wg_id), tn = t;
+  uint32_t xo[LPX], xn[LPX], wo[LPW];
+  x_offsets(t, xo);
+  int rd = 0, wr = 1;
+  bool in_flight = false;  // BIG: the tile's first stage was issued by the previous tile
+  for (int ti = wg_id; ti < total; ti += (int)gridDim.x) {
+    const bool more = BIG && ti + (int)gridDim.x < total;
+    w_offsets(t, wo);
+    if (BIG) {
+      if (!in_flight) {
+        issue_x(t, xo, 0, rd);
+        issue_w(t, wo, 0, rd);
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < NST - 1; ++s)
+        if (s < nk) {
+          issue_x(t, xo, s, s);
+          issue_w(t, wo, s, s);
+        }
+    }
+    const int gn0 = t.n0 + wn * WTN, wr0 = wm * WTM;
+    // the rows' weights: scale of h, factor of the bias, factor of gz
+    float rw[FM];
+    const bool weigh = MODE != EX_OUT || p.bias;  // uniform
 #pragma unroll
     for (int j = 0; j < FM; ++j) {
       const int r = wr0 + 32 * j + l32;
-      if (r >= rows) continue;
-#pragma unroll
-      for (int i = 0; i < FN; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int gn = gn0 + 32 * i + 8 * q + 4 * hi;
-          if (gn < p.N)
-            *(f32x4*)(out + (int64_t)(row0 + r) * p.N + gn) =
-                (f32x4){acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-        }
+      rw[j] = weigh && r < t.rows ? p.weight[t.row0 + r] : 0.f;
+      if (MODE != EX_HIDDEN_GRAD) rw[j] = row_scale(rw[j]);
     }
-    return;
-  }
-  if constexpr (MODE == EX_HIDDEN_GRAD) {
-#pragma unroll
-    for (int j = 0; j < FM; ++j) {
-      const int r = wr0 + 32 * j + l32;
-      const bool in = r < rows;
-      const float w = in ? (float)p.scale[p.slots[row0 + r]] : 0.f;
-#pragma unroll
-      for (int i = 0; i < FN; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int gn = gn0 + 32 * i + 8 * q + 4 * hi;
-          u32x2 d = {0u, 0u};
-          if (in && gn < p.N) d = *(const u32x2*)(p.mul + (int64_t)(row0 + r) * p.N + gn);
-          acc[i][j][4 * q + 0] *= w * bf16_lo(d[0]);
-          acc[i][j][4 * q + 1] *= w * bf16_hi(d[0]);
-          acc[i][j][4 * q + 2] *= w * bf16_lo(d[1]);
-          acc[i][j][4 * q + 3] *= w * bf16_hi(d[1]);
-        }
-    }
-  }
-  // bf16 through this wave's LDS slab, 16-byte rows out
-  lds_barrier();  // every wave is done reading the ring
-  constexpr int SRB = WTN * 2, CPR = WTN / 8, RPI = 64 / CPR, NIT = WTM / RPI;
-  char* slab = lds + wave * SLAB;
-  const int c = lane % CPR, gn = gn0 + 8 * c;
-  const bool col = gn < p.N;  // N is a multiple of 8: the whole 16-byte run
-  auto to_slab = [&](auto f) {
+    // the bias as the accumulators' first C operand (columns 8q + 4hi + e of each 32)
 #pragma unroll
     for (int i = 0; i < FN; ++i)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int nl = 32 * i + 8 * q + 4 * hi;
+        u32x2 bb = {0u, 0u};
+        if (MODE != EX_HIDDEN_GRAD && p.bias)
+          bb = *(const u32x2*)(p.bias + (int64_t)t.e * p.N + min(gn0 + 32 * i + 8 * q + 4 * hi, p.N - 4));
+        const float b4[4] = {bf16_lo(bb[0]), bf16_hi(bb[0]), bf16_lo(bb[1]), bf16_hi(bb[1])};
 #pragma unroll
-        for (int j = 0; j < FM; ++j) {
-          float v[4];
+        for (int j = 0; j < FM; ++j)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) v[x] = f(acc[i][j][4 * q + x]);
-          const int ml = 32 * j + l32;
-          const u32x2 w2 = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
-          *(u32x2*)(slab + ml * SRB + (((nl >> 3) ^ (ml & (CPR - 1))) << 4) + 8 * hi) = w2;
+          for (int x = 0; x < 4; ++x) acc[i][j][4 * q + x] = MODE == EX_OUT ? rw[j] * b4[x] : b4[x];
+      }
+    if (more) {
+      tn = tile_at(ti + (int)gridDim.x);
+      if (GATHER) x_offsets(tn, xn);
+    }
+
+    bf16x8 af[2][FN], bfr[2][FM];
+    if constexpr (BIG) {
+      in_flight = false;
+      for (int kt = 0; kt < nk; ++kt) {
+        wait_vmcnt(0);
+        lds_barrier();  // the stage has landed for every wave; slot wr is free
+        const bool step = kt + 1 < nk;
+        if (step) {
+          issue_x(t, xo, kt + 1, wr);
+        } else if (more) {
+          uint32_t wn_[LPW];
+          if (!GATHER) x_offsets(tn, xn);
+          w_offsets(tn, wn_);
+          issue_x(tn, xn, 0, wr);
+          issue_w(tn, wn_, 0, wr);
+          in_flight = true;
+        }
+        const char* st = lds + rd * STAGE;
+        load_frags(st, 0, af[0], bfr[0]);
+#pragma unroll
+        for (int kk = 0; kk < BK / 16; ++kk) {
+          const int cb = kk & 1;
+          if (kk + 1 < BK / 16) load_frags(st, kk + 1, af[cb ^ 1], bfr[cb ^ 1]);
+#pragma unroll
+          for (int i = 0; i < FN; ++i)
+#pragma unroll
+            for (int j = 0; j < FM; ++j)
+              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af[cb][i], bfr[cb][j], acc[i][j], 0, 0, 0);
+          if (kk == 0 && step) {  // the weights' copies behind the first MFMAs
+            __builtin_amdgcn_sched_barrier(0);
+            issue_w(t, wo, kt + 1, wr);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+        __builtin_amdgcn_iglp_opt(1);
+        rd ^= 1;
+        wr ^= 1;
+      }
+    } else {
+      rd = 0;
+      for (int kt = 0; kt < nk; ++kt) {
+        if (NST > 2 && kt + NST - 2 < nk) wait_vmcnt((NST - 2) * (LPX + LPW));
+        else wait_vmcnt(0);
+        lds_barrier();  // landed for every wave, and the slot read last step is free
+        const int ws = rd == 0 ? NST - 1 : rd - 1;
+        if (kt + NST - 1 < nk) {
+          issue_x(t, xo, kt + NST - 1, ws);
+          issue_w(t, wo, kt + NST - 1, ws);
+        }
+        const char* st = lds + rd * STAGE;
+        rd = rd + 1 == NST ? 0 : rd + 1;
+        load_frags(st, 0, af[0], bfr[0]);
+#pragma unroll
+        for (int kk = 0; kk < BK / 16; ++kk) {
+          const int cb = kk & 1;
+          if (kk + 1 < BK / 16) load_frags(st, kk + 1, af[cb ^ 1], bfr[cb ^ 1]);
+#pragma unroll
+          for (int i = 0; i < FN; ++i)
+#pragma unroll
+            for (int j = 0; j < FM; ++j)
+              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af[cb][i], bfr[cb][j], acc[i][j], 0, 0, 0);
         }
       }
-  };
-  auto from_slab = [&](bf16* dst) {
+    }
+
+    // ---- epilogue ----
+    if constexpr (MODE == EX_OUT) {  // fp32, straight from the accumulators
+      float* out = (float*)p.out;
 #pragma unroll
-    for (int it = 0; it < NIT; ++it) {
-      const int sl = RPI * it + lane / CPR;
-      if (col && wr0 + sl < rows)
-        *(u32x4*)(dst + (int64_t)(row0 + wr0 + sl) * p.N + gn) = *(const u32x4*)(slab + sl * SRB + ((c ^ (sl & (CPR - 1))) << 4));
+      for (int j = 0; j < FM; ++j) {
+        const int r = wr0 + 32 * j + l32;
+        if (r >= t.rows) continue;
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int gn = gn0 + 32 * i + 8 * q + 4 * hi;
+            if (gn < p.N)
+              *(f32x4*)(out + (int64_t)(t.row0 + r) * p.N + gn) =
+                  (f32x4){acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+          }
+      }
+    } else {
+      // two bytes a value through this wave's LDS slab, 16-byte rows out; BIG: half the
+      // wave's rows at a time, in the slot read last (the other takes the next tile)
+      lds_barrier();  // every wave is done reading the last stage
+      constexpr int SRB = WTN * 2, CPR = WTN / 8, RPI = 64 / CPR, NIT = HM * 32 / RPI;
+      char* slab = lds + (BIG ? wr * STAGE : 0) + wave * SLAB;
+      const int c = lane % CPR, gn = gn0 + 8 * c;
+      const bool col = gn < p.N;  // N is a multiple of 8: the whole 16-byte run
+      auto to_slab = [&](int half, auto pack) {
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int nl = 32 * i + 8 * q + 4 * hi;
+#pragma unroll
+            for (int jj = 0; jj < HM; ++jj) {
+              const int ml = 32 * jj + l32;
+              *(u32x2*)(slab + ml * SRB + (((nl >> 3) ^ (ml & (CPR - 1))) << 4) + 8 * hi) = pack(i, half * HM + jj, q);
+            }
+          }
+      };
+      auto from_slab = [&](int half, void* dst) {
+        const int r0 = wr0 + half * HM * 32;
+#pragma unroll
+        for (int it = 0; it < NIT; ++it) {
+          const int sl = RPI * it + lane / CPR;
+          const u32x4 v = *(const u32x4*)(slab + sl * SRB + ((c ^ (sl & (CPR - 1))) << 4));
+          if (col && r0 + sl < t.rows) *(u32x4*)((char*)dst + ((int64_t)(t.row0 + r0 + sl) * p.N + gn) * 2) = v;
+        }
+      };
+#pragma unroll
+      for (int half = 0; half < HALVES; ++half) {
+        if constexpr (MODE == EX_HIDDEN) {
+          to_slab(half, [&](int i, int j, int q) {
+            float v[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              float y, d;
+              gelu_both(acc[i][j][4 * q + x], y, d);
+              v[x] = y * rw[j];
+            }
+            return (u32x2){pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+          });
+          from_slab(half, p.out);
+          if (p.out2) {
+            to_slab(half, [&](int i, int j, int q) {
+              f16x4 v;
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                float z = acc[i][j][4 * q + x], y, d;
+                asm volatile("" : "+v"(z));  // computed again: the first pass's values would stay in registers
+                gelu_both(z, y, d);
+                v[x] = (_Float16)d;
+              }
+              return __builtin_bit_cast(u32x2, v);
+            });
+            from_slab(half, p.out2);
+          }
+        } else {
+          to_slab(half, [&](int i, int j, int q) {
+            const int r = wr0 + 32 * j + l32, g = gn0 + 32 * i + 8 * q + 4 * hi;
+            f16x4 d = {0, 0, 0, 0};
+            if (r < t.rows && g < p.N) d = *(const f16x4*)(p.mul + (int64_t)(t.row0 + r) * p.N + g);
+            float v[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) v[x] = acc[i][j][4 * q + x] * (rw[j] * (float)d[x]);
+            return (u32x2){pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+          });
+          from_slab(half, p.out);
+        }
+      }
     }
-  };
-  if constexpr (MODE == EX_HIDDEN) {
-    to_slab([](float x) {
-      float y, d;
-      gelu_both(x, y, d);
-      return y;
-    });
-    from_slab((bf16*)p.out);
-    if (p.out2) {
-      to_slab([](float x) {
-        float y, d;
-        gelu_both(x, y, d);
-        return d;
-      });
-      from_slab(p.out2);
-    }
-  } else {
-    to_slab([](float x) { return x; });
-    from_slab((bf16*)p.out);
+    if (!BIG) return;
+    t = tn;
+#pragma unroll
+    for (int j = 0; j < LPX; ++j) xo[j] = xn[j];
   }
+#endif
 }
 
-// ---- out[t] = residual[t] + sum over s of w y (y fp32 rows), eight channels a thread ----
+// ---- out[t] = residual[t] + sum over s of y_r, eight channels a thread; without weights: dx ----
 struct ExpertCombine {
   const float* y;
-  const bf16* yb;         // the backward's rows instead of y (no weights)
-  const bf16* weights;
+  const bf16* weights;    // [T, k] or null; a pair whose weight is nothing adds nothing
   const int32_t* slot_row;
   const bf16* residual;
   bf16* out;
@@ -286,7 +425,6 @@ struct ExpertCombine {
   int chunks, top_k;
 };
 
-template <bool BWD>
 __global__ __launch_bounds__(256) void expert_combine_kernel(ExpertCombine p) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= p.n) return;
@@ -294,7 +432,7 @@ __global__ __launch_bounds__(256) void expert_combine_kernel(ExpertCombine p) {
   const int c = (int)(i - t * p.chunks) * 8;
   const int64_t ld = (int64_t)p.chunks * 8;
   float a[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (!BWD && p.residual) {
+  if (p.residual) {
     const u32x4 r = *(const u32x4*)(p.residual + t * p.ldr + c);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -304,158 +442,134 @@ __global__ __launch_bounds__(256) void expert_combine_kernel(ExpertCombine p) {
   }
   for (int s = 0; s < p.top_k; ++s) {
     const int r = p.slot_row[t * p.top_k + s];
-    if (r < 0) continue;
-    if (BWD) {
-      const u32x4 v = *(const u32x4*)(p.yb + (int64_t)r * ld + c);
+    if (r < 0 || (p.weights && no_weight((float)p.weights[t * p.top_k + s]))) continue;
+    const f32x4 u = *(const f32x4*)(p.y + (int64_t)r * ld + c), v = *(const f32x4*)(p.y + (int64_t)r * ld + c + 4);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        a[2 * e] += bf16_lo(v[e]);
-        a[2 * e + 1] += bf16_hi(v[e]);
-      }
-    } else {
-      const float w = (float)p.weights[t * p.top_k + s];
-      const f32x4 u = *(const f32x4*)(p.y + (int64_t)r * ld + c), v = *(const f32x4*)(p.y + (int64_t)r * ld + c + 4);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        a[e] = fmaf(w, u[e], a[e]);
-        a[4 + e] = fmaf(w, v[e], a[4 + e]);
-      }
+    for (int e = 0; e < 4; ++e) {
+      a[e] += u[e];
+      a[4 + e] += v[e];
     }
   }
   *(u32x4*)(p.out + i * 8) = (u32x4){pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]), pack_bf16x2(a[4], a[5]), pack_bf16x2(a[6], a[7])};
 }
 
-// ---- the pairs' half of the backward: gs_r = w g[t] and dw = <g[t], y_r>; a wave a pair ----
-struct ExpertScatter {
-  const bf16* g;  // [T, N]
-  const float* y;
-  const bf16* weights;
-  const int32_t* slot_row;
-  bf16* gs;       // or null
-  bf16* dw;       // or null
-  int64_t pairs;
-  int top_k, N;
-};
-
-__global__ __launch_bounds__(256) void expert_scatter_kernel(ExpertScatter p) {
+// ---- dw = <g[t], y_r> / w'; a wave a pair ----
+__global__ __launch_bounds__(256) void expert_dweight_kernel(const bf16* g, const float* yy, const bf16* weights,
+                                                             const int32_t* slot_row, bf16* dw, int64_t pairs, int top_k,
+                                                             int N) {
   const int64_t s = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
-  if (s >= p.pairs) return;
-  const int r = p.slot_row[s];
+  if (s >= pairs) return;
+  const int r = slot_row[s];
   if (r < 0) {
-    if (p.dw && lane == 0) p.dw[s] = (bf16)0.f;
+    if (lane == 0) dw[s] = (bf16)0.f;
     return;
   }
-  const bf16* g = p.g + s / p.top_k * p.N;
-  const float* y = p.y + (int64_t)r * p.N;
-  const float w = (float)p.weights[s];
+  g += s / top_k * N;
+  const float* y = yy + (int64_t)r * N;
   float d = 0.f;
-  for (int c = lane * 8; c < p.N; c += 512) {
+  for (int c = lane * 8; c < N; c += 512) {
     const u32x4 v = *(const u32x4*)(g + c);
-    u32x4 o;
+    const f32x4 a = *(const f32x4*)(y + c), b = *(const f32x4*)(y + c + 4);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float a = bf16_lo(v[e]), b = bf16_hi(v[e]);
-      o[e] = pack_bf16x2(w * a, w * b);
-      if (p.dw) d = fmaf(b, y[c + 2 * e + 1], fmaf(a, y[c + 2 * e], d));
-    }
-    if (p.gs) *(u32x4*)(p.gs + (int64_t)r * p.N + c) = o;
-  }
-  if (p.dw) {
-#pragma unroll
-    for (int k = 32; k; k >>= 1) d += __shfl_xor(d, k);
-    if (lane == 0) p.dw[s] = (bf16)d;
-  }
-}
-
-// ---- w[e] [R, C] -> wt[e] [C, R], 64 x 64 tiles through LDS ----
-__global__ __launch_bounds__(256) void expert_transpose_kernel(const bf16* __restrict__ w, bf16* __restrict__ wt, int R, int C) {
-  __shared__ bf16 s[64][72];
-  const int64_t base = (int64_t)blockIdx.z * R * C;
-  const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64, tid = threadIdx.x;
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int r = (tid >> 3) + 32 * k, c = (tid & 7) * 8;
-    if (r0 + r < R && c0 + c < C) *(u32x4*)&s[r][c] = *(const u32x4*)(w + base + (int64_t)(r0 + r) * C + c0 + c);
-  }
-  __syncthreads();
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int c = (tid >> 3) + 32 * k, r = (tid & 7) * 8;
-    if (c0 + c < C && r0 + r < R) {
-      bf16x8 v;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = s[r + e][c];
-      *(bf16x8*)(wt + base + (int64_t)(c0 + c) * R + r0 + r) = v;
+    for (int e = 0; e < 2; ++e) {
+      d = fmaf(bf16_hi(v[e]), a[2 * e + 1], fmaf(bf16_lo(v[e]), a[2 * e], d));
+      d = fmaf(bf16_hi(v[2 + e]), b[2 * e + 1], fmaf(bf16_lo(v[2 + e]), b[2 * e], d));
     }
   }
+#pragma unroll
+  for (int k = 32; k; k >>= 1) d += __shfl_xor(d, k);
+  if (lane == 0) dw[s] = (bf16)(d / row_scale((float)weights[s]));
 }
 
 // ---- the weights' gradients: out[e] [N, K] = sum over the expert's rows of g[r, n] x[r, k] ----
 // One 256 x 256 tile of one expert a workgroup, stages of 64 rows; both operands are read
-// transposed out of LDS (ds_read_b64_tr_b16), the column sums of g by a ones operand.
+// transposed out of LDS (ds_read_b64_tr_b16).  The bias's gradient is one more product, of
+// ones (dW1) or the rows' weights (dW2) with the fragments of g at hand.  One of the operands
+// is gathered by token.  Experts are taken by falling number of rows, so that the largest
+// does not start last.
 struct ExpertWgrad {
   const bf16* g;
   const bf16* x;
-  const int32_t* rows;  // gather of x, or null
+  const int32_t* token;
+  const float* weight;  // OF_G: a row whose weight is nothing counts as zero
   const int32_t* offsets;
   bf16* out;
   bf16* bias_out;       // [E, N] or null
   int64_t ldg, ldx;
-  int N, K, nt, kt, top_k;
+  int N, K, nt, kt, experts;
 };
 
 constexpr int EW_BK = 64, EW_HALF = EW_BK * 512, EW_STAGE = 2 * EW_HALF;
 
-template <bool GATHER>
+// OF_G: g is gathered (dout), x are rows (h); else x is gathered and g are rows (gz).
+template <bool OF_G>
 __global__ __launch_bounds__(512, 1) void expert_wgrad_kernel(ExpertWgrad p) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr int NW = 8, LPW = EW_HALF / 1024 / NW;
   __shared__ __attribute__((aligned(1024))) char lds[2 * EW_STAGE];
+  __shared__ __attribute__((aligned(8))) bf16 wbuf[2][EW_BK];  // the bias's other operand, by row
   const int tid = (int)__builtin_amdgcn_workitem_id_x();
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n16 = lane & 15, g4 = lane >> 4;
   const int wk = wave >> 2, wn = wave & 3;  // wave tile: 128 k x 64 n
   const uint32_t lds_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
 
-  int w = xcd_tile_order((int)gridDim.x, (int)__builtin_amdgcn_workgroup_id_x());
-  const int tk = w % p.kt;
-  w /= p.kt;
-  const int tn = w % p.nt, e = w / p.nt;
+  const int id = (int)__builtin_amdgcn_workgroup_id_x(), per = p.nt * p.kt;
+  int e = id / per;
+  const int tk = id % per % p.kt, tn = id % per / p.kt;
+  if (p.experts <= 64) {  // the e-th largest: every wave ranks the experts, one a lane
+    const int n = lane < p.experts ? p.offsets[lane + 1] - p.offsets[lane] : -1;
+    int before = 0;
+    for (int i = 0; i < p.experts; ++i) {
+      const int o = __builtin_amdgcn_readlane(n, i);
+      before += o > n || (o == n && i < lane);
+    }
+    e = __ffsll(__ballot(lane < p.experts && before == e)) - 1;
+  }
+  e = __builtin_amdgcn_readfirstlane(e);
   const int k0 = tk * 256, n0 = tn * 256;
   const int row0 = p.offsets[e], rows = p.offsets[e + 1] - row0;
   const int nk = (rows + EW_BK - 1) / EW_BK;
 
-  uint32_t vx[LPW], vg[LPW];  // GATHER: vx without the row
+  uint32_t vx[LPW], vg[LPW];  // the gathered one's without the row
   int rr[LPW];
 #pragma unroll
   for (int j = 0; j < LPW; ++j) {
     const int row = 2 * (j * NW + wave) + (lane >> 5), c = (lane & 31) ^ ((row & 7) << 1);
     rr[j] = row;
-    vx[j] = k0 + 8 * c < p.K ? (uint32_t)((GATHER ? 0 : row * p.ldx * 2) + c * 16) : OOB;
-    vg[j] = n0 + 8 * c < p.N ? (uint32_t)(row * p.ldg * 2 + c * 16) : OOB;
+    vx[j] = k0 + 8 * c < p.K ? (uint32_t)((OF_G ? row * p.ldx * 2 : 0) + c * 16) : OOB;
+    vg[j] = n0 + 8 * c < p.N ? (uint32_t)((OF_G ? 0 : row * p.ldg * 2) + c * 16) : OOB;
   }
-  const char* xb = (const char*)(p.x + (GATHER ? 0 : (int64_t)row0 * p.ldx) + k0);
-  const char* gb = (const char*)(p.g + (int64_t)row0 * p.ldg + n0);
-  uint32_t tok[LPW];  // GATHER: byte offsets of the next stage's rows of x
+  const char* xb = (const char*)(p.x + (OF_G ? (int64_t)row0 * p.ldx : 0) + k0);
+  const char* gb = (const char*)(p.g + (OF_G ? 0 : (int64_t)row0 * p.ldg) + n0);
+  const uint32_t ldt = (uint32_t)((OF_G ? p.ldg : p.ldx) * 2);
+  // a stage ahead: its gathered rows' byte offsets, and the bias operand's values
+  uint32_t tok[LPW];
+  const bool sums_wg = p.bias_out && tk == 0, sums = sums_wg && wk == 0;  // uniform per workgroup, per wave
+  float wnext = 0.f;
   auto fetch = [&](int kt) {
-    if constexpr (GATHER) {
 #pragma unroll
-      for (int j = 0; j < LPW; ++j) {
-        const int r = kt * EW_BK + rr[j];
-        tok[j] = r < rows ? (uint32_t)(p.rows[row0 + r] / p.top_k) * (uint32_t)(p.ldx * 2) : 0u;
-      }
+    for (int j = 0; j < LPW; ++j) {
+      const int r = kt * EW_BK + rr[j];
+      tok[j] = OOB;
+      if (r < rows && !(OF_G && no_weight(p.weight[row0 + r]))) tok[j] = (uint32_t)p.token[row0 + r] * ldt;
+    }
+    if (sums_wg && tid < EW_BK) {
+      const int r = kt * EW_BK + tid;
+      wnext = r < rows ? (OF_G ? p.weight[row0 + r] : 1.f) : 0.f;
     }
   };
   auto issue = [&](int kt, int slot, bool is_g) {
     const int left = rows - kt * EW_BK;
-    const u32x4 r = is_g ? make_rsrc(gb + (int64_t)kt * EW_BK * p.ldg * 2, OOB)
-                         : make_rsrc(GATHER ? xb : xb + (int64_t)kt * EW_BK * p.ldx * 2, OOB);
+    const bool gathered = is_g == OF_G;
+    const char* base = is_g ? gb : xb;
+    const u32x4 r = make_rsrc(gathered ? base : base + (int64_t)kt * EW_BK * (is_g ? p.ldg : p.ldx) * 2, OOB);
     const uint32_t dst = lds_base + slot * EW_STAGE + (is_g ? EW_HALF : 0) + wave * 1024;
 #pragma unroll
     for (int j = 0; j < LPW; ++j) {
       uint32_t vo = is_g ? vg[j] : vx[j];
-      if (GATHER && !is_g && vo != OOB) vo += tok[j];
-      if (left < EW_BK && rr[j] >= left) vo = OOB;
+      if (gathered) vo = vo == OOB || tok[j] == OOB ? OOB : vo + tok[j];
+      else if (left < EW_BK && rr[j] >= left) vo = OOB;
       dma_row16(r, dst + j * NW * 1024, vo);
     }
   };
@@ -483,22 +597,23 @@ __global__ __launch_bounds__(512, 1) void expert_wgrad_kernel(ExpertWgrad p) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[i][j] = bacc[j];
   }
-  bf16x8 ones;
-#pragma unroll
-  for (int k = 0; k < 8; ++k) ones[k] = (bf16)1.f;
-  const bool sums = p.bias_out && tk == 0 && wk == 0;  // uniform per wave
+  // bias operand: rows 4 g4 .. + 3 and 16 + 4 g4 .. + 3 of a sub-step, as the fragments
   if (nk > 0) {
     fetch(0);
     issue(0, 0, false);
     issue(0, 0, true);
+    if (sums_wg && tid < EW_BK) wbuf[0][tid] = (bf16)wnext;
     fetch(1);
   }
   for (int kt = 0; kt < nk; ++kt) {
     wait_vmcnt(0);
+    wait_lgkm0();   // wbuf
     lds_barrier();  // the stage has landed for every wave; the other slot is free
     const int wr = (kt + 1) & 1;
-    if (kt + 1 < nk) {
-      issue(kt + 1, wr, false);
+    const bool step = kt + 1 < nk;
+    if (step) {
+      issue(kt + 1, wr, OF_G);  // the gathered operand, whose offsets the next fetch overwrites
+      if (sums_wg && tid < EW_BK) wbuf[wr][tid] = (bf16)wnext;
       fetch(kt + 2);
     }
     const char* st = lds + (kt & 1) * EW_STAGE;
@@ -514,12 +629,14 @@ __global__ __launch_bounds__(512, 1) void expert_wgrad_kernel(ExpertWgrad p) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[j], acc[i][j], 0, 0, 0);
       if (sums) {
+        const bf16x4 lo = *(const bf16x4*)&wbuf[kt & 1][32 * kk + 4 * g4], hi = *(const bf16x4*)&wbuf[kt & 1][32 * kk + 16 + 4 * g4];
+        const bf16x8 w8 = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) bacc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, b[j], bacc[j], 0, 0, 0);
+        for (int j = 0; j < 4; ++j) bacc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w8, b[j], bacc[j], 0, 0, 0);
       }
-      if (kk == 0 && kt + 1 < nk) {
+      if (kk == 0 && step) {
         __builtin_amdgcn_sched_barrier(0);
-        issue(kt + 1, wr, true);
+        issue(kt + 1, wr, !OF_G);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -547,30 +664,59 @@ __global__ __launch_bounds__(512, 1) void expert_wgrad_kernel(ExpertWgrad p) {
 #endif
 }
 
-// Rows of a tile: 64 where an expert has fewer than 96 rows on average, else 128.
-static int expert_tile(int64_t pairs, int experts) { return pairs < 96 * (int64_t)experts ? 64 : 128; }
+// Rows of a tile: 256 where the products fill the chip with 256 x 256 tiles, 64 where an
+// expert has fewer than 96 rows on average, else 128.
+static int expert_tile(int64_t pairs, int experts, int64_t width) {
+  if (pairs < 96 * (int64_t)experts) return 64;
+  return pairs >= 512 * (int64_t)experts && (pairs / 256) * ((width + 255) / 256) >= 200 ? 256 : 128;
+}
+static int expert_tile(const strata_hip_expert_mlp_args* a) {
+  return expert_tile(a->tokens * (int64_t)a->top_k, a->experts, std::min(std::min(a->dim, a->hidden), a->out_dim));
+}
 
-template <int MODE>
+static int expert_cus() {
+  static int cached[64] = {};
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+  if (cached[dev] == 0) {
+    int n = 0;
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
+    cached[dev] = n;
+  }
+  return cached[dev];
+}
+
+template <int MODE, bool WT>
 static int launch_expert_gemm(ExpertGemm p, int64_t pairs, int experts, int tile, hipStream_t st) {
   p.nt = (p.N + tile - 1) / tile;
   const int64_t mt = pairs / tile + std::min<int64_t>(experts, pairs), total = mt * p.nt;
   if (total > 0x7fffffff) return fail(STRATA_HIP_EUNSUPPORTED, "expert_mlp: problem too large for one launch");
-  if (tile == 128)
-    hipLaunchKernelGGL((expert_gemm_kernel<128, 128, 4, 2, 2, MODE>), dim3((unsigned)total), dim3(512), 0, st, p);
+  if (tile == 256)
+    hipLaunchKernelGGL((expert_gemm_kernel<256, 256, 2, 4, 2, MODE, WT>), dim3((unsigned)std::min<int64_t>(total, expert_cus())),
+                       dim3(512), 0, st, p);
+  else if (tile == 128)
+    hipLaunchKernelGGL((expert_gemm_kernel<128, 128, 4, 2, 2, MODE, WT>), dim3((unsigned)total), dim3(512), 0, st, p);
   else
-    hipLaunchKernelGGL((expert_gemm_kernel<64, 64, 2, 2, 4, MODE>), dim3((unsigned)total), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((expert_gemm_kernel<64, 64, 2, 2, 4, MODE, WT>), dim3((unsigned)total), dim3(256), 0, st, p);
   return check_launch("expert_gemm_kernel");
 }
 
-static int launch_wgrad(const ExpertWgrad& q, int experts, hipStream_t st) {
-  ExpertWgrad p = q;
+template <bool OF_G>
+static int launch_wgrad(ExpertWgrad p, hipStream_t st) {
   p.nt = (p.N + 255) / 256;
   p.kt = (p.K + 255) / 256;
-  const int64_t total = (int64_t)p.nt * p.kt * experts;
+  const int64_t total = (int64_t)p.nt * p.kt * p.experts;
   if (total > 0x7fffffff) return fail(STRATA_HIP_EUNSUPPORTED, "expert_mlp_bwd: problem too large for one launch");
-  if (p.rows) hipLaunchKernelGGL(expert_wgrad_kernel<true>, dim3((unsigned)total), dim3(512), 0, st, p);
-  else hipLaunchKernelGGL(expert_wgrad_kernel<false>, dim3((unsigned)total), dim3(512), 0, st, p);
+  hipLaunchKernelGGL(expert_wgrad_kernel<OF_G>, dim3((unsigned)total), dim3(512), 0, st, p);
   return check_launch("expert_wgrad_kernel");
+}
+
+static int launch_combine(ExpertCombine c, int64_t tokens, int width, hipStream_t st) {
+  c.chunks = width / 8;
+  c.n = tokens * c.chunks;
+  if (c.n > 0x7fffffffll * 256) return fail(STRATA_HIP_EUNSUPPORTED, "expert_mlp: problem too large for one launch");
+  hipLaunchKernelGGL(expert_combine_kernel, dim3((unsigned)((c.n + 255) / 256)), dim3(256), 0, st, c);
+  return check_launch("expert_combine_kernel");
 }
 
 static int expert_check(const std::string& name, const strata_hip_expert_mlp_args* a) {
@@ -582,12 +728,12 @@ static int expert_check(const std::string& name, const strata_hip_expert_mlp_arg
   const int64_t pairs = a->tokens * (int64_t)a->top_k;
   if (a->experts > 512 || pairs > 0x7ffffff0 || a->dim > 32768 || a->hidden > 32768 || a->out_dim > 32768)
     return fail(STRATA_HIP_EUNSUPPORTED, name + ": at most 512 experts, widths 32768 and 2^31 pairs");
-  if (a->tile != expert_tile(pairs, a->experts)) return fail(STRATA_HIP_EINVAL, name + ": tile is not strata_hip_expert_tile()'s");
+  if (a->tile != expert_tile(a)) return fail(STRATA_HIP_EINVAL, name + ": tile is not strata_hip_expert_tile()'s");
   if (!a->w1 || !a->w2 || !a->offsets || !a->tiles) return fail(STRATA_HIP_EINVAL, name + ": null pointer");
   if (((uintptr_t)a->w1 & 15) || ((uintptr_t)a->w2 & 15) || ((uintptr_t)a->b1 & 7) || ((uintptr_t)a->b2 & 7))
     return fail(STRATA_HIP_EINVAL, name + ": weights must be 16-byte, biases 8-byte aligned");
   if (pairs == 0) return STRATA_HIP_OK;
-  if (!a->x || !a->weights || !a->row_slot || !a->slot_row || !a->h || !a->y)
+  if (!a->x || !a->weights || !a->row_token || !a->row_weight || !a->slot_row || !a->h || !a->y)
     return fail(STRATA_HIP_EINVAL, name + ": null pointer");
   if (((uintptr_t)a->x & 15) || ((uintptr_t)a->h & 15) || ((uintptr_t)a->y & 15) || ((uintptr_t)a->dact & 15) || a->ldx % 8 ||
       (a->tokens > 1 && a->ldx < a->dim))
@@ -602,7 +748,9 @@ static int expert_check(const std::string& name, const strata_hip_expert_mlp_arg
 
 using namespace strata;
 
-extern "C" int32_t strata_hip_expert_tile(int64_t pairs, int32_t experts) { return expert_tile(pairs, experts); }
+extern "C" int32_t strata_hip_expert_tile(int64_t pairs, int32_t experts, int32_t dim, int32_t hidden, int32_t out_dim) {
+  return expert_tile(pairs, experts, std::min(std::min(dim, hidden), out_dim));
+}
 
 extern "C" int strata_hip_expert_mlp(const strata_hip_expert_mlp_args* a, void* stream) {
   if (const int rc = expert_check("expert_mlp", a)) return rc;
@@ -613,29 +761,27 @@ extern "C" int strata_hip_expert_mlp(const strata_hip_expert_mlp_args* a, void* 
   hipStream_t st = (hipStream_t)stream;
   const int64_t pairs = a->tokens * (int64_t)a->top_k;
   ExpertGemm g = {};
+  g.token = a->row_token;
+  g.weight = a->row_weight;
   g.offsets = a->offsets;
   g.tiles = a->tiles;
-  g.top_k = a->top_k;
   g.x = (const bf16*)a->x;
   g.ldx = a->ldx;
-  g.rows = a->row_slot;
   g.w = (const bf16*)a->w1;
   g.bias = (const bf16*)a->b1;
   g.out = a->h;
-  g.out2 = (bf16*)a->dact;
+  g.out2 = (_Float16*)a->dact;
   g.N = a->hidden;
   g.K = a->dim;
-  if (const int rc = launch_expert_gemm<EX_HIDDEN>(g, pairs, a->experts, a->tile, st)) return rc;
+  if (const int rc = launch_expert_gemm<EX_HIDDEN, false>(g, pairs, a->experts, a->tile, st)) return rc;
   g.x = (const bf16*)a->h;
   g.ldx = a->hidden;
-  g.rows = nullptr;
   g.w = (const bf16*)a->w2;
   g.bias = (const bf16*)a->b2;
   g.out = a->y;
-  g.out2 = nullptr;
   g.N = a->out_dim;
   g.K = a->hidden;
-  if (const int rc = launch_expert_gemm<EX_OUT>(g, pairs, a->experts, a->tile, st)) return rc;
+  if (const int rc = launch_expert_gemm<EX_OUT, false>(g, pairs, a->experts, a->tile, st)) return rc;
   ExpertCombine c = {};
   c.y = a->y;
   c.weights = (const bf16*)a->weights;
@@ -643,12 +789,8 @@ extern "C" int strata_hip_expert_mlp(const strata_hip_expert_mlp_args* a, void* 
   c.residual = (const bf16*)a->residual;
   c.ldr = a->ldr;
   c.out = (bf16*)a->out;
-  c.chunks = a->out_dim / 8;
   c.top_k = a->top_k;
-  c.n = a->tokens * c.chunks;
-  if (c.n > 0x7fffffffll * 256) return fail(STRATA_HIP_EUNSUPPORTED, "expert_mlp: problem too large for one launch");
-  hipLaunchKernelGGL(expert_combine_kernel<false>, dim3((unsigned)((c.n + 255) / 256)), dim3(256), 0, st, c);
-  return check_launch("expert_combine_kernel");
+  return launch_combine(c, a->tokens, a->out_dim, st);
 }
 
 extern "C" int strata_hip_expert_mlp_bwd(const strata_hip_expert_mlp_bwd_args* b, void* stream) {
@@ -658,104 +800,77 @@ extern "C" int strata_hip_expert_mlp_bwd(const strata_hip_expert_mlp_bwd_args* b
   if (const int rc = expert_check(name, a)) return rc;
   hipStream_t st = (hipStream_t)stream;
   const int64_t pairs = a->tokens * (int64_t)a->top_k;
-  const bool hid = b->dx || b->dw1 || b->db1;  // gradients below the hidden layer
+  const bool hid = b->dx || b->dw1;  // gradients below the hidden layer
   if (pairs > 0) {
     if (!b->dout || ((uintptr_t)b->dout & 15)) return fail(STRATA_HIP_EINVAL, name + ": dout must be given, 16-byte aligned");
-    if ((b->dw2 || b->db2) && !b->gs) return fail(STRATA_HIP_EINVAL, name + ": gs is needed for dw2 and db2");
-    if (hid && (!a->dact || !b->gz || !b->w2t)) return fail(STRATA_HIP_EINVAL, name + ": dact, gz and w2t are needed for dx, dw1 and db1");
-    if (b->dx && (!b->dxs || !b->w1t)) return fail(STRATA_HIP_EINVAL, name + ": dxs and w1t are needed for dx");
+    if (hid && (!a->dact || !b->gz)) return fail(STRATA_HIP_EINVAL, name + ": dact and gz are needed for dx and dw1");
+    if (b->dx && !b->dxs) return fail(STRATA_HIP_EINVAL, name + ": dxs is needed for dx");
   }
   if ((b->db2 && !b->dw2) || (b->db1 && !b->dw1)) return fail(STRATA_HIP_EINVAL, name + ": a bias gradient comes with its weight's");
-  const void* all[] = {b->gs, b->gz, b->dxs, b->w1t, b->w2t, b->dx, b->dw1, b->dw2};
+  const void* all[] = {b->gz, b->dxs, b->dx, b->dw1, b->dw2};
   for (const void* q : all)
     if ((uintptr_t)q & 15) return fail(STRATA_HIP_EINVAL, name + ": workspaces and gradients must be 16-byte aligned");
-  if (pairs > 0 && (b->dweights || b->dw2)) {
-    ExpertScatter s = {};
-    s.g = (const bf16*)b->dout;
-    s.y = a->y;
-    s.weights = (const bf16*)a->weights;
-    s.slot_row = a->slot_row;
-    s.gs = b->dw2 ? (bf16*)b->gs : nullptr;
-    s.dw = (bf16*)b->dweights;
-    s.pairs = pairs;
-    s.top_k = a->top_k;
-    s.N = a->out_dim;
-    hipLaunchKernelGGL(expert_scatter_kernel, dim3((unsigned)((pairs + 3) / 4)), dim3(256), 0, st, s);
-    if (const int rc = check_launch("expert_scatter_kernel")) return rc;
+  if (pairs > 0 && b->dweights) {
+    hipLaunchKernelGGL(expert_dweight_kernel, dim3((unsigned)((pairs + 3) / 4)), dim3(256), 0, st, (const bf16*)b->dout, a->y,
+                       (const bf16*)a->weights, a->slot_row, (bf16*)b->dweights, pairs, a->top_k, a->out_dim);
+    if (const int rc = check_launch("expert_dweight_kernel")) return rc;
   }
-  auto transpose = [&](const void* w, void* wt, int R, int C) {
-    hipLaunchKernelGGL(expert_transpose_kernel, dim3((C + 63) / 64, (R + 63) / 64, a->experts), dim3(256), 0, st,
-                       (const bf16*)w, (bf16*)wt, R, C);
-    return check_launch("expert_transpose_kernel");
-  };
+  ExpertWgrad w = {};
+  w.token = a->row_token;
+  w.weight = a->row_weight;
+  w.offsets = a->offsets;
+  w.experts = a->experts;
   if (b->dw2) {  // without rows: zeros
-    ExpertWgrad w = {};
-    w.g = (const bf16*)b->gs;
+    w.g = (const bf16*)b->dout;
     w.x = (const bf16*)a->h;
-    w.offsets = a->offsets;
     w.out = (bf16*)b->dw2;
     w.bias_out = (bf16*)b->db2;
     w.ldg = a->out_dim;
     w.ldx = a->hidden;
     w.N = a->out_dim;
     w.K = a->hidden;
-    w.top_k = 1;
-    if (const int rc = launch_wgrad(w, a->experts, st)) return rc;
+    if (const int rc = launch_wgrad<true>(w, st)) return rc;
   }
-  if (!hid) return STRATA_HIP_OK;
   ExpertGemm g = {};
+  g.token = a->row_token;
+  g.weight = a->row_weight;
   g.offsets = a->offsets;
   g.tiles = a->tiles;
-  g.top_k = a->top_k;
-  if (pairs > 0) {
-    if (const int rc = transpose(a->w2, b->w2t, a->out_dim, a->hidden)) return rc;
+  if (hid && pairs > 0) {
     g.x = (const bf16*)b->dout;
     g.ldx = a->out_dim;
-    g.rows = a->row_slot;
-    g.slots = a->row_slot;
-    g.scale = (const bf16*)a->weights;
-    g.w = (const bf16*)b->w2t;
-    g.mul = (const bf16*)a->dact;
+    g.w = (const bf16*)a->w2;
+    g.mul = (const _Float16*)a->dact;
     g.out = b->gz;
     g.N = a->hidden;
     g.K = a->out_dim;
-    if (const int rc = launch_expert_gemm<EX_HIDDEN_GRAD>(g, pairs, a->experts, a->tile, st)) return rc;
+    if (const int rc = launch_expert_gemm<EX_HIDDEN_GRAD, true>(g, pairs, a->experts, a->tile, st)) return rc;
   }
   if (b->dw1) {
-    ExpertWgrad w = {};
     w.g = (const bf16*)b->gz;
     w.x = (const bf16*)a->x;
-    w.rows = a->row_slot;
-    w.offsets = a->offsets;
     w.out = (bf16*)b->dw1;
     w.bias_out = (bf16*)b->db1;
     w.ldg = a->hidden;
     w.ldx = a->ldx;
     w.N = a->hidden;
     w.K = a->dim;
-    w.top_k = a->top_k;
-    if (const int rc = launch_wgrad(w, a->experts, st)) return rc;
+    if (const int rc = launch_wgrad<false>(w, st)) return rc;
   }
   if (b->dx && pairs > 0) {
-    if (const int rc = transpose(a->w1, b->w1t, a->hidden, a->dim)) return rc;
     g.x = (const bf16*)b->gz;
     g.ldx = a->hidden;
-    g.rows = nullptr;
-    g.w = (const bf16*)b->w1t;
+    g.w = (const bf16*)a->w1;
     g.out = b->dxs;
     g.N = a->dim;
     g.K = a->hidden;
-    if (const int rc = launch_expert_gemm<EX_INPUT_GRAD>(g, pairs, a->experts, a->tile, st)) return rc;
+    if (const int rc = launch_expert_gemm<EX_OUT, true>(g, pairs, a->experts, a->tile, st)) return rc;
     ExpertCombine c = {};
-    c.yb = (const bf16*)b->dxs;
+    c.y = b->dxs;
     c.slot_row = a->slot_row;
     c.out = (bf16*)b->dx;
-    c.chunks = a->dim / 8;
     c.top_k = a->top_k;
-    c.n = a->tokens * c.chunks;
-    if (c.n > 0x7fffffffll * 256) return fail(STRATA_HIP_EUNSUPPORTED, name + ": problem too large for one launch");
-    hipLaunchKernelGGL(expert_combine_kernel<true>, dim3((unsigned)((c.n + 255) / 256)), dim3(256), 0, st, c);
-    return check_launch("expert_combine_kernel");
+    return launch_combine(c, a->tokens, a->dim, st);
   }
   return STRATA_HIP_OK;
 }

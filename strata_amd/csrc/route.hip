@@ -252,7 +252,7 @@ __global__ __launch_bounds__(256) void route_bwd_kernel(RouteParams p) {
 // ---------------------------------------------------------------------------
 // The plan: the chosen (token, slot) pairs in the order of their experts, pairs of one
 // expert in their own order, by a counting sort whose result depends on nothing else.
-//   row_slot[r]  the pair token * top_k + slot of row r
+//   row_token[r], row_weight[r]  the token and the weight of row r's pair
 //   slot_row[s]  the row of pair s, -1 where its index names no expert
 //   offsets[e]   the first row of expert e; offsets[E] the number of rows
 //   tiles        [n, then n pairs (expert, first row)]: `tile` rows of one expert each
@@ -264,13 +264,15 @@ constexpr int PLAN_N = 1024, PLAN_WAVES = PLAN_N / 64, PLAN_MAX_E = 512;
 
 struct PlanParams {
   const int32_t* index;
-  int32_t* row_slot;
+  const bf16* weights;
+  int32_t* row_token;
+  float* row_weight;
   int32_t* slot_row;
   int32_t* offsets;
   int32_t* tiles;
   int32_t* counts;  // [blocks][E]
   int64_t n;        // pairs
-  int experts, tile, bits, blocks;
+  int experts, top_k, tile, bits, blocks;
 };
 
 __device__ __forceinline__ int plan_expert(const PlanParams& p, int64_t s) {
@@ -422,7 +424,10 @@ __global__ __launch_bounds__(PLAN_N) void plan_place_kernel(PlanParams p) {
   if (s < p.n) {
     const int r = e >= 0 ? cnt[wave * E + e] + rank : -1;
     p.slot_row[s] = r;
-    if (r >= 0) p.row_slot[r] = (int32_t)s;
+    if (r >= 0) {
+      p.row_token[r] = (int32_t)s / p.top_k;
+      p.row_weight[r] = (float)p.weights[s];
+    }
   }
 }
 
@@ -521,14 +526,17 @@ extern "C" int64_t strata_hip_expert_plan_workspace(int64_t pairs, int32_t exper
 extern "C" int strata_hip_expert_plan(const strata_hip_expert_plan_args* a, void* stream) {
   using namespace strata;
   if (!a) return fail(STRATA_HIP_EINVAL, "expert_plan: null args");
-  if (a->pairs < 0 || a->experts <= 0 || a->tile <= 0) return fail(STRATA_HIP_EINVAL, "expert_plan: bad sizes");
+  if (a->pairs < 0 || a->experts <= 0 || a->tile <= 0 || a->top_k <= 0 || a->pairs % a->top_k) return fail(STRATA_HIP_EINVAL, "expert_plan: bad sizes");
   if (a->experts > PLAN_MAX_E) return fail(STRATA_HIP_EUNSUPPORTED, "expert_plan: at most 512 experts");
   if (a->pairs > 0x7ffffff0) return fail(STRATA_HIP_EUNSUPPORTED, "expert_plan: too many pairs");
-  if (!a->offsets || !a->tiles || (a->pairs > 0 && (!a->index || !a->row_slot || !a->slot_row)))
+  if (!a->offsets || !a->tiles || (a->pairs > 0 && (!a->index || !a->weights || !a->row_token || !a->row_weight || !a->slot_row)))
     return fail(STRATA_HIP_EINVAL, "expert_plan: null pointer");
   PlanParams p;
   p.index = a->index;
-  p.row_slot = a->row_slot;
+  p.weights = (const bf16*)a->weights;
+  p.row_token = a->row_token;
+  p.row_weight = a->row_weight;
+  p.top_k = a->top_k;
   p.slot_row = a->slot_row;
   p.offsets = a->offsets;
   p.tiles = a->tiles;

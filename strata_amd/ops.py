@@ -1536,20 +1536,28 @@ def _ptr(t: Optional[Tensor]) -> Optional[int]:
     return t.data_ptr() if t is not None else None
 
 
-def _expert_plan(index: Tensor, experts: int) -> tuple[Tensor, int]:
-    """The plan of ``strata_hip_expert_plan`` in one int32 tensor, [row_slot | slot_row | offsets |
-    tiles], and the rows of a tile."""
-    i = index.contiguous()
-    n = i.numel()
-    lib = _lib.load()
-    tile = int(lib.strata_hip_expert_tile(n, experts))
-    plan = torch.empty(2 * n + experts + 2 + 2 * (n // tile + experts), dtype=torch.int32, device=index.device)
-    nws = int(lib.strata_hip_expert_plan_workspace(n, experts))
+def _expert_tile(pairs: int, w1: Tensor, w2: Tensor) -> int:
+    E, H, C = w1.shape
+    return int(_lib.function("strata_hip_expert_tile")(pairs, E, C, H, w2.shape[1]))
+
+
+def _plan_size(pairs: int, experts: int, tile: int) -> int:
+    return 3 * pairs + experts + 2 + 2 * (pairs // tile + experts)
+
+
+def _expert_plan(index: Tensor, weights: Tensor, experts: int, tile: int) -> Tensor:
+    """The plan of ``strata_hip_expert_plan`` in one int32 tensor:
+    [row_token | row_weight (fp32) | slot_row | offsets | tiles]."""
+    i, w = index.contiguous(), weights.contiguous()
+    n, k = i.numel(), i.shape[-1]
+    plan = torch.empty(_plan_size(n, experts, tile), dtype=torch.int32, device=index.device)
+    nws = int(_lib.function("strata_hip_expert_plan_workspace")(n, experts))
     ws = torch.empty(nws, dtype=torch.int32, device=index.device) if nws else None
     p = plan.data_ptr()
-    a = _lib.ExpertPlanArgs(i.data_ptr(), p, p + 4 * n, p + 8 * n, p + 4 * (2 * n + experts + 1), _ptr(ws), n, experts, tile)
+    a = _lib.ExpertPlanArgs(i.data_ptr(), w.data_ptr(), p, p + 4 * n, p + 8 * n, p + 12 * n, p + 4 * (3 * n + experts + 1),
+                            _ptr(ws), n, k, experts, tile, 0)
     _launch("strata_hip_expert_plan", a, index)
-    return plan, tile
+    return plan
 
 
 def _expert_args(x, weights, plan, tile, w1, b1, w2, b2, h, dact, y):
@@ -1558,9 +1566,9 @@ def _expert_args(x, weights, plan, tile, w1, b1, w2, b2, h, dact, y):
     T, xp, ldx, x2 = _dense_rows(x, C)
     w, w1, b1, w2, b2 = weights.contiguous(), _dense(w1), _dense(b1), _dense(w2), _dense(b2)
     n, p = T * k, plan.data_ptr()
-    a = _lib.ExpertMlpArgs(xp, w.data_ptr(), p, p + 4 * n, p + 8 * n, p + 4 * (2 * n + E + 1), w1.data_ptr(), _ptr(b1),
-                           w2.data_ptr(), _ptr(b2), None, None, h.data_ptr(), _ptr(dact), y.data_ptr(), T, ldx, 0, k, E, C, H,
-                           N, tile)
+    a = _lib.ExpertMlpArgs(xp, w.data_ptr(), p, p + 4 * n, p + 8 * n, p + 12 * n, p + 4 * (3 * n + E + 1), w1.data_ptr(),
+                           _ptr(b1), w2.data_ptr(), _ptr(b2), None, None, h.data_ptr(), _ptr(dact), y.data_ptr(), T, ldx, 0,
+                           k, E, C, H, N, tile)
     return a, (x2, w, w1, b1, w2, b2)
 
 
@@ -1570,9 +1578,10 @@ def _expert_forward(name, x, weights, index, w1, b1, w2, b2, residual, save: boo
     n = index.numel()
     out = torch.empty((*x.shape[:-1], N), dtype=torch.bfloat16, device=x.device)
     h = torch.empty((n, H), dtype=torch.bfloat16, device=x.device)
-    dact = torch.empty_like(h) if save else None
+    dact = torch.empty((n, H), dtype=torch.float16, device=x.device) if save else None
     y = torch.empty((n, N), dtype=torch.float32, device=x.device)
-    plan, tile = _expert_plan(index, E)
+    tile = _expert_tile(n, w1, w2)
+    plan = _expert_plan(index, weights, E, tile)
     a, keep = _expert_args(x, weights, plan, tile, w1, b1, w2, b2, h, dact, y)
     if residual is not None:
         _, a.residual, a.ldr, r2 = _dense_rows(residual, N)
@@ -1607,10 +1616,9 @@ def expert_mlp_train(x: Tensor, weights: Tensor, index: Tensor, w1: Tensor, b1: 
 @expert_mlp_train.register_fake
 def _(x, weights, index, w1, b1, w2, b2, residual):
     n, E, H, N = index.numel(), w1.shape[0], w1.shape[1], w2.shape[1]
-    tile = int(_lib.load().strata_hip_expert_tile(n, E))
-    return (x.new_empty((*x.shape[:-1], N)), x.new_empty((n, H)), x.new_empty((n, H)),
+    return (x.new_empty((*x.shape[:-1], N)), x.new_empty((n, H)), x.new_empty((n, H), dtype=torch.float16),
             x.new_empty((n, N), dtype=torch.float32),
-            x.new_empty((2 * n + E + 2 + 2 * (n // tile + E),), dtype=torch.int32))
+            x.new_empty((_plan_size(n, E, _expert_tile(n, w1, w2)),), dtype=torch.int32))
 
 
 @torch.library.custom_op("strata_hip::expert_mlp_bwd", mutates_args=())
@@ -1620,9 +1628,9 @@ def expert_mlp_bwd(dout: Tensor, x: Tensor, weights: Tensor, w1: Tensor, b1: Opt
     """Gradients of ``expert_mlp_train`` at ``(x, weights, w1, b1, w2, b2)``, an empty tensor where
     ``need`` asks for none (a bias's comes from its weight's launch)."""
     E, H, C = w1.shape
-    N, k = w2.shape[1], weights.shape[-1]
+    N = w2.shape[1]
     n = h.shape[0]
-    tile = int(_lib.load().strata_hip_expert_tile(n, E))
+    tile = _expert_tile(n, w1, w2)
     a, keep = _expert_args(x, weights, plan, tile, w1, b1, w2, b2, h, dact, y)
     new = lambda *shape: torch.empty(shape, dtype=torch.bfloat16, device=x.device)  # noqa: E731
     want_x, want_wt = need[0], need[1]
@@ -1633,10 +1641,9 @@ def expert_mlp_bwd(dout: Tensor, x: Tensor, weights: Tensor, w1: Tensor, b1: Opt
     dw1, db1 = (new(E, H, C), new(E, H) if b1 is not None else None) if want_1 else (None, None)
     dw2, db2 = (new(E, N, H), new(E, N) if b2 is not None else None) if want_2 else (None, None)
     g = _dense(dout)
-    gs = new(n, N) if want_2 else None
-    gz, w2t = (new(n, H), new(E, H, N)) if hid else (None, None)
-    dxs, w1t = (new(n, C), new(E, C, H)) if want_x else (None, None)
-    b = _lib.ExpertMlpBwdArgs(a, g.data_ptr(), *(_ptr(t) for t in (dx, dwt, dw1, db1, dw2, db2, gs, gz, dxs, w1t, w2t)))
+    gz = new(n, H) if hid else None
+    dxs = torch.empty((n, C), dtype=torch.float32, device=x.device) if want_x else None
+    b = _lib.ExpertMlpBwdArgs(a, g.data_ptr(), *(_ptr(t) for t in (dx, dwt, dw1, db1, dw2, db2, gz, dxs)))
     _launch("strata_hip_expert_mlp_bwd", b, x)
     return [t if t is not None and wanted else new(0) for t, wanted in zip((dx, dwt, dw1, db1, dw2, db2), need)]
 
@@ -1684,7 +1691,7 @@ def expert_mlp(x: Tensor, weights: Tensor, index: Tensor, w1: Tensor, b1: Option
     ``expert_route`` gives them, w1 ``[E, H, C]``, b1 ``[E, H]`` or None, w2 ``[E, N, H]``, b2
     ``[E, N]`` or None, residual ``[..., N]`` or None; widths multiples of 8, x and the output under
     2 GiB.  An index outside ``[0, E)`` adds nothing, and the same expert may stand in two slots.
-    No token is dropped for an expert's load.  Differentiable once, in every argument but the
+    No token is dropped for an expert's load; a weight under 2^-100 counts as 0.  Differentiable once, in every argument but the
     index."""
     ts = (x, weights, w1, b1, w2, b2, residual)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):

@@ -114,19 +114,19 @@ def test_plan_refusals_and_sizes(lib):
     assert lib.strata_hip_expert_plan_workspace(1024, 8) == 0 and lib.strata_hip_expert_plan_workspace(1025, 8) == 16
     for over, code in ((dict(pairs=-1), _lib.EINVAL), (dict(experts=0), _lib.EINVAL), (dict(tile=0), _lib.EINVAL),
                        (dict(experts=513), _lib.EUNSUPPORTED), (dict(offsets=None), _lib.EINVAL),
-                       (dict(row_slot=None), _lib.EINVAL), (dict(pairs=2000, workspace=None), _lib.EINVAL)):
-        a = _lib.ExpertPlanArgs(*[0x1000] * 6, 100, 8, 64)
+                       (dict(row_token=None), _lib.EINVAL), (dict(weights=None), _lib.EINVAL), (dict(top_k=3), _lib.EINVAL), (dict(pairs=2000, workspace=None), _lib.EINVAL)):
+        a = _lib.ExpertPlanArgs(*[0x1000] * 8, 100, 2, 8, 64, 0)
         for k, v in over.items():
             setattr(a, k, v)
         assert lib.strata_hip_expert_plan(ctypes.byref(a), None) == code, over
 
 
 def _mlp_args(lib, **over):
-    a = _lib.ExpertMlpArgs(*[0x1000] * 15, 16, 64, 64, 2, 8, 64, 128, 64, 0)
+    a = _lib.ExpertMlpArgs(*[0x1000] * 16, 16, 64, 64, 2, 8, 64, 128, 64, 0)
     for k, v in over.items():
         setattr(a, k, v)
     if a.tile == 0:
-        a.tile = lib.strata_hip_expert_tile(a.tokens * a.top_k, a.experts)
+        a.tile = lib.strata_hip_expert_tile(a.tokens * a.top_k, a.experts, a.dim, a.hidden, a.out_dim)
     return a
 
 
@@ -140,16 +140,16 @@ def _mlp_args(lib, **over):
 def test_mlp_refusals(lib, over, code, msg):
     a = _mlp_args(lib, **over)
     assert lib.strata_hip_expert_mlp(ctypes.byref(a), None) == code and msg in lib.strata_hip_last_error().decode()
-    b = _lib.ExpertMlpBwdArgs(a, *[0x1000] * 12)
+    b = _lib.ExpertMlpBwdArgs(a, *[0x1000] * 9)
     assert lib.strata_hip_expert_mlp_bwd(ctypes.byref(b), None) == code
 
 
 @pytest.mark.parametrize("over,msg", [
-    (dict(dout=None), "dout"), (dict(gs=None), "gs"), (dict(gz=None), "gz"), (dict(w2t=None), "w2t"), (dict(dxs=None), "dxs"),
+    (dict(dout=None), "dout"), (dict(gz=None), "gz"), (dict(dxs=None), "dxs"),
     (dict(dw2=None), "bias gradient"), (dict(dw1=None), "bias gradient"), (dict(dx=0x1008), "aligned"),
 ])
 def test_mlp_bwd_refusals(lib, over, msg):
-    b = _lib.ExpertMlpBwdArgs(_mlp_args(lib), *[0x1000] * 12)
+    b = _lib.ExpertMlpBwdArgs(_mlp_args(lib), *[0x1000] * 9)
     for k, v in over.items():
         setattr(b, k, v)
     assert lib.strata_hip_expert_mlp_bwd(ctypes.byref(b), None) == _lib.EINVAL

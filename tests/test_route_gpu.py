@@ -13,7 +13,7 @@ import pytest
 import torch
 
 from oracle import experts as O
-from strata_amd import _lib, ops
+from strata_amd import ops
 
 pytestmark = pytest.mark.gpu
 U = 2.0**-24
@@ -158,30 +158,31 @@ def test_route_repeats_and_replays(gpu):
         assert all(torch.equal(x, y) and torch.equal(x, z) for x, y, z in zip(want, got, again))
 
 
+@pytest.mark.parametrize("tile", [64, 128, 256])
 @pytest.mark.parametrize("n,E", [(0, 3), (1, 1), (2, 8), (63, 5), (64, 64), (65, 2), (1000, 100), (1024, 512), (1025, 8),
                                  (5000, 1), (4097, 300), (70000, 24), (40000, 512)])
-def test_plan(gpu, n, E):
+def test_plan(gpu, n, E, tile):
     """Rows sorted by expert, stable; offsets and tiles; indices that name no expert left out."""
-    print(f"plan {n} {E}", flush=True)
+    print(f"plan {n} {E} {tile}", flush=True)
     g = torch.Generator().manual_seed(n)
+    k = next(d for d in (3, 2, 1) if n % d == 0)
     idx = (torch.rand(n, generator=g) ** 2 * E).int()
     idx[torch.rand(n, generator=g) < 0.1] = -1
     if n > 4:
         idx[3], idx[4] = E, 2**31 - 1
-    plan, tile = ops._expert_plan(idx.to(gpu), E)
-    plan = plan.cpu()
-    row_slot, slot_row, off = plan[:n], plan[n:2 * n], plan[2 * n:2 * n + E + 1]
-    tiles = plan[2 * n + E + 1:]
+    w = torch.randn(n, generator=g).bfloat16()
+    plan = ops._expert_plan(idx.view(-1, k).to(gpu), w.view(-1, k).to(gpu), E, tile).cpu()
+    token, weight, slot_row, off = plan[:n], plan[n:2 * n].view(torch.float32), plan[2 * n:3 * n], plan[3 * n:3 * n + E + 1]
+    tiles = plan[3 * n + E + 1:]
     ok = (idx >= 0) & (idx < E)
     order = torch.where(ok, idx, E).sort(stable=True).indices[: int(ok.sum())]
     R = order.numel()
-    assert torch.equal(row_slot[:R].long(), order)
+    assert torch.equal(token[:R].long(), order // k) and torch.equal(weight[:R], w[order].float())
     want = torch.full((n,), -1, dtype=torch.int32)
     want[order] = torch.arange(R, dtype=torch.int32)
     assert torch.equal(slot_row, want)
     count = torch.bincount(idx[ok].long(), minlength=E)
     assert torch.equal(off.long(), torch.cat([torch.zeros(1, dtype=torch.int64), count.cumsum(0)]))
-    wt = [(e, int(off[e]) + k) for e in range(E) for k in range(0, int(count[e]), tile)]
+    wt = [(e, int(off[e]) + r) for e in range(E) for r in range(0, int(count[e]), tile)]
     assert int(tiles[0]) == len(wt)
     assert tiles[1:1 + 2 * len(wt)].view(-1, 2).tolist() == [list(t) for t in wt]
-    assert tile == _lib.load().strata_hip_expert_tile(n, E)
