@@ -25,7 +25,7 @@
 
 namespace strata {
 
-typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 __device__ __forceinline__ void gelu_both(float x, float& y, float& d) {
   // x s and its derivative s + x s (1 - s) 2u' with s = sigmoid(2u), u = sqrt(2/pi) (x + 0.044715 x^3)
@@ -54,6 +54,7 @@ struct ExpertGemm {
   const int32_t* tiles;
   int64_t ldx;
   int N, K, nt;
+  int round;             // 256 x 256 tiles that run at once
 };
 
 enum { EX_HIDDEN = 0, EX_OUT = 1, EX_HIDDEN_GRAD = 2 };
@@ -72,13 +73,19 @@ struct ExpertTile {
   int e, row0, rows, n0;
 };
 
+// The plan by scalar loads: they are counted apart from the copies in flight.
+__device__ __forceinline__ int plan_load(const int32_t* p, int i) {
+  return ((const __attribute__((address_space(4))) int32_t*)(uintptr_t)p)[__builtin_amdgcn_readfirstlane(i)];
+}
+
 // BM x BN tiles of the experts' products: x and w stream into an LDS ring of NST stages of
 // 64 columns (buffer_load ... lds) ahead of v_mfma_f32_32x32x16_bf16, whose A operand the
 // weights are: a lane owns four consecutive columns of one row.
 // BIG: 256 x 256, one workgroup a CU walks over the tiles; the last step of a tile starts
-// the next one's first stage, whose rows' tokens were loaded a tile ahead.  Otherwise one
-// tile a workgroup and several workgroups a CU.
-template <int BM, int BN, int WGM, int WGN, int NST, int MODE, bool WT>
+// the next one's first stage.  Otherwise one tile a workgroup and several workgroups a CU.
+// TAIL: the 256 x 256 tiles of a last round that would leave half of the CUs or more idle,
+// each as four 128 x 128 ones (the same sums in the same order).
+template <int BM, int BN, int WGM, int WGN, int NST, int MODE, bool WT, bool TAIL>
 __global__ __launch_bounds__(64 * WGM * WGN, 1) void expert_gemm_kernel(ExpertGemm p) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr bool BIG = BM == 256, GATHER = MODE != EX_OUT;
@@ -88,41 +95,70 @@ __global__ __launch_bounds__(64 * WGM * WGN, 1) void expert_gemm_kernel(ExpertGe
   constexpr int XB = BM * ROWB, XCH = XB / 1024, STAGE = XB + BN * ROWB;
   constexpr int LPX = XCH / NW, LPW = BN * ROWB / 1024 / NW;  // 1-KiB copies a wave and stage
   constexpr int WLPR = BN / 8, WRPC = 64 / WLPR;             // WT: lanes a row, rows a copy
-  constexpr int HALVES = BIG ? 2 : 1, HM = FM / HALVES;
-  constexpr int SLAB = HM * 32 * WTN * 2;
+  constexpr int SLAB = 32 * WTN * 4;
   static_assert(WTM % 32 == 0 && WTN % 32 == 0 && XCH % NW == 0 && (STAGE / 1024) % NW == 0, "wave tile / stage layout");
   static_assert(NW * SLAB <= (BIG ? STAGE : NST * STAGE) && (!BIG || NST == 2), "the epilogue slabs fit the ring");
-  __shared__ __attribute__((aligned(1024))) char lds[NST * STAGE];
+  // BIG: what a tile needs besides its stages, copied to LDS a tile ahead and read where it is
+  // used (loads into registers would wait, in order, for the copies and stores before them):
+  // the rows' tokens, their weights, the columns' bias.
+  constexpr int TOKENS = 0, WEIGHTS = BM * 4, BIAS = BM * 8, META = BM * 8 + BN * 2;
+  __shared__ __attribute__((aligned(1024))) char lds[NST * STAGE + (BIG ? 2 * META : 0)];
 
   const int tid = (int)__builtin_amdgcn_workitem_id_x();
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int wm = wave / WGN, wn = wave % WGN, l32 = lane & 31, hi = lane >> 5;
   const uint32_t lds_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+  const bool weigh = MODE != EX_OUT || p.bias, biased = MODE != EX_HIDDEN_GRAD && p.bias;  // uniform
 
   // The grid is sized for the most tiles that the pairs can make; the plan says how many there are.
-  const int mt = p.tiles[0], total = mt * p.nt, wg_id = (int)__builtin_amdgcn_workgroup_id_x();
+  const int mt = plan_load(p.tiles, 0), all = mt * p.nt, wg_id = (int)__builtin_amdgcn_workgroup_id_x();
+  int tail = BIG || TAIL ? all > p.round ? all % p.round : 0 : 0;
+  if (2 * tail > p.round) tail = 0;
+  const int total = BIG ? all - tail : TAIL ? 4 * tail : all;
   if (wg_id >= total) return;
   auto tile_at = [&](int t) {
-    const int wg = xcd_tile_order(total, t);
-    constexpr int GRP = BIG ? 4 : 8;  // row panels x every column panel, row panel fastest
+    const int wg = xcd_tile_order(all, TAIL ? all - tail + t / 4 : t);
+    constexpr int GRP = BIG || TAIL ? 4 : 8;  // row panels x every column panel, row panel fastest
     const int gi = wg / (GRP * p.nt), li = wg % (GRP * p.nt), gmn = min(GRP, mt - gi * GRP);
     const int tm = gi * GRP + li % gmn;
     ExpertTile r;
-    r.e = p.tiles[1 + 2 * tm];
-    r.row0 = p.tiles[2 + 2 * tm];
-    r.rows = min(p.offsets[r.e + 1] - r.row0, BM);
-    r.n0 = (li / gmn) * BN;
+    r.e = plan_load(p.tiles, 1 + 2 * tm);
+    r.row0 = plan_load(p.tiles, 2 + 2 * tm);
+    r.rows = plan_load(p.offsets, r.e + 1) - r.row0;
+    r.n0 = (li / gmn) * (TAIL ? 2 * BN : BN);
+    if (TAIL) {
+      r.rows = min(r.rows, 2 * BM) - BM * (t >> 1 & 1);
+      r.row0 += BM * (t >> 1 & 1);
+      r.n0 += BN * (t & 1);
+    }
+    r.rows = min(r.rows, BM);
     return r;
   };
   const int nk = (p.K + BK - 1) / BK, ktail = p.K % BK;
-  // lane offsets of a tile's x rows
-  auto x_offsets = [&](const ExpertTile& t, uint32_t (&vo)[LPX]) {
+  // wave w copies dwords 64 (w % 4) .. of the rows' tokens (w < 4) or weights, and of the bias
+  auto issue_meta = [&](const ExpertTile& t, int buf) {
+    const uint32_t dst = lds_base + NST * STAGE + buf * META;
+    const int i = 64 * (wave & 3) + lane;
+    const uint32_t vo = i < t.rows ? 4u * i : OOB;
+    if (wave < 4) {
+      if (GATHER) dma_dword(make_rsrc(p.token + t.row0, OOB), dst + TOKENS + 256 * wave, vo);
+    } else if (weigh) {
+      dma_dword(make_rsrc(p.weight + t.row0, OOB), dst + WEIGHTS + 256 * (wave - 4), vo);
+    }
+    if (biased && wave < BN / 128) {
+      const int c = 128 * wave + 2 * lane;
+      dma_dword(make_rsrc(p.bias + (int64_t)t.e * p.N + t.n0, OOB), dst + BIAS + 256 * wave, t.n0 + c < p.N ? 2u * c : OOB);
+    }
+  };
+  // lane offsets of a tile's x rows (BIG: their tokens in LDS buffer buf)
+  auto x_offsets = [&](const ExpertTile& t, uint32_t (&vo)[LPX], int buf) {
 #pragma unroll
     for (int j = 0; j < LPX; ++j) {
       const int row = RPC * (j * NW + wave) + lane / CH;
       const uint32_t chunk = ((lane % CH) ^ ex_swz(row)) * 16;
       int64_t at = row;
-      if (GATHER && row < t.rows) at = p.token[t.row0 + row];
+      if (GATHER && BIG) at = *(const int*)(lds + NST * STAGE + buf * META + TOKENS + 4 * row);
+      else if (GATHER && row < t.rows) at = p.token[t.row0 + row];
       vo[j] = row < t.rows ? (uint32_t)(at * p.ldx * 2) + chunk : OOB;
     }
   };
@@ -142,28 +178,29 @@ __global__ __launch_bounds__(64 * WGM * WGN, 1) void expert_gemm_kernel(ExpertGe
     const bf16* base = GATHER ? p.x : p.x + (int64_t)t.row0 * p.ldx;
     const u32x4 r = make_rsrc((const char*)base + (int64_t)kt * BK * 2, OOB);
     const uint32_t dst = lds_base + slot * STAGE + wave * 1024;
-    const bool last = ktail && kt == nk - 1;  // uniform: chunks at or past K read as zero
+    if (ktail && kt == nk - 1) {  // uniform: chunks at or past K read as zero
 #pragma unroll
-    for (int j = 0; j < LPX; ++j) {
-      uint32_t o = vo[j];
-      if (last && ((lane % CH) ^ ex_swz(RPC * (j * NW + wave) + lane / CH)) * 8 >= ktail) o = OOB;
-      dma_row16(r, dst + j * NW * 1024, o);
+      for (int j = 0; j < LPX; ++j)
+        dma_row16(r, dst + j * NW * 1024, ((lane % CH) ^ ex_swz(RPC * (j * NW + wave) + lane / CH)) * 8 >= ktail ? OOB : vo[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < LPX; ++j) dma_row16(r, dst + j * NW * 1024, vo[j]);
     }
   };
   auto issue_w = [&](const ExpertTile& t, const uint32_t (&vo)[LPW], int kt, int slot) {
     const bf16* base = p.w + (int64_t)t.e * p.N * p.K + (WT ? (int64_t)kt * BK * p.N + t.n0 : (int64_t)t.n0 * p.K + kt * BK);
     const u32x4 r = make_rsrc(base, OOB);
     const uint32_t dst = lds_base + slot * STAGE + XB + wave * 1024;
-    const bool last = ktail && kt == nk - 1;
+    if (ktail && kt == nk - 1) {
 #pragma unroll
-    for (int j = 0; j < LPW; ++j) {
-      uint32_t o = vo[j];
-      if (last) {
-        if (WT ? WRPC * (j * NW + wave) + lane / WLPR >= ktail
-               : ((lane % CH) ^ ex_swz(RPC * (j * NW + wave) + lane / CH)) * 8 >= ktail)
-          o = OOB;
+      for (int j = 0; j < LPW; ++j) {
+        const bool past = WT ? WRPC * (j * NW + wave) + lane / WLPR >= ktail
+                             : ((lane % CH) ^ ex_swz(RPC * (j * NW + wave) + lane / CH)) * 8 >= ktail;
+        dma_row16(r, dst + j * NW * 1024, past ? OOB : vo[j]);
       }
-      dma_row16(r, dst + j * NW * 1024, o);
+    } else {
+#pragma unroll
+      for (int j = 0; j < LPW; ++j) dma_row16(r, dst + j * NW * 1024, vo[j]);
     }
   };
 
@@ -203,84 +240,70 @@ __global__ __launch_bounds__(64 * WGM * WGN, 1) void expert_gemm_kernel(ExpertGe
 
   f32x16 acc[FN][FM];
   ExpertTile t = tile_at(wg_id), tn = t;
-  uint32_t xo[LPX], xn[LPX], wo[LPW];
-  x_offsets(t, xo);
+  if (TAIL && (t.rows <= 0 || t.n0 >= p.N)) return;
+  uint32_t xo[LPX], wo[LPW];
+  int mb = 0;  // the tile's buffer
+  if (BIG) {
+    issue_meta(t, 0);
+    wait_vmcnt(0);
+    lds_barrier();
+  }
+  // BIG: slot rd holds the next stage to read, wr takes the next issue
   int rd = 0, wr = 1;
-  bool in_flight = false;  // BIG: the tile's first stage was issued by the previous tile
+  bool in_flight = false;  // the tile's first stage was issued by the previous tile
   for (int ti = wg_id; ti < total; ti += (int)gridDim.x) {
     const bool more = BIG && ti + (int)gridDim.x < total;
-    w_offsets(t, wo);
-    if (BIG) {
+    const int gn0 = t.n0 + wn * WTN, wr0 = wm * WTM;
+    bf16x8 af[2][FN], bfr[2][FM];
+    auto multiply = [&](int cb) {
+#pragma unroll
+      for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int j = 0; j < FM; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af[cb][i], bfr[cb][j], acc[i][j], 0, 0, 0);
+    };
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+      for (int j = 0; j < FM; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+    if constexpr (BIG) {
+      if (!in_flight) {
+        if (ti != wg_id) {  // a product of one step: the tile's tokens are waited for here
+          wait_vmcnt(0);
+          lds_barrier();
+        }
+        x_offsets(t, xo, mb);
+      }
+      w_offsets(t, wo);
       if (!in_flight) {
         issue_x(t, xo, 0, rd);
         issue_w(t, wo, 0, rd);
       }
-    } else {
-#pragma unroll
-      for (int s = 0; s < NST - 1; ++s)
-        if (s < nk) {
-          issue_x(t, xo, s, s);
-          issue_w(t, wo, s, s);
-        }
-    }
-    const int gn0 = t.n0 + wn * WTN, wr0 = wm * WTM;
-    // the rows' weights: scale of h, factor of the bias, factor of gz
-    float rw[FM];
-    const bool weigh = MODE != EX_OUT || p.bias;  // uniform
-#pragma unroll
-    for (int j = 0; j < FM; ++j) {
-      const int r = wr0 + 32 * j + l32;
-      rw[j] = weigh && r < t.rows ? p.weight[t.row0 + r] : 0.f;
-      if (MODE != EX_HIDDEN_GRAD) rw[j] = row_scale(rw[j]);
-    }
-    // the bias as the accumulators' first C operand (columns 8q + 4hi + e of each 32)
-#pragma unroll
-    for (int i = 0; i < FN; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        u32x2 bb = {0u, 0u};
-        if (MODE != EX_HIDDEN_GRAD && p.bias)
-          bb = *(const u32x2*)(p.bias + (int64_t)t.e * p.N + min(gn0 + 32 * i + 8 * q + 4 * hi, p.N - 4));
-        const float b4[4] = {bf16_lo(bb[0]), bf16_hi(bb[0]), bf16_lo(bb[1]), bf16_hi(bb[1])};
-#pragma unroll
-        for (int j = 0; j < FM; ++j)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) acc[i][j][4 * q + x] = MODE == EX_OUT ? rw[j] * b4[x] : b4[x];
-      }
-    if (more) {
-      tn = tile_at(ti + (int)gridDim.x);
-      if (GATHER) x_offsets(tn, xn);
-    }
-
-    bf16x8 af[2][FN], bfr[2][FM];
-    if constexpr (BIG) {
+      if (more) tn = tile_at(ti + (int)gridDim.x);
       in_flight = false;
-      for (int kt = 0; kt < nk; ++kt) {
+      auto kstep = [&](int kt, auto last) {
+        constexpr bool LAST = decltype(last)::value;
         wait_vmcnt(0);
         lds_barrier();  // the stage has landed for every wave; slot wr is free
-        const bool step = kt + 1 < nk;
-        if (step) {
+        if (more && kt == 0) issue_meta(tn, mb ^ 1);
+        if (!LAST) {
           issue_x(t, xo, kt + 1, wr);
-        } else if (more) {
-          uint32_t wn_[LPW];
-          if (!GATHER) x_offsets(tn, xn);
-          w_offsets(tn, wn_);
-          issue_x(tn, xn, 0, wr);
-          issue_w(tn, wn_, 0, wr);
+        } else if (more && kt > 0) {  // the next tile's first stage
+          w_offsets(tn, wo);
+          x_offsets(tn, xo, mb ^ 1);
+          issue_x(tn, xo, 0, wr);
+          issue_w(tn, wo, 0, wr);
           in_flight = true;
         }
         const char* st = lds + rd * STAGE;
         load_frags(st, 0, af[0], bfr[0]);
 #pragma unroll
         for (int kk = 0; kk < BK / 16; ++kk) {
-          const int cb = kk & 1;
-          if (kk + 1 < BK / 16) load_frags(st, kk + 1, af[cb ^ 1], bfr[cb ^ 1]);
-#pragma unroll
-          for (int i = 0; i < FN; ++i)
-#pragma unroll
-            for (int j = 0; j < FM; ++j)
-              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af[cb][i], bfr[cb][j], acc[i][j], 0, 0, 0);
-          if (kk == 0 && step) {  // the weights' copies behind the first MFMAs
+          if (kk + 1 < BK / 16) load_frags(st, kk + 1, af[(kk + 1) & 1], bfr[(kk + 1) & 1]);
+          multiply(kk & 1);
+          if (kk == 0 && !LAST) {  // the weights' copies behind the first MFMAs
             __builtin_amdgcn_sched_barrier(0);
             issue_w(t, wo, kt + 1, wr);
             __builtin_amdgcn_sched_barrier(0);
@@ -289,9 +312,18 @@ __global__ __launch_bounds__(64 * WGM * WGN, 1) void expert_gemm_kernel(ExpertGe
         __builtin_amdgcn_iglp_opt(1);
         rd ^= 1;
         wr ^= 1;
-      }
+      };
+      for (int kt = 0; kt + 1 < nk; ++kt) kstep(kt, std::false_type{});
+      kstep(nk - 1, std::true_type{});
     } else {
-      rd = 0;
+      x_offsets(t, xo, 0);
+      w_offsets(t, wo);
+#pragma unroll
+      for (int s = 0; s < NST - 1; ++s)
+        if (s < nk) {
+          issue_x(t, xo, s, s);
+          issue_w(t, wo, s, s);
+        }
       for (int kt = 0; kt < nk; ++kt) {
         if (NST > 2 && kt + NST - 2 < nk) wait_vmcnt((NST - 2) * (LPX + LPW));
         else wait_vmcnt(0);
@@ -308,108 +340,98 @@ __global__ __launch_bounds__(64 * WGM * WGN, 1) void expert_gemm_kernel(ExpertGe
         for (int kk = 0; kk < BK / 16; ++kk) {
           const int cb = kk & 1;
           if (kk + 1 < BK / 16) load_frags(st, kk + 1, af[cb ^ 1], bfr[cb ^ 1]);
-#pragma unroll
-          for (int i = 0; i < FN; ++i)
-#pragma unroll
-            for (int j = 0; j < FM; ++j)
-              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af[cb][i], bfr[cb][j], acc[i][j], 0, 0, 0);
+          multiply(cb);
         }
       }
     }
 
-    // ---- epilogue ----
-    if constexpr (MODE == EX_OUT) {  // fp32, straight from the accumulators
-      float* out = (float*)p.out;
+    // ---- epilogue: 32 rows of the wave's tile at a time through its LDS slab in fp32, back as
+    // eight consecutive columns a lane, so that every load and store moves whole 16-byte runs of
+    // a row (BIG: the slabs are in the slot read last, the other takes the next tile's stage)
+    lds_barrier();  // every wave is done reading the last stage
+    constexpr int NCH = WTN / 4, LPR = WTN / 8, RPI = 64 / LPR, NIT = 32 / RPI;
+    char* slab = lds + (BIG ? wr * STAGE : 0) + wave * SLAB;
+    const char* meta = lds + NST * STAGE + mb * META;
+    const int lrow = lane / LPR, lc = lane % LPR, gn = gn0 + 8 * lc;
+    const bool col = gn < p.N;  // N is a multiple of 8: the whole run
+    float b8[8];
+    {
+      u32x4 b = {0u, 0u, 0u, 0u};
+      if (biased) b = BIG ? *(const u32x4*)(meta + BIAS + 2 * (wn * WTN + 8 * lc)) : *(const u32x4*)(p.bias + (int64_t)t.e * p.N + min(gn, p.N - 8));
 #pragma unroll
-      for (int j = 0; j < FM; ++j) {
-        const int r = wr0 + 32 * j + l32;
-        if (r >= t.rows) continue;
-#pragma unroll
-        for (int i = 0; i < FN; ++i)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int gn = gn0 + 32 * i + 8 * q + 4 * hi;
-            if (gn < p.N)
-              *(f32x4*)(out + (int64_t)(t.row0 + r) * p.N + gn) =
-                  (f32x4){acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-          }
+      for (int x = 0; x < 4; ++x) {
+        b8[2 * x] = bf16_lo(b[x]);
+        b8[2 * x + 1] = bf16_hi(b[x]);
       }
-    } else {
-      // two bytes a value through this wave's LDS slab, 16-byte rows out; BIG: half the
-      // wave's rows at a time, in the slot read last (the other takes the next tile)
-      lds_barrier();  // every wave is done reading the last stage
-      constexpr int SRB = WTN * 2, CPR = WTN / 8, RPI = 64 / CPR, NIT = HM * 32 / RPI;
-      char* slab = lds + (BIG ? wr * STAGE : 0) + wave * SLAB;
-      const int c = lane % CPR, gn = gn0 + 8 * c;
-      const bool col = gn < p.N;  // N is a multiple of 8: the whole 16-byte run
-      auto to_slab = [&](int half, auto pack) {
+    }
+    f16x8 dv[2][NIT];  // HIDDEN_GRAD: gelu' of this pass and the next, loaded before this pass's stores
+    auto load_mul = [&](int j) {
 #pragma unroll
-        for (int i = 0; i < FN; ++i)
+      for (int it = 0; it < NIT; ++it) {
+        const int r = wr0 + 32 * j + RPI * it + lrow;
+        dv[j & 1][it] = (f16x8){};
+        if (col && r < t.rows) dv[j & 1][it] = *(const f16x8*)(p.mul + (int64_t)(t.row0 + r) * p.N + gn);
+      }
+    };
+    if (MODE == EX_HIDDEN_GRAD) load_mul(0);
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int nl = 32 * i + 8 * q + 4 * hi;
+    for (int j = 0; j < FM; ++j) {
 #pragma unroll
-            for (int jj = 0; jj < HM; ++jj) {
-              const int ml = 32 * jj + l32;
-              *(u32x2*)(slab + ml * SRB + (((nl >> 3) ^ (ml & (CPR - 1))) << 4) + 8 * hi) = pack(i, half * HM + jj, q);
-            }
+      for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *(f32x4*)(slab + l32 * (WTN * 4) + (((8 * i + 2 * q + hi) ^ (l32 & (NCH - 1))) << 4)) =
+              (f32x4){acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+      if (MODE == EX_HIDDEN_GRAD && j + 1 < FM) load_mul(j + 1);
+#pragma unroll
+      for (int it = 0; it < NIT; ++it) {
+        const int sl = RPI * it + lrow, r = wr0 + 32 * j + sl;
+        const f32x4 z0 = *(const f32x4*)(slab + sl * (WTN * 4) + (((2 * lc) ^ (sl & (NCH - 1))) << 4));
+        const f32x4 z1 = *(const f32x4*)(slab + sl * (WTN * 4) + (((2 * lc + 1) ^ (sl & (NCH - 1))) << 4));
+        float v[8] = {z0[0], z0[1], z0[2], z0[3], z1[0], z1[1], z1[2], z1[3]};
+        // the row's weight: scale of h, factor of the bias, factor of gz
+        float w = 0.f;
+        if (weigh) w = BIG ? *(const float*)(meta + WEIGHTS + 4 * r) : r < t.rows ? p.weight[t.row0 + r] : 0.f;
+        if (MODE != EX_HIDDEN_GRAD) w = row_scale(w);
+        const bool in = col && r < t.rows;
+        const int64_t at = (int64_t)(t.row0 + r) * p.N + gn;
+        if constexpr (MODE == EX_OUT) {
+          f32x4 o0, o1;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            o0[x] = fmaf(w, b8[x], v[x]);
+            o1[x] = fmaf(w, b8[4 + x], v[4 + x]);
           }
-      };
-      auto from_slab = [&](int half, void* dst) {
-        const int r0 = wr0 + half * HM * 32;
-#pragma unroll
-        for (int it = 0; it < NIT; ++it) {
-          const int sl = RPI * it + lane / CPR;
-          const u32x4 v = *(const u32x4*)(slab + sl * SRB + ((c ^ (sl & (CPR - 1))) << 4));
-          if (col && r0 + sl < t.rows) *(u32x4*)((char*)dst + ((int64_t)(t.row0 + r0 + sl) * p.N + gn) * 2) = v;
-        }
-      };
-#pragma unroll
-      for (int half = 0; half < HALVES; ++half) {
-        if constexpr (MODE == EX_HIDDEN) {
-          to_slab(half, [&](int i, int j, int q) {
-            float v[4];
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              float y, d;
-              gelu_both(acc[i][j][4 * q + x], y, d);
-              v[x] = y * rw[j];
-            }
-            return (u32x2){pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
-          });
-          from_slab(half, p.out);
-          if (p.out2) {
-            to_slab(half, [&](int i, int j, int q) {
-              f16x4 v;
-#pragma unroll
-              for (int x = 0; x < 4; ++x) {
-                float z = acc[i][j][4 * q + x], y, d;
-                asm volatile("" : "+v"(z));  // computed again: the first pass's values would stay in registers
-                gelu_both(z, y, d);
-                v[x] = (_Float16)d;
-              }
-              return __builtin_bit_cast(u32x2, v);
-            });
-            from_slab(half, p.out2);
+          if (in) {
+            *(f32x4*)((float*)p.out + at) = o0;
+            *(f32x4*)((float*)p.out + at + 4) = o1;
           }
         } else {
-          to_slab(half, [&](int i, int j, int q) {
-            const int r = wr0 + 32 * j + l32, g = gn0 + 32 * i + 8 * q + 4 * hi;
-            f16x4 d = {0, 0, 0, 0};
-            if (r < t.rows && g < p.N) d = *(const f16x4*)(p.mul + (int64_t)(t.row0 + r) * p.N + g);
-            float v[4];
+          f16x8 d8;
+          u32x4 o;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) v[x] = acc[i][j][4 * q + x] * (rw[j] * (float)d[x]);
-            return (u32x2){pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
-          });
-          from_slab(half, p.out);
+          for (int x = 0; x < 8; ++x) {
+            if constexpr (MODE == EX_HIDDEN) {
+              float y, d;
+              gelu_both(v[x] + b8[x], y, d);
+              v[x] = y * w;
+              d8[x] = (_Float16)d;
+            } else {
+              v[x] *= w * (float)dv[j & 1][it][x];
+            }
+          }
+#pragma unroll
+          for (int x = 0; x < 4; ++x) o[x] = pack_bf16x2(v[2 * x], v[2 * x + 1]);
+          if (in) {
+            __builtin_nontemporal_store(o, (u32x4*)((bf16*)p.out + at));
+            if (MODE == EX_HIDDEN && p.out2) __builtin_nontemporal_store(__builtin_bit_cast(u32x4, d8), (u32x4*)(p.out2 + at));
+          }
         }
       }
     }
     if (!BIG) return;
     t = tn;
-#pragma unroll
-    for (int j = 0; j < LPX; ++j) xo[j] = xn[j];
+    mb ^= 1;
   }
 #endif
 }
@@ -508,7 +530,9 @@ __global__ __launch_bounds__(512, 1) void expert_wgrad_kernel(ExpertWgrad p) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr int NW = 8, LPW = EW_HALF / 1024 / NW;
   __shared__ __attribute__((aligned(1024))) char lds[2 * EW_STAGE];
-  __shared__ __attribute__((aligned(8))) bf16 wbuf[2][EW_BK];  // the bias's other operand, by row
+  // a stage's tokens and weights, copied three stages ahead: loads into registers would wait,
+  // in order, for the copies before them
+  __shared__ __attribute__((aligned(1024))) char meta[4][2][EW_BK * 4];
   const int tid = (int)__builtin_amdgcn_workitem_id_x();
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n16 = lane & 15, g4 = lane >> 4;
   const int wk = wave >> 2, wn = wave & 3;  // wave tile: 128 k x 64 n
@@ -528,7 +552,7 @@ __global__ __launch_bounds__(512, 1) void expert_wgrad_kernel(ExpertWgrad p) {
   }
   e = __builtin_amdgcn_readfirstlane(e);
   const int k0 = tk * 256, n0 = tn * 256;
-  const int row0 = p.offsets[e], rows = p.offsets[e + 1] - row0;
+  const int row0 = plan_load(p.offsets, e), rows = plan_load(p.offsets, e + 1) - row0;
   const int nk = (rows + EW_BK - 1) / EW_BK;
 
   uint32_t vx[LPW], vg[LPW];  // the gathered one's without the row
@@ -543,20 +567,22 @@ __global__ __launch_bounds__(512, 1) void expert_wgrad_kernel(ExpertWgrad p) {
   const char* xb = (const char*)(p.x + (OF_G ? (int64_t)row0 * p.ldx : 0) + k0);
   const char* gb = (const char*)(p.g + (OF_G ? 0 : (int64_t)row0 * p.ldg) + n0);
   const uint32_t ldt = (uint32_t)((OF_G ? p.ldg : p.ldx) * 2);
-  // a stage ahead: its gathered rows' byte offsets, and the bias operand's values
-  uint32_t tok[LPW];
-  const bool sums_wg = p.bias_out && tk == 0, sums = sums_wg && wk == 0;  // uniform per workgroup, per wave
-  float wnext = 0.f;
-  auto fetch = [&](int kt) {
+  const bool sums = p.bias_out && tk == 0 && wk == 0;  // uniform per wave
+  const uint32_t meta_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)meta;
+  auto issue_meta = [&](int kt) {  // wave 0: tokens, wave 1: weights
+    const int r = kt * EW_BK + lane;
+    const uint32_t vo = r < rows ? 4u * r : OOB;
+    if (wave == 0) dma_dword(make_rsrc(p.token + row0, OOB), meta_base + (kt & 3) * 2 * EW_BK * 4, vo);
+    if (wave == 1) dma_dword(make_rsrc(p.weight + row0, OOB), meta_base + ((kt & 3) * 2 + 1) * EW_BK * 4, vo);
+  };
+  uint32_t vt[LPW];  // the gathered operand's offsets of the stage issued next
+  auto offsets = [&](int kt) {
 #pragma unroll
     for (int j = 0; j < LPW; ++j) {
-      const int r = kt * EW_BK + rr[j];
-      tok[j] = OOB;
-      if (r < rows && !(OF_G && no_weight(p.weight[row0 + r]))) tok[j] = (uint32_t)p.token[row0 + r] * ldt;
-    }
-    if (sums_wg && tid < EW_BK) {
-      const int r = kt * EW_BK + tid;
-      wnext = r < rows ? (OF_G ? p.weight[row0 + r] : 1.f) : 0.f;
+      const uint32_t vo = OF_G ? vg[j] : vx[j];
+      bool in = rr[j] < rows - kt * EW_BK && vo != OOB;
+      if (OF_G) in = in && !no_weight(*(const float*)(meta[kt & 3][1] + 4 * rr[j]));
+      vt[j] = in ? vo + *(const uint32_t*)(meta[kt & 3][0] + 4 * rr[j]) * ldt : OOB;
     }
   };
   auto issue = [&](int kt, int slot, bool is_g) {
@@ -565,12 +591,12 @@ __global__ __launch_bounds__(512, 1) void expert_wgrad_kernel(ExpertWgrad p) {
     const char* base = is_g ? gb : xb;
     const u32x4 r = make_rsrc(gathered ? base : base + (int64_t)kt * EW_BK * (is_g ? p.ldg : p.ldx) * 2, OOB);
     const uint32_t dst = lds_base + slot * EW_STAGE + (is_g ? EW_HALF : 0) + wave * 1024;
+    if (gathered || left >= EW_BK) {
 #pragma unroll
-    for (int j = 0; j < LPW; ++j) {
-      uint32_t vo = is_g ? vg[j] : vx[j];
-      if (gathered) vo = vo == OOB || tok[j] == OOB ? OOB : vo + tok[j];
-      else if (left < EW_BK && rr[j] >= left) vo = OOB;
-      dma_row16(r, dst + j * NW * 1024, vo);
+      for (int j = 0; j < LPW; ++j) dma_row16(r, dst + j * NW * 1024, gathered ? vt[j] : is_g ? vg[j] : vx[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < LPW; ++j) dma_row16(r, dst + j * NW * 1024, rr[j] < left ? (is_g ? vg[j] : vx[j]) : OOB);
     }
   };
 
@@ -597,25 +623,24 @@ __global__ __launch_bounds__(512, 1) void expert_wgrad_kernel(ExpertWgrad p) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[i][j] = bacc[j];
   }
-  // bias operand: rows 4 g4 .. + 3 and 16 + 4 g4 .. + 3 of a sub-step, as the fragments
   if (nk > 0) {
-    fetch(0);
-    issue(0, 0, false);
-    issue(0, 0, true);
-    if (sums_wg && tid < EW_BK) wbuf[0][tid] = (bf16)wnext;
-    fetch(1);
-  }
-  for (int kt = 0; kt < nk; ++kt) {
+    issue_meta(0);
+    if (nk > 1) issue_meta(1);
+    if (nk > 2) issue_meta(2);
     wait_vmcnt(0);
-    wait_lgkm0();   // wbuf
+    lds_barrier();
+    offsets(0);
+    issue(0, 0, OF_G);
+    issue(0, 0, !OF_G);
+    offsets(1);
+  }
+  auto stage = [&](int kt, auto with_sums) {
+    wait_vmcnt(0);
     lds_barrier();  // the stage has landed for every wave; the other slot is free
     const int wr = (kt + 1) & 1;
     const bool step = kt + 1 < nk;
-    if (step) {
-      issue(kt + 1, wr, OF_G);  // the gathered operand, whose offsets the next fetch overwrites
-      if (sums_wg && tid < EW_BK) wbuf[wr][tid] = (bf16)wnext;
-      fetch(kt + 2);
-    }
+    if (step) issue(kt + 1, wr, OF_G);
+    if (kt + 3 < nk) issue_meta(kt + 3);
     const char* st = lds + (kt & 1) * EW_STAGE;
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
@@ -624,13 +649,21 @@ __global__ __launch_bounds__(512, 1) void expert_wgrad_kernel(ExpertWgrad p) {
       for (int j = 0; j < 4; ++j) b[j] = frag(st, bo[j], kk);
 #pragma unroll
       for (int i = 0; i < 8; ++i) a[i] = frag(st, ao[i], kk);
+      if (kk == 1) offsets(kt + 2);
 #pragma unroll
       for (int i = 0; i < 8; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[j], acc[i][j], 0, 0, 0);
-      if (sums) {
-        const bf16x4 lo = *(const bf16x4*)&wbuf[kt & 1][32 * kk + 4 * g4], hi = *(const bf16x4*)&wbuf[kt & 1][32 * kk + 16 + 4 * g4];
-        const bf16x8 w8 = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      if constexpr (decltype(with_sums)::value) {
+        // the bias's other operand: ones, or the weights of rows 4 g4 .. + 3 and 16 + 4 g4 .. + 3, as the fragments
+        bf16x8 w8;
+        const char* m = meta[kt & 3][1] + 4 * (32 * kk + 4 * g4);
+        const f32x4 lo = OF_G ? *(const f32x4*)m : (f32x4){1.f, 1.f, 1.f, 1.f}, up = OF_G ? *(const f32x4*)(m + 64) : lo;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          w8[x] = (bf16)lo[x];
+          w8[4 + x] = (bf16)up[x];
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j) bacc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w8, b[j], bacc[j], 0, 0, 0);
       }
@@ -640,7 +673,11 @@ __global__ __launch_bounds__(512, 1) void expert_wgrad_kernel(ExpertWgrad p) {
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-  }
+  };
+  if (sums)
+    for (int kt = 0; kt < nk; ++kt) stage(kt, std::true_type{});
+  else
+    for (int kt = 0; kt < nk; ++kt) stage(kt, std::false_type{});
   if (sums && g4 == 0) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -691,13 +728,16 @@ static int launch_expert_gemm(ExpertGemm p, int64_t pairs, int experts, int tile
   p.nt = (p.N + tile - 1) / tile;
   const int64_t mt = pairs / tile + std::min<int64_t>(experts, pairs), total = mt * p.nt;
   if (total > 0x7fffffff) return fail(STRATA_HIP_EUNSUPPORTED, "expert_mlp: problem too large for one launch");
-  if (tile == 256)
-    hipLaunchKernelGGL((expert_gemm_kernel<256, 256, 2, 4, 2, MODE, WT>), dim3((unsigned)std::min<int64_t>(total, expert_cus())),
+  if (tile == 256) {
+    p.round = expert_cus();
+    hipLaunchKernelGGL((expert_gemm_kernel<256, 256, 2, 4, 2, MODE, WT, false>), dim3((unsigned)std::min<int64_t>(total, p.round)),
                        dim3(512), 0, st, p);
-  else if (tile == 128)
-    hipLaunchKernelGGL((expert_gemm_kernel<128, 128, 4, 2, 2, MODE, WT>), dim3((unsigned)total), dim3(512), 0, st, p);
+    if (total > p.round)
+      hipLaunchKernelGGL((expert_gemm_kernel<128, 128, 4, 2, 4, MODE, WT, true>), dim3((unsigned)(p.round / 2 * 4)), dim3(512), 0, st, p);
+  } else if (tile == 128)
+    hipLaunchKernelGGL((expert_gemm_kernel<128, 128, 4, 2, 2, MODE, WT, false>), dim3((unsigned)total), dim3(512), 0, st, p);
   else
-    hipLaunchKernelGGL((expert_gemm_kernel<64, 64, 2, 2, 4, MODE, WT>), dim3((unsigned)total), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((expert_gemm_kernel<64, 64, 2, 2, 4, MODE, WT, false>), dim3((unsigned)total), dim3(256), 0, st, p);
   return check_launch("expert_gemm_kernel");
 }
 
