@@ -649,7 +649,7 @@ int strata_hip_expert_plan(const strata_hip_expert_plan_args* args, void* stream
  * screamcast/checkpoint_compat.py:243-249) with weights of its own for each expert:
  *   out[t] = residual[t] + sum over s of weights[t, s] (gelu(x[t] w1_e^T + b1_e) w2_e^T + b2_e)
  * for the pairs (t, s) that the plan (strata_hip_expert_plan with tile =
- * strata_hip_expert_tile()) gives a row; e is the row's expert.
+ * strata_hip_expert_tile(), train = 1 with dact) gives a row; e is the row's expert.
  * x: [tokens, dim], row stride ldx; weights: [tokens, top_k]; w1 [experts, hidden, dim],
  * b1 [experts, hidden] or NULL, w2 [experts, out_dim, hidden], b2 [experts, out_dim] or NULL,
  * residual [tokens, out_dim] (row stride ldr) or NULL, out [tokens, out_dim]: bf16, contiguous
@@ -680,7 +680,8 @@ typedef struct strata_hip_expert_mlp_args {
   int32_t top_k, experts, dim, hidden, out_dim, tile;
 } strata_hip_expert_mlp_args;
 
-int32_t strata_hip_expert_tile(int64_t pairs, int32_t experts, int32_t dim, int32_t hidden, int32_t out_dim);
+int32_t strata_hip_expert_tile(int64_t pairs, int32_t experts, int32_t dim, int32_t hidden, int32_t out_dim,
+                               int32_t train);
 int strata_hip_expert_mlp(const strata_hip_expert_mlp_args* args, void* stream);
 
 /* Gradients of strata_hip_expert_mlp for dout [tokens, out_dim] bf16 contiguous; `fwd` as in the

@@ -461,7 +461,7 @@ EXPORTS = {
     "strata_hip_expert_route_bwd": ([ctypes.POINTER(ExpertRouteArgs), ctypes.c_void_p], ctypes.c_int),
     "strata_hip_expert_plan": ([ctypes.POINTER(ExpertPlanArgs), ctypes.c_void_p], ctypes.c_int),
     "strata_hip_expert_plan_workspace": ([ctypes.c_int64, ctypes.c_int32], ctypes.c_int64),
-    "strata_hip_expert_tile": ([ctypes.c_int64] + [ctypes.c_int32] * 4, ctypes.c_int32),
+    "strata_hip_expert_tile": ([ctypes.c_int64] + [ctypes.c_int32] * 5, ctypes.c_int32),
     "strata_hip_expert_mlp": ([ctypes.POINTER(ExpertMlpArgs), ctypes.c_void_p], ctypes.c_int),
     "strata_hip_expert_mlp_bwd": ([ctypes.POINTER(ExpertMlpBwdArgs), ctypes.c_void_p], ctypes.c_int),
     "strata_hip_adamw_workspace": ([ctypes.POINTER(AdamwTensor), ctypes.c_int64], ctypes.c_int64),

@@ -436,6 +436,69 @@ __global__ __launch_bounds__(64 * WGM * WGN, 1) void expert_gemm_kernel(ExpertGe
 #endif
 }
 
+// ---- few rows an expert (a token or a handful while serving): 16 rows x 16 columns a
+// workgroup, W waves with a share of K each, their sums added in LDS in wave order.  Bound by
+// reading the weights, which go straight into registers: a lane reads 32 bytes of a weight row,
+// four lanes its 128-byte line, and the contraction takes the columns in that order.
+template <int MODE, int W>
+__global__ __launch_bounds__(64 * W) void expert_few_kernel(ExpertGemm p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  __shared__ float red[W][16][20];
+  const int tid = (int)__builtin_amdgcn_workitem_id_x(), wave = tid >> 6, lane = tid & 63, n16 = lane & 15, g4 = lane >> 4;
+  const int id = (int)__builtin_amdgcn_workgroup_id_x();
+  if (id >= plan_load(p.tiles, 0) * p.nt) return;
+  const int tm = id / p.nt, n0 = id % p.nt * 16;
+  const int e = plan_load(p.tiles, 1 + 2 * tm), row0 = plan_load(p.tiles, 2 + 2 * tm);
+  const int rows = min(plan_load(p.offsets, e + 1) - row0, 16);
+  const bf16* w = p.w + ((int64_t)e * p.N + min(n0 + n16, p.N - 1)) * p.K;
+  const bool live = n16 < rows;
+  const bf16* x = p.x + (int64_t)(MODE == EX_HIDDEN ? (live ? p.token[row0 + n16] : 0) : row0 + (live ? n16 : 0)) * p.ldx;
+  constexpr int U = 4;
+  const int kc = (p.K + 64 * W - 1) / (64 * W) * 64, k0 = wave * kc, k1 = min(p.K, k0 + kc);
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  const u32x4 zero = {0u, 0u, 0u, 0u};
+  for (int k = k0; k < k1; k += 64 * U) {
+    u32x4 a[U][2], b[U][2];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int c = k + 64 * u + 16 * g4 + 8 * h;
+        a[u][h] = c < k1 ? *(const u32x4*)(w + c) : zero;
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int c = k + 64 * u + 16 * g4 + 8 * h;
+        b[u][h] = live && c < k1 ? *(const u32x4*)(x + c) : zero;
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a[u][h]), __builtin_bit_cast(bf16x8, b[u][h]),
+                                                      acc, 0, 0, 0);
+  }
+  *(f32x4*)&red[wave][n16][4 * g4] = acc;  // row n16, columns 4 g4 .. + 3
+  __syncthreads();
+  const int r = tid >> 4, c = tid & 15;
+  if (tid >= 256 || r >= rows || n0 + c >= p.N) return;
+  float z = 0.f;
+#pragma unroll
+  for (int i = 0; i < W; ++i) z += red[i][r][c];
+  const float b = p.bias ? (float)p.bias[(int64_t)e * p.N + n0 + c] : 0.f, s = row_scale(p.weight[row0 + r]);
+  const int64_t at = (int64_t)(row0 + r) * p.N + n0 + c;
+  if (MODE == EX_HIDDEN) {
+    float y, d;
+    gelu_both(z + b, y, d);
+    ((bf16*)p.out)[at] = (bf16)(y * s);
+  } else {
+    ((float*)p.out)[at] = fmaf(s, b, z);
+  }
+#endif
+}
+
 // ---- out[t] = residual[t] + sum over s of y_r, eight channels a thread; without weights: dx ----
 struct ExpertCombine {
   const float* y;
@@ -701,14 +764,15 @@ __global__ __launch_bounds__(512, 1) void expert_wgrad_kernel(ExpertWgrad p) {
 #endif
 }
 
-// Rows of a tile: 256 where the products fill the chip with 256 x 256 tiles, 64 where an
-// expert has fewer than 96 rows on average, else 128.
-static int expert_tile(int64_t pairs, int experts, int64_t width) {
+// Rows of a tile: 16 for fewer than 16 rows an expert without a backward, 256 where the products fill
+// the chip with 256 x 256 tiles, 64 where an expert has fewer than 96 rows on average, else 128.
+static int expert_tile(int64_t pairs, int experts, int64_t width, bool train) {
+  if (!train && pairs < 16 * (int64_t)experts) return 16;
   if (pairs < 96 * (int64_t)experts) return 64;
   return pairs >= 512 * (int64_t)experts && (pairs / 256) * ((width + 255) / 256) >= 200 ? 256 : 128;
 }
 static int expert_tile(const strata_hip_expert_mlp_args* a) {
-  return expert_tile(a->tokens * (int64_t)a->top_k, a->experts, std::min(std::min(a->dim, a->hidden), a->out_dim));
+  return expert_tile(a->tokens * (int64_t)a->top_k, a->experts, std::min(std::min(a->dim, a->hidden), a->out_dim), a->dact != nullptr);
 }
 
 static int expert_cus() {
@@ -728,6 +792,15 @@ static int launch_expert_gemm(ExpertGemm p, int64_t pairs, int experts, int tile
   p.nt = (p.N + tile - 1) / tile;
   const int64_t mt = pairs / tile + std::min<int64_t>(experts, pairs), total = mt * p.nt;
   if (total > 0x7fffffff) return fail(STRATA_HIP_EUNSUPPORTED, "expert_mlp: problem too large for one launch");
+  if constexpr (!WT && MODE != EX_HIDDEN_GRAD) {
+    if (tile == 16) {
+      if (p.K > 1024)
+        hipLaunchKernelGGL((expert_few_kernel<MODE, 16>), dim3((unsigned)total), dim3(1024), 0, st, p);
+      else
+        hipLaunchKernelGGL((expert_few_kernel<MODE, 4>), dim3((unsigned)total), dim3(256), 0, st, p);
+      return check_launch("expert_few_kernel");
+    }
+  }
   if (tile == 256) {
     p.round = expert_cus();
     hipLaunchKernelGGL((expert_gemm_kernel<256, 256, 2, 4, 2, MODE, WT, false>), dim3((unsigned)std::min<int64_t>(total, p.round)),
@@ -768,11 +841,12 @@ static int expert_check(const std::string& name, const strata_hip_expert_mlp_arg
   const int64_t pairs = a->tokens * (int64_t)a->top_k;
   if (a->experts > 512 || pairs > 0x7ffffff0 || a->dim > 32768 || a->hidden > 32768 || a->out_dim > 32768)
     return fail(STRATA_HIP_EUNSUPPORTED, name + ": at most 512 experts, widths 32768 and 2^31 pairs");
-  if (a->tile != expert_tile(a)) return fail(STRATA_HIP_EINVAL, name + ": tile is not strata_hip_expert_tile()'s");
+  if (pairs > 0 && a->tile != expert_tile(a)) return fail(STRATA_HIP_EINVAL, name + ": tile is not strata_hip_expert_tile()'s");
   if (!a->w1 || !a->w2 || !a->offsets || !a->tiles) return fail(STRATA_HIP_EINVAL, name + ": null pointer");
   if (((uintptr_t)a->w1 & 15) || ((uintptr_t)a->w2 & 15) || ((uintptr_t)a->b1 & 7) || ((uintptr_t)a->b2 & 7))
     return fail(STRATA_HIP_EINVAL, name + ": weights must be 16-byte, biases 8-byte aligned");
   if (pairs == 0) return STRATA_HIP_OK;
+  if (!a->dact && name != "expert_mlp") return fail(STRATA_HIP_EINVAL, name + ": dact is needed");
   if (!a->x || !a->weights || !a->row_token || !a->row_weight || !a->slot_row || !a->h || !a->y)
     return fail(STRATA_HIP_EINVAL, name + ": null pointer");
   if (((uintptr_t)a->x & 15) || ((uintptr_t)a->h & 15) || ((uintptr_t)a->y & 15) || ((uintptr_t)a->dact & 15) || a->ldx % 8 ||
@@ -788,8 +862,9 @@ static int expert_check(const std::string& name, const strata_hip_expert_mlp_arg
 
 using namespace strata;
 
-extern "C" int32_t strata_hip_expert_tile(int64_t pairs, int32_t experts, int32_t dim, int32_t hidden, int32_t out_dim) {
-  return expert_tile(pairs, experts, std::min(std::min(dim, hidden), out_dim));
+extern "C" int32_t strata_hip_expert_tile(int64_t pairs, int32_t experts, int32_t dim, int32_t hidden, int32_t out_dim,
+                                          int32_t train) {
+  return expert_tile(pairs, experts, std::min(std::min(dim, hidden), out_dim), train != 0);
 }
 
 extern "C" int strata_hip_expert_mlp(const strata_hip_expert_mlp_args* a, void* stream) {
@@ -843,7 +918,7 @@ extern "C" int strata_hip_expert_mlp_bwd(const strata_hip_expert_mlp_bwd_args* b
   const bool hid = b->dx || b->dw1;  // gradients below the hidden layer
   if (pairs > 0) {
     if (!b->dout || ((uintptr_t)b->dout & 15)) return fail(STRATA_HIP_EINVAL, name + ": dout must be given, 16-byte aligned");
-    if (hid && (!a->dact || !b->gz)) return fail(STRATA_HIP_EINVAL, name + ": dact and gz are needed for dx and dw1");
+    if (hid && !b->gz) return fail(STRATA_HIP_EINVAL, name + ": gz is needed for dx and dw1");
     if (b->dx && !b->dxs) return fail(STRATA_HIP_EINVAL, name + ": dxs is needed for dx");
   }
   if ((b->db2 && !b->dw2) || (b->db1 && !b->dw1)) return fail(STRATA_HIP_EINVAL, name + ": a bias gradient comes with its weight's");

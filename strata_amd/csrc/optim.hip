@@ -31,7 +31,7 @@ constexpr int AW_CHUNK = 4096;   // elements per workgroup of the step
 constexpr int AW_SUM = 16384;    // elements per workgroup of the sum of squares
 constexpr int AW_HEAD = 8;       // doubles before the partial sums
 constexpr int AW_PER = 48;       // tensors per launch: 80 bytes each in 4 KiB of arguments
-enum { AW_P32 = 1, AW_G32 = 2, AW_Q8 = 4, AW_ALIGNED = 8 };
+enum { AW_P32 = 1, AW_G32 = 2, AW_ALIGNED = 4 };
 
 struct AwTensor {
   void* p;
@@ -84,36 +84,37 @@ __global__ __launch_bounds__(256) void aw_sum_kernel(SumBatch b) {
   const uint32_t wide = b.wide[e];
   const int tid = threadIdx.x;
   double s = 0.;
-  if (wide & 1) {
-    const float* g = (const float*)b.g[e];
-    if ((wide & 2) && i1 - i0 == AW_SUM) {
-#pragma unroll 8
-      for (int k = 0; k < AW_SUM / 1024; ++k) {
-        const f32x4 v = *(const f32x4*)(g + i0 + 1024 * k + 4 * tid);
+  if ((wide & 2) && i1 - i0 == AW_SUM) {  // whole and aligned: eight 16-byte loads in flight a thread
+    constexpr int U = 8;
+    const int rounds = (wide & 1) ? AW_SUM / (1024 * U) : AW_SUM / (2048 * U);
+    const char* q = (const char*)b.g[e] + i0 * ((wide & 1) ? 4 : 2) + 16 * tid;
+    for (int k = 0; k < rounds; ++k, q += 4096 * U) {
+      u32x4 v[U];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s = fma((double)v[j], (double)v[j], s);
+      for (int u = 0; u < U; ++u) v[u] = *(const u32x4*)(q + 4096 * u);
+      if (wide & 1) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const double x = __uint_as_float(v[u][j]);
+            s = fma(x, x, s);
+          }
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const double lo = bf16_lo(v[u][j]), hi = bf16_hi(v[u][j]);
+            s = fma(lo, lo, s);
+            s = fma(hi, hi, s);
+          }
       }
-    } else {
-      for (int64_t i = i0 + tid; i < i1; i += 256) s = fma((double)g[i], (double)g[i], s);
     }
   } else {
-    const bf16* g = (const bf16*)b.g[e];
-    if ((wide & 2) && i1 - i0 == AW_SUM) {
-#pragma unroll 8
-      for (int k = 0; k < AW_SUM / 2048; ++k) {
-        const u32x4 v = *(const u32x4*)(g + i0 + 2048 * k + 8 * tid);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const double lo = bf16_lo(v[j]), hi = bf16_hi(v[j]);
-          s = fma(lo, lo, s);
-          s = fma(hi, hi, s);
-        }
-      }
-    } else {
-      for (int64_t i = i0 + tid; i < i1; i += 256) {
-        const double x = (float)g[i];
-        s = fma(x, x, s);
-      }
+    for (int64_t i = i0 + tid; i < i1; i += 256) {
+      const double x = (wide & 1) ? ((const float*)b.g[e])[i] : (float)((const bf16*)b.g[e])[i];
+      s = fma(x, x, s);
     }
   }
 #pragma unroll
@@ -161,7 +162,7 @@ __global__ __launch_bounds__(1024) void aw_head_kernel(double* head, const doubl
 // ---- the step ----
 struct AwShared {
   float c, rate, rbc2, eps, decay, b1, b2, omb1, omb2;
-  double dc, db1, db2, domb1, domb2;
+  double db1, db2, dg1, dg2;  // decays, and (1 - b1) c, (1 - b2) c^2
 };
 
 __device__ __forceinline__ float aw_update(const AwShared& s, float p, float m, float v) {
@@ -242,49 +243,57 @@ __device__ __forceinline__ double aw_value_v(int c, double scale) {
   const double r = (double)(c + 1) * (1. / 256.);
   return r * r * scale;
 }
-// The code nearest to steps * sqrt(x / scale): from 32 bits, then held to its borders
-// (k +- 1/2)^2 scale in 64.
+// The code nearest to steps * sqrt(x / scale), found in 32 bits; within 2e-4 of a border
+// (its 32-bit place is off by at most 7e-5) held to the border (k +- 1/2)^2 scale in 64.
 __device__ __forceinline__ int aw_code(double x, float scale, float inv, float steps, int lo, int hi) {
-  int k = (int)rintf(steps * __builtin_sqrtf((float)x * inv));
-  k = min(max(k, lo), hi);
-  const double q = x * ((double)steps * (double)steps), sc = (double)scale;
-  const double up = (double)k + .5, dn = (double)k - .5;
-  if (k < hi && q > up * up * sc) ++k;
-  else if (k > lo && q < dn * dn * sc) --k;
+  const float at = steps * __builtin_amdgcn_sqrtf((float)x * inv);
+  const float near = rintf(at);
+  int k = min(max((int)near, lo), hi);
+  if (fabsf(at - near) > 0.4998f) {
+    const double q = x * ((double)steps * (double)steps), sc = (double)scale;
+    const double up = (double)k + .5, dn = (double)k - .5;
+    if (k < hi && q > up * up * sc) ++k;
+    else if (k > lo && q < dn * dn * sc) --k;
+  }
   return k;
 }
 
 // The larger of two magnitudes; one that is no number stays (the block's scale then says so).
 __device__ __forceinline__ float aw_max(float a, float b) { return b > a || b != b ? b : a; }
 
-// 8-bit moments: 16 lanes take a block of 256, 16 consecutive elements each.
+// 8-bit moments: 32 lanes take a block of 256, eight consecutive elements each; a workgroup's
+// chunk is two rounds of eight blocks.  VALU and memory are close here (45 operations, four of
+// them square roots or reciprocals, for 10 bytes of a bf16 element): the squares of the codes are
+// taken in integers and the decays folded into the scales, so that a moment costs one
+// conversion, one product and one fused multiply-add in 64 bits.
 template <bool P32, bool G32, bool MASTER>
-__device__ __forceinline__ void aw_chunk8(const AwTensor& t, const AwShared& s, int64_t i0, int tid) {
-  const int64_t i = i0 + 16 * tid;
+__device__ __forceinline__ void aw_block8(const AwTensor& t, const AwShared& s, int64_t i, int left) {
   const int64_t blk = i / AW_BLOCK;
-  if (i0 + (tid / 16) * AW_BLOCK >= t.n) return;  // whole groups of 16 lanes leave
-  const int left = (int)min((int64_t)16, t.n - i);  // elements of this lane (0 or less: none)
-  const bool vec = (t.flags & AW_ALIGNED) && left == 16;
+  const bool vec = (t.flags & AW_ALIGNED) && left == 8;
   int8_t* mc = (int8_t*)t.m;
   uint8_t* vc = (uint8_t*)t.v;
-  float g[16], p[16];
-  int cm[16], cv[16];
+  float g[8], p[8];
+  int cm[8], cv[8];
+  const float scm = t.ms[blk], scv = t.vs[blk];
   if (vec) {
-    const u32x4 a = *(const u32x4*)(mc + i), b = *(const u32x4*)(vc + i);
+    const u32x2 a = *(const u32x2*)(mc + i), b = *(const u32x2*)(vc + i);
+    const f32x4 x0 = load4(t.g, i, G32), x1 = load4(t.g, i + 4, G32);
+    const f32x4 y0 = MASTER ? *(const f32x4*)(t.master + i) : load4(t.p, i, P32);
+    const f32x4 y1 = MASTER ? *(const f32x4*)(t.master + i + 4) : load4(t.p, i + 4, P32);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const f32x4 x = load4(t.g, i + 4 * k, G32), y = MASTER ? *(const f32x4*)(t.master + i + 4 * k) : load4(t.p, i + 4 * k, P32);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        g[4 * k + e] = x[e];
-        p[4 * k + e] = y[e];
-        cm[4 * k + e] = (int)(int8_t)(a[k] >> (8 * e));
-        cv[4 * k + e] = (int)((b[k] >> (8 * e)) & 255u);
-      }
+    for (int e = 0; e < 4; ++e) {
+      g[e] = x0[e];
+      g[4 + e] = x1[e];
+      p[e] = y0[e];
+      p[4 + e] = y1[e];
+      cm[e] = (int)(int8_t)(a[0] >> (8 * e));
+      cm[4 + e] = (int)(int8_t)(a[1] >> (8 * e));
+      cv[e] = (int)((b[0] >> (8 * e)) & 255u);
+      cv[4 + e] = (int)((b[1] >> (8 * e)) & 255u);
     }
   } else {
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
+    for (int k = 0; k < 8; ++k) {
       const bool in = k < left;
       g[k] = in ? load1(t.g, i + k, G32) : 0.f;
       p[k] = in ? (MASTER ? t.master[i + k] : load1(t.p, i + k, P32)) : 0.f;
@@ -292,55 +301,60 @@ __device__ __forceinline__ void aw_chunk8(const AwTensor& t, const AwShared& s, 
       cv[k] = in ? vc[i + k] : 0;
     }
   }
-  const double sm = (double)t.ms[blk], sv = (double)t.vs[blk];
-  double m[16], v[16];
+  const double sm = s.db1 * ((double)scm * (1. / 16129.)), sv = s.db2 * ((double)scv * (1. / 65536.));
+  double m[8], v[8];
   float am = 0.f, av = 0.f;
 #pragma unroll
-  for (int k = 0; k < 16; ++k) {
-    const double gd = (double)g[k] * s.dc;
-    m[k] = fma(s.domb1, gd, s.db1 * aw_value_m(cm[k], sm));
-    v[k] = fma(s.domb2 * gd, gd, s.db2 * aw_value_v(cv[k], sv));
+  for (int k = 0; k < 8; ++k) {
+    const double gd = (double)g[k];
+    m[k] = fma(s.dg1, gd, sm * (double)(cm[k] * abs(cm[k])));
+    v[k] = fma(s.dg2 * gd, gd, sv * (double)((cv[k] + 1) * (cv[k] + 1)));
+    const float mf = (float)m[k], vf = (float)v[k];
     if (k < left) {  // rounding keeps the order: the largest rounded is the largest, rounded
-      am = aw_max(am, fabsf((float)m[k]));
-      av = aw_max(av, (float)v[k]);
+      am = aw_max(am, fabsf(mf));
+      av = aw_max(av, vf);
     }
-    p[k] = aw_update(s, p[k], (float)m[k], (float)v[k]);
+    p[k] = aw_update(s, p[k], mf, vf);
   }
 #pragma unroll
-  for (int d = 1; d < 16; d <<= 1) {
+  for (int d = 1; d < 32; d <<= 1) {
     am = aw_max(am, __shfl_xor(am, d));
     av = aw_max(av, __shfl_xor(av, d));
   }
   const float im = am > 0.f ? 1.f / am : 0.f, iv = av > 0.f ? 1.f / av : 0.f;
 #pragma unroll
-  for (int k = 0; k < 16; ++k) {
+  for (int k = 0; k < 8; ++k) {
     const int c = aw_code(fabs(m[k]), am, im, 127.f, 0, 127);
     cm[k] = m[k] < 0. ? -c : c;
     cv[k] = aw_code(v[k], av, iv, 256.f, 1, 256) - 1;
   }
-  if ((tid & 15) == 0) {
+  if ((threadIdx.x & 31) == 0) {
     t.ms[blk] = am;
     t.vs[blk] = av;
   }
   if (vec) {
-    u32x4 a, b;
+    u32x2 a = {0u, 0u}, b = {0u, 0u};
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      a[k] = b[k] = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        a[k] |= (uint32_t)(cm[4 * k + e] & 255) << (8 * e);
-        b[k] |= (uint32_t)cv[4 * k + e] << (8 * e);
-      }
-      const f32x4 y = {p[4 * k], p[4 * k + 1], p[4 * k + 2], p[4 * k + 3]};
-      if (MASTER) *(f32x4*)(t.master + i + 4 * k) = y;
-      store4(t.p, i + 4 * k, P32, y);
+    for (int e = 0; e < 8; ++e) {
+      a[e >> 2] |= (uint32_t)(cm[e] & 255) << (8 * (e & 3));
+      b[e >> 2] |= (uint32_t)cv[e] << (8 * (e & 3));
     }
-    *(u32x4*)(mc + i) = a;
-    *(u32x4*)(vc + i) = b;
+    const f32x4 y0 = {p[0], p[1], p[2], p[3]}, y1 = {p[4], p[5], p[6], p[7]};
+    if (MASTER) {
+      *(f32x4*)(t.master + i) = y0;
+      *(f32x4*)(t.master + i + 4) = y1;
+    }
+    if (P32) {
+      store4(t.p, i, true, y0);
+      store4(t.p, i + 4, true, y1);
+    } else {
+      *(u32x4*)((bf16*)t.p + i) = (u32x4){pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]), pack_bf16x2(p[4], p[5]), pack_bf16x2(p[6], p[7])};
+    }
+    *(u32x2*)(mc + i) = a;
+    *(u32x2*)(vc + i) = b;
   } else {
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
+    for (int k = 0; k < 8; ++k) {
       if (k >= left) continue;
       mc[i + k] = (int8_t)cm[k];
       vc[i + k] = (uint8_t)cv[k];
@@ -351,32 +365,43 @@ __device__ __forceinline__ void aw_chunk8(const AwTensor& t, const AwShared& s, 
   }
 }
 
+template <bool P32, bool G32, bool MASTER>
+__device__ __forceinline__ void aw_chunk8(const AwTensor& t, const AwShared& s, int64_t i0, int tid) {
+#pragma unroll 1
+  for (int k = 0; k < AW_CHUNK / 2048; ++k) {
+    const int64_t i = i0 + 2048 * k + 8 * tid;
+    if (i0 + 2048 * k + (tid / 32) * AW_BLOCK >= t.n) return;  // whole groups of 32 lanes leave
+    aw_block8<P32, G32, MASTER>(t, s, i, (int)min((int64_t)8, t.n - i));  // a lane past the end: no elements
+  }
+}
+
+template <bool Q8>
 __global__ __launch_bounds__(256) void aw_step_kernel(AwBatch b) {
   const uint32_t wg = blockIdx.x;
   if (b.head[3] != 0.) return;
   const int e = find_entry(b.count, wg, [&](int i) { return b.t[i].first; });
   const AwTensor t = b.t[e];
   AwShared s;
-  s.dc = b.head[0];
-  s.c = (float)s.dc;
+  const double c = b.head[0];
+  s.c = (float)c;
   s.rate = t.lr * (float)b.head[1];
   s.rbc2 = (float)b.head[2];
   s.eps = b.eps;
   s.decay = t.decay;
   s.db1 = b.b1;
   s.db2 = b.b2;
-  s.domb1 = 1. - b.b1;
-  s.domb2 = 1. - b.b2;
-  s.b1 = (float)s.db1;
-  s.b2 = (float)s.db2;
-  s.omb1 = (float)s.domb1;
-  s.omb2 = (float)s.domb2;
+  s.dg1 = (1. - b.b1) * c;
+  s.dg2 = (1. - b.b2) * (c * c);
+  s.b1 = (float)b.b1;
+  s.b2 = (float)b.b2;
+  s.omb1 = (float)(1. - b.b1);
+  s.omb2 = (float)(1. - b.b2);
   const int64_t i0 = (int64_t)(wg - t.first) * AW_CHUNK;
   const int tid = threadIdx.x;
-  const bool q8 = t.flags & AW_Q8, p32 = t.flags & AW_P32, g32 = t.flags & AW_G32;
+  const bool p32 = t.flags & AW_P32, g32 = t.flags & AW_G32;
   auto go = [&](auto P, auto G, auto M) {
     constexpr bool p_ = decltype(P)::value, g_ = decltype(G)::value, m_ = decltype(M)::value;
-    if (q8) aw_chunk8<p_, g_, m_>(t, s, i0, tid);
+    if (Q8) aw_chunk8<p_, g_, m_>(t, s, i0, tid);
     else aw_chunk32<p_, g_, m_>(t, s, i0, tid);
   };
   if (p32) {
@@ -510,37 +535,41 @@ static int aw_launch(const strata_hip_adamw_args* a, hipStream_t st) {
   b.b1 = a->beta1;
   b.b2 = a->beta2;
   b.head = a->workspace;
-  uint32_t wgs = 0;
-  auto flush = [&]() -> int {
-    if (!b.count) return STRATA_HIP_OK;
-    hipLaunchKernelGGL(aw_step_kernel, dim3(wgs), dim3(256), 0, st, b);
-    b.count = 0;
-    wgs = 0;
-    return check_launch("adamw step");
-  };
-  for (int64_t i = 0; i < a->count; ++i) {
-    const strata_hip_adamw_tensor& t = a->tensors[i];
-    if (t.n == 0) continue;
-    AwTensor& o = b.t[b.count++];
-    o.p = t.param;
-    o.g = t.grad;
-    o.m = t.exp_avg;
-    o.v = t.exp_avg_sq;
-    o.ms = t.exp_avg_scale;
-    o.vs = t.exp_avg_sq_scale;
-    o.master = t.master;
-    o.n = t.n;
-    o.lr = (float)t.lr;
-    o.decay = (float)(1. - t.lr * t.weight_decay);
-    o.first = wgs;
-    const uintptr_t all = (uintptr_t)t.param | (uintptr_t)t.grad | (uintptr_t)t.exp_avg | (uintptr_t)t.exp_avg_sq | (uintptr_t)t.master;
-    o.flags = (t.param_dtype == STRATA_HIP_F32 ? AW_P32 : 0) | (t.grad_dtype == STRATA_HIP_F32 ? AW_G32 : 0) |
-              (t.state_bits == 8 ? AW_Q8 : 0) | ((all & 15) ? 0 : AW_ALIGNED);
-    wgs += (uint32_t)((t.n + AW_CHUNK - 1) / AW_CHUNK);
-    if (b.count == AW_PER)
-      if (const int rc = flush()) return rc;
+  for (const bool q8 : {false, true}) {  // a launch takes tensors of one kind of moments
+    uint32_t wgs = 0;
+    auto flush = [&]() -> int {
+      if (!b.count) return STRATA_HIP_OK;
+      if (q8) hipLaunchKernelGGL(aw_step_kernel<true>, dim3(wgs), dim3(256), 0, st, b);
+      else hipLaunchKernelGGL(aw_step_kernel<false>, dim3(wgs), dim3(256), 0, st, b);
+      b.count = 0;
+      wgs = 0;
+      return check_launch("adamw step");
+    };
+    for (int64_t i = 0; i < a->count; ++i) {
+      const strata_hip_adamw_tensor& t = a->tensors[i];
+      if (t.n == 0 || (t.state_bits == 8) != q8) continue;
+      AwTensor& o = b.t[b.count++];
+      o.p = t.param;
+      o.g = t.grad;
+      o.m = t.exp_avg;
+      o.v = t.exp_avg_sq;
+      o.ms = t.exp_avg_scale;
+      o.vs = t.exp_avg_sq_scale;
+      o.master = t.master;
+      o.n = t.n;
+      o.lr = (float)t.lr;
+      o.decay = (float)(1. - t.lr * t.weight_decay);
+      o.first = wgs;
+      const uintptr_t all = (uintptr_t)t.param | (uintptr_t)t.grad | (uintptr_t)t.exp_avg | (uintptr_t)t.exp_avg_sq | (uintptr_t)t.master;
+      o.flags = (t.param_dtype == STRATA_HIP_F32 ? AW_P32 : 0) | (t.grad_dtype == STRATA_HIP_F32 ? AW_G32 : 0) |
+                ((all & 15) ? 0 : AW_ALIGNED);
+      wgs += (uint32_t)((t.n + AW_CHUNK - 1) / AW_CHUNK);
+      if (b.count == AW_PER)
+        if (const int rc = flush()) return rc;
+    }
+    if (const int rc = flush()) return rc;
   }
-  return flush();
+  return STRATA_HIP_OK;
 }
 
 }  // namespace strata

@@ -256,8 +256,7 @@ __global__ __launch_bounds__(256) void route_bwd_kernel(RouteParams p) {
 //   slot_row[s]  the row of pair s, -1 where its index names no expert
 //   offsets[e]   the first row of expert e; offsets[E] the number of rows
 //   tiles        [n, then n pairs (expert, first row)]: `tile` rows of one expert each
-// Pairs are taken PLAN_N at a time: counted per block, the blocks' counts summed by one
-// workgroup, and placed by block, wave and lane (the lanes of a wave that name the same
+// Pairs are taken PLAN_N at a time: counted per block, the blocks' counts summed, and placed by block, wave and lane (the lanes of a wave that name the same
 // expert find each other by one ballot per bit of the expert's number).
 // ---------------------------------------------------------------------------
 constexpr int PLAN_N = 1024, PLAN_WAVES = PLAN_N / 64, PLAN_MAX_E = 512;
@@ -291,9 +290,9 @@ __global__ __launch_bounds__(PLAN_N) void plan_count_kernel(PlanParams p) {
   for (int i = tid; i < p.experts; i += PLAN_N) p.counts[(int64_t)blockIdx.x * p.experts + i] = cnt[i];
 }
 
-// Offsets and tiles from every expert's number of rows (in LDS); total[e] becomes the
-// expert's first row.
-__device__ __forceinline__ void plan_offsets(const PlanParams& p, int* total, int tid) {
+// Every expert's first row, into total[e], from its number of rows there (both in LDS); `write`:
+// also the plan's offsets and tiles.
+__device__ __forceinline__ void plan_offsets(const PlanParams& p, int* total, int tid, bool write) {
   __shared__ int row0[PLAN_MAX_E + 1], tile0[PLAN_MAX_E + 1];
   if (tid < 64) {  // one wave scans, 8 experts a lane
     constexpr int PER = PLAN_MAX_E / 64;
@@ -328,52 +327,64 @@ __device__ __forceinline__ void plan_offsets(const PlanParams& p, int* total, in
     }
   }
   __syncthreads();
-  for (int e = tid; e < p.experts; e += PLAN_N) {
-    const int n = total[e];
-    p.offsets[e] = row0[e];
-    for (int k = 0; k * p.tile < n; ++k) {
-      p.tiles[1 + 2 * (tile0[e] + k)] = e;
-      p.tiles[2 + 2 * (tile0[e] + k)] = row0[e] + k * p.tile;
+  for (int e = tid; e < p.experts; e += PLAN_N) total[e] = row0[e];
+  if (write) {
+    for (int e = tid; e < p.experts; e += PLAN_N) p.offsets[e] = row0[e];
+    const int tiles = tile0[PLAN_MAX_E];
+    for (int i = tid; i < tiles; i += PLAN_N) {  // the last expert whose tiles start at or before i
+      int lo = 0, hi = p.experts - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (tile0[mid] <= i) lo = mid;
+        else hi = mid - 1;
+      }
+      p.tiles[1 + 2 * i] = lo;
+      p.tiles[2 + 2 * i] = row0[lo] + (i - tile0[lo]) * p.tile;
+    }
+    if (tid == 0) {
+      p.offsets[p.experts] = row0[PLAN_MAX_E];
+      p.tiles[0] = tiles;
     }
   }
-  if (tid == 0) {
-    p.offsets[p.experts] = row0[PLAN_MAX_E];
-    p.tiles[0] = tile0[PLAN_MAX_E];
+  __syncthreads();
+}
+
+// Sums over the blocks' counts of expert tid % w (w: experts rounded up to a power of two), by
+// PLAN_N / w threads an expert: all of them into total[e] (LDS), those before this thread's run
+// of blocks, or before block `mine`, returned.
+__device__ __forceinline__ int plan_sum(const PlanParams& p, int* total, int* part, int w, int b0, int b1, int mine) {
+  const int tid = threadIdx.x, seg = PLAN_N / w, e = tid % w, g = tid / w;
+  int s = 0, m = 0;
+  if (e < p.experts) {
+#pragma unroll 8
+    for (int b = b0; b < b1; ++b) {
+      const int v = p.counts[(int64_t)b * p.experts + e];
+      s += v;
+      m += b < mine ? v : 0;
+    }
   }
+  part[tid] = s;
+  part[PLAN_N + tid] = m;
   __syncthreads();
-  for (int e = tid; e < p.experts; e += PLAN_N) total[e] = row0[e];
+  int before = 0, all = 0, mm = 0;
+  for (int k = 0; k < seg; ++k) {
+    const int v = part[k * w + e];
+    before += k < g ? v : 0;
+    all += v;
+    mm += part[PLAN_N + k * w + e];
+  }
+  if (e < p.experts && g == 0) total[e] = all;
   __syncthreads();
+  return mine >= 0 ? mm : before;
 }
 
 // The blocks' counts become each block's first row of each expert.
 __global__ __launch_bounds__(PLAN_N) void plan_scan_kernel(PlanParams p) {
-  __shared__ int total[PLAN_MAX_E];
-  __shared__ int part[PLAN_N];
-  const int tid = threadIdx.x, E = p.experts;
-  // SEG threads share an expert, each a run of blocks
-  int w = 1;
-  while (w < E) w <<= 1;  // experts rounded up to a power of two, at most PLAN_MAX_E
-  const int seg = PLAN_N / w, e = tid % w, g = tid / w;
-  const int per = (p.blocks + seg - 1) / seg, b0 = min(g * per, p.blocks), b1 = min(b0 + per, p.blocks);
-  int s = 0;
-  if (e < E) {
-#pragma unroll 8
-    for (int b = b0; b < b1; ++b) s += p.counts[(int64_t)b * E + e];
-  }
-  part[tid] = s;
-  __syncthreads();
-  int before = 0;
-  if (e < E) {
-    int all = 0;
-    for (int k = 0; k < seg; ++k) {
-      const int v = part[k * w + e];
-      before += k < g ? v : 0;
-      all += v;
-    }
-    if (g == 0) total[e] = all;
-  }
-  __syncthreads();
-  plan_offsets(p, total, tid);
+  __shared__ int total[PLAN_MAX_E], part[2 * PLAN_N];
+  const int tid = threadIdx.x, E = p.experts, w = 1 << p.bits, e = tid % w, g = tid / w;
+  const int per = (p.blocks + PLAN_N / w - 1) / (PLAN_N / w), b0 = min(g * per, p.blocks), b1 = min(b0 + per, p.blocks);
+  const int before = plan_sum(p, total, part, w, b0, b1, -1);
+  plan_offsets(p, total, tid, true);
   if (e < E) {
     int at = total[e] + before;
     for (int b = b0; b < b1; ++b) {
@@ -385,10 +396,11 @@ __global__ __launch_bounds__(PLAN_N) void plan_scan_kernel(PlanParams p) {
   }
 }
 
-// ONE: the whole plan in one block.
-template <bool ONE>
+// ONE: the whole plan in one block.  SUMS: every block sums the counts of the blocks before it
+// itself (the first also writes offsets and tiles), in the place of a launch of plan_scan_kernel.
+template <bool ONE, bool SUMS>
 __global__ __launch_bounds__(PLAN_N) void plan_place_kernel(PlanParams p) {
-  extern __shared__ int cnt[];  // [PLAN_WAVES][E] counts, then first rows; ONE: + [E] totals
+  extern __shared__ int cnt[];  // [PLAN_WAVES][E] counts, then first rows; + [E] totals
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, E = p.experts;
   int* total = cnt + PLAN_WAVES * E;
   for (int i = tid; i < PLAN_WAVES * E; i += PLAN_N) cnt[i] = 0;
@@ -410,10 +422,18 @@ __global__ __launch_bounds__(PLAN_N) void plan_place_kernel(PlanParams p) {
       total[i] = n;
     }
     __syncthreads();
-    plan_offsets(p, total, tid);
+    plan_offsets(p, total, tid, true);
+  }
+  if (SUMS) {
+    __shared__ int part[2 * PLAN_N];
+    const int w = 1 << p.bits, g = tid / w, per = (p.blocks + PLAN_N / w - 1) / (PLAN_N / w);
+    const int b0 = min(g * per, p.blocks), before = plan_sum(p, total, part, w, b0, min(b0 + per, p.blocks), blockIdx.x);
+    plan_offsets(p, total, tid, blockIdx.x == 0);
+    if (g == 0 && tid < E) total[tid] += before;
+    __syncthreads();
   }
   for (int i = tid; i < E; i += PLAN_N) {
-    int at = ONE ? total[i] : p.counts[(int64_t)blockIdx.x * E + i];
+    int at = ONE || SUMS ? total[i] : p.counts[(int64_t)blockIdx.x * E + i];
     for (int w = 0; w < PLAN_WAVES; ++w) {
       const int n = cnt[w * E + i];
       cnt[w * E + i] = at;
@@ -550,12 +570,18 @@ extern "C" int strata_hip_expert_plan(const strata_hip_expert_plan_args* a, void
   hipStream_t st = (hipStream_t)stream;
   const size_t smem = (size_t)(PLAN_WAVES + 1) * a->experts * 4;
   if (p.blocks <= 1) {
-    hipLaunchKernelGGL(plan_place_kernel<true>, dim3(1), dim3(PLAN_N), smem, st, p);
+    hipLaunchKernelGGL((plan_place_kernel<true, false>), dim3(1), dim3(PLAN_N), smem, st, p);
     return check_launch("expert_plan");
   }
   if (!a->workspace) return fail(STRATA_HIP_EINVAL, "expert_plan: null workspace");
   hipLaunchKernelGGL(plan_count_kernel, dim3((unsigned)p.blocks), dim3(PLAN_N), 0, st, p);
-  hipLaunchKernelGGL(plan_scan_kernel, dim3(1), dim3(PLAN_N), 0, st, p);
-  hipLaunchKernelGGL(plan_place_kernel<false>, dim3((unsigned)p.blocks), dim3(PLAN_N), smem, st, p);
+  // Up to 32768 counts every block sums them itself; beyond, that reading (the counts times the
+  // blocks) costs more than the launch of one workgroup that sums them once.
+  if ((int64_t)p.blocks * p.experts <= 32768) {
+    hipLaunchKernelGGL((plan_place_kernel<false, true>), dim3((unsigned)p.blocks), dim3(PLAN_N), smem, st, p);
+  } else {
+    hipLaunchKernelGGL(plan_scan_kernel, dim3(1), dim3(PLAN_N), 0, st, p);
+    hipLaunchKernelGGL((plan_place_kernel<false, false>), dim3((unsigned)p.blocks), dim3(PLAN_N), smem, st, p);
+  }
   return check_launch("expert_plan");
 }

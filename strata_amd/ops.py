@@ -17,6 +17,7 @@ import ctypes
 import math
 from typing import Optional, Sequence
 
+import numpy as np
 import torch
 from torch import Tensor
 
@@ -1416,7 +1417,72 @@ def _route_args(name, logits, bias, top_k, score, groups, top_groups, renormaliz
     return a, (l2, b)
 
 
+def _eager(*ts: Optional[Tensor]) -> bool:
+    """Whether these are plain tensors outside a tracing compiler: the operators of this section then
+    launch through a ``torch.autograd.Function`` of their own.  The custom op's dispatch and its
+    registered autograd cost 25 us a forward and 55 us a backward of host time beside it, more
+    than the kernels of a small call; traced calls and tensor subclasses go through the custom op."""
+    return not torch.compiler.is_compiling() and all(t is None or type(t) is Tensor or type(t) is torch.nn.Parameter
+                                                     for t in ts)
+
+
+def _wants_grad(*ts: Optional[Tensor]) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+def _route_forward(logits, top_k, score, bias, groups, top_groups, renormalize, scale):
+    name = "expert_route"
+    a, keep = _route_args(name, logits, bias, top_k, score, groups, top_groups, renormalize, scale)
+    shape = (*logits.shape[:-1], int(top_k))
+    weights = torch.empty(shape, dtype=logits.dtype, device=logits.device)
+    index = torch.empty(shape, dtype=torch.int32, device=logits.device)
+    a.weights, a.index = weights.data_ptr(), index.data_ptr()
+    _launch("strata_hip_expert_route", a, logits)
+    return weights, index
+
+
+def _route_backward(dweights, logits, index, top_k, score, bias, renormalize, scale):
+    name = "expert_route_bwd"
+    a, keep = _route_args(name, logits, bias, top_k, score, 1, 1, renormalize, scale)
+    _require_gpu(name, logits, dweights, index)
+    shape = (*logits.shape[:-1], int(top_k))
+    if dweights.dtype != logits.dtype or tuple(dweights.shape) != shape or index.dtype != torch.int32 \
+            or tuple(index.shape) != shape:
+        raise ValueError(f"{name}: dweights must be {logits.dtype} and index int32, {shape}")
+    d, i = dweights.contiguous(), index.contiguous()
+    out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    a.dweights, a.index, a.dlogits = d.data_ptr(), i.data_ptr(), out.data_ptr()
+    _launch("strata_hip_expert_route_bwd", a, logits)
+    return out
+
+
+class _ExpertRoute(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, top_k, score, bias, groups, top_groups, renormalize, scale):
+        weights, index = _route_forward(logits, top_k, score, bias, groups, top_groups, renormalize, scale)
+        ctx.mark_non_differentiable(index)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(logits, bias, index)
+        ctx.args = top_k, score, renormalize, scale
+        return weights, index
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dweights, _dindex):
+        if dweights is None:
+            return (None,) * 8
+        logits, bias, index = ctx.saved_tensors
+        top_k, score, renormalize, scale = ctx.args
+        return _route_backward(dweights, logits, index, top_k, score, bias, renormalize, scale), *(None,) * 7
+
+
 @torch.library.custom_op("strata_hip::expert_route", mutates_args=())
+def _expert_route_op(logits: Tensor, top_k: int, score: str = "softmax", bias: Optional[Tensor] = None, groups: int = 1,
+                     top_groups: int = 1, renormalize: bool = True, scale: float = 1.0) -> tuple[Tensor, Tensor]:
+    """``expert_route`` as a custom op."""
+    return _route_forward(logits, top_k, score, bias, groups, top_groups, renormalize, scale)
+
+
 def expert_route(logits: Tensor, top_k: int, score: str = "softmax", bias: Optional[Tensor] = None, groups: int = 1,
                  top_groups: int = 1, renormalize: bool = True, scale: float = 1.0) -> tuple[Tensor, Tensor]:
     """``top_k`` experts for each token and their weights, ``(weights, index)`` ``[..., top_k]`` from
@@ -1431,17 +1497,14 @@ def expert_route(logits: Tensor, top_k: int, score: str = "softmax", bias: Optio
     A logit (or bias) that is not finite masks its expert; a token with too few experts left has
     index -1 and weight 0 in the slots that stay empty.  At most 512 experts and top_k 64.  The
     backward gives the logits' gradient (none flows to the bias)."""
-    name = "expert_route"
-    a, keep = _route_args(name, logits, bias, top_k, score, groups, top_groups, renormalize, scale)
-    shape = (*logits.shape[:-1], int(top_k))
-    weights = torch.empty(shape, dtype=logits.dtype, device=logits.device)
-    index = torch.empty(shape, dtype=torch.int32, device=logits.device)
-    a.weights, a.index = weights.data_ptr(), index.data_ptr()
-    _launch("strata_hip_expert_route", a, logits)
-    return weights, index
+    if not _eager(logits, bias):
+        return _expert_route_op(logits, top_k, score, bias, groups, top_groups, renormalize, scale)
+    if _wants_grad(logits):
+        return _ExpertRoute.apply(logits, top_k, score, bias, groups, top_groups, renormalize, scale)
+    return _route_forward(logits, top_k, score, bias, groups, top_groups, renormalize, scale)
 
 
-@expert_route.register_fake
+@_expert_route_op.register_fake
 def _(logits, top_k, score="softmax", bias=None, groups=1, top_groups=1, renormalize=True, scale=1.0):
     shape = (*logits.shape[:-1], top_k)
     return logits.new_empty(shape), logits.new_empty(shape, dtype=torch.int32)
@@ -1451,18 +1514,7 @@ def _(logits, top_k, score="softmax", bias=None, groups=1, top_groups=1, renorma
 def expert_route_bwd(dweights: Tensor, logits: Tensor, index: Tensor, top_k: int, score: str, bias: Optional[Tensor],
                      renormalize: bool, scale: float) -> Tensor:
     """The gradient at the logits of ``expert_route``, from its index and the weights' gradient."""
-    name = "expert_route_bwd"
-    a, keep = _route_args(name, logits, bias, top_k, score, 1, 1, renormalize, scale)
-    _require_gpu(name, logits, dweights, index)
-    shape = (*logits.shape[:-1], int(top_k))
-    if dweights.dtype != logits.dtype or tuple(dweights.shape) != shape or index.dtype != torch.int32 \
-            or tuple(index.shape) != shape:
-        raise ValueError(f"{name}: dweights must be {logits.dtype} and index int32, {shape}")
-    d, i = dweights.contiguous(), index.contiguous()
-    out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    a.dweights, a.index, a.dlogits = d.data_ptr(), i.data_ptr(), out.data_ptr()
-    _launch("strata_hip_expert_route_bwd", a, logits)
-    return out
+    return _route_backward(dweights, logits, index, top_k, score, bias, renormalize, scale)
 
 
 @expert_route_bwd.register_fake
@@ -1481,7 +1533,7 @@ def _route_setup_context(ctx, inputs, output):
     ctx.save_for_backward(logits, bias, index)
 
 
-def _route_backward(ctx, dweights, _dindex):
+def _route_op_backward(ctx, dweights, _dindex):
     if dweights is None:
         return (None,) * 8
     logits, bias, index = ctx.saved_tensors
@@ -1489,7 +1541,7 @@ def _route_backward(ctx, dweights, _dindex):
     return d, None, None, None, None, None, None, None
 
 
-expert_route.register_autograd(_route_backward, setup_context=_route_setup_context)
+_expert_route_op.register_autograd(_route_op_backward, setup_context=_route_setup_context)
 
 
 # ---------------------------------------------------------------------------
@@ -1536,9 +1588,9 @@ def _ptr(t: Optional[Tensor]) -> Optional[int]:
     return t.data_ptr() if t is not None else None
 
 
-def _expert_tile(pairs: int, w1: Tensor, w2: Tensor) -> int:
+def _expert_tile(pairs: int, w1: Tensor, w2: Tensor, train: bool) -> int:
     E, H, C = w1.shape
-    return int(_lib.function("strata_hip_expert_tile")(pairs, E, C, H, w2.shape[1]))
+    return int(_lib.function("strata_hip_expert_tile")(pairs, E, C, H, w2.shape[1], int(train)))
 
 
 def _plan_size(pairs: int, experts: int, tile: int) -> int:
@@ -1580,7 +1632,7 @@ def _expert_forward(name, x, weights, index, w1, b1, w2, b2, residual, save: boo
     h = torch.empty((n, H), dtype=torch.bfloat16, device=x.device)
     dact = torch.empty((n, H), dtype=torch.float16, device=x.device) if save else None
     y = torch.empty((n, N), dtype=torch.float32, device=x.device)
-    tile = _expert_tile(n, w1, w2)
+    tile = _expert_tile(n, w1, w2, save)
     plan = _expert_plan(index, weights, E, tile)
     a, keep = _expert_args(x, weights, plan, tile, w1, b1, w2, b2, h, dact, y)
     if residual is not None:
@@ -1618,23 +1670,19 @@ def _(x, weights, index, w1, b1, w2, b2, residual):
     n, E, H, N = index.numel(), w1.shape[0], w1.shape[1], w2.shape[1]
     return (x.new_empty((*x.shape[:-1], N)), x.new_empty((n, H)), x.new_empty((n, H), dtype=torch.float16),
             x.new_empty((n, N), dtype=torch.float32),
-            x.new_empty((_plan_size(n, E, _expert_tile(n, w1, w2)),), dtype=torch.int32))
+            x.new_empty((_plan_size(n, E, _expert_tile(n, w1, w2, True)),), dtype=torch.int32))
 
 
-@torch.library.custom_op("strata_hip::expert_mlp_bwd", mutates_args=())
-def expert_mlp_bwd(dout: Tensor, x: Tensor, weights: Tensor, w1: Tensor, b1: Optional[Tensor], w2: Tensor,
-                   b2: Optional[Tensor], h: Tensor, dact: Tensor, y: Tensor, plan: Tensor,
-                   need: Sequence[bool]) -> list[Tensor]:
-    """Gradients of ``expert_mlp_train`` at ``(x, weights, w1, b1, w2, b2)``, an empty tensor where
-    ``need`` asks for none (a bias's comes from its weight's launch)."""
+def _expert_backward(dout, x, weights, w1, b1, w2, b2, h, dact, y, plan, need):
+    """Gradients at ``(x, weights, w1, b1, w2, b2)``, None where ``need`` asks for none."""
     E, H, C = w1.shape
     N = w2.shape[1]
     n = h.shape[0]
-    tile = _expert_tile(n, w1, w2)
+    tile = _expert_tile(n, w1, w2, True)
     a, keep = _expert_args(x, weights, plan, tile, w1, b1, w2, b2, h, dact, y)
     new = lambda *shape: torch.empty(shape, dtype=torch.bfloat16, device=x.device)  # noqa: E731
     want_x, want_wt = need[0], need[1]
-    want_1, want_2 = need[2] or (need[3] and b1 is not None), need[4] or (need[5] and b2 is not None)
+    want_1, want_2 = need[2] or need[3], need[4] or need[5]
     hid = want_x or want_1
     dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_x else None
     dwt = torch.empty(weights.shape, dtype=weights.dtype, device=x.device) if want_wt else None
@@ -1645,7 +1693,17 @@ def expert_mlp_bwd(dout: Tensor, x: Tensor, weights: Tensor, w1: Tensor, b1: Opt
     dxs = torch.empty((n, C), dtype=torch.float32, device=x.device) if want_x else None
     b = _lib.ExpertMlpBwdArgs(a, g.data_ptr(), *(_ptr(t) for t in (dx, dwt, dw1, db1, dw2, db2, gz, dxs)))
     _launch("strata_hip_expert_mlp_bwd", b, x)
-    return [t if t is not None and wanted else new(0) for t, wanted in zip((dx, dwt, dw1, db1, dw2, db2), need)]
+    return [t if wanted else None for t, wanted in zip((dx, dwt, dw1, db1, dw2, db2), need)]
+
+
+@torch.library.custom_op("strata_hip::expert_mlp_bwd", mutates_args=())
+def expert_mlp_bwd(dout: Tensor, x: Tensor, weights: Tensor, w1: Tensor, b1: Optional[Tensor], w2: Tensor,
+                   b2: Optional[Tensor], h: Tensor, dact: Tensor, y: Tensor, plan: Tensor,
+                   need: Sequence[bool]) -> list[Tensor]:
+    """Gradients of ``expert_mlp_train`` at ``(x, weights, w1, b1, w2, b2)``, an empty tensor where
+    ``need`` asks for none (a bias's comes from its weight's launch)."""
+    grads = _expert_backward(dout, x, weights, w1, b1, w2, b2, h, dact, y, plan, need)
+    return [g if g is not None else x.new_empty(0) for g in grads]
 
 
 @expert_mlp_bwd.register_fake
@@ -1667,7 +1725,7 @@ def _expert_setup_context(ctx, inputs, output):
     ctx.save_for_backward(x, weights, w1, b1, w2, b2, h, dact, y, plan)
 
 
-def _expert_backward(ctx, dout, *_unused):
+def _expert_op_backward(ctx, dout, *_unused):
     if dout is None:
         return (None,) * 8
     x, weights, w1, b1, w2, b2, h, dact, y, plan = ctx.saved_tensors
@@ -1678,7 +1736,26 @@ def _expert_backward(ctx, dout, *_unused):
     return gx, gwt, None, g1, gb1, g2, gb2, dout if ctx.has_res and n[7] else None
 
 
-expert_mlp_train.register_autograd(_expert_backward, setup_context=_expert_setup_context)
+expert_mlp_train.register_autograd(_expert_op_backward, setup_context=_expert_setup_context)
+
+
+class _ExpertMlp(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weights, index, w1, b1, w2, b2, residual):
+        out, h, dact, y, plan = _expert_forward("expert_mlp", x, weights, index, w1, b1, w2, b2, residual, True)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x, weights, w1, b1, w2, b2, h, dact, y, plan)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        if dout is None:
+            return (None,) * 8
+        n = ctx.needs_input_grad
+        need = (n[0], n[1], n[3], n[4], n[5], n[6])
+        gx, gwt, g1, gb1, g2, gb2 = _expert_backward(dout, *ctx.saved_tensors, need) if any(need) else (None,) * 6
+        return gx, gwt, None, g1, gb1, g2, gb2, dout if n[7] else None
 
 
 def expert_mlp(x: Tensor, weights: Tensor, index: Tensor, w1: Tensor, b1: Optional[Tensor], w2: Tensor,
@@ -1693,10 +1770,14 @@ def expert_mlp(x: Tensor, weights: Tensor, index: Tensor, w1: Tensor, b1: Option
     2 GiB.  An index outside ``[0, E)`` adds nothing, and the same expert may stand in two slots.
     No token is dropped for an expert's load; a weight under 2^-100 counts as 0.  Differentiable once, in every argument but the
     index."""
-    ts = (x, weights, w1, b1, w2, b2, residual)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
-        return expert_mlp_train(x, weights, index, w1, b1, w2, b2, residual)[0]
-    return expert_mlp_fwd(x, weights, index, w1, b1, w2, b2, residual)
+    grad = _wants_grad(x, weights, w1, b1, w2, b2, residual)
+    if not _eager(x, weights, index, w1, b1, w2, b2, residual):
+        if grad:
+            return expert_mlp_train(x, weights, index, w1, b1, w2, b2, residual)[0]
+        return expert_mlp_fwd(x, weights, index, w1, b1, w2, b2, residual)
+    if grad:
+        return _ExpertMlp.apply(x, weights, index, w1, b1, w2, b2, residual)
+    return _expert_forward("expert_mlp", x, weights, index, w1, b1, w2, b2, residual, False)[0]
 
 
 # ---------------------------------------------------------------------------
@@ -1728,63 +1809,85 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
     (fp64 ``[1]``), and one that is not finite leaves everything as it was, ``step`` too."""
     name = "adamw_step"
     n = len(params)
-    lists = [params, grads, exp_avgs, exp_avg_sqs]
-    for opt in (masters, exp_avg_scales, exp_avg_sq_scales):
-        lists.append([None] * n if opt is None else opt)
-    if any(len(x) != n for x in lists):
+    cols = {"params": params, "grads": grads, "exp_avgs": exp_avgs, "exp_avg_sqs": exp_avg_sqs, "masters": masters,
+            "exp_avg_scales": exp_avg_scales, "exp_avg_sq_scales": exp_avg_sq_scales}
+    if any(x is not None and len(x) != n for x in cols.values()):
         raise ValueError(f"{name}: the lists must have one entry for each of the {n} parameters")
-    lrs = [float(lr)] * n if isinstance(lr, (int, float)) else [float(x) for x in lr]
-    wds = [float(weight_decay)] * n if isinstance(weight_decay, (int, float)) else [float(x) for x in weight_decay]
-    if len(lrs) != n or len(wds) != n:
+    rates = [(float(r),) * n if isinstance(r, (int, float)) else tuple(map(float, r)) for r in (lr, weight_decay)]
+    if any(len(r) != n for r in rates):
         raise ValueError(f"{name}: lr and weight_decay must be numbers or have one entry for each parameter")
-    _require_gpu(name, step, *[t for x in lists for t in x])
+    _require_gpu(name, step)
     if step.dtype != torch.int64 or step.numel() != 1:
         raise ValueError(f"{name}: step must be an int64 tensor [1]")
     if max_norm is not None and not (0 < max_norm < math.inf):
         raise ValueError(f"{name}: max_norm must be positive and finite")
-    table = (_lib.AdamwTensor * max(n, 1))()
-    written = [step]
-    for i, (p, g, m, v, w, ms, vs) in enumerate(zip(*lists)):
-        k = p.numel()
-        codes = m.dtype == torch.int8
-        for t, what, dtypes, size in ((p, "params", _ADAMW_FLOATS, k), (g, "grads", _ADAMW_FLOATS, k),
-                                      (m, "exp_avgs", (torch.int8,) if codes else _F32, k),
-                                      (v, "exp_avg_sqs", (torch.uint8,) if codes else _F32, k),
-                                      (w, "masters", _F32, k),
-                                      (ms, "exp_avg_scales", _F32, -(-k // STATE_BLOCK)),
-                                      (vs, "exp_avg_sq_scales", _F32, -(-k // STATE_BLOCK))):
-            if t is None:
-                continue
-            if t.dtype not in dtypes or t.numel() != size or not t.is_contiguous():
-                raise ValueError(f"{name}: {what}[{i}] must be contiguous, of {size} elements and one of {dtypes}, "
-                                 f"got {t.dtype} {tuple(t.shape)}")
-        if codes == (ms is None) or codes == (vs is None):
-            raise ValueError(f"{name}: 8-bit moments come with their scales, fp32 ones without (tensor {i})")
-        if w is not None and p.dtype != torch.bfloat16:
-            raise ValueError(f"{name}: masters[{i}] belongs to a bfloat16 parameter")
-        table[i] = (p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), ms.data_ptr() if codes else None,
-                    vs.data_ptr() if codes else None, w.data_ptr() if w is not None else None, k, lrs[i], wds[i],
-                    _lib.F32 if p.dtype == torch.float32 else _lib.BF16,
-                    _lib.F32 if g.dtype == torch.float32 else _lib.BF16, 8 if codes else 32, 0)
-        written += [t for t in (p, m, v, w, ms, vs) if t is not None]
-    ws = torch.empty(int(_lib.function("strata_hip_adamw_workspace")(table, n)), dtype=torch.float64, device=step.device)
+    # Column by column: a step over many small tensors is bound by this host path (one call of each
+    # kind a tensor and column; a loop over tensors that checked each took 3.5 us a tensor).
+    dev, sizes = step.get_device(), [p.numel() for p in params]
+    blocks = [-(-k // STATE_BLOCK) for k in sizes]
+    table = np.zeros(max(n, 1), dtype=_ADAMW_TABLE)
+    dtypes, written = {}, [step]
+    for what, ts in cols.items():
+        if ts is None:
+            continue
+        some = ts if what in _ADAMW_ALWAYS else [t for t in ts if t is not None]
+        want = blocks if what.endswith("scales") else sizes
+        if some is not ts and len(some) != n:
+            want = [k for k, t in zip(want, ts) if t is not None]
+        dtypes[what] = [t.dtype for t in ts] if what in _ADAMW_ALWAYS else None
+        if any(t.get_device() != dev for t in some):
+            raise ValueError(f"{name}: every tensor must be on step's GPU (cuda:{dev}), {what} are not")
+        if not set(t.dtype for t in some) <= _ADAMW_DTYPES[what] or [t.numel() for t in some] != want \
+                or not all(t.is_contiguous() for t in some):
+            raise ValueError(f"{name}: {what} must be contiguous, of {'a scale for every 256 elements of ' if want is blocks else ''}"
+                             f"their parameter's size and of {sorted(map(str, _ADAMW_DTYPES[what]))}")
+        table[_ADAMW_FIELD[what]][:n] = [t.data_ptr() if t is not None else 0 for t in ts]
+        if what != "grads":
+            written += some
+    codes = [d == torch.int8 for d in dtypes.get("exp_avgs", ())]
+    if codes != [d == torch.uint8 for d in dtypes.get("exp_avg_sqs", ())]:
+        raise ValueError(f"{name}: exp_avgs and exp_avg_sqs must both be fp32, or int8 and uint8")
+    for what in ("exp_avg_scales", "exp_avg_sq_scales"):
+        ts = cols[what]
+        if (any(codes) if ts is None else codes != [t is not None for t in ts]):
+            raise ValueError(f"{name}: 8-bit moments come with their scales, fp32 ones without")
+    if n:
+        table["n"][:n], table["lr"][:n], table["weight_decay"][:n] = sizes, rates[0], rates[1]
+        table["param_dtype"][:n] = [d == torch.bfloat16 for d in dtypes["params"]]  # _lib.F32, _lib.BF16
+        table["grad_dtype"][:n] = [d == torch.bfloat16 for d in dtypes["grads"]]
+        table["state_bits"][:n] = [8 if c else 32 for c in codes]
+        if masters is not None and any(w is not None and d != torch.bfloat16 for w, d in zip(masters, dtypes["params"])):
+            raise ValueError(f"{name}: masters belong to bfloat16 parameters")
+    tp = ctypes.cast(table.ctypes.data, ctypes.POINTER(_lib.AdamwTensor))
+    ws = torch.empty(int(_lib.function("strata_hip_adamw_workspace")(tp, n)), dtype=torch.float64, device=step.device)
     norm = torch.empty(1, dtype=torch.float64, device=step.device) if max_norm is not None else None
-    a = _lib.AdamwArgs(table, n, step.data_ptr(), norm.data_ptr() if norm is not None else None, ws.data_ptr(),
+    a = _lib.AdamwArgs(tp, n, step.data_ptr(), norm.data_ptr() if norm is not None else None, ws.data_ptr(),
                        float(betas[0]), float(betas[1]), float(eps), float(max_norm or 0.0))
     _launch("strata_hip_adamw_step", a, step)
-    torch.autograd.graph.increment_version([t for t in written if not t.is_inference()])
+    if any(t.is_inference() for t in written):
+        written = [t for t in written if not t.is_inference()]
+    torch.autograd.graph.increment_version(written)
     return norm
 
 
-_ADAMW_FLOATS = (torch.bfloat16, torch.float32)
-_F32 = (torch.float32,)
+_ADAMW_ALWAYS = ("params", "grads", "exp_avgs", "exp_avg_sqs")
+_ADAMW_FIELD = {"params": "param", "grads": "grad", "exp_avgs": "exp_avg", "exp_avg_sqs": "exp_avg_sq", "masters": "master",
+                "exp_avg_scales": "exp_avg_scale", "exp_avg_sq_scales": "exp_avg_sq_scale"}
+_ADAMW_DTYPES = {"params": {torch.bfloat16, torch.float32}, "grads": {torch.bfloat16, torch.float32},
+                 "exp_avgs": {torch.float32, torch.int8}, "exp_avg_sqs": {torch.float32, torch.uint8},
+                 "masters": {torch.float32}, "exp_avg_scales": {torch.float32}, "exp_avg_sq_scales": {torch.float32}}
+_ADAMW_TABLE = np.dtype([(f, np.float64 if c is ctypes.c_double else np.int32 if c is ctypes.c_int32 else np.int64)
+                         for f, c in _lib.AdamwTensor._fields_])
 
 
-@torch.library.custom_op("strata_hip::adamw_state_values", mutates_args=())
 def adamw_state_values(codes: Tensor, scales: Tensor) -> Tensor:
     """The fp32 moments that ``adamw_step``'s 8-bit states stand for: ``scale * sign(c) (c / 127)^2``
     for int8 codes (exp_avg), ``scale * ((c + 1) / 256)^2`` for uint8 codes (exp_avg_sq), one scale
     for every 256 consecutive elements."""
+    return _state_values(codes, scales) if _eager(codes, scales) else _state_values_op(codes, scales)
+
+
+def _state_values(codes: Tensor, scales: Tensor) -> Tensor:
     name = "adamw_state_values"
     _require_gpu(name, codes, scales)
     if codes.dtype not in (torch.int8, torch.uint8) or scales.dtype != torch.float32:
@@ -1802,9 +1905,15 @@ def adamw_state_values(codes: Tensor, scales: Tensor) -> Tensor:
     return out
 
 
-@adamw_state_values.register_fake
+@torch.library.custom_op("strata_hip::adamw_state_values", mutates_args=())
+def _state_values_op(codes: Tensor, scales: Tensor) -> Tensor:
+    """``adamw_state_values`` as a custom op."""
+    return _state_values(codes, scales)
+
+
+@_state_values_op.register_fake
 def _(codes, scales):
     return torch.empty(codes.shape, dtype=torch.float32, device=codes.device)
 
 
-adamw_state_values.register_autograd(_no_backward("strata_hip::adamw_state_values"))
+_state_values_op.register_autograd(_no_backward("strata_hip::adamw_state_values"))

@@ -126,7 +126,7 @@ def _mlp_args(lib, **over):
     for k, v in over.items():
         setattr(a, k, v)
     if a.tile == 0:
-        a.tile = lib.strata_hip_expert_tile(a.tokens * a.top_k, a.experts, a.dim, a.hidden, a.out_dim)
+        a.tile = lib.strata_hip_expert_tile(a.tokens * a.top_k, a.experts, a.dim, a.hidden, a.out_dim, a.dact is not None)
     return a
 
 

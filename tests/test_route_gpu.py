@@ -158,9 +158,9 @@ def test_route_repeats_and_replays(gpu):
         assert all(torch.equal(x, y) and torch.equal(x, z) for x, y, z in zip(want, got, again))
 
 
-@pytest.mark.parametrize("tile", [64, 128, 256])
+@pytest.mark.parametrize("tile", [16, 64, 256])
 @pytest.mark.parametrize("n,E", [(0, 3), (1, 1), (2, 8), (63, 5), (64, 64), (65, 2), (1000, 100), (1024, 512), (1025, 8),
-                                 (5000, 1), (4097, 300), (70000, 24), (40000, 512)])
+                                 (5000, 1), (4097, 300), (70000, 24), (40000, 512), (70000, 512)])
 def test_plan(gpu, n, E, tile):
     """Rows sorted by expert, stable; offsets and tiles; indices that name no expert left out."""
     print(f"plan {n} {E} {tile}", flush=True)
