@@ -165,7 +165,15 @@ struct AwShared {
   double db1, db2, dg1, dg2;  // decays, and (1 - b1) c, (1 - b2) c^2
 };
 
+// FAST: within 2 u instead of 1/2 u in the root and in the quotient (v_sqrt_f32 and v_rcp_f32,
+// a root of less than 2^-96 taken of 2^32 times it), where the step is bound by its operations.
+template <bool FAST>
 __device__ __forceinline__ float aw_update(const AwShared& s, float p, float m, float v) {
+  if (FAST) {
+    const bool small = v < 0x1p-96f;
+    const float root = __builtin_amdgcn_sqrtf(small ? v * 0x1p32f : v) * (small ? 0x1p-16f : 1.f);
+    return fmaf(p, s.decay, -(s.rate * m) * __builtin_amdgcn_rcpf(fmaf(root, s.rbc2, s.eps)));
+  }
   const float denom = fmaf(__builtin_sqrtf(v), s.rbc2, s.eps);
   return fmaf(p, s.decay, -(s.rate * m) / denom);
 }
@@ -194,7 +202,7 @@ __device__ __forceinline__ void aw_chunk32(const AwTensor& t, const AwShared& s,
     g *= s.c;
     mm = fmaf(s.omb1, g, s.b1 * mm);
     vv = fmaf(s.omb2 * g, g, s.b2 * vv);
-    return aw_update(s, pp, mm, vv);
+    return aw_update<false>(s, pp, mm, vv);
   };
   if ((t.flags & AW_ALIGNED) && i0 + AW_CHUNK <= t.n) {
     f32x4 g[4], mm[4], vv[4], pp[4];
@@ -314,7 +322,7 @@ __device__ __forceinline__ void aw_block8(const AwTensor& t, const AwShared& s, 
       am = aw_max(am, fabsf(mf));
       av = aw_max(av, vf);
     }
-    p[k] = aw_update(s, p[k], mf, vf);
+    p[k] = aw_update<true>(s, p[k], mf, vf);
   }
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {

@@ -7,13 +7,15 @@
 //   index = the top_k largest keys left, the lower expert of two equal ones, -1 where none is left
 //   w = scale * s[index] (/ sum of the chosen s)
 //
-// A logit or bias that is not finite masks its expert.  Two keys s + bias of one token lie
-// closer together than 32-bit scores resolve in about one token of 1e5, so scores that
-// decide are held in 64 bits (v_fma_f64 issues at the rate of v_fma_f32 here).
+// A logit or bias that is not finite masks its expert.
 //
 // L lanes take a token, EPL consecutive experts each: the best key of a lane is found in
 // its registers, the token's by log2(L) exchanges, so a round of the choice costs a wave
-// EPL + 3 log2(L) operations for 64 / L tokens.
+// 3 EPL + 6 log2(L) operations for 64 / L tokens.  Bound by those operations: at [65536, 64]
+// fp32, 8 of 64 in 8 groups, the rows are read in a third of the time.
+//
+// Keys s + bias are first compared in 32 bits.  Where two that are compared lie closer together
+// than those are off by (a token in some hundred), the wave chooses again in 64 bits.
 #include "common.h"
 
 namespace strata {
@@ -42,170 +44,288 @@ __device__ __forceinline__ void route_store(void* p, int64_t i, float v) {
 }
 __device__ __forceinline__ bool is_finite(float x) { return fabsf(x) < __builtin_inff(); }
 
+// EPL consecutive elements from i on; VEC: as 16-byte (or one shorter) runs.
+template <typename T, int EPL, bool VEC>
+__device__ __forceinline__ void route_row(const void* p, int64_t i, int left, float other, float (&v)[EPL]) {
+  if constexpr (VEC && EPL >= 4) {
+    if (left >= EPL) {
+      if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int k = 0; k < EPL / 4; ++k) {
+          const f32x4 x = *(const f32x4*)((const float*)p + i + 4 * k);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[4 * k + e] = x[e];
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < EPL / 4; ++k) {
+          const u32x2 x = *(const u32x2*)((const bf16*)p + i + 4 * k);
+          v[4 * k] = bf16_lo(x[0]);
+          v[4 * k + 1] = bf16_hi(x[0]);
+          v[4 * k + 2] = bf16_lo(x[1]);
+          v[4 * k + 3] = bf16_hi(x[1]);
+        }
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < EPL; ++k) v[k] = k < left ? route_load<T>(p, i + k) : other;
+}
+
+// The value of the lane d away in a butterfly over lanes that agree in groups of d: moves
+// inside a row of 16 lanes, an exchange through LDS beyond.
+template <int D>
+__device__ __forceinline__ uint32_t swap_word(uint32_t v) {
+  if constexpr (D == 1) return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, true);        // quad 1 0 3 2
+  else if constexpr (D == 2) return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, true);   // quad 2 3 0 1
+  else if constexpr (D == 4) return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, true);  // half row mirrored
+  else if constexpr (D == 8) return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xf, 0xf, true);  // row mirrored
+  else return (uint32_t)__shfl_xor((int)v, D);
+}
+template <int D>
+__device__ __forceinline__ float swap_lane(float v) { return __uint_as_float(swap_word<D>(__float_as_uint(v))); }
+template <int D>
+__device__ __forceinline__ int swap_lane(int v) { return (int)swap_word<D>((uint32_t)v); }
+template <int D>
+__device__ __forceinline__ double swap_lane(double v) {
+  const u32x2 w = __builtin_bit_cast(u32x2, v);
+  return __builtin_bit_cast(double, (u32x2){swap_word<D>(w[0]), swap_word<D>(w[1])});
+}
+// f(integral_constant<int, d>) for d = 1, 2, 4 .. L / 2
+template <int L, typename F>
+__device__ __forceinline__ void butterfly(F f) {
+  if constexpr (L > 1) f(std::integral_constant<int, 1>{});
+  if constexpr (L > 2) f(std::integral_constant<int, 2>{});
+  if constexpr (L > 4) f(std::integral_constant<int, 4>{});
+  if constexpr (L > 8) f(std::integral_constant<int, 8>{});
+  if constexpr (L > 16) f(std::integral_constant<int, 16>{});
+  if constexpr (L > 32) f(std::integral_constant<int, 32>{});
+}
 template <int L, typename V>
 __device__ __forceinline__ V group_max(V v) {
-#pragma unroll
-  for (int d = 1; d < L; d <<= 1) {
-    const V o = __shfl_xor(v, d);
+  butterfly<L>([&](auto d) {
+    const V o = swap_lane<decltype(d)::value>(v);
     v = o > v ? o : v;
-  }
+  });
   return v;
 }
 template <int L, typename V>
 __device__ __forceinline__ V group_sum(V v) {
-#pragma unroll
-  for (int d = 1; d < L; d <<= 1) v += __shfl_xor(v, d);
+  butterfly<L>([&](auto d) { v += swap_lane<decltype(d)::value>(v); });
   return v;
+}
+// LDS written by lanes of a wave is read by others of the same wave.
+__device__ __forceinline__ void wave_sync() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_wave_barrier();
 }
 
 __device__ __forceinline__ float exp_of(float x) { return expf(x); }
 __device__ __forceinline__ double exp_of(double x) { return exp(x); }
 
-// KEY: the type that scores and keys are held in, double where they decide.
-template <typename T, typename KEY, int EPL, int L>
-__global__ __launch_bounds__(256) void route_kernel(RouteParams p) {
-  constexpr int TOK = 256 / L;
+// The choice of one token by its L lanes, into sel (scores) and chosen (experts) in LDS.  l: this
+// lane's logits, -inf where masked.  WIDE: keys are scores + bias, else the logits.  Returns
+// whether two keys (or groups) that were compared lie too close together for KEY's scores.
+template <typename KEY, bool WIDE, int EPL, int L>
+__device__ __forceinline__ bool route_choose(const RouteParams& p, const float (&l)[EPL], const float (&bias)[EPL], int lane,
+                                             char* scratch, float* sel, int* chosen) {
   constexpr KEY NONE = -__builtin_inf();
-  extern __shared__ char smem[];  // [TOK][top_k] scores; with groups [TOK][EPL * L] keys and [TOK][groups] sums before them
-  const int tid = threadIdx.x, lane = tid % L, tok = tid / L;
-  const int64_t t = (int64_t)blockIdx.x * TOK + tok;
-  const bool live = t < p.tokens;  // the other lanes of a wave wait for nobody: they follow with masked keys
-  const int E = p.experts, e0 = lane * EPL;
-  KEY key[EPL];
-  KEY sc[EPL];
-  KEY top = NONE;
-#pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    const bool in = live && e0 + i < E;
-    float l = in ? route_load<T>(p.logits, t * p.ld + e0 + i) : __builtin_inff();
-    if (in && p.bias && !is_finite(p.bias[e0 + i])) l = __builtin_inff();
-    key[i] = is_finite(l) ? (KEY)l : NONE;
-    top = key[i] > top ? key[i] : top;
-  }
+  constexpr bool CHECK = WIDE && sizeof(KEY) == 4;
+  const int e0 = lane * EPL;
+  KEY key[EPL], sc[EPL];
   if (p.score == STRATA_HIP_SCORE_SOFTMAX) {
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) top = fmaxf(top, l[i]);
     top = group_max<L>(top);
     KEY sum = 0;
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
-      sc[i] = key[i] > NONE ? exp_of(key[i] - top) : (KEY)0;
+      sc[i] = l[i] > -__builtin_inff() ? exp_of((KEY)l[i] - (KEY)top) : (KEY)0;
       sum += sc[i];
     }
     sum = group_sum<L>(sum);
-    const KEY r = sum > 0 ? (KEY)1 / sum : (KEY)0;
+    if (sizeof(KEY) == 8) {
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) sc[i] = sizeof(KEY) == 8 ? (sum > 0 ? sc[i] / sum : (KEY)0) : sc[i] * r;
+      for (int i = 0; i < EPL; ++i) sc[i] = sum > 0 ? sc[i] / sum : (KEY)0;
+    } else {
+      const KEY r = sum > 0 ? (KEY)1 / sum : (KEY)0;
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) sc[i] *= r;
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) sc[i] = key[i] > NONE ? (KEY)1 / ((KEY)1 + exp_of(-key[i])) : (KEY)0;
+    for (int i = 0; i < EPL; ++i) sc[i] = l[i] > -__builtin_inff() ? (KEY)1 / ((KEY)1 + exp_of(-(KEY)l[i])) : (KEY)0;
   }
-  if (p.bias || p.groups > 1) {
 #pragma unroll
-    for (int i = 0; i < EPL; ++i)
-      if (key[i] > NONE) key[i] = sc[i] + (p.bias ? (KEY)p.bias[e0 + i] : (KEY)0);
-  }
-  float* sel = (float*)smem + tok * p.top_k;
-  if (p.groups > 1) {
-    KEY* keys = (KEY*)(smem + ((TOK * p.top_k * 4 + 15) & ~15)) + tok * (EPL * L);
-    KEY* rank = (KEY*)(smem + ((TOK * p.top_k * 4 + 15) & ~15)) + TOK * (EPL * L) + tok * p.groups;
-    const int per = E / p.groups;
+  for (int i = 0; i < EPL; ++i) key[i] = l[i] > -__builtin_inff() ? (WIDE ? sc[i] + (KEY)bias[i] : (KEY)l[i]) : NONE;
+  bool close = false;
+  // What two 32-bit keys have to be apart, in units of 1 + |key|.  With u = 6e-8 an exponential is within 2 u,
+  // a sigmoid within 3.5 u, a softmax score within 16 u (its sum has 14 roundings) and a sum with the
+  // bias u further: 2 x 4.5 u and 2 x 17 u, with a margin of 2.  Groups' sums of two keys: twice that.
+  const float apart = p.score == STRATA_HIP_SCORE_SOFTMAX ? 4e-6f : 1e-6f;
+  auto near = [&](KEY a, KEY b) { return CHECK && fabsf((float)(a - b)) <= apart * (1.f + fabsf((float)a)); };
+  if (WIDE && p.groups > 1) {
+    KEY* keys = (KEY*)scratch;
+    KEY* rank = keys + EPL * L;
+    int* stays = (int*)(rank + p.groups);
+    const int per = p.experts / p.groups;
 #pragma unroll
     for (int i = 0; i < EPL; ++i) keys[e0 + i] = key[i];
-    __syncthreads();
+    wave_sync();
     for (int g = lane; g < p.groups; g += L) {
       KEY a = NONE, b = NONE;
       for (int i = 0; i < per; ++i) {
         const KEY k = keys[g * per + i];
-        if (k > a) {
-          b = a;
-          a = k;
-        } else if (k > b) {
-          b = k;
-        }
+        b = k > b ? (k > a ? a : k) : b;
+        a = k > a ? k : a;
       }
       rank[g] = b > NONE ? a + b : a;
     }
-    __syncthreads();
-    // a group stays if fewer than top_groups come before it
+    wave_sync();
+    for (int g = lane; g < p.groups; g += L) {  // a group stays if fewer than top_groups come before it
+      const KEY mine = rank[g];
+      int before = 0, sure = 0, may = 0;
+      const float room = 2.f * apart * (1.f + fabsf((float)mine));
+      for (int j = 0; j < p.groups; ++j) {
+        const KEY o = rank[j];
+        before += o > mine || (o == mine && j < g);
+        if (CHECK && j != g) {
+          sure += o > mine + room;
+          may += o >= mine - room;
+        }
+      }
+      stays[g] = before < p.top_groups;
+      if (CHECK && mine > NONE) close |= (sure < p.top_groups) != (may < p.top_groups);
+    }
+    wave_sync();
+    int g = e0 / per, in = e0 - g * per;
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
-      if (!(key[i] > NONE)) continue;
-      const int g = (e0 + i) / per;
-      const KEY mine = rank[g];
-      int before = 0;
-      for (int j = 0; j < p.groups; ++j) before += rank[j] > mine || (rank[j] == mine && j < g);
-      if (before >= p.top_groups) key[i] = NONE;
+      if (e0 + i < p.experts && !stays[g]) key[i] = NONE;
+      if (++in == per) {
+        in = 0;
+        ++g;
+      }
     }
   }
-  // the choice, one slot a round
-  float total = 0.f;
-  for (int s = 0; s < p.top_k; ++s) {
+  KEY last = NONE;
+  const int rounds = p.top_k + (CHECK && p.top_k < p.experts ? 1 : 0);  // the first one left out is compared too
+  for (int s = 0; s < rounds; ++s) {
     KEY best = NONE;
-    float bs = 0.f;
+    KEY bs = 0;
     int at = 0x7fffffff;
 #pragma unroll
     for (int i = 0; i < EPL; ++i)
       if (key[i] > best) {
         best = key[i];
-        bs = (float)sc[i];
+        bs = sc[i];
         at = e0 + i;
       }
-#pragma unroll
-    for (int d = 1; d < L; d <<= 1) {
-      const KEY o = __shfl_xor(best, d);
-      const float os = __shfl_xor(bs, d);
-      const int oa = __shfl_xor(at, d);
+    const int own = at;
+    butterfly<L>([&](auto d) {
+      const KEY o = swap_lane<decltype(d)::value>(best);
+      const int oa = swap_lane<decltype(d)::value>(at);
       if (o > best || (o == best && oa < at)) {
         best = o;
-        bs = os;
         at = oa;
       }
-    }
+    });
     const bool some = best > NONE;
+    if (CHECK && s > 0 && some) close |= near(last, best);
+    last = best;
+    if (s == p.top_k) break;
+    if (some ? own == at : lane == 0) {  // the chosen expert's lane
+      sel[s] = some ? (float)bs : 0.f;
+      chosen[s] = some ? at : -1;
+    }
 #pragma unroll
     for (int i = 0; i < EPL; ++i)
       if (e0 + i == at) key[i] = NONE;
-    total += bs;
-    if (lane == 0) {
-      sel[s] = some ? bs : 0.f;
-      if (live) p.index[t * p.top_k + s] = some ? at : -1;
+  }
+  return close;
+}
+
+template <typename T, bool WIDE, bool VEC, int EPL, int L>
+__global__ __launch_bounds__(256) void route_kernel(RouteParams p) {
+  constexpr int TOK = 256 / L;
+  extern __shared__ char smem[];  // a token: [top_k] scores, [top_k] experts; with groups the choice's scratch
+  const int tid = threadIdx.x, lane = tid % L, tok = tid / L;
+  const int64_t t = (int64_t)blockIdx.x * TOK + tok;
+  const bool live = t < p.tokens;  // the other lanes of a wave follow with masked logits
+  const int E = p.experts, e0 = lane * EPL, left = live ? max(E - e0, 0) : 0;
+  float l[EPL], bias[EPL];
+  route_row<T, EPL, VEC>(p.logits, t * p.ld + e0, left, __builtin_inff(), l);
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) bias[i] = 0.f;
+  if (WIDE && p.bias) route_row<float, EPL, VEC>(p.bias, e0, left, 0.f, bias);
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) l[i] = is_finite(l[i]) && is_finite(bias[i]) ? l[i] : -__builtin_inff();
+  float* sel = (float*)smem + tok * 2 * p.top_k;
+  int* chosen = (int*)sel + p.top_k;
+  const size_t fixed = ((size_t)TOK * p.top_k * 8 + 15) & ~(size_t)15;
+  char* scratch = smem + fixed + (size_t)tok * (EPL * L + 2 * p.groups) * 8;
+  const bool close = route_choose<float, WIDE, EPL, L>(p, l, bias, lane, scratch, sel, chosen);
+  if constexpr (WIDE) {
+    if (__any(close)) {
+      wave_sync();
+      route_choose<double, WIDE, EPL, L>(p, l, bias, lane, scratch, sel, chosen);
     }
   }
-  __syncthreads();
+  wave_sync();
   if (!live) return;
+  float total = 0.f;
+  for (int s = 0; s < p.top_k; ++s) total += sel[s];
   const float f = p.renormalize ? p.scale / (total > 0.f ? total : 1.f) : p.scale;
-  for (int s = lane; s < p.top_k; s += L) route_store<T>(p.weights, t * p.top_k + s, sel[s] * f);
+  for (int s = lane; s < p.top_k; s += L) {
+    route_store<T>(p.weights, t * p.top_k + s, sel[s] * f);
+    p.index[t * p.top_k + s] = chosen[s];
+  }
 }
 
 // The gradient at the logits.  With c the scale, S the sum of the chosen scores and a the
 // sum of dw s over them:  ds = c dw, or c / S (dw - a / S) renormalised;
 // softmax: dl = s (ds - sum of s ds), the sum zero when renormalised; sigmoid: dl = ds s (1 - s).
-template <typename T, int EPL, int L>
+// The chosen slots' dw reach their experts' lanes through a row of LDS.
+template <typename T, bool VEC, int EPL, int L>
 __global__ __launch_bounds__(256) void route_bwd_kernel(RouteParams p) {
   constexpr int TOK = 256 / L;
+  constexpr uint32_t FREE = 0x7fc0beefu;  // not chosen: no product makes these bits
+  extern __shared__ char smem[];           // [TOK][EPL * L] dw by expert
   const int tid = threadIdx.x, lane = tid % L, tok = tid / L;
   const int64_t t = (int64_t)blockIdx.x * TOK + tok;
   const bool live = t < p.tokens;
-  const int E = p.experts, e0 = lane * EPL;
-  float l[EPL], sc[EPL], om[EPL], dw[EPL];  // om: 1 - s of the sigmoid
-  bool chosen[EPL];
-  float top = -__builtin_inff();
+  const int E = p.experts, e0 = lane * EPL, left = live ? max(E - e0, 0) : 0;
+  float* row = (float*)smem + tok * (EPL * L);
+  float l[EPL], bias[EPL], sc[EPL], om[EPL], dw[EPL];  // om: 1 - s of the sigmoid
+  route_row<T, EPL, VEC>(p.logits, t * p.ld + e0, left, __builtin_inff(), l);
 #pragma unroll
   for (int i = 0; i < EPL; ++i) {
-    const bool in = live && e0 + i < E;
-    l[i] = in ? route_load<T>(p.logits, t * p.ld + e0 + i) : __builtin_inff();
-    if (in && p.bias && !is_finite(p.bias[e0 + i])) l[i] = __builtin_inff();
-    l[i] = is_finite(l[i]) ? l[i] : -__builtin_inff();
-    top = fmaxf(top, l[i]);
-    dw[i] = 0.f;
-    chosen[i] = false;
+    bias[i] = 0.f;
+    row[e0 + i] = __uint_as_float(FREE);
   }
+  if (p.bias) route_row<float, EPL, VEC>(p.bias, e0, left, 0.f, bias);
+  wave_sync();
+  if (live)
+    for (int s = lane; s < p.top_k; s += L) {
+      const int at = p.index[t * p.top_k + s];
+      if (at >= 0 && at < E) row[at] = route_load<T>(p.dweights, t * p.top_k + s);
+    }
   const float NONE = -__builtin_inff();
+  float top = NONE;
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) {
+    l[i] = is_finite(l[i]) && is_finite(bias[i]) ? l[i] : NONE;
+    top = fmaxf(top, l[i]);
+  }
   if (p.score == STRATA_HIP_SCORE_SOFTMAX) {
     top = group_max<L>(top);
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
       sc[i] = l[i] > NONE ? expf(l[i] - top) : 0.f;
+      om[i] = 0.f;
       sum += sc[i];
     }
     sum = group_sum<L>(sum);
@@ -221,18 +341,15 @@ __global__ __launch_bounds__(256) void route_bwd_kernel(RouteParams p) {
       om[i] = l[i] >= 0.f ? b : a;
     }
   }
+  wave_sync();
   float S = 0.f, a = 0.f;
-  for (int s = 0; s < p.top_k; ++s) {
-    const int at = live ? p.index[t * p.top_k + s] : -1;
-    const float d = live ? route_load<T>(p.dweights, t * p.top_k + s) : 0.f;
+  bool chosen[EPL];
 #pragma unroll
-    for (int i = 0; i < EPL; ++i)
-      if (e0 + i == at) {
-        chosen[i] = true;
-        dw[i] = d;
-        S += sc[i];
-        a = fmaf(d, sc[i], a);
-      }
+  for (int i = 0; i < EPL; ++i) {
+    dw[i] = row[e0 + i];
+    chosen[i] = __float_as_uint(dw[i]) != FREE;
+    S += chosen[i] ? sc[i] : 0.f;
+    a = chosen[i] ? fmaf(dw[i], sc[i], a) : a;
   }
   S = group_sum<L>(S);
   a = group_sum<L>(a);
@@ -240,13 +357,28 @@ __global__ __launch_bounds__(256) void route_bwd_kernel(RouteParams p) {
   const float c = norm ? p.scale / S : p.scale, mean = norm ? a / S : 0.f;
   const float back = p.renormalize ? 0.f : p.scale * a;
   if (!live) return;
+  float dl[EPL];
 #pragma unroll
   for (int i = 0; i < EPL; ++i) {
-    if (e0 + i >= E) continue;
     const float ds = chosen[i] ? c * (dw[i] - mean) : 0.f;
-    const float dl = p.score == STRATA_HIP_SCORE_SOFTMAX ? sc[i] * (ds - back) : ds * sc[i] * om[i];
-    route_store<T>(p.dlogits, t * E + e0 + i, l[i] > NONE ? dl : 0.f);
+    dl[i] = l[i] > NONE ? (p.score == STRATA_HIP_SCORE_SOFTMAX ? sc[i] * (ds - back) : ds * sc[i] * om[i]) : 0.f;
   }
+  if constexpr (VEC && EPL >= 4) {
+    if (left >= EPL) {
+#pragma unroll
+      for (int k = 0; k < EPL / 4; ++k) {
+        if constexpr (sizeof(T) == 4)
+          *(f32x4*)((float*)p.dlogits + t * E + e0 + 4 * k) = (f32x4){dl[4 * k], dl[4 * k + 1], dl[4 * k + 2], dl[4 * k + 3]};
+        else
+          *(u32x2*)((bf16*)p.dlogits + t * E + e0 + 4 * k) =
+              (u32x2){pack_bf16x2(dl[4 * k], dl[4 * k + 1]), pack_bf16x2(dl[4 * k + 2], dl[4 * k + 3])};
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < EPL; ++i)
+    if (i < left) route_store<T>(p.dlogits, t * E + e0 + i, dl[i]);
 }
 
 // ---------------------------------------------------------------------------
@@ -464,6 +596,12 @@ static int route_width(int experts, F f) {
   return f(integral_constant<int, 8>{}, integral_constant<int, 64>{});
 }
 
+// Rows of whole 16-byte runs: logits and bias aligned, experts a multiple of 4 (a lane's run of experts
+// is then whole or, the last one of 8, read one by one).
+static bool route_aligned(const strata_hip_expert_route_args* a, const float* bias) {
+  return a->experts % 4 == 0 && ((uintptr_t)a->logits & 15) == 0 && ((uintptr_t)bias & 15) == 0;
+}
+
 static int route_params(const char* name, const strata_hip_expert_route_args* a, RouteParams& p) {
   const std::string n(name);
   if (!a) return fail(STRATA_HIP_EINVAL, n + ": null args");
@@ -506,19 +644,27 @@ extern "C" int strata_hip_expert_route(const strata_hip_expert_route_args* a, vo
   if (const int rc = route_params("expert_route", a, p)) return rc;
   if (p.tokens == 0) return STRATA_HIP_OK;
   if (!p.logits || !p.weights || !p.index) return fail(STRATA_HIP_EINVAL, "expert_route: null pointer");
-  const bool wide = p.bias || p.groups > 1;
+  const bool wide = p.bias || p.groups > 1, vec = route_aligned(a, p.bias) && (p.ld % 4) == 0;
   return route_width(p.experts, [&](auto epl, auto l) {
     constexpr int EPL = decltype(epl)::value, L = decltype(l)::value, TOK = 256 / L;
     const dim3 grid((unsigned)((p.tokens + TOK - 1) / TOK));
-    size_t smem = ((size_t)TOK * p.top_k * 4 + 15) & ~(size_t)15;
-    if (p.groups > 1) smem += (size_t)TOK * (EPL * L + p.groups) * 8;
-    auto go = [&](auto t) {
-      using T = decltype(t);
-      if (wide) hipLaunchKernelGGL((route_kernel<T, double, EPL, L>), grid, dim3(256), smem, (hipStream_t)stream, p);
-      else hipLaunchKernelGGL((route_kernel<T, float, EPL, L>), grid, dim3(256), smem, (hipStream_t)stream, p);
+    size_t smem = ((size_t)TOK * p.top_k * 8 + 15) & ~(size_t)15;
+    if (p.groups > 1) smem += (size_t)TOK * (EPL * L + 2 * p.groups) * 8;
+    auto go = [&](auto t, auto w, auto v) {
+      hipLaunchKernelGGL((route_kernel<decltype(t), decltype(w)::value, decltype(v)::value, EPL, L>), grid, dim3(256), smem,
+                         (hipStream_t)stream, p);
     };
-    if (a->dtype == STRATA_HIP_F32) go(0.f);
-    else go((bf16)0.f);
+    auto with = [&](auto t, auto w) {
+      if (vec) go(t, w, std::true_type{});
+      else go(t, w, std::false_type{});
+    };
+    if (a->dtype == STRATA_HIP_F32) {
+      if (wide) with(0.f, std::true_type{});
+      else with(0.f, std::false_type{});
+    } else {
+      if (wide) with((bf16)0.f, std::true_type{});
+      else with((bf16)0.f, std::false_type{});
+    }
     return check_launch("expert_route");
   });
 }
@@ -529,11 +675,20 @@ extern "C" int strata_hip_expert_route_bwd(const strata_hip_expert_route_args* a
   if (const int rc = route_params("expert_route_bwd", a, p)) return rc;
   if (p.tokens == 0) return STRATA_HIP_OK;
   if (!p.logits || !p.dweights || !p.index || !p.dlogits) return fail(STRATA_HIP_EINVAL, "expert_route_bwd: null pointer");
+  const bool vec = route_aligned(a, p.bias) && (p.ld % 4) == 0 && ((uintptr_t)p.dlogits & 15) == 0;
   return route_width(p.experts, [&](auto epl, auto l) {
     constexpr int EPL = decltype(epl)::value, L = decltype(l)::value, TOK = 256 / L;
     const dim3 grid((unsigned)((p.tokens + TOK - 1) / TOK));
-    if (a->dtype == STRATA_HIP_F32) hipLaunchKernelGGL((route_bwd_kernel<float, EPL, L>), grid, dim3(256), 0, (hipStream_t)stream, p);
-    else hipLaunchKernelGGL((route_bwd_kernel<bf16, EPL, L>), grid, dim3(256), 0, (hipStream_t)stream, p);
+    auto go = [&](auto t, auto v) {
+      hipLaunchKernelGGL((route_bwd_kernel<decltype(t), decltype(v)::value, EPL, L>), grid, dim3(256), (size_t)TOK * EPL * L * 4,
+                         (hipStream_t)stream, p);
+    };
+    auto with = [&](auto t) {
+      if (vec) go(t, std::true_type{});
+      else go(t, std::false_type{});
+    };
+    if (a->dtype == STRATA_HIP_F32) with(0.f);
+    else with((bf16)0.f);
     return check_launch("expert_route_bwd");
   });
 }

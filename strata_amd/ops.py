@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import operator
 from typing import Optional, Sequence
 
 import numpy as np
@@ -1548,6 +1549,20 @@ _expert_route_op.register_autograd(_route_op_backward, setup_context=_route_setu
 # The experts' MLPs
 # ---------------------------------------------------------------------------
 def _expert_check(name, x, weights, index, w1, b1, w2, b2, residual):
+    lead, C = x.shape[:-1], x.shape[-1]
+    (E, H, C1), (E2, N, H2) = w1.shape if w1.dim() == 3 else (0, 0, -1), w2.shape if w2.dim() == 3 else (0, 0, -1)
+    bf16, dev = torch.bfloat16, x.get_device()
+    if (dev >= 0 and x.is_cuda and dev == weights.get_device() == index.get_device() == w1.get_device() == w2.get_device()
+            and x.dtype == bf16 and weights.dtype == bf16 and w1.dtype == bf16 and w2.dtype == bf16 and index.dtype == torch.int32
+            and C == C1 and E == E2 and H == H2 and C and H and N and E and not (C | H | N) % 8
+            and weights.shape == index.shape and weights.shape[:-1] == lead and weights.shape[-1]
+            and all(b is None or (b.dtype == bf16 and b.get_device() == dev and b.shape == (E, n)) for b, n in ((b1, H), (b2, N)))
+            and (residual is None or (residual.dtype == bf16 and residual.get_device() == dev and residual.shape == (*lead, N)))):
+        return
+    _expert_refuse(name, x, weights, index, w1, b1, w2, b2, residual)
+
+
+def _expert_refuse(name, x, weights, index, w1, b1, w2, b2, residual):
     _require_gpu(name, x, weights, index, w1, b1, w2, b2, residual)
     for t, nm in ((x, "x"), (weights, "weights"), (w1, "w1"), (b1, "b1"), (w2, "w2"), (b2, "b2"), (residual, "residual")):
         if t is not None and t.dtype != torch.bfloat16:
@@ -1568,6 +1583,7 @@ def _expert_check(name, x, weights, index, w1, b1, w2, b2, residual):
             raise ValueError(f"{name}: {nm} must be [{E}, {n}], got {tuple(b.shape)}")
     if residual is not None and tuple(residual.shape) != (*x.shape[:-1], N):
         raise ValueError(f"{name}: residual must have shape {(*x.shape[:-1], N)}, got {tuple(residual.shape)}")
+    raise ValueError(f"{name}: bad arguments")
 
 
 def _dense(t: Optional[Tensor]) -> Optional[Tensor]:
@@ -1823,25 +1839,29 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
         raise ValueError(f"{name}: max_norm must be positive and finite")
     # Column by column: a step over many small tensors is bound by this host path (one call of each
     # kind a tensor and column; a loop over tensors that checked each took 3.5 us a tensor).
-    dev, sizes = step.get_device(), [p.numel() for p in params]
+    dev, sizes = step.get_device(), list(map(Tensor.numel, params))
     blocks = [-(-k // STATE_BLOCK) for k in sizes]
     table = np.zeros(max(n, 1), dtype=_ADAMW_TABLE)
     dtypes, written = {}, [step]
     for what, ts in cols.items():
         if ts is None:
             continue
-        some = ts if what in _ADAMW_ALWAYS else [t for t in ts if t is not None]
         want = blocks if what.endswith("scales") else sizes
-        if some is not ts and len(some) != n:
-            want = [k for k, t in zip(want, ts) if t is not None]
-        dtypes[what] = [t.dtype for t in ts] if what in _ADAMW_ALWAYS else None
-        if any(t.get_device() != dev for t in some):
+        some = ts
+        if what not in _ADAMW_ALWAYS:
+            some = [t for t in ts if t is not None]
+            if len(some) != n:
+                want = [k for k, t in zip(want, ts) if t is not None]
+        kinds = list(map(_DTYPE_OF, some))
+        if n and set(map(Tensor.get_device, some)) - {dev}:
             raise ValueError(f"{name}: every tensor must be on step's GPU (cuda:{dev}), {what} are not")
-        if not set(t.dtype for t in some) <= _ADAMW_DTYPES[what] or [t.numel() for t in some] != want \
-                or not all(t.is_contiguous() for t in some):
+        if not _ADAMW_DTYPES[what].issuperset(kinds) or list(map(Tensor.numel, some)) != want \
+                or not all(map(Tensor.is_contiguous, some)):
             raise ValueError(f"{name}: {what} must be contiguous, of {'a scale for every 256 elements of ' if want is blocks else ''}"
                              f"their parameter's size and of {sorted(map(str, _ADAMW_DTYPES[what]))}")
-        table[_ADAMW_FIELD[what]][:n] = [t.data_ptr() if t is not None else 0 for t in ts]
+        dtypes[what] = kinds
+        table[_ADAMW_FIELD[what]][:n] = (list(map(Tensor.data_ptr, ts)) if len(some) == n
+                                         else [t.data_ptr() if t is not None else 0 for t in ts])
         if what != "grads":
             written += some
     codes = [d == torch.int8 for d in dtypes.get("exp_avgs", ())]
@@ -1864,12 +1884,14 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
     a = _lib.AdamwArgs(tp, n, step.data_ptr(), norm.data_ptr() if norm is not None else None, ws.data_ptr(),
                        float(betas[0]), float(betas[1]), float(eps), float(max_norm or 0.0))
     _launch("strata_hip_adamw_step", a, step)
-    if any(t.is_inference() for t in written):
-        written = [t for t in written if not t.is_inference()]
-    torch.autograd.graph.increment_version(written)
+    try:
+        torch.autograd.graph.increment_version(written)
+    except RuntimeError:  # tensors made in inference mode carry no version
+        torch.autograd.graph.increment_version([t for t in written if not t.is_inference()])
     return norm
 
 
+_DTYPE_OF = operator.attrgetter("dtype")
 _ADAMW_ALWAYS = ("params", "grads", "exp_avgs", "exp_avg_sqs")
 _ADAMW_FIELD = {"params": "param", "grads": "grad", "exp_avgs": "exp_avg", "exp_avg_sqs": "exp_avg_sq", "masters": "master",
                 "exp_avg_scales": "exp_avg_scale", "exp_avg_sq_scales": "exp_avg_sq_scale"}
