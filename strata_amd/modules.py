@@ -75,6 +75,60 @@ class GemmGeluMlp(nn.Module):
         return ops.gemm_bias_act(h, fc2.weight, fc2.bias, residual, _lib.ACT_NONE)
 
 
+class ExpertMlp(nn.Module):
+    """A sparse ``GemmGeluMlp``: every token takes ``top_k`` of ``experts`` MLPs.
+
+    ``router`` (Linear without a bias) gives a token's logits, ``ops.expert_route`` its experts and
+    their weights, ``ops.expert_mlp`` their weighted sum and the block's residual: the experts'
+    weights are stacked, ``w1 [E, H, C]``, ``b1 [E, H]``, ``w2 [E, N, H]``, ``b2 [E, N]``.  ``score``,
+    ``groups``, ``top_groups``, ``renormalize`` and ``scale`` are ``expert_route``'s.  With ``balance``
+    a buffer of that name (fp32 ``[E]``, zeros) is added to the scores for the choice alone; the
+    training loop moves it against the experts' load (``route`` returns the choice, ``bincount`` of
+    its index the load) and it stays fp32 when the module is cast.  bf16 on one GPU, as the MLP it
+    stands for; differentiable in x, the residual and every parameter."""
+
+    def __init__(self, in_features: int, hidden_features: int, experts: int, top_k: int = 2,
+                 out_features: Optional[int] = None, bias: bool = True, score: str = "softmax", groups: int = 1,
+                 top_groups: int = 1, renormalize: bool = True, scale: float = 1.0, balance: bool = False):
+        super().__init__()
+        out_features = out_features or in_features
+        if score not in ops.SCORES:
+            raise ValueError(f"score must be one of {sorted(ops.SCORES)}, got {score!r}")
+        if experts % groups or not 1 <= top_groups <= groups or not 1 <= top_k <= experts // groups * top_groups:
+            raise ValueError(f"top_k {top_k} of {experts} experts in {top_groups} of {groups} groups is not a choice")
+        self.top_k, self.score, self.groups, self.top_groups = top_k, score, groups, top_groups
+        self.renormalize, self.scale = renormalize, scale
+        self.router = nn.Linear(in_features, experts, bias=False)
+        self.w1 = nn.Parameter(torch.empty(experts, hidden_features, in_features))
+        self.b1 = nn.Parameter(torch.empty(experts, hidden_features)) if bias else None
+        self.w2 = nn.Parameter(torch.empty(experts, out_features, hidden_features))
+        self.b2 = nn.Parameter(torch.empty(experts, out_features)) if bias else None
+        self.register_buffer("balance", torch.zeros(experts) if balance else None)
+        with torch.no_grad():  # each expert as the Linear layers of the dense MLP start
+            for w, b in ((self.w1, self.b1), (self.w2, self.b2)):
+                bound = w.shape[2] ** -0.5
+                w.uniform_(-bound, bound)
+                if b is not None:
+                    b.uniform_(-bound, bound)
+
+    def _apply(self, fn, recurse=True):
+        balance = self.balance
+        super()._apply(fn, recurse)
+        if balance is not None and self.balance.dtype != torch.float32:
+            self.balance = balance.to(self.balance.device)
+        return self
+
+    def route(self, x: Tensor) -> tuple[Tensor, Tensor]:
+        """``(weights, index)`` ``[..., top_k]`` of tokens ``[..., C]``."""
+        logits = ops.gemm_bias_act(x, self.router.weight, None, None, _lib.ACT_NONE)
+        return ops.expert_route(logits, self.top_k, self.score, self.balance, self.groups, self.top_groups,
+                                self.renormalize, self.scale)
+
+    def forward(self, x: Tensor, residual: Optional[Tensor] = None) -> Tensor:
+        weights, index = self.route(x)
+        return ops.expert_mlp(x, weights, index, self.w1, self.b1, self.w2, self.b2, residual)
+
+
 class FusedNA3DAttention(nn.Module):
     """qkv GEMM -> (qk RMSNorm +) RoPE + QKV pack -> NA3D -> (gate) -> proj GEMM (+ residual).
 
@@ -229,18 +283,22 @@ class StrataBlock(nn.Module):
     ``x = x + proj(na3d(rope(qkv(LN(x)))))``; ``x = x + fc2(GELU(fc1(LN(x))))``
     with non-affine LayerNorms (eps 1e-6).  Stand-in for physicsnemo's
     ``StrataTransformer3DBlock`` (tests/test_dit_3d_pixel.py:109-111) with the
-    same parameter names and order.
+    same parameter names and order.  ``experts``: the MLP is an ``ExpertMlp`` of that
+    many experts (``expert_options``: its other arguments), which the reference's
+    block does not have.
     """
 
     def __init__(self, dim: int, num_heads: int, kernel_size, mlp_ratio: float = 4.0, dilation=1,
                  qkv_bias: bool = True, gated: bool = False, eps: float = 1e-6, qk_norm: bool = False,
-                 qk_norm_affine: bool = False, qk_norm_eps: float = 1e-6, depthwise: bool = False):
+                 qk_norm_affine: bool = False, qk_norm_eps: float = 1e-6, depthwise: bool = False, experts: int = 0,
+                 expert_options: Optional[dict] = None):
         super().__init__()
         self.eps = eps
         self.attn = FusedNA3DAttention(dim, num_heads, kernel_size, dilation, qkv_bias, gated,
                                        qk_norm=qk_norm, qk_norm_affine=qk_norm_affine, qk_norm_eps=qk_norm_eps,
                                        depthwise=depthwise)
-        self.mlp = GemmGeluMlp(dim, int(dim * mlp_ratio))
+        hidden = int(dim * mlp_ratio)
+        self.mlp = ExpertMlp(dim, hidden, experts, **(expert_options or {})) if experts else GemmGeluMlp(dim, hidden)
 
     def forward(self, x: Tensor, rope: Optional[tuple[Tensor, Tensor]] = None) -> Tensor:
         h = ops.layer_norm(x, self.eps)
@@ -409,6 +467,13 @@ def init_xavier_(module: nn.Module, generator: torch.Generator) -> None:
                 m.weight.copy_(w)
                 if m.bias is not None:
                     m.bias.zero_()
+        elif isinstance(m, ExpertMlp):
+            with torch.no_grad():
+                for t, b in ((m.w1, m.b1), (m.w2, m.b2)):
+                    bound = (6.0 / (t.shape[1] + t.shape[2])) ** 0.5
+                    t.copy_(torch.rand(t.shape, generator=generator, dtype=torch.float32) * (2 * bound) - bound)
+                    if b is not None:
+                        b.zero_()
 
 
 def block_param_names(gated: bool = False) -> Sequence[str]:

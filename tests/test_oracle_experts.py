@@ -166,3 +166,26 @@ def test_ops_refuse_cpu_tensors():
     w1, w2 = torch.zeros(3, 16, 8).bfloat16(), torch.zeros(3, 8, 16).bfloat16()
     with pytest.raises(ValueError, match="GPU"):
         ops.expert_mlp(x, w, torch.zeros(2, 1, dtype=torch.int32), w1, None, w2, None)
+
+
+def test_expert_modules_without_a_gpu():
+    from strata_amd.modules import ExpertMlp, StrataBlock, init_xavier_
+
+    blk = StrataBlock(64, 1, (3, 3, 3), experts=4, expert_options=dict(top_k=1, balance=True))
+    names = [n for n, _ in blk.named_parameters()]
+    assert names == ["attn.qkv.weight", "attn.qkv.bias", "attn.proj.weight", "attn.proj.bias", "mlp.w1", "mlp.b1", "mlp.w2",
+                     "mlp.b2", "mlp.router.weight"]
+    init_xavier_(blk, torch.Generator().manual_seed(0))
+    assert float(blk.mlp.w1.detach().abs().max()) <= (6 / (64 + 256)) ** 0.5 and not blk.mlp.b1.any()
+    blk.mlp.balance[1] = 1 / 3
+    blk.bfloat16()
+    assert blk.mlp.balance.dtype == torch.float32 and float(blk.mlp.balance[1]) == float(torch.tensor(1 / 3))
+    assert blk.mlp.w1.dtype == torch.bfloat16 and "mlp.balance" in blk.state_dict()
+    with pytest.raises(ValueError, match="not a choice"):
+        ExpertMlp(64, 64, 4, top_k=5)
+    with pytest.raises(ValueError, match="not a choice"):
+        ExpertMlp(64, 64, 8, top_k=3, groups=4, top_groups=1)
+    with pytest.raises(ValueError, match="score"):
+        ExpertMlp(64, 64, 4, score="tanh")
+    assert [n for n, _ in StrataBlock(64, 1, (3, 3, 3)).named_parameters()][4:] == [
+        "mlp.layers.0.weight", "mlp.layers.0.bias", "mlp.layers.2.weight", "mlp.layers.2.bias"]
