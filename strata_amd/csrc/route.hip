@@ -499,7 +499,8 @@ __device__ __forceinline__ int plan_sum(const PlanParams& p, int* total, int* pa
   part[PLAN_N + tid] = m;
   __syncthreads();
   int before = 0, all = 0, mm = 0;
-  for (int k = 0; k < seg; ++k) {
+  const int per = (p.blocks + seg - 1) / seg, used = (p.blocks + per - 1) / per;  // runs that hold blocks
+  for (int k = 0; k < used; ++k) {
     const int v = part[k * w + e];
     before += k < g ? v : 0;
     all += v;

@@ -1397,25 +1397,32 @@ gated_add.register_autograd(_no_backward("strata_hip::gated_add"))
 SCORES = {"softmax": _lib.SCORE_SOFTMAX, "sigmoid": _lib.SCORE_SIGMOID}
 
 
-def _route_args(name, logits, bias, top_k, score, groups, top_groups, renormalize, scale):
-    _require_gpu(name, logits, bias)
+def _route_args(name, logits, bias, top_k, score, groups, top_groups, renormalize, scale, weights, index, dweights, dlogits):
+    """The structure of strata_hip_expert_route and what it points into; the last four are pointers."""
     if score not in SCORES:
         raise ValueError(f"{name}: score must be one of {sorted(SCORES)}, got {score!r}")
+    dtype = _dtype_code(name, logits)
     if logits.dim() < 1:
         raise ValueError(f"{name}: logits must be [..., experts]")
     E = logits.shape[-1]
-    if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (E,)):
-        raise ValueError(f"{name}: bias must be float32 [{E}], got {bias.dtype} {tuple(bias.shape)}")
-    l2 = logits.reshape(-1, E)
-    if l2.stride(1) != 1:
-        l2 = l2.contiguous()
-    a = _lib.ExpertRouteArgs()
-    a.logits, a.tokens, a.ld = l2.data_ptr(), l2.shape[0], l2.stride(0) if l2.shape[0] > 1 else E
-    b = bias.contiguous() if bias is not None else None
-    a.bias = b.data_ptr() if b is not None else None
-    a.dtype, a.experts, a.top_k, a.score = _dtype_code(name, logits), E, int(top_k), SCORES[score]
-    a.groups, a.top_groups, a.renormalize, a.scale = int(groups), int(top_groups), int(bool(renormalize)), float(scale)
-    return a, (l2, b)
+    if bias is not None:
+        if bias.dtype != torch.float32 or tuple(bias.shape) != (E,):
+            raise ValueError(f"{name}: bias must be float32 [{E}], got {bias.dtype} {tuple(bias.shape)}")
+        bias = bias.contiguous()
+    rows = logits.numel() // E if E else 0
+    if logits.is_contiguous():
+        l2, ld = logits, E
+    else:
+        l2 = logits.reshape(-1, E)
+        if l2.stride(1) != 1:
+            l2 = l2.contiguous()
+        ld = l2.stride(0) if rows > 1 else E
+    a = _lib.ExpertRouteArgs(l2.data_ptr(), bias.data_ptr() if bias is not None else None, weights, index, dweights, dlogits,
+                             rows, ld, dtype, E, top_k, SCORES[score], groups, top_groups, 1 if renormalize else 0, scale)
+    return a, (l2, bias)
+
+
+_PLAIN = (Tensor, torch.nn.Parameter)
 
 
 def _eager(*ts: Optional[Tensor]) -> bool:
@@ -1423,36 +1430,45 @@ def _eager(*ts: Optional[Tensor]) -> bool:
     launch through a ``torch.autograd.Function`` of their own.  The custom op's dispatch and its
     registered autograd cost 25 us a forward and 55 us a backward of host time beside it, more
     than the kernels of a small call; traced calls and tensor subclasses go through the custom op."""
-    return not torch.compiler.is_compiling() and all(t is None or type(t) is Tensor or type(t) is torch.nn.Parameter
-                                                     for t in ts)
+    if torch.compiler.is_compiling():
+        return False
+    for t in ts:
+        if t is not None and type(t) not in _PLAIN:
+            return False
+    return True
 
 
 def _wants_grad(*ts: Optional[Tensor]) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _route_forward(logits, top_k, score, bias, groups, top_groups, renormalize, scale):
     name = "expert_route"
-    a, keep = _route_args(name, logits, bias, top_k, score, groups, top_groups, renormalize, scale)
+    _require_gpu(name, logits, bias)
     shape = (*logits.shape[:-1], int(top_k))
-    weights = torch.empty(shape, dtype=logits.dtype, device=logits.device)
+    weights = logits.new_empty(shape)
     index = torch.empty(shape, dtype=torch.int32, device=logits.device)
-    a.weights, a.index = weights.data_ptr(), index.data_ptr()
+    a, keep = _route_args(name, logits, bias, top_k, score, groups, top_groups, renormalize, scale, weights.data_ptr(),
+                          index.data_ptr(), None, None)
     _launch("strata_hip_expert_route", a, logits)
     return weights, index
 
 
 def _route_backward(dweights, logits, index, top_k, score, bias, renormalize, scale):
     name = "expert_route_bwd"
-    a, keep = _route_args(name, logits, bias, top_k, score, 1, 1, renormalize, scale)
-    _require_gpu(name, logits, dweights, index)
+    _require_gpu(name, logits, dweights, index, bias)
     shape = (*logits.shape[:-1], int(top_k))
     if dweights.dtype != logits.dtype or tuple(dweights.shape) != shape or index.dtype != torch.int32 \
             or tuple(index.shape) != shape:
         raise ValueError(f"{name}: dweights must be {logits.dtype} and index int32, {shape}")
     d, i = dweights.contiguous(), index.contiguous()
     out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    a.dweights, a.index, a.dlogits = d.data_ptr(), i.data_ptr(), out.data_ptr()
+    a, keep = _route_args(name, logits, bias, top_k, score, 1, 1, renormalize, scale, None, i.data_ptr(), d.data_ptr(),
+                          out.data_ptr())
     _launch("strata_hip_expert_route_bwd", a, logits)
     return out
 
@@ -1610,52 +1626,69 @@ def _expert_tile(pairs: int, w1: Tensor, w2: Tensor, train: bool) -> int:
 
 
 def _plan_size(pairs: int, experts: int, tile: int) -> int:
+    """int32 elements of a plan: row_token | row_weight (fp32) | slot_row | offsets | tiles."""
     return 3 * pairs + experts + 2 + 2 * (pairs // tile + experts)
 
 
+def _plan_args(index_ptr, weights_ptr, p, ws, n, k, experts, tile):
+    return _lib.ExpertPlanArgs(index_ptr, weights_ptr, p, p + 4 * n, p + 8 * n, p + 12 * n, p + 4 * (3 * n + experts + 1), ws, n,
+                               k, experts, tile, 0)
+
+
 def _expert_plan(index: Tensor, weights: Tensor, experts: int, tile: int) -> Tensor:
-    """The plan of ``strata_hip_expert_plan`` in one int32 tensor:
-    [row_token | row_weight (fp32) | slot_row | offsets | tiles]."""
+    """The plan of ``strata_hip_expert_plan`` in one int32 tensor (see ``_plan_size``)."""
     i, w = index.contiguous(), weights.contiguous()
-    n, k = i.numel(), i.shape[-1]
-    plan = torch.empty(_plan_size(n, experts, tile), dtype=torch.int32, device=index.device)
-    nws = int(_lib.function("strata_hip_expert_plan_workspace")(n, experts))
-    ws = torch.empty(nws, dtype=torch.int32, device=index.device) if nws else None
+    n = i.numel()
+    size = _plan_size(n, experts, tile)
+    plan = torch.empty(size + int(_lib.function("strata_hip_expert_plan_workspace")(n, experts)), dtype=torch.int32,
+                       device=index.device)
     p = plan.data_ptr()
-    a = _lib.ExpertPlanArgs(i.data_ptr(), w.data_ptr(), p, p + 4 * n, p + 8 * n, p + 12 * n, p + 4 * (3 * n + experts + 1),
-                            _ptr(ws), n, k, experts, tile, 0)
-    _launch("strata_hip_expert_plan", a, index)
+    _launch("strata_hip_expert_plan", _plan_args(i.data_ptr(), w.data_ptr(), p, p + 4 * size, n, i.shape[-1], experts, tile), index)
     return plan
 
 
-def _expert_args(x, weights, plan, tile, w1, b1, w2, b2, h, dact, y):
-    """The structure of strata_hip_expert_mlp without out and residual, and what it points into."""
-    C, E, H, N, k = x.shape[-1], w1.shape[0], w1.shape[1], w2.shape[1], weights.shape[-1]
+def _expert_space(n: int, E: int, H: int, N: int, tile: int, train: bool) -> tuple[int, int, int, int, int]:
+    """Byte offsets of dact, y, the plan and the plan's workspace behind h, and the size of all."""
+    dact = 2 * n * H
+    y = dact + (2 * n * H if train else 0)
+    plan = y + 4 * n * N
+    ws = plan + 4 * _plan_size(n, E, tile)
+    return dact, y, plan, ws, ws + 4 * int(_lib.function("strata_hip_expert_plan_workspace")(n, E))
+
+
+def _expert_args(x, weights, w1, b1, w2, b2, space: int, at, tile: int, train: bool):
+    """The structure of strata_hip_expert_mlp without out and residual, and what it points into.
+    ``space``: the address of the workspace that ``at`` (``_expert_space``) divides."""
+    E, H, C = w1.shape
+    N, k = w2.shape[1], weights.shape[-1]
     T, xp, ldx, x2 = _dense_rows(x, C)
     w, w1, b1, w2, b2 = weights.contiguous(), _dense(w1), _dense(b1), _dense(w2), _dense(b2)
-    n, p = T * k, plan.data_ptr()
+    n, p = T * k, space + at[2]
     a = _lib.ExpertMlpArgs(xp, w.data_ptr(), p, p + 4 * n, p + 8 * n, p + 12 * n, p + 4 * (3 * n + E + 1), w1.data_ptr(),
-                           _ptr(b1), w2.data_ptr(), _ptr(b2), None, None, h.data_ptr(), _ptr(dact), y.data_ptr(), T, ldx, 0,
-                           k, E, C, H, N, tile)
+                           _ptr(b1), w2.data_ptr(), _ptr(b2), None, None, space, space + at[0] if train else None,
+                           space + at[1], T, ldx, 0, k, E, C, H, N, tile)
     return a, (x2, w, w1, b1, w2, b2)
 
 
-def _expert_forward(name, x, weights, index, w1, b1, w2, b2, residual, save: bool):
+def _expert_forward(name, x, weights, index, w1, b1, w2, b2, residual, train: bool):
+    """``(out, space)``: the workspace holds the hidden activations, with ``train`` the GELU's derivative
+    at them, the experts' outputs and the plan, which a backward reads again."""
     _expert_check(name, x, weights, index, w1, b1, w2, b2, residual)
     E, H, N = w1.shape[0], w1.shape[1], w2.shape[1]
     n = index.numel()
-    out = torch.empty((*x.shape[:-1], N), dtype=torch.bfloat16, device=x.device)
-    h = torch.empty((n, H), dtype=torch.bfloat16, device=x.device)
-    dact = torch.empty((n, H), dtype=torch.float16, device=x.device) if save else None
-    y = torch.empty((n, N), dtype=torch.float32, device=x.device)
-    tile = _expert_tile(n, w1, w2, save)
-    plan = _expert_plan(index, weights, E, tile)
-    a, keep = _expert_args(x, weights, plan, tile, w1, b1, w2, b2, h, dact, y)
+    out = x.new_empty((*x.shape[:-1], N))
+    tile = _expert_tile(n, w1, w2, train)
+    at = _expert_space(n, E, H, N, tile, train)
+    space = torch.empty(at[4], dtype=torch.uint8, device=x.device)
+    a, keep = _expert_args(x, weights, w1, b1, w2, b2, space.data_ptr(), at, tile, train)
     if residual is not None:
         _, a.residual, a.ldr, r2 = _dense_rows(residual, N)
     a.out = out.data_ptr()
+    i = index.contiguous()
+    s = space.data_ptr()
+    _launch("strata_hip_expert_plan", _plan_args(i.data_ptr(), a.weights, s + at[2], s + at[3], n, a.top_k, E, tile), x)
     _launch("strata_hip_expert_mlp", a, x)
-    return out, h, dact, y, plan
+    return out, space
 
 
 @torch.library.custom_op("strata_hip::expert_mlp_fwd", mutates_args=())
@@ -1675,27 +1708,26 @@ expert_mlp_fwd.register_autograd(_no_backward("strata_hip::expert_mlp_fwd"))
 
 @torch.library.custom_op("strata_hip::expert_mlp_train", mutates_args=())
 def expert_mlp_train(x: Tensor, weights: Tensor, index: Tensor, w1: Tensor, b1: Optional[Tensor], w2: Tensor,
-                     b2: Optional[Tensor], residual: Optional[Tensor]) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
-    """``expert_mlp`` under autograd: the output and, for the backward, the hidden activations, the
-    GELU's derivative at them, the experts' outputs and the plan."""
+                     b2: Optional[Tensor], residual: Optional[Tensor]) -> tuple[Tensor, Tensor]:
+    """``expert_mlp`` under autograd: the output and, as bytes, what the backward reads again (the hidden
+    activations, the GELU's derivative at them, the experts' outputs and the plan)."""
     return _expert_forward("expert_mlp", x, weights, index, w1, b1, w2, b2, residual, True)
 
 
 @expert_mlp_train.register_fake
 def _(x, weights, index, w1, b1, w2, b2, residual):
     n, E, H, N = index.numel(), w1.shape[0], w1.shape[1], w2.shape[1]
-    return (x.new_empty((*x.shape[:-1], N)), x.new_empty((n, H)), x.new_empty((n, H), dtype=torch.float16),
-            x.new_empty((n, N), dtype=torch.float32),
-            x.new_empty((_plan_size(n, E, _expert_tile(n, w1, w2, True)),), dtype=torch.int32))
+    size = _expert_space(n, E, H, N, _expert_tile(n, w1, w2, True), True)[4]
+    return x.new_empty((*x.shape[:-1], N)), x.new_empty((size,), dtype=torch.uint8)
 
 
-def _expert_backward(dout, x, weights, w1, b1, w2, b2, h, dact, y, plan, need):
+def _expert_backward(dout, x, weights, w1, b1, w2, b2, space, need):
     """Gradients at ``(x, weights, w1, b1, w2, b2)``, None where ``need`` asks for none."""
     E, H, C = w1.shape
-    N = w2.shape[1]
-    n = h.shape[0]
+    N, n = w2.shape[1], weights.numel()
     tile = _expert_tile(n, w1, w2, True)
-    a, keep = _expert_args(x, weights, plan, tile, w1, b1, w2, b2, h, dact, y)
+    at = _expert_space(n, E, H, N, tile, True)
+    a, keep = _expert_args(x, weights, w1, b1, w2, b2, space.data_ptr(), at, tile, True)
     new = lambda *shape: torch.empty(shape, dtype=torch.bfloat16, device=x.device)  # noqa: E731
     want_x, want_wt = need[0], need[1]
     want_1, want_2 = need[2] or need[3], need[4] or need[5]
@@ -1714,16 +1746,15 @@ def _expert_backward(dout, x, weights, w1, b1, w2, b2, h, dact, y, plan, need):
 
 @torch.library.custom_op("strata_hip::expert_mlp_bwd", mutates_args=())
 def expert_mlp_bwd(dout: Tensor, x: Tensor, weights: Tensor, w1: Tensor, b1: Optional[Tensor], w2: Tensor,
-                   b2: Optional[Tensor], h: Tensor, dact: Tensor, y: Tensor, plan: Tensor,
-                   need: Sequence[bool]) -> list[Tensor]:
+                   b2: Optional[Tensor], space: Tensor, need: Sequence[bool]) -> list[Tensor]:
     """Gradients of ``expert_mlp_train`` at ``(x, weights, w1, b1, w2, b2)``, an empty tensor where
     ``need`` asks for none (a bias's comes from its weight's launch)."""
-    grads = _expert_backward(dout, x, weights, w1, b1, w2, b2, h, dact, y, plan, need)
+    grads = _expert_backward(dout, x, weights, w1, b1, w2, b2, space, need)
     return [g if g is not None else x.new_empty(0) for g in grads]
 
 
 @expert_mlp_bwd.register_fake
-def _(dout, x, weights, w1, b1, w2, b2, h, dact, y, plan, need):
+def _(dout, x, weights, w1, b1, w2, b2, space, need):
     return [torch.empty_like(t) if t is not None and wanted else x.new_empty(0)
             for t, wanted in zip((x, weights, w1, b1, w2, b2), need)]
 
@@ -1733,21 +1764,21 @@ expert_mlp_bwd.register_autograd(_no_backward("strata_hip::expert_mlp_bwd"))
 
 def _expert_setup_context(ctx, inputs, output):
     x, weights, index, w1, b1, w2, b2, residual = inputs
-    _, h, dact, y, plan = output
+    _, space = output
     ctx.has = [True, True, True, b1 is not None, True, b2 is not None]
     ctx.has_res = residual is not None
-    ctx.mark_non_differentiable(h, dact, y, plan)
+    ctx.mark_non_differentiable(space)
     ctx.set_materialize_grads(False)
-    ctx.save_for_backward(x, weights, w1, b1, w2, b2, h, dact, y, plan)
+    ctx.save_for_backward(x, weights, w1, b1, w2, b2, space)
 
 
 def _expert_op_backward(ctx, dout, *_unused):
     if dout is None:
         return (None,) * 8
-    x, weights, w1, b1, w2, b2, h, dact, y, plan = ctx.saved_tensors
+    x, weights, w1, b1, w2, b2, space = ctx.saved_tensors
     n = ctx.needs_input_grad
     need = [bool(q and has) for q, has in zip((n[0], n[1], n[3], n[4], n[5], n[6]), ctx.has)]
-    grads = expert_mlp_bwd(dout, x, weights, w1, b1, w2, b2, h, dact, y, plan, need) if any(need) else [None] * 6
+    grads = expert_mlp_bwd(dout, x, weights, w1, b1, w2, b2, space, need) if any(need) else [None] * 6
     gx, gwt, g1, gb1, g2, gb2 = (g if wanted else None for g, wanted in zip(grads, need))
     return gx, gwt, None, g1, gb1, g2, gb2, dout if ctx.has_res and n[7] else None
 
@@ -1758,9 +1789,9 @@ expert_mlp_train.register_autograd(_expert_op_backward, setup_context=_expert_se
 class _ExpertMlp(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weights, index, w1, b1, w2, b2, residual):
-        out, h, dact, y, plan = _expert_forward("expert_mlp", x, weights, index, w1, b1, w2, b2, residual, True)
+        out, space = _expert_forward("expert_mlp", x, weights, index, w1, b1, w2, b2, residual, True)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x, weights, w1, b1, w2, b2, h, dact, y, plan)
+        ctx.save_for_backward(x, weights, w1, b1, w2, b2, space)
         return out
 
     @staticmethod
@@ -1848,21 +1879,20 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
             continue
         want = blocks if what.endswith("scales") else sizes
         some = ts
-        if what not in _ADAMW_ALWAYS:
+        if what not in _ADAMW_ALWAYS and any(t is None for t in ts):
             some = [t for t in ts if t is not None]
-            if len(some) != n:
-                want = [k for k, t in zip(want, ts) if t is not None]
-        kinds = list(map(_DTYPE_OF, some))
-        if n and set(map(Tensor.get_device, some)) - {dev}:
+            want = [k for k, t in zip(want, ts) if t is not None]
+        if some and set(map(Tensor.get_device, some)) != {dev}:
             raise ValueError(f"{name}: every tensor must be on step's GPU (cuda:{dev}), {what} are not")
-        if not _ADAMW_DTYPES[what].issuperset(kinds) or list(map(Tensor.numel, some)) != want \
+        kinds = list(map(_DTYPE_OF, some))
+        if not _ADAMW_DTYPES[what].issuperset(kinds) or (what != "params" and list(map(Tensor.numel, some)) != want) \
                 or not all(map(Tensor.is_contiguous, some)):
             raise ValueError(f"{name}: {what} must be contiguous, of {'a scale for every 256 elements of ' if want is blocks else ''}"
                              f"their parameter's size and of {sorted(map(str, _ADAMW_DTYPES[what]))}")
         dtypes[what] = kinds
-        table[_ADAMW_FIELD[what]][:n] = (list(map(Tensor.data_ptr, ts)) if len(some) == n
-                                         else [t.data_ptr() if t is not None else 0 for t in ts])
-        if what != "grads":
+        ptrs = map(Tensor.data_ptr, ts) if some is ts else (t.data_ptr() if t is not None else 0 for t in ts)
+        table[_ADAMW_FIELD[what]][:n] = np.fromiter(ptrs, np.int64, n)
+        if what in ("params", "masters"):  # the moments are no one's graph's leaves
             written += some
     codes = [d == torch.int8 for d in dtypes.get("exp_avgs", ())]
     if codes != [d == torch.uint8 for d in dtypes.get("exp_avg_sqs", ())]:
@@ -1873,8 +1903,10 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
             raise ValueError(f"{name}: 8-bit moments come with their scales, fp32 ones without")
     if n:
         table["n"][:n], table["lr"][:n], table["weight_decay"][:n] = sizes, rates[0], rates[1]
-        table["param_dtype"][:n] = [d == torch.bfloat16 for d in dtypes["params"]]  # _lib.F32, _lib.BF16
-        table["grad_dtype"][:n] = [d == torch.bfloat16 for d in dtypes["grads"]]
+        for field, what in (("param_dtype", "params"), ("grad_dtype", "grads")):
+            kinds = dtypes[what]
+            same = kinds.count(kinds[0]) == n  # most often one type for all
+            table[field][:n] = _ADAMW_CODE[kinds[0]] if same else [_ADAMW_CODE[d] for d in kinds]
         table["state_bits"][:n] = [8 if c else 32 for c in codes]
         if masters is not None and any(w is not None and d != torch.bfloat16 for w, d in zip(masters, dtypes["params"])):
             raise ValueError(f"{name}: masters belong to bfloat16 parameters")
@@ -1891,6 +1923,7 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
     return norm
 
 
+_ADAMW_CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 _DTYPE_OF = operator.attrgetter("dtype")
 _ADAMW_ALWAYS = ("params", "grads", "exp_avgs", "exp_avg_sqs")
 _ADAMW_FIELD = {"params": "param", "grads": "grad", "exp_avgs": "exp_avg", "exp_avg_sqs": "exp_avg_sq", "masters": "master",

@@ -173,7 +173,7 @@ def test_plan(gpu, n, E, tile):
     w = torch.randn(n, generator=g).bfloat16()
     plan = ops._expert_plan(idx.view(-1, k).to(gpu), w.view(-1, k).to(gpu), E, tile).cpu()
     token, weight, slot_row, off = plan[:n], plan[n:2 * n].view(torch.float32), plan[2 * n:3 * n], plan[3 * n:3 * n + E + 1]
-    tiles = plan[3 * n + E + 1:]
+    tiles = plan[3 * n + E + 1:ops._plan_size(n, E, tile)]
     ok = (idx >= 0) & (idx < E)
     order = torch.where(ok, idx, E).sort(stable=True).indices[: int(ok.sum())]
     R = order.numel()
