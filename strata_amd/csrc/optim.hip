@@ -170,8 +170,13 @@ struct AwShared {
 template <bool FAST>
 __device__ __forceinline__ float aw_update(const AwShared& s, float p, float m, float v) {
   if (FAST) {
-    const bool small = v < 0x1p-96f;
-    const float root = __builtin_amdgcn_sqrtf(small ? v * 0x1p32f : v) * (small ? 0x1p-16f : 1.f);
+    float root;
+    if (s.eps >= 1e-10f) {  // uniform; a root under 2^-48 is then nothing beside eps
+      root = __builtin_amdgcn_sqrtf(v);
+    } else {
+      const bool small = v < 0x1p-96f;
+      root = __builtin_amdgcn_sqrtf(small ? v * 0x1p32f : v) * (small ? 0x1p-16f : 1.f);
+    }
     return fmaf(p, s.decay, -(s.rate * m) * __builtin_amdgcn_rcpf(fmaf(root, s.rbc2, s.eps)));
   }
   const float denom = fmaf(__builtin_sqrtf(v), s.rbc2, s.eps);
@@ -251,39 +256,33 @@ __device__ __forceinline__ double aw_value_v(int c, double scale) {
   const double r = (double)(c + 1) * (1. / 256.);
   return r * r * scale;
 }
-// The code nearest to steps * sqrt(x / scale), found in 32 bits; within 2e-4 of a border
-// (its 32-bit place is off by at most 7e-5) held to the border (k +- 1/2)^2 scale in 64.
-__device__ __forceinline__ int aw_code(double x, float scale, float inv, float steps, int lo, int hi) {
-  const float at = steps * __builtin_amdgcn_sqrtf((float)x * inv);
-  const float near = rintf(at);
-  int k = min(max((int)near, lo), hi);
-  if (fabsf(at - near) > 0.4998f) {
-    const double q = x * ((double)steps * (double)steps), sc = (double)scale;
-    const double up = (double)k + .5, dn = (double)k - .5;
-    if (k < hi && q > up * up * sc) ++k;
-    else if (k > lo && q < dn * dn * sc) --k;
-  }
+// A code found in 32 bits, held to its borders (k +- 1/2)^2 scale in 64.
+__device__ __forceinline__ int aw_settle(int k, double x, double scale, double steps, int lo, int hi) {
+  const double q = x * (steps * steps), up = (double)k + .5, dn = (double)k - .5;
+  if (k < hi && q > up * up * scale) ++k;
+  else if (k > lo && q < dn * dn * scale) --k;
   return k;
 }
 
-// The larger of two magnitudes; one that is no number stays (the block's scale then says so).
-__device__ __forceinline__ float aw_max(float a, float b) { return b > a || b != b ? b : a; }
-
 // 8-bit moments: 32 lanes take a block of 256, eight consecutive elements each; a workgroup's
-// chunk is two rounds of eight blocks.  VALU and memory are close here (45 operations, four of
-// them square roots or reciprocals, for 10 bytes of a bf16 element): the squares of the codes are
-// taken in integers and the decays folded into the scales, so that a moment costs one
-// conversion, one product and one fused multiply-add in 64 bits.
-template <bool P32, bool G32, bool MASTER>
+// chunk is two rounds of eight blocks.  VALU and memory are close here (some 50 operations, four of
+// them roots or reciprocals, for 10 bytes of a bf16 element): squares of codes are exact in
+// 32 bits, so that a moment costs two conversions, four products and a sum in 64 bits; these round
+// one by one, as the formula writes them, because a decayed scale and a share of a bf16 gradient
+// often add up to exactly half way between two 32-bit scales (0.9 s + 0.1 g); the largest magnitude is taken of the bits (one that
+// is no number stays: the block's scale then says so); and whether any of a lane's sixteen codes
+// is within 8e-5 of a border (a 32-bit place is off by at most 7e-5) is asked once, in a
+// seventh of all waves with yes.  VEC: a whole aligned run of eight, else `left` elements one by one.
+template <bool P32, bool G32, bool MASTER, bool VEC>
 __device__ __forceinline__ void aw_block8(const AwTensor& t, const AwShared& s, int64_t i, int left) {
+#pragma clang fp contract(off)
   const int64_t blk = i / AW_BLOCK;
-  const bool vec = (t.flags & AW_ALIGNED) && left == 8;
   int8_t* mc = (int8_t*)t.m;
   uint8_t* vc = (uint8_t*)t.v;
   float g[8], p[8];
-  int cm[8], cv[8];
+  uint32_t wm[2] = {0u, 0u}, wv[2] = {0u, 0u};  // four codes a word
   const float scm = t.ms[blk], scv = t.vs[blk];
-  if (vec) {
+  if constexpr (VEC) {
     const u32x2 a = *(const u32x2*)(mc + i), b = *(const u32x2*)(vc + i);
     const f32x4 x0 = load4(t.g, i, G32), x1 = load4(t.g, i + 4, G32);
     const f32x4 y0 = MASTER ? *(const f32x4*)(t.master + i) : load4(t.p, i, P32);
@@ -294,10 +293,11 @@ __device__ __forceinline__ void aw_block8(const AwTensor& t, const AwShared& s, 
       g[4 + e] = x1[e];
       p[e] = y0[e];
       p[4 + e] = y1[e];
-      cm[e] = (int)(int8_t)(a[0] >> (8 * e));
-      cm[4 + e] = (int)(int8_t)(a[1] >> (8 * e));
-      cv[e] = (int)((b[0] >> (8 * e)) & 255u);
-      cv[4 + e] = (int)((b[1] >> (8 * e)) & 255u);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      wm[h] = a[h];
+      wv[h] = b[h];
     }
   } else {
 #pragma unroll
@@ -305,47 +305,65 @@ __device__ __forceinline__ void aw_block8(const AwTensor& t, const AwShared& s, 
       const bool in = k < left;
       g[k] = in ? load1(t.g, i + k, G32) : 0.f;
       p[k] = in ? (MASTER ? t.master[i + k] : load1(t.p, i + k, P32)) : 0.f;
-      cm[k] = in ? mc[i + k] : 0;
-      cv[k] = in ? vc[i + k] : 0;
+      wm[k >> 2] |= (in ? (uint32_t)(uint8_t)mc[i + k] : 0u) << (8 * (k & 3));
+      wv[k >> 2] |= (in ? (uint32_t)vc[i + k] : 0u) << (8 * (k & 3));
     }
   }
-  const double sm = s.db1 * ((double)scm * (1. / 16129.)), sv = s.db2 * ((double)scv * (1. / 65536.));
+  const double sm = (double)scm * s.db1, sv = (double)scv * (1. / 65536.);
   double m[8], v[8];
-  float am = 0.f, av = 0.f;
+  float mf[8], vf[8];
+  uint32_t am = 0u, av = 0u;  // bits of the largest magnitudes
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
+    const float cm = (float)(int)(int8_t)(wm[k >> 2] >> (8 * (k & 3)));
+    const float cv = (float)((wv[k >> 2] >> (8 * (k & 3))) & 255u) + 1.f;
     const double gd = (double)g[k];
-    m[k] = fma(s.dg1, gd, sm * (double)(cm[k] * abs(cm[k])));
-    v[k] = fma(s.dg2 * gd, gd, sv * (double)((cv[k] + 1) * (cv[k] + 1)));
-    const float mf = (float)m[k], vf = (float)v[k];
-    if (k < left) {  // rounding keeps the order: the largest rounded is the largest, rounded
-      am = aw_max(am, fabsf(mf));
-      av = aw_max(av, vf);
+    m[k] = (double)(cm * fabsf(cm)) * (1. / 16129.) * sm + s.dg1 * gd;  // 127^2 / 16129 is 1
+    v[k] = (double)(cv * cv) * sv * s.db2 + s.dg2 * gd * gd;            // the first product is exact
+    mf[k] = (float)m[k];
+    vf[k] = (float)v[k];
+    if (VEC || k < left) {  // rounding keeps the order: the largest rounded is the largest, rounded
+      am = max(am, __float_as_uint(mf[k]) & 0x7fffffffu);
+      av = max(av, __float_as_uint(vf[k]) & 0x7fffffffu);
     }
-    p[k] = aw_update<true>(s, p[k], mf, vf);
+    p[k] = aw_update<true>(s, p[k], mf[k], vf[k]);
   }
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    am = aw_max(am, __shfl_xor(am, d));
-    av = aw_max(av, __shfl_xor(av, d));
+    am = max(am, (uint32_t)__shfl_xor((int)am, d));
+    av = max(av, (uint32_t)__shfl_xor((int)av, d));
   }
-  const float im = am > 0.f ? 1.f / am : 0.f, iv = av > 0.f ? 1.f / av : 0.f;
+  const float fm = __uint_as_float(am), fv = __uint_as_float(av);
+  const float im = fm > 0.f ? 16129.f / fm : 0.f, iv = fv > 0.f ? 65536.f / fv : 0.f;
+  int km[8], kv[8];
+  float dev = 0.f;
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
-    const int c = aw_code(fabs(m[k]), am, im, 127.f, 0, 127);
-    cm[k] = m[k] < 0. ? -c : c;
-    cv[k] = aw_code(v[k], av, iv, 256.f, 1, 256) - 1;
+    const float a = __builtin_amdgcn_sqrtf(fabsf(mf[k]) * im), b = fmaxf(__builtin_amdgcn_sqrtf(vf[k] * iv), 1.f);
+    const float ra = rintf(a), rb = rintf(b);
+    dev = fmaxf(dev, fmaxf(fabsf(a - ra), fabsf(b - rb)));
+    km[k] = (int)fminf(ra, 127.f);  // a block whose scale is no number or infinite: any code
+    kv[k] = (int)fminf(rb, 256.f);
   }
+  if (dev > 0.49992f) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      km[k] = aw_settle(km[k], fabs(m[k]), (double)fm, 127., 0, 127);
+      kv[k] = aw_settle(kv[k], v[k], (double)fv, 256., 1, 256);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) km[k] = mf[k] < 0.f ? -km[k] : km[k];
   if ((threadIdx.x & 31) == 0) {
-    t.ms[blk] = am;
-    t.vs[blk] = av;
+    t.ms[blk] = fm;
+    t.vs[blk] = fv;
   }
-  if (vec) {
+  if constexpr (VEC) {
     u32x2 a = {0u, 0u}, b = {0u, 0u};
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      a[e >> 2] |= (uint32_t)(cm[e] & 255) << (8 * (e & 3));
-      b[e >> 2] |= (uint32_t)cv[e] << (8 * (e & 3));
+      a[e >> 2] |= (uint32_t)(km[e] & 255) << (8 * (e & 3));
+      b[e >> 2] |= (uint32_t)(kv[e] - 1) << (8 * (e & 3));
     }
     const f32x4 y0 = {p[0], p[1], p[2], p[3]}, y1 = {p[4], p[5], p[6], p[7]};
     if (MASTER) {
@@ -364,8 +382,8 @@ __device__ __forceinline__ void aw_block8(const AwTensor& t, const AwShared& s, 
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       if (k >= left) continue;
-      mc[i + k] = (int8_t)cm[k];
-      vc[i + k] = (uint8_t)cv[k];
+      mc[i + k] = (int8_t)km[k];
+      vc[i + k] = (uint8_t)(kv[k] - 1);
       if (MASTER) t.master[i + k] = p[k];
       if (P32) ((float*)t.p)[i + k] = p[k];
       else ((bf16*)t.p)[i + k] = (bf16)p[k];
@@ -379,7 +397,10 @@ __device__ __forceinline__ void aw_chunk8(const AwTensor& t, const AwShared& s, 
   for (int k = 0; k < AW_CHUNK / 2048; ++k) {
     const int64_t i = i0 + 2048 * k + 8 * tid;
     if (i0 + 2048 * k + (tid / 32) * AW_BLOCK >= t.n) return;  // whole groups of 32 lanes leave
-    aw_block8<P32, G32, MASTER>(t, s, i, (int)min((int64_t)8, t.n - i));  // a lane past the end: no elements
+    // every lane of a block takes the same path: they exchange their largest magnitudes
+    const int64_t end = i0 + 2048 * k + (tid / 32 + 1) * AW_BLOCK;
+    if ((t.flags & AW_ALIGNED) && end <= t.n) aw_block8<P32, G32, MASTER, true>(t, s, i, 8);
+    else aw_block8<P32, G32, MASTER, false>(t, s, i, (int)min((int64_t)8, t.n - i));  // past the end: none
   }
 }
 

@@ -274,3 +274,20 @@ def test_optimizer_and_its_state_dict(gpu, bits):
         masters = [oa.state[p]["master"] for p in a.parameters()]
         for x, y in zip(masters, ps):  # three steps of lr at most 24 u each and |p| roundings, on both sides
             assert ((x - y).abs() <= 2 * 3 * U * (3 * y.abs() + 24 * 2e-2) + 1e-7).all()
+
+
+def test_8bit_scales_half_way_between_two(gpu):
+    """0.9 s + 0.1 g of the largest element often lies exactly between two fp32 scales: the 64-bit operations
+    round in the formula's order, so scales and codes are those of the formula, all of them."""
+    n = 256 * 4000
+    ts = _tensors([n], torch.bfloat16, torch.bfloat16, 8, False, 11, gpu)
+    before = _copy(ts)
+    ops.adamw_step(**ts, step=torch.full((1,), 4, dtype=torch.int64, device=gpu), **HP)
+    g = before["grads"][0].cpu().double()
+    m0 = O.unpack(before["exp_avgs"][0].cpu(), before["exp_avg_scales"][0].cpu())
+    v0 = O.unpack(before["exp_avg_sqs"][0].cpu(), before["exp_avg_sq_scales"][0].cpu())
+    _, m, v = O.adamw(m0, g, m0, v0, 5, 1e-3, HP["betas"], 1e-8, 0.0)
+    for k, x, signed in (("exp_avg", m, True), ("exp_avg_sq", v, False)):
+        codes, scale, _ = O.pack(x, signed)
+        assert (ts[k + "_scales"][0].cpu() != scale).sum() <= 4, k  # of 4000; ties of other codes than the largest
+        assert (ts[k + "s"][0].cpu() != codes).sum() <= 1, k
