@@ -1414,7 +1414,7 @@ def _route_args(name, logits, bias, top_k, score, groups, top_groups, renormaliz
         l2, ld = logits, E
     else:
         l2 = logits.reshape(-1, E)
-        if l2.stride(1) != 1:
+        if l2.stride(1) != 1 or (rows > 1 and l2.stride(0) < E):
             l2 = l2.contiguous()
         ld = l2.stride(0) if rows > 1 else E
     a = _lib.ExpertRouteArgs(l2.data_ptr(), bias.data_ptr() if bias is not None else None, weights, index, dweights, dlogits,
@@ -1611,9 +1611,12 @@ def _dense(t: Optional[Tensor]) -> Optional[Tensor]:
 
 
 def _dense_rows(t: Tensor, cols: int) -> tuple[int, int, int, Tensor]:
-    """``_row_view`` of t, or of a copy where t starts between 16-byte addresses."""
+    """``_row_view`` of t, or of a copy where t starts between 16-byte addresses or its rows overlap
+    (an expanded tensor)."""
     view = _row_view(t, cols)
-    return view if view[1] % 16 == 0 else _row_view(t.clone(memory_format=torch.contiguous_format), cols)
+    if view[1] % 16 == 0 and view[2] >= cols:
+        return view
+    return _row_view(t.clone(memory_format=torch.contiguous_format), cols)
 
 
 def _ptr(t: Optional[Tensor]) -> Optional[int]:

@@ -55,7 +55,7 @@ SHAPES = [
     # tokens, experts, top_k, dim, hidden, out_dim
     (1, 1, 1, 8, 8, 8), (1, 8, 2, 64, 128, 64), (3, 4, 3, 72, 40, 24), (64, 2, 1, 64, 64, 64), (65, 3, 2, 136, 72, 200),
     (130, 5, 2, 64, 264, 64), (200, 24, 3, 104, 56, 96), (300, 2, 2, 128, 256, 128), (513, 3, 1, 264, 136, 520),
-    (700, 4, 2, 96, 640, 96), (40, 64, 4, 32, 48, 32), (1500, 3, 2, 192, 128, 64),
+    (90, 70, 2, 32, 40, 24), (700, 4, 2, 96, 640, 96), (40, 64, 4, 32, 48, 32), (1500, 3, 2, 192, 128, 64),
     # 256 x 256 tiles, several a workgroup, ragged in every direction
     (26000, 3, 2, 264, 328, 296),
 ]
@@ -167,6 +167,21 @@ def test_layouts(gpu):
     out = _call(lead)
     assert tuple(out.shape) == (3, 4, 5, 64)
     _inside(out, want, "leading")
+    # one token for all rows, one residual, one expert's weights for all experts: their gradients are summed
+    d = _to(c, gpu, False)
+    leaves = [d["x"][:1].clone(), d["residual"][:1].clone(), d["w1"][:1].clone(), d["b2"][:1].clone()]
+    for t in leaves:
+        t.requires_grad_()
+    e = dict(d, x=leaves[0].expand(60, 64), residual=leaves[1].expand(60, 64), w1=leaves[2].expand(3, 48, 64), b2=leaves[3].expand(3, 64))
+    f = {n: t.detach().contiguous() for n, t in e.items()}
+    for n in ("x", "residual", "w1", "b2"):
+        f[n].requires_grad_()
+    got = _call(e)
+    assert torch.equal(got, _call(f))
+    ge = torch.autograd.grad(got, leaves, d["dout"])
+    gf = torch.autograd.grad(_call(f), [f[n] for n in ("x", "residual", "w1", "b2")], d["dout"])
+    for a, b in zip(ge, gf):
+        assert torch.equal(a, b.sum(0, keepdim=True))
     d = _to(c, gpu, True)
     ones = torch.ones((), device=gpu).bfloat16().expand(60, 64)
     full = torch.autograd.grad(_call(d), d["w2"], ones.contiguous())[0]
@@ -243,6 +258,36 @@ def test_another_stream_and_graph(gpu):
         again = _call(d)
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(again, want)
+
+
+def test_offsets_past_32_bits(gpu):
+    """2.2e9 hidden values: rows behind the 2^31st element, forward and backward, against the oracle at single
+    tokens and, for the weights' gradients, against one half of the tokens at a time."""
+    T, E, k, C, H, N = 270000, 2, 2, 64, 4096, 64
+    g = torch.Generator(device=gpu).manual_seed(15)
+    r = lambda *s, std=1.0: (torch.randn(*s, generator=g, device=gpu) * std).bfloat16()  # noqa: E731
+    d = dict(x=r(T, C), w1=r(E, H, C, std=C**-0.5), w2=r(E, N, H, std=H**-0.5), b1=r(E, H, std=0.2), b2=r(E, N, std=0.2),
+             residual=None, dout=r(T, N), weights=torch.rand(T, k, generator=g, device=gpu).bfloat16())
+    d["index"] = torch.randint(0, E, (T, k), generator=g, device=gpu, dtype=torch.int32)
+    for n in NAMES[:-1]:
+        d[n].requires_grad_()
+    out = _call(d)
+    names = list(NAMES[:-1])
+    grads = dict(zip(names, torch.autograd.grad(out, [d[n] for n in names], d["dout"])))
+    some = torch.cat([torch.arange(4), torch.randint(0, T, (40,), generator=torch.Generator().manual_seed(1)), torch.arange(T - 4, T)])
+    c = {n: t.detach().cpu() if t is not None else None for n, t in d.items() if n in ("w1", "w2", "b1", "b2")}
+    at = {n: d[n].detach()[some.to(gpu)].cpu() for n in ("x", "weights", "index", "dout")}
+    want = O.mlp_bounds(at["x"], at["weights"], at["index"], c["w1"], c["b1"], c["w2"], c["b2"], None, at["dout"])
+    pick = some.to(gpu)
+    _inside(out[pick], want["out"], "out")
+    for n in ("x", "weights"):
+        _inside(grads[n][pick], want[n], n)
+    parts = []
+    for lo, hi in ((0, T // 2), (T // 2, T)):
+        h = {n: (d[n].detach()[lo:hi] if n in ("x", "weights", "index", "dout") else d[n]) for n in d}
+        parts.append(torch.autograd.grad(_call(h), [d[n] for n in names[2:]], h["dout"]))
+    for n, a, b in zip(names[2:], *parts):  # each side rounded to bf16 once, at random
+        assert rel_l2(grads[n].float(), a.float() + b.float()) <= 2.0**-8, n
 
 
 def test_custom_ops_agree(gpu):

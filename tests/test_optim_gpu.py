@@ -291,3 +291,34 @@ def test_8bit_scales_half_way_between_two(gpu):
         codes, scale, _ = O.pack(x, signed)
         assert (ts[k + "_scales"][0].cpu() != scale).sum() <= 4, k  # of 4000; ties of other codes than the largest
         assert (ts[k + "s"][0].cpu() != codes).sum() <= 1, k
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_offsets_past_32_bits(gpu, bits):
+    """A tensor of 2^31 + 555 elements: its first and last ones against the oracle."""
+    n = 2**31 + 555
+    blocks = -(-n // 256)
+    p, g = (torch.full((n,), v, dtype=torch.bfloat16, device=gpu) for v in (0.5, 0.25))
+    ends = [slice(0, 300), slice(2**31 - 256, n)]
+    gen = torch.Generator().manual_seed(12)
+    for sl in ends:
+        k = p[sl].numel()
+        p[sl], g[sl] = torch.randn(k, generator=gen).to(gpu), torch.randn(k, generator=gen).to(gpu)
+    dt = (torch.int8, torch.uint8) if bits == 8 else (torch.float32,) * 2
+    ts = dict(params=[p], grads=[g], exp_avgs=[torch.zeros(n, dtype=dt[0], device=gpu)],
+              exp_avg_sqs=[torch.zeros(n, dtype=dt[1], device=gpu)])
+    if bits == 8:
+        ts |= {k: [torch.zeros(blocks, device=gpu)] for k in ("exp_avg_scales", "exp_avg_sq_scales")}
+    before = [(p[sl].cpu().double(), g[sl].cpu().double()) for sl in ends]
+    step = torch.zeros(1, dtype=torch.int64, device=gpu)
+    norm = ops.adamw_step(**ts, step=step, max_norm=1e9, **HP)
+    rest = n - sum(b[1].numel() for b in before)
+    want = math.sqrt(rest * 0.0625 + sum(float((b[1] ** 2).sum()) for b in before))
+    assert abs(float(norm) - want) <= 1e-12 * want
+    for sl, (p0, g0) in zip(ends, before):
+        new, m, v = O.adamw(p0, g0, 0 * p0, 0 * p0, 1, HP["lr"], HP["betas"], HP["eps"], HP["weight_decay"])
+        got = p[sl].cpu().double()
+        assert ((got - new).abs() <= U * (3 * p0.abs() + 24 * HP["lr"]) + 2.0**-8 * new.abs()).all()
+        if bits == 32:
+            assert ((ts["exp_avgs"][0][sl].cpu().double() - m).abs() <= 8 * U * m.abs() + 1e-44).all()
+    assert float(p[2**30]) == float(p[1000])

@@ -103,6 +103,11 @@ def test_route_layouts_and_leading_dims(gpu):
         assert tuple(w.shape) == (*v.shape[:-1], 4)
         assert torch.equal(i.cpu().view(-1, 4), want[1])
         assert (w.cpu().double().view(-1, 4) - want[0]).abs().max() <= 100 * U
+    row = l[:1].to(gpu).expand(5, 24)
+    w, i = ops.expert_route(row, 4)
+    assert torch.equal(i.cpu(), want[1][:1].expand(5, 4))
+    w, i = ops.expert_route(l[0].to(gpu), 4)
+    assert i.cpu().tolist() == want[1][0].tolist()
     w, i = ops.expert_route(torch.zeros(0, 3, 8, device=gpu), 2)
     assert tuple(w.shape) == tuple(i.shape) == (0, 3, 2)
 
