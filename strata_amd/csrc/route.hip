@@ -249,7 +249,7 @@ __device__ __forceinline__ bool route_choose(const RouteParams& p, const float (
 
 template <typename T, bool WIDE, bool VEC, int EPL, int L>
 __global__ __launch_bounds__(256) void route_kernel(RouteParams p) {
-  constexpr int TOK = 256 / L;
+  const int TOK = (int)blockDim.x / L;
   extern __shared__ char smem[];  // a token: [top_k] scores, [top_k] experts; with groups the choice's scratch
   const int tid = threadIdx.x, lane = tid % L, tok = tid / L;
   const int64_t t = (int64_t)blockIdx.x * TOK + tok;
@@ -647,12 +647,21 @@ extern "C" int strata_hip_expert_route(const strata_hip_expert_route_args* a, vo
   if (!p.logits || !p.weights || !p.index) return fail(STRATA_HIP_EINVAL, "expert_route: null pointer");
   const bool wide = p.bias || p.groups > 1, vec = route_aligned(a, p.bias) && (p.ld % 4) == 0;
   return route_width(p.experts, [&](auto epl, auto l) {
-    constexpr int EPL = decltype(epl)::value, L = decltype(l)::value, TOK = 256 / L;
-    const dim3 grid((unsigned)((p.tokens + TOK - 1) / TOK));
-    size_t smem = ((size_t)TOK * p.top_k * 8 + 15) & ~(size_t)15;
-    if (p.groups > 1) smem += (size_t)TOK * (EPL * L + 2 * p.groups) * 8;
+    constexpr int EPL = decltype(epl)::value, L = decltype(l)::value;
+    auto lds = [&](int threads) {
+      const size_t tok = threads / L;
+      return ((tok * p.top_k * 8 + 15) & ~(size_t)15) + (p.groups > 1 ? tok * (EPL * L + 2 * p.groups) * 8 : 0);
+    };
+    // The scratch of a choice in groups is up to 12 KiB a token: fewer tokens a workgroup where it passes
+    // 64 KiB (waves do not work together).  At 32 threads, four tokens of 512 experts, it is at most 50 KiB.
+    int threads = 256;
+    while (threads > 32 && lds(threads) > 65536) threads /= 2;
+    const size_t smem = lds(threads);
+    const int64_t tok = threads / L, wgs = (p.tokens + tok - 1) / tok;
+    if (smem > 65536 || wgs * threads >= 0x100000000ll) return fail(STRATA_HIP_EUNSUPPORTED, "expert_route: problem too large for one launch");
+    const dim3 grid((unsigned)wgs);
     auto go = [&](auto t, auto w, auto v) {
-      hipLaunchKernelGGL((route_kernel<decltype(t), decltype(w)::value, decltype(v)::value, EPL, L>), grid, dim3(256), smem,
+      hipLaunchKernelGGL((route_kernel<decltype(t), decltype(w)::value, decltype(v)::value, EPL, L>), grid, dim3(threads), smem,
                          (hipStream_t)stream, p);
     };
     auto with = [&](auto t, auto w) {
@@ -679,7 +688,9 @@ extern "C" int strata_hip_expert_route_bwd(const strata_hip_expert_route_args* a
   const bool vec = route_aligned(a, p.bias) && (p.ld % 4) == 0 && ((uintptr_t)p.dlogits & 15) == 0;
   return route_width(p.experts, [&](auto epl, auto l) {
     constexpr int EPL = decltype(epl)::value, L = decltype(l)::value, TOK = 256 / L;
-    const dim3 grid((unsigned)((p.tokens + TOK - 1) / TOK));
+    const int64_t wgs = (p.tokens + TOK - 1) / TOK;
+    if (wgs * 256 >= 0x100000000ll) return fail(STRATA_HIP_EUNSUPPORTED, "expert_route_bwd: problem too large for one launch");
+    const dim3 grid((unsigned)wgs);
     auto go = [&](auto t, auto v) {
       hipLaunchKernelGGL((route_bwd_kernel<decltype(t), decltype(v)::value, EPL, L>), grid, dim3(256), (size_t)TOK * EPL * L * 4,
                          (hipStream_t)stream, p);

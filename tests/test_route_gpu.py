@@ -81,6 +81,15 @@ def test_route_bias_and_groups(gpu, T, E, k, groups, top, with_bias, dtype):
         _check(lm, kw, got, dtype)
 
 
+@pytest.mark.parametrize("T,E,k,groups,top", [(70, 512, 16, 64, 8), (37, 512, 64, 512, 100), (75, 256, 8, 8, 4), (66, 320, 6, 160, 9)])
+def test_route_many_experts_in_groups(gpu, T, E, k, groups, top):
+    """Every token of a workgroup whose scratch is at its largest."""
+    print(f"route {T} {E} {k} groups {groups}/{top}", flush=True)
+    l = _logits(T, E, torch.float32, 8)
+    kw = dict(top_k=k, score="sigmoid", bias=torch.randn(E, generator=torch.Generator().manual_seed(3)), groups=groups, top_groups=top)
+    _check(l, kw, ops.expert_route(l.to(gpu), **dict(kw, bias=kw["bias"].to(gpu))), torch.float32)
+
+
 def test_route_near_ties_are_told_apart(gpu):
     """Keys s + bias whose difference a 32-bit sum loses: 64 bits choose, in either order."""
     l = torch.zeros(2, 8)
