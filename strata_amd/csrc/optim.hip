@@ -31,6 +31,7 @@ constexpr int AW_CHUNK = 4096;   // elements per workgroup of the step
 constexpr int AW_SUM = 16384;    // elements per workgroup of the sum of squares
 constexpr int AW_HEAD = 8;       // doubles before the partial sums
 constexpr int AW_PER = 48;       // tensors per launch: 80 bytes each in 4 KiB of arguments
+constexpr float AW_TINY = 0x1p-100f;  // 8-bit scales under it are places in 64 bits: the factor 65536 / scale leaves 32
 enum { AW_P32 = 1, AW_G32 = 2, AW_ALIGNED = 4 };
 
 struct AwTensor {
@@ -345,7 +346,13 @@ __device__ __forceinline__ void aw_block8(const AwTensor& t, const AwShared& s, 
     km[k] = (int)fminf(ra, 127.f);  // a block whose scale is no number or infinite: any code
     kv[k] = (int)fminf(rb, 256.f);
   }
-  if (dev > 0.49992f) {
+  if ((fm < AW_TINY && fm > 0.f) || (fv < AW_TINY && fv > 0.f)) {  // the same for a block's lanes
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      km[k] = fm > 0.f ? (int)fmin(rint(sqrt(fabs(m[k]) * 16129. / (double)fm)), 127.) : 0;
+      kv[k] = fv > 0.f ? (int)fmin(fmax(rint(sqrt(v[k] * 65536. / (double)fv)), 1.), 256.) : 1;
+    }
+  } else if (dev > 0.49992f) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       km[k] = aw_settle(km[k], fabs(m[k]), (double)fm, 127., 0, 127);
@@ -484,8 +491,10 @@ static int aw_check(const strata_hip_adamw_args* a) {
     return fail(STRATA_HIP_EINVAL, "adamw_step: eps must be finite and not negative");
   if (!std::isfinite(a->max_norm) || (a->max_norm > 0. && (!a->norm || ((uintptr_t)a->norm & 7))))
     return fail(STRATA_HIP_EINVAL, "adamw_step: max_norm must be finite and norm given with it, 8-byte aligned");
-  std::vector<std::pair<uintptr_t, uintptr_t>> written;
-  written.reserve((size_t)a->count * 6);
+  std::vector<std::pair<uintptr_t, uintptr_t>> written, read;
+  written.reserve((size_t)a->count * 6 + 1);
+  read.reserve((size_t)a->count);
+  written.emplace_back((uintptr_t)a->step, (uintptr_t)a->step + 8);
   int64_t chunks = 0;
   for (int64_t i = 0; i < a->count; ++i) {
     const strata_hip_adamw_tensor& t = a->tensors[i];
@@ -506,6 +515,7 @@ static int aw_check(const strata_hip_adamw_args* a) {
         ((uintptr_t)t.master % 4) || ((uintptr_t)t.exp_avg_scale % 4) || ((uintptr_t)t.exp_avg_sq_scale % 4))
       return fail(STRATA_HIP_EINVAL, "adamw_step: a tensor is not aligned to its elements");
     auto add = [&](const void* p, uintptr_t bytes) { written.emplace_back((uintptr_t)p, (uintptr_t)p + bytes); };
+    read.emplace_back((uintptr_t)t.grad, (uintptr_t)t.grad + gs * t.n);
     add(t.param, ps * t.n);
     add(t.exp_avg, ss * t.n);
     add(t.exp_avg_sq, ss * t.n);
@@ -516,11 +526,16 @@ static int aw_check(const strata_hip_adamw_args* a) {
     }
     chunks += (t.n + AW_CHUNK - 1) / AW_CHUNK;
   }
-  if (chunks > 0x7fffffff) return fail(STRATA_HIP_EUNSUPPORTED, "adamw_step: too many elements for one call");
+  if (chunks > 0xffffff) return fail(STRATA_HIP_EUNSUPPORTED, "adamw_step: too many elements for one call");
   std::sort(written.begin(), written.end());
   for (size_t i = 1; i < written.size(); ++i)
     if (written[i].first < written[i - 1].second)
       return fail(STRATA_HIP_EINVAL, "adamw_step: two of the tensors to update overlap");
+  for (const auto& r : read) {  // the ranges written are disjoint: the last one that starts before r ends
+    auto w = std::lower_bound(written.begin(), written.end(), std::make_pair(r.second, (uintptr_t)0));
+    if (w != written.begin() && (--w)->second > r.first)
+      return fail(STRATA_HIP_EINVAL, "adamw_step: a gradient overlaps a tensor to update");
+  }
   return STRATA_HIP_OK;
 }
 
@@ -625,7 +640,7 @@ extern "C" int strata_hip_adamw_state_values(const strata_hip_adamw_values_args*
   if (((uintptr_t)a->codes & 3) || ((uintptr_t)a->scales & 3) || ((uintptr_t)a->out & 15))
     return fail(STRATA_HIP_EINVAL, "adamw_state_values: codes must be 4-byte, out 16-byte aligned");
   const int64_t wgs = (a->n + 1023) / 1024;
-  if (wgs > 0x7fffffff) return fail(STRATA_HIP_EUNSUPPORTED, "adamw_state_values: too many elements for one call");
+  if (wgs > 0xffffff) return fail(STRATA_HIP_EUNSUPPORTED, "adamw_state_values: too many elements for one call");
   hipLaunchKernelGGL(aw_values_kernel, dim3((unsigned)wgs), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)a->codes,
                      a->scales, a->out, a->n, a->is_signed);
   return check_launch("adamw state values");

@@ -47,6 +47,16 @@ def test_c_entry_refuses(lib, over, tensor, second, msg):
     assert rc == _lib.EINVAL and msg in err
 
 
+@pytest.mark.parametrize("tensor,second,msg", [
+    (dict(grad=0x100000), {}, "gradient"), (dict(grad=0x1000c6), {}, "gradient"), ({}, dict(grad=0x130000), "gradient"),
+    (dict(grad=0x12018e), {}, "gradient"), (dict(param=0x1000), {}, "overlap"), (dict(exp_avg=0x1004), {}, "overlap"),
+])
+def test_c_entry_refuses_what_another_tensor_holds(lib, tensor, second, msg):
+    """A gradient, which other workgroups read than those that write, and the step count."""
+    rc, err = _call(lib, {}, tensor, second)
+    assert rc == _lib.EINVAL and msg in err
+
+
 def test_workspace(lib):
     t = (_lib.AdamwTensor * 3)()
     for i, n in enumerate((1, 16385, 0)):

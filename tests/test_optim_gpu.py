@@ -74,7 +74,8 @@ def _check(ts, before, t, coef, hp=HP, lrs=None, wds=None):
         b1, b2 = hp["betas"]
         p, m, v = O.adamw(base, g, m0, v0, t, lr, hp["betas"], hp["eps"], wd, coef)
         big = lr / (1 - b1**t) * (b1 * m0.abs() + (1 - b1) * (g * coef).abs()) / ((v / (1 - b2**t)).sqrt() + hp["eps"])
-        tol = U * (3 * base.abs() + 24 * big) + 1e-44
+        # a v under 2^-126 is rounded to a multiple of 2^-149: off by 2^-150, relative to v twice what its root is off by
+        tol = U * (3 * base.abs() + 24 * big) + big * torch.where(v < 2.0**-126, 2.0**-150 / v.clamp_min(1e-300), 0.0) + 1e-44
         if master is not None:
             got = ts["masters"][i].cpu().double()
             assert ((got - p).abs() <= tol).all(), i
@@ -291,6 +292,19 @@ def test_8bit_scales_half_way_between_two(gpu):
         codes, scale, _ = O.pack(x, signed)
         assert (ts[k + "_scales"][0].cpu() != scale).sum() <= 4, k  # of 4000; ties of other codes than the largest
         assert (ts[k + "s"][0].cpu() != codes).sum() <= 1, k
+
+
+@pytest.mark.parametrize("size,eps", [(1e-16, 1e-20), (1e-30, 1e-8)])
+def test_8bit_codes_of_tiny_gradients(gpu, size, eps):
+    """Blocks whose largest moment is so small that 65536 over it leaves fp32."""
+    hp = dict(HP, eps=eps)
+    ts = _tensors([3, 256, 1300], torch.float32, torch.float32, 8, False, 21, gpu, zero=True)
+    ts["grads"] = [g * size for g in ts["grads"]]
+    step = torch.zeros(1, dtype=torch.int64, device=gpu)
+    before = _copy(ts)
+    ops.adamw_step(**ts, step=step, **hp)
+    _check(ts, before, 1, 1.0, hp)
+    assert not any(ts["exp_avgs"][i][ts["grads"][i] == 0].any() for i in range(3))
 
 
 @pytest.mark.parametrize("bits", [32, 8])
