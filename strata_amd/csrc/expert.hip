@@ -538,11 +538,11 @@ __global__ __launch_bounds__(256) void expert_combine_kernel(ExpertCombine p) {
   *(u32x4*)(p.out + i * 8) = (u32x4){pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]), pack_bf16x2(a[4], a[5]), pack_bf16x2(a[6], a[7])};
 }
 
-// ---- dw = <g[t], y_r> / w'; a wave a pair ----
+// ---- dw = <g[t], y_r> / w'; a wave a pair (`pair0`: the launch's first one) ----
 __global__ __launch_bounds__(256) void expert_dweight_kernel(const bf16* g, const float* yy, const bf16* weights,
-                                                             const int32_t* slot_row, bf16* dw, int64_t pairs, int top_k,
-                                                             int N) {
-  const int64_t s = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+                                                             const int32_t* slot_row, bf16* dw, int64_t pair0, int64_t pairs,
+                                                             int top_k, int N) {
+  const int64_t s = pair0 + (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   if (s >= pairs) return;
   const int r = slot_row[s];
@@ -795,7 +795,9 @@ template <int MODE, bool WT>
 static int launch_expert_gemm(ExpertGemm p, int64_t pairs, int experts, int tile, hipStream_t st) {
   p.nt = (p.N + tile - 1) / tile;
   const int64_t mt = pairs / tile + std::min<int64_t>(experts, pairs), total = mt * p.nt;
-  if (total > 0x7fffffff) return fail(STRATA_HIP_EUNSUPPORTED, "expert_mlp: problem too large for one launch");
+  // 2^32 threads a launch (a grid of 256 x 256 tiles is not larger than the chip)
+  if (total > 0x7fffffff || (tile != 256 && total * (tile == 16 ? 1024 : tile == 64 ? 256 : 512) >= 0x100000000ll))
+    return fail(STRATA_HIP_EUNSUPPORTED, "expert_mlp: problem too large for one launch");
   if constexpr (!WT && MODE != EX_HIDDEN_GRAD) {
     if (tile == 16) {
       if (p.K > 1024)
@@ -829,7 +831,7 @@ static int launch_wgrad(ExpertWgrad p, hipStream_t st) {
   p.nt = (p.N + 255) / 256;
   p.kt = (p.K + 255) / 256;
   const int64_t total = (int64_t)p.nt * p.kt * p.experts;
-  if (total > 0x7fffffff) return fail(STRATA_HIP_EUNSUPPORTED, "expert_mlp_bwd: problem too large for one launch");
+  if (total * 512 >= 0x100000000ll) return fail(STRATA_HIP_EUNSUPPORTED, "expert_mlp_bwd: problem too large for one launch");
   hipLaunchKernelGGL(expert_wgrad_kernel<OF_G>, dim3((unsigned)total), dim3(512), 0, st, p);
   return check_launch("expert_wgrad_kernel");
 }
@@ -837,7 +839,7 @@ static int launch_wgrad(ExpertWgrad p, hipStream_t st) {
 static int launch_combine(ExpertCombine c, int64_t tokens, int width, hipStream_t st) {
   c.chunks = width / 8;
   c.n = tokens * c.chunks;
-  if (c.n > 0x7fffffffll * 256) return fail(STRATA_HIP_EUNSUPPORTED, "expert_mlp: problem too large for one launch");
+  if (c.n >= 0xffffff00ll) return fail(STRATA_HIP_EUNSUPPORTED, "expert_mlp: problem too large for one launch");
   hipLaunchKernelGGL(expert_combine_kernel, dim3((unsigned)((c.n + 255) / 256)), dim3(256), 0, st, c);
   return check_launch("expert_combine_kernel");
 }
@@ -853,8 +855,8 @@ static int expert_check(const std::string& name, const strata_hip_expert_mlp_arg
     return fail(STRATA_HIP_EUNSUPPORTED, name + ": at most 512 experts, widths 32768 and 2^31 pairs");
   if (pairs > 0 && a->tile != expert_tile(a)) return fail(STRATA_HIP_EINVAL, name + ": tile is not strata_hip_expert_tile()'s");
   if (!a->w1 || !a->w2 || !a->offsets || !a->tiles) return fail(STRATA_HIP_EINVAL, name + ": null pointer");
-  if (((uintptr_t)a->w1 & 15) || ((uintptr_t)a->w2 & 15) || ((uintptr_t)a->b1 & 7) || ((uintptr_t)a->b2 & 7))
-    return fail(STRATA_HIP_EINVAL, name + ": weights must be 16-byte, biases 8-byte aligned");
+  if (((uintptr_t)a->w1 & 15) || ((uintptr_t)a->w2 & 15) || ((uintptr_t)a->b1 & 15) || ((uintptr_t)a->b2 & 15))
+    return fail(STRATA_HIP_EINVAL, name + ": weights and biases must be 16-byte aligned");
   if (pairs == 0) return STRATA_HIP_OK;
   if (!a->dact && name != "expert_mlp") return fail(STRATA_HIP_EINVAL, name + ": dact is needed");
   if (!a->x || !a->weights || !a->row_token || !a->row_weight || !a->slot_row || !a->h || !a->y)
@@ -936,9 +938,13 @@ extern "C" int strata_hip_expert_mlp_bwd(const strata_hip_expert_mlp_bwd_args* b
   for (const void* q : all)
     if ((uintptr_t)q & 15) return fail(STRATA_HIP_EINVAL, name + ": workspaces and gradients must be 16-byte aligned");
   if (pairs > 0 && b->dweights) {
-    hipLaunchKernelGGL(expert_dweight_kernel, dim3((unsigned)((pairs + 3) / 4)), dim3(256), 0, st, (const bf16*)b->dout, a->y,
-                       (const bf16*)a->weights, a->slot_row, (bf16*)b->dweights, pairs, a->top_k, a->out_dim);
-    if (const int rc = check_launch("expert_dweight_kernel")) return rc;
+    constexpr int64_t MOST = 1ll << 25;  // pairs a launch: 2^31 threads
+    for (int64_t p0 = 0; p0 < pairs; p0 += MOST) {
+      hipLaunchKernelGGL(expert_dweight_kernel, dim3((unsigned)((std::min(pairs - p0, MOST) + 3) / 4)), dim3(256), 0, st,
+                         (const bf16*)b->dout, a->y, (const bf16*)a->weights, a->slot_row, (bf16*)b->dweights, p0, pairs, a->top_k,
+                         a->out_dim);
+      if (const int rc = check_launch("expert_dweight_kernel")) return rc;
+    }
   }
   ExpertWgrad w = {};
   w.token = a->row_token;

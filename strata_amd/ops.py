@@ -1751,14 +1751,25 @@ def _expert_backward(dout, x, weights, w1, b1, w2, b2, space, need):
 def expert_mlp_bwd(dout: Tensor, x: Tensor, weights: Tensor, w1: Tensor, b1: Optional[Tensor], w2: Tensor,
                    b2: Optional[Tensor], space: Tensor, need: Sequence[bool]) -> list[Tensor]:
     """Gradients of ``expert_mlp_train`` at ``(x, weights, w1, b1, w2, b2)``, an empty tensor where
-    ``need`` asks for none (a bias's comes from its weight's launch)."""
+    ``need`` asks for none (a bias's comes from its weight's launch).  ``space``: as
+    ``expert_mlp_train`` returned it for the same weights and index."""
+    name = "expert_mlp_bwd"
+    if w1.dim() != 3 or w2.dim() != 3 or weights.dim() < 1 or len(need) != 6:
+        raise ValueError(f"{name}: w1 [E, H, C], w2 [E, N, H], weights [..., top_k] and six answers in need expected")
+    # the index is in the plan: one of the weights' shape stands for it
+    _expert_check(name, x, weights, torch.empty_like(weights, dtype=torch.int32), w1, b1, w2, b2, None)
+    if dout.dtype != torch.bfloat16 or tuple(dout.shape) != (*x.shape[:-1], w2.shape[1]) or dout.get_device() != x.get_device():
+        raise ValueError(f"{name}: dout must be bfloat16 {(*x.shape[:-1], w2.shape[1])} on x's GPU, got {dout.dtype} {tuple(dout.shape)}")
+    size = _expert_space(weights.numel(), *w1.shape[:2], w2.shape[1], _expert_tile(weights.numel(), w1, w2, True), True)[4]
+    if space.dtype != torch.uint8 or space.numel() != size or not space.is_contiguous() or space.get_device() != x.get_device():
+        raise ValueError(f"{name}: space must be the {size} bytes of expert_mlp_train, got {space.dtype} {tuple(space.shape)}")
     grads = _expert_backward(dout, x, weights, w1, b1, w2, b2, space, need)
     return [g if g is not None else x.new_empty(0) for g in grads]
 
 
 @expert_mlp_bwd.register_fake
 def _(dout, x, weights, w1, b1, w2, b2, space, need):
-    return [torch.empty_like(t) if t is not None and wanted else x.new_empty(0)
+    return [t.new_empty(t.shape) if t is not None and wanted else x.new_empty(0)
             for t, wanted in zip((x, weights, w1, b1, w2, b2), need)]
 
 

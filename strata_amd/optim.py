@@ -28,7 +28,11 @@ class AdamW(torch.optim.Optimizer):
 
     ``lr`` and ``weight_decay`` may differ between parameter groups, ``betas`` and ``eps`` are
     the optimizer's.  One step count on the GPU serves every parameter: a step can be captured in
-    a graph (after one eager step has made the states)."""
+    a graph (after one eager step has made the states; the rates are those of the capture).
+
+    A master weight stands for its parameter once it exists, at the first step: a value written
+    into the parameter later (loaded weights, an average) goes into ``state[p]["master"]`` too, or
+    the next step takes it back."""
 
     def __init__(self, params, lr: float = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, state_bits: int = 32, master: bool = True,
@@ -43,6 +47,10 @@ class AdamW(torch.optim.Optimizer):
         self.betas, self.eps, self.max_norm = (float(betas[0]), float(betas[1])), float(eps), max_norm
         self.state_bits, self.master, self.min_8bit = state_bits, master, int(min_8bit)
         self.grad_norm: Optional[Tensor] = None
+
+    def __getstate__(self) -> dict:  # copies and pickles: torch's own keeps the groups and states alone
+        own = ("betas", "eps", "max_norm", "state_bits", "master", "min_8bit", "grad_norm")
+        return {**super().__getstate__(), **{k: self.__dict__[k] for k in own}}
 
     def add_param_group(self, group) -> None:
         for k in ("betas", "eps", "max_norm"):

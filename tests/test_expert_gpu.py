@@ -311,6 +311,55 @@ def test_custom_ops_agree(gpu):
     assert torch.equal(torch.autograd.grad(a[0], l, g)[0], torch.autograd.grad(b[0], l, g)[0])
 
 
+def test_traced_by_a_compiler(gpu):
+    """Forward and backward through torch.compile, x and w1 as transposed views."""
+    d = _to(_case(90, 4, 2, 64, 72, 64, 14), gpu, False)
+    d["x"] = d["x"].t().contiguous().t()
+    d["w1"] = d["w1"].transpose(1, 2).contiguous().transpose(1, 2)
+    for n in NAMES:
+        d[n].requires_grad_()
+    args = [d[n] for n in ("x", "weights", "index", "w1", "b1", "w2", "b2", "residual")]
+    want = ops.expert_mlp(*args)
+    got = torch.compile(lambda *a: ops.expert_mlp(*a), backend="aot_eager", fullgraph=True)(*args)
+    assert torch.equal(got, want)
+    for x, y in zip(torch.autograd.grad(got, [d[n] for n in NAMES], d["dout"]), torch.autograd.grad(want, [d[n] for n in NAMES], d["dout"])):
+        assert torch.equal(x, y)
+
+
+def test_two_streams_at_once(gpu):
+    """Two calls in flight with different choices: each has its own workspace."""
+    cases = [_to(_case(2000, 8, 2, 128, 256, 128, s), gpu, True) for s in (15, 16)]
+
+    def run(d):
+        out = _call(d)
+        return [out.detach(), *torch.autograd.grad(out, [d[n] for n in NAMES], d["dout"])]
+
+    want = [run(d) for d in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(4):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(run(cases[i]))
+    torch.cuda.synchronize()
+    for w, g in zip(want, got):
+        for r in g:
+            assert all(torch.equal(a, b) for a, b in zip(w, r))
+
+
+def test_backward_op_refuses(gpu):
+    d = _to(_case(8, 3, 2, 16, 24, 16, 11), gpu, False)
+    out, space = torch.ops.strata_hip.expert_mlp_train(*(d[n] for n in ("x", "weights", "index", "w1", "b1", "w2", "b2", "residual")))
+    a = dict(dout=d["dout"], x=d["x"], weights=d["weights"], w1=d["w1"], b1=d["b1"], w2=d["w2"], b2=d["b2"], space=space, need=[True] * 6)
+    assert all(t.numel() for t in torch.ops.strata_hip.expert_mlp_bwd(**a))
+    for over, msg in ((dict(dout=d["dout"][:4]), "dout"), (dict(dout=d["dout"].float()), "dout"), (dict(space=space[:-4]), "space"),
+                      (dict(space=space.view(torch.int32)), "space"), (dict(need=[True]), "need"), (dict(x=d["x"][:7]), "top_k"),
+                      (dict(w1=d["w1"][:2]), "E, H"), (dict(weights=d["weights"].float()), "bfloat16")):
+        with pytest.raises(ValueError, match=msg):
+            torch.ops.strata_hip.expert_mlp_bwd(**dict(a, **over))
+
+
 def test_refusals(gpu):
     c = _to(_case(8, 3, 2, 16, 24, 16, 11), gpu, False)
     for over, msg in ((dict(x=c["x"].float()), "bfloat16"), (dict(index=c["index"].long()), "int32"),

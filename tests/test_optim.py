@@ -102,3 +102,16 @@ def test_codes_are_the_nearest():
         assert ((r.clamp(min=low) - q).abs() <= 0.5 + 1e-4).all()
         if signed:
             assert (back[y == 0] == 0).all() and (back.sign() * y.sign() >= 0).all()
+
+
+def test_copies_and_pickles():
+    import copy
+    import pickle
+
+    p = torch.nn.Parameter(torch.zeros(8))
+    opt = AdamW([p], lr=0.5, betas=(0.8, 0.9), eps=1e-6, max_norm=2.0, state_bits=8, master=False, min_8bit=16)
+    opt.state[p] = opt._new_state(p, torch.ones(1, dtype=torch.int64))
+    for o in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        assert (o.betas, o.eps, o.max_norm, o.state_bits, o.master, o.min_8bit) == ((0.8, 0.9), 1e-6, 2.0, 8, False, 16)
+        q = o.param_groups[0]["params"][0]
+        assert o.param_groups[0]["lr"] == 0.5 and int(o.state[q]["step"]) == 1 and o.grad_norm is None

@@ -3,6 +3,8 @@ the operators without a GPU."""
 
 import ctypes
 import math
+import subprocess
+from pathlib import Path
 
 import pytest
 import torch
@@ -189,3 +191,51 @@ def test_expert_modules_without_a_gpu():
         ExpertMlp(64, 64, 4, score="tanh")
     assert [n for n, _ in StrataBlock(64, 1, (3, 3, 3)).named_parameters()][4:] == [
         "mlp.layers.0.weight", "mlp.layers.0.bias", "mlp.layers.2.weight", "mlp.layers.2.bias"]
+
+
+def test_traced_shapes():
+    """The custom ops under fake tensors: shapes, types and strides of what the kernels write."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        e = lambda *s, dtype=torch.bfloat16: torch.empty(*s, dtype=dtype, device="cuda")  # noqa: E731
+        w, i = ops.expert_route(e(5, 7, 8, dtype=torch.float32), 2)
+        assert w.shape == i.shape == (5, 7, 2) and (w.dtype, i.dtype) == (torch.float32, torch.int32)
+        assert torch.ops.strata_hip.expert_route_bwd(w, e(5, 7, 8, dtype=torch.float32), i, 2, "softmax", None, True, 1.0).shape == (5, 7, 8)
+        x, wt = e(7, 5, 64).transpose(0, 1), e(5, 7, 2)
+        w1, w2 = e(4, 64, 96).transpose(1, 2), e(4, 32, 96)
+        out = ops.expert_mlp(x, wt, i, w1, None, w2, e(4, 32))
+        assert out.shape == (5, 7, 32) and out.dtype == torch.bfloat16
+        out, space = torch.ops.strata_hip.expert_mlp_train(x, wt, i, w1, None, w2, e(4, 32), None)
+        tile = ops._expert_tile(70, w1, w2, True)
+        assert out.shape == (5, 7, 32) and space.dtype == torch.uint8 and space.numel() == ops._expert_space(70, 4, 96, 32, tile, True)[4]
+        need = [True, False, True, False, True, True]
+        g = torch.ops.strata_hip.expert_mlp_bwd(out, x, wt, w1, None, w2, e(4, 32), space, need)
+        assert [tuple(t.shape) for t in g] == [(5, 7, 64), (0,), (4, 96, 64), (0,), (4, 32, 96), (4, 32)]
+        assert all(t.is_contiguous() for t in g)
+        v = ops.adamw_state_values(e(300, dtype=torch.int8), e(2, dtype=torch.float32))
+        assert v.shape == (300,) and v.dtype == torch.float32
+
+
+STRUCTS = {"strata_hip_expert_route_args": _lib.ExpertRouteArgs, "strata_hip_expert_plan_args": _lib.ExpertPlanArgs,
+           "strata_hip_expert_mlp_args": _lib.ExpertMlpArgs, "strata_hip_expert_mlp_bwd_args": _lib.ExpertMlpBwdArgs,
+           "strata_hip_adamw_tensor": _lib.AdamwTensor, "strata_hip_adamw_args": _lib.AdamwArgs,
+           "strata_hip_adamw_values_args": _lib.AdamwValuesArgs}
+
+
+def test_struct_layouts_are_the_header_s(tmp_path):
+    """Every field's offset and every structure's size, as a C compiler lays the header out."""
+    header = Path(_lib.__file__).resolve().parents[1] / "include" / "strata_hip.h"
+    lines = [f'#include "{header}"', "#include <stddef.h>", "#include <stdio.h>", "int main(void) {"]
+    want = []
+    for name, st in STRUCTS.items():
+        lines.append(f'  printf("%zu\\n", sizeof({name}));')
+        want.append(ctypes.sizeof(st))
+        for f, _ in st._fields_:
+            lines.append(f'  printf("%zu\\n", offsetof({name}, {f}));')
+            want.append(getattr(st, f).offset)
+    src = tmp_path / "layout.c"
+    src.write_text("\n".join(lines + ["  return 0;", "}"]))
+    subprocess.run(["gcc", "-o", str(tmp_path / "layout"), str(src)], check=True)
+    got = subprocess.run([str(tmp_path / "layout")], check=True, capture_output=True, text=True).stdout.split()
+    assert [int(x) for x in got] == want
