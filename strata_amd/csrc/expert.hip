@@ -768,11 +768,16 @@ __global__ __launch_bounds__(512, 1) void expert_wgrad_kernel(ExpertWgrad p) {
 #endif
 }
 
-// Rows of a tile: 16 for fewer than 16 rows an expert without a backward, 256 where the products fill
-// the chip with 256 x 256 tiles, 64 where an expert has fewer than 192 rows on average, else 128.
+// Rows of a tile, by an expert's average rows.  Times of a whole forward replayed, us; E experts, C -> H -> C:
+//   under 4 without a backward: 16, few-rows kernel (8 pairs, E 8, 1024 -> 4096: 36 against 42 with 64;
+//     at 4 an expert 41 / 45, but E 32, 512 -> 1024 32 / 30; at 12 an expert 50 / 47);
+//   under 144: 64 (125 an expert, E 16, 768 -> 1536: 53 against 56 with 128; at 150 an expert 67 / 62;
+//     112, E 24, 384 -> 776: 47 / 51);
+//   256 where an expert has two such tiles and they fill the chip (2048 an expert, E 8, 1024 -> 2048:
+//     217 against 240 with 128; half of that 141 / 148; 1024 an expert, E 32, 512 -> 1024 150 / 154); else 128.
 static int expert_tile(int64_t pairs, int experts, int64_t width, bool train) {
-  if (!train && pairs < 16 * (int64_t)experts) return 16;
-  if (pairs < 192 * (int64_t)experts) return 64;
+  if (!train && pairs < 4 * (int64_t)experts) return 16;
+  if (pairs < 144 * (int64_t)experts) return 64;
   return pairs >= 512 * (int64_t)experts && (pairs / 256) * ((width + 255) / 256) >= 200 ? 256 : 128;
 }
 static int expert_tile(const strata_hip_expert_mlp_args* a) {
@@ -800,6 +805,8 @@ static int launch_expert_gemm(ExpertGemm p, int64_t pairs, int experts, int tile
     return fail(STRATA_HIP_EUNSUPPORTED, "expert_mlp: problem too large for one launch");
   if constexpr (!WT && MODE != EX_HIDDEN_GRAD) {
     if (tile == 16) {
+      // 16 waves a workgroup for a long contraction: one token, 1024 -> 4096 24.8 us against 26.0 with 4
+      // throughout (and 25.8 with 16 throughout); four tokens, 1024 -> 2048 28.5 against 27.5.
       if (p.K > 1024)
         hipLaunchKernelGGL((expert_few_kernel<MODE, 16>), dim3((unsigned)total), dim3(1024), 0, st, p);
       else

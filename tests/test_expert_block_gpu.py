@@ -8,6 +8,8 @@ gradient also takes the rounding of its logits (2^-8 |l|, |l| up to 3, in the we
 weights' gradient and of its own: 1.2e-2 + 3 x 2^-8 + 0.3e-2 = 2.6e-2: 4e-2.
 """
 
+import copy
+
 import pytest
 import torch
 import torch.nn.functional as F
@@ -16,6 +18,7 @@ from oracle import block as OB
 from oracle import experts as OE
 from oracle import optim as OO
 from oracle import rope as R
+from strata_amd import ops
 from strata_amd import rope as P
 from strata_amd.modules import ExpertMlp, StrataBlock, init_xavier_
 from strata_amd.optim import AdamW
@@ -133,6 +136,48 @@ def test_expert_mlp_served_from_a_graph(gpu):
                 want = mlp(x, res)
                 torch.cuda.synchronize()
                 assert torch.equal(out, want), (tokens, k)
+
+
+def test_training_step_replayed_from_a_graph(gpu):
+    """Routing, products, both backward passes, clipping and the step captured together: each replay as the
+    same step made eagerly on a copy.  No graph of the captured leaves is alive at the capture."""
+    torch.manual_seed(7)
+    mlp = ExpertMlp(64, 128, 8, 2, score="sigmoid").to(gpu).bfloat16()
+    twin = copy.deepcopy(mlp)
+    g = torch.Generator().manual_seed(8)
+    x, dy = (torch.randn(300, 64, generator=g).bfloat16().to(gpu) for _ in range(2))
+
+    def state(module):
+        ps = list(module.parameters())
+        zeros = lambda dt=torch.float32: [torch.zeros(p.shape, dtype=dt, device=gpu) for p in ps]  # noqa: E731
+        return ps, zeros(), zeros(), [p.detach().float() for p in ps], torch.zeros(1, dtype=torch.int64, device=gpu)
+
+    def step(module, ps, m, v, master, count):
+        grads = torch.autograd.grad(module(x), ps, dy)
+        with torch.no_grad():
+            return ops.adamw_step([p.detach() for p in ps], [t.contiguous() for t in grads], m, v, count, lr=1e-2, max_norm=0.5,
+                                  masters=master)
+
+    a, b = state(mlp), state(twin)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(mlp, *a)
+    torch.cuda.current_stream().wait_stream(side)
+    step(twin, *b)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = step(mlp, *a)
+    for k in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step(twin, *b)
+        torch.cuda.synchronize()
+        assert float(norm) == float(want) and int(a[4]) == int(b[4]) == k + 2
+        for p, q in zip(mlp.parameters(), twin.parameters()):
+            assert torch.equal(p, q), k
+        x.copy_(torch.randn(300, 64, generator=g).bfloat16())
 
 
 def test_tokens_do_not_depend_on_their_batch(gpu):

@@ -95,6 +95,14 @@ def test_few_rows(gpu, T, E, k, C, H, N):
     _inside(_call(d), want["out"], "plain")
 
 
+def test_few_rows_of_one_expert(gpu):
+    """17 tokens that all choose one of 8: a whole tile of 16 rows and one of a single row."""
+    c = _case(17, 8, 1, 80, 1032, 48, 17)
+    c["index"] = torch.full_like(c["index"], 5)
+    want = O.mlp_bounds(*(c[n] for n in ("x", "weights", "index", "w1", "b1", "w2", "b2", "residual")))
+    _inside(_call(_to(c, gpu, False)), want["out"], "out")
+
+
 def test_nothing_chosen_and_unused_experts(gpu):
     c = _case(70, 6, 2, 64, 72, 64, 3)
     c["index"][:] = -1
