@@ -31,7 +31,7 @@ constexpr int AW_CHUNK = 4096;   // elements per workgroup of the step
 constexpr int AW_SUM = 16384;    // elements per workgroup of the sum of squares
 constexpr int AW_HEAD = 8;       // doubles before the partial sums
 constexpr int AW_PER = 48;       // tensors per launch: 80 bytes each in 4 KiB of arguments
-constexpr float AW_TINY = 0x1p-100f;  // 8-bit scales under it are places in 64 bits: the factor 65536 / scale leaves 32
+constexpr float AW_TINY = 0x1p-100f;  // the places of 8-bit codes under such a scale are found 2^100 larger: 65536 / scale leaves 32 bits
 enum { AW_P32 = 1, AW_G32 = 2, AW_ALIGNED = 4 };
 
 struct AwTensor {
@@ -335,7 +335,18 @@ __device__ __forceinline__ void aw_block8(const AwTensor& t, const AwShared& s, 
     av = max(av, (uint32_t)__shfl_xor((int)av, d));
   }
   const float fm = __uint_as_float(am), fv = __uint_as_float(av);
-  const float im = fm > 0.f ? 16129.f / fm : 0.f, iv = fv > 0.f ? 65536.f / fv : 0.f;
+  float fms = fm, fvs = fv;
+  if (fm < AW_TINY) {  // the same for a block's lanes
+    fms *= 0x1p100f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) mf[k] = (float)(m[k] * 0x1p100);
+  }
+  if (fv < AW_TINY) {
+    fvs *= 0x1p100f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) vf[k] = (float)(v[k] * 0x1p100);
+  }
+  const float im = fms > 0.f ? 16129.f / fms : 0.f, iv = fvs > 0.f ? 65536.f / fvs : 0.f;
   int km[8], kv[8];
   float dev = 0.f;
 #pragma unroll
@@ -346,13 +357,7 @@ __device__ __forceinline__ void aw_block8(const AwTensor& t, const AwShared& s, 
     km[k] = (int)fminf(ra, 127.f);  // a block whose scale is no number or infinite: any code
     kv[k] = (int)fminf(rb, 256.f);
   }
-  if ((fm < AW_TINY && fm > 0.f) || (fv < AW_TINY && fv > 0.f)) {  // the same for a block's lanes
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      km[k] = fm > 0.f ? (int)fmin(rint(sqrt(fabs(m[k]) * 16129. / (double)fm)), 127.) : 0;
-      kv[k] = fv > 0.f ? (int)fmin(fmax(rint(sqrt(v[k] * 65536. / (double)fv)), 1.), 256.) : 1;
-    }
-  } else if (dev > 0.49992f) {
+  if (dev > 0.49992f) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       km[k] = aw_settle(km[k], fabs(m[k]), (double)fm, 127., 0, 127);
