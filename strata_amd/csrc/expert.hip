@@ -768,16 +768,18 @@ __global__ __launch_bounds__(512, 1) void expert_wgrad_kernel(ExpertWgrad p) {
 #endif
 }
 
-// Rows of a tile, by an expert's average rows.  Times of a whole forward replayed, us; E experts, C -> H -> C:
-//   under 4 without a backward: 16, few-rows kernel (8 pairs, E 8, 1024 -> 4096: 36 against 42 with 64;
-//     at 4 an expert 41 / 45, but E 32, 512 -> 1024 32 / 30; at 12 an expert 50 / 47);
-//   under 144: 64 (125 an expert, E 16, 768 -> 1536: 53 against 56 with 128; at 150 an expert 67 / 62;
-//     112, E 24, 384 -> 776: 47 / 51);
-//   256 where an expert has two such tiles and they fill the chip (2048 an expert, E 8, 1024 -> 2048:
-//     217 against 240 with 128; half of that 141 / 148; 1024 an expert, E 32, 512 -> 1024 150 / 154); else 128.
+// Rows of a tile.  Times of a whole forward replayed, us; E experts, C -> H -> C, a: pairs an expert:
+//   16 (the few-rows kernel) under 4 pairs an expert without a backward (a 1, E 8, 1024 -> 4096: 36 against
+//     42 with 64; a 4: 41 / 45, but E 32, 512 -> 1024 32 / 30; a 12: 50 / 47);
+//   64 where the narrowest product would have fewer than 130 tiles of 128 x 128, half of the CUs (some 100:
+//     E 8, 1024 -> 4096, a 150 77 against 82 with 128, E 4, 768 -> 1536, a 500 51 / 53; 129: E 24, 384 -> 776,
+//     a 169 47 / 51; 133: E 2, 1024 -> 4096, a 1000 95 / 86; 160: E 16, 768 -> 1536, a 150 67 / 62);
+//   256 where an expert has two such tiles and they fill the chip (a 2048, E 8, 1024 -> 2048: 217 against
+//     240 with 128; a 1024: 141 / 148; a 1024, E 32, 512 -> 1024: 150 / 154);
+//   else 128, also for a few rows of many experts (a 6, E 64, 1024 -> 1024: 60 against 62 with 64).
 static int expert_tile(int64_t pairs, int experts, int64_t width, bool train) {
   if (!train && pairs < 4 * (int64_t)experts) return 16;
-  if (pairs < 144 * (int64_t)experts) return 64;
+  if ((pairs / 128 + experts / 2) * ((width + 127) / 128) < 130) return 64;
   return pairs >= 512 * (int64_t)experts && (pairs / 256) * ((width + 255) / 256) >= 200 ? 256 : 128;
 }
 static int expert_tile(const strata_hip_expert_mlp_args* a) {

@@ -56,6 +56,8 @@ SHAPES = [
     (1, 1, 1, 8, 8, 8), (1, 8, 2, 64, 128, 64), (3, 4, 3, 72, 40, 24), (64, 2, 1, 64, 64, 64), (65, 3, 2, 136, 72, 200),
     (130, 5, 2, 64, 264, 64), (200, 24, 3, 104, 56, 96), (300, 2, 2, 128, 256, 128), (513, 3, 1, 264, 136, 520),
     (90, 70, 2, 32, 40, 24), (700, 4, 2, 96, 640, 96), (40, 64, 4, 32, 48, 32), (1500, 3, 2, 192, 128, 64),
+    # 128 x 128 tiles with a ring of four stages and of two
+    (700, 40, 2, 640, 520, 552), (2600, 8, 2, 1032, 1040, 1048),
     # 256 x 256 tiles, several a workgroup, ragged in every direction
     (26000, 3, 2, 264, 328, 296),
 ]
