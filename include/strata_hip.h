@@ -3,7 +3,9 @@
  * transformer block's hot path: 3D neighbourhood attention (NA3D), the
  * stereographic-RoPE + QKV-pack prologue, the bias/GELU/residual GEMM and the
  * non-affine LayerNorm; around it, the cube-sphere halo fill and the rollout
- * step's state normalisation / patchify and state update, and the NA3D backward.
+ * step's state normalisation / patchify and state update, and the NA3D backward;
+ * the MLP routed to experts, forward and backward, and the AdamW step over many
+ * tensors.
  *
  * Conventions shared by every entry point
  *   - All pointers are device pointers owned by the caller.  Every kernel is

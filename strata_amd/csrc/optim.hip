@@ -15,7 +15,12 @@
 // border between two codes one such rounding moves the state by a whole code.  The
 // norm's sum of squares runs in 64 bits too, in an order fixed by the sizes.
 //
-// Bound by memory.  The tensors' addresses travel in the launch's arguments, so nothing
+// Bound by memory with 32-bit moments: 133M bf16 elements with masters, twelve blocks 960 wide, 561 us
+// for 3.72 GB (6.6 TB/s, some of the gradients out of the caches) and 102 for the 266 MB of the norm
+// (2.6 TB/s: reading alone reaches 3.8 to 4.0 here); with 8-bit moments by operations and latency: 59M
+// bf16 elements 173 us for 0.60 GB (3.4 TB/s).  Few or small tensors: by the host, 1.5 us a tensor
+// (its checks and pointers), which a captured step does not pay.
+// The tensors' addresses travel in the launch's arguments, so nothing
 // is kept between calls; the step count lives on the device, so a captured step counts on.
 #include <algorithm>
 #include <cmath>

@@ -6,9 +6,10 @@ device.  There is no CPU or eager fallback: CPU tensors are rejected and a
 missing library raises.  Every op has a fake (meta) implementation so that
 ``torch.compile`` traces through it.  ``na3d_fwd`` (full-grid queries),
 ``gemm_bias_act`` (act none / GELU(tanh) with an added residual, and the
-sigmoid gate), ``mlp_gelu_train``, ``layer_norm`` and ``rope_qkv_pack`` (with or
-without qk_norm) have backwards on HIP kernels (a Linear's plain input gradient is
-torch's product); the other ops' autograd formulas raise.
+sigmoid gate), ``mlp_gelu_train``, ``layer_norm``, ``rope_qkv_pack`` (with or
+without qk_norm), ``expert_route`` and ``expert_mlp`` have backwards on HIP kernels (a
+Linear's plain input gradient is torch's product); the other ops' autograd formulas raise.
+``adamw_step`` updates its tensors in place and is an ordinary function.
 """
 
 from __future__ import annotations
