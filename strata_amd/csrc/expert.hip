@@ -55,6 +55,9 @@ struct ExpertGemm {
   int64_t ldx;
   int N, K, nt;
   int round;             // 256 x 256 tiles that run at once
+  const int32_t* index;  // without a plan: the pairs' experts and weights
+  const bf16* weights;
+  int pairs, top_k, experts;
 };
 
 enum { EX_HIDDEN = 0, EX_OUT = 1, EX_HIDDEN_GRAD = 2 };
@@ -448,19 +451,43 @@ __global__ __launch_bounds__(64 * WGM * WGN, 1) void expert_gemm_kernel(ExpertGe
 // four lanes its 128-byte line, and the contraction takes the columns in that order.  One token, two of
 // 8 experts, 1024 -> 4096: 6.6 and 7.6 us for 16.8 MB each (2.5 and 2.2 TB/s; a launch that does
 // nothing takes 2 to 3).
-template <int MODE, int W>
+// DIRECT: up to 16 pairs, without a plan (the call's first launch of four): row r is pair r, and every
+// wave finds its tile's expert, the tm-th that is named, and that expert's pairs from the index.
+constexpr int EX_DIRECT = 16;
+__device__ __forceinline__ int nth_bit(uint32_t m, int n) {
+  for (int i = 0; i < n; ++i) m &= m - 1;
+  return __ffs(m) - 1;  // -1: fewer than n + 1 bits
+}
+template <int MODE, int W, bool DIRECT>
 __global__ __launch_bounds__(64 * W) void expert_few_kernel(ExpertGemm p) {
 #if defined(__HIP_DEVICE_COMPILE__)
   __shared__ float red[W][16][20];
   const int tid = (int)__builtin_amdgcn_workitem_id_x(), wave = tid >> 6, lane = tid & 63, n16 = lane & 15, g4 = lane >> 4;
   const int id = (int)__builtin_amdgcn_workgroup_id_x();
-  if (id >= plan_load(p.tiles, 0) * p.nt) return;
   const int tm = id / p.nt, n0 = id % p.nt * 16;
-  const int e = plan_load(p.tiles, 1 + 2 * tm), row0 = plan_load(p.tiles, 2 + 2 * tm);
-  const int rows = min(plan_load(p.offsets, e + 1) - row0, 16);
+  int e, row0 = 0, rows;
+  uint32_t mine = 0u;  // DIRECT: the expert's pairs
+  if constexpr (DIRECT) {
+    int el = lane < p.pairs ? p.index[lane] : -1;
+    if (el >= p.experts) el = -1;
+    bool first = el >= 0;
+    for (int s = 0; s < p.pairs; ++s) first = first && !(s < lane && __builtin_amdgcn_readlane(el, s) == el);
+    const int lead = nth_bit((uint32_t)__ballot(first), tm);
+    if (lead < 0) return;  // uniform: fewer experts are named
+    e = __builtin_amdgcn_readlane(el, lead);
+    mine = (uint32_t)__ballot(el == e);
+    rows = __popc(mine);
+  } else {
+    if (tm >= plan_load(p.tiles, 0)) return;
+    e = plan_load(p.tiles, 1 + 2 * tm);
+    row0 = plan_load(p.tiles, 2 + 2 * tm);
+    rows = min(plan_load(p.offsets, e + 1) - row0, 16);
+  }
+  auto row_at = [&](int r) { return DIRECT ? max(nth_bit(mine, r), 0) : row0 + r; };
   const bf16* w = p.w + ((int64_t)e * p.N + min(n0 + n16, p.N - 1)) * p.K;
   const bool live = n16 < rows;
-  const bf16* x = p.x + (int64_t)(MODE == EX_HIDDEN ? (live ? p.token[row0 + n16] : 0) : row0 + (live ? n16 : 0)) * p.ldx;
+  const int xr = row_at(live ? n16 : 0);
+  const bf16* x = p.x + (int64_t)(MODE != EX_HIDDEN ? xr : DIRECT ? xr / p.top_k : live ? p.token[xr] : 0) * p.ldx;
   constexpr int U = 4;
   const int kc = (p.K + 64 * W - 1) / (64 * W) * 64, k0 = wave * kc, k1 = min(p.K, k0 + kc);
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
@@ -495,8 +522,10 @@ __global__ __launch_bounds__(64 * W) void expert_few_kernel(ExpertGemm p) {
   float z = 0.f;
 #pragma unroll
   for (int i = 0; i < W; ++i) z += red[i][r][c];
-  const float b = p.bias ? (float)p.bias[(int64_t)e * p.N + n0 + c] : 0.f, s = row_scale(p.weight[row0 + r]);
-  const int64_t at = (int64_t)(row0 + r) * p.N + n0 + c;
+  const int row = row_at(r);
+  const float b = p.bias ? (float)p.bias[(int64_t)e * p.N + n0 + c] : 0.f;
+  const float s = row_scale(DIRECT ? (float)p.weights[row] : p.weight[row]);
+  const int64_t at = (int64_t)row * p.N + n0 + c;
   if (MODE == EX_HIDDEN) {
     float y, d;
     gelu_both(z + b, y, d);
@@ -518,6 +547,7 @@ struct ExpertCombine {
   bf16* out;
   int64_t n, ldr;         // tokens * chunks of eight channels
   int chunks, top_k;
+  int experts;            // without a plan: slot_row is the index, a pair's row the pair; else 0
 };
 
 __global__ __launch_bounds__(256) void expert_combine_kernel(ExpertCombine p) {
@@ -536,7 +566,8 @@ __global__ __launch_bounds__(256) void expert_combine_kernel(ExpertCombine p) {
     }
   }
   for (int s = 0; s < p.top_k; ++s) {
-    const int r = p.slot_row[t * p.top_k + s];
+    int r = p.slot_row[t * p.top_k + s];
+    if (p.experts) r = (uint32_t)r < (uint32_t)p.experts ? (int)t * p.top_k + s : -1;
     if (r < 0 || (p.weights && no_weight((float)p.weights[t * p.top_k + s]))) continue;
     const f32x4 u = *(const f32x4*)(p.y + (int64_t)r * ld + c), v = *(const f32x4*)(p.y + (int64_t)r * ld + c + 4);
 #pragma unroll
@@ -782,7 +813,7 @@ __global__ __launch_bounds__(512, 1) void expert_wgrad_kernel(ExpertWgrad p) {
 #endif
 }
 
-// Rows of a tile.  Times of a whole forward replayed, us; E experts, C -> H -> C, a: pairs an expert:
+// 1: up to 16 pairs without a backward take no plan (`EX_DIRECT`); else rows of a tile.  Times of a whole forward replayed, us; E experts, C -> H -> C, a: pairs an expert:
 //   16 (the few-rows kernel) under 4 pairs an expert without a backward (a 1, E 8, 1024 -> 4096: 36 against
 //     42 with 64; a 4: 41 / 45, but E 32, 512 -> 1024 32 / 30; a 12: 50 / 47);
 //   64 where the narrowest product would have fewer than 130 tiles of 128 x 128, half of the CUs (some 100:
@@ -792,6 +823,7 @@ __global__ __launch_bounds__(512, 1) void expert_wgrad_kernel(ExpertWgrad p) {
 //     240 with 128; a 1024: 141 / 148; a 1024, E 32, 512 -> 1024: 150 / 154);
 //   else 128, also for a few rows of many experts (a 6, E 64, 1024 -> 1024: 60 against 62 with 64).
 static int expert_tile(int64_t pairs, int experts, int64_t width, bool train) {
+  if (!train && pairs <= EX_DIRECT) return 1;
   if (!train && pairs < 4 * (int64_t)experts) return 16;
   if ((pairs / 128 + experts / 2) * ((width + 127) / 128) < 130) return 64;
   return pairs >= 512 * (int64_t)experts && (pairs / 256) * ((width + 255) / 256) >= 200 ? 256 : 128;
@@ -814,19 +846,27 @@ static int expert_cus() {
 
 template <int MODE, bool WT>
 static int launch_expert_gemm(ExpertGemm p, int64_t pairs, int experts, int tile, hipStream_t st) {
-  p.nt = (p.N + tile - 1) / tile;
-  const int64_t mt = pairs / tile + std::min<int64_t>(experts, pairs), total = mt * p.nt;
+  const int cols = tile == 1 ? 16 : tile;
+  p.nt = (p.N + cols - 1) / cols;
+  const int64_t mt = tile == 1 ? std::min<int64_t>(experts, pairs) : pairs / tile + std::min<int64_t>(experts, pairs), total = mt * p.nt;
   // 2^32 threads a launch (a grid of 256 x 256 tiles is not larger than the chip)
-  if (total > 0x7fffffff || (tile != 256 && total * (tile == 16 ? 1024 : tile == 64 ? 256 : 512) >= 0x100000000ll))
+  if (total > 0x7fffffff || (tile != 256 && total * (tile <= 16 ? 1024 : tile == 64 ? 256 : 512) >= 0x100000000ll))
     return fail(STRATA_HIP_EUNSUPPORTED, "expert_mlp: problem too large for one launch");
   if constexpr (!WT && MODE != EX_HIDDEN_GRAD) {
+    if (tile == 1) {
+      if (p.K > 1024)
+        hipLaunchKernelGGL((expert_few_kernel<MODE, 16, true>), dim3((unsigned)total), dim3(1024), 0, st, p);
+      else
+        hipLaunchKernelGGL((expert_few_kernel<MODE, 4, true>), dim3((unsigned)total), dim3(256), 0, st, p);
+      return check_launch("expert_few_kernel");
+    }
     if (tile == 16) {
       // 16 waves a workgroup for a long contraction: one token, 1024 -> 4096 24.8 us against 26.0 with 4
       // throughout (and 25.8 with 16 throughout); four tokens, 1024 -> 2048 28.5 against 27.5.
       if (p.K > 1024)
-        hipLaunchKernelGGL((expert_few_kernel<MODE, 16>), dim3((unsigned)total), dim3(1024), 0, st, p);
+        hipLaunchKernelGGL((expert_few_kernel<MODE, 16, false>), dim3((unsigned)total), dim3(1024), 0, st, p);
       else
-        hipLaunchKernelGGL((expert_few_kernel<MODE, 4>), dim3((unsigned)total), dim3(256), 0, st, p);
+        hipLaunchKernelGGL((expert_few_kernel<MODE, 4, false>), dim3((unsigned)total), dim3(256), 0, st, p);
       return check_launch("expert_few_kernel");
     }
   }
@@ -877,12 +917,13 @@ static int expert_check(const std::string& name, const strata_hip_expert_mlp_arg
   if (a->experts > 512 || pairs > 0x7ffffff0 || a->dim > 32768 || a->hidden > 32768 || a->out_dim > 32768)
     return fail(STRATA_HIP_EUNSUPPORTED, name + ": at most 512 experts, widths 32768 and 2^31 pairs");
   if (pairs > 0 && a->tile != expert_tile(a)) return fail(STRATA_HIP_EINVAL, name + ": tile is not strata_hip_expert_tile()'s");
-  if (!a->w1 || !a->w2 || !a->offsets || !a->tiles) return fail(STRATA_HIP_EINVAL, name + ": null pointer");
+  const bool plan = a->tile != 1;
+  if (!a->w1 || !a->w2 || (plan && (!a->offsets || !a->tiles))) return fail(STRATA_HIP_EINVAL, name + ": null pointer");
   if (((uintptr_t)a->w1 & 15) || ((uintptr_t)a->w2 & 15) || ((uintptr_t)a->b1 & 15) || ((uintptr_t)a->b2 & 15))
     return fail(STRATA_HIP_EINVAL, name + ": weights and biases must be 16-byte aligned");
   if (pairs == 0) return STRATA_HIP_OK;
   if (!a->dact && name != "expert_mlp") return fail(STRATA_HIP_EINVAL, name + ": dact is needed");
-  if (!a->x || !a->weights || !a->row_token || !a->row_weight || !a->slot_row || !a->h || !a->y)
+  if (!a->x || !a->weights || (plan && (!a->row_token || !a->row_weight)) || !a->slot_row || !a->h || !a->y)
     return fail(STRATA_HIP_EINVAL, name + ": null pointer");
   if (((uintptr_t)a->x & 15) || ((uintptr_t)a->h & 15) || ((uintptr_t)a->y & 15) || ((uintptr_t)a->dact & 15) || a->ldx % 8 ||
       (a->tokens > 1 && a->ldx < a->dim))
@@ -915,6 +956,11 @@ extern "C" int strata_hip_expert_mlp(const strata_hip_expert_mlp_args* a, void* 
   g.weight = a->row_weight;
   g.offsets = a->offsets;
   g.tiles = a->tiles;
+  g.index = a->slot_row;
+  g.weights = (const bf16*)a->weights;
+  g.pairs = (int)std::min<int64_t>(pairs, EX_DIRECT);
+  g.top_k = a->top_k;
+  g.experts = a->experts;
   g.x = (const bf16*)a->x;
   g.ldx = a->ldx;
   g.w = (const bf16*)a->w1;
@@ -940,6 +986,7 @@ extern "C" int strata_hip_expert_mlp(const strata_hip_expert_mlp_args* a, void* 
   c.ldr = a->ldr;
   c.out = (bf16*)a->out;
   c.top_k = a->top_k;
+  c.experts = a->tile == 1 ? a->experts : 0;
   return launch_combine(c, a->tokens, a->out_dim, st);
 }
 

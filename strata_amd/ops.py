@@ -1656,6 +1656,8 @@ def _expert_space(n: int, E: int, H: int, N: int, tile: int, train: bool) -> tup
     dact = 2 * n * H
     y = dact + (2 * n * H if train else 0)
     plan = y + 4 * n * N
+    if tile == 1:  # no plan
+        return dact, y, plan, plan, plan
     ws = plan + 4 * _plan_size(n, E, tile)
     return dact, y, plan, ws, ws + 4 * int(_lib.function("strata_hip_expert_plan_workspace")(n, E))
 
@@ -1690,7 +1692,10 @@ def _expert_forward(name, x, weights, index, w1, b1, w2, b2, residual, train: bo
     a.out = out.data_ptr()
     i = index.contiguous()
     s = space.data_ptr()
-    _launch("strata_hip_expert_plan", _plan_args(i.data_ptr(), a.weights, s + at[2], s + at[3], n, a.top_k, E, tile), x)
+    if tile == 1:
+        a.slot_row = i.data_ptr()
+    else:
+        _launch("strata_hip_expert_plan", _plan_args(i.data_ptr(), a.weights, s + at[2], s + at[3], n, a.top_k, E, tile), x)
     _launch("strata_hip_expert_mlp", a, x)
     return out, space
 

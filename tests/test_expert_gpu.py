@@ -105,6 +105,26 @@ def test_few_rows_of_one_expert(gpu):
     _inside(_call(_to(c, gpu, False)), want["out"], "out")
 
 
+@pytest.mark.parametrize("T,E,k", [(1, 8, 2), (16, 3, 1), (4, 40, 4), (1, 2, 16), (8, 1, 2), (5, 512, 3)])
+def test_up_to_16_pairs(gpu, T, E, k):
+    """Served without a plan: the same expert in several slots, indexes outside the range, weights of zero."""
+    for seed, picks in ((18, None), (19, 0), (20, -1), (21, E)):
+        c = _case(T, E, k, 72, 1040, 136, seed)
+        if E < k:
+            g = torch.Generator().manual_seed(seed)
+            c["index"] = torch.randint(0, E, (T, k), generator=g, dtype=torch.int32)
+        if picks is not None:
+            c["index"].view(-1)[:: 2] = picks
+            c["weights"].view(-1)[1::3] = 0.0
+        want = O.mlp_bounds(*(c[n] for n in ("x", "weights", "index", "w1", "b1", "w2", "b2", "residual")))
+        d = _to(c, gpu, False)
+        out = _call(d)
+        _inside(out, want["out"], (T, E, k, picks))
+        with torch.enable_grad():  # the planned products give the same up to the contraction's order
+            planned = _call(dict(d, x=d["x"].clone().requires_grad_()))
+        _inside(planned.detach(), want["out"], (T, E, k, picks, "planned"))
+
+
 def test_nothing_chosen_and_unused_experts(gpu):
     c = _case(70, 6, 2, 64, 72, 64, 3)
     c["index"][:] = -1
