@@ -658,8 +658,10 @@ int strata_hip_expert_plan(const strata_hip_expert_plan_args* args, void* stream
  * where no stride is given, fp32 accumulation.  Widths multiples of 8, at most 32768; x and
  * out under 2 GiB.  Workspaces, rows of the plan's order (rows past the last one stay as they
  * were): h [pairs, hidden] bf16, y [pairs, out_dim] fp32, dact [pairs, hidden] fp16 or NULL:
- * gelu' for a backward, which reads h, y and dact again.  A weight under 2^-100 counts as 0.  x, w, h, y, dact, out, residual
- * 16-byte aligned, b1, b2 8-byte.  The order of every sum is fixed by the sizes and the plan.
+ * gelu' for a backward, which reads h, y and dact again.  A weight under 2^-100 counts as 0.
+ * Where strata_hip_expert_tile() says 1 (up to 16 pairs, no backward) there is no plan: slot_row is
+ * the index itself, and row_token, row_weight, offsets and tiles are not read.  x, w, b, h, y,
+ * dact, out, residual 16-byte aligned.  The order of every sum is fixed by the sizes and the plan.
  * ------------------------------------------------------------------------- */
 typedef struct strata_hip_expert_mlp_args {
   const void* x;

@@ -452,7 +452,8 @@ __global__ __launch_bounds__(64 * WGM * WGN, 1) void expert_gemm_kernel(ExpertGe
 // 8 experts, 1024 -> 4096: 6.6 and 7.6 us for 16.8 MB each (2.5 and 2.2 TB/s; a launch that does
 // nothing takes 2 to 3).
 // DIRECT: up to 16 pairs, without a plan (the call's first launch of four): row r is pair r, and every
-// wave finds its tile's expert, the tm-th that is named, and that expert's pairs from the index.
+// wave finds its tile's expert, the tm-th that is named, and that expert's pairs from the index
+// (the token's call 24.5 -> 21.9 us).
 constexpr int EX_DIRECT = 16;
 __device__ __forceinline__ int nth_bit(uint32_t m, int n) {
   for (int i = 0; i < n; ++i) m &= m - 1;

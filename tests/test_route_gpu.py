@@ -173,7 +173,7 @@ def test_route_repeats_and_replays(gpu):
 
 
 @pytest.mark.parametrize("tile", [16, 64, 256])
-@pytest.mark.parametrize("n,E", [(0, 3), (1, 1), (2, 8), (63, 5), (64, 64), (65, 2), (1000, 100), (1024, 512), (1025, 8),
+@pytest.mark.parametrize("n,E", [(0, 3), (1, 1), (2, 8), (63, 5), (64, 64), (65, 2), (1000, 100), (1024, 512), (1025, 8), (1026, 512), (2048, 24), (2049, 200), (4050, 24), (4096, 100), (4097, 100),
                                  (5000, 1), (4097, 300), (70000, 24), (40000, 512), (70000, 512)])
 def test_plan(gpu, n, E, tile):
     """Rows sorted by expert, stable; offsets and tiles; indices that name no expert left out."""
