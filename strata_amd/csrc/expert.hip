@@ -87,7 +87,7 @@ __device__ __forceinline__ int plan_load(const int32_t* p, int i) {
 // BIG: 256 x 256, one workgroup a CU walks over the tiles; the last step of a tile starts
 // the next one's first stage.  Otherwise one tile a workgroup and several workgroups a CU.
 // TAIL: the 256 x 256 tiles of a last round that would leave half of the CUs or more idle,
-// each as four 128 x 128 ones (the same sums in the same order).
+// each as four 128 x 128 or sixteen 64 x 64 ones (the same sums in the same order).
 // Bound by the matrix instructions and their feeding: 32768 pairs of 8 experts, 1024 -> 4096 ->
 // 1024, the two products forward with what a backward needs 348 and 308 us (790 and 893 TFLOP/s; a
 // dense library product of these sizes 217 and 188 without GELU, bias, gather or fp32 output), the
@@ -123,10 +123,11 @@ __global__ __launch_bounds__(64 * WGM * WGN, 1) void expert_gemm_kernel(ExpertGe
   const int mt = plan_load(p.tiles, 0), all = mt * p.nt, wg_id = (int)__builtin_amdgcn_workgroup_id_x();
   int tail = BIG || TAIL ? all > p.round ? all % p.round : 0 : 0;
   if (2 * tail > p.round) tail = 0;
-  const int total = BIG ? all - tail : TAIL ? 4 * tail : all;
+  constexpr int SUB = TAIL ? 256 / BM : 1;
+  const int total = BIG ? all - tail : TAIL ? SUB * SUB * tail : all;
   if (wg_id >= total) return;
   auto tile_at = [&](int t) {
-    const int wg = xcd_tile_order(all, TAIL ? all - tail + t / 4 : t);
+    const int wg = xcd_tile_order(all, TAIL ? all - tail + t / (SUB * SUB) : t);
     constexpr int GRP = BIG || TAIL ? 4 : 8;  // row panels x every column panel, row panel fastest
     const int gi = wg / (GRP * p.nt), li = wg % (GRP * p.nt), gmn = min(GRP, mt - gi * GRP);
     const int tm = gi * GRP + li % gmn;
@@ -134,11 +135,12 @@ __global__ __launch_bounds__(64 * WGM * WGN, 1) void expert_gemm_kernel(ExpertGe
     r.e = plan_load(p.tiles, 1 + 2 * tm);
     r.row0 = plan_load(p.tiles, 2 + 2 * tm);
     r.rows = plan_load(p.offsets, r.e + 1) - r.row0;
-    r.n0 = (li / gmn) * (TAIL ? 2 * BN : BN);
+    r.n0 = (li / gmn) * (SUB * BN);
     if (TAIL) {
-      r.rows = min(r.rows, 2 * BM) - BM * (t >> 1 & 1);
-      r.row0 += BM * (t >> 1 & 1);
-      r.n0 += BN * (t & 1);
+      const int sr = t / SUB % SUB, sc = t % SUB;
+      r.rows = min(r.rows, SUB * BM) - BM * sr;
+      r.row0 += BM * sr;
+      r.n0 += BN * sc;
     }
     r.rows = min(r.rows, BM);
     return r;
@@ -875,8 +877,16 @@ static int launch_expert_gemm(ExpertGemm p, int64_t pairs, int experts, int tile
     p.round = expert_cus();
     hipLaunchKernelGGL((expert_gemm_kernel<256, 256, 2, 4, 2, MODE, WT, false>), dim3((unsigned)std::min<int64_t>(total, p.round)),
                        dim3(512), 0, st, p);
-    if (total > p.round)
-      hipLaunchKernelGGL((expert_gemm_kernel<128, 128, 4, 2, 4, MODE, WT, true>), dim3((unsigned)(p.round / 2 * 4)), dim3(512), 0, st, p);
+    if (total > p.round) {
+      // The tail in 64 x 64 tiles where they are expected to fit the chip at one a CU, an expert's last tile being
+      // half full on average: 16 tiles, 4096 -> 1024, 45 -> 28 us (a whole training pass 1843 -> 1810); 64 tiles
+      // of 1024 -> 4096 in 64 x 64 ones: the pass 10 us slower.
+      const int64_t tail = (pairs / tile + experts / 2) * p.nt % p.round;
+      if (16 * tail <= p.round)
+        hipLaunchKernelGGL((expert_gemm_kernel<64, 64, 2, 2, 4, MODE, WT, true>), dim3((unsigned)(p.round / 2 * 16)), dim3(256), 0, st, p);
+      else
+        hipLaunchKernelGGL((expert_gemm_kernel<128, 128, 4, 2, 4, MODE, WT, true>), dim3((unsigned)(p.round / 2 * 4)), dim3(512), 0, st, p);
+    }
   } else if (tile == 128) {
     // A ring of four stages (one workgroup a CU) where one round of workgroups is expected, else of two
     // (two a CU): 4000 pairs, 16 experts, 768 columns of 1536 30 -> 23 us, 1536 of 768 26 against 28.
