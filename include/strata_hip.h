@@ -693,7 +693,8 @@ int strata_hip_expert_mlp(const strata_hip_expert_mlp_args* args, void* stream);
  * [tokens, dim], dweights [tokens, top_k], dw1, db1, dw2, db2 (the shapes of their weights, bf16)
  * may be NULL, a weight's only with its bias's; a dropped pair's dweights and an
  * unused expert's gradients are zero.  Workspaces: gz [pairs, hidden] bf16 for dx or dw1,
- * dxs [pairs, dim] fp32 for dx. */
+ * dxs [pairs, dim] fp32 for dx, wspace strata_hip_expert_mlp_bwd_workspace() fp32 for dw1 and dw2
+ * (NULL when that is 0). */
 typedef struct strata_hip_expert_mlp_bwd_args {
   strata_hip_expert_mlp_args fwd;
   const void* dout;
@@ -705,8 +706,10 @@ typedef struct strata_hip_expert_mlp_bwd_args {
   void* db2;
   void* gz;
   float* dxs;
+  float* wspace;
 } strata_hip_expert_mlp_bwd_args;
 
+int64_t strata_hip_expert_mlp_bwd_workspace(int64_t pairs, int32_t experts, int32_t dim, int32_t hidden, int32_t out_dim);
 int strata_hip_expert_mlp_bwd(const strata_hip_expert_mlp_bwd_args* args, void* stream);
 
 /* ---------------------------------------------------------------------------

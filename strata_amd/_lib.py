@@ -381,7 +381,7 @@ class ExpertMlpArgs(ctypes.Structure):
 
 class ExpertMlpBwdArgs(ctypes.Structure):
     _fields_ = [("fwd", ExpertMlpArgs)] + \
-        [(n, ctypes.c_void_p) for n in ("dout", "dx", "dweights", "dw1", "db1", "dw2", "db2", "gz", "dxs")]
+        [(n, ctypes.c_void_p) for n in ("dout", "dx", "dweights", "dw1", "db1", "dw2", "db2", "gz", "dxs", "wspace")]
 
 
 class AdamwTensor(ctypes.Structure):
@@ -461,6 +461,7 @@ EXPORTS = {
     "strata_hip_expert_route_bwd": ([ctypes.POINTER(ExpertRouteArgs), ctypes.c_void_p], ctypes.c_int),
     "strata_hip_expert_plan": ([ctypes.POINTER(ExpertPlanArgs), ctypes.c_void_p], ctypes.c_int),
     "strata_hip_expert_plan_workspace": ([ctypes.c_int64, ctypes.c_int32], ctypes.c_int64),
+    "strata_hip_expert_mlp_bwd_workspace": ([ctypes.c_int64] + [ctypes.c_int32] * 4, ctypes.c_int64),
     "strata_hip_expert_tile": ([ctypes.c_int64] + [ctypes.c_int32] * 5, ctypes.c_int32),
     "strata_hip_expert_mlp": ([ctypes.POINTER(ExpertMlpArgs), ctypes.c_void_p], ctypes.c_int),
     "strata_hip_expert_mlp_bwd": ([ctypes.POINTER(ExpertMlpBwdArgs), ctypes.c_void_p], ctypes.c_int),

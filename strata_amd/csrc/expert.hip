@@ -629,14 +629,17 @@ struct ExpertWgrad {
   const int32_t* offsets;
   bf16* out;
   bf16* bias_out;       // [E, N] or null
+  float* part;          // SPLIT: [split, E, N, K], then the bias's [split, E, N]
   int64_t ldg, ldx;
-  int N, K, nt, kt, experts;
+  int N, K, nt, kt, experts, split;
 };
 
 constexpr int EW_BK = 64, EW_HALF = EW_BK * 512, EW_STAGE = 2 * EW_HALF;
 
 // OF_G: g is gathered (dout), x are rows (h); else x is gathered and g are rows (gz).
-template <bool OF_G>
+// SPLIT: where the tiles are at most half as many as the CUs, an expert's rows are shared out over `split`
+// workgroups, whose fp32 sums are added in order by a second launch.
+template <bool OF_G, bool SPLIT>
 __global__ __launch_bounds__(512, 1) void expert_wgrad_kernel(ExpertWgrad p) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr int NW = 8, LPW = EW_HALF / 1024 / NW;
@@ -649,9 +652,10 @@ __global__ __launch_bounds__(512, 1) void expert_wgrad_kernel(ExpertWgrad p) {
   const int wk = wave >> 2, wn = wave & 3;  // wave tile: 128 k x 64 n
   const uint32_t lds_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
 
-  const int id = (int)__builtin_amdgcn_workgroup_id_x(), per = p.nt * p.kt;
+  const int id = (int)__builtin_amdgcn_workgroup_id_x(), per = p.nt * p.kt * (SPLIT ? p.split : 1);
   int e = id / per;
-  const int tk = id % per % p.kt, tn = id % per / p.kt;
+  const int tile = SPLIT ? id % per / p.split : id % per, share = SPLIT ? id % per % p.split : 0;
+  const int tk = tile % p.kt, tn = tile / p.kt;
   if (p.experts <= 64) {  // the e-th largest: every wave ranks the experts, one a lane
     const int n = lane < p.experts ? p.offsets[lane + 1] - p.offsets[lane] : -1;
     int before = 0;
@@ -663,7 +667,12 @@ __global__ __launch_bounds__(512, 1) void expert_wgrad_kernel(ExpertWgrad p) {
   }
   e = __builtin_amdgcn_readfirstlane(e);
   const int k0 = tk * 256, n0 = tn * 256;
-  const int row0 = plan_load(p.offsets, e), rows = plan_load(p.offsets, e + 1) - row0;
+  int row0 = plan_load(p.offsets, e), rows = plan_load(p.offsets, e + 1) - row0;
+  if (SPLIT) {  // whole stages
+    const int chunk = ((rows + EW_BK - 1) / EW_BK + p.split - 1) / p.split * EW_BK, first = min(share * chunk, rows);
+    row0 += first;
+    rows = min(chunk, rows - first);
+  }
   const int nk = (rows + EW_BK - 1) / EW_BK;
 
   uint32_t vx[LPW], vg[LPW];  // the gathered one's without the row
@@ -789,16 +798,32 @@ __global__ __launch_bounds__(512, 1) void expert_wgrad_kernel(ExpertWgrad p) {
     for (int kt = 0; kt < nk; ++kt) stage(kt, std::true_type{});
   else
     for (int kt = 0; kt < nk; ++kt) stage(kt, std::false_type{});
+  const int64_t of_e = SPLIT ? (int64_t)share * p.experts + e : e;
   if (sums && g4 == 0) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int n = n0 + 64 * wn + 16 * j + n16;
-      if (n < p.N) p.bias_out[(int64_t)e * p.N + n] = (bf16)bacc[j][0];
+      if (n >= p.N) continue;
+      if (SPLIT) p.part[(int64_t)p.split * p.experts * p.N * p.K + of_e * p.N + n] = bacc[j][0];
+      else p.bias_out[of_e * p.N + n] = (bf16)bacc[j][0];
     }
+  }
+  if constexpr (SPLIT) {
+    float* out = p.part + of_e * p.N * p.K;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int n = n0 + 64 * wn + 16 * j + n16;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int k = k0 + 128 * wk + 16 * i + 4 * g4;
+        if (n < p.N && k < p.K) *(f32x4*)(out + (int64_t)n * p.K + k) = acc[i][j];
+      }
+    }
+    return;
   }
   // 16 rows n x 128 columns k at a time through this wave's 4 KiB of the ring: rows of 256 bytes out
   lds_barrier();  // every wave is done reading the last stage
-  bf16* out = p.out + (int64_t)e * p.N * p.K;
+  bf16* out = p.out + of_e * p.N * p.K;
   char* slab = lds + wave * 4096;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -814,6 +839,24 @@ __global__ __launch_bounds__(512, 1) void expert_wgrad_kernel(ExpertWgrad p) {
     }
   }
 #endif
+}
+
+// The shares' sums, added in order and rounded once: n elements of the weights, then nb of the bias.
+__global__ __launch_bounds__(256) void expert_wgrad_sum_kernel(const float* part, bf16* out, int64_t n, bf16* bias_out, int64_t nb,
+                                                               int split) {
+  int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  const bool bias = i >= n;
+  if (bias) {
+    i -= n;
+    if (i >= nb) return;
+    part += n * split;
+    out = bias_out;
+    n = nb;
+  }
+  f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = 0; s < split; ++s) a += *(const f32x4*)(part + n * s + i);
+  *(u32x2*)(out + i) = (u32x2){pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3])};
 }
 
 // 1: up to 16 pairs without a backward take no plan (`EX_DIRECT`); else rows of a tile.  Times of a whole forward replayed, us; E experts, C -> H -> C, a: pairs an expert:
@@ -900,14 +943,39 @@ static int launch_expert_gemm(ExpertGemm p, int64_t pairs, int experts, int tile
   return check_launch("expert_gemm_kernel");
 }
 
+// Shares of an expert's rows in its weights' gradients: as many as fill the chip, of four stages or
+// more on average.  A whole forward and backward with one share / with these: 32768 tokens, 2 experts,
+// 128 -> 512 887 / 172 us; 8000, 2 of 2, 512 -> 1024 534 / 250; 16000, 2 of 8, 512 -> 512 420 / 306;
+// 1000, 2 of 2, 512 -> 512 110 / 100 (shares of two stages 97, of eight 110).
+static int wgrad_split(int64_t pairs, int experts, int N, int K) {
+  constexpr int64_t CUS = 256;
+  const int64_t tiles = (int64_t)experts * ((N + 255) / 256) * ((K + 255) / 256);
+  return (int)std::max<int64_t>(1, std::min<int64_t>({CUS / tiles, pairs / experts / (4 * EW_BK), 32}));
+}
+static int64_t wgrad_space(int64_t pairs, int experts, int N, int K) {
+  const int split = wgrad_split(pairs, experts, N, K);
+  return split > 1 ? (int64_t)split * experts * N * (K + 1) : 0;
+}
+
 template <bool OF_G>
-static int launch_wgrad(ExpertWgrad p, hipStream_t st) {
+static int launch_wgrad(ExpertWgrad p, int64_t pairs, float* space, hipStream_t st) {
   p.nt = (p.N + 255) / 256;
   p.kt = (p.K + 255) / 256;
-  const int64_t total = (int64_t)p.nt * p.kt * p.experts;
+  p.split = wgrad_split(pairs, p.experts, p.N, p.K);
+  p.part = space;
+  const int64_t total = (int64_t)p.nt * p.kt * p.experts * p.split;
   if (total * 512 >= 0x100000000ll) return fail(STRATA_HIP_EUNSUPPORTED, "expert_mlp_bwd: problem too large for one launch");
-  hipLaunchKernelGGL(expert_wgrad_kernel<OF_G>, dim3((unsigned)total), dim3(512), 0, st, p);
-  return check_launch("expert_wgrad_kernel");
+  if (p.split == 1) {
+    hipLaunchKernelGGL((expert_wgrad_kernel<OF_G, false>), dim3((unsigned)total), dim3(512), 0, st, p);
+    return check_launch("expert_wgrad_kernel");
+  }
+  if (!space || ((uintptr_t)space & 15)) return fail(STRATA_HIP_EINVAL, "expert_mlp_bwd: wspace is needed, 16-byte aligned");
+  hipLaunchKernelGGL((expert_wgrad_kernel<OF_G, true>), dim3((unsigned)total), dim3(512), 0, st, p);
+  if (const int rc = check_launch("expert_wgrad_kernel")) return rc;
+  const int64_t n = (int64_t)p.experts * p.N * p.K, nb = p.bias_out ? (int64_t)p.experts * p.N : 0;
+  hipLaunchKernelGGL(expert_wgrad_sum_kernel, dim3((unsigned)((n + nb + 1023) / 1024)), dim3(256), 0, st, space, p.out, n, p.bias_out,
+                     nb, p.split);
+  return check_launch("expert_wgrad_sum_kernel");
 }
 
 static int launch_combine(ExpertCombine c, int64_t tokens, int width, hipStream_t st) {
@@ -952,6 +1020,11 @@ using namespace strata;
 extern "C" int32_t strata_hip_expert_tile(int64_t pairs, int32_t experts, int32_t dim, int32_t hidden, int32_t out_dim,
                                           int32_t train) {
   return expert_tile(pairs, experts, std::min(std::min(dim, hidden), out_dim), train != 0);
+}
+
+extern "C" int64_t strata_hip_expert_mlp_bwd_workspace(int64_t pairs, int32_t experts, int32_t dim, int32_t hidden, int32_t out_dim) {
+  if (pairs <= 0 || experts <= 0 || dim <= 0 || hidden <= 0 || out_dim <= 0) return 0;
+  return std::max(wgrad_space(pairs, experts, out_dim, hidden), wgrad_space(pairs, experts, hidden, dim));
 }
 
 extern "C" int strata_hip_expert_mlp(const strata_hip_expert_mlp_args* a, void* stream) {
@@ -1015,7 +1088,7 @@ extern "C" int strata_hip_expert_mlp_bwd(const strata_hip_expert_mlp_bwd_args* b
     if (b->dx && !b->dxs) return fail(STRATA_HIP_EINVAL, name + ": dxs is needed for dx");
   }
   if ((b->db2 && !b->dw2) || (b->db1 && !b->dw1)) return fail(STRATA_HIP_EINVAL, name + ": a bias gradient comes with its weight's");
-  const void* all[] = {b->gz, b->dxs, b->dx, b->dw1, b->dw2};
+  const void* all[] = {b->gz, b->dxs, b->dx, b->dw1, b->dw2, b->db1, b->db2};
   for (const void* q : all)
     if ((uintptr_t)q & 15) return fail(STRATA_HIP_EINVAL, name + ": workspaces and gradients must be 16-byte aligned");
   if (pairs > 0 && b->dweights) {
@@ -1041,7 +1114,7 @@ extern "C" int strata_hip_expert_mlp_bwd(const strata_hip_expert_mlp_bwd_args* b
     w.ldx = a->hidden;
     w.N = a->out_dim;
     w.K = a->hidden;
-    if (const int rc = launch_wgrad<true>(w, st)) return rc;
+    if (const int rc = launch_wgrad<true>(w, pairs, b->wspace, st)) return rc;
   }
   ExpertGemm g = {};
   g.token = a->row_token;
@@ -1067,7 +1140,7 @@ extern "C" int strata_hip_expert_mlp_bwd(const strata_hip_expert_mlp_bwd_args* b
     w.ldx = a->ldx;
     w.N = a->hidden;
     w.K = a->dim;
-    if (const int rc = launch_wgrad<false>(w, st)) return rc;
+    if (const int rc = launch_wgrad<false>(w, pairs, b->wspace, st)) return rc;
   }
   if (b->dx && pairs > 0) {
     g.x = (const bf16*)b->gz;

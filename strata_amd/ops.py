@@ -1748,7 +1748,9 @@ def _expert_backward(dout, x, weights, w1, b1, w2, b2, space, need):
     g = _dense(dout)
     gz = new(n, H) if hid else None
     dxs = torch.empty((n, C), dtype=torch.float32, device=x.device) if want_x else None
-    b = _lib.ExpertMlpBwdArgs(a, g.data_ptr(), *(_ptr(t) for t in (dx, dwt, dw1, db1, dw2, db2, gz, dxs)))
+    shares = int(_lib.function("strata_hip_expert_mlp_bwd_workspace")(n, E, C, H, N)) if want_1 or want_2 else 0
+    wspace = torch.empty(shares, dtype=torch.float32, device=x.device) if shares else None
+    b = _lib.ExpertMlpBwdArgs(a, g.data_ptr(), *(_ptr(t) for t in (dx, dwt, dw1, db1, dw2, db2, gz, dxs, wspace)))
     _launch("strata_hip_expert_mlp_bwd", b, x)
     return [t if wanted else None for t, wanted in zip((dx, dwt, dw1, db1, dw2, db2), need)]
 

@@ -60,6 +60,8 @@ SHAPES = [
     (700, 40, 2, 640, 520, 552), (2600, 8, 2, 1032, 1040, 1048),
     # 256 x 256 tiles, several a workgroup, ragged in every direction
     (26000, 3, 2, 264, 328, 296),
+    # few tiles of the weights' gradients: their rows shared out, an expert's share empty or not whole
+    (600, 1, 1, 72, 40, 24), (1700, 4, 2, 264, 72, 136), (5000, 2, 1, 64, 520, 200),
     # the same with a last round in 64 x 64 tiles, and in 128 x 128 ones
     (34000, 2, 2, 136, 72, 200), (40000, 2, 2, 136, 264, 200),
 ]
