@@ -89,9 +89,9 @@ __device__ __forceinline__ int plan_load(const int32_t* p, int i) {
 // TAIL: the 256 x 256 tiles of a last round that would leave half of the CUs or more idle,
 // each as four 128 x 128 or sixteen 64 x 64 ones (the same sums in the same order).
 // Bound by the matrix instructions and their feeding: 32768 pairs of 8 experts, 1024 -> 4096 ->
-// 1024, the two products forward with what a backward needs 348 and 308 us (790 and 893 TFLOP/s; a
+// 1024, the two products forward with what a backward needs 351 and 291 us (783 and 945 TFLOP/s; a
 // dense library product of these sizes 217 and 188 without GELU, bias, gather or fp32 output), the
-// backward's 330 (gelu' and the weight in the epilogue) and 301; 54% of the cycles issue MFMAs in
+// backward's 330 to 350 (gelu' and the weight in the epilogue) and 291; 54% of the cycles issue MFMAs in
 // the second, 43% in the first, whose epilogue writes 520 MB; no LDS conflicts, 68 - 75% of the reads
 // hit L2.  Every 128 x 128 tiles instead: 20% slower; the K loop's barrier elsewhere: spills.
 template <int BM, int BN, int WGM, int WGN, int NST, int MODE, bool WT, bool TAIL>
