@@ -539,6 +539,78 @@ __global__ __launch_bounds__(64 * W) void expert_few_kernel(ExpertGemm p) {
 #endif
 }
 
+// Up to EX_FUSED pairs (a token while serving) of at most EX_FUSED_K columns together: the second product and
+// the sum over slots in one launch, 8 columns of every token a workgroup, whose 16 waves share the named
+// experts and their contractions.  Replayed, us, two launches / this one (with 16 columns): 2 pairs,
+// 1024 -> 4096 20.2 / 20.0 (22.8), 512 -> 2048 19.0 / 17.5 (17.3), 4 pairs, 512 -> 1024 18.8 / 17.3, but
+// 1024 -> 4096 24.9 / 31.0; the first called eagerly 21.2 / 18.8.
+constexpr int EX_FUSED = 4, EX_FUSED_K = 8192, EX_FUSED_N = 8;
+__global__ __launch_bounds__(1024) void expert_few_out_kernel(ExpertGemm p, const bf16* residual, int64_t ldr, bf16* out) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  __shared__ float red[16][EX_FUSED][20];
+  __shared__ int expert_at[EX_FUSED], rank_at[EX_FUSED];  // a pair's place among the named experts (-1), and among its expert's pairs
+  const int tid = (int)__builtin_amdgcn_workitem_id_x(), lane = tid & 63, n16 = lane & 15, g4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), n0 = (int)__builtin_amdgcn_workgroup_id_x() * EX_FUSED_N;
+  int el = lane < p.pairs ? p.index[lane] : -1;
+  if (el < 0 || el >= p.experts) el = -1;
+  int lead = lane, rank = 0;  // the first pair of this one's expert
+  for (int s = 0; s < p.pairs; ++s) {
+    const bool same = s < lane && __builtin_amdgcn_readlane(el, s) == el;
+    lead = same ? min(lead, s) : lead;
+    rank += same;
+  }
+  const uint32_t named = (uint32_t)__ballot(el >= 0 && lead == lane);
+  const int count = __popc(named), per = count ? 16 / count : 16;
+  if (wave == 0 && lane < p.pairs) {
+    expert_at[lane] = el >= 0 ? __popc(named & ((1u << lead) - 1)) : -1;
+    rank_at[lane] = rank;
+  }
+  const int place = wave / per, part = wave % per;
+  if (place < count) {  // uniform per wave
+    const int e = __builtin_amdgcn_readlane(el, nth_bit(named, place));
+    const uint32_t mine = (uint32_t)__ballot(el == e);
+    const bool live = n16 < __popc(mine);
+    const bf16* w = p.w + ((int64_t)e * p.N + n0 + n16 % EX_FUSED_N) * p.K;
+    const bf16* x = p.x + (int64_t)(live ? nth_bit(mine, n16) : 0) * p.ldx;
+    constexpr int U = 4;
+    const int kc = (p.K + 64 * per - 1) / (64 * per) * 64, k0 = part * kc, k1 = min(p.K, k0 + kc);
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    const u32x4 zero = {0u, 0u, 0u, 0u};
+    for (int k = k0; k < k1; k += 64 * U) {
+      u32x4 a[U][2], b[U][2];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int c = k + 64 * u + 16 * g4 + 8 * h;
+          a[u][h] = n16 < EX_FUSED_N && c < k1 ? *(const u32x4*)(w + c) : zero;
+          b[u][h] = live && c < k1 ? *(const u32x4*)(x + c) : zero;
+        }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a[u][h]), __builtin_bit_cast(bf16x8, b[u][h]),
+                                                        acc, 0, 0, 0);
+    }
+    if (n16 < EX_FUSED) *(f32x4*)&red[wave][n16][4 * g4] = acc;
+  }
+  __syncthreads();
+  const int t = tid / EX_FUSED_N, c = tid % EX_FUSED_N, n = n0 + c;  // N is a multiple of 8
+  if (t * p.top_k >= p.pairs) return;
+  float a = residual ? (float)residual[t * ldr + n] : 0.f;
+  for (int s = 0; s < p.top_k; ++s) {
+    const int pair = t * p.top_k + s, at = expert_at[pair];
+    const float w = (float)p.weights[pair];
+    if (at < 0 || no_weight(w)) continue;
+    float z = 0.f;
+    for (int i = 0; i < per; ++i) z += red[at * per + i][rank_at[pair]][c];
+    a += p.bias ? fmaf(w, (float)p.bias[(int64_t)p.index[pair] * p.N + n], z) : z;
+  }
+  out[(int64_t)t * p.N + n] = (bf16)a;
+#endif
+}
+
 // ---- out[t] = residual[t] + sum over s of y_r, eight channels a thread; without weights: dx ----
 // Bound by memory: 32768 tokens, 2 slots, 1024 channels with residual 78 us for 402 MB (5.1 TB/s); rows
 // loaded past the caches, where part of what the products just wrote still is: 15 us more.
@@ -1061,6 +1133,11 @@ extern "C" int strata_hip_expert_mlp(const strata_hip_expert_mlp_args* a, void* 
   g.out = a->y;
   g.N = a->out_dim;
   g.K = a->hidden;
+  if (a->tile == 1 && pairs <= EX_FUSED && pairs * a->hidden <= EX_FUSED_K) {
+    hipLaunchKernelGGL(expert_few_out_kernel, dim3((unsigned)(a->out_dim / EX_FUSED_N)), dim3(1024), 0, st, g, (const bf16*)a->residual,
+                       a->ldr, (bf16*)a->out);
+    return check_launch("expert_few_out_kernel");
+  }
   if (const int rc = launch_expert_gemm<EX_OUT, false>(g, pairs, a->experts, a->tile, st)) return rc;
   ExpertCombine c = {};
   c.y = a->y;

@@ -109,7 +109,8 @@ def test_few_rows_of_one_expert(gpu):
     _inside(_call(_to(c, gpu, False)), want["out"], "out")
 
 
-@pytest.mark.parametrize("T,E,k", [(1, 8, 2), (16, 3, 1), (4, 40, 4), (1, 2, 16), (8, 1, 2), (5, 512, 3)])
+@pytest.mark.parametrize("T,E,k", [(1, 8, 2), (16, 3, 1), (4, 40, 4), (1, 2, 16), (8, 1, 2), (5, 512, 3),
+                                   (1, 3, 1), (4, 2, 1), (1, 9, 3), (2, 5, 2), (1, 2, 4), (3, 1, 1)])
 def test_up_to_16_pairs(gpu, T, E, k):
     """Served without a plan: the same expert in several slots, indexes outside the range, weights of zero."""
     for seed, picks in ((18, None), (19, 0), (20, -1), (21, E)):
@@ -343,6 +344,17 @@ def test_custom_ops_agree(gpu):
     g = torch.ones_like(a[0])
     g[:, 0] = 2
     assert torch.equal(torch.autograd.grad(a[0], l, g)[0], torch.autograd.grad(b[0], l, g)[0])
+
+
+def test_the_same_graph_twice(gpu):
+    """A kept graph's second backward, after other calls, gives the first one's bits."""
+    d = _to(_case(400, 4, 2, 64, 136, 72, 22), gpu, True)
+    out = _call(d)
+    leaves = [d[n] for n in NAMES]
+    first = torch.autograd.grad(out, leaves, d["dout"], retain_graph=True)
+    torch.autograd.grad(_call(d), leaves, 2 * d["dout"])
+    again = torch.autograd.grad(out, leaves, d["dout"])
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
 
 
 def test_traced_by_a_compiler(gpu):
