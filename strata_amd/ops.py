@@ -1880,11 +1880,13 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
     n = len(params)
     cols = {"params": params, "grads": grads, "exp_avgs": exp_avgs, "exp_avg_sqs": exp_avg_sqs, "masters": masters,
             "exp_avg_scales": exp_avg_scales, "exp_avg_sq_scales": exp_avg_sq_scales}
-    if any(x is not None and len(x) != n for x in cols.values()):
-        raise ValueError(f"{name}: the lists must have one entry for each of the {n} parameters")
-    rates = [(float(r),) * n if isinstance(r, (int, float)) else tuple(map(float, r)) for r in (lr, weight_decay)]
-    if any(len(r) != n for r in rates):
-        raise ValueError(f"{name}: lr and weight_decay must be numbers or have one entry for each parameter")
+    for x in cols.values():
+        if x is not None and len(x) != n:
+            raise ValueError(f"{name}: the lists must have one entry for each of the {n} parameters")
+    rates = [float(r) if isinstance(r, (int, float)) else list(map(float, r)) for r in (lr, weight_decay)]
+    for r in rates:
+        if isinstance(r, list) and len(r) != n:
+            raise ValueError(f"{name}: lr and weight_decay must be numbers or have one entry for each parameter")
     _require_gpu(name, step)
     if step.dtype != torch.int64 or step.numel() != 1:
         raise ValueError(f"{name}: step must be an int64 tensor [1]")
@@ -1901,9 +1903,12 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
             continue
         want = blocks if what.endswith("scales") else sizes
         some = ts
-        if what not in _ADAMW_ALWAYS and any(t is None for t in ts):
+        if what not in _ADAMW_ALWAYS:
             some = [t for t in ts if t is not None]
-            want = [k for k, t in zip(want, ts) if t is not None]
+            if len(some) == n:
+                some = ts
+            else:
+                want = [k for k, t in zip(want, ts) if t is not None]
         if some and set(map(Tensor.get_device, some)) != {dev}:
             raise ValueError(f"{name}: every tensor must be on step's GPU (cuda:{dev}), {what} are not")
         kinds = list(map(_DTYPE_OF, some))
@@ -1916,12 +1921,14 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
         table[_ADAMW_FIELD[what]][:n] = np.fromiter(ptrs, np.int64, n)
         if what in ("params", "masters"):  # the moments are no one's graph's leaves
             written += some
-    codes = [d == torch.int8 for d in dtypes.get("exp_avgs", ())]
-    if codes != [d == torch.uint8 for d in dtypes.get("exp_avg_sqs", ())]:
+    m_kinds, v_kinds = dtypes["exp_avgs"], dtypes["exp_avg_sqs"]
+    plain = m_kinds.count(torch.float32) == n and v_kinds.count(torch.float32) == n  # no 8-bit moments
+    codes = None if plain else [d == torch.int8 for d in m_kinds]
+    if not plain and codes != [d == torch.uint8 for d in v_kinds]:
         raise ValueError(f"{name}: exp_avgs and exp_avg_sqs must both be fp32, or int8 and uint8")
     for what in ("exp_avg_scales", "exp_avg_sq_scales"):
         ts = cols[what]
-        if (any(codes) if ts is None else codes != [t is not None for t in ts]):
+        if (not plain) if ts is None else ([t is not None for t in ts] != (codes or [False] * n)):
             raise ValueError(f"{name}: 8-bit moments come with their scales, fp32 ones without")
     if n:
         table["n"][:n], table["lr"][:n], table["weight_decay"][:n] = sizes, rates[0], rates[1]
@@ -1929,7 +1936,7 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
             kinds = dtypes[what]
             same = kinds.count(kinds[0]) == n  # most often one type for all
             table[field][:n] = _ADAMW_CODE[kinds[0]] if same else [_ADAMW_CODE[d] for d in kinds]
-        table["state_bits"][:n] = [8 if c else 32 for c in codes]
+        table["state_bits"][:n] = 32 if plain else [8 if c else 32 for c in codes]
         if masters is not None and any(w is not None and d != torch.bfloat16 for w, d in zip(masters, dtypes["params"])):
             raise ValueError(f"{name}: masters belong to bfloat16 parameters")
     tp = ctypes.cast(table.ctypes.data, ctypes.POINTER(_lib.AdamwTensor))

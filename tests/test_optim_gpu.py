@@ -336,3 +336,30 @@ def test_offsets_past_32_bits(gpu, bits):
         if bits == 32:
             assert ((ts["exp_avgs"][0][sl].cpu().double() - m).abs() <= 8 * U * m.abs() + 1e-44).all()
     assert float(p[2**30]) == float(p[1000])
+
+
+def test_refusals(gpu):
+    """Kinds of moments that do not go together, sizes, layouts and places; nothing is changed by a refused call."""
+    ts = _tensors([300, 512], torch.bfloat16, torch.float32, 32, True, 31, gpu)
+    q8 = _tensors([300, 512], torch.bfloat16, torch.float32, 8, True, 31, gpu)
+    step = torch.zeros(1, dtype=torch.int64, device=gpu)
+    before = _copy(ts)
+    mix = lambda k: [ts[k][0], q8[k][1]]  # noqa: E731
+    for over, msg in (
+            (dict(exp_avgs=q8["exp_avgs"]), "both be fp32"), (dict(exp_avgs=mix("exp_avgs")), "both be fp32"),
+            (dict(exp_avg_scales=q8["exp_avg_scales"]), "scales"),
+            (dict(exp_avgs=q8["exp_avgs"], exp_avg_sqs=q8["exp_avg_sqs"], exp_avg_scales=None), "scales"),
+            (dict(exp_avgs=mix("exp_avgs"), exp_avg_sqs=mix("exp_avg_sqs"), exp_avg_scales=q8["exp_avg_scales"],
+                  exp_avg_sq_scales=q8["exp_avg_sq_scales"]), "scales"),
+            (dict(grads=ts["grads"][::-1]), "grads"), (dict(grads=[g.half() for g in ts["grads"]]), "grads"),
+            (dict(exp_avg_sqs=[t.repeat(2)[::2] for t in ts["exp_avg_sqs"]]), "contiguous"),
+            (dict(masters=[t.cpu() for t in ts["masters"]]), "step's GPU"), (dict(params=[t.float() for t in ts["params"]]), "masters"),
+            (dict(grads=[ts["exp_avgs"][0], ts["grads"][1]]), "gradient overlaps"), (dict(lr=[1e-3]), "one entry")):
+        with pytest.raises(ValueError, match=msg):
+            ops.adamw_step(**{**ts, **HP, "step": step, **over})
+    assert int(step) == 0
+    for k in ts:
+        assert all(x is None or torch.equal(x, y) for x, y in zip(ts[k], before[k])), k
+    both = {k: mix(k) for k in ts}
+    ops.adamw_step(**both, step=step, **HP)  # one of each kind in one call
+    assert int(step) == 1
