@@ -368,7 +368,8 @@ __global__ __launch_bounds__(64 * WGM * WGN, 1) void expert_gemm_kernel(ExpertGe
     float b8[8];
     {
       u32x4 b = {0u, 0u, 0u, 0u};
-      if (biased) b = BIG ? *(const u32x4*)(meta + BIAS + 2 * (wn * WTN + 8 * lc)) : *(const u32x4*)(p.bias + (int64_t)t.e * p.N + min(gn, p.N - 8));
+      if (biased)
+        b = BIG ? *(const u32x4*)(meta + BIAS + 2 * (wn * WTN + 8 * lc)) : *(const u32x4*)(p.bias + (int64_t)t.e * p.N + min(gn, p.N - 8));
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         b8[2 * x] = bf16_lo(b[x]);
@@ -931,7 +932,8 @@ __global__ __launch_bounds__(256) void expert_wgrad_sum_kernel(const float* part
   *(u32x2*)(out + i) = (u32x2){pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3])};
 }
 
-// 1: up to 16 pairs without a backward take no plan (`EX_DIRECT`); else rows of a tile.  Times of a whole forward replayed, us; E experts, C -> H -> C, a: pairs an expert:
+// 1: up to 16 pairs without a backward take no plan (`EX_DIRECT`); else rows of a tile.  Times of a
+// whole forward replayed, us; E experts, C -> H -> C, a: pairs an expert:
 //   16 (the few-rows kernel) under 4 pairs an expert without a backward (a 1, E 8, 1024 -> 4096: 36 against
 //     42 with 64; a 4: 41 / 45, but E 32, 512 -> 1024 32 / 30; a 12: 50 / 47);
 //   64 where the narrowest product would have fewer than 130 tiles of 128 x 128, half of the CUs (some 100:

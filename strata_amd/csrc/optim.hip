@@ -287,10 +287,10 @@ __device__ __forceinline__ int aw_settle(int k, double x, double scale, double s
 // them roots or reciprocals, for 10 bytes of a bf16 element): squares of codes are exact in
 // 32 bits, so that a moment costs two conversions, four products and a sum in 64 bits; these round
 // one by one, as the formula writes them, because a decayed scale and a share of a bf16 gradient
-// often add up to exactly half way between two 32-bit scales (0.9 s + 0.1 g); the largest magnitude is taken of the bits (one that
-// is no number stays: the block's scale then says so); and whether any of a lane's sixteen codes
-// is within 8e-5 of a border (a 32-bit place is off by at most 7e-5) is asked once, in a
-// seventh of all waves with yes.  VEC: a whole aligned run of eight, else `left` elements one by one.
+// often add up to exactly half way between two 32-bit scales (0.9 s + 0.1 g); the largest magnitude
+// is taken of the bits (one that is no number stays: the block's scale then says so); and whether
+// any of a lane's sixteen codes is within 8e-5 of a border (a 32-bit place is off by at most 7e-5)
+// is asked once, in a seventh of all waves with yes.  VEC: a whole aligned run of eight, else `left` elements one by one.
 template <bool P32, bool G32, bool MASTER, bool VEC>
 __device__ __forceinline__ void aw_block8(const AwTensor& t, const AwShared& s, int64_t i, int left) {
 #pragma clang fp contract(off)
@@ -403,7 +403,8 @@ __device__ __forceinline__ void aw_block8(const AwTensor& t, const AwShared& s, 
       store4(t.p, i, true, y0);
       store4(t.p, i + 4, true, y1);
     } else {
-      *(u32x4*)((bf16*)t.p + i) = (u32x4){pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]), pack_bf16x2(p[4], p[5]), pack_bf16x2(p[6], p[7])};
+      *(u32x4*)((bf16*)t.p + i) =
+          (u32x4){pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]), pack_bf16x2(p[4], p[5]), pack_bf16x2(p[6], p[7])};
     }
     store_once<u32x2>(mc + i, a);
     store_once<u32x2>(vc + i, b);

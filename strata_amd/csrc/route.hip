@@ -661,7 +661,8 @@ extern "C" int strata_hip_expert_route(const strata_hip_expert_route_args* a, vo
     while (threads > 32 && lds(threads) > 65536) threads /= 2;
     const size_t smem = lds(threads);
     const int64_t tok = threads / L, wgs = (p.tokens + tok - 1) / tok;
-    if (smem > 65536 || wgs * threads >= 0x100000000ll) return fail(STRATA_HIP_EUNSUPPORTED, "expert_route: problem too large for one launch");
+    if (smem > 65536 || wgs * threads >= 0x100000000ll)
+      return fail(STRATA_HIP_EUNSUPPORTED, "expert_route: problem too large for one launch");
     const dim3 grid((unsigned)wgs);
     auto go = [&](auto t, auto w, auto v) {
       hipLaunchKernelGGL((route_kernel<decltype(t), decltype(w)::value, decltype(v)::value, EPL, L>), grid, dim3(threads), smem,
@@ -716,7 +717,8 @@ extern "C" int64_t strata_hip_expert_plan_workspace(int64_t pairs, int32_t exper
 extern "C" int strata_hip_expert_plan(const strata_hip_expert_plan_args* a, void* stream) {
   using namespace strata;
   if (!a) return fail(STRATA_HIP_EINVAL, "expert_plan: null args");
-  if (a->pairs < 0 || a->experts <= 0 || a->tile <= 0 || a->top_k <= 0 || a->pairs % a->top_k) return fail(STRATA_HIP_EINVAL, "expert_plan: bad sizes");
+  if (a->pairs < 0 || a->experts <= 0 || a->tile <= 0 || a->top_k <= 0 || a->pairs % a->top_k)
+    return fail(STRATA_HIP_EINVAL, "expert_plan: bad sizes");
   if (a->experts > PLAN_MAX_E) return fail(STRATA_HIP_EUNSUPPORTED, "expert_plan: at most 512 experts");
   if (a->pairs > 0x7ffffff0) return fail(STRATA_HIP_EUNSUPPORTED, "expert_plan: too many pairs");
   if (!a->offsets || !a->tiles || (a->pairs > 0 && (!a->index || !a->weights || !a->row_token || !a->row_weight || !a->slot_row)))

@@ -1767,7 +1767,8 @@ def expert_mlp_bwd(dout: Tensor, x: Tensor, weights: Tensor, w1: Tensor, b1: Opt
     # the index is in the plan: one of the weights' shape stands for it
     _expert_check(name, x, weights, torch.empty_like(weights, dtype=torch.int32), w1, b1, w2, b2, None)
     if dout.dtype != torch.bfloat16 or tuple(dout.shape) != (*x.shape[:-1], w2.shape[1]) or dout.get_device() != x.get_device():
-        raise ValueError(f"{name}: dout must be bfloat16 {(*x.shape[:-1], w2.shape[1])} on x's GPU, got {dout.dtype} {tuple(dout.shape)}")
+        raise ValueError(f"{name}: dout must be bfloat16 {(*x.shape[:-1], w2.shape[1])} on x's GPU, got {dout.dtype} "
+                         f"{tuple(dout.shape)}")
     size = _expert_space(weights.numel(), *w1.shape[:2], w2.shape[1], _expert_tile(weights.numel(), w1, w2, True), True)[4]
     if space.dtype != torch.uint8 or space.numel() != size or not space.is_contiguous() or space.get_device() != x.get_device():
         raise ValueError(f"{name}: space must be the {size} bytes of expert_mlp_train, got {space.dtype} {tuple(space.shape)}")
@@ -1837,8 +1838,8 @@ def expert_mlp(x: Tensor, weights: Tensor, index: Tensor, w1: Tensor, b1: Option
     ``expert_route`` gives them, w1 ``[E, H, C]``, b1 ``[E, H]`` or None, w2 ``[E, N, H]``, b2
     ``[E, N]`` or None, residual ``[..., N]`` or None; widths multiples of 8, x and the output under
     2 GiB.  An index outside ``[0, E)`` adds nothing, and the same expert may stand in two slots.
-    No token is dropped for an expert's load; a weight under 2^-100 counts as 0.  Differentiable once, in every argument but the
-    index."""
+    No token is dropped for an expert's load; a weight under 2^-100 counts as 0.  Differentiable
+    once, in every argument but the index."""
     grad = _wants_grad(x, weights, w1, b1, w2, b2, residual)
     if not _eager(x, weights, index, w1, b1, w2, b2, residual):
         if grad:
