@@ -288,7 +288,9 @@ __global__ __launch_bounds__(256) void route_kernel(RouteParams p) {
 // The gradient at the logits.  With c the scale, S the sum of the chosen scores and a the
 // sum of dw s over them:  ds = c dw, or c / S (dw - a / S) renormalised;
 // softmax: dl = s (ds - sum of s ds), the sum zero when renormalised; sigmoid: dl = ds s (1 - s).
-// The chosen slots' dw reach their experts' lanes through a row of LDS.
+// The chosen slots' dw reach their experts' lanes through a row of LDS; renormalised, less the first
+// slot's (a common part of them changes nothing): one chosen expert, or equal dw, would leave the
+// roundings of dw in the place of a gradient of zero.
 template <typename T, bool VEC, int EPL, int L>
 __global__ __launch_bounds__(256) void route_bwd_kernel(RouteParams p) {
   constexpr int TOK = 256 / L;
@@ -308,11 +310,14 @@ __global__ __launch_bounds__(256) void route_bwd_kernel(RouteParams p) {
   }
   if (p.bias) route_row<float, EPL, VEC>(p.bias, e0, left, 0.f, bias);
   wave_sync();
-  if (live)
+  if (live) {
+    const int first = p.index[t * p.top_k];
+    const float common = p.renormalize && first >= 0 && first < E ? route_load<T>(p.dweights, t * p.top_k) : 0.f;
     for (int s = lane; s < p.top_k; s += L) {
       const int at = p.index[t * p.top_k + s];
-      if (at >= 0 && at < E) row[at] = route_load<T>(p.dweights, t * p.top_k + s);
+      if (at >= 0 && at < E) row[at] = route_load<T>(p.dweights, t * p.top_k + s) - common;
     }
+  }
   const float NONE = -__builtin_inff();
   float top = NONE;
 #pragma unroll

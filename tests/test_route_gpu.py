@@ -155,6 +155,19 @@ def test_route_gradient(gpu, T, E, k, score, renorm, dtype):
     assert (dl.cpu()[~ok] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_route_gradient_of_nothing(gpu, score, dtype):
+    """Renormalised weights of one chosen expert are constant, and equal gradients move nothing: zeros, not
+    the roundings of the gradients."""
+    l = _logits(70, 24, dtype, 9, 0.3).to(gpu)
+    dw = torch.randn(70, 1, generator=torch.Generator().manual_seed(1)).to(dtype).to(gpu)
+    for k in (1, 4):
+        x = l.clone().requires_grad_()
+        w, _ = ops.expert_route(x, k, score, renormalize=True, scale=2.5)
+        assert not torch.autograd.grad(w, x, dw.expand(70, k))[0].any()
+
+
 def test_route_repeats_and_replays(gpu):
     l = _logits(1000, 64, torch.float32, 8).to(gpu)
     b = (torch.randn(64, generator=torch.Generator().manual_seed(1)) * 0.1).to(gpu)
