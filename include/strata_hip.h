@@ -589,8 +589,8 @@ int strata_hip_gated_add(const strata_hip_gated_add_args* args, void* stream);
  *   largest sums of their two best keys stay (the lower of two equal groups)
  *   index[t, i] = the top_k largest keys left in falling order (the lower expert of two equal
  *   keys), -1 where none is left;  weights[t, i] = scale * s (/ sum of the chosen s), 0 with -1
- * A logit or bias that is not finite masks its expert (s = 0, never chosen).  Scores and keys
- * that decide (a bias or groups given) are held in 64 bits.  At most 512 experts, top_k 64.
+ * A logit or bias that is not finite masks its expert (s = 0, never chosen).  Keys (a bias or
+ * groups given) that 32 bits cannot tell apart are told apart in 64.  At most 512 experts, top_k 64.
  * logits: [tokens, experts], row stride ld; weights, dweights: [tokens, top_k] of the
  * logits' type; index: int32 [tokens, top_k]; dlogits: [tokens, experts] contiguous.
  * _bwd: dlogits from dweights and the forward's index (weights is not read).
