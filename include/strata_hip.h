@@ -589,6 +589,8 @@ int strata_hip_gated_add(const strata_hip_gated_add_args* args, void* stream);
  *   largest sums of their two best keys stay (the lower of two equal groups)
  *   index[t, i] = the top_k largest keys left in falling order (the lower expert of two equal
  *   keys), -1 where none is left;  weights[t, i] = scale * s (/ sum of the chosen s), 0 with -1
+ * A sum of chosen s too small for 32 bits is formed from the logits; s that are all 0 in 64 bits
+ * (softmax: 745 below the largest logit, sigmoid: below -709) give weights and a gradient of 0.
  * A logit or bias that is not finite masks its expert (s = 0, never chosen).  Keys (a bias or
  * groups given) that 32 bits cannot tell apart are told apart in 64.  At most 512 experts, top_k 64.
  * logits: [tokens, experts], row stride ld; weights, dweights: [tokens, top_k] of the

@@ -9,6 +9,12 @@
 //
 // A logit or bias that is not finite masks its expert.
 //
+// Renormalised weights of chosen scores that are all small are ratios of exponentials, relative
+// to the largest chosen logit m: s_i / s_j = exp(l_i - l_j) for a softmax, and for a sigmoid up to 1 + e^m.
+// Below a sum of 2^-30 weights and gradient are formed so: scores themselves are denormal in 32 bits
+// below a logit of -87 and 0 below -103, and 1 / sum is infinite.  Scores that are 0 in
+// 64 bits too (ROUTE_ZERO_*) give weights of 0.
+//
 // L lanes take a token, EPL consecutive experts each: the best key of a lane is found in
 // its registers, the token's by log2(L) exchanges, so a round of the choice costs a wave
 // 3 EPL + 6 log2(L) operations for 64 / L tokens.  Bound by those operations and their latency:
@@ -34,6 +40,9 @@ struct RouteParams {
 };
 
 constexpr int ROUTE_MAX_K = 64;
+constexpr float ROUTE_SMALL = 0x1p-30f;         // a sum of chosen scores under it is formed from the logits
+constexpr float ROUTE_ZERO_SOFTMAX = -745.f;    // exp of less is 0 in 64 bits
+constexpr float ROUTE_ZERO_SIGMOID = -709.75f;  // exp of minus less is infinite there
 
 template <typename T>
 __device__ __forceinline__ float route_load(const void* p, int64_t i) {
@@ -278,6 +287,32 @@ __global__ __launch_bounds__(256) void route_kernel(RouteParams p) {
   if (!live) return;
   float total = 0.f;
   for (int s = 0; s < p.top_k; ++s) total += sel[s];
+  if (p.renormalize && total < ROUTE_SMALL) {  // the same for a token's lanes
+    auto logit = [&](int s) { return chosen[s] >= 0 ? route_load<T>(p.logits, t * p.ld + chosen[s]) : -__builtin_inff(); };
+    float m = -__builtin_inff(), top = 0.f, sum = 0.f;
+#pragma unroll 1
+    for (int s = 0; s < p.top_k; ++s) m = fmaxf(m, logit(s));
+    if (p.score == STRATA_HIP_SCORE_SOFTMAX) {
+      top = -__builtin_inff();
+#pragma unroll 1
+      for (int e = lane; e < E; e += L) {
+        const float x = route_load<T>(p.logits, t * p.ld + e);
+        if (is_finite(x) && !(WIDE && p.bias && !is_finite(p.bias[e]))) top = fmaxf(top, x);
+      }
+      top = group_max<L>(top);
+    }
+    if (m - top >= (p.score == STRATA_HIP_SCORE_SOFTMAX ? ROUTE_ZERO_SOFTMAX : ROUTE_ZERO_SIGMOID)) {  // not with nothing chosen
+#pragma unroll 1
+      for (int s = 0; s < p.top_k; ++s) sum += expf(logit(s) - m);
+      const float f = p.scale / sum;
+#pragma unroll 1
+      for (int s = lane; s < p.top_k; s += L) {
+        route_store<T>(p.weights, t * p.top_k + s, expf(logit(s) - m) * f);
+        p.index[t * p.top_k + s] = chosen[s];
+      }
+      return;
+    }
+  }
   const float f = p.renormalize ? p.scale / (total > 0.f ? total : 1.f) : p.scale;
   for (int s = lane; s < p.top_k; s += L) {
     route_store<T>(p.weights, t * p.top_k + s, sel[s] * f);
@@ -359,6 +394,26 @@ __global__ __launch_bounds__(256) void route_bwd_kernel(RouteParams p) {
   }
   S = group_sum<L>(S);
   a = group_sum<L>(a);
+  if (p.renormalize && S < ROUTE_SMALL) {  // the same for a token's lanes: ratios in the place of scores
+    const bool softmax = p.score == STRATA_HIP_SCORE_SOFTMAX;
+    float m = NONE;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) m = chosen[i] ? fmaxf(m, l[i]) : m;
+    m = group_max<L>(m);
+    if (m - (softmax ? top : 0.f) >= (softmax ? ROUTE_ZERO_SOFTMAX : ROUTE_ZERO_SIGMOID)) {
+      S = 0.f;
+      a = 0.f;
+#pragma unroll
+      for (int i = 0; i < EPL; ++i)
+        if (chosen[i]) {
+          sc[i] = expf(l[i] - m);
+          S += sc[i];
+          a = fmaf(dw[i], sc[i], a);
+        }
+      S = group_sum<L>(S);
+      a = group_sum<L>(a);
+    }
+  }
   const bool norm = p.renormalize && S > 0.f;
   const float c = norm ? p.scale / S : p.scale, mean = norm ? a / S : 0.f;
   const float back = p.renormalize ? 0.f : p.scale * a;

@@ -1510,7 +1510,8 @@ def expert_route(logits: Tensor, top_k: int, score: str = "softmax", bias: Optio
     largest score + ``bias`` (fp32 ``[experts]``, for the balance of their load; it takes no part in
     the weights) are chosen in falling order, the lower one of two that are equal; of ``groups``
     equal groups only the ``top_groups`` with the largest sums of their two best count.  The weights
-    are ``scale`` times the chosen scores, divided by their sum with ``renormalize``.
+    are ``scale`` times the chosen scores, divided by their sum with ``renormalize`` (however small they are
+    in 32 bits; chosen scores that are all 0 in 64 bits, as a sigmoid's below -709, give weights of 0).
 
     A logit (or bias) that is not finite masks its expert; a token with too few experts left has
     index -1 and weight 0 in the slots that stay empty.  At most 512 experts and top_k 64.  The

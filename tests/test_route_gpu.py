@@ -213,3 +213,73 @@ def test_plan(gpu, n, E, tile):
     wt = [(e, int(off[e]) + r) for e in range(E) for r in range(0, int(count[e]), tile)]
     assert int(tiles[0]) == len(wt)
     assert tiles[1:1 + 2 * len(wt)].view(-1, 2).tolist() == [list(t) for t in wt]
+
+
+def _far(base, E, dtype, seed):
+    """Tokens whose logits lie near ``base``, every third one an ordinary one."""
+    g = torch.Generator().manual_seed(seed)
+    l = base + torch.randn(13, E, generator=g)
+    l[::3] -= base
+    return l.to(dtype)
+
+
+FAR = [-18.0, -21.0, -25.0, -60.0, -86.0, -87.5, -88.2, -89.0, -92.0, -95.0, -100.0, -104.0, -110.0, -200.0, -700.0]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("form", ["plain", "bias", "groups"])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_route_of_tiny_scores(gpu, score, form, dtype):
+    """Renormalised weights and their gradient where the chosen scores are small, denormal or 0 in 32 bits: the weights
+    are exp(l - m) / sum, m the largest chosen logit, up to 1 + e^m in a sigmoid.  Roundings: as in test_route (80 + top_k) u
+    and u of the exponent: |l - m|, or at most 25 where the scores' sum is above 2^-30 and they are taken as they are.
+    The gradient w (dw - mean): 25 for the exponent, 70 each for the sums of w and of w dw, 2 top_k, and some ten
+    of single operations, with |l - m| of at most 8: (240 + 2 top_k) u of w (|dw| + |dw of slot 0| + sum of w |dw|).
+    The reference's own: a softmax's s (ds - sum of s ds) leaves 2^-53 of each |dw| where the sum cancels to 0.
+    A softmax's chosen scores are small where its bias keeps it from the largest ones (here of two experts)."""
+    for base in FAR:
+        for E, k in ((8, 1), (8, 2), (24, 5), (64, 8), (132, 7)):
+            l = _far(base, E, dtype, E)
+            bias, groups, top = None, 1, 1
+            if form == "groups":
+                groups, top = E // 4, 2 + k // 4
+            if form != "plain" or score == "softmax":
+                bias = torch.zeros(E)
+            if score == "softmax":
+                l[:, E // 2: E // 2 + 2] = 0.0
+                bias[E // 2: E // 2 + 2] = -5.0
+            kw = dict(score=score, groups=groups, top_groups=top, renormalize=True, scale=2.5)
+            ww, wi = O.route(l, k, bias=bias, **kw)
+            x = l.to(gpu).requires_grad_()
+            w, i = ops.expert_route(x, k, bias=bias.to(gpu) if bias is not None else None, **kw)
+            what = (score, form, base, E, k)
+            assert torch.equal(i.cpu(), wi), what
+            lc = l.double().gather(1, wi.clamp_min(0).long())
+            half = 2.0**-8 if dtype == torch.bfloat16 else U
+            rel = U * ((lc - lc.amax(1, keepdim=True)).abs() + 25 + 80 + k) + half
+            assert torch.isfinite(w).all(), what
+            assert ((w.detach().cpu().double() - ww).abs() <= rel * ww + 1e-37).all(), what
+            dw = torch.randn(13, k, generator=torch.Generator().manual_seed(k)).to(dtype)
+            (dl,) = torch.autograd.grad(w, x, dw.to(gpu))
+            l64 = l.double().requires_grad_()
+            (want,) = torch.autograd.grad(O.route_weights(l64, wi, score, True, 2.5), l64, dw.double())
+            d = dw.double().abs()
+            mag = torch.zeros(13, E, dtype=torch.float64).scatter_add_(1, wi.long(), ww * (d + d[:, :1] + (ww * d).sum(1, keepdim=True) / 2.5))
+            tol = U * (240 + 2 * k) * mag + half * want.abs() + 2.5 * 2.0**-50 * d.sum(1, keepdim=True) + 1e-37
+            assert torch.isfinite(dl).all(), what
+            assert ((dl.cpu().double() - want).abs() <= tol).all(), what
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_route_of_scores_that_are_zero_in_64_bits(gpu, score):
+    """Logits so low that the scores are 0 in 64 bits too: an index, weights and gradients of 0."""
+    for low in (-1e3, -1e4, -1e30, torch.finfo(torch.float32).min):
+        l = torch.full((5, 8), low)
+        bias = torch.zeros(8)
+        if score == "softmax":
+            l[:, 3], bias[3] = 0.0, -5.0
+        x = l.to(gpu).requires_grad_()
+        w, i = ops.expert_route(x, 2, score, bias.to(gpu), renormalize=True)
+        assert i.tolist() == [[0, 1]] * 5 and not w.any(), low
+        (dl,) = torch.autograd.grad(w, x, torch.ones_like(w) + torch.arange(2, device=gpu))
+        assert not dl.any(), low
