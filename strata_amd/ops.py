@@ -22,6 +22,7 @@ from typing import Optional, Sequence
 import numpy as np
 import torch
 from torch import Tensor
+from torch.utils._device import DeviceContext
 
 from . import _lib
 
@@ -1424,14 +1425,27 @@ def _route_args(name, logits, bias, top_k, score, groups, top_groups, renormaliz
 
 
 _PLAIN = (Tensor, torch.nn.Parameter)
+_dispatch_modes, _function_modes = torch._C._len_torch_dispatch_stack, torch._C._len_torch_function_stack
+_functorch_level, _jit_trace = torch._C._functorch.peek_interpreter_stack, torch._C._get_tracing_state
+_batched = torch._C._functorch.is_legacy_batchedtensor  # gradients of autograd.grad(is_grads_batched=True)
+
+
+def _watched() -> bool:
+    """Whether someone is to see the operators that are called on plain tensors: a dispatch mode (make_fx,
+    fake tensors, selective checkpointing, counters), a functorch transform, a jit trace or a function mode
+    other than the one that sets the default device."""
+    if _dispatch_modes() or _functorch_level() is not None or _jit_trace() is not None:
+        return True
+    n = _function_modes()
+    return n > 0 and any(type(torch._C._get_function_stack_at(i)) is not DeviceContext for i in range(n))
 
 
 def _eager(*ts: Optional[Tensor]) -> bool:
-    """Whether these are plain tensors outside a tracing compiler: the operators of this section then
+    """Whether these are plain tensors that nothing traces or watches: the operators of this section then
     launch through a ``torch.autograd.Function`` of their own.  The custom op's dispatch and its
     registered autograd cost 25 us a forward and 55 us a backward of host time beside it, more
-    than the kernels of a small call; traced calls and tensor subclasses go through the custom op."""
-    if torch.compiler.is_compiling():
+    than the kernels of a small call; all other calls, and tensor subclasses, go through the custom op."""
+    if torch.compiler.is_compiling() or _watched():
         return False
     for t in ts:
         if t is not None and type(t) not in _PLAIN:
@@ -1444,6 +1458,7 @@ def _wants_grad(*ts: Optional[Tensor]) -> bool:
         for t in ts:
             if t is not None and t.requires_grad:
                 return True
+        return _functorch_level() is not None  # what a transform wraps may want one that the wrapper does not show
     return False
 
 
@@ -1491,7 +1506,8 @@ class _ExpertRoute(torch.autograd.Function):
             return (None,) * 8
         logits, bias, index = ctx.saved_tensors
         top_k, score, renormalize, scale = ctx.args
-        return _route_backward(dweights, logits, index, top_k, score, bias, renormalize, scale), *(None,) * 7
+        call = _route_backward if _eager(dweights, logits, bias) and not _batched(dweights) else expert_route_bwd
+        return call(dweights, logits, index, top_k, score, bias, renormalize, scale), *(None,) * 7
 
 
 @torch.library.custom_op("strata_hip::expert_route", mutates_args=())
@@ -1823,9 +1839,15 @@ class _ExpertMlp(torch.autograd.Function):
     def backward(ctx, dout):
         if dout is None:
             return (None,) * 8
-        n = ctx.needs_input_grad
+        n, saved = ctx.needs_input_grad, ctx.saved_tensors
         need = (n[0], n[1], n[3], n[4], n[5], n[6])
-        gx, gwt, g1, gb1, g2, gb2 = _expert_backward(dout, *ctx.saved_tensors, need) if any(need) else (None,) * 6
+        if not any(need):
+            grads = (None,) * 6
+        elif _eager(dout, *saved) and not _batched(dout):
+            grads = _expert_backward(dout, *saved, need)
+        else:
+            grads = [g if wanted else None for g, wanted in zip(expert_mlp_bwd(dout, *saved, need), need)]
+        gx, gwt, g1, gb1, g2, gb2 = grads
         return gx, gwt, None, g1, gb1, g2, gb2, dout if n[7] else None
 
 
@@ -1879,6 +1901,8 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
     ``weight_decay`` may be one number for every tensor.  With ``max_norm`` the norm is returned
     (fp64 ``[1]``), and one that is not finite leaves everything as it was, ``step`` too."""
     name = "adamw_step"
+    if _jit_trace() is not None or torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+        raise RuntimeError(f"{name}: no operator, a trace of it would leave the step out")
     n = len(params)
     cols = {"params": params, "grads": grads, "exp_avgs": exp_avgs, "exp_avg_sqs": exp_avg_sqs, "masters": masters,
             "exp_avg_scales": exp_avg_scales, "exp_avg_sq_scales": exp_avg_sq_scales}

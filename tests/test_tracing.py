@@ -1,0 +1,129 @@
+"""The experts' operators and the 8-bit moments' values where something traces, transforms or watches the calls: it sees the
+custom ops.  On the CPU, with the launches left out."""
+
+import pytest
+import torch
+from torch.fx.experimental.proxy_tensor import make_fx
+from torch.overrides import TorchFunctionMode
+from torch.utils._python_dispatch import TorchDispatchMode
+
+from strata_amd import ops
+
+BF16 = torch.bfloat16
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    seen = []
+    monkeypatch.setattr(ops, "_launch", lambda name, *a: seen.append(name))
+    monkeypatch.setattr(ops, "_require_gpu", lambda *a: None)
+    monkeypatch.setattr(ops, "_expert_check", lambda *a: None)
+    return seen
+
+
+def _mlp_args(T=6, E=4, k=2, C=16, H=24):
+    g = torch.Generator().manual_seed(0)
+    r = lambda *s: torch.randn(*s, generator=g).to(BF16)  # noqa: E731
+    return r(T, C), r(T, k), torch.randint(0, E, (T, k), generator=g, dtype=torch.int32), r(E, H, C), None, r(E, C, H), r(E, C)
+
+
+def _route(l):
+    return ops.expert_route(l, 2)[0]
+
+
+def _values(c):
+    return ops.adamw_state_values(c, torch.ones(1))
+
+
+def _calls():
+    x, *rest = _mlp_args()
+    return {"route": (_route, torch.randn(6, 8), "expert_route"), "mlp": (lambda x: ops.expert_mlp(x, *rest), x, "expert_mlp_fwd"),
+            "values": (_values, torch.zeros(8, dtype=torch.int8), "adamw_state_values")}
+
+
+@pytest.mark.parametrize("which", ["route", "mlp", "values"])
+def test_make_fx_records_the_op(launches, which):
+    f, x, op = _calls()[which]
+    targets = [str(n.target) for n in make_fx(f)(x).graph.nodes]
+    assert f"strata_hip.{op}.default" in targets, targets
+
+
+@pytest.mark.parametrize("which", ["route", "mlp"])
+def test_make_fx_records_the_backward(launches, which):
+    f, x, op = _calls()[which]
+    grad = lambda x: torch.autograd.grad(f(x).sum(), x)[0]  # noqa: E731
+    targets = [str(n.target) for n in make_fx(grad)(x.clone().requires_grad_()).graph.nodes]
+    op = op.replace("_fwd", "")
+    assert f"strata_hip.{op}_bwd.default" in targets and any(f"strata_hip.{op}" in t and "bwd" not in t for t in targets), targets
+
+
+@pytest.mark.parametrize("which", ["route", "mlp"])
+def test_a_backward_alone_is_recorded(launches, which):
+    """The forward outside the trace, the gradient inside."""
+    f, x, op = _calls()[which]
+    x = x.clone().requires_grad_()
+    y = f(x)
+    targets = [str(n.target) for n in make_fx(lambda d: torch.autograd.grad(y, x, d, retain_graph=True)[0])(torch.ones_like(y)).graph.nodes]
+    assert f"strata_hip.{op.replace('_fwd', '')}_bwd.default" in targets, targets
+
+
+@pytest.mark.parametrize("which", ["route", "mlp", "values"])
+def test_jit_trace_records_the_op(launches, which):
+    f, x, op = _calls()[which]
+    with torch.no_grad():
+        assert f"strata_hip::{op}" in str(torch.jit.trace(f, x, check_trace=False).graph)
+
+
+@pytest.mark.parametrize("which", ["route", "mlp", "values"])
+def test_modes_see_the_op(launches, which):
+    f, x, op = _calls()[which]
+    seen = []
+
+    class Dispatch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    class Function(TorchFunctionMode):
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    for mode in (Dispatch, Function):
+        seen.clear()
+        with mode():
+            f(x)
+        assert any(op in s for s in seen), (mode, seen)
+
+
+@pytest.mark.parametrize("which", ["route", "mlp", "values"])
+def test_vmap(launches, which):
+    f, x, _ = _calls()[which]
+    assert torch.vmap(f)(torch.stack([x, x, x])).shape[0] == 3 and len(launches) >= 3
+
+
+def test_batched_gradients_of_the_routing(launches):
+    x = torch.randn(6, 8, requires_grad=True)
+    (g,) = torch.autograd.grad(_route(x), x, torch.ones(3, 6, 2), is_grads_batched=True)
+    assert g.shape == (3, 6, 8) and launches.count("strata_hip_expert_route_bwd") == 3
+
+
+@pytest.mark.parametrize("which", ["route", "mlp", "values"])
+def test_plain_calls_take_the_short_path(launches, monkeypatch, which):
+    f, x, op = _calls()[which]
+
+    def no(*a, **k):
+        raise AssertionError("custom op called")
+
+    for name in ("_expert_route_op", "expert_mlp_fwd", "expert_mlp_train", "_state_values_op"):
+        monkeypatch.setattr(ops, name, no)
+    f(x)
+    with torch.device("cpu"):
+        f(x)
+    assert launches
+
+
+def test_a_trace_of_the_step_is_refused():
+    t = [torch.zeros(4)]
+    with pytest.raises(RuntimeError, match="trace"):
+        make_fx(lambda p: ops.adamw_step([p], t, t, t, torch.zeros(1, dtype=torch.int64)))(torch.zeros(4))
