@@ -1458,7 +1458,8 @@ def _wants_grad(*ts: Optional[Tensor]) -> bool:
         for t in ts:
             if t is not None and t.requires_grad:
                 return True
-        return _functorch_level() is not None  # what a transform wraps may want one that the wrapper does not show
+        # what a transform wraps may want one that the wrapper does not show
+        return not torch.compiler.is_compiling() and _functorch_level() is not None
     return False
 
 

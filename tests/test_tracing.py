@@ -127,3 +127,17 @@ def test_a_trace_of_the_step_is_refused():
     t = [torch.zeros(4)]
     with pytest.raises(RuntimeError, match="trace"):
         make_fx(lambda p: ops.adamw_step([p], t, t, t, torch.zeros(1, dtype=torch.int64)))(torch.zeros(4))
+
+
+def test_compiled_inference_takes_the_inference_op(launches):
+    """With gradients enabled but asked of nothing: the op that keeps nothing."""
+    _, *rest = _mlp_args()
+    seen = []
+
+    def backend(gm, _example):
+        seen.extend(str(n.target) for n in gm.graph.nodes)
+        return gm.forward
+
+    torch._dynamo.reset()
+    torch.compile(lambda x: ops.expert_mlp(x, *rest), backend=backend, fullgraph=True)(_mlp_args()[0])
+    assert any("expert_mlp_fwd" in t for t in seen) and not any("expert_mlp_train" in t for t in seen), seen
