@@ -1669,11 +1669,20 @@ def _expert_plan(index: Tensor, weights: Tensor, experts: int, tile: int) -> Ten
     return plan
 
 
+_TRAIN_TILE = 64    # the fewest rows of a tile under a backward
+_PLAN_BLOCK = 1024  # pairs that the plan counts together
+
+
 def _expert_space(n: int, E: int, H: int, N: int, tile: int, train: bool) -> tuple[int, int, int, int, int]:
-    """Byte offsets of dact, y, the plan and the plan's workspace behind h, and the size of all."""
+    """Byte offsets of dact, y, the plan and the plan's workspace behind h, and the size of all.  With
+    ``train`` they are the same for every tile and plain arithmetic, so that a number of tokens that a
+    compiler left open stays open."""
     dact = 2 * n * H
     y = dact + (2 * n * H if train else 0)
     plan = y + 4 * n * N
+    if train:
+        ws = plan + 4 * _plan_size(n, E, _TRAIN_TILE)
+        return dact, y, plan, ws, ws + 4 * E * ((n + _PLAN_BLOCK - 1) // _PLAN_BLOCK)
     if tile == 1:  # no plan
         return dact, y, plan, plan, plan
     ws = plan + 4 * _plan_size(n, E, tile)
@@ -1744,7 +1753,7 @@ def expert_mlp_train(x: Tensor, weights: Tensor, index: Tensor, w1: Tensor, b1: 
 @expert_mlp_train.register_fake
 def _(x, weights, index, w1, b1, w2, b2, residual):
     n, E, H, N = index.numel(), w1.shape[0], w1.shape[1], w2.shape[1]
-    size = _expert_space(n, E, H, N, _expert_tile(n, w1, w2, True), True)[4]
+    size = _expert_space(n, E, H, N, _TRAIN_TILE, True)[4]
     return x.new_empty((*x.shape[:-1], N)), x.new_empty((size,), dtype=torch.uint8)
 
 
@@ -1787,7 +1796,7 @@ def expert_mlp_bwd(dout: Tensor, x: Tensor, weights: Tensor, w1: Tensor, b1: Opt
     if dout.dtype != torch.bfloat16 or tuple(dout.shape) != (*x.shape[:-1], w2.shape[1]) or dout.get_device() != x.get_device():
         raise ValueError(f"{name}: dout must be bfloat16 {(*x.shape[:-1], w2.shape[1])} on x's GPU, got {dout.dtype} "
                          f"{tuple(dout.shape)}")
-    size = _expert_space(weights.numel(), *w1.shape[:2], w2.shape[1], _expert_tile(weights.numel(), w1, w2, True), True)[4]
+    size = _expert_space(weights.numel(), *w1.shape[:2], w2.shape[1], _TRAIN_TILE, True)[4]
     if space.dtype != torch.uint8 or space.numel() != size or not space.is_contiguous() or space.get_device() != x.get_device():
         raise ValueError(f"{name}: space must be the {size} bytes of expert_mlp_train, got {space.dtype} {tuple(space.shape)}")
     grads = _expert_backward(dout, x, weights, w1, b1, w2, b2, space, need)

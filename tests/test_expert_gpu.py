@@ -419,3 +419,23 @@ def test_refusals(gpu):
     (g,) = torch.autograd.grad(out.float().square().sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="differentiate twice"):
         g.sum().backward()
+
+
+def test_compiled_for_any_number_of_tokens(gpu):
+    """One compilation, several numbers of tokens: outputs and gradients as the direct calls'."""
+    from torch._dynamo.testing import CompileCounterWithBackend
+
+    base = _to(_case(8, 4, 2, 64, 72, 64, 23), gpu, False)
+    shared = [base[n].requires_grad_() for n in ("w1", "b1", "w2", "b2")]
+    counter = CompileCounterWithBackend("aot_eager")
+    torch._dynamo.reset()
+    f = torch.compile(lambda x, w, i, r: ops.expert_mlp(x, w, i, *shared, r), backend=counter, fullgraph=True, dynamic=True)
+    for T in (8, 333, 65, 2000):
+        d = _to(_case(T, 4, 2, 64, 72, 64, T), gpu, False)
+        x = d["x"].requires_grad_()
+        args = x, d["weights"], d["index"], d["residual"]
+        got, want = f(*args), ops.expert_mlp(*args[:3], *shared, args[3])
+        assert torch.equal(got, want), T
+        for a, b in zip(torch.autograd.grad(got, [x, *shared], d["dout"]), torch.autograd.grad(want, [x, *shared], d["dout"])):
+            assert torch.equal(a, b), T
+    assert counter.frame_count == 1

@@ -141,3 +141,51 @@ def test_compiled_inference_takes_the_inference_op(launches):
     torch._dynamo.reset()
     torch.compile(lambda x: ops.expert_mlp(x, *rest), backend=backend, fullgraph=True)(_mlp_args()[0])
     assert any("expert_mlp_fwd" in t for t in seen) and not any("expert_mlp_train" in t for t in seen), seen
+
+
+def test_training_leaves_the_number_of_tokens_open():
+    """The workspace's size under fake tensors is arithmetic of the tokens, and no size becomes a constant."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.symbolic_shapes import DimDynamic, ShapeEnv, StatelessSymbolicContext
+
+    env = ShapeEnv()
+    x, w, i, w1, b1, w2, b2 = _mlp_args(T=90)
+    with FakeTensorMode(shape_env=env) as mode:
+        open_rows = StatelessSymbolicContext(dynamic_sizes=[DimDynamic.DYNAMIC, DimDynamic.STATIC])
+        x, w, i = (mode.from_tensor(t, symbolic_context=open_rows, static_shapes=False) for t in (x, w, i))
+        w1, w2, b2 = (mode.from_tensor(t, static_shapes=True) for t in (w1, w2, b2))
+        out, space = torch.ops.strata_hip.expert_mlp_train(x, w, i, w1, b1, w2, b2, None)
+        grads = torch.ops.strata_hip.expert_mlp_bwd(out, x, w, w1, b1, w2, b2, space, [True, True, True, False, True, True])
+    for size in (x.shape[0], out.shape[0], space.shape[0], grads[0].shape[0]):
+        assert isinstance(size, torch.SymInt) and size.node.expr.free_symbols, size
+    assert not env.replacements, env.replacements
+
+
+@pytest.mark.parametrize("train", [False, True])
+def test_compiled_once_for_every_number_of_tokens(launches, train):
+    from torch._dynamo.testing import CompileCounterWithBackend
+
+    *_, w1, b1, w2, b2 = _mlp_args()
+    w1.requires_grad_(train)
+    counter = CompileCounterWithBackend("aot_eager")
+    torch._dynamo.reset()
+    f = torch.compile(lambda x, w, i: ops.expert_mlp(x, w, i, w1, b1, w2, b2), backend=counter, fullgraph=True, dynamic=True)
+    for T in (6, 90, 33, 5000):
+        y = f(*_mlp_args(T)[:3])
+        if train:
+            torch.autograd.grad(y.sum(), w1)
+    assert counter.frame_count == 1
+
+
+def test_training_workspace_holds_every_plan():
+    """Its size is taken for the smallest tile: no tile under a backward is smaller, no plan's workspace larger."""
+    from strata_amd import _lib
+
+    lib = _lib.load()
+    for n in (1, 63, 1023, 1024, 1025, 4000, 70001, 1 << 20):
+        for E in (1, 8, 60, 512):
+            dact, y, plan, ws, size = ops._expert_space(n, E, 64, 64, 64, True)
+            assert size - ws >= 4 * lib.strata_hip_expert_plan_workspace(n, E)
+            for width in (8, 768, 4096):
+                tile = lib.strata_hip_expert_tile(n, E, width, width, width, 1)
+                assert tile >= ops._TRAIN_TILE and ws - plan >= 4 * ops._plan_size(n, E, tile)
