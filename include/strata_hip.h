@@ -760,6 +760,10 @@ typedef struct strata_hip_adamw_args {
 
 int64_t strata_hip_adamw_workspace(const strata_hip_adamw_tensor* tensors, int64_t count);
 int strata_hip_adamw_step(const strata_hip_adamw_args* args, void* stream);
+/* The same for tensors that have not all taken the same steps: steps[i], of a HOST array of args->count
+ * device pointers, is the step count of tensor i (args->step is not read); tensors may share one, each is
+ * counted up once.  The norm is still that of all gradients.  workspace: 4 * count doubles more. */
+int strata_hip_adamw_step_counts(const strata_hip_adamw_args* args, int64_t* const* steps, void* stream);
 
 /* out[i] = what code i of an 8-bit moment stands for (see strata_hip_adamw_step), f32;
  * is_signed: 1 for exp_avg codes, 0 for exp_avg_sq codes.  codes 4-byte, out 16-byte aligned. */

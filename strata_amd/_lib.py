@@ -467,6 +467,8 @@ EXPORTS = {
     "strata_hip_expert_mlp_bwd": ([ctypes.POINTER(ExpertMlpBwdArgs), ctypes.c_void_p], ctypes.c_int),
     "strata_hip_adamw_workspace": ([ctypes.POINTER(AdamwTensor), ctypes.c_int64], ctypes.c_int64),
     "strata_hip_adamw_step": ([ctypes.POINTER(AdamwArgs), ctypes.c_void_p], ctypes.c_int),
+    "strata_hip_adamw_step_counts": (
+        [ctypes.POINTER(AdamwArgs), ctypes.POINTER(ctypes.c_void_p), ctypes.c_void_p], ctypes.c_int),
     "strata_hip_adamw_state_values": ([ctypes.POINTER(AdamwValuesArgs), ctypes.c_void_p], ctypes.c_int),
     "strata_hip_last_error": ([], ctypes.c_char_p),
     "strata_hip_abi_version": ([], ctypes.c_int),

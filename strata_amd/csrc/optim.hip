@@ -25,6 +25,7 @@
 #include <algorithm>
 #include <cmath>
 #include <new>
+#include <unordered_map>
 #include <vector>
 
 #include "common.h"
@@ -36,8 +37,9 @@ constexpr int AW_CHUNK = 4096;   // elements per workgroup of the step
 constexpr int AW_SUM = 16384;    // elements per workgroup of the sum of squares
 constexpr int AW_HEAD = 8;       // doubles before the partial sums
 constexpr int AW_PER = 48;       // tensors per launch: 80 bytes each in 4 KiB of arguments
+constexpr int AW_COUNTS = 448;   // step counts per launch of their own
 constexpr float AW_TINY = 0x1p-100f;  // the places of 8-bit codes under such a scale are found 2^100 larger: 65536 / scale leaves 32 bits
-enum { AW_P32 = 1, AW_G32 = 2, AW_ALIGNED = 4 };
+enum { AW_P32 = 1, AW_G32 = 2, AW_ALIGNED = 4, AW_COUNT_SHIFT = 8 };  // above: which step count is the tensor's
 
 struct AwTensor {
   void* p;
@@ -58,7 +60,7 @@ struct AwBatch {
   int count;
   float eps;
   double b1, b2;
-  const double* head;    // what aw_head_kernel left, see there
+  const double* head;    // what aw_head_kernel left for each step count, see there
 };
 struct SumBatch {
   const void* g[3 * AW_PER];
@@ -140,18 +142,24 @@ __global__ __launch_bounds__(256) void aw_sum_kernel(SumBatch b) {
   if (tid == 0) b.part[wg] = ((red[0] + red[1]) + red[2]) + red[3];
 }
 
-// ---- what every element shares: head[0] the factor c, [1] 1 / (1 - b1^t),
-// [2] 1 / sqrt(1 - b2^t), [3] 1 where the step is left out (a norm that is not finite).
-// One workgroup; the partial sums in a fixed order.
-__global__ __launch_bounds__(1024) void aw_head_kernel(double* head, const double* part, int64_t parts, int64_t* step,
-                                                       double* norm, double max_norm, double b1, double b2) {
+// ---- what every element of the tensors of one step count shares: head[0] the factor c,
+// [1] 1 / (1 - b1^t), [2] 1 / sqrt(1 - b2^t), [3] 1 where the step is left out (a norm that is not finite).
+struct AwNorm {
+  const double* part;
+  int64_t parts;
+  double* norm;  // or null: no clipping
+  double max_norm, b1, b2;
+};
+
+// c and whether the step is left out, in thread 0 of 1024; the partial sums in a fixed order.
+__device__ __forceinline__ void aw_clip(const AwNorm& a, double& c, bool& skip) {
   __shared__ double red[16];
   const int tid = threadIdx.x;
-  double c = 1.;
-  bool skip = false;
-  if (norm) {
+  c = 1.;
+  skip = false;
+  if (a.norm) {
     double s = 0.;
-    for (int64_t i = tid; i < parts; i += 1024) s += part[i];
+    for (int64_t i = tid; i < a.parts; i += 1024) s += a.part[i];
 #pragma unroll
     for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
     if ((tid & 63) == 0) red[tid >> 6] = s;
@@ -159,19 +167,47 @@ __global__ __launch_bounds__(1024) void aw_head_kernel(double* head, const doubl
     if (tid == 0) {
       for (int k = 1; k < 16; ++k) s += red[k];
       const double nrm = sqrt(s);
-      *norm = nrm;
+      *a.norm = nrm;
       skip = !(nrm < __builtin_inf());
-      c = fmin(1., max_norm / (nrm + 1e-6));
+      c = fmin(1., a.max_norm / (nrm + 1e-6));
     }
   }
-  if (tid == 0) {
-    const int64_t t = *step + (skip ? 0 : 1);
-    *step = t;
-    head[0] = c;
-    head[1] = 1. / (1. - pow(b1, (double)t));
-    head[2] = 1. / sqrt(1. - pow(b2, (double)t));
-    head[3] = skip ? 1. : 0.;
+}
+__device__ __forceinline__ void aw_count(const AwNorm& a, double* head, int64_t* step, double c, bool skip) {
+  const int64_t t = *step + (skip ? 0 : 1);
+  *step = t;
+  head[0] = c;
+  head[1] = 1. / (1. - pow(a.b1, (double)t));
+  head[2] = 1. / sqrt(1. - pow(a.b2, (double)t));
+  head[3] = skip ? 1. : 0.;
+}
+
+__global__ __launch_bounds__(1024) void aw_head_kernel(AwNorm a, double* head, int64_t* step) {
+  double c;
+  bool skip;
+  aw_clip(a, c, skip);
+  if (threadIdx.x == 0) aw_count(a, head, step, c, skip);
+}
+
+// Several counts, each with its head: the factor is the same for all.
+struct AwCounts {
+  int64_t* step[AW_COUNTS];
+  int count;
+};
+static_assert(sizeof(AwCounts) + sizeof(AwNorm) + 8 <= 4096, "kernel arguments");
+__global__ __launch_bounds__(1024) void aw_heads_kernel(AwNorm a, double* heads, AwCounts s) {
+  __shared__ double shared_c;
+  __shared__ int shared_skip;
+  double c;
+  bool skip;
+  aw_clip(a, c, skip);
+  if (threadIdx.x == 0) {
+    shared_c = c;
+    shared_skip = skip;
   }
+  __syncthreads();
+  const int k = threadIdx.x;
+  if (k < s.count) aw_count(a, heads + 4 * k, s.step[k], shared_c, shared_skip != 0);
 }
 
 // ---- the step ----
@@ -440,11 +476,12 @@ __global__ __launch_bounds__(256) void aw_step_kernel(AwBatch b) {
   if (b.head[3] != 0.) return;
   const int e = find_entry(b.count, wg, [&](int i) { return b.t[i].first; });
   const AwTensor t = b.t[e];
+  const double* head = b.head + 4 * (t.flags >> AW_COUNT_SHIFT);
   AwShared s;
-  const double c = b.head[0];
+  const double c = head[0];
   s.c = (float)c;
-  s.rate = t.lr * (float)b.head[1];
-  s.rbc2 = (float)b.head[2];
+  s.rate = t.lr * (float)head[1];
+  s.rbc2 = (float)head[2];
   s.eps = b.eps;
   s.decay = t.decay;
   s.db1 = b.b1;
@@ -503,11 +540,32 @@ static int64_t aw_parts(const strata_hip_adamw_tensor* t, int64_t count) {
   return parts;
 }
 
-static int aw_check(const strata_hip_adamw_args* a) {
-  if (!a) return fail(STRATA_HIP_EINVAL, "adamw_step: null args");
-  if (a->count < 0 || (a->count > 0 && !a->tensors)) return fail(STRATA_HIP_EINVAL, "adamw_step: bad tensor list");
-  if (!a->step || !a->workspace || ((uintptr_t)a->step & 7) || ((uintptr_t)a->workspace & 7))
-    return fail(STRATA_HIP_EINVAL, "adamw_step: step and workspace must be given, 8-byte aligned");
+// The distinct step counts of a call (`of`: which one each tensor has), in the order of their first tensors.
+struct AwSteps {
+  std::vector<int64_t*> each;
+  std::vector<uint32_t> of;
+};
+
+static void aw_steps(const strata_hip_adamw_args* a, int64_t* const* steps, AwSteps& s) {
+  if (!steps) {
+    s.each.push_back(a->step);
+    return;
+  }
+  std::unordered_map<int64_t*, uint32_t> seen;
+  s.of.resize((size_t)a->count);
+  for (int64_t i = 0; i < a->count; ++i) {
+    const auto at = seen.emplace(steps[i], (uint32_t)s.each.size());
+    if (at.second) s.each.push_back(steps[i]);
+    s.of[(size_t)i] = at.first->second;
+  }
+}
+
+static int aw_check(const strata_hip_adamw_args* a, const AwSteps& steps) {
+  for (const int64_t* step : steps.each)
+    if (!step || ((uintptr_t)step & 7)) return fail(STRATA_HIP_EINVAL, "adamw_step: step must be given, 8-byte aligned");
+  if (!a->workspace || ((uintptr_t)a->workspace & 7))
+    return fail(STRATA_HIP_EINVAL, "adamw_step: workspace must be given, 8-byte aligned");
+  if (steps.each.size() > 0xffffff) return fail(STRATA_HIP_EUNSUPPORTED, "adamw_step: too many step counts for one call");
   if (!(a->beta1 >= 0. && a->beta1 < 1. && a->beta2 >= 0. && a->beta2 < 1.))
     return fail(STRATA_HIP_EINVAL, "adamw_step: betas must lie in [0, 1)");
   if (!(a->eps >= 0.) || !std::isfinite(a->eps))
@@ -515,9 +573,9 @@ static int aw_check(const strata_hip_adamw_args* a) {
   if (!std::isfinite(a->max_norm) || (a->max_norm > 0. && (!a->norm || ((uintptr_t)a->norm & 7))))
     return fail(STRATA_HIP_EINVAL, "adamw_step: max_norm must be finite and norm given with it, 8-byte aligned");
   std::vector<std::pair<uintptr_t, uintptr_t>> written, read;
-  written.reserve((size_t)a->count * 6 + 1);
+  written.reserve((size_t)a->count * 6 + steps.each.size());
   read.reserve((size_t)a->count);
-  written.emplace_back((uintptr_t)a->step, (uintptr_t)a->step + 8);
+  for (const int64_t* step : steps.each) written.emplace_back((uintptr_t)step, (uintptr_t)step + 8);
   int64_t chunks = 0;
   for (int64_t i = 0; i < a->count; ++i) {
     const strata_hip_adamw_tensor& t = a->tensors[i];
@@ -562,8 +620,12 @@ static int aw_check(const strata_hip_adamw_args* a) {
   return STRATA_HIP_OK;
 }
 
-static int aw_launch(const strata_hip_adamw_args* a, hipStream_t st) {
-  if (const int rc = aw_check(a)) return rc;
+static int aw_launch(const strata_hip_adamw_args* a, int64_t* const* steps, hipStream_t st) {
+  if (!a) return fail(STRATA_HIP_EINVAL, "adamw_step: null args");
+  if (a->count < 0 || (a->count > 0 && !a->tensors)) return fail(STRATA_HIP_EINVAL, "adamw_step: bad tensor list");
+  AwSteps counts;
+  aw_steps(a, steps, counts);
+  if (const int rc = aw_check(a, counts)) return rc;
   double* part = a->workspace + AW_HEAD;
   int64_t parts = 0;
   if (a->max_norm > 0.) {
@@ -593,15 +655,30 @@ static int aw_launch(const strata_hip_adamw_args* a, hipStream_t st) {
     }
     if (const int rc = flush()) return rc;
   }
-  hipLaunchKernelGGL(aw_head_kernel, dim3(1), dim3(1024), 0, st, a->workspace, part, parts, a->step,
-                     a->max_norm > 0. ? a->norm : nullptr, a->max_norm, a->beta1, a->beta2);
-  if (const int rc = check_launch("adamw head")) return rc;
+  const bool clip = a->max_norm > 0.;
+  const AwNorm norm = {part, parts, clip ? a->norm : nullptr, a->max_norm, a->beta1, a->beta2};
+  double* heads = a->workspace;
+  if (counts.each.size() == 1) {
+    hipLaunchKernelGGL(aw_head_kernel, dim3(1), dim3(1024), 0, st, norm, heads, counts.each[0]);
+    if (const int rc = check_launch("adamw head")) return rc;
+  } else {
+    heads = part + aw_parts(a->tensors, a->count);
+    AwCounts c;
+    size_t k = 0;
+    do {  // without a tensor: the norm alone
+      c.count = (int)std::min(counts.each.size() - k, (size_t)AW_COUNTS);
+      std::copy_n(counts.each.begin() + k, c.count, c.step);
+      hipLaunchKernelGGL(aw_heads_kernel, dim3(1), dim3(1024), 0, st, norm, heads + 4 * k, c);
+      if (const int rc = check_launch("adamw heads")) return rc;
+      k += AW_COUNTS;
+    } while (k < counts.each.size());
+  }
   AwBatch b;
   b.count = 0;
   b.eps = (float)a->eps;
   b.b1 = a->beta1;
   b.b2 = a->beta2;
-  b.head = a->workspace;
+  b.head = heads;
   for (const bool q8 : {false, true}) {  // a launch takes tensors of one kind of moments
     uint32_t wgs = 0;
     auto flush = [&]() -> int {
@@ -629,7 +706,7 @@ static int aw_launch(const strata_hip_adamw_args* a, hipStream_t st) {
       o.first = wgs;
       const uintptr_t all = (uintptr_t)t.param | (uintptr_t)t.grad | (uintptr_t)t.exp_avg | (uintptr_t)t.exp_avg_sq | (uintptr_t)t.master;
       o.flags = (t.param_dtype == STRATA_HIP_F32 ? AW_P32 : 0) | (t.grad_dtype == STRATA_HIP_F32 ? AW_G32 : 0) |
-                ((all & 15) ? 0 : AW_ALIGNED);
+                ((all & 15) ? 0 : AW_ALIGNED) | (steps ? counts.of[(size_t)i] << AW_COUNT_SHIFT : 0);
       wgs += (uint32_t)((t.n + AW_CHUNK - 1) / AW_CHUNK);
       if (b.count == AW_PER)
         if (const int rc = flush()) return rc;
@@ -648,7 +725,16 @@ extern "C" int64_t strata_hip_adamw_workspace(const strata_hip_adamw_tensor* ten
 
 extern "C" int strata_hip_adamw_step(const strata_hip_adamw_args* a, void* stream) {
   try {
-    return strata::aw_launch(a, (hipStream_t)stream);
+    return strata::aw_launch(a, nullptr, (hipStream_t)stream);
+  } catch (const std::bad_alloc&) {
+    return strata::fail(STRATA_HIP_EUNSUPPORTED, "adamw_step: out of host memory");
+  }
+}
+
+extern "C" int strata_hip_adamw_step_counts(const strata_hip_adamw_args* a, int64_t* const* steps, void* stream) {
+  if (!steps) return strata::fail(STRATA_HIP_EINVAL, "adamw_step: null steps");
+  try {
+    return strata::aw_launch(a, steps, (hipStream_t)stream);
   } catch (const std::bad_alloc&) {
     return strata::fail(STRATA_HIP_EUNSUPPORTED, "adamw_step: out of host memory");
   }

@@ -1890,7 +1890,7 @@ STATE_BLOCK = 256  # consecutive elements that share a scale of an 8-bit moment
 
 
 def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequence[Tensor],
-               exp_avg_sqs: Sequence[Tensor], step: Tensor, *, lr: float | Sequence[float] = 1e-3,
+               exp_avg_sqs: Sequence[Tensor], step: Tensor | Sequence[Tensor], *, lr: float | Sequence[float] = 1e-3,
                betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                weight_decay: float | Sequence[float] = 0.01, max_norm: Optional[float] = None,
                masters: Optional[Sequence[Optional[Tensor]]] = None,
@@ -1907,7 +1907,8 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
     codes with fp32 scales ``[ceil(numel / 256)]`` in ``exp_avg_scales`` / ``exp_avg_sq_scales``
     (``adamw_state_values`` says what they stand for; zero codes and scales are zero moments).
     ``masters``: fp32 weights (or None) that a bf16 parameter is rounded from.  ``step`` is an int64
-    tensor ``[1]`` on the GPU, counted up, so that a captured step counts on; ``lr`` and
+    tensor ``[1]`` on the GPU, counted up, so that a captured step counts on, or one for each parameter
+    (the same tensor where they have taken the same steps: it is counted up once); ``lr`` and
     ``weight_decay`` may be one number for every tensor.  With ``max_norm`` the norm is returned
     (fp64 ``[1]``), and one that is not finite leaves everything as it was, ``step`` too."""
     name = "adamw_step"
@@ -1923,8 +1924,16 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
     for r in rates:
         if isinstance(r, list) and len(r) != n:
             raise ValueError(f"{name}: lr and weight_decay must be numbers or have one entry for each parameter")
-    _require_gpu(name, step)
-    if step.dtype != torch.int64 or step.numel() != 1:
+    steps, each = None, [step]
+    if not isinstance(step, Tensor):
+        steps = list(step)
+        if len(steps) != n or not n:
+            raise ValueError(f"{name}: step must be a tensor or have one for each of the {n} parameters")
+        each = list({id(t): t for t in steps}.values())
+        step = each[0]
+        steps = steps if len(each) > 1 else None
+    _require_gpu(name, *each)
+    if any(t.dtype != torch.int64 or t.numel() != 1 for t in each):
         raise ValueError(f"{name}: step must be an int64 tensor [1]")
     if max_norm is not None and not (0 < max_norm < math.inf):
         raise ValueError(f"{name}: max_norm must be positive and finite")
@@ -1933,7 +1942,7 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
     dev, sizes = step.get_device(), list(map(Tensor.numel, params))
     blocks = [-(-k // STATE_BLOCK) for k in sizes]
     table = np.zeros(max(n, 1), dtype=_ADAMW_TABLE)
-    dtypes, written = {}, [step]
+    dtypes, written = {}, each
     for what, ts in cols.items():
         if ts is None:
             continue
@@ -1976,11 +1985,15 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
         if masters is not None and any(w is not None and d != torch.bfloat16 for w, d in zip(masters, dtypes["params"])):
             raise ValueError(f"{name}: masters belong to bfloat16 parameters")
     tp = ctypes.cast(table.ctypes.data, ctypes.POINTER(_lib.AdamwTensor))
-    ws = torch.empty(int(_lib.function("strata_hip_adamw_workspace")(tp, n)), dtype=torch.float64, device=step.device)
+    doubles = int(_lib.function("strata_hip_adamw_workspace")(tp, n)) + (4 * n if steps else 0)
+    ws = torch.empty(doubles, dtype=torch.float64, device=step.device)
     norm = torch.empty(1, dtype=torch.float64, device=step.device) if max_norm is not None else None
     a = _lib.AdamwArgs(tp, n, step.data_ptr(), norm.data_ptr() if norm is not None else None, ws.data_ptr(),
                        float(betas[0]), float(betas[1]), float(eps), float(max_norm or 0.0))
-    _launch("strata_hip_adamw_step", a, step)
+    if steps:
+        _launch("strata_hip_adamw_step_counts", a, step, (ctypes.c_void_p * n)(*map(Tensor.data_ptr, steps)))
+    else:
+        _launch("strata_hip_adamw_step", a, step)
     try:
         torch.autograd.graph.increment_version(written)
     except RuntimeError:  # tensors made in inference mode carry no version

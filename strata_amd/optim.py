@@ -27,8 +27,10 @@ class AdamW(torch.optim.Optimizer):
                 left out whole.
 
     ``lr`` and ``weight_decay`` may differ between parameter groups, ``betas`` and ``eps`` are
-    the optimizer's.  One step count on the GPU serves every parameter: a step can be captured in
-    a graph (after one eager step has made the states; the rates are those of the capture).
+    the optimizer's.  A parameter counts the steps that it took (with a gradient), for its bias corrections;
+    parameters that have taken the same ones share a count, which lives on the GPU.  A step can be
+    captured in a graph, after one eager step with the same gradients has made the states and counts (the
+    rates are those of the capture).
 
     A master weight stands for its parameter once it exists, at the first step: a value written
     into the parameter later (loaded weights, an average) goes into ``state[p]["master"]`` too, or
@@ -72,6 +74,22 @@ class AdamW(torch.optim.Optimizer):
             s["master"] = p.detach().float()
         return s
 
+    def _uncaptured(self) -> None:
+        if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW: a step is captured after an eager one with the same gradients, which makes its states")
+
+    def _split_counts(self, states: list[dict]) -> None:
+        """States that this step leaves out keep their count: a copy of one that they share with others."""
+        taking, counts, kept = set(map(id, states)), {id(s["step"]) for s in states}, {}
+        for s in self.state.values():
+            step = s.get("step")
+            if step is None or id(s) in taking or id(step) not in counts:
+                continue
+            if id(step) not in kept:
+                self._uncaptured()
+                kept[id(step)] = step.clone()
+            s["step"] = kept[id(step)]
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
@@ -90,29 +108,34 @@ class AdamW(torch.optim.Optimizer):
                 wds.append(group["weight_decay"])
         if not ps:
             return loss
-        step = next((s["step"] for s in self.state.values() if "step" in s), None)
-        if step is None:
+        new = [p for p in ps if not self.state[p]]
+        if new:
+            self._uncaptured()
             step = torch.zeros(1, dtype=torch.int64, device=ps[0].device)
-        for p in ps:
-            if not self.state[p]:
+            for p in new:
                 self.state[p].update(self._new_state(p, step))
         states = [self.state[p] for p in ps]
+        if len(self.state) > len(ps):
+            self._split_counts(states)
         self.grad_norm = ops.adamw_step(
             ps, [p.grad.contiguous() for p in ps], [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states],
-            step, lr=lrs, betas=self.betas, eps=self.eps, weight_decay=wds, max_norm=self.max_norm,
+            [s["step"] for s in states], lr=lrs, betas=self.betas, eps=self.eps, weight_decay=wds, max_norm=self.max_norm,
             masters=[s.get("master") for s in states], exp_avg_scales=[s.get("exp_avg_scale") for s in states],
             exp_avg_sq_scales=[s.get("exp_avg_sq_scale") for s in states])
         return loss
 
     def load_state_dict(self, state_dict) -> None:
         """As torch's, but every state keeps the type it was saved in (torch's would round the fp32
-        moments and master weights of a bf16 parameter to bf16)."""
+        moments and master weights of a bf16 parameter to bf16), and equal counts become one."""
         super().load_state_dict(state_dict)
         saved = chain.from_iterable(g["params"] for g in state_dict["param_groups"])
-        step = None
+        counts, values = {}, {}
         for i, p in zip(saved, chain.from_iterable(g["params"] for g in self.param_groups)):
             if i not in state_dict["state"]:
                 continue
             s = {k: v.detach().to(p.device, copy=True) for k, v in state_dict["state"][i].items()}
-            step = s["step"] = s["step"] if step is None else step
+            one = state_dict["state"][i]["step"]
+            if id(one) not in values:
+                values[id(one)] = int(one)
+            s["step"] = counts.setdefault(values[id(one)], s["step"])
             self.state[p] = s

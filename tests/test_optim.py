@@ -115,3 +115,90 @@ def test_copies_and_pickles():
         assert (o.betas, o.eps, o.max_norm, o.state_bits, o.master, o.min_8bit) == ((0.8, 0.9), 1e-6, 2.0, 8, False, 16)
         q = o.param_groups[0]["params"][0]
         assert o.param_groups[0]["lr"] == 0.5 and int(o.state[q]["step"]) == 1 and o.grad_norm is None
+
+
+def test_c_entry_with_counts_refuses(lib):
+    """Each tensor's own count: given, aligned, apart from what is written and read."""
+    t = (_lib.AdamwTensor * 2)()
+    for i in range(2):
+        base = 0x100000 * (i + 1)
+        t[i] = (base, base + 0x10000, base + 0x20000, base + 0x30000, None, None, None, 100, 1e-3, 0.1, _lib.BF16, _lib.BF16, 32, 0)
+    a = _lib.AdamwArgs(t, 2, None, 0x2000, 0x3000, 0.9, 0.95, 1e-8, 0.0)
+    for steps, msg in (((0x1000, None), "step"), ((0x1000, 0x1104), "aligned"), ((0x1000, 0x100000), "overlap"),
+                       ((0x1000, 0x110000), "gradient"), ((0x120008, 0x1000), "overlap")):
+        rc = lib.strata_hip_adamw_step_counts(ctypes.byref(a), (ctypes.c_void_p * 2)(*steps), None)
+        assert rc == _lib.EINVAL and msg in lib.strata_hip_last_error().decode(), steps
+    assert lib.strata_hip_adamw_step_counts(ctypes.byref(a), None, None) == _lib.EINVAL
+
+
+def test_ops_refuse_bad_counts():
+    p, step = [torch.zeros(4)] * 2, torch.zeros(1, dtype=torch.int64)
+    with pytest.raises(ValueError, match="one for each"):
+        ops.adamw_step(p, p, p, p, [step])
+    with pytest.raises(ValueError, match="GPU"):
+        ops.adamw_step(p, p, p, p, [step, step])
+
+
+@pytest.fixture
+def counted(monkeypatch):
+    """AdamW whose steps only count; (the optimizer, its parameters, step(which have gradients), counts)."""
+    def fake(params, grads, m, v, step, **kw):
+        for t in {id(t): t for t in step}.values():
+            t += 1
+
+    monkeypatch.setattr(ops, "adamw_step", fake)
+    ps = [torch.nn.Parameter(torch.zeros(4)) for _ in range(4)]
+    opt = AdamW(ps)
+
+    def step(which):
+        for k, p in enumerate(ps):
+            p.grad = torch.ones(4) if k in which else None
+        opt.step()
+
+    return opt, ps, step, lambda: [int(opt.state[p]["step"]) if opt.state.get(p) else 0 for p in ps]
+
+
+def test_each_parameter_counts_its_own_steps(counted):
+    """As torch's: late ones, ones left out for a while, a group added later; those alike share a count."""
+    opt, ps, step, counts = counted
+    ref = torch.optim.AdamW([p.detach().clone().requires_grad_() for p in ps])
+    for which in ((0, 1), (0, 1), (0, 1, 2), (0, 2), (2, 3), (0, 1, 2, 3), (1,), (0, 1, 2, 3)):
+        for k, q in enumerate(ref.param_groups[0]["params"]):
+            q.grad = torch.ones(4) if k in which else None
+        ref.step()
+        step(which)
+        want = [int(ref.state[q]["step"]) if q in ref.state else 0 for q in ref.param_groups[0]["params"]]
+        assert counts() == want, which
+    late = torch.nn.Parameter(torch.zeros(4))
+    opt.add_param_group(dict(params=[late]))
+    late.grad = torch.ones(4)
+    step(range(4))
+    assert int(opt.state[late]["step"]) == 1 and counts() == [w + 1 for w in want]
+
+
+def test_counts_are_shared_and_survive_a_state_dict(counted):
+    opt, ps, step, counts = counted
+    step((0, 1))
+    step((0, 1, 2, 3))
+    assert opt.state[ps[0]]["step"] is opt.state[ps[1]]["step"] and opt.state[ps[2]]["step"] is opt.state[ps[3]]["step"]
+    other = AdamW([torch.nn.Parameter(torch.zeros(4)) for _ in ps])
+    other.load_state_dict(opt.state_dict())
+    loaded = [other.state[p]["step"] for p in other.param_groups[0]["params"]]
+    assert [int(t) for t in loaded] == counts() == [2, 2, 1, 1] and loaded[0] is loaded[1] and loaded[2] is loaded[3]
+    assert not {id(t) for t in loaded} & {id(s["step"]) for s in opt.state.values()}
+
+
+def test_a_capture_makes_no_states(counted, monkeypatch):
+    """States and counts made inside a capture would be made again by every replay."""
+    opt, ps, step, counts = counted
+    monkeypatch.setattr(torch.cuda, "is_initialized", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="eager"):
+        step((0, 1))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    step((0, 1))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    step((0, 1))
+    with pytest.raises(RuntimeError, match="eager"):
+        step((0,))
+    assert counts() == [2, 2, 0, 0]

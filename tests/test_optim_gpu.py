@@ -363,3 +363,92 @@ def test_refusals(gpu):
     both = {k: mix(k) for k in ts}
     ops.adamw_step(**both, step=step, **HP)  # one of each kind in one call
     assert int(step) == 1
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("clip", [None, 0.7])
+def test_counts_of_their_own(gpu, bits, clip):
+    """Tensors of three counts in one call, one norm over all of them."""
+    ts = _tensors(SIZES, torch.bfloat16, torch.float32, bits, True, 41, gpu)
+    n = len(SIZES)
+    kinds = [torch.full((1,), k, dtype=torch.int64, device=gpu) for k in (0, 7, 400)]
+    steps = [kinds[i % 3] for i in range(n)]
+    norm = O.global_norm([g.cpu() for g in ts["grads"]])
+    for more in (1, 2):
+        before = _copy(ts)
+        got = ops.adamw_step(**ts, step=steps, max_norm=clip, **HP)
+        assert [int(k) for k in kinds] == [more, 7 + more, 400 + more]
+        assert got is None if clip is None else abs(float(got) - norm) <= 1e-12 * norm
+        for k in range(3):
+            part = lambda d: {c: x[k::3] for c, x in d.items()}  # noqa: E731
+            _check(part(ts), part(before), int(kinds[k]), min(1.0, clip / (norm + 1e-6)) if clip else 1.0)
+
+
+def test_more_counts_than_a_launch_takes(gpu):
+    """A count for each of 1000 tensors, and a norm that is not finite: all stay."""
+    ts = _tensors([3] * 1000, torch.float32, torch.float32, 32, False, 42, gpu)
+    steps = list(torch.arange(1000, device=gpu).split(1))
+    before = _copy(ts)
+    norm = float(ops.adamw_step(**ts, step=steps, max_norm=1.0, **HP))
+    assert torch.cat(steps).tolist() == list(range(1, 1001))
+    for i in (0, 1, 447, 448, 449, 895, 896, 999):
+        one = lambda d: {c: x[i:i + 1] for c, x in d.items()}  # noqa: E731
+        _check(one(ts), one(before), i + 1, min(1.0, 1.0 / (norm + 1e-6)))
+    ts["grads"][500][1] = math.nan
+    before = _copy(ts)
+    assert math.isnan(float(ops.adamw_step(**ts, step=steps, max_norm=1.0, **HP)))
+    assert torch.cat(steps).tolist() == list(range(1, 1001))
+    assert all(torch.equal(x, y) for x, y in zip(ts["params"], before["params"]))
+
+
+def test_late_and_missing_parameters_as_torch(gpu):
+    """Parameters without a gradient at first, for a while, and a group added later, against torch's step in 64 bits.
+    8 steps, each off by at most 24 u of its size (up to 12 lr while the moments are young, the errors of
+    the moments' up to 8 steps among them) and 3 u of |p|."""
+    lr, gen = 1e-2, torch.Generator().manual_seed(43)
+    start = [torch.randn(300, generator=gen) * 0.1 for _ in range(4)]
+    ps = [torch.nn.Parameter(t.to(gpu)) for t in start]
+    qs = [torch.nn.Parameter(t.double()) for t in start]
+    ours, ref = AdamW(ps[:3], lr=lr, max_norm=3.0), torch.optim.AdamW(qs[:3], lr=lr)
+    for k, which in enumerate(((0,), (0, 1), (0, 1), (0, 2), (0, 1, 2), (1,), (0, 1, 2, 3), (0, 1, 2, 3))):
+        if k == 6:
+            ours.add_param_group(dict(params=[ps[3]]))
+            ref.add_param_group(dict(params=[qs[3]]))
+        for i in range(4):
+            g = torch.randn(300, generator=gen)
+            ps[i].grad = g.to(gpu) if i in which else None
+            qs[i].grad = g.double() if i in which else None
+        torch.nn.utils.clip_grad_norm_([q for q in qs if q.grad is not None], 3.0)
+        ours.step()
+        ref.step()
+        for i in range(4):
+            tol = (k + 1) * U * (3 * qs[i].detach().abs() + 24 * 12 * lr * (k + 1))
+            assert ((ps[i].detach().cpu().double() - qs[i].detach()).abs() <= tol).all(), (k, i)
+
+
+def test_counts_replayed_from_a_graph(gpu):
+    """A captured step of an optimizer with two counts, replayed between eager work, as the eager one."""
+    gen = torch.Generator().manual_seed(44)
+    start, grads = ([torch.randn(500, generator=gen) for _ in range(3)] for _ in range(2))
+
+    def make():
+        ps = [torch.nn.Parameter(t.to(gpu)) for t in start]
+        opt = AdamW(ps, max_norm=1.0)
+        for which in ((0, 2), (0, 1, 2)):
+            for i, p in enumerate(ps):
+                p.grad = grads[i].to(gpu) if i in which else None
+            opt.step()
+        return ps, opt
+
+    (a, oa), (b, ob) = make(), make()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        oa.step()
+    for k in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        ob.step()
+        torch.cuda.synchronize()
+        assert [int(oa.state[p]["step"]) for p in a] == [int(ob.state[p]["step"]) for p in b] == [3 + k, 2 + k, 3 + k]
+        assert all(torch.equal(x, y) for x, y in zip(a, b)) and float(oa.grad_norm) == float(ob.grad_norm)
