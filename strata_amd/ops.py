@@ -17,9 +17,10 @@ from __future__ import annotations
 import ctypes
 import math
 import operator
+import struct
+from itertools import repeat
 from typing import Optional, Sequence
 
-import numpy as np
 import torch
 from torch import Tensor
 from torch.utils._device import DeviceContext
@@ -1941,7 +1942,7 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
     # kind a tensor and column; a loop over tensors that checked each took 3.5 us a tensor).
     dev, sizes = step.get_device(), list(map(Tensor.numel, params))
     blocks = [-(-k // STATE_BLOCK) for k in sizes]
-    table = np.zeros(max(n, 1), dtype=_ADAMW_TABLE)
+    table = dict.fromkeys(_ADAMW_FIELDS, repeat(0))
     dtypes, written = {}, each
     for what, ts in cols.items():
         if ts is None:
@@ -1963,7 +1964,7 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
                              f"their parameter's size and of {sorted(map(str, _ADAMW_DTYPES[what]))}")
         dtypes[what] = kinds
         ptrs = map(Tensor.data_ptr, ts) if some is ts else (t.data_ptr() if t is not None else 0 for t in ts)
-        table[_ADAMW_FIELD[what]][:n] = np.fromiter(ptrs, np.int64, n)
+        table[_ADAMW_FIELD[what]] = ptrs
         if what in ("params", "masters"):  # the moments are no one's graph's leaves
             written += some
     m_kinds, v_kinds = dtypes["exp_avgs"], dtypes["exp_avg_sqs"]
@@ -1976,15 +1977,14 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
         if (not plain) if ts is None else ([t is not None for t in ts] != (codes or [False] * n)):
             raise ValueError(f"{name}: 8-bit moments come with their scales, fp32 ones without")
     if n:
-        table["n"][:n], table["lr"][:n], table["weight_decay"][:n] = sizes, rates[0], rates[1]
+        table["n"] = sizes
+        table["lr"], table["weight_decay"] = (r if isinstance(r, list) else repeat(r) for r in rates)
         for field, what in (("param_dtype", "params"), ("grad_dtype", "grads")):
-            kinds = dtypes[what]
-            same = kinds.count(kinds[0]) == n  # most often one type for all
-            table[field][:n] = _ADAMW_CODE[kinds[0]] if same else [_ADAMW_CODE[d] for d in kinds]
-        table["state_bits"][:n] = 32 if plain else [8 if c else 32 for c in codes]
+            table[field] = map(_ADAMW_CODE.__getitem__, dtypes[what])
+        table["state_bits"] = repeat(32) if plain else [8 if c else 32 for c in codes]
         if masters is not None and any(w is not None and d != torch.bfloat16 for w, d in zip(masters, dtypes["params"])):
             raise ValueError(f"{name}: masters belong to bfloat16 parameters")
-    tp = ctypes.cast(table.ctypes.data, ctypes.POINTER(_lib.AdamwTensor))
+    tp = (_lib.AdamwTensor * n).from_buffer_copy(b"".join(map(_ADAMW_ROW, *table.values())) if n else b"")
     doubles = int(_lib.function("strata_hip_adamw_workspace")(tp, n)) + (4 * n if steps else 0)
     ws = torch.empty(doubles, dtype=torch.float64, device=step.device)
     norm = torch.empty(1, dtype=torch.float64, device=step.device) if max_norm is not None else None
@@ -2009,8 +2009,8 @@ _ADAMW_FIELD = {"params": "param", "grads": "grad", "exp_avgs": "exp_avg", "exp_
 _ADAMW_DTYPES = {"params": {torch.bfloat16, torch.float32}, "grads": {torch.bfloat16, torch.float32},
                  "exp_avgs": {torch.float32, torch.int8}, "exp_avg_sqs": {torch.float32, torch.uint8},
                  "masters": {torch.float32}, "exp_avg_scales": {torch.float32}, "exp_avg_sq_scales": {torch.float32}}
-_ADAMW_TABLE = np.dtype([(f, np.float64 if c is ctypes.c_double else np.int32 if c is ctypes.c_int32 else np.int64)
-                         for f, c in _lib.AdamwTensor._fields_])
+_ADAMW_FIELDS = [f for f, _ in _lib.AdamwTensor._fields_]
+_ADAMW_ROW = struct.Struct("".join({ctypes.c_double: "d", ctypes.c_int32: "i"}.get(c, "q") for _, c in _lib.AdamwTensor._fields_)).pack
 
 
 def adamw_state_values(codes: Tensor, scales: Tensor) -> Tensor:

@@ -202,3 +202,35 @@ def test_a_capture_makes_no_states(counted, monkeypatch):
     with pytest.raises(RuntimeError, match="eager"):
         step((0,))
     assert counts() == [2, 2, 0, 0]
+
+
+def test_the_package_needs_no_numpy():
+    """Imported, and the rows of a step's tensors laid out, where numpy is not installed."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = """
+import sys
+sys.modules["numpy"] = None
+import ctypes, torch
+from strata_amd import _lib, ops, optim, modules
+rows = []
+ops._require_gpu = lambda *a: None
+ops._launch = lambda name, a, *r: rows.extend([getattr(a.tensors[i], f) for f, _ in _lib.AdamwTensor._fields_] for i in range(a.count))
+p, q = torch.zeros(300, dtype=torch.bfloat16), torch.zeros(5)
+g = [torch.zeros(300), torch.zeros(5)]
+m, v = [torch.zeros(300, dtype=torch.int8), torch.zeros(5)], [torch.zeros(300, dtype=torch.uint8), torch.zeros(5)]
+s, w = [torch.zeros(2), None], [torch.zeros(300), None]
+ops.adamw_step([p, q], g, m, v, torch.zeros(1, dtype=torch.int64), lr=[0.1, 0.2], weight_decay=0.3, masters=w, exp_avg_scales=s, exp_avg_sq_scales=s)
+a = lambda t: None if t is None else t.data_ptr()
+for i, row in enumerate(rows):
+    assert row == [a((p, q)[i]), a(g[i]), a(m[i]), a(v[i]), a(s[i]), a(s[i]), a(w[i]), (300, 5)[i], (0.1, 0.2)[i], 0.3,
+                   (_lib.BF16, _lib.F32)[i], _lib.F32, (8, 32)[i], 0], row
+rows.clear()
+ops.adamw_step([], [], [], [], torch.zeros(1, dtype=torch.int64))
+assert not rows
+"""
+    r = subprocess.run([sys.executable, "-W", "ignore", "-c", code], capture_output=True, text=True,
+                       cwd=Path(_lib.__file__).resolve().parents[1])
+    assert r.returncode == 0, r.stderr[-2000:]
