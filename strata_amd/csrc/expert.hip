@@ -30,12 +30,14 @@ namespace strata {
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 __device__ __forceinline__ void gelu_both(float x, float& y, float& d) {
-  // x s and its derivative s + x s (1 - s) 2u' with s = sigmoid(2u), u = sqrt(2/pi) (x + 0.044715 x^3)
+  // x s and its derivative s + x s (1 - s) 2u' with s = sigmoid(2u), u = sqrt(2/pi) (x + 0.044715 x^3).
+  // Beyond 1e15 s is 0 or 1, and x^2, held there, stays finite: 0 times it is 0.
   constexpr float c = 0.7978845608028654f, k1 = 2.f * 1.4426950408889634f * c;
-  const float t = x * fmaf(k1 * 0.044715f, x * x, k1);
+  const float xx = fminf(x * x, 1e30f);
+  const float t = x * fmaf(k1 * 0.044715f, xx, k1);
   const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-t));
   y = x * s;
-  d = fmaf(y * (1.f - s), 2.f * c * fmaf(3.f * 0.044715f, x * x, 1.f), s);
+  d = fmaf(y * (1.f - s), 2.f * c * fmaf(3.f * 0.044715f, xx, 1.f), s);
 }
 
 // Whether a pair's weight counts as nothing, and what its row is scaled by (a weight that

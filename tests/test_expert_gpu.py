@@ -439,3 +439,20 @@ def test_compiled_for_any_number_of_tokens(gpu):
         for a, b in zip(torch.autograd.grad(got, [x, *shared], d["dout"]), torch.autograd.grad(want, [x, *shared], d["dout"])):
             assert torch.equal(a, b), T
     assert counter.frame_count == 1
+
+
+def test_gelu_of_far_values(gpu):
+    """Hidden pre-activations whose squares leave fp32: GELU's derivative is 1 or 0 there, not 0 times infinity."""
+    far = torch.tensor([2.0**70, -(2.0**70), 2.0**64, -(2.0**64), 2.0**40, -(2.0**40), 2.0**120, -(2.0**120)])
+    T, n = 200, 8
+    ones = lambda *s: torch.ones(*s, device=gpu).bfloat16()  # noqa: E731
+    b1 = far.to(gpu).bfloat16()[None].requires_grad_()
+    w1 = torch.zeros(1, n, n, device=gpu).bfloat16().requires_grad_()
+    w2 = (ones(1, n, n) * 2.0**-60).requires_grad_()
+    x, w, i = ones(T, n).requires_grad_(), ones(T, 1), torch.zeros(T, 1, dtype=torch.int32, device=gpu)
+    out = ops.expert_mlp(x, w, i, w1, b1, w2, None)
+    assert torch.equal(out, (ones(T, n).float() * far.clamp_min(0).sum().item() * 2.0**-60).bfloat16())
+    dx, db1, dw1, dw2 = torch.autograd.grad(out, [x, b1, w1, w2], ones(T, n))
+    d = (far > 0).float().to(gpu)
+    assert torch.equal(db1.float(), (d * T * n * 2.0**-60)[None]) and torch.equal(dw1.float(), (d * T * n * 2.0**-60)[None, :, None].expand(1, n, n))
+    assert not dx.any() and torch.equal(dw2.float(), (far.clamp_min(0).to(gpu) * T)[None, None].expand(1, n, n))
