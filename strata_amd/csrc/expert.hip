@@ -553,7 +553,8 @@ constexpr int EX_FUSED = 4, EX_FUSED_K = 8192, EX_FUSED_N = 8;
 __global__ __launch_bounds__(1024) void expert_few_out_kernel(ExpertGemm p, const bf16* residual, int64_t ldr, bf16* out) {
 #if defined(__HIP_DEVICE_COMPILE__)
   __shared__ float red[16][EX_FUSED][20];
-  __shared__ int expert_at[EX_FUSED], rank_at[EX_FUSED];  // a pair's place among the named experts (-1), and among its expert's pairs
+  // a pair's expert (the index is read once), its place among the named ones (-1), the pair's among its expert's
+  __shared__ int expert_of[EX_FUSED], expert_at[EX_FUSED], rank_at[EX_FUSED];
   const int tid = (int)__builtin_amdgcn_workitem_id_x(), lane = tid & 63, n16 = lane & 15, g4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), n0 = (int)__builtin_amdgcn_workgroup_id_x() * EX_FUSED_N;
   int el = lane < p.pairs ? p.index[lane] : -1;
@@ -567,6 +568,7 @@ __global__ __launch_bounds__(1024) void expert_few_out_kernel(ExpertGemm p, cons
   const uint32_t named = (uint32_t)__ballot(el >= 0 && lead == lane);
   const int count = __popc(named), per = count ? 16 / count : 16;
   if (wave == 0 && lane < p.pairs) {
+    expert_of[lane] = el;
     expert_at[lane] = el >= 0 ? __popc(named & ((1u << lead) - 1)) : -1;
     rank_at[lane] = rank;
   }
@@ -610,7 +612,7 @@ __global__ __launch_bounds__(1024) void expert_few_out_kernel(ExpertGemm p, cons
     if (at < 0 || no_weight(w)) continue;
     float z = 0.f;
     for (int i = 0; i < per; ++i) z += red[at * per + i][rank_at[pair]][c];
-    a += p.bias ? fmaf(w, (float)p.bias[(int64_t)p.index[pair] * p.N + n], z) : z;
+    a += p.bias ? fmaf(w, (float)p.bias[(int64_t)expert_of[pair] * p.N + n], z) : z;
   }
   out[(int64_t)t * p.N + n] = (bf16)a;
 #endif

@@ -239,3 +239,11 @@ def test_struct_layouts_are_the_header_s(tmp_path):
     subprocess.run(["gcc", "-o", str(tmp_path / "layout"), str(src)], check=True)
     got = subprocess.run([str(tmp_path / "layout")], check=True, capture_output=True, text=True).stdout.split()
     assert [int(x) for x in got] == want
+
+
+def test_kernels_without_a_plan_read_an_index_once():
+    """They check the index that they read and form addresses from it: a second read would not be the checked one."""
+    src = (Path(_lib.__file__).resolve().parent / "csrc" / "expert.hip").read_text()
+    for kernel in ("void expert_few_kernel(", "void expert_few_out_kernel("):
+        body = src[src.index(kernel):]
+        assert body[: body.index("\n}\n")].count("p.index[") == 1, kernel
