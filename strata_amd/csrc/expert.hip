@@ -546,10 +546,12 @@ __global__ __launch_bounds__(64 * W) void expert_few_kernel(ExpertGemm p) {
 
 // Up to EX_FUSED pairs (a token while serving) of at most EX_FUSED_K columns together: the second product and
 // the sum over slots in one launch, 8 columns of every token a workgroup, whose 16 waves share the named
-// experts and their contractions.  Replayed, us, two launches / this one (with 16 columns): 2 pairs,
-// 1024 -> 4096 20.2 / 20.0 (22.8), 512 -> 2048 19.0 / 17.5 (17.3), 4 pairs, 512 -> 1024 18.8 / 17.3, but
-// 1024 -> 4096 24.9 / 31.0; the first called eagerly 21.2 / 18.8.
-constexpr int EX_FUSED = 4, EX_FUSED_K = 8192, EX_FUSED_N = 8;
+// experts and their contractions.  Two launches / this one, of 512 and 1024 columns, replayed, us (the whole call; called
+// from Python the launch saved is 2.5 more): 1 pair, 4096 hidden columns 13.6 / 10.8 and 14.4 / 11.5; 2 pairs, 2048 12.2 / 11.4
+// and 13.1 / 12.1, 4096 14.8 / 15.0 and 17.2 / 16.6, 5632 17.4 / 18.2 and 21.2 / 22.1; 3 pairs, 1024 11.6 / 11.3 and
+// 12.3 / 11.9, 2816 14.9 / 17.0 and 17.7 / 19.5; 4 pairs, 512 11.1 / 10.7 and 12.5 / 11.7, 2048 14.3 / 16.6 and 17.2 / 18.3.
+// Of pairs x columns up to 6144, 8192, 9216 and 12288 the last but one loses the least on average, both ways of calling.
+constexpr int EX_FUSED = 4, EX_FUSED_K = 9216, EX_FUSED_N = 8;
 __global__ __launch_bounds__(1024) void expert_few_out_kernel(ExpertGemm p, const bf16* residual, int64_t ldr, bf16* out) {
 #if defined(__HIP_DEVICE_COMPILE__)
   __shared__ float red[16][EX_FUSED][20];
@@ -942,16 +944,19 @@ __global__ __launch_bounds__(256) void expert_wgrad_sum_kernel(const float* part
 // whole forward replayed, us; E experts, C -> H -> C, a: pairs an expert:
 //   16 (the few-rows kernel) under 4 pairs an expert without a backward (a 1, E 8, 1024 -> 4096: 36 against
 //     42 with 64; a 4: 41 / 45, but E 32, 512 -> 1024 32 / 30; a 12: 50 / 47);
-//   64 where the narrowest product would have fewer than 130 tiles of 128 x 128, half of the CUs (some 100:
-//     E 8, 1024 -> 4096, a 150 77 against 82 with 128, E 4, 768 -> 1536, a 500 51 / 53; 129: E 24, 384 -> 776,
-//     a 169 47 / 51; 133: E 2, 1024 -> 4096, a 1000 95 / 86; 160: E 16, 768 -> 1536, a 150 67 / 62);
+//   64 where the narrowest product would have fewer than 140 tiles of 128 x 128.  Over 12 families of E, k, C and H
+//     (E 2 to 64, C 256 to 1024, H 384 to 4096) at 64 to 225 such tiles, forward and training, the better of the two
+//     changes between 96 (E 40, 256 -> 1024) and 192 (E 64, 384 -> 384), mostly around 130 to 150, and a rule
+//     loses against the better one on average 2.5% with 104, 1.1 with 128, 0.6 with 136 to 144, 0.8 with 160,
+//     1.4 with 164 (E 8, 512 -> 2048: at 104 57.3 with 64 against 56.4 with 128, at 144 72.9 / 66.2; E 16, 768 ->
+//     1536: at 126 50.5 / 61.1, at 162 62.4 / 56.4; E 2, 1024 -> 4096: at 112 78.8 / 80.3, at 136 105.4 / 93.5);
 //   256 where an expert has two such tiles and they fill the chip (a 2048, E 8, 1024 -> 2048: 217 against
 //     240 with 128; a 1024: 141 / 148; a 1024, E 32, 512 -> 1024: 150 / 154);
 //   else 128, also for a few rows of many experts (a 6, E 64, 1024 -> 1024: 60 against 62 with 64).
 static int expert_tile(int64_t pairs, int experts, int64_t width, bool train) {
   if (!train && pairs <= EX_DIRECT) return 1;
   if (!train && pairs < 4 * (int64_t)experts) return 16;
-  if ((pairs / 128 + experts / 2) * ((width + 127) / 128) < 130) return 64;
+  if ((pairs / 128 + experts / 2) * ((width + 127) / 128) < 140) return 64;
   return pairs >= 512 * (int64_t)experts && (pairs / 256) * ((width + 255) / 256) >= 200 ? 256 : 128;
 }
 static int expert_tile(const strata_hip_expert_mlp_args* a) {
@@ -1027,6 +1032,8 @@ static int launch_expert_gemm(ExpertGemm p, int64_t pairs, int experts, int tile
 // more on average.  A whole forward and backward with one share / with these: 32768 tokens, 2 experts,
 // 128 -> 512 887 / 172 us; 8000, 2 of 2, 512 -> 1024 534 / 250; 16000, 2 of 8, 512 -> 512 420 / 306;
 // 1000, 2 of 2, 512 -> 512 110 / 100 (shares of two stages 97, of eight 110).
+// CUS is the whole chip's number, not the current device's: a caller sizes the workspace by this rule, maybe
+// while another device is current than the launch's.
 static int wgrad_split(int64_t pairs, int experts, int N, int K) {
   constexpr int64_t CUS = 256;
   const int64_t tiles = (int64_t)experts * ((N + 255) / 256) * ((K + 255) / 256);
