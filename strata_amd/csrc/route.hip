@@ -15,7 +15,7 @@
 // below a logit of -87 and 0 below -103, and 1 / sum is infinite.  Scores that are 0 in
 // 64 bits too (ROUTE_ZERO_*) give weights of 0.
 //
-// L lanes take a token, EPL consecutive experts each: the best key of a lane is found in
+// L lanes take a token, EPL (up to 8) consecutive experts each: the best key of a lane is found in
 // its registers, the token's by log2(L) exchanges, so a round of the choice costs a wave
 // 3 EPL + 6 log2(L) operations for 64 / L tokens.  Bound by those operations and their latency:
 // [65536, 64] fp32, 8 of 64 in 4 of 8 groups with a bias 30 us (17 MB read in 4), its gradient 12 us
@@ -172,8 +172,9 @@ __device__ __forceinline__ bool route_choose(const RouteParams& p, const float (
   for (int i = 0; i < EPL; ++i) key[i] = l[i] > -__builtin_inff() ? (WIDE ? sc[i] + (KEY)bias[i] : (KEY)l[i]) : NONE;
   bool close = false;
   // What two 32-bit keys have to be apart, in units of 1 + |key|.  With u = 6e-8 an exponential is within 2 u,
-  // a sigmoid within 3.5 u, a softmax score within 16 u (its sum has 14 roundings) and a sum with the
-  // bias u further: 2 x 4.5 u and 2 x 17 u, with a margin of 2.  Groups' sums of two keys: twice that.
+  // a sigmoid within 3.5 u, a softmax score within 16 u (its sum has 13 roundings: 8 scores a lane at most,
+  // exchanged by 64 lanes at most) and a sum with the bias u further: 2 x 4.5 u and 2 x 17 u, with a margin of 2.
+  // Groups' sums of two keys: twice that.
   const float apart = p.score == STRATA_HIP_SCORE_SOFTMAX ? 4e-6f : 1e-6f;
   auto near = [&](KEY a, KEY b) { return CHECK && fabsf((float)(a - b)) <= apart * (1.f + fabsf((float)a)); };
   if (WIDE && p.groups > 1) {
@@ -259,7 +260,7 @@ __device__ __forceinline__ bool route_choose(const RouteParams& p, const float (
 
 template <typename T, bool WIDE, bool VEC, int EPL, int L>
 __global__ __launch_bounds__(256) void route_kernel(RouteParams p) {
-  const int TOK = (int)blockDim.x / L;
+  constexpr int TOK = 256 / L;
   extern __shared__ char smem[];  // a token: [top_k] scores, [top_k] experts; with groups the choice's scratch
   const int tid = threadIdx.x, lane = tid % L, tok = tid / L;
   const int64_t t = (int64_t)blockIdx.x * TOK + tok;
@@ -647,7 +648,7 @@ __global__ __launch_bounds__(PLAN_N) void plan_place_kernel(PlanParams p) {
   }
 }
 
-// Lanes a token and experts a lane.
+// f(experts a lane, lanes a token).
 template <typename F>
 static int route_width(int experts, F f) {
   using std::integral_constant;
@@ -711,21 +712,15 @@ extern "C" int strata_hip_expert_route(const strata_hip_expert_route_args* a, vo
   const bool wide = p.bias || p.groups > 1, vec = route_aligned(a, p.bias) && (p.ld % 4) == 0;
   return route_width(p.experts, [&](auto epl, auto l) {
     constexpr int EPL = decltype(epl)::value, L = decltype(l)::value;
-    auto lds = [&](int threads) {
-      const size_t tok = threads / L;
-      return ((tok * p.top_k * 8 + 15) & ~(size_t)15) + (p.groups > 1 ? tok * (EPL * L + 2 * p.groups) * 8 : 0);
-    };
-    // The scratch of a choice in groups is up to 12 KiB a token: fewer tokens a workgroup where it passes
-    // 64 KiB (waves do not work together).  At 32 threads, four tokens of 512 experts, it is at most 50 KiB.
-    int threads = 256;
-    while (threads > 32 && lds(threads) > 65536) threads /= 2;
-    const size_t smem = lds(threads);
-    const int64_t tok = threads / L, wgs = (p.tokens + tok - 1) / tok;
-    if (smem > 65536 || wgs * threads >= 0x100000000ll)
+    constexpr int TOK = 256 / L;
+    // At most 64 KiB: with E experts rounded up to EPL * L and no more groups or slots than experts, 2048 EPL (3 E + min(E, 64)) / E.
+    const size_t smem = (((size_t)TOK * p.top_k * 8 + 15) & ~(size_t)15) + (p.groups > 1 ? (size_t)TOK * (EPL * L + 2 * p.groups) * 8 : 0);
+    const int64_t wgs = (p.tokens + TOK - 1) / TOK;
+    if (smem > 65536 || wgs * 256 >= 0x100000000ll)
       return fail(STRATA_HIP_EUNSUPPORTED, "expert_route: problem too large for one launch");
     const dim3 grid((unsigned)wgs);
     auto go = [&](auto t, auto w, auto v) {
-      hipLaunchKernelGGL((route_kernel<decltype(t), decltype(w)::value, decltype(v)::value, EPL, L>), grid, dim3(threads), smem,
+      hipLaunchKernelGGL((route_kernel<decltype(t), decltype(w)::value, decltype(v)::value, EPL, L>), grid, dim3(256), smem,
                          (hipStream_t)stream, p);
     };
     auto with = [&](auto t, auto w) {

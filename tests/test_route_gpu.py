@@ -283,3 +283,18 @@ def test_route_of_scores_that_are_zero_in_64_bits(gpu, score):
         assert i.tolist() == [[0, 1]] * 5 and not w.any(), low
         (dl,) = torch.autograd.grad(w, x, torch.ones_like(w) + torch.arange(2, device=gpu))
         assert not dl.any(), low
+
+
+@pytest.mark.parametrize("E", [64, 132, 300, 512])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_route_near_ties_of_many_experts(gpu, score, E):
+    """A bias that lifts every score to within a rounding of 1: all keys s + bias lie within 1.2e-7 of each
+    other, and 64 bits choose."""
+    for seed in range(12):
+        l = _logits(1, E, torch.float32, seed)
+        s, _ = O.scores(l, score)
+        bias = (1.0 - s[0]).float()
+        for groups, top in ((1, 1), (E // 4, 5)):
+            _, want = O.route(l, 9, score, bias, groups, top)
+            _, got = ops.expert_route(l.to(gpu), 9, score, bias.to(gpu), groups, top)
+            assert torch.equal(got.cpu(), want), (seed, groups)
