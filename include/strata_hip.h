@@ -591,7 +591,7 @@ int strata_hip_gated_add(const strata_hip_gated_add_args* args, void* stream);
  *   keys), -1 where none is left;  weights[t, i] = scale * s (/ sum of the chosen s), 0 with -1
  * A sum of chosen s too small for 32 bits is formed from the logits; s that are all 0 in 64 bits
  * (softmax: 745 below the largest logit, sigmoid: below -709) give weights and a gradient of 0.
- * A logit or bias that is not finite masks its expert (s = 0, never chosen).  Keys (a bias or
+ * A logit or bias that is not finite masks its expert (s = 0, never chosen, not in the softmax's sum).  Keys (a bias or
  * groups given) that 32 bits cannot tell apart are told apart in 64.  At most 512 experts, top_k 64.
  * logits: [tokens, experts], row stride ld; weights, dweights: [tokens, top_k] of the
  * logits' type; index: int32 [tokens, top_k]; dlogits: [tokens, experts] contiguous.
@@ -601,7 +601,7 @@ enum strata_hip_score { STRATA_HIP_SCORE_SOFTMAX = 0, STRATA_HIP_SCORE_SIGMOID =
 
 typedef struct strata_hip_expert_route_args {
   const void* logits;
-  const float* bias;     /* [experts] or NULL; takes part in the choice, not in the weights */
+  const float* bias;     /* [experts] or NULL; a finite one takes part in the choice alone */
   void* weights;
   int32_t* index;        /* out; in for _bwd */
   const void* dweights;  /* _bwd only */

@@ -1525,13 +1525,13 @@ def expert_route(logits: Tensor, top_k: int, score: str = "softmax", bias: Optio
     router logits ``[..., experts]`` (bf16 or fp32; the weights have their type, the index is int32).
 
     Scores are the ``"softmax"`` of a token's logits or their ``"sigmoid"``.  The experts with the
-    largest score + ``bias`` (fp32 ``[experts]``, for the balance of their load; it takes no part in
-    the weights) are chosen in falling order, the lower one of two that are equal; of ``groups``
+    largest score + ``bias`` (fp32 ``[experts]``, for the balance of their load; a finite one takes no part
+    in the weights) are chosen in falling order, the lower one of two that are equal; of ``groups``
     equal groups only the ``top_groups`` with the largest sums of their two best count.  The weights
     are ``scale`` times the chosen scores, divided by their sum with ``renormalize`` (however small they are
     in 32 bits; chosen scores that are all 0 in 64 bits, as a sigmoid's below -709, give weights of 0).
 
-    A logit (or bias) that is not finite masks its expert; a token with too few experts left has
+    A logit or bias that is not finite masks its expert, for the softmax's sum too; a token with too few experts left has
     index -1 and weight 0 in the slots that stay empty.  At most 512 experts and top_k 64.  The
     backward gives the logits' gradient (none flows to the bias)."""
     if not _eager(logits, bias):

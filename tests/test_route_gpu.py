@@ -298,3 +298,20 @@ def test_route_near_ties_of_many_experts(gpu, score, E):
             _, want = O.route(l, 9, score, bias, groups, top)
             _, got = ops.expert_route(l.to(gpu), 9, score, bias.to(gpu), groups, top)
             assert torch.equal(got.cpu(), want), (seed, groups)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_route_bias_that_is_not_finite(gpu, bad):
+    """It masks its expert as a logit would: never chosen, not in the softmax's sum, a gradient of 0."""
+    l = _logits(40, 24, torch.float32, 10)
+    bias = torch.zeros(24)
+    bias[[5, 17]] = bad
+    gone = l.clone()
+    gone[:, [5, 17]] = -math.inf
+    x, y = l.to(gpu).requires_grad_(), gone.to(gpu).requires_grad_()
+    got = ops.expert_route(x, 4, "softmax", bias.to(gpu), renormalize=False)
+    want = ops.expert_route(y, 4, "softmax", torch.zeros(24, device=gpu), renormalize=False)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and not ((got[1] == 5) | (got[1] == 17)).any()
+    d = torch.randn(40, 4, generator=torch.Generator().manual_seed(2)).to(gpu)
+    gx, gy = torch.autograd.grad(got[0], x, d)[0], torch.autograd.grad(want[0], y, d)[0]
+    assert torch.equal(gx, gy) and not gx[:, [5, 17]].any()
