@@ -24,7 +24,7 @@
 // is kept between calls; the step count lives on the device, so a captured step counts on.
 #include <algorithm>
 #include <cmath>
-#include <new>
+#include <exception>
 #include <unordered_map>
 #include <vector>
 
@@ -726,7 +726,7 @@ extern "C" int64_t strata_hip_adamw_workspace(const strata_hip_adamw_tensor* ten
 extern "C" int strata_hip_adamw_step(const strata_hip_adamw_args* a, void* stream) {
   try {
     return strata::aw_launch(a, nullptr, (hipStream_t)stream);
-  } catch (const std::bad_alloc&) {
+  } catch (const std::exception&) {  // no memory for the lists, or more than a list can hold
     return strata::fail(STRATA_HIP_EUNSUPPORTED, "adamw_step: out of host memory");
   }
 }
@@ -735,7 +735,7 @@ extern "C" int strata_hip_adamw_step_counts(const strata_hip_adamw_args* a, int6
   if (!steps) return strata::fail(STRATA_HIP_EINVAL, "adamw_step: null steps");
   try {
     return strata::aw_launch(a, steps, (hipStream_t)stream);
-  } catch (const std::bad_alloc&) {
+  } catch (const std::exception&) {  // no memory for the lists, or more than a list can hold
     return strata::fail(STRATA_HIP_EUNSUPPORTED, "adamw_step: out of host memory");
   }
 }

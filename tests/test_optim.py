@@ -234,3 +234,22 @@ assert not rows
     r = subprocess.run([sys.executable, "-W", "ignore", "-c", code], capture_output=True, text=True,
                        cwd=Path(_lib.__file__).resolve().parents[1])
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("count", [1 << 44, 1 << 60])
+def test_c_entry_returns_where_a_list_cannot_be_held(count):
+    """More tensors than host memory, or than a vector, holds: an error, no exception across the C boundary."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = f"""
+import ctypes
+from strata_amd import _lib
+lib = _lib.load()
+t = (_lib.AdamwTensor * 1)()
+a = _lib.AdamwArgs(t, {count}, 0x1000, 0x2000, 0x3000, 0.9, 0.95, 1e-8, 0.0)
+assert lib.strata_hip_adamw_step(ctypes.byref(a), None) == _lib.EUNSUPPORTED
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=Path(_lib.__file__).resolve().parents[1])
+    assert r.returncode == 0, (r.returncode, r.stderr[-500:])
