@@ -544,13 +544,14 @@ __global__ __launch_bounds__(64 * W) void expert_few_kernel(ExpertGemm p) {
 #endif
 }
 
-// Up to EX_FUSED pairs (a token while serving) of at most EX_FUSED_K columns together: the second product and
+// One pair, or up to EX_FUSED (a token while serving) of at most EX_FUSED_K columns together: the second product and
 // the sum over slots in one launch, 8 columns of every token a workgroup, whose 16 waves share the named
 // experts and their contractions.  Two launches / this one, of 512 and 1024 columns, replayed, us (the whole call; called
 // from Python the launch saved is 2.5 more): 1 pair, 4096 hidden columns 13.6 / 10.8 and 14.4 / 11.5; 2 pairs, 2048 12.2 / 11.4
 // and 13.1 / 12.1, 4096 14.8 / 15.0 and 17.2 / 16.6, 5632 17.4 / 18.2 and 21.2 / 22.1; 3 pairs, 1024 11.6 / 11.3 and
 // 12.3 / 11.9, 2816 14.9 / 17.0 and 17.7 / 19.5; 4 pairs, 512 11.1 / 10.7 and 12.5 / 11.7, 2048 14.3 / 16.6 and 17.2 / 18.3.
-// Of pairs x columns up to 6144, 8192, 9216 and 12288 the last but one loses the least on average, both ways of calling.
+// One pair gains at every width (16384: 29.3 / 22.7 and 35.1 / 28.1); for 2 to 4 pairs limits of 6144, 8192, 9216 and 12288
+// pairs x columns lose 1.4, 1.1, 1.0 and 1.4% on average over both ways of calling.
 constexpr int EX_FUSED = 4, EX_FUSED_K = 9216, EX_FUSED_N = 8;
 __global__ __launch_bounds__(1024) void expert_few_out_kernel(ExpertGemm p, const bf16* residual, int64_t ldr, bf16* out) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -946,7 +947,7 @@ __global__ __launch_bounds__(256) void expert_wgrad_sum_kernel(const float* part
 //     42 with 64; a 4: 41 / 45, but E 32, 512 -> 1024 32 / 30; a 12: 50 / 47);
 //   64 where the narrowest product would have fewer than 140 tiles of 128 x 128.  Over 12 families of E, k, C and H
 //     (E 2 to 64, C 256 to 1024, H 384 to 4096) at 64 to 225 such tiles, forward and training, the better of the two
-//     changes between 96 (E 40, 256 -> 1024) and 192 (E 64, 384 -> 384), mostly around 130 to 150, and a rule
+//     changes between 104 (E 8, 512 -> 2048) and 192 (E 64, 384 -> 384), mostly around 130 to 150, and a rule
 //     loses against the better one on average 2.5% with 104, 1.1 with 128, 0.6 with 136 to 144, 0.8 with 160,
 //     1.4 with 164 (E 8, 512 -> 2048: at 104 57.3 with 64 against 56.4 with 128, at 144 72.9 / 66.2; E 16, 768 ->
 //     1536: at 126 50.5 / 61.1, at 162 62.4 / 56.4; E 2, 1024 -> 4096: at 112 78.8 / 80.3, at 136 105.4 / 93.5);
@@ -1148,7 +1149,7 @@ extern "C" int strata_hip_expert_mlp(const strata_hip_expert_mlp_args* a, void* 
   g.out = a->y;
   g.N = a->out_dim;
   g.K = a->hidden;
-  if (a->tile == 1 && pairs <= EX_FUSED && pairs * a->hidden <= EX_FUSED_K) {
+  if (a->tile == 1 && (pairs == 1 || (pairs <= EX_FUSED && pairs * a->hidden <= EX_FUSED_K))) {
     hipLaunchKernelGGL(expert_few_out_kernel, dim3((unsigned)(a->out_dim / EX_FUSED_N)), dim3(1024), 0, st, g, (const bf16*)a->residual,
                        a->ldr, (bf16*)a->out);
     return check_launch("expert_few_out_kernel");

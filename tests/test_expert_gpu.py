@@ -456,3 +456,15 @@ def test_gelu_of_far_values(gpu):
     d = (far > 0).float().to(gpu)
     assert torch.equal(db1.float(), (d * T * n * 2.0**-60)[None]) and torch.equal(dw1.float(), (d * T * n * 2.0**-60)[None, :, None].expand(1, n, n))
     assert not dx.any() and torch.equal(dw2.float(), (far.clamp_min(0).to(gpu) * T)[None, None].expand(1, n, n))
+
+
+@pytest.mark.parametrize("k,H", [(1, 9224), (1, 16392), (1, 32768), (2, 4608), (2, 4616), (3, 3064), (3, 3088), (4, 2304), (4, 2312)])
+def test_fused_second_product_at_its_limits(gpu, k, H):
+    """A token's pairs just under and over the width that one launch takes, and one pair of any width."""
+    print(f"experts, one token {k} {H}", flush=True)
+    c = _case(1, 5, k, 64, H, 72, 24, dropped=0.0)
+    want = O.mlp_bounds(*(c[n] for n in ("x", "weights", "index", "w1", "b1", "w2", "b2", "residual")))
+    d = _to(c, gpu, False)
+    out = _call(d)
+    _inside(out, want["out"], "out")
+    assert torch.equal(out, _call(d))
