@@ -1426,27 +1426,25 @@ def _route_args(name, logits, bias, top_k, score, groups, top_groups, renormaliz
 
 
 _PLAIN = (Tensor, torch.nn.Parameter)
+_is_compiling = torch.compiler.is_compiling
 _dispatch_modes, _function_modes = torch._C._len_torch_dispatch_stack, torch._C._len_torch_function_stack
 _functorch_level, _jit_trace = torch._C._functorch.peek_interpreter_stack, torch._C._get_tracing_state
 _batched = torch._C._functorch.is_legacy_batchedtensor  # gradients of autograd.grad(is_grads_batched=True)
 
 
-def _watched() -> bool:
-    """Whether someone is to see the operators that are called on plain tensors: a dispatch mode (make_fx,
-    fake tensors, selective checkpointing, counters), a functorch transform, a jit trace or a function mode
-    other than the one that sets the default device."""
-    if _dispatch_modes() or _functorch_level() is not None or _jit_trace() is not None:
-        return True
-    n = _function_modes()
-    return n > 0 and any(type(torch._C._get_function_stack_at(i)) is not DeviceContext for i in range(n))
+def _foreign_function_mode() -> bool:
+    """Whether a function mode is active other than the one that sets the default device."""
+    return any(type(torch._C._get_function_stack_at(i)) is not DeviceContext for i in range(_function_modes()))
 
 
 def _eager(*ts: Optional[Tensor]) -> bool:
-    """Whether these are plain tensors that nothing traces or watches: the operators of this section then
-    launch through a ``torch.autograd.Function`` of their own.  The custom op's dispatch and its
-    registered autograd cost 25 us a forward and 55 us a backward of host time beside it, more
-    than the kernels of a small call; all other calls, and tensor subclasses, go through the custom op."""
-    if torch.compiler.is_compiling() or _watched():
+    """Whether these are plain tensors that nothing traces or watches: no compiler, dispatch mode (make_fx,
+    fake tensors, selective checkpointing, counters), functorch transform, jit trace or function mode.  The
+    operators of this section then launch through a ``torch.autograd.Function`` of their own.  The
+    custom op's dispatch and its registered autograd cost 25 us a forward and 55 us a backward of host
+    time beside it, more than the kernels of a small call; all other calls go through the custom op."""
+    if _is_compiling() or _dispatch_modes() or _functorch_level() is not None or _jit_trace() is not None \
+            or (_function_modes() and _foreign_function_mode()):
         return False
     for t in ts:
         if t is not None and type(t) not in _PLAIN:
@@ -1459,8 +1457,6 @@ def _wants_grad(*ts: Optional[Tensor]) -> bool:
         for t in ts:
             if t is not None and t.requires_grad:
                 return True
-        # what a transform wraps may want one that the wrapper does not show
-        return not torch.compiler.is_compiling() and _functorch_level() is not None
     return False
 
 
@@ -1876,7 +1872,8 @@ def expert_mlp(x: Tensor, weights: Tensor, index: Tensor, w1: Tensor, b1: Option
     once, in every argument but the index."""
     grad = _wants_grad(x, weights, w1, b1, w2, b2, residual)
     if not _eager(x, weights, index, w1, b1, w2, b2, residual):
-        if grad:
+        # what a transform wraps may want a gradient that the wrapper does not show
+        if grad or (torch.is_grad_enabled() and not _is_compiling() and _functorch_level() is not None):
             return expert_mlp_train(x, weights, index, w1, b1, w2, b2, residual)[0]
         return expert_mlp_fwd(x, weights, index, w1, b1, w2, b2, residual)
     if grad:

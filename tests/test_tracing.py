@@ -189,3 +189,13 @@ def test_training_workspace_holds_every_plan():
             for width in (8, 768, 4096):
                 tile = lib.strata_hip_expert_tile(n, E, width, width, width, 1)
                 assert tile >= ops._TRAIN_TILE and ws - plan >= 4 * ops._plan_size(n, E, tile)
+
+
+def test_vmap_over_a_leaf_keeps_its_gradient(launches):
+    """Under vmap the tensors' wrappers show no wish for gradients; the leaves behind them have one."""
+    x, w, i, w1, _, w2, b2 = _mlp_args()
+    w1.requires_grad_()
+    xs = torch.stack([x, x, x]).requires_grad_()
+    out = torch.vmap(lambda x: ops.expert_mlp(x, w, i, w1, None, w2, b2))(xs)
+    gx, g1 = torch.autograd.grad(out.sum(), [xs, w1])
+    assert gx.shape == xs.shape and g1.shape == w1.shape and launches.count("strata_hip_expert_mlp_bwd") == 3
