@@ -621,6 +621,40 @@ typedef struct strata_hip_expert_route_args {
 int strata_hip_expert_route(const strata_hip_expert_route_args* args, void* stream);
 int strata_hip_expert_route_bwd(const strata_hip_expert_route_args* args, void* stream);
 
+/* What keeps the routing balanced: the balance loss, the z-loss and the experts' load.
+ *   s = softmax of a token's logits over its experts that are not masked (finite logits), or sigmoid(l) divided by their sum
+ *   `sequences` runs of equally many tokens, n of them with an expert left: f = experts * load / (top_k n), P = sum of s / n
+ *   *balance = mean over sequences with n > 0 of sum over experts of f P;  *z = mean over tokens of (log-sum-exp of the logits)^2
+ *   load[e] = entries of index that name e (others outside [0, experts) count nowhere), in all sequences
+ * logits: [tokens, experts], row stride ld; index: [tokens, top_k] int32; state: [2 + sequences * experts] f32, kept for
+ * _bwd; workspace: strata_hip_expert_balance_workspace() bytes, 8-byte aligned.  Without tokens the losses are 0.
+ * _bwd: dlogits [tokens, experts] contiguous, of the logits' type, from the losses' gradients dbalance and dz (device
+ * scalars; NULL: 0) and state; index, balance, z, load and workspace are not read.  No gradient flows through load.
+ * At most 512 experts and 65536 sequences.  Results do not depend on timing. */
+typedef struct strata_hip_expert_balance_args {
+  const void* logits;
+  const int32_t* index;
+  float* balance;
+  float* z;
+  int32_t* load;
+  float* state;          /* out; in for _bwd */
+  const float* dbalance; /* _bwd only */
+  const float* dz;       /* _bwd only */
+  void* dlogits;         /* _bwd only */
+  void* workspace;
+  int64_t tokens;
+  int64_t ld;
+  int64_t sequences;
+  int32_t dtype;         /* strata_hip_dtype of logits and dlogits */
+  int32_t experts;
+  int32_t top_k;
+  int32_t score;         /* strata_hip_score */
+} strata_hip_expert_balance_args;
+
+int64_t strata_hip_expert_balance_workspace(int64_t tokens, int64_t sequences, int32_t experts);
+int strata_hip_expert_balance(const strata_hip_expert_balance_args* args, void* stream);
+int strata_hip_expert_balance_bwd(const strata_hip_expert_balance_args* args, void* stream);
+
 /* The order in which the experts' products take the chosen (token, slot) pairs: by expert,
  * pairs of one expert in their own order.  An index outside [0, experts) drops its pair.
  * index: [pairs], pair = token * top_k + slot; weights: bf16 [pairs].  Out: row_token[r] and

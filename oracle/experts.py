@@ -172,3 +172,31 @@ def mlp_bounds(x, weights, index, w1, b1, w2, b2, residual, dout=None) -> dict:
         if residual is not None:
             res["residual"] = (g_all, torch.zeros_like(g_all))
     return res
+
+
+def balance(logits: Tensor, index: Tensor, score: str = "softmax", sequences: int = 1) -> tuple[Tensor, Tensor, Tensor]:
+    """``(balance, z, load)`` in float64 / int32 from logits [T, E] and index [T, k], token by token; differentiable in
+    the logits (float64 ones)."""
+    T, E = logits.shape
+    k, per = index.shape[1], T // sequences
+    ok = torch.isfinite(logits)
+    load, terms, squares = torch.zeros(E, dtype=torch.int32), [], []
+    for g in range(sequences):
+        scores_of, named = [], torch.zeros(E, dtype=torch.float64)
+        for t in range(g * per, (g + 1) * per):
+            for e in index[t].tolist():
+                if 0 <= e < E:
+                    named[e] += 1
+            if not ok[t].any():
+                continue
+            at = ok[t].nonzero()[:, 0]
+            l = logits[t, at].double()
+            squares.append(torch.logsumexp(l, 0) ** 2)
+            key = l if score == "softmax" else torch.nn.functional.logsigmoid(l)
+            scores_of.append(torch.zeros(E, dtype=torch.float64).index_add(0, at, torch.softmax(key, 0)))
+        load += named.int()
+        n = len(scores_of)
+        if n:
+            terms.append((named * E / (k * n) * (sum(scores_of) / n)).sum())
+    zero = torch.zeros((), dtype=torch.float64)
+    return sum(terms, zero) / max(len(terms), 1), sum(squares, zero) / max(len(squares), 1), load

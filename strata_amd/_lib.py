@@ -354,6 +354,13 @@ class ExpertRouteArgs(ctypes.Structure):
     ]
 
 
+class ExpertBalanceArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("logits", "index", "balance", "z", "load", "state", "dbalance", "dz", "dlogits",
+                                               "workspace")] + \
+        [(n, ctypes.c_int64) for n in ("tokens", "ld", "sequences")] + \
+        [(n, ctypes.c_int32) for n in ("dtype", "experts", "top_k", "score")]
+
+
 class ExpertPlanArgs(ctypes.Structure):
     _fields_ = [
         ("index", ctypes.c_void_p),
@@ -459,6 +466,9 @@ EXPORTS = {
     "strata_hip_gated_add": ([ctypes.POINTER(GatedAddArgs), ctypes.c_void_p], ctypes.c_int),
     "strata_hip_expert_route": ([ctypes.POINTER(ExpertRouteArgs), ctypes.c_void_p], ctypes.c_int),
     "strata_hip_expert_route_bwd": ([ctypes.POINTER(ExpertRouteArgs), ctypes.c_void_p], ctypes.c_int),
+    "strata_hip_expert_balance": ([ctypes.POINTER(ExpertBalanceArgs), ctypes.c_void_p], ctypes.c_int),
+    "strata_hip_expert_balance_bwd": ([ctypes.POINTER(ExpertBalanceArgs), ctypes.c_void_p], ctypes.c_int),
+    "strata_hip_expert_balance_workspace": ([ctypes.c_int64, ctypes.c_int64, ctypes.c_int32], ctypes.c_int64),
     "strata_hip_expert_plan": ([ctypes.POINTER(ExpertPlanArgs), ctypes.c_void_p], ctypes.c_int),
     "strata_hip_expert_plan_workspace": ([ctypes.c_int64, ctypes.c_int32], ctypes.c_int64),
     "strata_hip_expert_mlp_bwd_workspace": ([ctypes.c_int64] + [ctypes.c_int32] * 4, ctypes.c_int64),

@@ -14,6 +14,7 @@ or a missing HIP library raise.
 
 from __future__ import annotations
 
+import threading
 from typing import Optional, Sequence
 
 import torch
@@ -83,8 +84,8 @@ class ExpertMlp(nn.Module):
     weights are stacked, ``w1 [E, H, C]``, ``b1 [E, H]``, ``w2 [E, N, H]``, ``b2 [E, N]``.  ``score``,
     ``groups``, ``top_groups``, ``renormalize`` and ``scale`` are ``expert_route``'s.  With ``balance``
     a buffer of that name (fp32 ``[E]``, zeros) is added to the scores for the choice alone; the
-    training loop moves it against the experts' load (``route`` returns the choice, ``bincount`` of
-    its index the load) and it stays fp32 when the module is cast.  bf16 on one GPU, as the MLP it
+    training loop moves it against the experts' load and it stays fp32 when the module is cast.  ``RoutingLosses``
+    collects that load and the losses that keep it even.  bf16 on one GPU, as the MLP it
     stands for; differentiable in x, the residual and every parameter."""
 
     def __init__(self, in_features: int, hidden_features: int, experts: int, top_k: int = 2,
@@ -121,12 +122,58 @@ class ExpertMlp(nn.Module):
     def route(self, x: Tensor) -> tuple[Tensor, Tensor]:
         """``(weights, index)`` ``[..., top_k]`` of tokens ``[..., C]``."""
         logits = ops.gemm_bias_act(x, self.router.weight, None, None, _lib.ACT_NONE)
-        return ops.expert_route(logits, self.top_k, self.score, self.balance, self.groups, self.top_groups,
-                                self.renormalize, self.scale)
+        weights, index = ops.expert_route(logits, self.top_k, self.score, self.balance, self.groups, self.top_groups,
+                                          self.renormalize, self.scale)
+        if RoutingLosses._active():
+            RoutingLosses._active()[-1]._collect(self, logits, index)
+        return weights, index
 
     def forward(self, x: Tensor, residual: Optional[Tensor] = None) -> Tensor:
         weights, index = self.route(x)
         return ops.expert_mlp(x, weights, index, self.w1, self.b1, self.w2, self.b2, residual)
+
+
+class RoutingLosses:
+    """Collects the losses that keep the routing balanced from every ``ExpertMlp`` that runs inside it::
+
+        with RoutingLosses() as routing:
+            out = model(x)
+        loss = task(out) + 1e-2 * routing.balance + 1e-3 * routing.z
+
+    ``balance`` and ``z`` are the sums over the calls collected (fp32 scalars, see ``ops.expert_balance``; None without
+    any), ``load`` a list of ``(mlp, int32 [experts])``, in the order of the calls.  With ``per_sample`` each entry of a
+    call's first axis is balanced by itself.  The losses hold the calls' autograd graph: let go of this object before a
+    backward is captured.  It belongs to the thread that entered it, and a region that ``torch.utils.checkpoint`` runs
+    again in the backward does not run inside it."""
+
+    _local = threading.local()
+
+    def __init__(self, per_sample: bool = False):
+        self.per_sample = per_sample
+        self.balance: Optional[Tensor] = None
+        self.z: Optional[Tensor] = None
+        self.load: list[tuple[ExpertMlp, Tensor]] = []
+
+    @classmethod
+    def _active(cls) -> list["RoutingLosses"]:
+        stack = getattr(cls._local, "stack", None)
+        if stack is None:
+            stack = cls._local.stack = []
+        return stack
+
+    def __enter__(self) -> "RoutingLosses":
+        self._active().append(self)
+        return self
+
+    def __exit__(self, *exc) -> None:
+        self._active().remove(self)
+
+    def _collect(self, mlp: ExpertMlp, logits: Tensor, index: Tensor) -> None:
+        sequences = logits.shape[0] if self.per_sample and logits.dim() > 1 else 1
+        balance, z, load = ops.expert_balance(logits, index, mlp.score, max(sequences, 1))
+        self.balance = balance if self.balance is None else self.balance + balance
+        self.z = z if self.z is None else self.z + z
+        self.load.append((mlp, load))
 
 
 class FusedNA3DAttention(nn.Module):

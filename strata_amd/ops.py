@@ -7,7 +7,7 @@ missing library raises.  Every op has a fake (meta) implementation so that
 ``torch.compile`` traces through it.  ``na3d_fwd`` (full-grid queries),
 ``gemm_bias_act`` (act none / GELU(tanh) with an added residual, and the
 sigmoid gate), ``mlp_gelu_train``, ``layer_norm``, ``rope_qkv_pack`` (with or
-without qk_norm), ``expert_route`` and ``expert_mlp`` have backwards on HIP kernels (a
+without qk_norm), ``expert_route``, ``expert_balance`` and ``expert_mlp`` have backwards on HIP kernels (a
 Linear's plain input gradient is torch's product); the other ops' autograd formulas raise.
 ``adamw_step`` updates its tensors in place and is an ordinary function.
 """
@@ -49,6 +49,7 @@ __all__ = [
     "layer_norm_modulate",
     "gated_add",
     "expert_route",
+    "expert_balance",
     "expert_mlp",
     "adamw_step",
     "adamw_state_values",
@@ -1575,6 +1576,156 @@ def _route_op_backward(ctx, dweights, _dindex):
 
 
 _expert_route_op.register_autograd(_route_op_backward, setup_context=_route_setup_context)
+
+
+# ---------------------------------------------------------------------------
+# The balance of the routing
+# ---------------------------------------------------------------------------
+def _balance_args(name, logits, top_k, score, sequences, state, index=None, balance=None, z=None, load=None, dbalance=None,
+                  dz=None, dlogits=None, workspace=None):
+    """The structure of strata_hip_expert_balance and what it points into; state and what follows are pointers."""
+    if score not in SCORES:
+        raise ValueError(f"{name}: score must be one of {sorted(SCORES)}, got {score!r}")
+    dtype = _dtype_code(name, logits)
+    if logits.dim() < 1 or not logits.shape[-1]:
+        raise ValueError(f"{name}: logits must be [..., experts]")
+    E = logits.shape[-1]
+    rows = logits.numel() // E
+    if sequences < 1 or rows % sequences:
+        raise ValueError(f"{name}: {rows} tokens are no whole number for each of {sequences} sequences")
+    if logits.is_contiguous():
+        l2, ld = logits, E
+    else:
+        l2 = logits.reshape(-1, E)
+        if l2.stride(1) != 1 or (rows > 1 and l2.stride(0) < E):
+            l2 = l2.contiguous()
+        ld = l2.stride(0) if rows > 1 else E
+    return _lib.ExpertBalanceArgs(l2.data_ptr(), index, balance, z, load, state, dbalance, dz, dlogits, workspace, rows, ld, sequences,
+                                  dtype, E, top_k, SCORES[score]), l2
+
+
+def _balance_forward(logits, index, score, sequences):
+    name = "expert_balance"
+    dev = _require_gpu(name, logits, index)
+    if index.dtype != torch.int32 or index.dim() != logits.dim() or index.shape[:-1] != logits.shape[:-1] or not index.shape[-1]:
+        raise ValueError(f"{name}: index must be int32 {[*logits.shape[:-1], 'top_k']}, got {index.dtype} {list(index.shape)}")
+    E, i, n = logits.shape[-1], index.contiguous(), int(sequences)
+    balance, z = torch.empty((), device=dev), torch.empty((), device=dev)
+    load = torch.empty(E, dtype=torch.int32, device=dev)
+    state = torch.empty(2 + max(n, 0) * E, device=dev)
+    rows = logits.numel() // max(E, 1)
+    ws = torch.empty(_lib.function("strata_hip_expert_balance_workspace")(rows, n, E), dtype=torch.uint8, device=dev)
+    a, keep = _balance_args(name, logits, index.shape[-1], score, n, state.data_ptr(), i.data_ptr(), balance.data_ptr(),
+                            z.data_ptr(), load.data_ptr(), workspace=ws.data_ptr())
+    _launch("strata_hip_expert_balance", a, logits)
+    return balance, z, load, state
+
+
+def _balance_backward(dbalance, dz, logits, state, top_k, score, sequences):
+    name = "expert_balance_bwd"
+    _require_gpu(name, logits, state, dbalance, dz)
+    if any(d is not None and (d.dtype != torch.float32 or d.numel() != 1) for d in (dbalance, dz)):
+        raise ValueError(f"{name}: the gradients of the losses must be float32 scalars")
+    if state.dtype != torch.float32 or state.numel() != 2 + sequences * logits.shape[-1] or not state.is_contiguous():
+        raise ValueError(f"{name}: state must be the forward's")
+    out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    a, keep = _balance_args(name, logits, top_k, score, sequences, state.data_ptr(),
+                            dbalance=dbalance.data_ptr() if dbalance is not None else None,
+                            dz=dz.data_ptr() if dz is not None else None, dlogits=out.data_ptr())
+    _launch("strata_hip_expert_balance_bwd", a, logits)
+    return out
+
+
+class _ExpertBalance(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, index, score, sequences):
+        balance, z, load, state = _balance_forward(logits, index, score, sequences)
+        ctx.mark_non_differentiable(load)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(logits, state)
+        ctx.args = index.shape[-1], score, int(sequences)
+        return balance, z, load
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dbalance, dz, _dload):
+        if dbalance is None and dz is None:
+            return (None,) * 4
+        logits, state = ctx.saved_tensors
+        plain = _eager(dbalance, dz, logits) and not any(d is not None and _batched(d) for d in (dbalance, dz))
+        return (_balance_backward if plain else expert_balance_bwd)(dbalance, dz, logits, state, *ctx.args), None, None, None
+
+
+@torch.library.custom_op("strata_hip::expert_balance", mutates_args=())
+def _expert_balance_op(logits: Tensor, index: Tensor, score: str = "softmax",
+                       sequences: int = 1) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    """``expert_balance`` as a custom op, with what its backward needs behind the load."""
+    return _balance_forward(logits, index, score, sequences)
+
+
+def expert_balance(logits: Tensor, index: Tensor, score: str = "softmax", sequences: int = 1) -> tuple[Tensor, Tensor, Tensor]:
+    """``(balance, z, load)`` of a routing: the loss that keeps the experts' load even, the z-loss that
+    keeps the logits small (fp32 scalars) and every expert's number of entries in ``index`` (int32 ``[experts]``).
+
+    logits ``[..., experts]`` (bf16 or fp32) and index (int32 ``[..., top_k]``) are those of ``expert_route``,
+    and so is ``score``.  A token's scores s are the softmax of its logits, or their sigmoids divided by the
+    sum of them::
+
+        f = experts * load / (top_k * n),  P = sum over tokens of s / n      (of a sequence's n tokens)
+        balance = mean over sequences of sum over experts of f * P           (1 where the load is even)
+        z = mean over tokens of logsumexp(logits) ** 2
+
+    ``sequences`` splits the tokens into so many equal runs (a batch's samples, say), each balanced by itself.  A
+    logit that is not finite masks its expert; a token without any (padding) counts in neither loss, and a
+    sequence of such tokens is left out of the mean.  An index outside ``[0, experts)`` counts nowhere.  Differentiable
+    once in the logits; no gradient flows through the load.  At most 512 experts and 65536 sequences."""
+    if not _eager(logits, index):
+        return _expert_balance_op(logits, index, score, sequences)[:3]
+    if _wants_grad(logits):
+        return _ExpertBalance.apply(logits, index, score, sequences)
+    return _balance_forward(logits, index, score, sequences)[:3]
+
+
+@_expert_balance_op.register_fake
+def _(logits, index, score="softmax", sequences=1):
+    E = logits.shape[-1]
+    f32 = dict(dtype=torch.float32)
+    return (logits.new_empty((), **f32), logits.new_empty((), **f32), logits.new_empty(E, dtype=torch.int32),
+            logits.new_empty(2 + sequences * E, **f32))
+
+
+@torch.library.custom_op("strata_hip::expert_balance_bwd", mutates_args=())
+def expert_balance_bwd(dbalance: Optional[Tensor], dz: Optional[Tensor], logits: Tensor, state: Tensor, top_k: int, score: str,
+                       sequences: int) -> Tensor:
+    """The gradient at the logits of ``expert_balance`` from its losses' gradients (None: 0) and its state."""
+    return _balance_backward(dbalance, dz, logits, state, top_k, score, sequences)
+
+
+@expert_balance_bwd.register_fake
+def _(dbalance, dz, logits, state, top_k, score, sequences):
+    return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+
+
+expert_balance_bwd.register_autograd(_no_backward("strata_hip::expert_balance_bwd"))
+
+
+def _balance_setup_context(ctx, inputs, output):
+    logits, index, score, sequences = inputs
+    _, _, load, state = output
+    ctx.mark_non_differentiable(load, state)
+    ctx.set_materialize_grads(False)
+    ctx.save_for_backward(logits, state)
+    ctx.args = index.shape[-1], score, sequences
+
+
+def _balance_op_backward(ctx, dbalance, dz, _dload, _dstate):
+    if dbalance is None and dz is None:
+        return (None,) * 4
+    logits, state = ctx.saved_tensors
+    return expert_balance_bwd(dbalance, dz, logits, state, *ctx.args), None, None, None
+
+
+_expert_balance_op.register_autograd(_balance_op_backward, setup_context=_balance_setup_context)
 
 
 # ---------------------------------------------------------------------------
