@@ -812,6 +812,55 @@ typedef struct strata_hip_adamw_values_args {
 
 int strata_hip_adamw_state_values(const strata_hip_adamw_values_args* args, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Orthogonalisation of matrices by Newton-Schulz products, and the Muon step on it (an optimizer of the
+ * training step, train.py:1163-1170, for its matrices; no counterpart in the reference).
+ *   _orthogonalize: X = grad / max(|grad|, eps), |.| the root of the sum of squares; for each of `steps` triples (a, b, c):
+ *     A = X X^T,  X = a X + (b A + c A A) X   (of the transpose, where a matrix is taller than wide);  param = X
+ *   _muon_step: m = momentum m + (1 - momentum) grad;  u = momentum m + (1 - momentum) grad with nesterov, else m
+ *     param = param (1 - lr weight_decay) - lr s orthogonalize(u)
+ *     s = sqrt(max(1, rows / cols)) (ORIGINAL) or 0.2 sqrt(max(rows, cols)) (MATCH_RMS_ADAMW)
+ * matrices: a HOST array, read during the call, of stacks [batch, rows, cols] (each matrix by itself), contiguous and aligned
+ * to their elements (16-byte alignment of all of a stack's arrays and cols % 4 == 0 are the fast path); bf16 or f32,
+ * momentum and master (f32 weights that a bf16 parameter is rounded from, or NULL) f32.  What is written may overlap
+ * nothing (STRATA_HIP_EINVAL).  coefficients: a HOST array [steps, 3], which should keep singular values under 8.  At most 64
+ * steps, 2^20 rows and columns, the shorter side 2^15, 2^31 elements a stack and 2^34 in all, sides counted as the
+ * next multiple of 64.  workspace: strata_hip_muon_workspace() bytes of device memory (-1: sizes past these), 256-byte aligned.
+ * precise 0: products of fp16 operands (the result is off by about 1e-3); 1: of operands of twice the bits, at three
+ * times the cost (about 1e-6).  Sums are f32, norms 64-bit; results do not depend on timing, nor on the other matrices.
+ * ------------------------------------------------------------------------- */
+enum strata_hip_adjust { STRATA_HIP_ADJUST_ORIGINAL = 0, STRATA_HIP_ADJUST_MATCH_RMS_ADAMW = 1 };
+
+typedef struct strata_hip_muon_matrix {
+  void* param;          /* weights; _orthogonalize: the result */
+  const void* grad;     /* _orthogonalize: the matrices */
+  float* momentum;      /* _muon_step */
+  float* master;        /* _muon_step, or NULL */
+  int64_t batch, rows, cols;
+  double lr;
+  double weight_decay;
+  int32_t param_dtype;  /* strata_hip_dtype */
+  int32_t grad_dtype;
+  int32_t precise;
+  int32_t reserved0;
+} strata_hip_muon_matrix;
+
+typedef struct strata_hip_muon_args {
+  const strata_hip_muon_matrix* matrices;
+  int64_t count;
+  const double* coefficients;
+  void* workspace;
+  double momentum, eps;
+  int32_t steps;
+  int32_t nesterov;
+  int32_t adjust;       /* strata_hip_adjust */
+  int32_t reserved0;
+} strata_hip_muon_args;
+
+int64_t strata_hip_muon_workspace(const strata_hip_muon_matrix* matrices, int64_t count);
+int strata_hip_muon_step(const strata_hip_muon_args* args, void* stream);
+int strata_hip_orthogonalize(const strata_hip_muon_args* args, void* stream);
+
 int strata_hip_abi_version(void);
 
 #ifdef __cplusplus

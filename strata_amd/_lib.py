@@ -37,6 +37,9 @@ RES_MUL = 1
 SCORE_SOFTMAX = 0
 SCORE_SIGMOID = 1
 
+ADJUST_ORIGINAL = 0
+ADJUST_MATCH_RMS_ADAMW = 1
+
 ROPE_HALF = 0
 ROPE_INTERLEAVED = 1
 
@@ -435,6 +438,27 @@ class AdamwValuesArgs(ctypes.Structure):
     ]
 
 
+class MuonMatrix(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("param", "grad", "momentum", "master")] + \
+        [(n, ctypes.c_int64) for n in ("batch", "rows", "cols")] + \
+        [(n, ctypes.c_double) for n in ("lr", "weight_decay")] + [(n, ctypes.c_int32) for n in ("param_dtype", "grad_dtype", "precise", "reserved0")]
+
+
+class MuonArgs(ctypes.Structure):
+    _fields_ = [
+        ("matrices", ctypes.POINTER(MuonMatrix)),
+        ("count", ctypes.c_int64),
+        ("coefficients", ctypes.POINTER(ctypes.c_double)),
+        ("workspace", ctypes.c_void_p),
+        ("momentum", ctypes.c_double),
+        ("eps", ctypes.c_double),
+        ("steps", ctypes.c_int32),
+        ("nesterov", ctypes.c_int32),
+        ("adjust", ctypes.c_int32),
+        ("reserved0", ctypes.c_int32),
+    ]
+
+
 EXPORTS = {
     "strata_hip_na3d_fwd": ([ctypes.POINTER(Na3dArgs), ctypes.c_void_p], ctypes.c_int),
     "strata_hip_na3d_fwd_rope_q": (
@@ -480,6 +504,9 @@ EXPORTS = {
     "strata_hip_adamw_step_counts": (
         [ctypes.POINTER(AdamwArgs), ctypes.POINTER(ctypes.c_void_p), ctypes.c_void_p], ctypes.c_int),
     "strata_hip_adamw_state_values": ([ctypes.POINTER(AdamwValuesArgs), ctypes.c_void_p], ctypes.c_int),
+    "strata_hip_muon_workspace": ([ctypes.POINTER(MuonMatrix), ctypes.c_int64], ctypes.c_int64),
+    "strata_hip_muon_step": ([ctypes.POINTER(MuonArgs), ctypes.c_void_p], ctypes.c_int),
+    "strata_hip_orthogonalize": ([ctypes.POINTER(MuonArgs), ctypes.c_void_p], ctypes.c_int),
     "strata_hip_last_error": ([], ctypes.c_char_p),
     "strata_hip_abi_version": ([], ctypes.c_int),
 }

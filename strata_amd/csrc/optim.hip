@@ -28,7 +28,7 @@
 #include <unordered_map>
 #include <vector>
 
-#include "common.h"
+#include "optim.h"
 
 namespace strata {
 
@@ -608,16 +608,7 @@ static int aw_check(const strata_hip_adamw_args* a, const AwSteps& steps) {
     chunks += (t.n + AW_CHUNK - 1) / AW_CHUNK;
   }
   if (chunks > 0xffffff) return fail(STRATA_HIP_EUNSUPPORTED, "adamw_step: too many elements for one call");
-  std::sort(written.begin(), written.end());
-  for (size_t i = 1; i < written.size(); ++i)
-    if (written[i].first < written[i - 1].second)
-      return fail(STRATA_HIP_EINVAL, "adamw_step: two of the tensors to update overlap");
-  for (const auto& r : read) {  // the ranges written are disjoint: the last one that starts before r ends
-    auto w = std::lower_bound(written.begin(), written.end(), std::make_pair(r.second, (uintptr_t)0));
-    if (w != written.begin() && (--w)->second > r.first)
-      return fail(STRATA_HIP_EINVAL, "adamw_step: a gradient overlaps a tensor to update");
-  }
-  return STRATA_HIP_OK;
+  return check_ranges("adamw_step", written, read);
 }
 
 static int aw_launch(const strata_hip_adamw_args* a, int64_t* const* steps, hipStream_t st) {

@@ -9,7 +9,7 @@ missing library raises.  Every op has a fake (meta) implementation so that
 sigmoid gate), ``mlp_gelu_train``, ``layer_norm``, ``rope_qkv_pack`` (with or
 without qk_norm), ``expert_route``, ``expert_balance`` and ``expert_mlp`` have backwards on HIP kernels (a
 Linear's plain input gradient is torch's product); the other ops' autograd formulas raise.
-``adamw_step`` updates its tensors in place and is an ordinary function.
+``adamw_step`` and ``muon_step`` update their tensors in place and are ordinary functions.
 """
 
 from __future__ import annotations
@@ -53,6 +53,8 @@ __all__ = [
     "expert_mlp",
     "adamw_step",
     "adamw_state_values",
+    "orthogonalize",
+    "muon_step",
 ]
 
 
@@ -2142,11 +2144,16 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
         _launch("strata_hip_adamw_step_counts", a, step, (ctypes.c_void_p * n)(*map(Tensor.data_ptr, steps)))
     else:
         _launch("strata_hip_adamw_step", a, step)
-    try:
-        torch.autograd.graph.increment_version(written)
-    except RuntimeError:  # tensors made in inference mode carry no version
-        torch.autograd.graph.increment_version([t for t in written if not t.is_inference()])
+    _written(written)
     return norm
+
+
+def _written(ts: Sequence[Tensor]) -> None:
+    """Tells autograd that these were changed in place."""
+    try:
+        torch.autograd.graph.increment_version(ts)
+    except RuntimeError:  # tensors made in inference mode carry no version
+        torch.autograd.graph.increment_version([t for t in ts if not t.is_inference()])
 
 
 _ADAMW_CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
@@ -2198,3 +2205,177 @@ def _(codes, scales):
 
 
 _state_values_op.register_autograd(_no_backward("strata_hip::adamw_state_values"))
+
+
+# ---------------------------------------------------------------------------
+# Orthogonalised updates
+# ---------------------------------------------------------------------------
+ADJUSTS = {"original": _lib.ADJUST_ORIGINAL, "match_rms_adamw": _lib.ADJUST_MATCH_RMS_ADAMW}
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
+
+
+def _newton_schulz(name: str, coefficients, steps: Optional[int], eps: float):
+    """A ctypes array of the steps' triples, and how many."""
+    rows = list(coefficients)
+    if not rows or not isinstance(rows[0], (int, float)):
+        if steps is not None and steps != len(rows):
+            raise ValueError(f"{name}: {len(rows)} triples of coefficients for {steps} steps")
+        flat = [float(c) for row in rows for c in row]
+        if any(len(row) != 3 for row in rows):
+            raise ValueError(f"{name}: coefficients must be three numbers, or three for each step")
+        steps = len(rows)
+    else:
+        if len(rows) != 3:
+            raise ValueError(f"{name}: coefficients must be three numbers, or three for each step")
+        steps = 5 if steps is None else int(steps)
+        flat = [float(c) for c in rows] * max(steps, 0)
+    if not 0 <= steps <= 64:
+        raise ValueError(f"{name}: between 0 and 64 steps, got {steps}")
+    if not all(map(math.isfinite, flat)):
+        raise ValueError(f"{name}: coefficients must be finite")
+    if not 0 < eps < math.inf:
+        raise ValueError(f"{name}: eps must be positive and finite, got {eps}")
+    return flat, steps
+
+
+def _muon_space(name: str, table, n: int, dev) -> Tensor:
+    size = int(_lib.function("strata_hip_muon_workspace")(table, n))
+    if size < 0:
+        _lib.raise_error(name, _lib.EUNSUPPORTED)
+    return torch.empty(size, dtype=torch.uint8, device=dev)
+
+
+def orthogonalize(x: Tensor, coefficients: Sequence[float] | Sequence[Sequence[float]] = NEWTON_SCHULZ,
+                  steps: Optional[int] = None, eps: float = 1e-7, precise: Optional[bool] = None) -> Tensor:
+    """Matrices with the singular vectors of x's and singular values near 1, by Newton-Schulz products (the update
+    of ``muon_step``)::
+
+        X = x / max(norm(x), eps)                               (the root of the sum of squares)
+        X = a X + (b A + c A A) X,  A = X X^T                   (5 times, or ``steps``)
+
+    x ``[..., rows, cols]`` in bf16 or fp32, every matrix by itself; the result has its shape and type.  A matrix taller
+    than wide is treated as its transpose, which gives the same.  ``coefficients`` are (a, b, c), or such a triple
+    for each step; they should keep singular values under 8.  The usual ones bring values from 0.001 on
+    to about [0.7, 1.2], not to 1.
+
+    ``precise`` (of fp32 matrices where it is not given): the products' operands keep 22 bits, at three times the cost, and the result is
+    off by about 1e-6 of its norm; otherwise fp16 operands with fp32 sums, off by about 1e-3, less than
+    a bf16 result's own rounding.  A matrix with a value that is not finite becomes NaN, a zero one stays zero.
+    Not differentiable.  At most 2^20 rows and columns, 2^15 of the fewer of them."""
+    flat, steps = _newton_schulz("orthogonalize", coefficients, steps, eps)
+    if _eager(x):
+        return _orthogonalize(x, flat, eps, precise)
+    return _orthogonalize_op(x, flat, float(eps), precise)
+
+
+def _orthogonalize(x: Tensor, coefficients: Sequence[float], eps: float, precise: Optional[bool]) -> Tensor:
+    name = "orthogonalize"
+    _require_gpu(name, x)
+    code = _dtype_code(name, x)
+    if x.dim() < 2:
+        raise ValueError(f"{name}: expected matrices [..., rows, cols], got shape {list(x.shape)}")
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise RuntimeError(f"{name}: not differentiable, call it under torch.no_grad() or on a detached tensor")
+    if len(coefficients) % 3:
+        raise ValueError(f"{name}: three coefficients for each step")
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    n = x.numel()
+    if not n:
+        return out
+    rows, cols = x.shape[-2:]
+    s = x.contiguous()
+    t = (_lib.MuonMatrix * 1)((out.data_ptr(), s.data_ptr(), None, None, n // (rows * cols), rows, cols, 0.0, 0.0, code, code,
+                               int(code == _lib.F32 if precise is None else precise), 0))
+    ws = _muon_space(name, t, 1, x.device)
+    a = _lib.MuonArgs(t, 1, (ctypes.c_double * len(coefficients))(*coefficients), ws.data_ptr(), 0.0, float(eps),
+                      len(coefficients) // 3, 0, _lib.ADJUST_ORIGINAL, 0)
+    _launch("strata_hip_orthogonalize", a, x)
+    return out
+
+
+@torch.library.custom_op("strata_hip::orthogonalize", mutates_args=())
+def _orthogonalize_op(x: Tensor, coefficients: Sequence[float], eps: float, precise: Optional[bool]) -> Tensor:
+    """``orthogonalize`` as a custom op, with three coefficients for each step."""
+    return _orthogonalize(x, coefficients, eps, precise)
+
+
+@_orthogonalize_op.register_fake
+def _(x, coefficients, eps, precise):
+    return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
+_orthogonalize_op.register_autograd(_no_backward("strata_hip::orthogonalize"))
+
+
+def muon_step(params: Sequence[Tensor], grads: Sequence[Tensor], momentums: Sequence[Tensor], *,
+              lr: float | Sequence[float] = 1e-3, momentum: float = 0.95, nesterov: bool = True,
+              weight_decay: float | Sequence[float] = 0.1, adjust: str = "original",
+              coefficients: Sequence[float] | Sequence[Sequence[float]] = NEWTON_SCHULZ, steps: Optional[int] = None,
+              eps: float = 1e-7, masters: Optional[Sequence[Optional[Tensor]]] = None, precise: Optional[bool] = None) -> None:
+    """One Muon step, in place, over many contiguous matrices of one GPU::
+
+        m = momentum m + (1 - momentum) grad
+        u = momentum m + (1 - momentum) grad with nesterov, else m
+        p = p (1 - lr weight_decay) - lr s orthogonalize(u)
+
+    s = sqrt(max(1, rows / cols)) with ``adjust="original"``, 0.2 sqrt(max(rows, cols)) with ``"match_rms_adamw"``
+    (updates as large as AdamW's, so that its rates carry over).  A parameter has two dimensions, or more before
+    them: a stack of matrices, each with an update of its own (the experts' weights).  Parameters and gradients
+    are bf16 or fp32, momentums fp32; ``masters`` are fp32 weights (or None) that a bf16 parameter is rounded
+    from.  ``lr`` and ``weight_decay`` may be one number for every tensor; ``coefficients``, ``steps``, ``eps`` and
+    ``precise`` are ``orthogonalize``'s (where ``precise`` is not given, that of fp32 weights, masters among them).
+    The step's host work is proportional to the tensors, its launches are not: all matrices share them."""
+    name = "muon_step"
+    if _jit_trace() is not None or torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+        raise RuntimeError(f"{name}: no operator, a trace of it would leave the step out")
+    if adjust not in ADJUSTS:
+        raise ValueError(f"{name}: adjust must be one of {sorted(ADJUSTS)}, got {adjust!r}")
+    if not 0 <= momentum < 1:
+        raise ValueError(f"{name}: momentum must lie in [0, 1), got {momentum}")
+    flat, steps = _newton_schulz(name, coefficients, steps, eps)
+    n = len(params)
+    cols = {"params": params, "grads": grads, "momentums": momentums, "masters": masters}
+    for x in cols.values():
+        if x is not None and len(x) != n:
+            raise ValueError(f"{name}: the lists must have one entry for each of the {n} parameters")
+    rates = [[float(r)] * n if isinstance(r, (int, float)) else list(map(float, r)) for r in (lr, weight_decay)]
+    if any(len(r) != n for r in rates):
+        raise ValueError(f"{name}: lr and weight_decay must be numbers or have one entry for each parameter")
+    if not n:
+        return
+    dev, shapes = params[0].get_device(), [p.shape for p in params]
+    _require_gpu(name, params[0])
+    some = {}
+    for what, ts in cols.items():
+        if ts is None:
+            continue
+        want = shapes
+        if what == "masters":
+            want = [s for s, t in zip(shapes, ts) if t is not None]
+            ts = [t for t in ts if t is not None]
+        some[what] = ts
+        if ts and set(map(Tensor.get_device, ts)) != {dev}:
+            raise ValueError(f"{name}: every tensor must be on the first parameter's GPU (cuda:{dev}), {what} are not")
+        if not _MUON_DTYPES[what].issuperset(map(_DTYPE_OF, ts)) or [t.shape for t in ts] != want or not all(map(Tensor.is_contiguous, ts)):
+            raise ValueError(f"{name}: {what} must be contiguous, of their parameter's shape and of {sorted(map(str, _MUON_DTYPES[what]))}")
+    if min(map(len, shapes)) < 2:
+        raise ValueError(f"{name}: parameters must be matrices or stacks of them, got shape {list(min(shapes, key=len))}")
+    rows = []
+    for p, g, m, w, s, r, d in zip(params, grads, momentums, masters or repeat(None), shapes, *rates):
+        k = s[-2] * s[-1]
+        code = _ADAMW_CODE[p.dtype]
+        if w is not None and code != _lib.BF16:
+            raise ValueError(f"{name}: masters belong to bfloat16 parameters")
+        rows.append(_MUON_ROW(p.data_ptr(), g.data_ptr(), m.data_ptr(), 0 if w is None else w.data_ptr(), p.numel() // k if k else 0, s[-2], s[-1],
+                              r, d, code, _ADAMW_CODE[g.dtype], (code == _lib.F32 or w is not None) if precise is None else bool(precise), 0))
+    table = (_lib.MuonMatrix * n).from_buffer_copy(b"".join(rows))
+    ws = _muon_space(name, table, n, params[0].device)
+    a = _lib.MuonArgs(table, n, (ctypes.c_double * len(flat))(*flat), ws.data_ptr(), float(momentum), float(eps), steps, int(nesterov),
+                      ADJUSTS[adjust], 0)
+    _launch("strata_hip_muon_step", a, params[0])
+    _written([*params, *some.get("masters", ())])
+
+
+_MUON_DTYPES = {"params": {torch.bfloat16, torch.float32}, "grads": {torch.bfloat16, torch.float32}, "momentums": {torch.float32},
+                "masters": {torch.float32}}
+_MUON_ROW = struct.Struct("".join({ctypes.c_double: "d", ctypes.c_int32: "i"}.get(c, "q") for _, c in _lib.MuonMatrix._fields_)).pack

@@ -1,18 +1,24 @@
-"""AdamW for the training of the block modules, one fused step over all parameters.
+"""AdamW and Muon for the training of the block modules, one fused step over all parameters.
 
-Stands where the reference's training loop clips its gradients and steps its optimizer
-(train.py:1163-1170).  ``torch.ops``-level form: :func:`strata_amd.ops.adamw_step`.
+They stand where the reference's training loop clips its gradients and steps its optimizer
+(train.py:1163-1170).  ``torch.ops``-level forms: :func:`strata_amd.ops.adamw_step`, :func:`strata_amd.ops.muon_step`.
 """
 
 from __future__ import annotations
 
 from itertools import chain
-from typing import Optional
+from typing import Optional, Sequence
 
 import torch
-from torch import Tensor
+from torch import Tensor, nn
 
 from . import ops
+from .modules import ExpertMlp
+
+
+def _uncaptured(name: str) -> None:
+    if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{name}: a step is captured after an eager one with the same gradients, which makes its states")
 
 
 class AdamW(torch.optim.Optimizer):
@@ -74,10 +80,6 @@ class AdamW(torch.optim.Optimizer):
             s["master"] = p.detach().float()
         return s
 
-    def _uncaptured(self) -> None:
-        if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("AdamW: a step is captured after an eager one with the same gradients, which makes its states")
-
     def _split_counts(self, states: list[dict]) -> None:
         """States that this step leaves out keep their count: a copy of one that they share with others."""
         taking, counts, kept = set(map(id, states)), {id(s["step"]) for s in states}, {}
@@ -86,7 +88,7 @@ class AdamW(torch.optim.Optimizer):
             if step is None or id(s) in taking or id(step) not in counts:
                 continue
             if id(step) not in kept:
-                self._uncaptured()
+                _uncaptured("AdamW")
                 kept[id(step)] = step.clone()
             s["step"] = kept[id(step)]
 
@@ -110,7 +112,7 @@ class AdamW(torch.optim.Optimizer):
             return loss
         new = [p for p in ps if not self.state[p]]
         if new:
-            self._uncaptured()
+            _uncaptured("AdamW")
             step = torch.zeros(1, dtype=torch.int64, device=ps[0].device)
             for p in new:
                 self.state[p].update(self._new_state(p, step))
@@ -139,3 +141,104 @@ class AdamW(torch.optim.Optimizer):
                 values[id(one)] = int(one)
             s["step"] = counts.setdefault(values[id(one)], s["step"])
             self.state[p] = s
+
+
+class Muon(torch.optim.Optimizer):
+    """Muon over the matrices of one GPU: the momentum's singular values are brought near 1 before it is
+    subtracted (``ops.muon_step``).
+
+    Parameters have two dimensions, or more before them: a stack of matrices, each with an update of its own, as the
+    experts' ``w1`` and ``w2``.  Vectors, and what is no matrix to multiply by (embeddings, convolutions, the
+    experts' ``b1`` and ``b2``), belong to another optimizer; ``matrices`` tells them apart::
+
+        some, rest = matrices(model)
+        steps = [Muon(some, lr=2e-3, adjust="match_rms_adamw"), AdamW(rest, lr=2e-3)]
+
+    adjust      "original": updates times sqrt(max(1, rows / cols)).  "match_rms_adamw": times
+                0.2 sqrt(max(rows, cols)), as large as AdamW's, whose rates and decay then carry over.
+    master      fp32 weights kept beside bf16 parameters, which are rounded from them.
+    precise     operands of 22 bits at three times the products' cost; where it is not given, for fp32 weights, masters among
+                them.  False: fp16 operands, an update off by about 1e-3 of its size.
+
+    ``lr`` and ``weight_decay`` may differ between parameter groups, the rest is the optimizer's.  The momentum is
+    fp32.  A step can be captured in a graph, after one eager step with the same gradients has made the states (the
+    rates are those of the capture).  A master weight stands for its parameter as ``AdamW``'s does."""
+
+    def __init__(self, params, lr: float = 1e-3, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.1,
+                 adjust: str = "original", coefficients: Sequence = ops.NEWTON_SCHULZ, steps: Optional[int] = None,
+                 eps: float = 1e-7, master: bool = True, precise: Optional[bool] = None):
+        if adjust not in ops.ADJUSTS:
+            raise ValueError(f"Muon: adjust must be one of {sorted(ops.ADJUSTS)}, got {adjust!r}")
+        if not 0.0 <= momentum < 1.0:
+            raise ValueError(f"Muon: momentum must lie in [0, 1), got {momentum}")
+        ops._newton_schulz("Muon", coefficients, steps, eps)
+        self.momentum, self.nesterov, self.adjust, self.eps = float(momentum), bool(nesterov), adjust, float(eps)
+        self.coefficients, self.steps, self.master, self.precise = tuple(coefficients), steps, master, precise
+        super().__init__(params, dict(lr=lr, weight_decay=weight_decay))
+
+    _OWN = ("momentum", "nesterov", "adjust", "eps", "coefficients", "steps", "master", "precise")
+
+    def __getstate__(self) -> dict:  # copies and pickles: torch's own keeps the groups and states alone
+        return {**super().__getstate__(), **{k: self.__dict__[k] for k in self._OWN}}
+
+    def add_param_group(self, group) -> None:
+        for k in self._OWN:
+            if isinstance(group, dict) and k in group:
+                raise ValueError(f"Muon: {k} is the optimizer's, not a parameter group's")
+        super().add_param_group(group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dim() < 2:
+                self.param_groups.pop()
+                raise ValueError(f"Muon: parameters must be matrices or stacks of them, got shape {list(p.shape)}")
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        ps, lrs, wds = [], [], []
+        for group in self.param_groups:
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse:
+                    raise ValueError("Muon: sparse gradients are not supported")
+                ps.append(p)
+                lrs.append(group["lr"])
+                wds.append(group["weight_decay"])
+        if not ps:
+            return loss
+        for p in ps:
+            if not self.state[p]:
+                _uncaptured("Muon")
+                self.state[p]["momentum"] = torch.zeros(p.shape, device=p.device)
+                if self.master and p.dtype == torch.bfloat16:
+                    self.state[p]["master"] = p.detach().float()
+        states = [self.state[p] for p in ps]
+        ops.muon_step(
+            ps, [p.grad.contiguous() for p in ps], [s["momentum"] for s in states], lr=lrs, momentum=self.momentum,
+            nesterov=self.nesterov, weight_decay=wds, adjust=self.adjust, coefficients=self.coefficients, steps=self.steps,
+            eps=self.eps, masters=[s.get("master") for s in states], precise=self.precise)
+        return loss
+
+    def load_state_dict(self, state_dict) -> None:
+        """As torch's, but every state keeps the type it was saved in."""
+        super().load_state_dict(state_dict)
+        saved = chain.from_iterable(g["params"] for g in state_dict["param_groups"])
+        for i, p in zip(saved, chain.from_iterable(g["params"] for g in self.param_groups)):
+            if i in state_dict["state"]:
+                self.state[p] = {k: v.detach().to(p.device, copy=True) for k, v in state_dict["state"][i].items()}
+
+
+def matrices(module: nn.Module) -> tuple[list[nn.Parameter], list[nn.Parameter]]:
+    """A module's parameters as ``(matrices, rest)``, each in the module's order: the weights of its
+    ``nn.Linear`` and the stacked weights of its ``ExpertMlp``; and all others, for ``AdamW``."""
+    some = set()
+    for m in module.modules():
+        if isinstance(m, nn.Linear):
+            some.add(m.weight)
+        elif isinstance(m, ExpertMlp):
+            some |= {m.w1, m.w2}
+    every = list(module.parameters())
+    return [p for p in every if p in some], [p for p in every if p not in some]
