@@ -5,20 +5,22 @@
 //   p <- p (1 - lr decay) - lr adjust X
 //
 // A matrix m x n (m <= n) lives in a workspace as [m', n'], both rounded up to 64 and zero beyond m and n, which every
-// product leaves zero: no product has an edge to watch.  Matrices of one shape stand one behind the other, and a launch takes
-// the tiles of all shapes: three launches a step, whatever the number of matrices.  A and P are symmetric: only tiles on
-// and above the diagonal are computed and also written transposed, so that a step costs m m n + m m m + 2 m m n
-// operations instead of 4 m m n + 2 m m m.  P X reads X along its rows, transposed out of LDS (ds_read_b64_tr_b16).
+// product leaves zero: no product has an edge to watch.  It stands there in panels of 32 columns, [n' / 32][m'][32], so
+// that what a stage of a product copies to LDS is one piece (rows of n' elements instead: 8 to 30% slower).  Matrices of one
+// shape stand one behind the other, and a launch takes the tiles of all shapes: three launches a step, whatever the
+// number of matrices.  A and P are symmetric: only tiles on and above the diagonal are computed and also written
+// transposed, so that a step costs m m n + m m m + 2 m m n operations instead of 4 m m n + 2 m m m.  P X reads X along its
+// rows, transposed out of LDS (ds_read_b64_tr_b16).
 //
 // What is rounded: the products' operands are fp16, scaled by powers of two (X 2^12, A and P 2^10: there is room up to
 // 16 and 64, the usual coefficients keep them under 2 and 8; most values lie at 1 / sqrt(n), well above the 2^-14 where
-// fp16 loses bits), sums are fp32.
-// Singular values near 0 grow 3.4-fold a step with all the noise among them, so it is the early roundings
-// of X that show, and those of its term a X alone (P is small then): X is held as the sum of two fp16, of which the
-// products take the first, in all steps but the last two.  Simulated, the result is off by 0.3e-3 to 1.5e-3 for
-// noise, decaying and low-rank spectra (3.8e-3 without the second fp16, 10 to 30e-3 with iterates in bf16), below the 1.7e-3
-// of a bf16 result's own rounding.  `precise`: X, A and P are sums of two fp16 throughout and a product is three, high
-// high, high low and low high: 0.2e-6 to 0.7e-6.
+// fp16 loses bits), sums are fp32.  Singular values near 0 grow 3.4-fold a step with all the noise among them, so it is
+// the early roundings of X that show, and those of its term a X alone (P is small then): X is held as the sum of two
+// fp16, of which the products take the first, in the first two steps.  Simulated, the result is off by 0.7e-3 to 1.5e-3 for noise,
+// decaying and low-rank spectra (3.7e-3 without the second fp16, 10 to 30e-3 with iterates in bf16), below the 1.7e-3 of
+// a bf16 result's own rounding; a second fp16 in later steps gains nothing and costs 50 us of 350 a product of 133 M
+// elements.  `precise`: X, A and P are sums of two fp16 throughout and a product is three, high high, high low and low
+// high: off by 1e-6 to 3e-6, as products of fp32 are.
 #include <algorithm>
 #include <cmath>
 #include <exception>
@@ -35,10 +37,12 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int MU_PAD = 64;       // rows and columns of a matrix in the workspace are multiples of it
+constexpr int MU_K = 32;         // columns that stand together there, row by row: X[np / 32][mp][32]
 constexpr int MU_CHUNK = 8192;   // elements a workgroup of the momentum's pass
+constexpr int MU_LO_STEPS = 2;   // steps whose X has its second fp16, where not all have
 constexpr int MU_PER = 40;       // tensors a launch, and shapes: kernel arguments are 4 KiB
 constexpr float MU_X = 0x1p12f, MU_A = 0x1p10f;  // scales of X, and of A and P
-enum { MU_P32 = 1, MU_G32 = 2, MU_TALL = 4, MU_ALIGNED = 8, MU_NESTEROV = 16, MU_STEP = 32 };
+enum { MU_P32 = 1, MU_G32 = 2, MU_TALL = 4, MU_ALIGNED = 8, MU_NESTEROV = 16, MU_STEP = 32, MU_LO = 64 };
 
 struct MuTensor {
   void* p;           // weights, or the result of an orthogonalisation alone
@@ -133,7 +137,8 @@ struct MuTile {
   int64_t base;   // first element of the matrix in its tensor
   int64_t at;     // first element of the tile in the workspace
   int64_t row0, col0;
-  int64_t np;
+  int panel;      // elements of MU_K columns there
+  __device__ __forceinline__ int64_t element(int row, int col) const { return at + (int64_t)(col / MU_K) * panel + row * MU_K + col % MU_K; }
 };
 __device__ __forceinline__ MuTile mu_tile(const MuTensor& t, uint32_t local) {
   const bool tall = t.flags & MU_TALL;
@@ -143,8 +148,8 @@ __device__ __forceinline__ MuTile mu_tile(const MuTensor& t, uint32_t local) {
   const int64_t ti = k / nt, tj = k % nt;
   MuTile r;
   r.base = (int64_t)mat * t.rows * t.cols;
-  r.np = nt * 64;
-  r.at = ((int64_t)mat * mt * 64 + ti * 64) * r.np + tj * 64;
+  r.panel = (int)mt * 64 * MU_K;
+  r.at = (int64_t)mat * mt * 64 * nt * 64 + tj * (64 / MU_K) * r.panel + ti * 64 * MU_K;
   r.row0 = (tall ? tj : ti) * 64;
   r.col0 = (tall ? ti : tj) * 64;
   return r;
@@ -171,6 +176,17 @@ __global__ __launch_bounds__(256) void muon_pack_kernel(MuBatch b) {
   const double norm = sqrt(((red[0] + red[1]) + red[2]) + red[3]);
   const double scale = norm == 0. ? 0. : MU_X / (norm < b.eps ? b.eps : norm);  // 64-bit: of tiny updates it leaves fp32
   const int r = tid >> 4, c = (tid & 15) * 4;
+  auto write = [&](int row, const float (&v)[4]) {
+    f16x4 h, l;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      h[e] = (f16)v[e];
+      l[e] = (f16)(v[e] - (float)h[e]);
+    }
+    const int64_t at = x.element(row, c);
+    *(f16x4*)(t.x + at) = h;
+    *(f16x4*)(t.xlo + at) = l;
+  };
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int64_t row = x.row0 + 16 * k + r, col = x.col0 + c, i = x.base + row * t.cols + col;
@@ -188,23 +204,15 @@ __global__ __launch_bounds__(256) void muon_pack_kernel(MuBatch b) {
           if (col + e < t.cols) v[e] = one(mu_load(t.g, i + e, g32), t.m ? t.m[i + e] : 0.f);
       }
     }
+    if (!tall) write(16 * k + r, v);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) tile[16 * k + r][c + e] = v[e];
+    for (int e = 0; e < 4; ++e)
+      if (tall) tile[16 * k + r][c + e] = v[e];
   }
+  if (!tall) return;  // uniform
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    f16x4 h, l;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float v = tall ? tile[c + e][16 * k + r] : tile[16 * k + r][c + e];
-      h[e] = (f16)v;
-      l[e] = (f16)(v - (float)h[e]);
-    }
-    const int64_t at = x.at + (16 * k + r) * x.np + c;
-    *(f16x4*)(t.x + at) = h;
-    *(f16x4*)(t.xlo + at) = l;
-  }
+  for (int k = 0; k < 4; ++k) write(16 * k + r, {tile[c][16 * k + r], tile[c + 1][16 * k + r], tile[c + 2][16 * k + r], tile[c + 3][16 * k + r]});
 }
 
 // ---- the weights' update from X, or X itself ----
@@ -214,34 +222,57 @@ __global__ __launch_bounds__(256) void muon_apply_kernel(MuBatch b) {
   const MuTensor& t = b.t[mu_entry(b.count, wg, [&](int i) { return b.t[i].first; })];
   const MuTile x = mu_tile(t, wg - t.first);
   const int tid = threadIdx.x, r = tid >> 4, c = (tid & 15) * 4;
-  const bool p32 = t.flags & MU_P32, tall = t.flags & MU_TALL;
+  const bool p32 = t.flags & MU_P32, tall = t.flags & MU_TALL, step = t.flags & MU_STEP, two = t.flags & MU_LO;
+  const bool wide = (t.flags & MU_ALIGNED) && x.col0 + c + 4 <= t.cols;
+  const int64_t first = x.base + (x.row0 + r) * t.cols + x.col0 + c;
+  f32x4 p[4] = {}, v[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    const int64_t at = x.at + (16 * k + r) * x.np + c;
-    const f16x4 h = *(const f16x4*)(t.x + at), l = *(const f16x4*)(t.xlo + at);
+    const int64_t i = first + 16 * k * t.cols;
+    if (!step || x.row0 + 16 * k + r >= t.rows) continue;
+    if (wide) p[k] = t.master ? *(const f32x4*)(t.master + i) : mu_load4(t.p, i, p32);
+    else
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float v = ((float)h[e] + (float)l[e]) * (1.f / MU_X);
-      if (tall) tile[c + e][16 * k + r] = v;
-      else tile[16 * k + r][c + e] = v;
-    }
+      for (int e = 0; e < 4; ++e)
+        if (x.col0 + c + e < t.cols) p[k][e] = t.master ? t.master[i + e] : mu_load(t.p, i + e, p32);
   }
-  __syncthreads();
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    const int64_t row = x.row0 + 16 * k + r, col = x.col0 + c, i = x.base + row * t.cols + col;
-    if (row >= t.rows) continue;
+    const int64_t at = x.element(16 * k + r, c);
+    const f16x4 h = *(const f16x4*)(t.x + at), l = two ? *(const f16x4*)(t.xlo + at) : (f16x4){};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (col + e >= t.cols) continue;
-      float v = tile[16 * k + r][c + e];
-      if (t.flags & MU_STEP) {  // uniform
-        const float p = t.master ? t.master[i + e] : mu_load(t.p, i + e, p32);
-        v = fmaf(-t.rate, v, p * t.decay);
+    for (int e = 0; e < 4; ++e) v[k][e] = ((float)h[e] + (float)l[e]) * (1.f / MU_X);
+  }
+  if (tall) {  // uniform
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) tile[c + e][16 * k + r] = v[k][e];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[k][e] = tile[16 * k + r][c + e];
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int64_t i = first + 16 * k * t.cols;
+    if (x.row0 + 16 * k + r >= t.rows) continue;
+    if (step)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[k][e] = fmaf(-t.rate, v[k][e], p[k][e] * t.decay);
+    if (wide) {
+      if (t.master) *(f32x4*)(t.master + i) = v[k];
+      if (p32) *(f32x4*)((float*)t.p + i) = v[k];
+      else *(u32x2*)((bf16*)t.p + i) = (u32x2){pack_bf16x2(v[k][0], v[k][1]), pack_bf16x2(v[k][2], v[k][3])};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (x.col0 + c + e >= t.cols) continue;
+        if (t.master) t.master[i + e] = v[k][e];
+        if (p32) ((float*)t.p)[i + e] = v[k][e];
+        else ((bf16*)t.p)[i + e] = (bf16)v[k][e];
       }
-      if (t.master) t.master[i + e] = v;
-      if (p32) ((float*)t.p)[i + e] = v;
-      else ((bf16*)t.p)[i + e] = (bf16)v;
     }
   }
 }
@@ -254,39 +285,89 @@ struct MuShape {
   f16* out;
   int mp, np, count;
   int tiles;      // of all its matrices
-  uint32_t first;
   int flags;
 };
 struct MuGemm {
   MuShape s[MU_PER];
+  uint32_t first[MU_PER];  // a shape's first workgroup
   int count;
   float alpha, beta;  // of the product and of d
 };
 static_assert(sizeof(MuGemm) <= 4096, "kernel arguments");
 enum { MU_GRAM = 0, MU_POLY = 1, MU_UPDATE = 2 };
-enum { MU_THREE = 1, MU_LO_IN = 2, MU_LO_OUT = 4 };  // high high, high low, low high; d has, out gets its second fp16
+enum { MU_LO_IN = 1, MU_LO_OUT = 2 };  // d has, out gets its second fp16
 
-// 16-byte chunks of an LDS row are stored at their index xor these: rows of 64 columns read 16 bytes a lane by 32
-// rows at one chunk, rows of BN columns read transposed by 8 rows at 4 chunks.
-__device__ __forceinline__ int mu_swz(int row) { return (row & 7) ^ ((row >> 3) & 1); }
-template <int BN>
-__device__ __forceinline__ int mu_wswz(int row) {
-  return BN == 64 ? ((row >> 1) & 1) << 2 : (row & 3) << 2;
+// Chunks of 16 bytes of an LDS row of MU_K columns are stored at their index xor this: the 16 rows that an instruction's
+// lanes read at one chunk lie in all banks.  (Rows that are read transposed, 4 of 64 bytes at once, are so by themselves.)
+__device__ __forceinline__ int mu_swz(int row) { return (row >> 2) & 3; }
+
+// 32 x 32 fp16 as the matrix instructions leave them, a lane with columns 8 q + 4 hi .. + 3 of row l32 in halves q & 1 of
+// w[q / 2], to rows as memory has them: w[t] is columns mu_chunk(lane) .. + 7 of row 16 t + lane % 16, so that 64 lanes
+// write 1 KiB in one piece.  mu_unrows is the way back.
+__device__ __forceinline__ void mu_swap32(u32x4& w) {
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(w[x], w[x + 2], false, false);
+    w[x] = r[0];
+    w[x + 2] = r[1];
+  }
+}
+__device__ __forceinline__ void mu_swap16(u32x4 (&w)[2]) {
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(w[0][x], w[1][x], false, false);
+    w[0][x] = r[0];
+    w[1][x] = r[1];
+  }
+}
+__device__ __forceinline__ void mu_rows(u32x4 (&w)[2]) {
+  mu_swap32(w[0]);
+  mu_swap32(w[1]);
+  mu_swap16(w);
+}
+__device__ __forceinline__ void mu_unrows(u32x4 (&w)[2]) {
+  mu_swap16(w);
+  mu_swap32(w[0]);
+  mu_swap32(w[1]);
+}
+__device__ __forceinline__ int mu_chunk(int lane) { return 16 * ((lane >> 4) & 1) + 8 * (lane >> 5); }
+// Four lanes with four columns each of one row after the other: the transpose, lane k with column k of the four rows.
+__device__ __forceinline__ u32x2 mu_quads(u32x2 w, int lane) {
+  const bool odd = lane & 1, up = lane & 2;
+  uint32_t e[2];
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {  // columns 2 x + odd of rows lane & ~1, + 1
+    const uint32_t o = (uint32_t)__builtin_amdgcn_mov_dpp((int)w[x], 0xb1, 0xf, 0xf, true);
+    e[x] = odd ? __builtin_amdgcn_perm(w[x], o, 0x07060302) : __builtin_amdgcn_perm(o, w[x], 0x05040100);
+  }
+  const uint32_t o = (uint32_t)__builtin_amdgcn_mov_dpp((int)(up ? e[0] : e[1]), 0x4e, 0xf, 0xf, true);
+  return up ? (u32x2){o, e[1]} : (u32x2){e[0], o};
 }
 
-template <int BM, int BN, int WGM, int WGN, int NST, int MODE>
+template <int N>
+__device__ __forceinline__ void mu_wait() {  // all but the last N copies have landed
+  static_assert(N < 64, "vmcnt");
+  __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
+}
+
+// T x T tiles of one product, by WGM x WGN waves with v_mfma_f32_32x32x16_f16, whose A operand the product's columns are: a
+// lane owns four consecutive columns of one row.  Both operands (PARTS 2: and their second fp16) stream into an LDS ring of
+// NST stages of MU_K columns (buffer_load ... lds); the fragments of 16 columns are read while those before them
+// multiply, over the stages' borders too, so stage kt + 1 has landed when kt begins.
+// Bound by the matrix instructions and the power that they draw (the clock falls from 2.4 to 1.8 GHz): 48 matrices 960 x 960 to 960 x
+// 3840, P X 312 us (814 TFLOP/s; a library product of 960 x 960 x 3840 by 12 910, of 8192^3 1216), X X^T 178 us (716 of the
+// half that is needed, 256 x 256 tiles on the diagonal and the edge 42% more); 79% of a 256 x 256 tile's cycles in the
+// loop issue them, its start and epilogue are 26% of P X.  128 x 128 tiles wait for L2 (16 KiB a stage of 256 cycles); of two fp16
+// they multiply three times and do not.
+template <int T, int WGM, int WGN, int NST, int PARTS, int MODE>
 __global__ __launch_bounds__(64 * WGM * WGN, 1) void muon_gemm_kernel(MuGemm p) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr bool WT = MODE == MU_UPDATE, SYM = !WT;
-  static_assert(!SYM || BM == BN, "square tiles");
-  constexpr int BK = 64, NW = WGM * WGN;
-  constexpr int WTM = BM / WGM, WTN = BN / WGN, FM = WTM / 32, FN = WTN / 32;
-  constexpr int ROWB = BK * 2, CH = ROWB / 16, RPC = 1024 / ROWB;
-  constexpr int XB = BM * ROWB, STAGE = XB + BN * ROWB;
-  constexpr int LPX = XB / 1024 / NW, LPW = BN * ROWB / 1024 / NW;  // 1-KiB copies a wave and stage
-  constexpr int WLPR = BN / 8, WRPC = 64 / WLPR;
-  constexpr int SLAB = 32 * WTN * 4;
-  static_assert(WTM % 32 == 0 && WTN % 32 == 0 && LPX > 0 && LPW > 0 && NW * SLAB <= NST * STAGE, "wave tile, stage and slab layout");
+  constexpr int NW = WGM * WGN, KS = MU_K / 16;
+  constexpr int WTM = T / WGM, WTN = T / WGN, FM = WTM / 32, FN = WTN / 32;
+  constexpr int ROWB = MU_K * 2, PB = T * ROWB, XB = PARTS * PB, STAGE = 2 * XB;  // one fp16 of an operand, an operand, a stage
+  constexpr int LP = PB / 1024 / NW, COPIES = 2 * PARTS * LP;                      // 1-KiB copies a wave
+  static_assert(WTM % 32 == 0 && WTN % 32 == 0 && PB % (1024 * NW) == 0 && NST >= 3, "layout");
   __shared__ __attribute__((aligned(1024))) char lds[NST * STAGE];
 
   const int tid = (int)__builtin_amdgcn_workitem_id_x();
@@ -296,10 +377,11 @@ __global__ __launch_bounds__(64 * WGM * WGN, 1) void muon_gemm_kernel(MuGemm p) 
 
   // Each shape's tiles are dealt to the XCDs in blocks: one matrix's on one XCD, every XCD with its share of every shape.
   const uint32_t wg = (uint32_t)__builtin_amdgcn_workgroup_id_x();
-  const MuShape& s = p.s[mu_entry(p.count, wg, [&](int i) { return p.s[i].first; })];
-  const int id = xcd_tile_order(s.tiles, (int)(wg - s.first));
-  const int mp = s.mp, np = s.np;
-  const int mt = (mp + BM - 1) / BM, nt = (np + BN - 1) / BN, per = SYM ? mt * (mt + 1) / 2 : mt * nt;
+  const int entry = __builtin_popcountll(__ballot(lane < p.count && p.first[lane < MU_PER ? lane : 0] <= wg)) - 1;
+  const MuShape& s = p.s[entry];
+  const int id = xcd_tile_order(s.tiles, (int)(wg - p.first[entry]));
+  const int mp = s.mp, np = s.np, flags = s.flags, count = s.count;
+  const int mt = (mp + T - 1) / T, nt = (np + T - 1) / T, per = SYM ? mt * (mt + 1) / 2 : mt * nt;
   const int mat = id / per, k = id % per;
   int tm, tn;
   if (SYM) {  // the k-th pair tm <= tn
@@ -311,76 +393,46 @@ __global__ __launch_bounds__(64 * WGM * WGN, 1) void muon_gemm_kernel(MuGemm p) 
     tm = k % mt;
     tn = k / mt;
   }
-  const int row0 = tm * BM, n0 = tn * BN;
-  // the x operand is [mp, ldx], the w operand [mp, ldw] (its rows are columns of the product, in UPDATE the contraction)
-  const int ldx = MODE == MU_GRAM ? np : mp, ldw = MODE == MU_POLY ? mp : np, ldo = MODE == MU_UPDATE ? np : mp;
-  const int64_t xs = (int64_t)mp * ldx, ws = (int64_t)mp * ldw, os = (int64_t)mp * ldo;
-  const int K = MODE == MU_GRAM ? np : mp, cols = SYM ? mp : np;
-  const f16* const xb = s.x + mat * xs + (int64_t)row0 * ldx;
-  const f16* const wb = s.w + mat * ws + (WT ? (int64_t)n0 : (int64_t)n0 * ldw);
-  const int nk1 = K / BK, nk = s.flags & MU_THREE ? 3 * nk1 : nk1;
+  const int row0 = tm * T, n0 = tn * T;
+  const int64_t square = (int64_t)mp * mp, wide = (int64_t)mp * np;
+  const int64_t xs = MODE == MU_GRAM ? wide : square, ws = MODE == MU_POLY ? square : wide, os = MODE == MU_UPDATE ? wide : square;
+  const int cols = SYM ? mp : np, nk = (MODE == MU_GRAM ? np : mp) / MU_K;
+  const int panel = mp * MU_K;  // elements of MU_K columns
+  const f16* xp = s.x + mat * xs + row0 * MU_K;
+  const f16* wp = s.w + mat * ws + (WT ? (int64_t)(n0 / MU_K) * panel : n0 * MU_K);
+  const int64_t xlo = count * xs, wlo = count * ws;
 
-  uint32_t xo[LPX], wo[LPW];
+  // A stage is MU_K columns of T rows, 16 rows a copy, or (WT) MU_K rows of T columns, half a panel's a copy.
+  uint32_t xo[LP], wo[LP];
 #pragma unroll
-  for (int j = 0; j < LPX; ++j) {
-    const int row = RPC * (j * NW + wave) + lane / CH;
-    xo[j] = row0 + row < mp ? (uint32_t)row * (uint32_t)ldx * 2u + (((lane % CH) ^ mu_swz(row)) * 16) : OOB;
+  for (int j = 0; j < LP; ++j) {
+    const int u = j * NW + wave, row = 16 * u + lane / 4;
+    const uint32_t chunk = ((lane % 4) ^ mu_swz(row)) * 16;
+    xo[j] = row0 + row < mp ? row * ROWB + chunk : OOB;
+    if (WT) wo[j] = n0 + (u / 2) * MU_K < np ? (uint32_t)(u / 2) * (panel * 2) + (u % 2) * 1024 + lane * 16 : OOB;
+    else wo[j] = n0 + row < mp ? row * ROWB + chunk : OOB;
   }
+  uint32_t to = lds_base + wave * 1024;  // where the next stage goes
+  int staged = 0;
+  // Copies c0 .. c1 of the next stage; past the last one they read nothing and write zeros that nobody reads.
+  auto issue = [&](int c0, int c1) {
 #pragma unroll
-  for (int j = 0; j < LPW; ++j) {
-    if (WT) {
-      const int row = WRPC * (j * NW + wave) + lane / WLPR, chunk = (lane % WLPR) ^ mu_wswz<BN>(row);
-      wo[j] = n0 + 8 * chunk < np ? (uint32_t)row * (uint32_t)ldw * 2u + chunk * 16 : OOB;
-    } else {
-      const int row = RPC * (j * NW + wave) + lane / CH;
-      wo[j] = n0 + row < mp ? (uint32_t)row * (uint32_t)ldw * 2u + (((lane % CH) ^ mu_swz(row)) * 16) : OOB;
+    for (int c = c0; c < c1; ++c) {
+      const int part = c / (2 * LP), j = c % LP, w = c / LP % 2;
+      const f16* const base = (w ? wp : xp) + (part ? w ? wlo : xlo : 0);
+      dma_row16(make_rsrc(base, staged < nk ? OOB : 0), to + w * XB + part * PB + j * NW * 1024, w ? wo[j] : xo[j]);
     }
-  }
-  auto issue = [&](int kt, int slot) {
-    const int seg = kt / nk1, kk = kt - seg * nk1;
-    const u32x4 rx = make_rsrc(xb + (seg == 2 ? s.count * xs : 0) + (int64_t)kk * BK, OOB);
-    const u32x4 rw = make_rsrc(wb + (seg == 1 ? s.count * ws : 0) + (WT ? (int64_t)kk * BK * ldw : (int64_t)kk * BK), OOB);
-    const uint32_t dst = lds_base + slot * STAGE + wave * 1024;
-#pragma unroll
-    for (int j = 0; j < LPX; ++j) dma_row16(rx, dst + j * NW * 1024, xo[j]);
-#pragma unroll
-    for (int j = 0; j < LPW; ++j) dma_row16(rw, dst + XB + j * NW * 1024, wo[j]);
+    if (c1 == COPIES) {
+      xp += panel;
+      wp += WT ? MU_K * MU_K : panel;
+      ++staged;
+      to = to == lds_base + wave * 1024 + (NST - 1) * STAGE ? lds_base + wave * 1024 : to + STAGE;
+    }
   };
+#pragma unroll
+  for (int q = 0; q < NST - 1; ++q) issue(0, COPIES);
 
-  // LDS offsets of the fragments; K sub-steps 2, 3 of K-contiguous rows are at offset ^ 64
-  uint32_t aoff[FN][WT ? 1 : 2], boff[FM][2];
-#pragma unroll
-  for (int i = 0; i < FN; ++i) {
-    if (WT) {
-      const int r4 = (lane & 15) >> 2, c = (wn * WTN + 32 * i) / 8 + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-      aoff[i][0] = XB + (8 * hi + r4) * (BN * 2) + ((c ^ mu_wswz<BN>(r4)) << 4) + 8 * (lane & 1);
-    } else {
-      const int row = wn * WTN + 32 * i + l32;
-      for (int kk = 0; kk < 2; ++kk) aoff[i][WT ? 0 : kk] = XB + row * ROWB + ((2 * kk + hi) ^ mu_swz(row)) * 16;
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < FM; ++j) {
-    const int row = wm * WTM + 32 * j + l32;
-    for (int kk = 0; kk < 2; ++kk) boff[j][kk] = row * ROWB + ((2 * kk + hi) ^ mu_swz(row)) * 16;
-  }
-  auto load_frags = [&](const char* st, int kk, f16x8 (&a)[FN], f16x8 (&b)[FM]) {
-#pragma unroll
-    for (int i = 0; i < FN; ++i) {
-      if constexpr (WT) {
-        const char* q = st + aoff[i][0] + kk * 16 * (BN * 2);
-        typedef __fp16 h16x4 __attribute__((ext_vector_type(4)));
-        const f16x4 lo = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16(LDS_PTR(h16x4, q)));
-        const f16x4 up = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16(LDS_PTR(h16x4, q + 4 * (BN * 2))));
-        a[i] = __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7);
-      } else {
-        a[i] = *(const f16x8*)(st + (aoff[i][kk & 1] ^ ((kk >> 1) * 64)));
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < FM; ++j) b[j] = *(const f16x8*)(st + (boff[j][kk & 1] ^ ((kk >> 1) * 64)));
-  };
-
+  const int gn0 = n0 + wn * WTN, gr0 = row0 + wm * WTM;
   f32x16 acc[FN][FM];
 #pragma unroll
   for (int i = 0; i < FN; ++i)
@@ -388,92 +440,140 @@ __global__ __launch_bounds__(64 * WGM * WGN, 1) void muon_gemm_kernel(MuGemm p) 
     for (int j = 0; j < FM; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+
+  // LDS offsets of the fragments
+  uint32_t aoff[FN][WT ? 1 : KS], boff[FM][KS];
 #pragma unroll
-  for (int q = 0; q < NST - 1; ++q)
-    if (q < nk) issue(q, q);
-  int rd = 0;
-  for (int kt = 0; kt < nk; ++kt) {
-    if (NST > 2 && kt + NST - 2 < nk) wait_vmcnt((NST - 2) * (LPX + LPW));
-    else wait_vmcnt(0);
-    lds_barrier();  // landed for every wave, and the slot read last step is free
-    if (kt + NST - 1 < nk) issue(kt + NST - 1, rd == 0 ? NST - 1 : rd - 1);
-    const char* st = lds + rd * STAGE;
-    rd = rd + 1 == NST ? 0 : rd + 1;
-    f16x8 af[2][FN], bfr[2][FM];
-    load_frags(st, 0, af[0], bfr[0]);
-#pragma unroll
-    for (int kk = 0; kk < BK / 16; ++kk) {
-      const int cb = kk & 1;
-      if (kk + 1 < BK / 16) load_frags(st, kk + 1, af[cb ^ 1], bfr[cb ^ 1]);
-#pragma unroll
-      for (int i = 0; i < FN; ++i)
-#pragma unroll
-        for (int j = 0; j < FM; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[cb][i], bfr[cb][j], acc[i][j], 0, 0, 0);
+  for (int i = 0; i < FN; ++i) {
+    if (WT) {
+      const int r4 = (lane & 15) >> 2, c = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+      aoff[i][0] = XB + ((wn * WTN + 32 * i) / MU_K) * (MU_K * ROWB) + (8 * hi + r4) * ROWB + c * 16 + 8 * (lane & 1);
+    } else {
+      const int row = wn * WTN + 32 * i + l32;
+      for (int kk = 0; kk < KS; ++kk) aoff[i][WT ? 0 : kk] = XB + row * ROWB + ((2 * kk + hi) ^ mu_swz(row)) * 16;
     }
   }
-
-  // ---- epilogue: 32 rows of the wave's tile at a time through its slab of the ring in fp32, back as eight columns a lane
-  lds_barrier();  // every wave is done reading the last stage
-  constexpr int NCH = WTN / 4, LPR = WTN / 8, RPI = 64 / LPR, NIT = 32 / RPI;
-  char* slab = lds + wave * SLAB;
-  const int lrow = lane / LPR, lc = lane % LPR, gn = n0 + wn * WTN + 8 * lc;
-  const bool mirror = SYM && tm != tn;
-  f16* const out = s.out + mat * os;
-  const int64_t olo = s.count * os;  // from a value's first fp16 to its second
-  const f16* const d = s.d + mat * os;
-  auto place = [&](int row, int chunk) { return slab + row * (WTN * 4) + ((chunk ^ (row & (NCH - 1))) << 4); };
-  auto split = [&](const float (&v)[8], f16x8& h, f16x8& l) {
-#pragma unroll
-    for (int x = 0; x < 8; ++x) {
-      h[x] = (f16)v[x];
-      l[x] = (f16)(v[x] - (float)h[x]);
-    }
-  };
 #pragma unroll
   for (int j = 0; j < FM; ++j) {
+    const int row = wm * WTM + 32 * j + l32;
+    for (int kk = 0; kk < KS; ++kk) boff[j][kk] = row * ROWB + ((2 * kk + hi) ^ mu_swz(row)) * 16;
+  }
+  auto load_frags = [&](const char* st, int kk, f16x8 (&a)[PARTS][FN], f16x8 (&b)[PARTS][FM]) {
 #pragma unroll
-    for (int i = 0; i < FN; ++i)
+    for (int part = 0; part < PARTS; ++part) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *(f32x4*)place(l32, 8 * i + 2 * q + hi) = (f32x4){acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-#pragma unroll
-    for (int it = 0; it < NIT; ++it) {
-      const int sl = RPI * it + lrow, r = row0 + wm * WTM + 32 * j + sl;
-      const bool in = r < mp && gn < cols;
-      const f32x4 z0 = *(const f32x4*)place(sl, 2 * lc), z1 = *(const f32x4*)place(sl, 2 * lc + 1);
-      float v[8] = {z0[0], z0[1], z0[2], z0[3], z1[0], z1[1], z1[2], z1[3]};
-      const int64_t at = (int64_t)r * ldo + gn;
-      f16x8 h = {}, l = {};
-      if (MODE != MU_GRAM && in) {
-        h = *(const f16x8*)(d + at);
-        if (s.flags & MU_LO_IN) l = *(const f16x8*)(d + olo + at);
-      }
-#pragma unroll
-      for (int x = 0; x < 8; ++x) v[x] = MODE == MU_GRAM ? v[x] * p.alpha : fmaf(v[x], p.alpha, p.beta * ((float)h[x] + (float)l[x]));
-      split(v, h, l);
-      if (in) {
-        *(f16x8*)(out + at) = h;
-        if (s.flags & MU_LO_OUT) *(f16x8*)(out + olo + at) = l;
-      }
-      if (mirror) {
-        *(f32x4*)place(sl, 2 * lc) = (f32x4){v[0], v[1], v[2], v[3]};
-        *(f32x4*)place(sl, 2 * lc + 1) = (f32x4){v[4], v[5], v[6], v[7]};
-      }
-    }
-    if (mirror) {  // four lanes a column, eight rows each
-#pragma unroll
-      for (int it = 0; it < WTN / 16; ++it) {
-        const int c = 16 * it + (lane >> 2), r8 = (lane & 3) * 8;
-        float v[8];
-#pragma unroll
-        for (int x = 0; x < 8; ++x) v[x] = *(const float*)(place(r8 + x, c >> 2) + 4 * (c & 3));
-        f16x8 h, l;
-        split(v, h, l);
-        const int r = row0 + wm * WTM + 32 * j + r8, g = n0 + wn * WTN + c;
-        if (r < mp && g < mp) {
-          *(f16x8*)(out + (int64_t)g * ldo + r) = h;
-          if (s.flags & MU_LO_OUT) *(f16x8*)(out + olo + (int64_t)g * ldo + r) = l;
+      for (int i = 0; i < FN; ++i) {
+        if constexpr (WT) {
+          const char* q = st + aoff[i][0] + part * PB + kk * 16 * ROWB;
+          typedef __fp16 h16x4 __attribute__((ext_vector_type(4)));
+          const f16x4 lo = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16(LDS_PTR(h16x4, q)));
+          const f16x4 up = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16(LDS_PTR(h16x4, q + 4 * ROWB)));
+          a[part][i] = __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7);
+        } else {
+          a[part][i] = *(const f16x8*)(st + part * PB + aoff[i][kk]);
         }
+      }
+#pragma unroll
+      for (int j = 0; j < FM; ++j) b[part][j] = *(const f16x8*)(st + part * PB + boff[j][kk]);
+    }
+  };
+
+  constexpr int PRODUCTS = PARTS == 2 ? 3 : 1, GROUPS = KS * PRODUCTS * FN;
+  f16x8 af[2][PARTS][FN], bf[2][PARTS][FM];
+  mu_wait<(NST - 2) * COPIES>();
+  lds_barrier();
+  load_frags(lds, 0, af[0], bf[0]);
+  const char* st = lds;
+  for (int kt = 0; kt < nk; ++kt) {
+    mu_wait<(NST - 3) * COPIES>();
+    wait_lgkm0();  // this stage's first fragments, read among the products before: the slot of kt - 1 is read, no later wait counts them
+    lds_barrier();     // stage kt + 1 landed for every wave, and the slot of kt - 1 is free
+    const char* const next = st == lds + (NST - 1) * STAGE ? lds : st + STAGE;
+#pragma unroll
+    for (int kk = 0; kk < KS; ++kk) {
+      const int cb = kk & 1;
+      if (kk + 1 < KS) load_frags(st, kk + 1, af[cb ^ 1], bf[cb ^ 1]);
+      else load_frags(next, 0, af[cb ^ 1], bf[cb ^ 1]);  // after the last stage: read for nothing
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int pr = 0; pr < PRODUCTS; ++pr)
+#pragma unroll
+        for (int i = 0; i < FN; ++i) {
+#pragma unroll
+          for (int j = 0; j < FM; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[cb][PARTS == 2 && pr == 1][i], bf[cb][PARTS == 2 && pr == 2][j], acc[i][j], 0, 0, 0);
+          // the copies between the products: issued at once they would hold up the products behind them
+          const int g = (kk * PRODUCTS + pr) * FN + i;
+          __builtin_amdgcn_sched_barrier(0);
+          issue(COPIES * g / GROUPS, COPIES * (g + 1) / GROUPS);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    st = next;
+  }
+  wait_vmcnt(0);
+  // ---- epilogue, 32 x 32 at a time in registers
+  const bool mirror = SYM && tm != tn;
+  f16* const __restrict__ out = s.out + mat * os;
+  const int64_t olo = count * os;  // from a value's first fp16 to its second
+  const f16* const __restrict__ d = s.d + mat * os;
+  auto element = [&](int row, int col) { return (int64_t)(col / MU_K) * panel + row * MU_K + col % MU_K; };
+#pragma unroll
+  for (int i = 0; i < FN; ++i) {
+    const int c0 = gn0 + 32 * i;
+    if (c0 >= cols) continue;  // cols is a multiple of 64
+    u32x4 dh[FM][2], dl[FM][2];  // what the columns are added to: all their loads before their stores
+    if (MODE != MU_GRAM) {
+#pragma unroll
+      for (int j = 0; j < FM; ++j)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int64_t at = gr0 + 32 * j < mp ? element(gr0 + 32 * j + 16 * t + (lane & 15), c0 + mu_chunk(lane)) : 0;
+          dh[j][t] = *(const u32x4*)(d + at);
+          dl[j][t] = flags & MU_LO_IN ? *(const u32x4*)(d + olo + at) : (u32x4){};
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+      if (gr0 + 32 * j >= mp) continue;
+      float v[16];
+      if (MODE != MU_GRAM) {
+        mu_unrows(dh[j]);
+        if (flags & MU_LO_IN) mu_unrows(dl[j]);
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const f16x8 h = __builtin_bit_cast(f16x8, dh[j][t]), l = __builtin_bit_cast(f16x8, dl[j][t]);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const float a = acc[i][j][8 * t + x];
+          v[8 * t + x] = MODE == MU_GRAM ? a * p.alpha : fmaf(a, p.alpha, p.beta * ((float)h[x] + (float)l[x]));
+        }
+      }
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+        if (part && !(flags & MU_LO_OUT)) break;
+        f16* const o = out + part * olo;
+        u32x4 w[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          f16x8 h;
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            h[x] = (f16)v[8 * t + x];
+            v[8 * t + x] -= (float)h[x];
+          }
+          w[t] = __builtin_bit_cast(u32x4, h);
+          if (mirror) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+              *(u32x2*)(o + element(c0 + 16 * t + 8 * q + 4 * hi + (lane & 3), gr0 + 32 * j + (l32 & 28))) =
+                  mu_quads((u32x2){w[t][2 * q], w[t][2 * q + 1]}, lane);
+          }
+        }
+        mu_rows(w);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) *(u32x4*)(o + element(gr0 + 32 * j + 16 * t + (lane & 15), c0 + mu_chunk(lane))) = w[t];
       }
     }
   }
@@ -584,39 +684,85 @@ static int mu_check(const std::string& n, const strata_hip_muon_args* a, bool st
   return check_ranges(n, written, read);
 }
 
-// One product of every group, the longest first: `fill` sets the operands of a shape.
-template <int MODE, typename F>
-static int mu_products(const MuPlan& q, MuGemm& b, hipStream_t st, F fill) {
-  constexpr int T = 128;
+// Tiles of T x T a product of a group takes.
+static int64_t mu_tiles(const MuGroup& g, int T, int mode) {
+  const int64_t mt = (g.mp + T - 1) / T, nt = (g.np + T - 1) / T;
+  return g.count * (mode == MU_UPDATE ? mt * nt : mt * (mt + 1) / 2);  // at most 2^22 (mu_sizes)
+}
+static int64_t mu_length(const MuGroup& g, int mode) { return (mode == MU_GRAM ? g.np : g.mp) / MU_K; }
+
+// The tile of a launch, by an estimate of its cycles: rounds of the 256 CUs, each of the tiles' stages at what one costs with so
+// many tiles on a CU, and what a tile costs besides; at least the longest tile alone.  Measured in cycles a stage, one
+// tile alone on a CU and as many as fit: 64 x 64 240 and 480 (3), 128 x 128 530 and 850 (2), 256 x 256 1300; of two fp16
+// 64 x 64 400 and 670 (2), 128 x 128 1150; besides them 5000, 11000, 17000 (7000, 12000).  What it decides: 960 x 3840 alone, X X^T
+// 16 us on 64 x 64, 32 on 128 x 128, 73 on 256 x 256; 72 matrices of 512 columns 53, 41, 50; 48 of 960 P X 485, 395, 336.
+static int mu_tile_size(const std::vector<const MuGroup*>& groups, int mode, bool precise) {
+  struct Cost {
+    int tile, fit;
+    double alone, more, fixed;  // a stage: alone + more for each other tile on the CU
+  };
+  static constexpr Cost plain[3] = {{64, 3, 240., 120., 5e3}, {128, 2, 530., 320., 11e3}, {256, 1, 1300., 0., 17e3}};
+  static constexpr Cost two[2] = {{64, 2, 400., 270., 7e3}, {128, 1, 1150., 0., 12e3}};
+  int best = 0;
+  double least = 0.;
+  for (int i = 0; i < (precise ? 2 : 3); ++i) {
+    const Cost& c = precise ? two[i] : plain[i];
+    double tiles = 0., stages = 0., longest = 0.;
+    for (const MuGroup* g : groups) {
+      const double n = (double)mu_tiles(*g, c.tile, mode), k = (double)mu_length(*g, mode);
+      tiles += n;
+      stages += n * k;
+      longest = std::max(longest, k);
+    }
+    const double mean = stages / tiles, round = 256. * c.fit, full = std::floor(tiles / round), rest = std::ceil((tiles - full * round) / 256.);
+    auto of = [&](double on, double k) { return k * (c.alone + c.more * (on - 1.)) + c.fixed; };
+    const double t = std::max(full * of(c.fit, mean) + (rest > 0. ? of(rest, mean) : 0.), of(1., longest));
+    if (!best || t < least) best = c.tile, least = t;
+  }
+  return best;
+}
+
+// One product of every group of one precision, the longest first: `fill` sets the operands of a shape.
+template <int MODE, int PARTS, typename F>
+static int mu_products_of(const MuPlan& q, MuGemm& b, hipStream_t st, F fill) {
   std::vector<const MuGroup*> order;
-  for (const MuGroup& g : q.groups) order.push_back(&g);
-  auto length = [](const MuGroup* g) { return (MODE == MU_GRAM ? g->np : g->mp) * (g->precise ? 3 : 1); };
-  std::stable_sort(order.begin(), order.end(), [&](const MuGroup* x, const MuGroup* y) { return length(x) > length(y); });
+  for (const MuGroup& g : q.groups)
+    if (g.precise == (PARTS == 2)) order.push_back(&g);
+  if (order.empty()) return STRATA_HIP_OK;
+  std::stable_sort(order.begin(), order.end(), [](const MuGroup* x, const MuGroup* y) { return mu_length(*x, MODE) > mu_length(*y, MODE); });
+  const int T = mu_tile_size(order, MODE, PARTS == 2);
   b.count = 0;
   uint32_t tiles = 0;
   auto flush = [&]() -> int {
     if (!b.count) return STRATA_HIP_OK;
-    hipLaunchKernelGGL((muon_gemm_kernel<T, T, 4, 2, 2, MODE>), dim3(tiles), dim3(512), 0, st, b);
+    if (T == 64) hipLaunchKernelGGL((muon_gemm_kernel<64, 2, 2, PARTS == 2 ? 4 : 6, PARTS, MODE>), dim3(tiles), dim3(256), 0, st, b);
+    else if (T == 128) hipLaunchKernelGGL((muon_gemm_kernel<128, 2, 2, PARTS == 2 ? 5 : 4, PARTS, MODE>), dim3(tiles), dim3(256), 0, st, b);
+    else if constexpr (PARTS == 1) hipLaunchKernelGGL((muon_gemm_kernel<256, 2, 4, 4, 1, MODE>), dim3(tiles), dim3(512), 0, st, b);
     b.count = 0;
     tiles = 0;
     return check_launch("muon products");
   };
   for (const MuGroup* g : order) {
-    const int64_t mt = (g->mp + T - 1) / T, nt = (g->np + T - 1) / T;
-    const int64_t n = g->count * (MODE == MU_UPDATE ? mt * nt : mt * (mt + 1) / 2);  // at most 2^22 (mu_sizes)
+    const int64_t n = mu_tiles(*g, T, MODE);
     if (b.count == MU_PER || tiles + n > (1 << 22))
       if (const int rc = flush()) return rc;
+    b.first[b.count] = tiles;
     MuShape& s = b.s[b.count++];
     s.mp = (int)g->mp;
     s.np = (int)g->np;
     s.count = (int)g->count;
     s.tiles = (int)n;
-    s.first = tiles;
-    s.flags = g->precise ? MU_THREE | MU_LO_IN | MU_LO_OUT : 0;
+    s.flags = PARTS == 2 ? MU_LO_IN | MU_LO_OUT : 0;
     fill(*g, s);
     tiles += (uint32_t)n;
   }
   return flush();
+}
+
+template <int MODE, typename F>
+static int mu_products(const MuPlan& q, MuGemm& b, hipStream_t st, F fill) {
+  const int rc = mu_products_of<MODE, 1>(q, b, st, fill);
+  return rc ? rc : mu_products_of<MODE, 2>(q, b, st, fill);
 }
 
 static int mu_launch(const std::string& name, const strata_hip_muon_args* a, bool step, hipStream_t st) {
@@ -666,7 +812,7 @@ static int mu_launch(const std::string& name, const strata_hip_muon_args* a, boo
       const uintptr_t at = (uintptr_t)t.grad | (uintptr_t)t.momentum | (uintptr_t)t.param | (uintptr_t)t.master;
       o.flags = (t.param_dtype == STRATA_HIP_F32 ? MU_P32 : 0) | (t.grad_dtype == STRATA_HIP_F32 ? MU_G32 : 0) |
                 (t.rows > t.cols ? MU_TALL : 0) | ((at & 15) || t.cols % 4 ? 0 : MU_ALIGNED) | (a->nesterov ? MU_NESTEROV : 0) |
-                (step ? MU_STEP : 0);
+                (step ? MU_STEP : 0) | (g.precise ? MU_LO : 0);
       const double adjust = a->adjust == STRATA_HIP_ADJUST_MATCH_RMS_ADAMW ? 0.2 * std::sqrt((double)std::max(t.rows, t.cols))
                                                                            : std::sqrt(std::max(1., (double)t.rows / (double)t.cols));
       o.rate = (float)(t.lr * adjust);
@@ -697,8 +843,7 @@ static int mu_launch(const std::string& name, const strata_hip_muon_args* a, boo
       return rc;
     b.alpha = 1.f / MU_A;
     b.beta = (float)c[0];
-    // X's second fp16: into all steps but the last two, and the last one's result, which the weights take
-    const int lo = (k < a->steps - 2 ? MU_LO_IN : 0) | (k + 1 < a->steps - 2 || k + 1 == a->steps ? MU_LO_OUT : 0);
+    const int lo = (k < MU_LO_STEPS ? MU_LO_IN : 0) | (k + 1 < MU_LO_STEPS ? MU_LO_OUT : 0);
     if (const int rc = mu_products<MU_UPDATE>(q, b, st, [&](const MuGroup& g, MuShape& s) {
           s.flags |= lo;
           s.x = halves + g.p;
