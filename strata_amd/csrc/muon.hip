@@ -77,6 +77,13 @@ __device__ __forceinline__ int mu_entry(int count, uint32_t wg, F first) {
   return lo;
 }
 
+// v, rounded to fp32.  Some variants of a kernel would otherwise round a multiply-add straight to fp16 (v_fma_mixlo_f16) or
+// merge it with the subtraction of its first fp16: a matrix's result would depend on the tile that the others call for.
+__device__ __forceinline__ float mu_rounded(float v) {
+  asm("" : "+v"(v));
+  return v;
+}
+
 __device__ __forceinline__ float mu_load(const void* p, int64_t i, bool wide) {
   return wide ? ((const float*)p)[i] : (float)((const bf16*)p)[i];
 }
@@ -377,9 +384,11 @@ __global__ __launch_bounds__(64 * WGM * WGN, 1) void muon_gemm_kernel(MuGemm p) 
 
   // Each shape's tiles are dealt to the XCDs in blocks: one matrix's on one XCD, every XCD with its share of every shape.
   const uint32_t wg = (uint32_t)__builtin_amdgcn_workgroup_id_x();
+  MuShape s = p.s[0];  // loaded while the entries are looked over
+  uint32_t first = 0;
   const int entry = __builtin_popcountll(__ballot(lane < p.count && p.first[lane < MU_PER ? lane : 0] <= wg)) - 1;
-  const MuShape& s = p.s[entry];
-  const int id = xcd_tile_order(s.tiles, (int)(wg - p.first[entry]));
+  if (entry) s = p.s[entry], first = p.first[entry];
+  const int id = xcd_tile_order(s.tiles, (int)(wg - first));
   const int mp = s.mp, np = s.np, flags = s.flags, count = s.count;
   const int mt = (mp + T - 1) / T, nt = (np + T - 1) / T, per = SYM ? mt * (mt + 1) / 2 : mt * nt;
   const int mat = id / per, k = id % per;
@@ -547,7 +556,7 @@ __global__ __launch_bounds__(64 * WGM * WGN, 1) void muon_gemm_kernel(MuGemm p) 
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
           const float a = acc[i][j][8 * t + x];
-          v[8 * t + x] = MODE == MU_GRAM ? a * p.alpha : fmaf(a, p.alpha, p.beta * ((float)h[x] + (float)l[x]));
+          v[8 * t + x] = mu_rounded(MODE == MU_GRAM ? a * p.alpha : fmaf(a, p.alpha, p.beta * ((float)h[x] + (float)l[x])));
         }
       }
 #pragma unroll
@@ -561,7 +570,7 @@ __global__ __launch_bounds__(64 * WGM * WGN, 1) void muon_gemm_kernel(MuGemm p) 
 #pragma unroll
           for (int x = 0; x < 8; ++x) {
             h[x] = (f16)v[8 * t + x];
-            v[8 * t + x] -= (float)h[x];
+            v[8 * t + x] = v[8 * t + x] - (float)h[x];
           }
           w[t] = __builtin_bit_cast(u32x4, h);
           if (mirror) {
@@ -580,6 +589,299 @@ __global__ __launch_bounds__(64 * WGM * WGN, 1) void muon_gemm_kernel(MuGemm p) 
 #endif
 }
 
+// ---- small matrices: the whole step in one workgroup and launch ----
+// X (as two fp16) and A, which P takes the place of, stay in LDS, in the workspace's layout; u in registers until its norm
+// is known.  Eight waves share the 32 x 32 blocks of a product: of 128 x 128 two each, of 64 x 64 half of the contraction
+// each.  Bound by latencies and the conversions of the results: 128 x 128 alone 32 us, 9200 cycles a step
+// (in eighteen launches 77), 21600 to bring u into LDS.
+constexpr int MU_SMALL_PER = 32;  // tensors a launch
+struct MuSmall {
+  MuTensor t[MU_SMALL_PER];
+  float co[64][3];
+  int count, steps;
+  float mu, omu;
+  double eps;
+};
+static_assert(sizeof(MuSmall) <= 4096, "kernel arguments");
+
+// MP x n matrices, n <= NP: the shorter side rounded up to MP, the longer one to 64.
+template <int MP, int NP, int PARTS>
+__global__ __launch_bounds__(512, 1) void muon_small_kernel(MuSmall b) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  constexpr int XB = MP * NP * 2, AB = MP * MP * 2;  // bytes of one fp16 of X, of A
+  constexpr int HALVES = MP == 64 ? 2 : 1;           // of a contraction, to a wave each
+  constexpr int GB = MP == 64 ? 1 : 2, UB = MP * NP / 1024 / 8;  // blocks a wave of A and P, and of X
+  constexpr int EPT = MP * NP / 512 / 4;             // runs of four elements a thread
+  __shared__ __attribute__((aligned(1024))) char lds[2 * XB + PARTS * AB + (HALVES == 2 ? MP * MP * 4 : 0)];
+  __shared__ double red[8];
+  char* const xl = lds;
+  char* const al = lds + 2 * XB;
+  float* const shares = (float*)(al + PARTS * AB);
+
+  const uint32_t wg = blockIdx.x;
+  const MuTensor& t = b.t[mu_entry(b.count, wg, [&](int i) { return b.t[i].first; })];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, hi = lane >> 5;
+  const int rows = (int)t.rows, cols = (int)t.cols, n = rows * cols;
+  const bool tall = t.flags & MU_TALL, g32 = t.flags & MU_G32, p32 = t.flags & MU_P32, nesterov = t.flags & MU_NESTEROV;
+  const bool aligned = t.flags & MU_ALIGNED, step = t.flags & MU_STEP, runs = cols % 4 == 0;
+  const int np = ((tall ? rows : cols) + 63) / 64 * 64;
+  const int64_t base = (int64_t)(wg - t.first) * n;
+
+  // Element (row, col) of a matrix of MP rows in panels of 32 columns, 16-byte chunks swizzled.
+  auto place = [](int row, int col) { return (col / MU_K) * (MP * MU_K * 2) + row * (MU_K * 2) + (((col % MU_K) / 8) ^ mu_swz(row)) * 16 + (col % 8) * 2; };
+
+  for (int i = tid; i < 2 * XB / 16; i += 512) *(u32x4*)(xl + 16 * i) = (u32x4){};
+  // u, and m <- mu m + (1 - mu) g
+  float u[EPT][4];
+  double s = 0.;
+#pragma unroll
+  for (int k = 0; k < EPT; ++k) {
+    const int e0 = 4 * (tid + 512 * k);
+    float g[4] = {0.f, 0.f, 0.f, 0.f}, m[4] = {0.f, 0.f, 0.f, 0.f};
+    const bool whole = aligned && e0 < n;  // n is a multiple of 4 then
+    if (whole) {
+      const f32x4 v = mu_load4(t.g, base + e0, g32);
+      const f32x4 w = t.m ? *(const f32x4*)(t.m + base + e0) : (f32x4){};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) g[e] = v[e], m[e] = w[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e0 + e < n) {
+          g[e] = mu_load(t.g, base + e0 + e, g32);
+          if (t.m) m[e] = t.m[base + e0 + e];
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      m[e] = fmaf(b.mu, m[e], b.omu * g[e]);
+      u[k][e] = !t.m ? g[e] : nesterov ? fmaf(b.mu, m[e], b.omu * g[e]) : m[e];
+      s = fma((double)u[k][e], (double)u[k][e], s);
+    }
+    if (!t.m) continue;
+    if (whole) *(f32x4*)(t.m + base + e0) = (f32x4){m[0], m[1], m[2], m[3]};
+    else
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e0 + e < n) t.m[base + e0 + e] = m[e];
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
+  if (lane == 0) red[wave] = s;
+  __syncthreads();
+  s = 0.;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) s += red[w];
+  const double norm = sqrt(s), scale = norm == 0. ? 0. : MU_X / (norm < b.eps ? b.eps : norm);
+  // Runs of four elements lie in one row where cols is a multiple of 4, of X or (tall) of four rows of one swizzle.
+#pragma unroll
+  for (int k = 0; k < EPT; ++k) {
+    const int e0 = 4 * (tid + 512 * k);
+    if (e0 >= n) continue;
+    int row = e0 / cols, col = e0 - row * cols;
+    f16x4 h, l;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float v = (float)((double)u[k][e] * scale);
+      h[e] = (f16)v;
+      l[e] = (f16)(v - (float)h[e]);
+    }
+    if (runs && !tall) {
+      const int at = place(row, col);
+      *(f16x4*)(xl + at) = h;
+      *(f16x4*)(xl + XB + at) = l;
+    } else {
+      int at = tall ? place(col, row) : place(row, col);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (e0 + e >= n) break;
+        *(f16*)(xl + at) = h[e];
+        *(f16*)(xl + XB + at) = l[e];
+        if (runs) {
+          at += MU_K * 2;
+        } else {
+          if (++col == cols) col = 0, ++row;
+          at = tall ? place(col, row) : place(row, col);
+        }
+      }
+    }
+  }
+  __syncthreads();
+
+  typedef __fp16 h16x4 __attribute__((ext_vector_type(4)));
+  auto frag = [&](const char* m, int row, int k0) { return *(const f16x8*)(m + place(row, k0 + 8 * hi)); };  // 16 columns from k0 on
+  auto frag_t = [&](const char* m, int k0, int c0) {  // rows k0 .. + 15 of columns c0 .. + 31, transposed
+    const int row = k0 + 8 * hi + ((lane & 15) >> 2), col = c0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    const f16x4 lo = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16(LDS_PTR(h16x4, m + place(row, col))));
+    const f16x4 up = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16(LDS_PTR(h16x4, m + place(row + 4, col))));
+    return __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  auto multiply = [&](f32x16& acc, const f16x8 (&a)[PARTS], const f16x8 (&c)[PARTS]) {
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], c[0], acc, 0, 0, 0);
+    if constexpr (PARTS == 2) {
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1], c[0], acc, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], c[1], acc, 0, 0, 0);
+    }
+  };
+  // Blocks of m m^T, m [MP, K] at stride `part` between its two fp16: of a wave, with its share of the contraction.
+  auto square = [&](f32x16 (&acc)[GB], const char* m, int part, int K) {
+    const int half = HALVES == 2 ? wave / 4 : 0, block = HALVES == 2 ? wave % 4 : wave * GB;
+    const int r0 = block / (MP / 32) * 32, k0 = half * (K / HALVES), k1 = k0 + K / HALVES;
+#pragma unroll
+    for (int i = 0; i < GB; ++i) acc[i] = (f32x16){};
+#pragma unroll 2
+    for (int k = k0; k < k1; k += 32) {  // K is a multiple of 64
+      f16x8 x[2][PARTS], w[2][GB][PARTS];
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int q = 0; q < PARTS; ++q) {
+          x[kk][q] = frag(m + q * part, r0 + l32, k + 16 * kk);
+#pragma unroll
+          for (int i = 0; i < GB; ++i) w[kk][i][q] = frag(m + q * part, (block + i) % (MP / 32) * 32 + l32, k + 16 * kk);
+        }
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int i = 0; i < GB; ++i) multiply(acc[i], w[kk][i], x[kk]);
+    }
+    if constexpr (HALVES == 2) {  // the upper waves' shares are added to the lower ones'
+      if (half)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) *(f32x4*)(shares + ((block * 4 + r) * 64 + lane) * 4) = (f32x4){acc[0][4 * r], acc[0][4 * r + 1], acc[0][4 * r + 2], acc[0][4 * r + 3]};
+      __syncthreads();
+      if (!half)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[0][r] += shares[((block * 4 + r / 4) * 64 + lane) * 4 + r % 4];
+    }
+  };
+  // alpha acc + beta d at block (r0, c0) of a matrix, four columns at once, written over d once every wave has read.
+  auto combine = [&](f32x16& acc, const char* d, int part, bool two, int r0, int c0, float alpha, float beta) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int at = place(r0 + l32, c0 + 8 * q + 4 * hi);
+      f16x4 h = {}, l = {};
+      if (d) h = *(const f16x4*)(d + at);
+      if (d && two) l = *(const f16x4*)(d + part + at);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) acc[4 * q + x] = fmaf(acc[4 * q + x], alpha, beta * ((float)h[x] + (float)l[x]));
+    }
+  };
+  auto write = [&](const f32x16& acc, char* o, int part, bool two, int r0, int c0) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int at = place(r0 + l32, c0 + 8 * q + 4 * hi);
+      f16x4 h, l;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        h[x] = (f16)acc[4 * q + x];
+        l[x] = (f16)(acc[4 * q + x] - (float)h[x]);
+      }
+      *(f16x4*)(o + at) = h;
+      if (two) *(f16x4*)(o + part + at) = l;
+    }
+  };
+  const int block = HALVES == 2 ? wave % 4 : wave * GB, r0 = block / (MP / 32) * 32;
+  const bool mine = HALVES == 1 || wave < 4;  // holds blocks of A and P
+  for (int k = 0; k < b.steps; ++k) {
+    f32x16 acc[GB];
+    square(acc, xl, XB, np);
+    if (mine)
+#pragma unroll
+      for (int i = 0; i < GB; ++i) {
+        combine(acc[i], nullptr, 0, false, 0, 0, MU_A / (MU_X * MU_X), 0.f);
+        write(acc[i], al, AB, PARTS == 2, r0, (block + i) % (MP / 32) * 32);
+      }
+    __syncthreads();
+    square(acc, al, AB, MP);
+    if (mine)
+#pragma unroll
+      for (int i = 0; i < GB; ++i) combine(acc[i], al, AB, PARTS == 2, r0, (block + i) % (MP / 32) * 32, b.co[k][2] / MU_A, b.co[k][1]);
+    __syncthreads();
+    if (mine)
+#pragma unroll
+      for (int i = 0; i < GB; ++i) write(acc[i], al, AB, PARTS == 2, r0, (block + i) % (MP / 32) * 32);
+    __syncthreads();
+    f32x16 x[UB];
+#pragma unroll
+    for (int i = 0; i < UB; ++i) {
+      const int blk = wave + 8 * i, rr = blk % (MP / 32) * 32, cc = blk / (MP / 32) * 32;
+      if (cc >= np) continue;
+      x[i] = (f32x16){};
+#pragma unroll
+      for (int kk = 0; kk < MP; kk += 16) {
+        f16x8 w[PARTS], p[PARTS];
+#pragma unroll
+        for (int q = 0; q < PARTS; ++q) {
+          w[q] = frag_t(xl + q * XB, kk, cc);
+          p[q] = frag(al + q * AB, rr + l32, kk);
+        }
+        multiply(x[i], w, p);
+      }
+      combine(x[i], xl, XB, PARTS == 2 || k < MU_LO_STEPS, rr, cc, 1.f / MU_A, b.co[k][0]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < UB; ++i) {
+      const int blk = wave + 8 * i, rr = blk % (MP / 32) * 32, cc = blk / (MP / 32) * 32;
+      if (cc < np) write(x[i], xl, XB, PARTS == 2 || k + 1 < MU_LO_STEPS, rr, cc);
+    }
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int k = 0; k < EPT; ++k) {
+    const int e0 = 4 * (tid + 512 * k);
+    if (e0 >= n) continue;
+    int row = e0 / cols, col = e0 - row * cols;
+    float v[4];
+    const bool whole = aligned;
+    f32x4 p = {};
+    if (step && whole) p = t.master ? *(const f32x4*)(t.master + base + e0) : mu_load4(t.p, base + e0, p32);
+    f16x4 h = {}, l = {};
+    if (runs && !tall) {
+      const int at = place(row, col);
+      h = *(const f16x4*)(xl + at);
+      if (PARTS == 2) l = *(const f16x4*)(xl + XB + at);
+    } else {
+      int at = tall ? place(col, row) : place(row, col);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (e0 + e >= n) break;
+        h[e] = *(const f16*)(xl + at);
+        if (PARTS == 2) l[e] = *(const f16*)(xl + XB + at);
+        if (runs) {
+          at += MU_K * 2;
+        } else {
+          if (++col == cols) col = 0, ++row;
+          at = tall ? place(col, row) : place(row, col);
+        }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[e] = ((float)h[e] + (float)l[e]) * (1.f / MU_X);
+      if (!step) continue;
+      if (!whole && e0 + e < n) p[e] = t.master ? t.master[base + e0 + e] : mu_load(t.p, base + e0 + e, p32);
+      v[e] = fmaf(-t.rate, v[e], p[e] * t.decay);
+    }
+    if (whole) {
+      if (t.master) *(f32x4*)(t.master + base + e0) = (f32x4){v[0], v[1], v[2], v[3]};
+      if (p32) *(f32x4*)((float*)t.p + base + e0) = (f32x4){v[0], v[1], v[2], v[3]};
+      else *(u32x2*)((bf16*)t.p + base + e0) = (u32x2){pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (e0 + e >= n) continue;
+        if (t.master) t.master[base + e0 + e] = v[e];
+        if (p32) ((float*)t.p)[base + e0 + e] = v[e];
+        else ((bf16*)t.p)[base + e0 + e] = (bf16)v[e];
+      }
+    }
+  }
+#endif
+}
+
 // ---- the host's side ----
 struct MuGroup {  // matrices of one shape and precision
   int64_t m, n, mp, np, count;
@@ -588,11 +890,23 @@ struct MuGroup {  // matrices of one shape and precision
 };
 struct MuPlan {
   std::vector<MuGroup> groups;
-  std::vector<int> of;             // a tensor's group
+  std::vector<int> of;             // a tensor's group, or -1: empty, or all are small
   std::vector<int64_t> at, parts;  // its first matrix there, and its first sum of squares
   int64_t sums = 0, halves = 0, bytes = 0;
 };
 
+// Matrices that a workgroup can take whole: the variant of muon_small_kernel, or -1.
+static int mu_small(const strata_hip_muon_matrix& t) {
+  const int64_t m = std::min(t.rows, t.cols), n = std::max(t.rows, t.cols);
+  return m <= 64 && n <= 128 ? 0 : m <= 64 && n <= 384 ? 1 : n <= 128 ? 2 : -1;
+}
+// Whether a call's matrices all are.  Beside others they go with them, whose launches they do not lengthen (two of 128 x 128 among
+// eight matrices in fp32: 109 us; first by themselves 150).
+static bool mu_all_small(const strata_hip_muon_matrix* ts, int64_t count) {
+  for (int64_t i = 0; i < count; ++i)
+    if (ts[i].rows && ts[i].cols && ts[i].batch && mu_small(ts[i]) < 0) return false;
+  return true;
+}
 static int64_t mu_chunks(const strata_hip_muon_matrix& t) { return (t.rows * t.cols + MU_CHUNK - 1) / MU_CHUNK; }
 static int64_t mu_up(int64_t n) { return (n + MU_PAD - 1) / MU_PAD * MU_PAD; }
 
@@ -615,13 +929,14 @@ static int mu_sizes(const std::string& n, const strata_hip_muon_matrix* ts, int6
 // A matrix has room for two fp16 a value of X; A and P have it where `precise`.
 static MuPlan mu_plan(const strata_hip_muon_matrix* ts, int64_t count) {
   MuPlan q;
+  const bool small = mu_all_small(ts, count);
   std::map<std::tuple<int64_t, int64_t, bool>, int> seen;
   for (int64_t i = 0; i < count; ++i) {
     const int64_t m = std::min(ts[i].rows, ts[i].cols), n = std::max(ts[i].rows, ts[i].cols);
     const bool precise = ts[i].precise != 0;
     q.at.push_back(0);
     q.parts.push_back(q.sums);
-    if (m <= 0 || ts[i].batch <= 0) {
+    if (m <= 0 || ts[i].batch <= 0 || small) {
       q.of.push_back(-1);
       continue;
     }
@@ -679,7 +994,7 @@ static int mu_check(const std::string& n, const strata_hip_muon_args* a, bool st
     if (step) written.emplace_back((uintptr_t)t.momentum, (uintptr_t)t.momentum + 4 * all);
     if (t.master) written.emplace_back((uintptr_t)t.master, (uintptr_t)t.master + 4 * all);
   }
-  if (!written.empty() && (!a->workspace || ((uintptr_t)a->workspace & 255)))
+  if (!mu_all_small(a->matrices, a->count) && (!a->workspace || ((uintptr_t)a->workspace & 255)))
     return fail(STRATA_HIP_EINVAL, n + ": workspace must be given, 256-byte aligned");
   return check_ranges(n, written, read);
 }
@@ -693,15 +1008,15 @@ static int64_t mu_length(const MuGroup& g, int mode) { return (mode == MU_GRAM ?
 
 // The tile of a launch, by an estimate of its cycles: rounds of the 256 CUs, each of the tiles' stages at what one costs with so
 // many tiles on a CU, and what a tile costs besides; at least the longest tile alone.  Measured in cycles a stage, one
-// tile alone on a CU and as many as fit: 64 x 64 240 and 480 (3), 128 x 128 530 and 850 (2), 256 x 256 1300; of two fp16
-// 64 x 64 400 and 670 (2), 128 x 128 1150; besides them 5000, 11000, 17000 (7000, 12000).  What it decides: 960 x 3840 alone, X X^T
+// tile alone on a CU and as many as fit: 64 x 64 240 and 480 (3), 128 x 128 530 and 850 (2), 256 x 256 1400; of two fp16
+// 64 x 64 400 and 670 (2), 128 x 128 1150; besides them 5000, 11000, 20000 (7000, 12000).  What it decides: 960 x 3840 alone, X X^T
 // 16 us on 64 x 64, 32 on 128 x 128, 73 on 256 x 256; 72 matrices of 512 columns 53, 41, 50; 48 of 960 P X 485, 395, 336.
 static int mu_tile_size(const std::vector<const MuGroup*>& groups, int mode, bool precise) {
   struct Cost {
     int tile, fit;
     double alone, more, fixed;  // a stage: alone + more for each other tile on the CU
   };
-  static constexpr Cost plain[3] = {{64, 3, 240., 120., 5e3}, {128, 2, 530., 320., 11e3}, {256, 1, 1300., 0., 17e3}};
+  static constexpr Cost plain[3] = {{64, 3, 240., 120., 5e3}, {128, 2, 530., 320., 11e3}, {256, 1, 1400., 0., 20e3}};
   static constexpr Cost two[2] = {{64, 2, 400., 270., 7e3}, {128, 1, 1150., 0., 12e3}};
   int best = 0;
   double least = 0.;
@@ -765,10 +1080,73 @@ static int mu_products(const MuPlan& q, MuGemm& b, hipStream_t st, F fill) {
   return rc ? rc : mu_products_of<MODE, 2>(q, b, st, fill);
 }
 
+// What the kernels are told of a tensor, but for its place in the workspace.
+static MuTensor mu_tensor(const strata_hip_muon_args* a, const strata_hip_muon_matrix& t, bool step) {
+  MuTensor o = {};
+  o.p = t.param;
+  o.g = t.grad;
+  o.m = t.momentum;
+  o.master = t.master;
+  o.rows = t.rows;
+  o.cols = t.cols;
+  const uintptr_t at = (uintptr_t)t.grad | (uintptr_t)t.momentum | (uintptr_t)t.param | (uintptr_t)t.master;
+  o.flags = (t.param_dtype == STRATA_HIP_F32 ? MU_P32 : 0) | (t.grad_dtype == STRATA_HIP_F32 ? MU_G32 : 0) |
+            (t.rows > t.cols ? MU_TALL : 0) | ((at & 15) || t.cols % 4 ? 0 : MU_ALIGNED) | (a->nesterov ? MU_NESTEROV : 0) |
+            (step ? MU_STEP : 0) | (t.precise ? MU_LO : 0);
+  const double adjust = a->adjust == STRATA_HIP_ADJUST_MATCH_RMS_ADAMW ? 0.2 * std::sqrt((double)std::max(t.rows, t.cols))
+                                                                       : std::sqrt(std::max(1., (double)t.rows / (double)t.cols));
+  o.rate = (float)(t.lr * adjust);
+  o.decay = (float)(1. - t.lr * t.weight_decay);
+  return o;
+}
+
+template <int MP, int NP, int PARTS>
+static int mu_small_launch(const strata_hip_muon_args* a, int kind, bool step, hipStream_t st) {
+  MuSmall b;
+  b.count = 0;
+  b.steps = a->steps;
+  b.mu = (float)a->momentum;
+  b.omu = (float)(1. - a->momentum);
+  b.eps = a->eps;
+  for (int i = 0; i < 3 * a->steps; ++i) b.co[i / 3][i % 3] = (float)a->coefficients[i];
+  uint32_t wgs = 0;
+  auto flush = [&]() -> int {
+    if (!b.count) return STRATA_HIP_OK;
+    hipLaunchKernelGGL((muon_small_kernel<MP, NP, PARTS>), dim3(wgs), dim3(512), 0, st, b);
+    b.count = 0;
+    wgs = 0;
+    return check_launch("muon small");
+  };
+  for (int64_t i = 0; i < a->count; ++i) {
+    const strata_hip_muon_matrix& t = a->matrices[i];
+    if (!t.rows || !t.cols || !t.batch || mu_small(t) != kind || (t.precise != 0) != (PARTS == 2)) continue;
+    if (b.count == MU_SMALL_PER || wgs + t.batch > (1 << 22))
+      if (const int rc = flush()) return rc;
+    b.t[b.count] = mu_tensor(a, t, step);
+    b.t[b.count++].first = wgs;
+    wgs += (uint32_t)t.batch;
+  }
+  return flush();
+}
+
 static int mu_launch(const std::string& name, const strata_hip_muon_args* a, bool step, hipStream_t st) {
   if (const int rc = mu_check(name, a, step)) return rc;
+  if (mu_all_small(a->matrices, a->count)) {
+    int kinds = 0;
+    for (int64_t i = 0; i < a->count; ++i) {
+      const strata_hip_muon_matrix& t = a->matrices[i];
+      if (t.rows && t.cols && t.batch) kinds |= 1 << (2 * mu_small(t) + (t.precise != 0));
+    }
+    int rc = STRATA_HIP_OK;
+    if (!rc && kinds & 1) rc = mu_small_launch<64, 128, 1>(a, 0, step, st);
+    if (!rc && kinds & 2) rc = mu_small_launch<64, 128, 2>(a, 0, step, st);
+    if (!rc && kinds & 4) rc = mu_small_launch<64, 384, 1>(a, 1, step, st);
+    if (!rc && kinds & 8) rc = mu_small_launch<64, 384, 2>(a, 1, step, st);
+    if (!rc && kinds & 16) rc = mu_small_launch<128, 128, 1>(a, 2, step, st);
+    if (!rc && kinds & 32) rc = mu_small_launch<128, 128, 2>(a, 2, step, st);
+    return rc;
+  }
   const MuPlan q = mu_plan(a->matrices, a->count);
-  if (q.groups.empty()) return STRATA_HIP_OK;
   double* const sums = (double*)a->workspace;
   f16* const halves = (f16*)((char*)a->workspace + (q.sums * 8 + 255) / 256 * 256);
   int last = 0;  // which X a pass reads or writes
@@ -798,25 +1176,12 @@ static int mu_launch(const std::string& name, const strata_hip_muon_args* a, boo
       if (b.count == MU_PER || wgs + n > (1 << 23))
         if (const int rc = flush()) return rc;
       MuTensor& o = b.t[b.count++];
-      o.p = t.param;
-      o.g = t.grad;
-      o.m = t.momentum;
-      o.master = t.master;
+      o = mu_tensor(a, t, step);
       o.x = halves + g.x[last] + q.at[(size_t)i] * g.mp * g.np;
       o.xlo = o.x + g.count * g.mp * g.np;
       o.part = sums + q.parts[(size_t)i];
-      o.rows = t.rows;
-      o.cols = t.cols;
       o.first = wgs;
       o.per = (uint32_t)per;
-      const uintptr_t at = (uintptr_t)t.grad | (uintptr_t)t.momentum | (uintptr_t)t.param | (uintptr_t)t.master;
-      o.flags = (t.param_dtype == STRATA_HIP_F32 ? MU_P32 : 0) | (t.grad_dtype == STRATA_HIP_F32 ? MU_G32 : 0) |
-                (t.rows > t.cols ? MU_TALL : 0) | ((at & 15) || t.cols % 4 ? 0 : MU_ALIGNED) | (a->nesterov ? MU_NESTEROV : 0) |
-                (step ? MU_STEP : 0) | (g.precise ? MU_LO : 0);
-      const double adjust = a->adjust == STRATA_HIP_ADJUST_MATCH_RMS_ADAMW ? 0.2 * std::sqrt((double)std::max(t.rows, t.cols))
-                                                                           : std::sqrt(std::max(1., (double)t.rows / (double)t.cols));
-      o.rate = (float)(t.lr * adjust);
-      o.decay = (float)(1. - t.lr * t.weight_decay);
       wgs += (uint32_t)n;
     }
     return flush();

@@ -48,7 +48,7 @@ def test_values_come_near_one():
 
 def _row(i, **over):
     base = 0x1000000 * (i + 1)
-    t = _lib.MuonMatrix(base, base + 0x100000, base + 0x200000, None, 1, 64, 32, 1e-3, 0.1, _lib.BF16, _lib.BF16, 0, 0)
+    t = _lib.MuonMatrix(base, base + 0x100000, base + 0x200000, None, 1, 136, 136, 1e-3, 0.1, _lib.BF16, _lib.BF16, 0, 0)
     for k, v in over.items():
         setattr(t, k, v)
     return t
@@ -77,7 +77,7 @@ NAN, INF = float("nan"), float("inf")
     ({}, dict(param=None), {}, "null"), ({}, dict(grad=None), {}, "null"), ({}, dict(momentum=None), {}, "null"),
     ({}, dict(param_dtype=_lib.F32, master=0x9000000), {}, "master"), ({}, dict(param=0x1000001), {}, "aligned"),
     ({}, dict(momentum=0x1200002), {}, "aligned"), ({}, {}, dict(param=0x1000000), "overlap"),
-    ({}, {}, dict(param=0x1000000 + 64 * 32 * 2 - 2), "overlap"), ({}, dict(batch=257), {}, "overlap"),
+    ({}, {}, dict(param=0x1000000 + 136 * 136 * 2 - 2), "overlap"), ({}, dict(batch=257), {}, "overlap"),
     ({}, dict(grad=0x1000000), {}, "gradient"), ({}, dict(grad=0x2200000), {}, "gradient"), ({}, dict(master=0x2000000), {}, "overlap"),
 ])
 def test_c_entry_refuses(lib, over, first, second, msg):
@@ -105,10 +105,11 @@ def test_sizes_past_the_grids(lib, size):
 
 
 def test_workspace_and_empty_calls(lib):
-    t = (_lib.MuonMatrix * 3)(_row(0, rows=65, cols=3), _row(1, rows=0), _row(2, rows=3, cols=65, precise=1, batch=2))
-    one = lambda pad, halves: 8 * pad + 2 * halves  # noqa: E731
-    both = one(32, 2 * 2 * 64 * 128 + 2 * 64 * 64 + 2 * (2 * 2 * 64 * 128 + 2 * 2 * 64 * 64))
-    assert lib.strata_hip_muon_workspace(t, 3) == both and lib.strata_hip_muon_workspace(None, 0) == 0
+    """Sums of squares, and X twice, A and P in fp16; nothing for matrices that all are small, which one workgroup takes whole."""
+    t = (_lib.MuonMatrix * 4)(_row(0, rows=200, cols=65), _row(1, rows=0), _row(2, rows=65, cols=200, precise=1, batch=2), _row(3, rows=64, cols=384))
+    size = 8 * 32 + 2 * (4 * 64 * 384 + 2 * 64 * 64) + 2 * (4 * 128 * 256 + 2 * 128 * 128) + 2 * 2 * (4 * 128 * 256 + 4 * 128 * 128)
+    assert lib.strata_hip_muon_workspace(t, 4) == size and lib.strata_hip_muon_workspace(None, 0) == 0
+    assert lib.strata_hip_muon_workspace(ctypes.byref(t[3]), 1) == 0
     none = (_lib.MuonMatrix * 2)(_row(0, rows=0), _row(1, batch=0))
     a = _lib.MuonArgs(none, 2, None, None, 0.9, 1e-7, 0, 1, 0, 0)
     assert lib.strata_hip_muon_step(ctypes.byref(a), None) == _lib.OK  # nothing to do, nothing launched
@@ -123,15 +124,16 @@ def test_c_entry_returns_where_a_list_cannot_be_held(lib):
     from pathlib import Path
 
     code = f"""
-import ctypes, mmap
+import ctypes, mmap, resource
 from strata_amd import _lib
 lib = _lib.load()
+n = (96 << 26) // {ctypes.sizeof(_lib.MuonMatrix)}
 zeros = mmap.mmap(-1, 96 << 26, flags=mmap.MAP_PRIVATE | mmap.MAP_ANONYMOUS | 0x4000)  # no pages until they are written
 t = ctypes.cast(ctypes.addressof(ctypes.c_char.from_buffer(zeros)), ctypes.POINTER(_lib.MuonMatrix))
-import resource
+t[n - 1] = (0x1000000, 0x2000000, 0x3000000, None, 1, 200, 200, 0.1, 0.1, 0, 0, 0, 0)
 resource.setrlimit(resource.RLIMIT_AS, (int(open("/proc/self/statm").read().split()[0]) * 4096 + (64 << 20),) * 2)
-assert lib.strata_hip_muon_workspace(t, (96 << 26) // {ctypes.sizeof(_lib.MuonMatrix)}) == -1
-a = _lib.MuonArgs(t, (96 << 26) // {ctypes.sizeof(_lib.MuonMatrix)}, None, 0x100, 0.9, 1e-7, 0, 1, 0, 0)
+assert lib.strata_hip_muon_workspace(t, n) == -1
+a = _lib.MuonArgs(t, n, None, 0x100, 0.9, 1e-7, 0, 1, 0, 0)
 assert lib.strata_hip_muon_step(ctypes.byref(a), None) == _lib.EUNSUPPORTED
 """
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=Path(_lib.__file__).resolve().parents[1])

@@ -46,7 +46,7 @@ def check(got, x, precise, **kw):
 
 
 SHAPES = [(1, 1), (1, 2), (1, 777), (500, 1), (2, 3), (63, 65), (64, 64), (65, 64), (100, 300), (128, 128), (129, 127), (130, 257),
-          (192, 640), (513, 96), (300, 290)]
+          (192, 640), (513, 96), (300, 290), (64, 384), (300, 40), (64, 385), (128, 129), (65, 128), (66, 512)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
@@ -83,6 +83,19 @@ def test_stacks_strides_and_transposes(gpu, dtype):
     odd = torch.zeros(x.numel() + 1, dtype=dtype, device=gpu)[1:].view(x.shape)
     odd.copy_(x)
     assert torch.equal(ops.orthogonalize(odd), y)
+
+
+@pytest.mark.parametrize("count,rows,cols,dtype", [(100, 130, 260, BF16), (70, 512, 600, BF16), (150, 260, 300, F32), (64, 513, 400, BF16),
+                                                   (90, 384, 260, F32), (300, 64, 200, F32), (300, 100, 120, BF16)])
+def test_many_matrices(gpu, count, rows, cols, dtype):
+    """Enough of them for every tile of the products: each as alone, to the bit, and some against the oracle."""
+    g = torch.Generator(device=gpu).manual_seed(count)
+    x = (torch.randn(count, rows, cols, generator=g, device=gpu) * torch.exp(torch.randn(count, rows, 1, generator=g, device=gpu))).to(dtype)
+    y = ops.orthogonalize(x)
+    for i in (0, count // 2, count - 1):
+        check(y[i].cpu(), x[i].cpu(), dtype == F32)
+        assert torch.equal(y[i], ops.orthogonalize(x[i]))
+    assert torch.equal(ops.orthogonalize(x), y)
 
 
 def test_steps_and_coefficients(gpu):
@@ -185,18 +198,24 @@ def test_steps_match_the_oracle(gpu, p_dtype, g_dtype, master, offset):
         assert all(torch.equal(a, b) for a, b in zip(ts["grads"], before["grads"]))
 
 
-def test_many_tensors_rates_and_types_in_one_call(gpu):
-    """More tensors and more shapes than a launch takes; every matrix as in a call of its own, to the bit."""
+@pytest.mark.parametrize("big", [False, True], ids=["small", "with-large"])
+def test_many_tensors_rates_and_types_in_one_call(gpu, big):
+    """More tensors and more shapes than a launch takes; every matrix as in a call of its own, to the bit (small ones
+    where all are small)."""
     a = _tensors([(k % 7 + 1, 3 * k + 1) for k in range(50)], F32, F32, False, 2, gpu)
     b = _tensors([(24, 40)] * 45, BF16, BF16, True, 3, gpu)
     c = _tensors([(40, 24), (24, 40), (70, 3)], BF16, F32, False, 4, gpu)
-    ts = {k: a[k] + b[k] + c[k] for k in a}
+    sets = [a, b, c]
+    if big:
+        sets += [_tensors([(k % 5 + 1, 400 + 70 * k) for k in range(43)], F32, BF16, False, 5, gpu),
+                 _tensors([(400, 70 + 66 * (k % 2)) for k in range(46)], BF16, F32, False, 6, gpu)]
+    ts = {k: [t for s in sets for t in s[k]] for k in a}
     n = len(ts["params"])
     lrs, wds = [1e-2 * (1 + i % 3) for i in range(n)], [0.1 * (i % 2) for i in range(n)]
     before = _copy(ts)
     ops.muon_step(**ts, lr=lrs, weight_decay=wds, momentum=0.95)
     _check_step(ts, before, lrs=lrs, wds=wds)
-    for i in (0, 3, 49, 50, 94, 95, 96, 97):
+    for i in (98, 100, 139, 140, 141, 185, 186) if big else (0, 3, 49, 50, 94, 95, 96, 97):
         one = {k: x[i:i + 1] for k, x in _copy(before).items()}
         ops.muon_step(**one, lr=lrs[i], weight_decay=wds[i], momentum=0.95)
         for k in one:
