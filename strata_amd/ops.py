@@ -1612,15 +1612,15 @@ def _balance_forward(logits, index, score, sequences):
     if index.dtype != torch.int32 or index.dim() != logits.dim() or index.shape[:-1] != logits.shape[:-1] or not index.shape[-1]:
         raise ValueError(f"{name}: index must be int32 {[*logits.shape[:-1], 'top_k']}, got {index.dtype} {list(index.shape)}")
     E, i, n = logits.shape[-1], index.contiguous(), int(sequences)
-    balance, z = torch.empty((), device=dev), torch.empty((), device=dev)
-    load = torch.empty(E, dtype=torch.int32, device=dev)
-    state = torch.empty(2 + max(n, 0) * E, device=dev)
+    new, f32 = logits.new_empty, torch.float32
+    balance, z, state = new((), dtype=f32), new((), dtype=f32), new(2 + max(n, 0) * E, dtype=f32)
+    load = new(E, dtype=torch.int32)
     rows = logits.numel() // max(E, 1)
-    ws = torch.empty(_lib.function("strata_hip_expert_balance_workspace")(rows, n, E), dtype=torch.uint8, device=dev)
+    ws = new(_lib.function("strata_hip_expert_balance_workspace")(rows, n, E), dtype=torch.uint8)
     a, keep = _balance_args(name, logits, index.shape[-1], score, n, state.data_ptr(), i.data_ptr(), balance.data_ptr(),
                             z.data_ptr(), load.data_ptr(), workspace=ws.data_ptr())
     _launch("strata_hip_expert_balance", a, logits)
-    return balance, z, load, state
+    return balance, z, load, state, a
 
 
 def _balance_backward(dbalance, dz, logits, state, top_k, score, sequences):
@@ -1641,28 +1641,39 @@ def _balance_backward(dbalance, dz, logits, state, top_k, score, sequences):
 class _ExpertBalance(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, index, score, sequences):
-        balance, z, load, state = _balance_forward(logits, index, score, sequences)
+        balance, z, load, state, call = _balance_forward(logits, index, score, sequences)
         ctx.mark_non_differentiable(load)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(logits, state)
         ctx.args = index.shape[-1], score, int(sequences)
+        ctx.call = (call, logits.shape, logits.dtype) if logits.is_contiguous() else None
         return balance, z, load
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dbalance, dz, _dload):
+        """Autograd runs this in a thread of its own, where every step takes two to three times as long: the forward's checked
+        arguments are taken over, but for the tensors' places."""
         if dbalance is None and dz is None:
             return (None,) * 4
         logits, state = ctx.saved_tensors
-        plain = _eager(dbalance, dz, logits) and not any(d is not None and _batched(d) for d in (dbalance, dz))
-        return (_balance_backward if plain else expert_balance_bwd)(dbalance, dz, logits, state, *ctx.args), None, None, None
+        if torch.is_grad_enabled() or not _eager(dbalance, dz, logits) or any(d is not None and _batched(d) for d in (dbalance, dz)):
+            return expert_balance_bwd(dbalance, dz, logits, state, *ctx.args), None, None, None  # whose own gradient is refused
+        if ctx.call is None or (logits.shape, logits.dtype) != ctx.call[1:] or not logits.is_contiguous():  # hooks may change them
+            return _balance_backward(dbalance, dz, logits, state, *ctx.args), None, None, None
+        out = torch.empty_like(logits)
+        a = _lib.ExpertBalanceArgs.from_buffer_copy(ctx.call[0])
+        a.logits, a.state, a.dlogits = logits.data_ptr(), state.data_ptr(), out.data_ptr()
+        a.dbalance = None if dbalance is None else dbalance.data_ptr()
+        a.dz = None if dz is None else dz.data_ptr()
+        _launch("strata_hip_expert_balance_bwd", a, logits)
+        return out, None, None, None
 
 
 @torch.library.custom_op("strata_hip::expert_balance", mutates_args=())
 def _expert_balance_op(logits: Tensor, index: Tensor, score: str = "softmax",
                        sequences: int = 1) -> tuple[Tensor, Tensor, Tensor, Tensor]:
     """``expert_balance`` as a custom op, with what its backward needs behind the load."""
-    return _balance_forward(logits, index, score, sequences)
+    return _balance_forward(logits, index, score, sequences)[:4]
 
 
 def expert_balance(logits: Tensor, index: Tensor, score: str = "softmax", sequences: int = 1) -> tuple[Tensor, Tensor, Tensor]:

@@ -171,6 +171,38 @@ def test_either_loss_alone_has_a_gradient(launches):
         assert torch.autograd.grad(out, x)[0].shape == x.shape and launches == ["strata_hip_expert_balance", "strata_hip_expert_balance_bwd"]
 
 
+def test_differentiable_once(launches):
+    x = torch.randn(6, 4, requires_grad=True)
+    b = ops.expert_balance(x, torch.zeros(6, 2, dtype=torch.int32))[0]
+    (g,) = torch.autograd.grad(b, x, create_graph=True)
+    with pytest.raises(RuntimeError, match="forward-only"):
+        torch.autograd.grad(g.sum(), x)
+
+
+def test_backward_takes_the_saved_tensors_as_they_come_back(launches, monkeypatch):
+    """Of another place, type or layout where hooks changed them; strided logits; a graph kept and run twice."""
+    seen = []
+    monkeypatch.setattr(ops, "_launch", lambda name, a, t, *r: seen.append((name, a.logits, a.dlogits, a.dtype, a.ld, a.tokens)))
+    index = torch.zeros(6, 2, dtype=torch.int32)
+    for change, code in ((lambda t: t.clone(), _lib.F32), (lambda t: t.bfloat16() if t.dim() == 2 else t, _lib.BF16),
+                         (lambda t: t.t().contiguous().t() if t.dim() == 2 else t, _lib.F32)):
+        x = torch.randn(6, 4, requires_grad=True)
+        kept = []
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: kept.append(change(t)) or kept[-1]):
+            b = ops.expert_balance(x, index)[0]
+        seen.clear()
+        for _ in range(2):
+            g = torch.autograd.grad(b, x, retain_graph=True)[0]
+        assert g.shape == x.shape and [s[0] for s in seen] == ["strata_hip_expert_balance_bwd"] * 2
+        assert {s[3] for s in seen} == {code} and all(s[4:] == (4, 6) for s in seen)
+        if change(x.detach()).is_contiguous():
+            assert [s[1] for s in seen] == [t.data_ptr() for t in kept if t.dim() == 2]
+    wide = torch.randn(6, 9, requires_grad=True)
+    seen.clear()
+    torch.autograd.grad(ops.expert_balance(wide[:, 1:5], index)[1], wide)
+    assert [s[4] for s in seen] == [9, 9]
+
+
 def test_compiled_with_its_gradient(launches):
     i = torch.zeros(6, 2, dtype=torch.int32)
     torch._dynamo.reset()
