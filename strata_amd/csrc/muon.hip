@@ -77,11 +77,24 @@ __device__ __forceinline__ int mu_entry(int count, uint32_t wg, F first) {
   return lo;
 }
 
-// v, rounded to fp32.  Some variants of a kernel would otherwise round a multiply-add straight to fp16 (v_fma_mixlo_f16) or
-// merge it with the subtraction of its first fp16: a matrix's result would depend on the tile that the others call for.
+// v, rounded to fp32.  A product or multiply-add that is converted to fp16 may otherwise be rounded straight to it
+// (v_fma_mixlo_f16) where it is stored and by way of fp32 where it is subtracted, of which a second fp16 would not be the rest; and
+// a matrix's result would depend on the variant of the kernel.
 __device__ __forceinline__ float mu_rounded(float v) {
   asm("" : "+v"(v));
   return v;
+}
+
+// MU_X / max(norm, eps) as f 2^k: of tiny and huge updates it leaves fp32, and a product of 64 bits costs eight times two of 32.
+struct MuScale {
+  float f;
+  int k;
+  __device__ __forceinline__ float operator()(float u) const { return mu_rounded(ldexpf(u, k) * f); }  // exact, then one rounding
+};
+__device__ __forceinline__ MuScale mu_scale(double norm, double eps) {
+  int k = 0;
+  const double f = frexp(norm == 0. ? 0. : MU_X / (norm < eps ? eps : norm), &k);  // NaN stays NaN
+  return {(float)f, k};
 }
 
 __device__ __forceinline__ float mu_load(const void* p, int64_t i, bool wide) {
@@ -181,7 +194,7 @@ __global__ __launch_bounds__(256) void muon_pack_kernel(MuBatch b) {
   if ((tid & 63) == 0) red[tid >> 6] = s;
   __syncthreads();
   const double norm = sqrt(((red[0] + red[1]) + red[2]) + red[3]);
-  const double scale = norm == 0. ? 0. : MU_X / (norm < b.eps ? b.eps : norm);  // 64-bit: of tiny updates it leaves fp32
+  const MuScale scale = mu_scale(norm, b.eps);
   const int r = tid >> 4, c = (tid & 15) * 4;
   auto write = [&](int row, const float (&v)[4]) {
     f16x4 h, l;
@@ -198,7 +211,7 @@ __global__ __launch_bounds__(256) void muon_pack_kernel(MuBatch b) {
   for (int k = 0; k < 4; ++k) {
     const int64_t row = x.row0 + 16 * k + r, col = x.col0 + c, i = x.base + row * t.cols + col;
     float v[4] = {0.f, 0.f, 0.f, 0.f};
-    auto one = [&](float g, float m) { return (float)((double)(t.m ? nesterov ? fmaf(b.mu, m, b.omu * g) : m : g) * scale); };
+    auto one = [&](float g, float m) { return scale(t.m ? nesterov ? fmaf(b.mu, m, b.omu * g) : m : g); };
     if (row < t.rows) {
       if ((t.flags & MU_ALIGNED) && col + 4 <= t.cols) {
         const f32x4 g = t.m && !nesterov ? (f32x4){0.f, 0.f, 0.f, 0.f} : mu_load4(t.g, i, g32);
@@ -590,10 +603,10 @@ __global__ __launch_bounds__(64 * WGM * WGN, 1) void muon_gemm_kernel(MuGemm p) 
 }
 
 // ---- small matrices: the whole step in one workgroup and launch ----
-// X (as two fp16) and A, which P takes the place of, stay in LDS, in the workspace's layout; u in registers until its norm
-// is known.  Eight waves share the 32 x 32 blocks of a product: of 128 x 128 two each, of 64 x 64 half of the contraction
-// each.  Bound by latencies and the conversions of the results: 128 x 128 alone 32 us, 9200 cycles a step
-// (in eighteen launches 77), 21600 to bring u into LDS.
+// X (as two fp16) and A, which P takes the place of, stay in LDS, in the workspace's layout.  Sixteen waves take a 32 x 32
+// block of a product of 128 x 128 each (eight take two: 30 us), eight one of 64 x 64 with half of the contraction.  Bound by
+// latencies and the conversions of the results: 128 x 128 alone 24 us (eighteen launches: 77), of which a step is 8300 cycles with 3
+// x 1024 of matrix instructions, and 16000 go into u, its norm and the result.
 constexpr int MU_SMALL_PER = 32;  // tensors a launch
 struct MuSmall {
   MuTensor t[MU_SMALL_PER];
@@ -606,14 +619,13 @@ static_assert(sizeof(MuSmall) <= 4096, "kernel arguments");
 
 // MP x n matrices, n <= NP: the shorter side rounded up to MP, the longer one to 64.
 template <int MP, int NP, int PARTS>
-__global__ __launch_bounds__(512, 1) void muon_small_kernel(MuSmall b) {
+__global__ __launch_bounds__(MP == 64 ? 512 : 1024, 1) void muon_small_kernel(MuSmall b) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr int XB = MP * NP * 2, AB = MP * MP * 2;  // bytes of one fp16 of X, of A
   constexpr int HALVES = MP == 64 ? 2 : 1;           // of a contraction, to a wave each
-  constexpr int GB = MP == 64 ? 1 : 2, UB = MP * NP / 1024 / 8;  // blocks a wave of A and P, and of X
-  constexpr int EPT = MP * NP / 512 / 4;             // runs of four elements a thread
+  constexpr int NT = MP == 64 ? 512 : 1024, NW = NT / 64, UB = MP * NP / 1024 / NW;  // threads, waves, blocks of X a wave (of A one)
   __shared__ __attribute__((aligned(1024))) char lds[2 * XB + PARTS * AB + (HALVES == 2 ? MP * MP * 4 : 0)];
-  __shared__ double red[8];
+  __shared__ double red[NW];
   char* const xl = lds;
   char* const al = lds + 2 * XB;
   float* const shares = (float*)(al + PARTS * AB);
@@ -623,47 +635,66 @@ __global__ __launch_bounds__(512, 1) void muon_small_kernel(MuSmall b) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, hi = lane >> 5;
   const int rows = (int)t.rows, cols = (int)t.cols, n = rows * cols;
   const bool tall = t.flags & MU_TALL, g32 = t.flags & MU_G32, p32 = t.flags & MU_P32, nesterov = t.flags & MU_NESTEROV;
-  const bool aligned = t.flags & MU_ALIGNED, step = t.flags & MU_STEP, runs = cols % 4 == 0;
+  const bool aligned = t.flags & MU_ALIGNED, step = t.flags & MU_STEP;
   const int np = ((tall ? rows : cols) + 63) / 64 * 64;
   const int64_t base = (int64_t)(wg - t.first) * n;
 
   // Element (row, col) of a matrix of MP rows in panels of 32 columns, 16-byte chunks swizzled.
   auto place = [](int row, int col) { return (col / MU_K) * (MP * MU_K * 2) + row * (MU_K * 2) + (((col % MU_K) / 8) ^ mu_swz(row)) * 16 + (col % 8) * 2; };
 
-  for (int i = tid; i < 2 * XB / 16; i += 512) *(u32x4*)(xl + 16 * i) = (u32x4){};
-  // u, and m <- mu m + (1 - mu) g
-  float u[EPT][4];
+  for (int i = tid; i < 2 * XB / 16; i += NT) *(u32x4*)(xl + 16 * i) = (u32x4){};
+  __syncthreads();
+  // Runs of four elements where they lie in one row and memory allows, or single ones.  The loops are short: a workgroup alone
+  // fetches every instruction of them anew, and unrolled to the end they took three times as long.
+  const float inverse = 1.f / (float)cols;
+  auto row_of = [&](int e) { return (int)(((float)e + 0.5f) * inverse); };  // e / cols: off from the next one by 1 / 2 cols, e < 2^21
+  auto at_of = [&](int e) {
+    const int row = row_of(e), col = e - row * cols;
+    return tall ? place(col, row) : place(row, col);
+  };
+  // u, and m <- mu m + (1 - mu) g.  u's upper and lower 16 bits take the places of X's two fp16 until the norm is known.
   double s = 0.;
+  auto momentum = [&](float g, float& m) {
+    m = fmaf(b.mu, m, b.omu * g);
+    const float u = !t.m ? g : nesterov ? fmaf(b.mu, m, b.omu * g) : m;
+    s = fma((double)u, (double)u, s);
+    return __float_as_uint(u);
+  };
+  if (aligned) {
+#pragma unroll 4
+    for (int e0 = 4 * tid; e0 < n; e0 += 4 * NT) {
+      const f32x4 g = mu_load4(t.g, base + e0, g32);
+      f32x4 m = t.m ? *(const f32x4*)(t.m + base + e0) : (f32x4){};
+      uint32_t u[4];
 #pragma unroll
-  for (int k = 0; k < EPT; ++k) {
-    const int e0 = 4 * (tid + 512 * k);
-    float g[4] = {0.f, 0.f, 0.f, 0.f}, m[4] = {0.f, 0.f, 0.f, 0.f};
-    const bool whole = aligned && e0 < n;  // n is a multiple of 4 then
-    if (whole) {
-      const f32x4 v = mu_load4(t.g, base + e0, g32);
-      const f32x4 w = t.m ? *(const f32x4*)(t.m + base + e0) : (f32x4){};
+      for (int e = 0; e < 4; ++e) {
+        float v = m[e];
+        u[e] = momentum(g[e], v);
+        m[e] = v;
+      }
+      if (t.m) *(f32x4*)(t.m + base + e0) = m;
+      const int at = at_of(e0);
+      if (!tall) {
+        *(u32x2*)(xl + at) = (u32x2){__builtin_amdgcn_perm(u[1], u[0], 0x07060302), __builtin_amdgcn_perm(u[3], u[2], 0x07060302)};
+        *(u32x2*)(xl + XB + at) = (u32x2){__builtin_amdgcn_perm(u[1], u[0], 0x05040100), __builtin_amdgcn_perm(u[3], u[2], 0x05040100)};
+      } else {  // four rows of one swizzle
 #pragma unroll
-      for (int e = 0; e < 4; ++e) g[e] = v[e], m[e] = w[e];
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (e0 + e < n) {
-          g[e] = mu_load(t.g, base + e0 + e, g32);
-          if (t.m) m[e] = t.m[base + e0 + e];
+        for (int e = 0; e < 4; ++e) {
+          *(uint16_t*)(xl + at + e * MU_K * 2) = (uint16_t)(u[e] >> 16);
+          *(uint16_t*)(xl + XB + at + e * MU_K * 2) = (uint16_t)u[e];
         }
+      }
     }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      m[e] = fmaf(b.mu, m[e], b.omu * g[e]);
-      u[k][e] = !t.m ? g[e] : nesterov ? fmaf(b.mu, m[e], b.omu * g[e]) : m[e];
-      s = fma((double)u[k][e], (double)u[k][e], s);
+  } else {
+#pragma unroll 4
+    for (int e = tid; e < n; e += NT) {
+      float m = t.m ? t.m[base + e] : 0.f;
+      const uint32_t u = momentum(mu_load(t.g, base + e, g32), m);
+      if (t.m) t.m[base + e] = m;
+      const int at = at_of(e);
+      *(uint16_t*)(xl + at) = (uint16_t)(u >> 16);
+      *(uint16_t*)(xl + XB + at) = (uint16_t)u;
     }
-    if (!t.m) continue;
-    if (whole) *(f32x4*)(t.m + base + e0) = (f32x4){m[0], m[1], m[2], m[3]};
-    else
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (e0 + e < n) t.m[base + e0 + e] = m[e];
   }
 #pragma unroll
   for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
@@ -671,40 +702,23 @@ __global__ __launch_bounds__(512, 1) void muon_small_kernel(MuSmall b) {
   __syncthreads();
   s = 0.;
 #pragma unroll
-  for (int w = 0; w < 8; ++w) s += red[w];
-  const double norm = sqrt(s), scale = norm == 0. ? 0. : MU_X / (norm < b.eps ? b.eps : norm);
-  // Runs of four elements lie in one row where cols is a multiple of 4, of X or (tall) of four rows of one swizzle.
-#pragma unroll
-  for (int k = 0; k < EPT; ++k) {
-    const int e0 = 4 * (tid + 512 * k);
-    if (e0 >= n) continue;
-    int row = e0 / cols, col = e0 - row * cols;
+  for (int w = 0; w < NW; ++w) s += red[w];
+  const MuScale scale = mu_scale(sqrt(s), b.eps);
+#pragma unroll 2
+  for (int i = tid; i < MP * np / 4; i += NT) {
+    u32x2* const hp = (u32x2*)(xl + 8 * i);
+    u32x2* const lp = (u32x2*)(xl + XB + 8 * i);
+    const u32x2 up = *hp, low = *lp;
     f16x4 h, l;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float v = (float)((double)u[k][e] * scale);
+      const uint32_t u = __builtin_amdgcn_perm(up[e / 2], low[e / 2], e % 2 ? 0x07060302 : 0x05040100);
+      const float v = scale(__uint_as_float(u));
       h[e] = (f16)v;
       l[e] = (f16)(v - (float)h[e]);
     }
-    if (runs && !tall) {
-      const int at = place(row, col);
-      *(f16x4*)(xl + at) = h;
-      *(f16x4*)(xl + XB + at) = l;
-    } else {
-      int at = tall ? place(col, row) : place(row, col);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (e0 + e >= n) break;
-        *(f16*)(xl + at) = h[e];
-        *(f16*)(xl + XB + at) = l[e];
-        if (runs) {
-          at += MU_K * 2;
-        } else {
-          if (++col == cols) col = 0, ++row;
-          at = tall ? place(col, row) : place(row, col);
-        }
-      }
-    }
+    *(f16x4*)hp = h;
+    *(f16x4*)lp = l;
   }
   __syncthreads();
 
@@ -724,35 +738,31 @@ __global__ __launch_bounds__(512, 1) void muon_small_kernel(MuSmall b) {
     }
   };
   // Blocks of m m^T, m [MP, K] at stride `part` between its two fp16: of a wave, with its share of the contraction.
-  auto square = [&](f32x16 (&acc)[GB], const char* m, int part, int K) {
-    const int half = HALVES == 2 ? wave / 4 : 0, block = HALVES == 2 ? wave % 4 : wave * GB;
+  auto square = [&](f32x16& acc, const char* m, int part, int K) {
+    const int half = HALVES == 2 ? wave / 4 : 0, block = HALVES == 2 ? wave % 4 : wave;
     const int r0 = block / (MP / 32) * 32, k0 = half * (K / HALVES), k1 = k0 + K / HALVES;
-#pragma unroll
-    for (int i = 0; i < GB; ++i) acc[i] = (f32x16){};
+    acc = (f32x16){};
 #pragma unroll 2
     for (int k = k0; k < k1; k += 32) {  // K is a multiple of 64
-      f16x8 x[2][PARTS], w[2][GB][PARTS];
+      f16x8 x[2][PARTS], w[2][PARTS];
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
         for (int q = 0; q < PARTS; ++q) {
           x[kk][q] = frag(m + q * part, r0 + l32, k + 16 * kk);
-#pragma unroll
-          for (int i = 0; i < GB; ++i) w[kk][i][q] = frag(m + q * part, (block + i) % (MP / 32) * 32 + l32, k + 16 * kk);
+          w[kk][q] = frag(m + q * part, block % (MP / 32) * 32 + l32, k + 16 * kk);
         }
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-        for (int i = 0; i < GB; ++i) multiply(acc[i], w[kk][i], x[kk]);
+      for (int kk = 0; kk < 2; ++kk) multiply(acc, w[kk], x[kk]);
     }
     if constexpr (HALVES == 2) {  // the upper waves' shares are added to the lower ones'
       if (half)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) *(f32x4*)(shares + ((block * 4 + r) * 64 + lane) * 4) = (f32x4){acc[0][4 * r], acc[0][4 * r + 1], acc[0][4 * r + 2], acc[0][4 * r + 3]};
+        for (int r = 0; r < 4; ++r) *(f32x4*)(shares + ((block * 4 + r) * 64 + lane) * 4) = (f32x4){acc[4 * r], acc[4 * r + 1], acc[4 * r + 2], acc[4 * r + 3]};
       __syncthreads();
       if (!half)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc[0][r] += shares[((block * 4 + r / 4) * 64 + lane) * 4 + r % 4];
+        for (int r = 0; r < 16; ++r) acc[r] += shares[((block * 4 + r / 4) * 64 + lane) * 4 + r % 4];
     }
   };
   // alpha acc + beta d at block (r0, c0) of a matrix, four columns at once, written over d once every wave has read.
@@ -772,40 +782,40 @@ __global__ __launch_bounds__(512, 1) void muon_small_kernel(MuSmall b) {
     for (int q = 0; q < 4; ++q) {
       const int at = place(r0 + l32, c0 + 8 * q + 4 * hi);
       f16x4 h, l;
+      if (two) {
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        h[x] = (f16)acc[4 * q + x];
-        l[x] = (f16)(acc[4 * q + x] - (float)h[x]);
+        for (int x = 0; x < 4; ++x) {
+          const float v = mu_rounded(acc[4 * q + x]);
+          h[x] = (f16)v;
+          l[x] = (f16)(v - (float)h[x]);
+        }
+        *(f16x4*)(o + part + at) = l;
+      } else {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) h[x] = (f16)acc[4 * q + x];
       }
       *(f16x4*)(o + at) = h;
-      if (two) *(f16x4*)(o + part + at) = l;
     }
   };
-  const int block = HALVES == 2 ? wave % 4 : wave * GB, r0 = block / (MP / 32) * 32;
+  const int block = HALVES == 2 ? wave % 4 : wave, r0 = block / (MP / 32) * 32, c0 = block % (MP / 32) * 32;
   const bool mine = HALVES == 1 || wave < 4;  // holds blocks of A and P
   for (int k = 0; k < b.steps; ++k) {
-    f32x16 acc[GB];
+    f32x16 acc;
     square(acc, xl, XB, np);
-    if (mine)
-#pragma unroll
-      for (int i = 0; i < GB; ++i) {
-        combine(acc[i], nullptr, 0, false, 0, 0, MU_A / (MU_X * MU_X), 0.f);
-        write(acc[i], al, AB, PARTS == 2, r0, (block + i) % (MP / 32) * 32);
-      }
+    if (mine) {
+      combine(acc, nullptr, 0, false, 0, 0, MU_A / (MU_X * MU_X), 0.f);
+      write(acc, al, AB, PARTS == 2, r0, c0);
+    }
     __syncthreads();
     square(acc, al, AB, MP);
-    if (mine)
-#pragma unroll
-      for (int i = 0; i < GB; ++i) combine(acc[i], al, AB, PARTS == 2, r0, (block + i) % (MP / 32) * 32, b.co[k][2] / MU_A, b.co[k][1]);
+    if (mine) combine(acc, al, AB, PARTS == 2, r0, c0, b.co[k][2] / MU_A, b.co[k][1]);
     __syncthreads();
-    if (mine)
-#pragma unroll
-      for (int i = 0; i < GB; ++i) write(acc[i], al, AB, PARTS == 2, r0, (block + i) % (MP / 32) * 32);
+    if (mine) write(acc, al, AB, PARTS == 2, r0, c0);
     __syncthreads();
     f32x16 x[UB];
 #pragma unroll
     for (int i = 0; i < UB; ++i) {
-      const int blk = wave + 8 * i, rr = blk % (MP / 32) * 32, cc = blk / (MP / 32) * 32;
+      const int blk = wave + NW * i, rr = blk % (MP / 32) * 32, cc = blk / (MP / 32) * 32;
       if (cc >= np) continue;
       x[i] = (f32x16){};
 #pragma unroll
@@ -823,60 +833,43 @@ __global__ __launch_bounds__(512, 1) void muon_small_kernel(MuSmall b) {
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < UB; ++i) {
-      const int blk = wave + 8 * i, rr = blk % (MP / 32) * 32, cc = blk / (MP / 32) * 32;
+      const int blk = wave + NW * i, rr = blk % (MP / 32) * 32, cc = blk / (MP / 32) * 32;
       if (cc < np) write(x[i], xl, XB, PARTS == 2 || k + 1 < MU_LO_STEPS, rr, cc);
     }
     __syncthreads();
   }
 
+  auto value = [&](int at) { return ((float)*(const f16*)(xl + at) + (PARTS == 2 ? (float)*(const f16*)(xl + XB + at) : 0.f)) * (1.f / MU_X); };
+  if (aligned) {
+#pragma unroll 4
+    for (int e0 = 4 * tid; e0 < n; e0 += 4 * NT) {
+      f32x4 p = {}, v;
+      if (step) p = t.master ? *(const f32x4*)(t.master + base + e0) : mu_load4(t.p, base + e0, p32);
+      const int at = at_of(e0);
+      if (!tall) {
+        const f16x4 h = *(const f16x4*)(xl + at), l = PARTS == 2 ? *(const f16x4*)(xl + XB + at) : (f16x4){};
 #pragma unroll
-  for (int k = 0; k < EPT; ++k) {
-    const int e0 = 4 * (tid + 512 * k);
-    if (e0 >= n) continue;
-    int row = e0 / cols, col = e0 - row * cols;
-    float v[4];
-    const bool whole = aligned;
-    f32x4 p = {};
-    if (step && whole) p = t.master ? *(const f32x4*)(t.master + base + e0) : mu_load4(t.p, base + e0, p32);
-    f16x4 h = {}, l = {};
-    if (runs && !tall) {
-      const int at = place(row, col);
-      h = *(const f16x4*)(xl + at);
-      if (PARTS == 2) l = *(const f16x4*)(xl + XB + at);
-    } else {
-      int at = tall ? place(col, row) : place(row, col);
+        for (int e = 0; e < 4; ++e) v[e] = ((float)h[e] + (float)l[e]) * (1.f / MU_X);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = value(at + e * MU_K * 2);
+      }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if (e0 + e >= n) break;
-        h[e] = *(const f16*)(xl + at);
-        if (PARTS == 2) l[e] = *(const f16*)(xl + XB + at);
-        if (runs) {
-          at += MU_K * 2;
-        } else {
-          if (++col == cols) col = 0, ++row;
-          at = tall ? place(col, row) : place(row, col);
-        }
+        if (step) v[e] = fmaf(-t.rate, v[e], p[e] * t.decay);
       }
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      v[e] = ((float)h[e] + (float)l[e]) * (1.f / MU_X);
-      if (!step) continue;
-      if (!whole && e0 + e < n) p[e] = t.master ? t.master[base + e0 + e] : mu_load(t.p, base + e0 + e, p32);
-      v[e] = fmaf(-t.rate, v[e], p[e] * t.decay);
-    }
-    if (whole) {
-      if (t.master) *(f32x4*)(t.master + base + e0) = (f32x4){v[0], v[1], v[2], v[3]};
-      if (p32) *(f32x4*)((float*)t.p + base + e0) = (f32x4){v[0], v[1], v[2], v[3]};
+      if (t.master) *(f32x4*)(t.master + base + e0) = v;
+      if (p32) *(f32x4*)((float*)t.p + base + e0) = v;
       else *(u32x2*)((bf16*)t.p + base + e0) = (u32x2){pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (e0 + e >= n) continue;
-        if (t.master) t.master[base + e0 + e] = v[e];
-        if (p32) ((float*)t.p)[base + e0 + e] = v[e];
-        else ((bf16*)t.p)[base + e0 + e] = (bf16)v[e];
-      }
+    }
+  } else {
+#pragma unroll 4
+    for (int e = tid; e < n; e += NT) {
+      float v = value(at_of(e));
+      if (step) v = fmaf(-t.rate, v, (t.master ? t.master[base + e] : mu_load(t.p, base + e, p32)) * t.decay);
+      if (t.master) t.master[base + e] = v;
+      if (p32) ((float*)t.p)[base + e] = v;
+      else ((bf16*)t.p)[base + e] = (bf16)v;
     }
   }
 #endif
@@ -1112,7 +1105,7 @@ static int mu_small_launch(const strata_hip_muon_args* a, int kind, bool step, h
   uint32_t wgs = 0;
   auto flush = [&]() -> int {
     if (!b.count) return STRATA_HIP_OK;
-    hipLaunchKernelGGL((muon_small_kernel<MP, NP, PARTS>), dim3(wgs), dim3(512), 0, st, b);
+    hipLaunchKernelGGL((muon_small_kernel<MP, NP, PARTS>), dim3(wgs), dim3(MP == 64 ? 512 : 1024), 0, st, b);
     b.count = 0;
     wgs = 0;
     return check_launch("muon small");
