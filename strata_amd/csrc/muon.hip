@@ -378,7 +378,9 @@ __device__ __forceinline__ void mu_wait() {  // all but the last N copies have l
 // 3840, P X 312 us (814 TFLOP/s; a library product of 960 x 960 x 3840 by 12 910, of 8192^3 1216), X X^T 178 us (716 of the
 // half that is needed, 256 x 256 tiles on the diagonal and the edge 42% more); 79% of a 256 x 256 tile's cycles in the
 // loop issue them, its start and epilogue are 26% of P X.  128 x 128 tiles wait for L2 (16 KiB a stage of 256 cycles); of two fp16
-// they multiply three times and do not.
+// they multiply three times and do not; there P X takes two stages only, so that another tile of the CU multiplies during
+// one's start and epilogue (24 matrices of 640 columns 140 us, with five stages and one tile a CU 163; X X^T with its longer
+// contraction 98 and 87).
 template <int T, int WGM, int WGN, int NST, int PARTS, int MODE>
 __global__ __launch_bounds__(64 * WGM * WGN, 1) void muon_gemm_kernel(MuGemm p) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -387,7 +389,7 @@ __global__ __launch_bounds__(64 * WGM * WGN, 1) void muon_gemm_kernel(MuGemm p) 
   constexpr int WTM = T / WGM, WTN = T / WGN, FM = WTM / 32, FN = WTN / 32;
   constexpr int ROWB = MU_K * 2, PB = T * ROWB, XB = PARTS * PB, STAGE = 2 * XB;  // one fp16 of an operand, an operand, a stage
   constexpr int LP = PB / 1024 / NW, COPIES = 2 * PARTS * LP;                      // 1-KiB copies a wave
-  static_assert(WTM % 32 == 0 && WTN % 32 == 0 && PB % (1024 * NW) == 0 && NST >= 3, "layout");
+  static_assert(WTM % 32 == 0 && WTN % 32 == 0 && PB % (1024 * NW) == 0 && NST >= 2, "layout");
   __shared__ __attribute__((aligned(1024))) char lds[NST * STAGE];
 
   const int tid = (int)__builtin_amdgcn_workitem_id_x();
@@ -502,20 +504,24 @@ __global__ __launch_bounds__(64 * WGM * WGN, 1) void muon_gemm_kernel(MuGemm p) 
 
   constexpr int PRODUCTS = PARTS == 2 ? 3 : 1, GROUPS = KS * PRODUCTS * FN;
   f16x8 af[2][PARTS][FN], bf[2][PARTS][FM];
-  mu_wait<(NST - 2) * COPIES>();
-  lds_barrier();
-  load_frags(lds, 0, af[0], bf[0]);
+  constexpr bool AHEAD = NST > 2;  // two stages: the first fragments of one are read once it has landed, while other workgroups multiply
+  if constexpr (AHEAD) {
+    mu_wait<(NST - 2) * COPIES>();
+    lds_barrier();
+    load_frags(lds, 0, af[0], bf[0]);
+  }
   const char* st = lds;
   for (int kt = 0; kt < nk; ++kt) {
-    mu_wait<(NST - 3) * COPIES>();
-    wait_lgkm0();  // this stage's first fragments, read among the products before: the slot of kt - 1 is read, no later wait counts them
-    lds_barrier();     // stage kt + 1 landed for every wave, and the slot of kt - 1 is free
+    mu_wait<AHEAD ? (NST - 3) * COPIES : 0>();
+    wait_lgkm0();   // the slot of kt - 1 is read, and this stage's first fragments are there: no later wait counts them
+    lds_barrier();  // stage kt + 1 (or kt) landed for every wave, and the slot of kt - 1 is free
     const char* const next = st == lds + (NST - 1) * STAGE ? lds : st + STAGE;
+    if constexpr (!AHEAD) load_frags(st, 0, af[0], bf[0]);
 #pragma unroll
     for (int kk = 0; kk < KS; ++kk) {
       const int cb = kk & 1;
       if (kk + 1 < KS) load_frags(st, kk + 1, af[cb ^ 1], bf[cb ^ 1]);
-      else load_frags(next, 0, af[cb ^ 1], bf[cb ^ 1]);  // after the last stage: read for nothing
+      else if (AHEAD) load_frags(next, 0, af[cb ^ 1], bf[cb ^ 1]);  // after the last stage: read for nothing
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int pr = 0; pr < PRODUCTS; ++pr)
@@ -1002,7 +1008,7 @@ static int64_t mu_length(const MuGroup& g, int mode) { return (mode == MU_GRAM ?
 // The tile of a launch, by an estimate of its cycles: rounds of the 256 CUs, each of the tiles' stages at what one costs with so
 // many tiles on a CU, and what a tile costs besides; at least the longest tile alone.  Measured in cycles a stage, one
 // tile alone on a CU and as many as fit: 64 x 64 240 and 480 (3), 128 x 128 530 and 850 (2), 256 x 256 1400; of two fp16
-// 64 x 64 400 and 670 (2), 128 x 128 1150; besides them 5000, 11000, 20000 (7000, 12000).  What it decides: 960 x 3840 alone, X X^T
+// 64 x 64 400 and 670 (2), 128 x 128 1150, in P X 1300 and 2800 (2); besides them 5000, 11000, 20000 (7000, 12000).  What it decides: 960 x 3840 alone, X X^T
 // 16 us on 64 x 64, 32 on 128 x 128, 73 on 256 x 256; 72 matrices of 512 columns 53, 41, 50; 48 of 960 P X 485, 395, 336.
 static int mu_tile_size(const std::vector<const MuGroup*>& groups, int mode, bool precise) {
   struct Cost {
@@ -1010,7 +1016,8 @@ static int mu_tile_size(const std::vector<const MuGroup*>& groups, int mode, boo
     double alone, more, fixed;  // a stage: alone + more for each other tile on the CU
   };
   static constexpr Cost plain[3] = {{64, 3, 240., 120., 5e3}, {128, 2, 530., 320., 11e3}, {256, 1, 1400., 0., 20e3}};
-  static constexpr Cost two[2] = {{64, 2, 400., 270., 7e3}, {128, 1, 1150., 0., 12e3}};
+  static constexpr Cost square[2] = {{64, 2, 400., 270., 7e3}, {128, 1, 1150., 0., 12e3}}, update[2] = {{64, 2, 400., 270., 7e3}, {128, 2, 1300., 1500., 12e3}};
+  const Cost* const two = mode == MU_UPDATE ? update : square;
   int best = 0;
   double least = 0.;
   for (int i = 0; i < (precise ? 2 : 3); ++i) {
@@ -1044,6 +1051,7 @@ static int mu_products_of(const MuPlan& q, MuGemm& b, hipStream_t st, F fill) {
   auto flush = [&]() -> int {
     if (!b.count) return STRATA_HIP_OK;
     if (T == 64) hipLaunchKernelGGL((muon_gemm_kernel<64, 2, 2, PARTS == 2 ? 4 : 6, PARTS, MODE>), dim3(tiles), dim3(256), 0, st, b);
+    else if constexpr (PARTS == 2 && MODE == MU_UPDATE) hipLaunchKernelGGL((muon_gemm_kernel<128, 4, 2, 2, 2, MU_UPDATE>), dim3(tiles), dim3(512), 0, st, b);
     else if (T == 128) hipLaunchKernelGGL((muon_gemm_kernel<128, 2, 2, PARTS == 2 ? 5 : 4, PARTS, MODE>), dim3(tiles), dim3(256), 0, st, b);
     else if constexpr (PARTS == 1) hipLaunchKernelGGL((muon_gemm_kernel<256, 2, 4, 4, 1, MODE>), dim3(tiles), dim3(512), 0, st, b);
     b.count = 0;
