@@ -899,12 +899,24 @@ static int mu_small(const strata_hip_muon_matrix& t) {
   const int64_t m = std::min(t.rows, t.cols), n = std::max(t.rows, t.cols);
   return m <= 64 && n <= 128 ? 0 : m <= 64 && n <= 384 ? 1 : n <= 128 ? 2 : -1;
 }
-// Whether a call's matrices all are.  Beside others they go with them, whose launches they do not lengthen (two of 128 x 128 among
-// eight matrices in fp32: 109 us; first by themselves 150).
-static bool mu_all_small(const strata_hip_muon_matrix* ts, int64_t count) {
-  for (int64_t i = 0; i < count; ++i)
-    if (ts[i].rows && ts[i].cols && ts[i].batch && mu_small(ts[i]) < 0) return false;
-  return true;
+// What a call's matrices all are.
+struct MuCall {
+  // Small.  Beside others such matrices go with them, whose launches they do not lengthen (two of 128 x 128 among eight
+  // matrices in fp32: 109 us; first by themselves 150).
+  bool small = true;
+  // At most 64 on the shorter side: few singular values, over which fp16's roundings do not even out (4e-3 of a row's result).
+  // All of them take two fp16, which costs such a call little, its launches being mostly latency; among others they would add launches.
+  bool narrow = true;
+  bool precise(const strata_hip_muon_matrix& t) const { return narrow || t.precise; }
+};
+static MuCall mu_call(const strata_hip_muon_matrix* ts, int64_t count) {
+  MuCall c;
+  for (int64_t i = 0; i < count; ++i) {
+    if (!ts[i].rows || !ts[i].cols || !ts[i].batch) continue;
+    c.small &= mu_small(ts[i]) >= 0;
+    c.narrow &= std::min(ts[i].rows, ts[i].cols) <= 64;
+  }
+  return c;
 }
 static int64_t mu_chunks(const strata_hip_muon_matrix& t) { return (t.rows * t.cols + MU_CHUNK - 1) / MU_CHUNK; }
 static int64_t mu_up(int64_t n) { return (n + MU_PAD - 1) / MU_PAD * MU_PAD; }
@@ -928,14 +940,14 @@ static int mu_sizes(const std::string& n, const strata_hip_muon_matrix* ts, int6
 // A matrix has room for two fp16 a value of X; A and P have it where `precise`.
 static MuPlan mu_plan(const strata_hip_muon_matrix* ts, int64_t count) {
   MuPlan q;
-  const bool small = mu_all_small(ts, count);
+  const MuCall call = mu_call(ts, count);
   std::map<std::tuple<int64_t, int64_t, bool>, int> seen;
   for (int64_t i = 0; i < count; ++i) {
     const int64_t m = std::min(ts[i].rows, ts[i].cols), n = std::max(ts[i].rows, ts[i].cols);
-    const bool precise = ts[i].precise != 0;
+    const bool precise = call.precise(ts[i]);
     q.at.push_back(0);
     q.parts.push_back(q.sums);
-    if (m <= 0 || ts[i].batch <= 0 || small) {
+    if (m <= 0 || ts[i].batch <= 0 || call.small) {
       q.of.push_back(-1);
       continue;
     }
@@ -993,7 +1005,7 @@ static int mu_check(const std::string& n, const strata_hip_muon_args* a, bool st
     if (step) written.emplace_back((uintptr_t)t.momentum, (uintptr_t)t.momentum + 4 * all);
     if (t.master) written.emplace_back((uintptr_t)t.master, (uintptr_t)t.master + 4 * all);
   }
-  if (!mu_all_small(a->matrices, a->count) && (!a->workspace || ((uintptr_t)a->workspace & 255)))
+  if (!mu_call(a->matrices, a->count).small && (!a->workspace || ((uintptr_t)a->workspace & 255)))
     return fail(STRATA_HIP_EINVAL, n + ": workspace must be given, 256-byte aligned");
   return check_ranges(n, written, read);
 }
@@ -1082,7 +1094,7 @@ static int mu_products(const MuPlan& q, MuGemm& b, hipStream_t st, F fill) {
 }
 
 // What the kernels are told of a tensor, but for its place in the workspace.
-static MuTensor mu_tensor(const strata_hip_muon_args* a, const strata_hip_muon_matrix& t, bool step) {
+static MuTensor mu_tensor(const strata_hip_muon_args* a, const strata_hip_muon_matrix& t, const MuCall& call, bool step) {
   MuTensor o = {};
   o.p = t.param;
   o.g = t.grad;
@@ -1093,7 +1105,7 @@ static MuTensor mu_tensor(const strata_hip_muon_args* a, const strata_hip_muon_m
   const uintptr_t at = (uintptr_t)t.grad | (uintptr_t)t.momentum | (uintptr_t)t.param | (uintptr_t)t.master;
   o.flags = (t.param_dtype == STRATA_HIP_F32 ? MU_P32 : 0) | (t.grad_dtype == STRATA_HIP_F32 ? MU_G32 : 0) |
             (t.rows > t.cols ? MU_TALL : 0) | ((at & 15) || t.cols % 4 ? 0 : MU_ALIGNED) | (a->nesterov ? MU_NESTEROV : 0) |
-            (step ? MU_STEP : 0) | (t.precise ? MU_LO : 0);
+            (step ? MU_STEP : 0) | (call.precise(t) ? MU_LO : 0);
   const double adjust = a->adjust == STRATA_HIP_ADJUST_MATCH_RMS_ADAMW ? 0.2 * std::sqrt((double)std::max(t.rows, t.cols))
                                                                        : std::sqrt(std::max(1., (double)t.rows / (double)t.cols));
   o.rate = (float)(t.lr * adjust);
@@ -1102,7 +1114,7 @@ static MuTensor mu_tensor(const strata_hip_muon_args* a, const strata_hip_muon_m
 }
 
 template <int MP, int NP, int PARTS>
-static int mu_small_launch(const strata_hip_muon_args* a, int kind, bool step, hipStream_t st) {
+static int mu_small_launch(const strata_hip_muon_args* a, const MuCall& call, int kind, bool step, hipStream_t st) {
   MuSmall b;
   b.count = 0;
   b.steps = a->steps;
@@ -1120,10 +1132,10 @@ static int mu_small_launch(const strata_hip_muon_args* a, int kind, bool step, h
   };
   for (int64_t i = 0; i < a->count; ++i) {
     const strata_hip_muon_matrix& t = a->matrices[i];
-    if (!t.rows || !t.cols || !t.batch || mu_small(t) != kind || (t.precise != 0) != (PARTS == 2)) continue;
+    if (!t.rows || !t.cols || !t.batch || mu_small(t) != kind || call.precise(t) != (PARTS == 2)) continue;
     if (b.count == MU_SMALL_PER || wgs + t.batch > (1 << 22))
       if (const int rc = flush()) return rc;
-    b.t[b.count] = mu_tensor(a, t, step);
+    b.t[b.count] = mu_tensor(a, t, call, step);
     b.t[b.count++].first = wgs;
     wgs += (uint32_t)t.batch;
   }
@@ -1132,19 +1144,20 @@ static int mu_small_launch(const strata_hip_muon_args* a, int kind, bool step, h
 
 static int mu_launch(const std::string& name, const strata_hip_muon_args* a, bool step, hipStream_t st) {
   if (const int rc = mu_check(name, a, step)) return rc;
-  if (mu_all_small(a->matrices, a->count)) {
+  const MuCall call = mu_call(a->matrices, a->count);
+  if (call.small) {
     int kinds = 0;
     for (int64_t i = 0; i < a->count; ++i) {
       const strata_hip_muon_matrix& t = a->matrices[i];
-      if (t.rows && t.cols && t.batch) kinds |= 1 << (2 * mu_small(t) + (t.precise != 0));
+      if (t.rows && t.cols && t.batch) kinds |= 1 << (2 * mu_small(t) + call.precise(t));
     }
     int rc = STRATA_HIP_OK;
-    if (!rc && kinds & 1) rc = mu_small_launch<64, 128, 1>(a, 0, step, st);
-    if (!rc && kinds & 2) rc = mu_small_launch<64, 128, 2>(a, 0, step, st);
-    if (!rc && kinds & 4) rc = mu_small_launch<64, 384, 1>(a, 1, step, st);
-    if (!rc && kinds & 8) rc = mu_small_launch<64, 384, 2>(a, 1, step, st);
-    if (!rc && kinds & 16) rc = mu_small_launch<128, 128, 1>(a, 2, step, st);
-    if (!rc && kinds & 32) rc = mu_small_launch<128, 128, 2>(a, 2, step, st);
+    if (!rc && kinds & 1) rc = mu_small_launch<64, 128, 1>(a, call, 0, step, st);
+    if (!rc && kinds & 2) rc = mu_small_launch<64, 128, 2>(a, call, 0, step, st);
+    if (!rc && kinds & 4) rc = mu_small_launch<64, 384, 1>(a, call, 1, step, st);
+    if (!rc && kinds & 8) rc = mu_small_launch<64, 384, 2>(a, call, 1, step, st);
+    if (!rc && kinds & 16) rc = mu_small_launch<128, 128, 1>(a, call, 2, step, st);
+    if (!rc && kinds & 32) rc = mu_small_launch<128, 128, 2>(a, call, 2, step, st);
     return rc;
   }
   const MuPlan q = mu_plan(a->matrices, a->count);
@@ -1177,7 +1190,7 @@ static int mu_launch(const std::string& name, const strata_hip_muon_args* a, boo
       if (b.count == MU_PER || wgs + n > (1 << 23))
         if (const int rc = flush()) return rc;
       MuTensor& o = b.t[b.count++];
-      o = mu_tensor(a, t, step);
+      o = mu_tensor(a, t, call, step);
       o.x = halves + g.x[last] + q.at[(size_t)i] * g.mp * g.np;
       o.xlo = o.x + g.count * g.mp * g.np;
       o.part = sums + q.parts[(size_t)i];

@@ -2269,9 +2269,10 @@ def orthogonalize(x: Tensor, coefficients: Sequence[float] | Sequence[Sequence[f
     for each step; they should keep singular values under 8.  The usual ones bring values from 0.001 on
     to about [0.7, 1.2], not to 1.
 
-    ``precise`` (of fp32 matrices where it is not given): the products' operands keep 22 bits, at three times the cost, and the result is
-    off by about 1e-6 of its norm; otherwise fp16 operands with fp32 sums, off by about 1e-3, less than
-    a bf16 result's own rounding.  A matrix with a value that is not finite becomes NaN, a zero one stays zero.
+    ``precise`` (of fp32 matrices where it is not given): the products' operands keep 22 bits, at three times the cost,
+    and the result is off by about 1e-6 of its norm; otherwise fp16 operands with fp32 sums, off by about 1e-3, less
+    than a bf16 result's own rounding (3e-3 where one direction is much stronger than all others; matrices with
+    a side of at most 64 keep 22 bits).  A matrix with a value that is not finite becomes NaN, a zero one stays zero.
     Not differentiable.  At most 2^20 rows and columns, 2^15 of the fewer of them."""
     flat, steps = _newton_schulz("orthogonalize", coefficients, steps, eps)
     if _eager(x):
