@@ -541,7 +541,6 @@ __global__ __launch_bounds__(64 * WGM * WGN, 1) void muon_gemm_kernel(MuGemm p) 
   }
   wait_vmcnt(0);
   // ---- epilogue, 32 x 32 at a time in registers
-  const bool mirror = SYM && tm != tn;
   f16* const __restrict__ out = s.out + mat * os;
   const int64_t olo = count * os;  // from a value's first fp16 to its second
   const f16* const __restrict__ d = s.d + mat * os;
@@ -563,7 +562,9 @@ __global__ __launch_bounds__(64 * WGM * WGN, 1) void muon_gemm_kernel(MuGemm p) 
     }
 #pragma unroll
     for (int j = 0; j < FM; ++j) {
-      if (gr0 + 32 * j >= mp) continue;
+      // Blocks below the diagonal are mirror images in the diagonal's tiles too: of two fp16 their sums have another order.
+      if (gr0 + 32 * j >= mp || (SYM && gr0 + 32 * j > c0)) continue;
+      const bool mirror = SYM && gr0 + 32 * j < c0;
       float v[16];
       if (MODE != MU_GRAM) {
         mu_unrows(dh[j]);
@@ -604,6 +605,151 @@ __global__ __launch_bounds__(64 * WGM * WGN, 1) void muon_gemm_kernel(MuGemm p) 
         for (int t = 0; t < 2; ++t) *(u32x4*)(o + element(gr0 + 32 * j + 16 * t + (lane & 15), c0 + mu_chunk(lane))) = w[t];
       }
     }
+  }
+#endif
+}
+
+// ---- P and X <- a X + P X of slim matrices in one launch ----
+// A whole (at most 128 x 128) and 128 columns of X lie in LDS; a workgroup makes 64 rows of P from A for itself, which costs it 0.7 us
+// where a launch costs 4 to 5, and multiplies them by its columns: eight waves with a 32 x 32 block each.  The same sums in
+// the same order as muon_gemm_kernel's.  Bound by latencies: eight matrices of 128 columns
+// in fp32 7.8 us (P and X by themselves 5.6 and 5.7), of which the start and 160 KiB of copies are 2.
+struct MuSlim {
+  MuShape s[MU_PER];  // x: A, w: X
+  uint32_t first[MU_PER];
+  int count;
+  float a, b, c;
+};
+static_assert(sizeof(MuSlim) <= 4096, "kernel arguments");
+
+template <int MP, int PARTS>
+__global__ __launch_bounds__(512, 1) void muon_slim_kernel(MuSlim p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  constexpr int AB = MP * MP * 2, XB = MP * 128 * 2, PB = 64 * MP * 2;  // bytes of one fp16 of A, of the columns, of 64 rows of P
+  __shared__ __attribute__((aligned(1024))) char lds[PARTS * (AB + XB + PB)];
+  char* const xl = lds + PARTS * AB;
+  char* const pl = xl + PARTS * XB;
+  const int tid = (int)__builtin_amdgcn_workitem_id_x();
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
+  const uint32_t lds_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+  const uint32_t wg = (uint32_t)__builtin_amdgcn_workgroup_id_x();
+  MuShape s = p.s[0];
+  uint32_t first = 0;
+  const int entry = __builtin_popcountll(__ballot(lane < p.count && p.first[lane < MU_PER ? lane : 0] <= wg)) - 1;
+  if (entry) s = p.s[entry], first = p.first[entry];
+  const int np = s.np, flags = s.flags, across = (np + 127) / 128, per = MP / 64 * across;
+  const int id = (int)(wg - first), mat = id / per, rest = id % per, r0 = rest / across * 64, n0 = rest % across * 128;
+  const int64_t wide = (int64_t)MP * np;
+
+  // Both are whole panels, 16 rows a copy.
+  auto copy = [&](const f16* from, uint32_t to, int panels) {
+    for (int u = wave; u < panels * (MP / 16); u += 8) {
+      const int row = 16 * (u % (MP / 16)) + lane / 4;
+      const uint32_t at = (uint32_t)(u / (MP / 16)) * (MP * MU_K * 2) + row * (MU_K * 2) + ((lane % 4) ^ mu_swz(row)) * 16;
+      dma_row16(make_rsrc(from, OOB), to + u * 1024, at);
+    }
+  };
+  const int panels = min(4, (np - n0) / MU_K);  // the rest of LDS is multiplied for nobody
+#pragma unroll
+  for (int q = 0; q < PARTS; ++q) {
+    copy(s.x + mat * (int64_t)(MP * MP) + q * s.count * (int64_t)(MP * MP), lds_base + q * AB, MP / MU_K);
+    copy(s.w + mat * wide + q * s.count * wide + (int64_t)n0 * MP, lds_base + PARTS * AB + q * XB, panels);
+  }
+  auto place = [](int rows, int row, int col) { return (col / MU_K) * (rows * MU_K * 2) + row * (MU_K * 2) + (((col % MU_K) / 8) ^ mu_swz(row)) * 16 + (col % 8) * 2; };
+  const int br = wave / 4 * 32, bc = wave % 4 * 32;  // this wave's block: of X, and of the rows of P
+  wait_vmcnt(0);
+  lds_barrier();
+
+  auto multiply = [&](f32x16& acc, const f16x8 (&w)[PARTS], const f16x8 (&x)[PARTS], bool lower) {
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(w[0], x[0], acc, 0, 0, 0);
+    if constexpr (PARTS == 2) {  // below P's diagonal in the order of the block whose image it is
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(w[lower ? 0 : 1], x[lower ? 1 : 0], acc, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(w[lower ? 1 : 0], x[lower ? 0 : 1], acc, 0, 0, 0);
+    }
+  };
+  const int pr = MP == 64 ? wave / 2 * 32 : br, pc = MP == 64 ? wave % 2 * 32 : bc;
+  auto square = [&](bool lower) {
+    f32x16 acc = {};
+#pragma unroll
+    for (int k = 0; k < MP; k += 16) {
+      f16x8 x[PARTS], w[PARTS];
+#pragma unroll
+      for (int q = 0; q < PARTS; ++q) {
+        x[q] = *(const f16x8*)(lds + q * AB + place(MP, r0 + pr + l32, k + 8 * hi));
+        w[q] = *(const f16x8*)(lds + q * AB + place(MP, pc + l32, k + 8 * hi));
+      }
+      multiply(acc, w, x, lower);
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int at = place(MP, r0 + pr + l32, pc + 8 * q + 4 * hi), to = place(64, pr + l32, pc + 8 * q + 4 * hi);
+      const f16x4 dh = *(const f16x4*)(lds + at), dl = PARTS == 2 ? *(const f16x4*)(lds + AB + at) : (f16x4){};
+      f16x4 h, l;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const float v = mu_rounded(fmaf(acc[4 * q + x], p.c / MU_A, p.b * ((float)dh[x] + (float)dl[x])));
+        h[x] = (f16)v;
+        l[x] = (f16)(v - (float)h[x]);
+      }
+      *(f16x4*)(pl + to) = h;
+      if (PARTS == 2) *(f16x4*)(pl + PB + to) = l;
+    }
+  };
+  if (MP == 128 || wave < 4) {
+    if (r0 + pr > pc) square(true);
+    else square(false);
+  }
+  __syncthreads();
+
+  const int c0 = n0 + bc;
+  if (c0 >= np) return;
+  f32x16 acc = {};
+#pragma unroll
+  for (int k = 0; k < MP; k += 16) {
+    f16x8 x[PARTS], w[PARTS];
+#pragma unroll
+    for (int q = 0; q < PARTS; ++q) {
+      typedef __fp16 h16x4 __attribute__((ext_vector_type(4)));
+      const int row = k + 8 * hi + ((lane & 15) >> 2), col = bc + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+      const char* const m = xl + q * XB;
+      const f16x4 lo = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16(LDS_PTR(h16x4, m + place(MP, row, col))));
+      const f16x4 up = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16(LDS_PTR(h16x4, m + place(MP, row + 4, col))));
+      w[q] = __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7);
+      x[q] = *(const f16x8*)(pl + q * PB + place(64, br + l32, k + 8 * hi));
+    }
+    multiply(acc, w, x, false);
+  }
+  // a X: X's second fp16 from LDS, or (of the first steps where only a X has it) from memory
+  const int64_t panel = MP * MU_K, block = (int64_t)(c0 / MU_K) * panel + (r0 + br) * MU_K;
+  float v[16];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int at = place(MP, r0 + br + l32, bc + 8 * q + 4 * hi);
+    const f16x4 h = *(const f16x4*)(xl + at);
+    f16x4 l = {};
+    if (PARTS == 2) l = *(const f16x4*)(xl + XB + at);
+    else if (flags & MU_LO_IN) l = *(const f16x4*)(s.w + (s.count + mat) * wide + block + l32 * MU_K + 8 * q + 4 * hi);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) v[4 * q + x] = mu_rounded(fmaf(acc[4 * q + x], 1.f / MU_A, p.a * ((float)h[x] + (float)l[x])));
+  }
+#pragma unroll
+  for (int part = 0; part < 2; ++part) {
+    if (part && !(flags & MU_LO_OUT)) break;
+    f16* const o = s.out + (part * s.count + mat) * wide + block;
+    u32x4 w[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      f16x8 h;
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        h[x] = (f16)v[8 * t + x];
+        v[8 * t + x] = v[8 * t + x] - (float)h[x];
+      }
+      w[t] = __builtin_bit_cast(u32x4, h);
+    }
+    mu_rows(w);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) *(u32x4*)(o + (16 * t + (lane & 15)) * MU_K + mu_chunk(lane)) = w[t];
   }
 #endif
 }
@@ -907,6 +1053,8 @@ struct MuCall {
   // At most 64 on the shorter side: few singular values, over which fp16's roundings do not even out (4e-3 of a row's result).
   // All of them take two fp16, which costs such a call little, its launches being mostly latency; among others they would add launches.
   bool narrow = true;
+  // At most 128 on it: a step is two launches (muon_slim_kernel).
+  bool slim = true;
   bool precise(const strata_hip_muon_matrix& t) const { return narrow || t.precise; }
 };
 static MuCall mu_call(const strata_hip_muon_matrix* ts, int64_t count) {
@@ -915,6 +1063,7 @@ static MuCall mu_call(const strata_hip_muon_matrix* ts, int64_t count) {
     if (!ts[i].rows || !ts[i].cols || !ts[i].batch) continue;
     c.small &= mu_small(ts[i]) >= 0;
     c.narrow &= std::min(ts[i].rows, ts[i].cols) <= 64;
+    c.slim &= std::min(ts[i].rows, ts[i].cols) <= 128;
   }
   return c;
 }
@@ -1087,6 +1236,36 @@ static int mu_products_of(const MuPlan& q, MuGemm& b, hipStream_t st, F fill) {
   return flush();
 }
 
+// P and P X of the groups of one height and precision.
+template <int MP, int PARTS, typename F>
+static int mu_slim_launch(const MuPlan& q, MuSlim& b, hipStream_t st, F fill) {
+  b.count = 0;
+  uint32_t tiles = 0;
+  auto flush = [&]() -> int {
+    if (!b.count) return STRATA_HIP_OK;
+    hipLaunchKernelGGL((muon_slim_kernel<MP, PARTS>), dim3(tiles), dim3(512), 0, st, b);
+    b.count = 0;
+    tiles = 0;
+    return check_launch("muon slim products");
+  };
+  for (const MuGroup& g : q.groups) {
+    if (g.mp != MP || g.precise != (PARTS == 2)) continue;
+    const int64_t n = g.count * (MP / 64) * ((g.np + 127) / 128);  // at most 2^22 (mu_sizes)
+    if (b.count == MU_PER || tiles + n > (1 << 22))
+      if (const int rc = flush()) return rc;
+    b.first[b.count] = tiles;
+    MuShape& s = b.s[b.count++];
+    s.mp = (int)g.mp;
+    s.np = (int)g.np;
+    s.count = (int)g.count;
+    s.tiles = (int)n;
+    s.flags = PARTS == 2 ? MU_LO_IN | MU_LO_OUT : 0;
+    fill(g, s);
+    tiles += (uint32_t)n;
+  }
+  return flush();
+}
+
 template <int MODE, typename F>
 static int mu_products(const MuPlan& q, MuGemm& b, hipStream_t st, F fill) {
   const int rc = mu_products_of<MODE, 1>(q, b, st, fill);
@@ -1213,6 +1392,30 @@ static int mu_launch(const std::string& name, const strata_hip_muon_args* a, boo
           s.out = halves + g.a;
         }))
       return rc;
+    // X's second fp16 goes into the first steps
+    const int lo = (k < MU_LO_STEPS ? MU_LO_IN : 0) | (k + 1 < MU_LO_STEPS ? MU_LO_OUT : 0);
+    auto update = [&](const MuGroup& g, MuShape& s) {
+      s.flags |= lo;
+      s.w = s.d = halves + g.x[last];
+      s.out = halves + g.x[last ^ 1];
+    };
+    if (call.slim) {
+      MuSlim m;
+      m.a = (float)c[0];
+      m.b = (float)c[1];
+      m.c = (float)c[2];
+      auto both = [&](const MuGroup& g, MuShape& s) {
+        update(g, s);
+        s.x = halves + g.a;
+      };
+      int rc = mu_slim_launch<64, 1>(q, m, st, both);
+      if (!rc) rc = mu_slim_launch<64, 2>(q, m, st, both);
+      if (!rc) rc = mu_slim_launch<128, 1>(q, m, st, both);
+      if (!rc) rc = mu_slim_launch<128, 2>(q, m, st, both);
+      if (rc) return rc;
+      last ^= 1;
+      continue;
+    }
     b.alpha = (float)(c[2] / MU_A);
     b.beta = (float)c[1];
     if (const int rc = mu_products<MU_POLY>(q, b, st, [&](const MuGroup& g, MuShape& s) {
@@ -1222,12 +1425,9 @@ static int mu_launch(const std::string& name, const strata_hip_muon_args* a, boo
       return rc;
     b.alpha = 1.f / MU_A;
     b.beta = (float)c[0];
-    const int lo = (k < MU_LO_STEPS ? MU_LO_IN : 0) | (k + 1 < MU_LO_STEPS ? MU_LO_OUT : 0);
     if (const int rc = mu_products<MU_UPDATE>(q, b, st, [&](const MuGroup& g, MuShape& s) {
-          s.flags |= lo;
+          update(g, s);
           s.x = halves + g.p;
-          s.w = s.d = halves + g.x[last];
-          s.out = halves + g.x[last ^ 1];
         }))
       return rc;
     last ^= 1;

@@ -222,6 +222,25 @@ def test_many_tensors_rates_and_types_in_one_call(gpu, big):
             assert one[k][0] is None or torch.equal(one[k][0], ts[k][i]), (i, k)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
+def test_slim_matrices_beside_others(gpu, dtype):
+    """A shorter side of 65 to 128: a step of two launches in a call of such alone, of three beside wider ones, and the same bits."""
+    specs = [(100, 400), (500, 70), (3, 128, 200), (2, 77, 1030), (128, 129), (64, 500), (700, 30)]
+    ts = _tensors(specs, dtype, dtype, False, 21, gpu)
+    wide = _tensors([(200, 330)], dtype, dtype, False, 22, gpu)
+    both = {k: x + wide[k] for k, x in _copy(ts).items()}
+    before = _copy(ts)
+    ops.muon_step(**ts, **HP)
+    ops.muon_step(**both, **HP)
+    _check_step(ts, before)
+    for k in ts:
+        assert all(a is None or torch.equal(a, b) for a, b in zip(ts[k], both[k])), k
+    for i in (0, 3):
+        one = {k: x[i:i + 1] for k, x in before.items()}
+        ops.muon_step(**one, **HP)
+        assert torch.equal(one["params"][0], ts["params"][i])
+
+
 def test_neighbours_in_memory_stay(gpu):
     """Tensors that are views of one buffer, with elements between them that are not theirs."""
     for shape in ((17, 31), (32, 40)):
