@@ -1312,7 +1312,7 @@ static int mu_small_launch(const strata_hip_muon_args* a, const MuCall& call, in
   for (int64_t i = 0; i < a->count; ++i) {
     const strata_hip_muon_matrix& t = a->matrices[i];
     if (!t.rows || !t.cols || !t.batch || mu_small(t) != kind || call.precise(t) != (PARTS == 2)) continue;
-    if (b.count == MU_SMALL_PER || wgs + t.batch > (1 << 22))
+    if (b.count == MU_SMALL_PER || wgs + t.batch > (1 << 21))  // 1024 threads each: a grid holds less than 2^32
       if (const int rc = flush()) return rc;
     b.t[b.count] = mu_tensor(a, t, call, step);
     b.t[b.count++].first = wgs;

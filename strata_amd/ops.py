@@ -2336,7 +2336,8 @@ def muon_step(params: Sequence[Tensor], grads: Sequence[Tensor], momentums: Sequ
     are bf16 or fp32, momentums fp32; ``masters`` are fp32 weights (or None) that a bf16 parameter is rounded
     from.  ``lr`` and ``weight_decay`` may be one number for every tensor; ``coefficients``, ``steps``, ``eps`` and
     ``precise`` are ``orthogonalize``'s (where ``precise`` is not given, that of fp32 weights, masters among them).
-    The step's host work is proportional to the tensors, its launches are not: all matrices share them."""
+    A gradient that is not finite makes its own matrix NaN.  The step's host work is proportional to the tensors, its
+    launches are not: all matrices share them."""
     name = "muon_step"
     if _jit_trace() is not None or torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
         raise RuntimeError(f"{name}: no operator, a trace of it would leave the step out")

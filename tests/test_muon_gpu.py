@@ -98,6 +98,20 @@ def test_many_matrices(gpu, count, rows, cols, dtype):
     assert torch.equal(ops.orthogonalize(x), y)
 
 
+@pytest.mark.parametrize("count,rows,cols", [(64000, 130, 256), (240000, 64, 128)])
+def test_offsets_past_32_bits(gpu, count, rows, cols):
+    """Stacks of nearly 2^31 elements, whose workspace has more: the first and last matrices as alone, to the bit."""
+    x = torch.empty(count, rows, cols, dtype=BF16, device=gpu)
+    g = torch.Generator(device=gpu).manual_seed(1)
+    x.fill_(0.5)
+    for i in (0, 1, count // 2, count - 1):
+        x[i] = torch.randn(rows, cols, generator=g, device=gpu)
+    y = ops.orthogonalize(x)
+    for i in (0, 1, 2, count // 2, count - 1):
+        assert torch.equal(y[i], ops.orthogonalize(x[i])), i
+    check(y[count - 1].cpu(), x[count - 1].cpu(), False)
+
+
 def test_steps_and_coefficients(gpu):
     x = matrix(90, 200, "plain", 3).float()
     for co in ((O.NEWTON_SCHULZ,) * 2, (O.NEWTON_SCHULZ,), (), ((4.0848, -6.8946, 2.9270), (3.9505, -6.3029, 2.6377), (3.7418, -5.5913, 2.3037)),
