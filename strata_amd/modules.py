@@ -143,8 +143,9 @@ class RoutingLosses:
     ``balance`` and ``z`` are the sums over the calls collected (fp32 scalars, see ``ops.expert_balance``; None without
     any), ``load`` a list of ``(mlp, int32 [experts])``, in the order of the calls.  With ``per_sample`` each entry of a
     call's first axis is balanced by itself.  The losses hold the calls' autograd graph: let go of this object before a
-    backward is captured.  It belongs to the thread that entered it, and a region that ``torch.utils.checkpoint`` runs
-    again in the backward does not run inside it."""
+    backward is captured.  It belongs to the thread that entered it.  What ``torch.utils.checkpoint`` runs opens one of its
+    own and returns its losses: around a checkpoint they have no gradient (reentrant) or its backward raises, since the
+    forward is run again outside."""
 
     _local = threading.local()
 

@@ -1611,7 +1611,7 @@ def _balance_forward(logits, index, score, sequences):
     dev = _require_gpu(name, logits, index)
     if index.dtype != torch.int32 or index.dim() != logits.dim() or index.shape[:-1] != logits.shape[:-1] or not index.shape[-1]:
         raise ValueError(f"{name}: index must be int32 {[*logits.shape[:-1], 'top_k']}, got {index.dtype} {list(index.shape)}")
-    E, i, n = logits.shape[-1], index.contiguous(), int(sequences)
+    E, i, n = logits.shape[-1], index.contiguous(), operator.index(sequences)
     new, f32 = logits.new_empty, torch.float32
     balance, z, state = new((), dtype=f32), new((), dtype=f32), new(2 + max(n, 0) * E, dtype=f32)
     load = new(E, dtype=torch.int32)
@@ -2336,8 +2336,8 @@ def muon_step(params: Sequence[Tensor], grads: Sequence[Tensor], momentums: Sequ
     are bf16 or fp32, momentums fp32; ``masters`` are fp32 weights (or None) that a bf16 parameter is rounded
     from.  ``lr`` and ``weight_decay`` may be one number for every tensor; ``coefficients``, ``steps``, ``eps`` and
     ``precise`` are ``orthogonalize``'s (where ``precise`` is not given, that of fp32 weights, masters among them).
-    A gradient that is not finite makes its own matrix NaN.  The step's host work is proportional to the tensors, its
-    launches are not: all matrices share them."""
+    A gradient that is not finite makes its own matrix NaN.  The step's host work is proportional to the tensors; up to
+    40 tensors, and 40 shapes of matrices, share a launch."""
     name = "muon_step"
     if _jit_trace() is not None or torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
         raise RuntimeError(f"{name}: no operator, a trace of it would leave the step out")

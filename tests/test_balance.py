@@ -108,6 +108,12 @@ def test_refused_arguments(launches, logits, index, kw, match):
     assert not launches
 
 
+def test_a_fraction_of_a_sequence_is_refused(launches):
+    with pytest.raises(TypeError, match="integer"):
+        ops.expert_balance(torch.randn(6, 4), torch.zeros(6, 2, dtype=torch.int32), sequences=1.5)
+    assert not launches
+
+
 def test_refused_by_the_library():
     lib = _lib.load()
     a = _lib.ExpertBalanceArgs()

@@ -198,3 +198,33 @@ def test_routing_losses_of_a_block(gpu):
     assert mlp is block.mlp and torch.equal(load.cpu(), want[2])
     (1e-2 * routing.balance + 1e-3 * routing.z).backward()
     assert block.mlp.router.weight.grad.abs().sum() > 0 and block.mlp.w1.grad is None
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_routing_losses_inside_a_checkpoint(gpu, reentrant):
+    """Losses that the region returns have the gradients of the plain run; collected around one that is not
+    reentrant, its backward raises."""
+    from torch.utils.checkpoint import CheckpointError, checkpoint
+
+    torch.manual_seed(0)
+    mlp = modules.ExpertMlp(128, 256, 6).to(gpu).bfloat16()
+    x = torch.randn(90, 128, device=gpu).bfloat16().requires_grad_()
+
+    def region(x):
+        with modules.RoutingLosses() as routing:
+            y = mlp(x)
+        return y.float().square().mean() + routing.balance + 1e-2 * routing.z
+
+    wanted = [x, *mlp.parameters()]
+    region(x).backward()
+    want = [t.grad for t in wanted]
+    for t in wanted:
+        t.grad = None
+    checkpoint(region, x, use_reentrant=reentrant).backward()
+    for t, w in zip(wanted, want):
+        assert torch.equal(t.grad, w)
+    if not reentrant:
+        with modules.RoutingLosses() as routing:
+            y = checkpoint(mlp, x, use_reentrant=False)
+        with pytest.raises(CheckpointError):
+            (y.float().sum() + routing.balance).backward()
