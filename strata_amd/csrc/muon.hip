@@ -376,7 +376,8 @@ __device__ __forceinline__ void mu_wait() {  // all but the last N copies have l
 // multiply, over the stages' borders too, so stage kt + 1 has landed when kt begins.
 // Bound by the matrix instructions and the power that they draw (the clock falls from 2.4 to 1.8 GHz): 48 matrices 960 x 960 to 960 x
 // 3840, P X 312 us (814 TFLOP/s; a library product of 960 x 960 x 3840 by 12 910, of 8192^3 1216), X X^T 178 us (716 of the
-// half that is needed, 256 x 256 tiles on the diagonal and the edge 42% more); 79% of a 256 x 256 tile's cycles in the
+// half that is needed; 256 x 256 tiles on the diagonal and the edge are 42% more, of which 32 x 32 blocks that nobody writes are
+// left out: 209 -> 194 us in a whole step, P X 385 -> 371); 79% of a 256 x 256 tile's cycles in the
 // loop issue them, its start and epilogue are 26% of P X.  128 x 128 tiles wait for L2 (16 KiB a stage of 256 cycles); of two fp16
 // they multiply three times and do not; there P X takes two stages only, so that another tile of the CU multiplies during
 // one's start and epilogue (24 matrices of 640 columns 140 us, with five stages and one tile a CU 163; X X^T with its longer
@@ -394,7 +395,8 @@ __global__ __launch_bounds__(64 * WGM * WGN, 1) void muon_gemm_kernel(MuGemm p) 
 
   const int tid = (int)__builtin_amdgcn_workitem_id_x();
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-  const int wm = wave / WGN, wn = wave % WGN, l32 = lane & 31, hi = lane >> 5;
+  // Two waves of a SIMD are four apart: in a tile of 256 on the diagonal they have 6 to 14 blocks on and above it, of 16.
+  const int wm = wave / WGN, wn = NW == 8 && SYM && wm ? WGN - 1 - wave % WGN : wave % WGN, l32 = lane & 31, hi = lane >> 5;
   const uint32_t lds_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
 
   // Each shape's tiles are dealt to the XCDs in blocks: one matrix's on one XCD, every XCD with its share of every shape.
@@ -510,35 +512,50 @@ __global__ __launch_bounds__(64 * WGM * WGN, 1) void muon_gemm_kernel(MuGemm p) 
     lds_barrier();
     load_frags(lds, 0, af[0], bf[0]);
   }
-  const char* st = lds;
-  for (int kt = 0; kt < nk; ++kt) {
-    mu_wait<AHEAD ? (NST - 3) * COPIES : 0>();
-    wait_lgkm0();   // the slot of kt - 1 is read, and this stage's first fragments are there: no later wait counts them
-    lds_barrier();  // stage kt + 1 (or kt) landed for every wave, and the slot of kt - 1 is free
-    const char* const next = st == lds + (NST - 1) * STAGE ? lds : st + STAGE;
-    if constexpr (!AHEAD) load_frags(st, 0, af[0], bf[0]);
+  // The 32 x 32 blocks of 32 columns that are written: none beyond the matrix, and none below the diagonal.  The others are not
+  // multiplied, which saves their power more than time: a tile's slowest wave mostly has all of its blocks.
+  int blocks[FN];
+  bool every = true;
 #pragma unroll
-    for (int kk = 0; kk < KS; ++kk) {
-      const int cb = kk & 1;
-      if (kk + 1 < KS) load_frags(st, kk + 1, af[cb ^ 1], bf[cb ^ 1]);
-      else if (AHEAD) load_frags(next, 0, af[cb ^ 1], bf[cb ^ 1]);  // after the last stage: read for nothing
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int pr = 0; pr < PRODUCTS; ++pr)
-#pragma unroll
-        for (int i = 0; i < FN; ++i) {
-#pragma unroll
-          for (int j = 0; j < FM; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[cb][PARTS == 2 && pr == 1][i], bf[cb][PARTS == 2 && pr == 2][j], acc[i][j], 0, 0, 0);
-          // the copies between the products: issued at once they would hold up the products behind them
-          const int g = (kk * PRODUCTS + pr) * FN + i;
-          __builtin_amdgcn_sched_barrier(0);
-          issue(COPIES * g / GROUPS, COPIES * (g + 1) / GROUPS);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-    }
-    st = next;
+  for (int i = 0; i < FN; ++i) {
+    const int c0 = gn0 + 32 * i, last = SYM ? c0 : mp - 32;
+    blocks[i] = c0 < cols && gr0 <= last ? min((last - gr0) / 32 + 1, FM) : 0;
+    every = every && blocks[i] == FM;
   }
+  auto loop = [&](auto all) {
+    const char* st = lds;
+    for (int kt = 0; kt < nk; ++kt) {
+      mu_wait<AHEAD ? (NST - 3) * COPIES : 0>();
+      wait_lgkm0();   // the slot of kt - 1 is read, and this stage's first fragments are there: no later wait counts them
+      lds_barrier();  // stage kt + 1 (or kt) landed for every wave, and the slot of kt - 1 is free
+      const char* const next = st == lds + (NST - 1) * STAGE ? lds : st + STAGE;
+      if constexpr (!AHEAD) load_frags(st, 0, af[0], bf[0]);
+#pragma unroll
+      for (int kk = 0; kk < KS; ++kk) {
+        const int cb = kk & 1;
+        if (kk + 1 < KS) load_frags(st, kk + 1, af[cb ^ 1], bf[cb ^ 1]);
+        else if (AHEAD) load_frags(next, 0, af[cb ^ 1], bf[cb ^ 1]);  // after the last stage: read for nothing
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int pr = 0; pr < PRODUCTS; ++pr)
+#pragma unroll
+          for (int i = 0; i < FN; ++i) {
+#pragma unroll
+            for (int j = 0; j < FM; ++j)
+              if (decltype(all)::value || j < blocks[i])
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[cb][PARTS == 2 && pr == 1][i], bf[cb][PARTS == 2 && pr == 2][j], acc[i][j], 0, 0, 0);
+            // the copies between the products: issued at once they would hold up the products behind them
+            const int g = (kk * PRODUCTS + pr) * FN + i;
+            __builtin_amdgcn_sched_barrier(0);
+            issue(COPIES * g / GROUPS, COPIES * (g + 1) / GROUPS);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+      }
+      st = next;
+    }
+  };
+  if (every) loop(std::true_type{});
+  else loop(std::false_type{});
   wait_vmcnt(0);
   // ---- epilogue, 32 x 32 at a time in registers
   f16* const __restrict__ out = s.out + mat * os;
@@ -1170,7 +1187,7 @@ static int64_t mu_length(const MuGroup& g, int mode) { return (mode == MU_GRAM ?
 // many tiles on a CU, and what a tile costs besides; at least the longest tile alone.  Measured in cycles a stage, one
 // tile alone on a CU and as many as fit: 64 x 64 240 and 480 (3), 128 x 128 530 and 850 (2), 256 x 256 1400; of two fp16
 // 64 x 64 400 and 670 (2), 128 x 128 1150, in P X 1300 and 2800 (2); besides them 5000, 11000, 20000 (7000, 12000).  What it decides: 960 x 3840 alone, X X^T
-// 16 us on 64 x 64, 32 on 128 x 128, 73 on 256 x 256; 72 matrices of 512 columns 53, 41, 50; 48 of 960 P X 485, 395, 336.
+// 17 us on 64 x 64, 33 on 128 x 128, 75 on 256 x 256; 72 matrices of 512 columns 53, 41, 47; 48 of 960 P X 570, 423, 362.
 static int mu_tile_size(const std::vector<const MuGroup*>& groups, int mode, bool precise) {
   struct Cost {
     int tile, fit;
