@@ -20,7 +20,7 @@
 // decaying and low-rank spectra (3.7e-3 without the second fp16, 10 to 30e-3 with iterates in bf16), below the 1.7e-3 of
 // a bf16 result's own rounding; a second fp16 in later steps gains nothing and costs 50 us of 350 a product of 133 M
 // elements.  `precise`: X, A and P are sums of two fp16 throughout and a product is three, high high, high low and low
-// high: off by 1e-6 to 3e-6, as products of fp32 are.
+// high (a small matrix's low low too): off by 0.8e-6 to 2e-6, as products of fp32 are.
 #include <algorithm>
 #include <cmath>
 #include <exception>
@@ -459,13 +459,19 @@ __global__ __launch_bounds__(64 * WGM * WGN, 1) void muon_gemm_kernel(MuGemm p) 
   for (int q = 0; q < NST - 1; ++q) issue(0, COPIES);
 
   const int gn0 = n0 + wn * WTN, gr0 = row0 + wm * WTM;
-  f32x16 acc[FN][FM];
+  // Over the long contraction of X X^T the products with a second fp16 have a sum of their own, 2^-11 of the other: a third of the
+  // roundings (8 x 1000 off by 1.1e-6 instead of 2.2e-6, 384 x 776 by 1.55e-6 instead of 1.65e-6; the times within 1%).
+  constexpr int SUMS = PARTS == 2 && MODE == MU_GRAM ? 2 : 1;
+  f32x16 acc[FN][FM], low[SUMS == 2 ? FN : 1][FM];
 #pragma unroll
   for (int i = 0; i < FN; ++i)
 #pragma unroll
     for (int j = 0; j < FM; ++j)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+      for (int r = 0; r < 16; ++r) {
+        acc[i][j][r] = 0.f;
+        if (SUMS == 2) low[i][j][r] = 0.f;
+      }
 
   // LDS offsets of the fragments
   uint32_t aoff[FN][WT ? 1 : KS], boff[FM][KS];
@@ -542,8 +548,10 @@ __global__ __launch_bounds__(64 * WGM * WGN, 1) void muon_gemm_kernel(MuGemm p) 
           for (int i = 0; i < FN; ++i) {
 #pragma unroll
             for (int j = 0; j < FM; ++j)
-              if (decltype(all)::value || j < blocks[i])
-                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[cb][PARTS == 2 && pr == 1][i], bf[cb][PARTS == 2 && pr == 2][j], acc[i][j], 0, 0, 0);
+              if (decltype(all)::value || j < blocks[i]) {
+                f32x16& sum = SUMS == 2 && pr ? low[SUMS == 2 ? i : 0][j] : acc[i][j];
+                sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[cb][PARTS == 2 && pr == 1][i], bf[cb][PARTS == 2 && pr == 2][j], sum, 0, 0, 0);
+              }
             // the copies between the products: issued at once they would hold up the products behind them
             const int g = (kk * PRODUCTS + pr) * FN + i;
             __builtin_amdgcn_sched_barrier(0);
@@ -557,6 +565,13 @@ __global__ __launch_bounds__(64 * WGM * WGN, 1) void muon_gemm_kernel(MuGemm p) 
   if (every) loop(std::true_type{});
   else loop(std::false_type{});
   wait_vmcnt(0);
+  if constexpr (SUMS == 2)
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+      for (int j = 0; j < FM; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][j][r] += low[i][j][r];
   // ---- epilogue, 32 x 32 at a time in registers
   f16* const __restrict__ out = s.out + mat * os;
   const int64_t olo = count * os;  // from a value's first fp16 to its second
@@ -899,17 +914,27 @@ __global__ __launch_bounds__(MP == 64 ? 512 : 1024, 1) void muon_small_kernel(Mu
     const f16x4 up = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16(LDS_PTR(h16x4, m + place(row + 4, col))));
     return __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7);
   };
-  auto multiply = [&](f32x16& acc, const f16x8 (&a)[PARTS], const f16x8 (&c)[PARTS]) {
+  // The products with a second fp16 have a sum of their own, 2^-11 of the other, whose roundings are nothing beside it.  That of
+  // two second ones is 2^-24 of a value, but of one sign on A's diagonal, which few rows show: 8 x 200 off by 0.83e-6 (0.96e-6
+  // without it, 1.08e-6 in one sum; 0.77e-6 with products of fp32) in 32 us instead of 29, 128 x 128 0.77e-6 (0.84, 1.11; 1.34).
+  auto multiply = [&](f32x16& acc, f32x16& low, const f16x8 (&a)[PARTS], const f16x8 (&c)[PARTS]) {
     acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], c[0], acc, 0, 0, 0);
     if constexpr (PARTS == 2) {
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1], c[0], acc, 0, 0, 0);
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], c[1], acc, 0, 0, 0);
+      low = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1], c[0], low, 0, 0, 0);
+      low = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], c[1], low, 0, 0, 0);
+      low = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1], c[1], low, 0, 0, 0);
     }
+  };
+  auto join = [&](f32x16& acc, const f32x16& low) {
+    if constexpr (PARTS == 2)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[r] += low[r];
   };
   // Blocks of m m^T, m [MP, K] at stride `part` between its two fp16: of a wave, with its share of the contraction.
   auto square = [&](f32x16& acc, const char* m, int part, int K) {
     const int half = HALVES == 2 ? wave / 4 : 0, block = HALVES == 2 ? wave % 4 : wave;
     const int r0 = block / (MP / 32) * 32, k0 = half * (K / HALVES), k1 = k0 + K / HALVES;
+    f32x16 low = {};
     acc = (f32x16){};
 #pragma unroll 2
     for (int k = k0; k < k1; k += 32) {  // K is a multiple of 64
@@ -922,8 +947,9 @@ __global__ __launch_bounds__(MP == 64 ? 512 : 1024, 1) void muon_small_kernel(Mu
           w[kk][q] = frag(m + q * part, block % (MP / 32) * 32 + l32, k + 16 * kk);
         }
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk) multiply(acc, w[kk], x[kk]);
+      for (int kk = 0; kk < 2; ++kk) multiply(acc, low, w[kk], x[kk]);
     }
+    join(acc, low);
     if constexpr (HALVES == 2) {  // the upper waves' shares are added to the lower ones'
       if (half)
 #pragma unroll
@@ -986,6 +1012,7 @@ __global__ __launch_bounds__(MP == 64 ? 512 : 1024, 1) void muon_small_kernel(Mu
     for (int i = 0; i < UB; ++i) {
       const int blk = wave + NW * i, rr = blk % (MP / 32) * 32, cc = blk / (MP / 32) * 32;
       if (cc >= np) continue;
+      f32x16 low = {};
       x[i] = (f32x16){};
 #pragma unroll
       for (int kk = 0; kk < MP; kk += 16) {
@@ -995,8 +1022,9 @@ __global__ __launch_bounds__(MP == 64 ? 512 : 1024, 1) void muon_small_kernel(Mu
           w[q] = frag_t(xl + q * XB, kk, cc);
           p[q] = frag(al + q * AB, rr + l32, kk);
         }
-        multiply(x[i], w, p);
+        multiply(x[i], low, w, p);
       }
+      join(x[i], low);
       combine(x[i], xl, XB, PARTS == 2 || k < MU_LO_STEPS, rr, cc, 1.f / MU_A, b.co[k][0]);
     }
     __syncthreads();
