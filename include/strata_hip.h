@@ -826,9 +826,9 @@ int strata_hip_adamw_state_values(const strata_hip_adamw_values_args* args, void
  * nothing (STRATA_HIP_EINVAL).  coefficients: a HOST array [steps, 3], which should keep singular values under 8.  At most 64
  * steps, 2^20 rows and columns, the shorter side 2^15, 2^31 elements a stack and 2^34 in all, sides counted as the
  * next multiple of 64.  workspace: strata_hip_muon_workspace() bytes of device memory (-1: sizes past these), 256-byte aligned.
- * precise 0: products of fp16 operands (the result is off by about 1e-3); 1: of operands of twice the bits, at three
- * times the cost (about 1e-6), as in calls whose matrices all have a side of at most 64.  Sums are f32, norms 64-bit; results do
- * not depend on timing.  A call whose matrices all have at most 64 x 384 or 128 x 128 takes each in one workgroup; but for
+ * bits of the products' operands: 11 (an fp16; the result is off by about 1e-3) or 22 (two, at three times the cost; about
+ * 1e-6), as in calls whose matrices all have a side of at most 64; 0: 22 where `precise`, else 11.  Sums are f32, norms 64-bit;
+ * results do not depend on timing.  A call whose matrices all have at most 64 x 384 or 128 x 128 takes each in one workgroup; but for
  * these two kinds of call a matrix's bits do not depend on the others.
  * ------------------------------------------------------------------------- */
 enum strata_hip_adjust { STRATA_HIP_ADJUST_ORIGINAL = 0, STRATA_HIP_ADJUST_MATCH_RMS_ADAMW = 1 };
@@ -844,7 +844,7 @@ typedef struct strata_hip_muon_matrix {
   int32_t param_dtype;  /* strata_hip_dtype */
   int32_t grad_dtype;
   int32_t precise;
-  int32_t reserved0;
+  int32_t bits;         /* 0, 11 or 22 */
 } strata_hip_muon_matrix;
 
 typedef struct strata_hip_muon_args {

@@ -441,7 +441,7 @@ class AdamwValuesArgs(ctypes.Structure):
 class MuonMatrix(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in ("param", "grad", "momentum", "master")] + \
         [(n, ctypes.c_int64) for n in ("batch", "rows", "cols")] + \
-        [(n, ctypes.c_double) for n in ("lr", "weight_decay")] + [(n, ctypes.c_int32) for n in ("param_dtype", "grad_dtype", "precise", "reserved0")]
+        [(n, ctypes.c_double) for n in ("lr", "weight_decay")] + [(n, ctypes.c_int32) for n in ("param_dtype", "grad_dtype", "precise", "bits")]
 
 
 class MuonArgs(ctypes.Structure):

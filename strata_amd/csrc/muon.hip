@@ -12,15 +12,15 @@
 // transposed, so that a step costs m m n + m m m + 2 m m n operations instead of 4 m m n + 2 m m m.  P X reads X along its
 // rows, transposed out of LDS (ds_read_b64_tr_b16).
 //
-// What is rounded: the products' operands are fp16, scaled by powers of two (X 2^12, A and P 2^10: there is room up to
-// 16 and 64, the usual coefficients keep them under 2 and 8; most values lie at 1 / sqrt(n), well above the 2^-14 where
-// fp16 loses bits), sums are fp32.  Singular values near 0 grow 3.4-fold a step with all the noise among them, so it is
-// the early roundings of X that show, and those of its term a X alone (P is small then): X is held as the sum of two
-// fp16, of which the products take the first, in the first two steps.  Simulated, the result is off by 0.7e-3 to 1.5e-3 for noise,
-// decaying and low-rank spectra (3.7e-3 without the second fp16, 10 to 30e-3 with iterates in bf16), below the 1.7e-3 of
-// a bf16 result's own rounding; a second fp16 in later steps gains nothing and costs 50 us of 350 a product of 133 M
-// elements.  `precise`: X, A and P are sums of two fp16 throughout and a product is three, high high, high low and low
-// high (a small matrix's low low too): off by 0.8e-6 to 2e-6, as products of fp32 are.
+// What is rounded: the products' operands are sums of two fp16 (22 bits), scaled by powers of two (X 2^12, A and P 2^10: there is
+// room up to 16 and 64, the usual coefficients keep them under 2 and 8; most values lie at 1 / sqrt(n), well above the 2^-14 where
+// fp16 loses bits), sums are fp32.  A product is three, high high, high low and low high (a small matrix's low low too): the result
+// is off by 0.8e-6 to 2e-6, as with products of fp32, which a bf16 result's rounding of 1.7e-3 hides.
+//
+// Where fewer bits are asked for, the operands are one fp16.  Singular values near 0 grow 3.4-fold a step with all the noise among
+// them, so it is the early roundings of X that show, and those of its term a X alone (P is small then): X is held as the sum of two
+// fp16, of which the products take the first, in the first two steps.  Simulated, the result is off by 0.7e-3 to 1.5e-3 for noise
+// (3.7e-3 without the second fp16, 10 to 30e-3 with iterates in bf16).
 #include <algorithm>
 #include <cmath>
 #include <exception>
@@ -1100,7 +1100,7 @@ struct MuCall {
   bool narrow = true;
   // At most 128 on it: a step is two launches (muon_slim_kernel).
   bool slim = true;
-  bool precise(const strata_hip_muon_matrix& t) const { return narrow || t.precise; }
+  bool precise(const strata_hip_muon_matrix& t) const { return narrow || (t.bits ? t.bits == 22 : t.precise); }
 };
 static MuCall mu_call(const strata_hip_muon_matrix* ts, int64_t count) {
   MuCall c;
@@ -1188,6 +1188,7 @@ static int mu_check(const std::string& n, const strata_hip_muon_args* a, bool st
     const bool p32 = t.param_dtype == STRATA_HIP_F32, g32 = t.grad_dtype == STRATA_HIP_F32;
     if ((!p32 && t.param_dtype != STRATA_HIP_BF16) || (!g32 && t.grad_dtype != STRATA_HIP_BF16))
       return fail(STRATA_HIP_EINVAL, n + ": matrices must be bf16 or f32");
+    if (t.bits != 0 && t.bits != 11 && t.bits != 22) return fail(STRATA_HIP_EINVAL, n + ": operands have 11 or 22 bits");
     if (!t.param || !t.grad || (step && !t.momentum)) return fail(STRATA_HIP_EINVAL, n + ": null tensor");
     if (!step && t.momentum) return fail(STRATA_HIP_EINVAL, n + ": a momentum is the step's");
     if (t.master && (p32 || !step)) return fail(STRATA_HIP_EINVAL, n + ": master weights are for bf16 parameters");

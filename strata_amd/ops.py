@@ -2269,10 +2269,9 @@ def orthogonalize(x: Tensor, coefficients: Sequence[float] | Sequence[Sequence[f
     for each step; they should keep singular values under 8.  The usual ones bring values from 0.001 on
     to about [0.7, 1.2], not to 1.
 
-    ``precise`` (of fp32 matrices where it is not given): the products' operands keep 22 bits, at three times the cost,
-    and the result is off by about 1e-6 of its norm; otherwise fp16 operands with fp32 sums, off by about 1e-3, less
-    than a bf16 result's own rounding (3e-3 where one direction is much stronger than all others; matrices with
-    a side of at most 64 keep 22 bits).  A matrix with a value that is not finite becomes NaN, a zero one stays zero.
+    The products' operands keep 22 bits, and the result is off by about 1e-6 of its norm before it is rounded.  ``precise=False``:
+    fp16 operands with fp32 sums, at a third of the products' cost, off by about 1e-3 (3e-3 where singular values decay over
+    several decades; matrices with a side of at most 64 keep 22 bits).  A matrix with a value that is not finite becomes NaN, a zero one stays zero.
     Not differentiable.  At most 2^20 rows and columns, 2^15 of the fewer of them."""
     flat, steps = _newton_schulz("orthogonalize", coefficients, steps, eps)
     if _eager(x):
@@ -2297,7 +2296,7 @@ def _orthogonalize(x: Tensor, coefficients: Sequence[float], eps: float, precise
     rows, cols = x.shape[-2:]
     s = x.contiguous()
     t = (_lib.MuonMatrix * 1)((out.data_ptr(), s.data_ptr(), None, None, n // (rows * cols), rows, cols, 0.0, 0.0, code, code,
-                               int(code == _lib.F32 if precise is None else precise), 0))
+                               int(precise is None or bool(precise)), 0))
     ws = _muon_space(name, t, 1, x.device)
     a = _lib.MuonArgs(t, 1, (ctypes.c_double * len(coefficients))(*coefficients), ws.data_ptr(), 0.0, float(eps),
                       len(coefficients) // 3, 0, _lib.ADJUST_ORIGINAL, 0)
@@ -2335,7 +2334,7 @@ def muon_step(params: Sequence[Tensor], grads: Sequence[Tensor], momentums: Sequ
     them: a stack of matrices, each with an update of its own (the experts' weights).  Parameters and gradients
     are bf16 or fp32, momentums fp32; ``masters`` are fp32 weights (or None) that a bf16 parameter is rounded
     from.  ``lr`` and ``weight_decay`` may be one number for every tensor; ``coefficients``, ``steps``, ``eps`` and
-    ``precise`` are ``orthogonalize``'s (where ``precise`` is not given, that of fp32 weights, masters among them).
+    ``precise`` are ``orthogonalize``'s.
     A gradient that is not finite makes its own matrix NaN.  The step's host work is proportional to the tensors; up to
     40 tensors, and 40 shapes of matrices, share a launch."""
     name = "muon_step"
@@ -2373,14 +2372,14 @@ def muon_step(params: Sequence[Tensor], grads: Sequence[Tensor], momentums: Sequ
             raise ValueError(f"{name}: {what} must be contiguous, of their parameter's shape and of {sorted(map(str, _MUON_DTYPES[what]))}")
     if min(map(len, shapes)) < 2:
         raise ValueError(f"{name}: parameters must be matrices or stacks of them, got shape {list(min(shapes, key=len))}")
-    rows = []
+    rows, bits = [], 22 if precise is None else 0  # of the operands; 0: as precise has it
     for p, g, m, w, s, r, d in zip(params, grads, momentums, masters or repeat(None), shapes, *rates):
         k = s[-2] * s[-1]
         code = _ADAMW_CODE[p.dtype]
         if w is not None and code != _lib.BF16:
             raise ValueError(f"{name}: masters belong to bfloat16 parameters")
         rows.append(_MUON_ROW(p.data_ptr(), g.data_ptr(), m.data_ptr(), 0 if w is None else w.data_ptr(), p.numel() // k if k else 0, s[-2], s[-1],
-                              r, d, code, _ADAMW_CODE[g.dtype], (code == _lib.F32 or w is not None) if precise is None else bool(precise), 0))
+                              r, d, code, _ADAMW_CODE[g.dtype], (code == _lib.F32 or w is not None) if precise is None else bool(precise), bits))
     table = (_lib.MuonMatrix * n).from_buffer_copy(b"".join(rows))
     ws = _muon_space(name, table, n, params[0].device)
     a = _lib.MuonArgs(table, n, (ctypes.c_double * len(flat))(*flat), ws.data_ptr(), float(momentum), float(eps), steps, int(nesterov),

@@ -157,8 +157,8 @@ class Muon(torch.optim.Optimizer):
     adjust      "original": updates times sqrt(max(1, rows / cols)).  "match_rms_adamw": times
                 0.2 sqrt(max(rows, cols)), as large as AdamW's, whose rates and decay then carry over.
     master      fp32 weights kept beside bf16 parameters, which are rounded from them.
-    precise     operands of 22 bits at three times the products' cost; where it is not given, for fp32 weights, masters among
-                them.  False: fp16 operands, an update off by about 1e-3 of its size.
+    precise     False: fp16 operands at a third of the products' cost, an update off by about 1e-3 of its size.  Otherwise
+                operands of 22 bits, off by about 1e-6.
 
     ``lr`` and ``weight_decay`` may differ between parameter groups, the rest is the optimizer's.  The momentum is
     fp32.  A step can be captured in a graph, after one eager step with the same gradients has made the states (the

@@ -1,0 +1,57 @@
+"""Which operands the products of orthogonalised updates take, without a GPU."""
+
+import ctypes
+
+import pytest
+import torch
+
+from oracle import optim as O
+from strata_amd import _lib, ops
+from strata_amd.optim import Muon
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    seen = []
+    monkeypatch.setattr(ops, "_launch", lambda name, a, *t: seen.append([(a.matrices[i].precise, a.matrices[i].bits) for i in range(a.count)]))
+    monkeypatch.setattr(ops, "_require_gpu", lambda *a: torch.device("cpu"))
+    return seen
+
+
+def fine(precise, bits):
+    return bits == 22 or (bits == 0 and precise == 1)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("precise", [None, True, False])
+def test_fewer_bits_are_asked_for(launches, dtype, precise):
+    """Operands of 22 bits for every type, unless the caller wants less."""
+    x = torch.zeros(200, 300, dtype=dtype)
+    ops.orthogonalize(x, precise=precise)
+    ops.muon_step([x, x.clone()], [x, x], [torch.zeros(200, 300)] * 2, precise=precise,
+                  masters=[torch.zeros(200, 300) if dtype == torch.bfloat16 else None, None])
+    p = torch.nn.Parameter(x.clone())
+    p.grad = x.clone()
+    Muon([p], master=False, precise=precise).step()
+    assert len(launches) == 3 and all(fine(*row) == (precise is not False) for call in launches for row in call)
+
+
+@pytest.mark.parametrize("bits", [-1, 1, 16, 24])
+def test_c_entries_refuse_other_bits(bits):
+    lib = _lib.load()
+    for entry, momentum in (("muon_step", 0x3000000), ("orthogonalize", None)):
+        t = (_lib.MuonMatrix * 1)((0x1000000, 0x2000000, momentum, None, 1, 136, 136, 1e-3, 0.1, _lib.BF16, _lib.BF16, 0, bits))
+        a = _lib.MuonArgs(t, 1, (ctypes.c_double * 15)(*O.NEWTON_SCHULZ * 5), 0x100, 0.95, 1e-7, 5, 1, 0, 0)
+        assert getattr(lib, "strata_hip_" + entry)(ctypes.byref(a), None) == _lib.EINVAL
+        assert "bits" in lib.strata_hip_last_error().decode()
+
+
+def test_workspace_of_operands_of_22_bits():
+    """A and P, too, are two fp16."""
+    lib = _lib.load()
+    size = {}
+    for precise, bits in ((0, 0), (0, 11), (1, 11), (0, 22), (1, 0), (1, 22)):
+        t = (_lib.MuonMatrix * 1)((0x1000000, 0x2000000, 0x3000000, None, 1, 200, 300, 1e-3, 0.1, _lib.BF16, _lib.BF16, precise, bits))
+        size[precise, bits] = lib.strata_hip_muon_workspace(t, 1)
+    assert size[0, 0] == size[0, 11] == size[1, 11] == 256 + 2 * (4 * 256 * 320 + 2 * 256 * 256)
+    assert size[0, 22] == size[1, 0] == size[1, 22] == 256 + 2 * (4 * 256 * 320 + 4 * 256 * 256)

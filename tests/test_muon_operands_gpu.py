@@ -1,0 +1,61 @@
+"""How exact orthogonalised updates are on the GPU, against their float64 oracle.
+
+``FINE`` bounds the error of operands of 22 bits relative to the result's norm.  X = x / |x| of noise has singular values that
+all grow alike, so a step's relative errors are kept and add up as independent ones: thirty roundings (five steps, of X in
+X X^T twice, of A in A A twice, of P, of X in P X), each of half a step of two fp16 (2^-22), as much for the product
+of the two second ones that is left out and as much for the fp32 sums: sqrt(30) 3 2^-22 = 3.9e-6.  Operands of 16 bits are off by
+sqrt(30) times the 0.4 of half a step 2^-16 that a rounding has in the mean: 3e-5.
+
+A result y + e of bf16 differs from y rounded only where a border of the rounding lies between them: for the error e_i the
+chance is |e_i| / step_i and the difference step_i, so that the mean of its square is step_i |e_i| <= 2^-7 |y_i| |e_i|, in all
+at most 2^-7 |y| |e|.  Twice that is asked for.
+"""
+
+import pytest
+import torch
+
+from oracle import optim as O
+from strata_amd import ops
+
+pytestmark = pytest.mark.gpu
+BF16, F32 = torch.bfloat16, torch.float32
+FINE = 4e-6
+
+
+def noise(*shape, seed=1):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed), dtype=torch.float64)
+
+
+def rounded_alike(got, want, size):
+    """Of ``got`` in bf16 and the exact ``want``, whose part that the products make has the norm ``size``."""
+    off = float((got.double() - want.to(BF16).double()).norm())
+    tol = 2 * (2.0**-7 * float(want.norm()) * FINE * size) ** 0.5
+    print(f"  {off:.2e} of {tol:.2e}", flush=True)
+    assert off <= tol
+
+
+SHAPES = [(128, 128), (70, 400), (300, 512), (600, 513), (960, 130), (40, 3000), (64, 64)]
+
+
+@pytest.mark.parametrize("rows,cols", SHAPES)
+def test_a_bf16_result_is_the_exact_one_rounded(gpu, rows, cols):
+    x = noise(rows, cols).to(BF16)
+    print(f"orthogonalize {rows} {cols}", flush=True)
+    want, _ = O.orthogonalize(x.double())
+    rounded_alike(ops.orthogonalize(x.to(gpu)).cpu(), want, float(want.norm()))
+
+
+def test_a_step_of_bf16_weights_is_the_exact_one_rounded(gpu):
+    """Weights of zero (a layer that starts as the identity's branch) are the update alone."""
+    shapes = [(300, 512), (128, 128), (512, 300), (24, 960)]
+    for start in (0.0, 0.02):
+        p = [(noise(*s, seed=2) * start).to(BF16) for s in shapes]
+        g, m = [noise(*s, seed=3).to(BF16) for s in shapes], [noise(*s, seed=4).float() for s in shapes]
+        q = [t.to(gpu) for t in p]
+        ops.muon_step(q, [t.to(gpu) for t in g], [t.to(gpu) for t in m], lr=2e-2, weight_decay=0.1, adjust="match_rms_adamw")
+        for a, b, c, d in zip(p, q, g, m):
+            want, _, _ = O.muon(a.double(), c.double(), d.double(), 2e-2, 0.95, True, 0.1, "match_rms_adamw")
+            print(f"muon {tuple(a.shape)} from {start}", flush=True)
+            # p (1 - lr decay) is off by 3 roundings of fp32 itself
+            base = a.double() * (1 - 2e-3)
+            rounded_alike(b.cpu(), want, float((want - base).norm()) + 3 * 2.0**-24 / FINE * float(base.norm()))
