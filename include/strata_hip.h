@@ -827,7 +827,7 @@ int strata_hip_adamw_state_values(const strata_hip_adamw_values_args* args, void
  * steps, 2^20 rows and columns, the shorter side 2^15, 2^31 elements a stack and 2^34 in all, sides counted as the
  * next multiple of 64.  workspace: strata_hip_muon_workspace() bytes of device memory (-1: sizes past these), 256-byte aligned.
  * bits of the products' operands: 11 (an fp16; the result is off by about 1e-3) or 22 (two, at three times the cost; about
- * 1e-6), as in calls whose matrices all have a side of at most 64; 0: 22 where `precise`, else 11.  Sums are f32, norms 64-bit;
+ * 1e-6), which matrices with a side of at most 64 always have; 0: 22 where `precise`, else 11.  Sums are f32, norms 64-bit;
  * results do not depend on timing.  A call whose matrices all have at most 64 x 384 or 128 x 128 takes each in one workgroup; but for
  * these two kinds of call a matrix's bits do not depend on the others.
  * ------------------------------------------------------------------------- */

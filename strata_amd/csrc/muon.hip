@@ -1090,24 +1090,24 @@ static int mu_small(const strata_hip_muon_matrix& t) {
   const int64_t m = std::min(t.rows, t.cols), n = std::max(t.rows, t.cols);
   return m <= 64 && n <= 128 ? 0 : m <= 64 && n <= 384 ? 1 : n <= 128 ? 2 : -1;
 }
+// Whether a matrix's operands are two fp16.  With few singular values (at most 64) one fp16's roundings do not even out: 3 to 4e-3 of
+// a row's result, 2.5e-3 of 24 x 960.  Such matrices are small beside the others of a call, and so is what three products of theirs cost.
+static bool mu_precise(const strata_hip_muon_matrix& t) {
+  return std::min(t.rows, t.cols) <= 64 || (t.bits ? t.bits == 22 : t.precise != 0);
+}
 // What a call's matrices all are.
 struct MuCall {
   // Small.  Beside others such matrices go with them, whose launches they do not lengthen (two of 128 x 128 among eight
   // matrices in fp32: 109 us; first by themselves 150).
   bool small = true;
-  // At most 64 on the shorter side: few singular values, over which fp16's roundings do not even out (4e-3 of a row's result).
-  // All of them take two fp16, which costs such a call little, its launches being mostly latency; among others they would add launches.
-  bool narrow = true;
-  // At most 128 on it: a step is two launches (muon_slim_kernel).
+  // At most 128 on the shorter side: a step is two launches (muon_slim_kernel).
   bool slim = true;
-  bool precise(const strata_hip_muon_matrix& t) const { return narrow || (t.bits ? t.bits == 22 : t.precise); }
 };
 static MuCall mu_call(const strata_hip_muon_matrix* ts, int64_t count) {
   MuCall c;
   for (int64_t i = 0; i < count; ++i) {
     if (!ts[i].rows || !ts[i].cols || !ts[i].batch) continue;
     c.small &= mu_small(ts[i]) >= 0;
-    c.narrow &= std::min(ts[i].rows, ts[i].cols) <= 64;
     c.slim &= std::min(ts[i].rows, ts[i].cols) <= 128;
   }
   return c;
@@ -1138,7 +1138,7 @@ static MuPlan mu_plan(const strata_hip_muon_matrix* ts, int64_t count) {
   std::map<std::tuple<int64_t, int64_t, bool>, int> seen;
   for (int64_t i = 0; i < count; ++i) {
     const int64_t m = std::min(ts[i].rows, ts[i].cols), n = std::max(ts[i].rows, ts[i].cols);
-    const bool precise = call.precise(ts[i]);
+    const bool precise = mu_precise(ts[i]);
     q.at.push_back(0);
     q.parts.push_back(q.sums);
     if (m <= 0 || ts[i].batch <= 0 || call.small) {
@@ -1161,7 +1161,8 @@ static MuPlan mu_plan(const strata_hip_muon_matrix* ts, int64_t count) {
     };
     for (int64_t& x : g.x) x = take(2 * g.count * g.mp * g.np);
     g.a = take((g.precise ? 2 : 1) * g.count * g.mp * g.mp);
-    g.p = take((g.precise ? 2 : 1) * g.count * g.mp * g.mp);
+    // narrow ones' P does not leave LDS in a slim call
+    g.p = call.slim && g.mp == MU_PAD ? 0 : take((g.precise ? 2 : 1) * g.count * g.mp * g.mp);
   }
   q.bytes = (q.sums * 8 + 255) / 256 * 256 + q.halves * 2;
   return q;
@@ -1319,7 +1320,7 @@ static int mu_products(const MuPlan& q, MuGemm& b, hipStream_t st, F fill) {
 }
 
 // What the kernels are told of a tensor, but for its place in the workspace.
-static MuTensor mu_tensor(const strata_hip_muon_args* a, const strata_hip_muon_matrix& t, const MuCall& call, bool step) {
+static MuTensor mu_tensor(const strata_hip_muon_args* a, const strata_hip_muon_matrix& t, bool step) {
   MuTensor o = {};
   o.p = t.param;
   o.g = t.grad;
@@ -1330,7 +1331,7 @@ static MuTensor mu_tensor(const strata_hip_muon_args* a, const strata_hip_muon_m
   const uintptr_t at = (uintptr_t)t.grad | (uintptr_t)t.momentum | (uintptr_t)t.param | (uintptr_t)t.master;
   o.flags = (t.param_dtype == STRATA_HIP_F32 ? MU_P32 : 0) | (t.grad_dtype == STRATA_HIP_F32 ? MU_G32 : 0) |
             (t.rows > t.cols ? MU_TALL : 0) | ((at & 15) || t.cols % 4 ? 0 : MU_ALIGNED) | (a->nesterov ? MU_NESTEROV : 0) |
-            (step ? MU_STEP : 0) | (call.precise(t) ? MU_LO : 0);
+            (step ? MU_STEP : 0) | (mu_precise(t) ? MU_LO : 0);
   const double adjust = a->adjust == STRATA_HIP_ADJUST_MATCH_RMS_ADAMW ? 0.2 * std::sqrt((double)std::max(t.rows, t.cols))
                                                                        : std::sqrt(std::max(1., (double)t.rows / (double)t.cols));
   o.rate = (float)(t.lr * adjust);
@@ -1339,7 +1340,7 @@ static MuTensor mu_tensor(const strata_hip_muon_args* a, const strata_hip_muon_m
 }
 
 template <int MP, int NP, int PARTS>
-static int mu_small_launch(const strata_hip_muon_args* a, const MuCall& call, int kind, bool step, hipStream_t st) {
+static int mu_small_launch(const strata_hip_muon_args* a, int kind, bool step, hipStream_t st) {
   MuSmall b;
   b.count = 0;
   b.steps = a->steps;
@@ -1357,10 +1358,10 @@ static int mu_small_launch(const strata_hip_muon_args* a, const MuCall& call, in
   };
   for (int64_t i = 0; i < a->count; ++i) {
     const strata_hip_muon_matrix& t = a->matrices[i];
-    if (!t.rows || !t.cols || !t.batch || mu_small(t) != kind || call.precise(t) != (PARTS == 2)) continue;
+    if (!t.rows || !t.cols || !t.batch || mu_small(t) != kind || mu_precise(t) != (PARTS == 2)) continue;
     if (b.count == MU_SMALL_PER || wgs + t.batch > (1 << 21))  // 1024 threads each: a grid holds less than 2^32
       if (const int rc = flush()) return rc;
-    b.t[b.count] = mu_tensor(a, t, call, step);
+    b.t[b.count] = mu_tensor(a, t, step);
     b.t[b.count++].first = wgs;
     wgs += (uint32_t)t.batch;
   }
@@ -1374,15 +1375,13 @@ static int mu_launch(const std::string& name, const strata_hip_muon_args* a, boo
     int kinds = 0;
     for (int64_t i = 0; i < a->count; ++i) {
       const strata_hip_muon_matrix& t = a->matrices[i];
-      if (t.rows && t.cols && t.batch) kinds |= 1 << (2 * mu_small(t) + call.precise(t));
+      if (t.rows && t.cols && t.batch) kinds |= 1 << (2 * mu_small(t) + mu_precise(t));
     }
     int rc = STRATA_HIP_OK;
-    if (!rc && kinds & 1) rc = mu_small_launch<64, 128, 1>(a, call, 0, step, st);
-    if (!rc && kinds & 2) rc = mu_small_launch<64, 128, 2>(a, call, 0, step, st);
-    if (!rc && kinds & 4) rc = mu_small_launch<64, 384, 1>(a, call, 1, step, st);
-    if (!rc && kinds & 8) rc = mu_small_launch<64, 384, 2>(a, call, 1, step, st);
-    if (!rc && kinds & 16) rc = mu_small_launch<128, 128, 1>(a, call, 2, step, st);
-    if (!rc && kinds & 32) rc = mu_small_launch<128, 128, 2>(a, call, 2, step, st);
+    if (kinds & 2) rc = mu_small_launch<64, 128, 2>(a, 0, step, st);
+    if (!rc && kinds & 8) rc = mu_small_launch<64, 384, 2>(a, 1, step, st);
+    if (!rc && kinds & 16) rc = mu_small_launch<128, 128, 1>(a, 2, step, st);
+    if (!rc && kinds & 32) rc = mu_small_launch<128, 128, 2>(a, 2, step, st);
     return rc;
   }
   const MuPlan q = mu_plan(a->matrices, a->count);
@@ -1415,7 +1414,7 @@ static int mu_launch(const std::string& name, const strata_hip_muon_args* a, boo
       if (b.count == MU_PER || wgs + n > (1 << 23))
         if (const int rc = flush()) return rc;
       MuTensor& o = b.t[b.count++];
-      o = mu_tensor(a, t, call, step);
+      o = mu_tensor(a, t, step);
       o.x = halves + g.x[last] + q.at[(size_t)i] * g.mp * g.np;
       o.xlo = o.x + g.count * g.mp * g.np;
       o.part = sums + q.parts[(size_t)i];
@@ -1454,8 +1453,7 @@ static int mu_launch(const std::string& name, const strata_hip_muon_args* a, boo
         update(g, s);
         s.x = halves + g.a;
       };
-      int rc = mu_slim_launch<64, 1>(q, m, st, both);
-      if (!rc) rc = mu_slim_launch<64, 2>(q, m, st, both);
+      int rc = mu_slim_launch<64, 2>(q, m, st, both);
       if (!rc) rc = mu_slim_launch<128, 1>(q, m, st, both);
       if (!rc) rc = mu_slim_launch<128, 2>(q, m, st, both);
       if (rc) return rc;

@@ -55,3 +55,17 @@ def test_workspace_of_operands_of_22_bits():
         size[precise, bits] = lib.strata_hip_muon_workspace(t, 1)
     assert size[0, 0] == size[0, 11] == size[1, 11] == 256 + 2 * (4 * 256 * 320 + 2 * 256 * 256)
     assert size[0, 22] == size[1, 0] == size[1, 22] == 256 + 2 * (4 * 256 * 320 + 4 * 256 * 256)
+
+
+def test_narrow_matrices_keep_22_bits_beside_wide_ones():
+    """Room for two fp16 of a router's A and P in a call of fp16 operands; P's only beside matrices that are not slim."""
+    lib = _lib.load()
+    row = lambda rows, cols, bits: (0x1000000, 0x2000000, 0x3000000, None, 1, rows, cols, 1e-3, 0.1, _lib.BF16, _lib.BF16, 0, bits)  # noqa: E731
+
+    def size(*rows):
+        return int(lib.strata_hip_muon_workspace((_lib.MuonMatrix * len(rows))(*rows), len(rows)))
+
+    wide, narrow = 4 * 256 * 320 + 2 * 256 * 256, 4 * 64 * 960 + 4 * 64 * 64
+    for bits in (0, 11, 22):
+        assert size(row(24, 960, bits), row(200, 300, 11)) == 256 + 2 * (wide + narrow)
+        assert size(row(24, 960, bits)) == 256 + 2 * (narrow - 2 * 64 * 64)

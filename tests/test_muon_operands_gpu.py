@@ -59,3 +59,21 @@ def test_a_step_of_bf16_weights_is_the_exact_one_rounded(gpu):
             # p (1 - lr decay) is off by 3 roundings of fp32 itself
             base = a.double() * (1 - 2e-3)
             rounded_alike(b.cpu(), want, float((want - base).norm()) + 3 * 2.0**-24 / FINE * float(base.norm()))
+
+
+@pytest.mark.parametrize("p_dtype", [BF16, F32])
+def test_narrow_matrices_beside_wide_ones_of_fewer_bits(gpu, p_dtype):
+    """A side of at most 64 keeps 22 bits whatever the call's other matrices take: routers beside the other weights of a model."""
+    narrow, wide = [(24, 960), (960, 64), (1, 700), (8, 1000)], [(300, 512), (130, 70)]
+    for shapes in (narrow + wide[:1], narrow + wide[1:], narrow + wide):
+        p = [torch.zeros(s, dtype=p_dtype, device=gpu) for s in shapes]
+        g = [noise(*s, seed=5).to(p_dtype) for s in shapes]
+        m = [noise(*s, seed=6).float() for s in shapes]
+        ops.muon_step(p, [t.to(gpu) for t in g], [t.to(gpu) for t in m], lr=1e-2, weight_decay=0.0, precise=False)
+        for i in range(len(narrow)):
+            want, _, _ = O.muon(torch.zeros(shapes[i], dtype=torch.float64), g[i].double(), m[i].double(), 1e-2, decay=0.0)
+            print(f"muon {shapes[i]} beside {shapes[4:]}", flush=True)
+            if p_dtype == BF16:
+                rounded_alike(p[i].cpu(), want, float(want.norm()))
+            else:
+                assert float((p[i].cpu().double() - want).norm()) <= FINE * float(want.norm())
