@@ -59,7 +59,7 @@ def orthogonalize(x, coefficients=(NEWTON_SCHULZ,) * 5, eps=1e-7, precise=False)
     spread and independent: the operands' (half a step of fp16, 2^-11; of two fp16 2^-22, three times that with the
     product of the two lower halves left out), sums in fp32 of K / 16 + 16 roundings of at most the norms of what they multiply,
     the fp16 parts' absolute step under 2^-14 (X is held times 2^12, A and P times 2^10).  ``precise``: two fp16
-    everywhere; otherwise for a X alone, in the first two steps."""
+    everywhere; otherwise for a X alone, in the first three steps."""
     tall = x.shape[0] > x.shape[1]
     x = x.T if tall else x
     m, n = x.shape
@@ -68,7 +68,7 @@ def orthogonalize(x, coefficients=(NEWTON_SCHULZ,) * 5, eps=1e-7, precise=False)
     op, subx, suba = (two if precise else half), 2.0**-25 / 2**12, 2.0**-25 / 2**10
     norm = torch.linalg.norm
     summed = lambda k: math.sqrt(k / 16 + 16) * 2.0**-24  # noqa: E731
-    kept = lambda k: precise or k < min(2, len(coefficients))  # noqa: E731  (X into step k, in the end the result, is two fp16)
+    kept = lambda k: precise or k < min(3, len(coefficients))  # noqa: E731  (X into step k, in the end the result, is two fp16)
     first = (two if kept(0) else half) * norm(s)
     E = torch.full((m, m), float(first) ** 2 / (m * n) + subx**2, dtype=torch.float64)
     rest = torch.full((m,), (n - m) * float(E[0, 0]), dtype=torch.float64)  # the n - m directions that x has not

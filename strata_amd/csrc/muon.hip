@@ -19,8 +19,9 @@
 //
 // Where fewer bits are asked for, the operands are one fp16.  Singular values near 0 grow 3.4-fold a step with all the noise among
 // them, so it is the early roundings of X that show, and those of its term a X alone (P is small then): X is held as the sum of two
-// fp16, of which the products take the first, in the first two steps.  Simulated, the result is off by 0.7e-3 to 1.5e-3 for noise
-// (3.7e-3 without the second fp16, 10 to 30e-3 with iterates in bf16).
+// fp16, of which the products take the first, in the first three steps.  Simulated, 512 x 600 is off by 1.3e-3 for noise and 0.9e-3,
+// 1.1e-3 and 1.3e-3 for singular values that decay over two, three and four decades (1.2, 1.4, 2.4 and 3.1e-3 with a second
+// fp16 in two steps; 10 to 30e-3 with iterates in bf16), 128 x 128 by up to 1.5e-3.
 #include <algorithm>
 #include <cmath>
 #include <exception>
@@ -39,7 +40,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 constexpr int MU_PAD = 64;       // rows and columns of a matrix in the workspace are multiples of it
 constexpr int MU_K = 32;         // columns that stand together there, row by row: X[np / 32][mp][32]
 constexpr int MU_CHUNK = 8192;   // elements a workgroup of the momentum's pass
-constexpr int MU_LO_STEPS = 2;   // steps whose X has its second fp16, where not all have
+constexpr int MU_LO_STEPS = 3;   // steps whose X has its second fp16, where not all have
 constexpr int MU_PER = 40;       // tensors a launch, and shapes: kernel arguments are 4 KiB
 constexpr float MU_X = 0x1p12f, MU_A = 0x1p10f;  // scales of X, and of A and P
 enum { MU_P32 = 1, MU_G32 = 2, MU_TALL = 4, MU_ALIGNED = 8, MU_NESTEROV = 16, MU_STEP = 32, MU_LO = 64 };

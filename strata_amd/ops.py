@@ -2270,8 +2270,8 @@ def orthogonalize(x: Tensor, coefficients: Sequence[float] | Sequence[Sequence[f
     to about [0.7, 1.2], not to 1.
 
     The products' operands keep 22 bits, and the result is off by about 1e-6 of its norm before it is rounded.  ``precise=False``:
-    fp16 operands with fp32 sums, at a third of the products' cost, off by about 1e-3 (3e-3 where singular values decay over
-    several decades; matrices with a side of at most 64 keep 22 bits).  A matrix with a value that is not finite becomes NaN, a zero one stays zero.
+    fp16 operands with fp32 sums, at a third of the products' cost, off by 1e-3 to 2e-3 (matrices with a side of at most 64
+    keep 22 bits).  A matrix with a value that is not finite becomes NaN, a zero one stays zero.
     Not differentiable.  At most 2^20 rows and columns, 2^15 of the fewer of them."""
     flat, steps = _newton_schulz("orthogonalize", coefficients, steps, eps)
     if _eager(x):
