@@ -627,7 +627,8 @@ int strata_hip_expert_route_bwd(const strata_hip_expert_route_args* args, void* 
  *   *balance = mean over sequences with n > 0 of sum over experts of f P;  *z = mean over tokens of (log-sum-exp of the logits)^2
  *   load[e] = entries of index that name e (others outside [0, experts) count nowhere), in all sequences
  * logits: [tokens, experts], row stride ld; index: [tokens, top_k] int32; state: [2 + sequences * experts] f32, kept for
- * _bwd; workspace: strata_hip_expert_balance_workspace() bytes, 8-byte aligned.  Without tokens the losses are 0.
+ * _bwd; workspace: strata_hip_expert_balance_workspace() bytes (-1: sizes past those below), 8-byte aligned.  Without tokens the losses
+ * are 0.
  * _bwd: dlogits [tokens, experts] contiguous, of the logits' type, from the losses' gradients dbalance and dz (device
  * scalars; NULL: 0) and state; index, balance, z, load and workspace are not read.  No gradient flows through load.
  * At most 512 experts and 65536 sequences.  Results do not depend on timing. */

@@ -335,17 +335,22 @@ static int64_t balance_wgs(int64_t per, int64_t sequences, int experts) {
   return std::min(most, rounds);
 }
 
+static int balance_sizes(const std::string& n, int64_t tokens, int64_t sequences, int experts, int top_k) {
+  if (tokens < 0 || sequences <= 0 || experts <= 0 || top_k <= 0)
+    return fail(STRATA_HIP_EINVAL, n + ": bad tokens, sequences, experts or top_k");
+  if (experts > ROUTE_MAX_E) return fail(STRATA_HIP_EUNSUPPORTED, n + ": at most 512 experts");
+  if (tokens > 0x7fffffff / top_k || sequences > (1 << 16))
+    return fail(STRATA_HIP_EUNSUPPORTED, n + ": more than 2^31 - 1 chosen pairs or 65536 sequences");
+  return STRATA_HIP_OK;
+}
+
 static int balance_params(const std::string& n, const strata_hip_expert_balance_args* a, BalanceParams& p) {
   if (!a) return fail(STRATA_HIP_EINVAL, n + ": null args");
-  if (a->tokens < 0 || a->sequences <= 0 || a->experts <= 0 || a->top_k <= 0)
-    return fail(STRATA_HIP_EINVAL, n + ": bad tokens, sequences, experts or top_k");
+  if (const int rc = balance_sizes(n, a->tokens, a->sequences, a->experts, a->top_k)) return rc;
   if (a->tokens % a->sequences) return fail(STRATA_HIP_EINVAL, n + ": the tokens are no whole number for each sequence");
   if (a->dtype != STRATA_HIP_F32 && a->dtype != STRATA_HIP_BF16) return fail(STRATA_HIP_EINVAL, n + ": bad dtype");
   if (a->score != STRATA_HIP_SCORE_SOFTMAX && a->score != STRATA_HIP_SCORE_SIGMOID) return fail(STRATA_HIP_EINVAL, n + ": bad score");
-  if (a->experts > ROUTE_MAX_E) return fail(STRATA_HIP_EUNSUPPORTED, n + ": at most 512 experts");
   if (a->tokens > 1 && a->ld < a->experts) return fail(STRATA_HIP_EINVAL, n + ": row stride smaller than the row");
-  if (a->tokens > 0x7fffffff / a->top_k || a->sequences > (1 << 16))
-    return fail(STRATA_HIP_EUNSUPPORTED, n + ": more than 2^31 - 1 chosen pairs or 65536 sequences");
   if (!a->state || ((uintptr_t)a->state & 3)) return fail(STRATA_HIP_EINVAL, n + ": null state");
   if (a->tokens > 0 && !a->logits) return fail(STRATA_HIP_EINVAL, n + ": null pointer");
   p = {};
@@ -389,7 +394,8 @@ static bool balance_aligned(const strata_hip_expert_balance_args* a) {
 }  // namespace strata
 
 extern "C" int64_t strata_hip_expert_balance_workspace(int64_t tokens, int64_t sequences, int32_t experts) {
-  if (tokens <= 0 || sequences <= 0 || experts <= 0) return 0;
+  if (const int rc = strata::balance_sizes("expert_balance_workspace", tokens, sequences, experts, 1)) return rc == STRATA_HIP_EUNSUPPORTED ? -1 : 0;
+  if (tokens == 0) return 0;
   return strata::balance_wgs(tokens / sequences, sequences, experts) * sequences * (12 + 8 * (int64_t)experts);
 }
 

@@ -1616,7 +1616,10 @@ def _balance_forward(logits, index, score, sequences):
     balance, z, state = new((), dtype=f32), new((), dtype=f32), new(2 + max(n, 0) * E, dtype=f32)
     load = new(E, dtype=torch.int32)
     rows = logits.numel() // max(E, 1)
-    ws = new(_lib.function("strata_hip_expert_balance_workspace")(rows, n, E), dtype=torch.uint8)
+    size = _lib.function("strata_hip_expert_balance_workspace")(rows, n, E)
+    if size < 0:
+        _lib.raise_error(name, _lib.EUNSUPPORTED)
+    ws = new(size, dtype=torch.uint8)
     a, keep = _balance_args(name, logits, index.shape[-1], score, n, state.data_ptr(), i.data_ptr(), balance.data_ptr(),
                             z.data_ptr(), load.data_ptr(), workspace=ws.data_ptr())
     _launch("strata_hip_expert_balance", a, logits)
