@@ -1583,8 +1583,7 @@ _expert_route_op.register_autograd(_route_op_backward, setup_context=_route_setu
 # ---------------------------------------------------------------------------
 # The balance of the routing
 # ---------------------------------------------------------------------------
-def _balance_args(name, logits, top_k, score, sequences, state, index=None, balance=None, z=None, load=None, dbalance=None,
-                  dz=None, dlogits=None, workspace=None):
+def _balance_args(name, logits, top_k, score, sequences, state=None, dbalance=None, dz=None, dlogits=None):
     """The structure of strata_hip_expert_balance and what it points into; state and what follows are pointers."""
     if score not in SCORES:
         raise ValueError(f"{name}: score must be one of {sorted(SCORES)}, got {score!r}")
@@ -1593,7 +1592,7 @@ def _balance_args(name, logits, top_k, score, sequences, state, index=None, bala
         raise ValueError(f"{name}: logits must be [..., experts]")
     E = logits.shape[-1]
     rows = logits.numel() // E
-    if sequences < 1 or rows % sequences:
+    if not 1 <= sequences <= max(rows, 65536) or rows % sequences:
         raise ValueError(f"{name}: {rows} tokens are no whole number for each of {sequences} sequences")
     if logits.is_contiguous():
         l2, ld = logits, E
@@ -1602,26 +1601,26 @@ def _balance_args(name, logits, top_k, score, sequences, state, index=None, bala
         if l2.stride(1) != 1 or (rows > 1 and l2.stride(0) < E):
             l2 = l2.contiguous()
         ld = l2.stride(0) if rows > 1 else E
-    return _lib.ExpertBalanceArgs(l2.data_ptr(), index, balance, z, load, state, dbalance, dz, dlogits, workspace, rows, ld, sequences,
+    return _lib.ExpertBalanceArgs(l2.data_ptr(), None, None, None, None, state, dbalance, dz, dlogits, None, rows, ld, sequences,
                                   dtype, E, top_k, SCORES[score]), l2
 
 
 def _balance_forward(logits, index, score, sequences):
     name = "expert_balance"
     dev = _require_gpu(name, logits, index)
-    if index.dtype != torch.int32 or index.dim() != logits.dim() or index.shape[:-1] != logits.shape[:-1] or not index.shape[-1]:
+    if not logits.dim() or index.dtype != torch.int32 or index.dim() != logits.dim() or index.shape[:-1] != logits.shape[:-1] \
+            or not index.shape[-1]:
         raise ValueError(f"{name}: index must be int32 {[*logits.shape[:-1], 'top_k']}, got {index.dtype} {list(index.shape)}")
     E, i, n = logits.shape[-1], index.contiguous(), operator.index(sequences)
-    new, f32 = logits.new_empty, torch.float32
-    balance, z, state = new((), dtype=f32), new((), dtype=f32), new(2 + max(n, 0) * E, dtype=f32)
-    load = new(E, dtype=torch.int32)
-    rows = logits.numel() // max(E, 1)
-    size = _lib.function("strata_hip_expert_balance_workspace")(rows, n, E)
+    a, keep = _balance_args(name, logits, index.shape[-1], score, n)
+    size = _lib.function("strata_hip_expert_balance_workspace")(a.tokens, n, E)
     if size < 0:
         _lib.raise_error(name, _lib.EUNSUPPORTED)
-    ws = new(size, dtype=torch.uint8)
-    a, keep = _balance_args(name, logits, index.shape[-1], score, n, state.data_ptr(), i.data_ptr(), balance.data_ptr(),
-                            z.data_ptr(), load.data_ptr(), workspace=ws.data_ptr())
+    new, f32 = logits.new_empty, torch.float32
+    balance, z, state = new((), dtype=f32), new((), dtype=f32), new(2 + n * E, dtype=f32)
+    load, ws = new(E, dtype=torch.int32), new(size, dtype=torch.uint8)
+    a.index, a.balance, a.z, a.load = i.data_ptr(), balance.data_ptr(), z.data_ptr(), load.data_ptr()
+    a.state, a.workspace = state.data_ptr(), ws.data_ptr()
     _launch("strata_hip_expert_balance", a, logits)
     return balance, z, load, state, a
 

@@ -35,3 +35,23 @@ def test_too_many_experts_are_refused(launches, experts):
     with pytest.raises(_lib.StrataHipError, match="512 experts"):
         ops.expert_balance(torch.zeros(3, experts), torch.zeros(3, 1, dtype=torch.int32))
     assert not launches
+
+
+@pytest.mark.parametrize("rows,sequences", [(0, 1 << 50), (0, 1 << 64), (0, (1 << 64) + 1), (6, 1 << 50), (6, -(1 << 50)), (0, 0)])
+def test_numbers_of_sequences_are_checked_before_anything_is_allocated(launches, rows, sequences):
+    with pytest.raises(ValueError, match="whole number"):
+        ops.expert_balance(torch.zeros(rows, 4), torch.zeros(rows, 1, dtype=torch.int32), sequences=sequences)
+    assert not launches
+
+
+def test_too_many_sequences_are_refused(launches):
+    with pytest.raises(_lib.StrataHipError, match="65536 sequences"):
+        ops.expert_balance(torch.zeros(65537, 2), torch.zeros(65537, 1, dtype=torch.int32), sequences=65537)
+    ops.expert_balance(torch.zeros(65536, 2), torch.zeros(65536, 1, dtype=torch.int32), sequences=65536)
+    assert launches == ["strata_hip_expert_balance"]
+
+
+def test_one_number_is_no_row_of_logits(launches):
+    with pytest.raises(ValueError, match="index must be int32"):
+        ops.expert_balance(torch.zeros(()), torch.zeros((), dtype=torch.int32))
+    assert not launches
