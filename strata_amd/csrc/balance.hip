@@ -41,6 +41,7 @@ struct BalanceParams {
   int32_t* tokens_of;  // its tokens that count
   int64_t per, ld;     // tokens of a sequence
   int64_t run;         // tokens of a workgroup
+  int64_t first;       // the launch's first token (backward)
   int experts, top_k, score, sequences, wgs_of;  // workgroups of a sequence
 };
 
@@ -270,7 +271,7 @@ template <typename T, bool VEC, bool SIGMOID, int L>
 __global__ __launch_bounds__(256) void balance_bwd_kernel(BalanceParams p) {
   constexpr int TOK = 256 / L;
   const int tid = threadIdx.x, lane = tid % L, tok = tid / L, E = p.experts, e0 = lane * BAL_EPL;
-  const int64_t t = (int64_t)blockIdx.x * TOK + tok, total = p.per * p.sequences;
+  const int64_t t = p.first + (int64_t)blockIdx.x * TOK + tok, total = p.per * p.sequences;
   const bool live = t < total;
   const int left = live ? E - e0 : 0;
   float l[BAL_EPL], s[BAL_EPL], soft[BAL_EPL], f[BAL_EPL], lse;
@@ -439,12 +440,15 @@ extern "C" int strata_hip_expert_balance_bwd(const strata_hip_expert_balance_arg
   const bool vec = balance_aligned(a) && ((uintptr_t)p.dlogits & 15) == 0 && p.experts % 8 == 0;
   return balance_width(p.experts, [&](auto lanes) {
     constexpr int L = decltype(lanes)::value, TOK = 256 / L;
-    const int64_t wgs = (a->tokens + TOK - 1) / TOK;
-    if (wgs * 256 >= 0x100000000ll) return fail(STRATA_HIP_EUNSUPPORTED, "expert_balance_bwd: problem too large for one launch");
-    balance_pick(a, vec, [&](auto t, auto v, auto s) {
-      hipLaunchKernelGGL((balance_bwd_kernel<decltype(t), decltype(v)::value, decltype(s)::value, L>), dim3((unsigned)wgs), dim3(256), 0,
-                         (hipStream_t)stream, p);
-    });
-    return check_launch("expert_balance_bwd");
+    constexpr int64_t MOST = 0xffffffff / 256;  // workgroups: a grid holds less than 2^32 threads
+    for (; p.first < a->tokens; p.first += MOST * TOK) {
+      const int64_t wgs = std::min(MOST, (a->tokens - p.first + TOK - 1) / TOK);
+      balance_pick(a, vec, [&](auto t, auto v, auto s) {
+        hipLaunchKernelGGL((balance_bwd_kernel<decltype(t), decltype(v)::value, decltype(s)::value, L>), dim3((unsigned)wgs), dim3(256), 0,
+                           (hipStream_t)stream, p);
+      });
+      if (const int rc = check_launch("expert_balance_bwd")) return rc;
+    }
+    return (int)STRATA_HIP_OK;
   });
 }
