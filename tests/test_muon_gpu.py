@@ -2,7 +2,8 @@
 
 The oracle gives, with each result, the norm of the error that the kernels' roundings make (``oracle.optim.orthogonalize``: each
 rounding counted as half a step, independent and evenly spread; simulated with the kernels' roundings, the error is a
-seventh to a half of it); the result's own rounding is half a step of its type.  The momentum is one rounded product, a rounded
+sixth to an eleventh of it with operands of one fp16, a 36th to a 370th with two: test_muon_operands_gpu has tight
+bounds); the result's own rounding is half a step of its type.  The momentum is one rounded product, a rounded
 constant each and a fused sum: 4 u of the two terms.  p (1 - lr decay) - rate o: a rounded constant, product, rate and
 result, 3 u of |p| and 3 u of the update.
 """

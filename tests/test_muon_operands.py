@@ -69,3 +69,31 @@ def test_narrow_matrices_keep_22_bits_beside_wide_ones():
     for bits in (0, 11, 22):
         assert size(row(24, 960, bits), row(200, 300, 11)) == 256 + 2 * (wide + narrow)
         assert size(row(24, 960, bits)) == 256 + 2 * (narrow - 2 * 64 * 64)
+
+
+def _off(x, cut):
+    """The error of products whose operands are an fp16 and the rest as another, of ``cut`` bits, as the kernels scale them."""
+    def two(v, scale):
+        h = (v * scale).half().double()
+        step = 2.0 ** (torch.frexp(v * scale - h)[1].double() - cut)
+        return h / scale, ((v * scale - h) / step).round() * step / scale
+
+    def product(p, q):
+        return (p[0] @ q[0] + p[1] @ q[0] + p[0] @ q[1]).float().double()
+
+    a, b, c = O.NEWTON_SCHULZ
+    want, _ = O.orthogonalize(x)
+    X = two(x / x.norm(), 2.0**12)
+    for _ in range(5):
+        A = two(product(X, (X[0].T, X[1].T)), 2.0**10)
+        P = two((b * (A[0] + A[1]) + c * product(A, A)).float().double(), 2.0**10)
+        X = two((a * (X[0] + X[1]) + product(P, X)).float().double(), 2.0**12)
+    return float((X[0] + X[1] - want).norm() / want.norm())
+
+
+@pytest.mark.parametrize("rows,cols", [(60, 90), (300, 512), (8, 1000)])
+def test_the_bound_notices_operands_of_16_bits(rows, cols):
+    """The GPU tests ask for 4e-6 of operands of 22 bits: less than half of it as the kernels round, five times as much with second
+    fp16 of four bits."""
+    x = torch.randn(rows, cols, generator=torch.Generator().manual_seed(1), dtype=torch.float64)
+    assert _off(x, 11) <= 2e-6 and _off(x, 4) >= 2e-5

@@ -98,3 +98,34 @@ def test_operands_of_11_bits_where_singular_values_decay(gpu, rows, cols):
         off = float((got - want).norm() / want.norm())
         print(f"orthogonalize {rows} {cols} over {decades} decades: {off:.2e}", flush=True)
         assert off <= 1.7e-3
+
+
+@pytest.mark.parametrize("rows,cols", [(512, 600), (300, 512), (130, 257), (128, 128), (960, 960), (200, 1500), (8, 1000), (8, 200), (384, 776), (1, 500)])
+def test_operands_of_22_bits(gpu, rows, cols):
+    """Matrices alone, in a stack, and as the steps of fp32 weights and of masters: all of one exactness."""
+    x = noise(rows, cols).float()
+    want, _ = O.orthogonalize(x.double())
+    size = float(want.norm())
+    got = {"alone": ops.orthogonalize(x.to(gpu)), "stack": ops.orthogonalize(torch.stack([x, 2 * x, x]).to(gpu))[2]}
+    zero = lambda t=F32: torch.zeros(rows, cols, dtype=t, device=gpu)  # noqa: E731
+    p, master = zero(), zero()
+    kw = dict(lr=1.0, momentum=0.0, weight_decay=0.0)
+    ops.muon_step([p], [x.to(gpu)], [zero()], **kw)
+    ops.muon_step([zero(BF16)], [x.to(gpu)], [zero()], masters=[master], **kw)
+    scale = -max(1.0, rows / cols) ** 0.5
+    got.update(weights=p / scale, masters=master / scale)
+    for what, y in got.items():
+        off = float((y.cpu().double() - want).norm()) / size
+        print(f"{rows} {cols} {what}: {off:.2e}", flush=True)
+        assert off <= FINE, what
+
+
+@pytest.mark.parametrize("rows,cols", [(8, 1000), (384, 776), (8, 200), (128, 128)])
+def test_the_second_products_have_sums_of_their_own(gpu, rows, cols):
+    """A sum of X X^T on the diagonal is of positive terms.  In one sum with the products of the second fp16 it would be rounded three
+    times as often as by itself (twice as off, 2.2e-6 of 8 x 1000): at most 2e-6 is what is documented."""
+    x = noise(rows, cols).float()
+    want, _ = O.orthogonalize(x.double())
+    off = float((ops.orthogonalize(x.to(gpu)).cpu().double() - want).norm() / want.norm())
+    print(f"{rows} {cols}: {off:.2e}", flush=True)
+    assert off <= 2e-6
