@@ -129,3 +129,69 @@ def test_the_second_products_have_sums_of_their_own(gpu, rows, cols):
     off = float((ops.orthogonalize(x.to(gpu)).cpu().double() - want).norm() / want.norm())
     print(f"{rows} {cols}: {off:.2e}", flush=True)
     assert off <= 2e-6
+
+
+def fewer_bits(got, x):
+    """``got``: the result of x with fp16 operands, within 2.1e-3 (the kernels' roundings taken on the CPU: 1.9e-3 for a side of 65,
+    less for longer ones) and its own rounding."""
+    want, _ = O.orthogonalize(x.double())
+    off = float((got.double() - want).norm() / want.norm())
+    print(f"  {tuple(x.shape)}: {off:.2e}", flush=True)
+    assert off <= (2.1e-3**2 + ((2.0**-8 / 2) ** 2 if got.dtype == BF16 else 0)) ** 0.5
+
+
+@pytest.mark.parametrize("count,rows,cols,dtype", [(100, 130, 260, BF16), (70, 512, 600, BF16), (150, 260, 300, F32), (64, 513, 400, BF16),
+                                                   (90, 384, 260, F32), (20, 960, 1920, BF16), (300, 100, 120, BF16), (40, 400, 90, F32)])
+def test_many_matrices_of_fewer_bits(gpu, count, rows, cols, dtype):
+    """Enough of them for every tile of the products of one fp16: each as alone, to the bit, and some against the oracle."""
+    g = torch.Generator(device=gpu).manual_seed(count)
+    x = torch.randn(count, rows, cols, generator=g, device=gpu).to(dtype)
+    y = ops.orthogonalize(x, precise=False)
+    for i in (0, count // 2, count - 1):
+        fewer_bits(y[i].cpu(), x[i].cpu())
+        assert torch.equal(y[i], ops.orthogonalize(x[i], precise=False))
+    assert torch.equal(ops.orthogonalize(x, precise=False), y)
+
+
+def test_offsets_past_32_bits_of_fewer_bits(gpu):
+    x = torch.empty(64000, 130, 256, dtype=BF16, device=gpu).fill_(0.5)
+    g = torch.Generator(device=gpu).manual_seed(1)
+    for i in (0, 1, 32000, 63999):
+        x[i] = torch.randn(130, 256, generator=g, device=gpu)
+    y = ops.orthogonalize(x, precise=False)
+    for i in (0, 1, 2, 32000, 63999):
+        assert torch.equal(y[i], ops.orthogonalize(x[i], precise=False)), i
+    fewer_bits(y[63999].cpu(), x[63999].cpu())
+
+
+def test_a_step_of_every_precision_at_once(gpu):
+    """Narrow, slim and wide matrices with and without masters, in steps of 22 bits, of 11 and of each by its type (the C interface's
+    ``precise`` without ``bits``): every matrix as in a call of its own, to the bit."""
+    import ctypes
+
+    from strata_amd import _lib
+
+    shapes = [(24, 960), (100, 400), (300, 512), (512, 300), (2, 130, 200), (1, 2000), (700, 130)]
+    def tensors():
+        g = torch.Generator().manual_seed(3)
+        r = lambda s: torch.randn(s, generator=g)  # noqa: E731
+        return [dict(p=(r(s) * 0.02).to(t).to(gpu), g=r(s).to(BF16).to(gpu), m=r(s).to(gpu), w=(r(s) * 0.02).to(gpu) if i % 3 == 1 else None)
+                for i, s in enumerate(shapes) for t in ((BF16,) if i % 3 == 1 else (BF16, F32))]
+
+    def step(ts, bits):
+        table = (_lib.MuonMatrix * len(ts))(*[
+            (t["p"].data_ptr(), t["g"].data_ptr(), t["m"].data_ptr(), None if t["w"] is None else t["w"].data_ptr(),
+             t["p"][..., 0, 0].numel(), *t["p"].shape[-2:], 1e-2, 0.1, int(t["p"].dtype == BF16) * _lib.BF16 + int(t["p"].dtype == F32) * _lib.F32, _lib.BF16,
+             int(t["p"].dtype == F32 or t["w"] is not None), bits) for t in ts])
+        ws = torch.empty(_lib.load().strata_hip_muon_workspace(table, len(ts)), dtype=torch.uint8, device=gpu)
+        a = _lib.MuonArgs(table, len(ts), (ctypes.c_double * 15)(*O.NEWTON_SCHULZ * 5), ws.data_ptr(), 0.95, 1e-7, 5, 1, 0, 0)
+        _lib.call("strata_hip_muon_step", a, torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+
+    for bits in (0, 11, 22):
+        ts, alone = tensors(), tensors()
+        step(ts, bits)
+        for i, (a, b) in enumerate(zip(ts, alone)):
+            step([b], bits)
+            for k in "pmw":
+                assert a[k] is None or torch.equal(a[k], b[k]), (bits, i, k)
