@@ -40,6 +40,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 constexpr int MU_PAD = 64;       // rows and columns of a matrix in the workspace are multiples of it
 constexpr int MU_K = 32;         // columns that stand together there, row by row: X[np / 32][mp][32]
 constexpr int MU_CHUNK = 8192;   // elements a workgroup of the momentum's pass
+constexpr int MU_SUMS = 1024;    // sums of squares a matrix from which on they are added up by a launch of their own
 constexpr int MU_LO_STEPS = 3;   // steps whose X has its second fp16, where not all have
 constexpr int MU_PER = 40;       // tensors a launch, and shapes: kernel arguments are 4 KiB
 constexpr float MU_X = 0x1p12f, MU_A = 0x1p10f;  // scales of X, and of A and P
@@ -152,6 +153,29 @@ __global__ __launch_bounds__(256) void muon_momentum_kernel(MuBatch b) {
   if (tid == 0) t.part[local] = ((red[0] + red[1]) + red[2]) + red[3];
 }
 
+// ---- a matrix's sums of squares, added up into the first ----
+// Every tile of the next pass adds up its matrix's sums, 1024 of them 8 KiB from L2, for which a launch would cost more.  Of more
+// than that a workgroup makes one, or the pass would read as the square of the matrix (4096 x 131072 without steps 1.7 instead of
+// 5.4 ms, 32768 x 65536 6.2 instead of 70; 4096 x 8192 0.090 and 0.094).
+__global__ __launch_bounds__(1024) void muon_norm_kernel(MuBatch b) {
+  const uint32_t wg = blockIdx.x;
+  const MuTensor& t = b.t[mu_entry(b.count, wg, [&](int i) { return b.t[i].first; })];
+  const int tid = threadIdx.x;
+  const int64_t chunks = (t.rows * t.cols + MU_CHUNK - 1) / MU_CHUNK;
+  double* const part = t.part + (wg - t.first) * chunks;
+  double s = 0.;
+#pragma unroll 8
+  for (int64_t k = tid; k < chunks; k += 1024) s += part[k];
+#pragma unroll
+  for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
+  __shared__ double red[16];
+  if ((tid & 63) == 0) red[tid >> 6] = s;
+  __syncthreads();  // every sum is read
+  if (tid) return;
+  for (int w = 1; w < 16; ++w) s += red[w];
+  part[0] = s;
+}
+
 // A tile of 64 x 64 of one matrix: `x` tile (ti, tj) of the workspace, whose source tile is the same or, of a tall
 // matrix, the transposed one.
 struct MuTile {
@@ -189,7 +213,7 @@ __global__ __launch_bounds__(256) void muon_pack_kernel(MuBatch b) {
   const int64_t n = t.rows * t.cols;
   const uint32_t chunks = (uint32_t)((n + MU_CHUNK - 1) / MU_CHUNK);
   double s = 0.;
-  for (uint32_t k = tid; k < chunks; k += 256) s += t.part[(int64_t)mat * chunks + k];
+  for (uint32_t k = tid; k < (chunks > MU_SUMS ? 1 : chunks); k += 256) s += t.part[(int64_t)mat * chunks + k];
 #pragma unroll
   for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
   if ((tid & 63) == 0) red[tid >> 6] = s;
@@ -1390,7 +1414,7 @@ static int mu_launch(const std::string& name, const strata_hip_muon_args* a, boo
   f16* const halves = (f16*)((char*)a->workspace + (q.sums * 8 + 255) / 256 * 256);
   int last = 0;  // which X a pass reads or writes
 
-  // kind 0: momentum and sums, 1: X, 2: the update
+  // kind 0: momentum and sums, 1: X, 2: the update, 3: the sums of matrices that have many
   auto tensors = [&](int kind) -> int {
     MuBatch b;
     b.count = 0;
@@ -1401,6 +1425,7 @@ static int mu_launch(const std::string& name, const strata_hip_muon_args* a, boo
     auto flush = [&]() -> int {
       if (!b.count) return STRATA_HIP_OK;
       if (kind == 0) hipLaunchKernelGGL(muon_momentum_kernel, dim3(wgs), dim3(256), 0, st, b);
+      else if (kind == 3) hipLaunchKernelGGL(muon_norm_kernel, dim3(wgs), dim3(1024), 0, st, b);
       else if (kind == 1) hipLaunchKernelGGL(muon_pack_kernel, dim3(wgs), dim3(256), 0, st, b);
       else hipLaunchKernelGGL(muon_apply_kernel, dim3(wgs), dim3(256), 0, st, b);
       b.count = 0;
@@ -1411,7 +1436,8 @@ static int mu_launch(const std::string& name, const strata_hip_muon_args* a, boo
       if (q.of[(size_t)i] < 0) continue;
       const strata_hip_muon_matrix& t = a->matrices[i];
       const MuGroup& g = q.groups[(size_t)q.of[(size_t)i]];
-      const int64_t per = kind == 0 ? mu_chunks(t) : (g.mp / 64) * (g.np / 64), n = per * t.batch;
+      if (kind == 3 && mu_chunks(t) <= MU_SUMS) continue;
+      const int64_t per = kind == 0 ? mu_chunks(t) : kind == 3 ? 1 : (g.mp / 64) * (g.np / 64), n = per * t.batch;
       if (b.count == MU_PER || wgs + n > (1 << 23))
         if (const int rc = flush()) return rc;
       MuTensor& o = b.t[b.count++];
@@ -1427,6 +1453,7 @@ static int mu_launch(const std::string& name, const strata_hip_muon_args* a, boo
   };
 
   if (const int rc = tensors(0)) return rc;
+  if (const int rc = tensors(3)) return rc;
   if (const int rc = tensors(1)) return rc;
   MuGemm b;
   for (int k = 0; k < a->steps; ++k) {
