@@ -73,9 +73,9 @@ class AdamW(torch.optim.Optimizer):
             blocks = -(-n // ops.STATE_BLOCK)
             s["exp_avg"] = torch.zeros(p.shape, dtype=torch.int8, device=p.device)
             s["exp_avg_sq"] = torch.zeros(p.shape, dtype=torch.uint8, device=p.device)
-            s["exp_avg_scale"], s["exp_avg_sq_scale"] = torch.zeros(2, blocks, device=p.device).unbind()
+            s["exp_avg_scale"], s["exp_avg_sq_scale"] = torch.zeros(2, blocks, dtype=torch.float32, device=p.device).unbind()
         else:
-            s["exp_avg"], s["exp_avg_sq"] = (torch.zeros(p.shape, device=p.device) for _ in range(2))
+            s["exp_avg"], s["exp_avg_sq"] = (torch.zeros(p.shape, dtype=torch.float32, device=p.device) for _ in range(2))
         if self.master and p.dtype == torch.bfloat16:
             s["master"] = p.detach().float()
         return s
@@ -212,7 +212,7 @@ class Muon(torch.optim.Optimizer):
         for p in ps:
             if not self.state[p]:
                 _uncaptured("Muon")
-                self.state[p]["momentum"] = torch.zeros(p.shape, device=p.device)
+                self.state[p]["momentum"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
                 if self.master and p.dtype == torch.bfloat16:
                     self.state[p]["master"] = p.detach().float()
         states = [self.state[p] for p in ps]

@@ -1,0 +1,34 @@
+"""The optimizers' states and arguments, without a GPU."""
+
+import pytest
+import torch
+
+from strata_amd import ops
+from strata_amd.optim import AdamW, Muon
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    seen = []
+    monkeypatch.setattr(ops, "_launch", lambda name, *a: seen.append(name))
+    monkeypatch.setattr(ops, "_require_gpu", lambda *a: torch.device("cpu"))
+    return seen
+
+
+@pytest.mark.parametrize("default", [torch.bfloat16, torch.float64, torch.float16])
+def test_states_are_fp32_whatever_torch_makes_by_default(launches, default):
+    """A model built under ``torch.set_default_dtype`` steps all the same."""
+    before = torch.get_default_dtype()
+    try:
+        torch.set_default_dtype(default)
+        for make in (Muon, AdamW, lambda ps: AdamW(ps, state_bits=8, min_8bit=1)):
+            for dtype in (torch.bfloat16, torch.float32):
+                p = torch.nn.Parameter(torch.ones(4, 300, dtype=dtype))
+                p.grad = torch.ones_like(p)
+                opt = make([p])
+                opt.step()
+                state = {k: v.dtype for k, v in opt.state[p].items() if k != "step"}
+                assert set(state.values()) <= {torch.float32, torch.int8, torch.uint8}, state
+    finally:
+        torch.set_default_dtype(before)
+    assert len(launches) == 6
