@@ -2229,7 +2229,7 @@ NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
 
 def _newton_schulz(name: str, coefficients, steps: Optional[int], eps: float):
     """A ctypes array of the steps' triples, and how many."""
-    rows = list(coefficients)
+    rows, steps = list(coefficients), None if steps is None else operator.index(steps)
     if not rows or not isinstance(rows[0], (int, float)):
         if steps is not None and steps != len(rows):
             raise ValueError(f"{name}: {len(rows)} triples of coefficients for {steps} steps")
@@ -2240,7 +2240,7 @@ def _newton_schulz(name: str, coefficients, steps: Optional[int], eps: float):
     else:
         if len(rows) != 3:
             raise ValueError(f"{name}: coefficients must be three numbers, or three for each step")
-        steps = 5 if steps is None else int(steps)
+        steps = 5 if steps is None else steps
         flat = [float(c) for c in rows] * max(steps, 0)
     if not 0 <= steps <= 64:
         raise ValueError(f"{name}: between 0 and 64 steps, got {steps}")

@@ -171,9 +171,10 @@ class Muon(torch.optim.Optimizer):
             raise ValueError(f"Muon: adjust must be one of {sorted(ops.ADJUSTS)}, got {adjust!r}")
         if not 0.0 <= momentum < 1.0:
             raise ValueError(f"Muon: momentum must lie in [0, 1), got {momentum}")
+        coefficients = tuple(coefficients)
         ops._newton_schulz("Muon", coefficients, steps, eps)
         self.momentum, self.nesterov, self.adjust, self.eps = float(momentum), bool(nesterov), adjust, float(eps)
-        self.coefficients, self.steps, self.master, self.precise = tuple(coefficients), steps, master, precise
+        self.coefficients, self.steps, self.master, self.precise = coefficients, steps, master, precise
         super().__init__(params, dict(lr=lr, weight_decay=weight_decay))
 
     _OWN = ("momentum", "nesterov", "adjust", "eps", "coefficients", "steps", "master", "precise")

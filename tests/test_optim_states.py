@@ -32,3 +32,19 @@ def test_states_are_fp32_whatever_torch_makes_by_default(launches, default):
     finally:
         torch.set_default_dtype(before)
     assert len(launches) == 6
+
+
+def test_coefficients_that_can_be_read_once(launches):
+    """An iterator's triples are the optimizer's, not the check's alone."""
+    p = torch.nn.Parameter(torch.ones(4, 6))
+    opt = Muon([p], coefficients=iter([(1.5, -0.5, 0.0)] * 3))
+    assert opt.coefficients == ((1.5, -0.5, 0.0),) * 3
+
+
+@pytest.mark.parametrize("steps", [2.7, 3.0, "3"])
+def test_a_fraction_of_a_step_is_refused(launches, steps):
+    x = torch.ones(4, 6)
+    for call in (lambda: ops.orthogonalize(x, steps=steps), lambda: ops.muon_step([x], [x], [x], steps=steps), lambda: Muon([torch.nn.Parameter(x)], steps=steps)):
+        with pytest.raises(TypeError, match="integer"):
+            call()
+    assert not launches
