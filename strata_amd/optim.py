@@ -234,12 +234,16 @@ class Muon(torch.optim.Optimizer):
 
 def matrices(module: nn.Module) -> tuple[list[nn.Parameter], list[nn.Parameter]]:
     """A module's parameters as ``(matrices, rest)``, each in the module's order: the weights of its
-    ``nn.Linear`` and the stacked weights of its ``ExpertMlp``; and all others, for ``AdamW``."""
-    some = set()
+    ``nn.Linear`` (one that an embedding shares stays with the rest) and the stacked weights of its
+    ``ExpertMlp``; and all others, for ``AdamW``."""
+    some, tables = set(), set()
     for m in module.modules():
         if isinstance(m, nn.Linear):
             some.add(m.weight)
         elif isinstance(m, ExpertMlp):
             some |= {m.w1, m.w2}
+        elif isinstance(m, (nn.Embedding, nn.EmbeddingBag)):
+            tables.add(m.weight)
+    some -= tables
     every = list(module.parameters())
     return [p for p in every if p in some], [p for p in every if p not in some]

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from strata_amd import ops
-from strata_amd.optim import AdamW, Muon
+from strata_amd.optim import AdamW, Muon, matrices
 
 
 @pytest.fixture
@@ -48,3 +48,10 @@ def test_a_fraction_of_a_step_is_refused(launches, steps):
         with pytest.raises(TypeError, match="integer"):
             call()
     assert not launches
+
+
+def test_an_embedding_that_a_linear_layer_shares_is_no_matrix():
+    net = torch.nn.ModuleList([torch.nn.Linear(6, 8, bias=False), torch.nn.Embedding(9, 6), torch.nn.Linear(6, 9, bias=False)])
+    net[2].weight = net[1].weight
+    some, rest = matrices(net)
+    assert [p is q for p, q in zip(some + rest, (net[0].weight, net[1].weight))] == [True, True] and len(some) == len(rest) == 1
