@@ -12,8 +12,8 @@
 //
 // A lane holds 8 consecutive experts of a token and L lanes a token, so that a token's row is read in 16-byte runs
 // and needs log2(L) exchanges.  A workgroup takes a run of one sequence's tokens and leaves an fp32 sum of scores and
-// a load for every expert; one workgroup adds these up in 64 bits, in an order fixed by the sizes.  Loads are integers,
-// so that LDS atomics may add them in any order.
+// a load for every expert; one workgroup (of many sequences one for each 64, and another one) adds these up in 64 bits, in an order
+// fixed by the sizes.  Loads are integers, so that LDS atomics may add them in any order.
 //
 // Bound by the operations, exponentials of 32 bits (five an element with sigmoid scores), and for few tokens by the three
 // launches: 65536 tokens of 64 experts in fp32 28 us for the sums (0.6 TB/s), 16 to add 512 workgroups' up, 29 for the gradient
@@ -39,6 +39,9 @@ struct BalanceParams {
   int32_t* counts;  // its loads [wgs, experts]
   double* zs;       // its sum of lse^2
   int32_t* tokens_of;  // its tokens that count
+  double* balances;    // of more than BAL_GROUP sequences: a finishing workgroup's sum over them,
+  int32_t* counted;    // its sequences that count,
+  int32_t* loads;      // and its load [finishing workgroups, experts]
   int64_t per, ld;     // tokens of a sequence
   int64_t run;         // tokens of a workgroup
   int64_t first;       // the launch's first token (backward)
@@ -46,6 +49,7 @@ struct BalanceParams {
 };
 
 constexpr int BAL_EPL = 8;
+constexpr int BAL_GROUP = 64;  // sequences that one workgroup adds up
 constexpr float BAL_NONE = -__builtin_inff();
 
 // The token's scores and log-sum-exp from its logits (-inf where masked); soft: the softmax, where it is not the score.
@@ -156,24 +160,19 @@ __global__ __launch_bounds__(256) void balance_stats_kernel(BalanceParams p) {
   }
 }
 
-// The workgroups' sums added up: a sequence is taken by 16 / (sequences, rounded up to a power of two) waves, one at least,
-// that share its workgroups; a lane takes every 64th expert.
-__global__ __launch_bounds__(1024) void balance_finish_kernel(BalanceParams p) {
-  constexpr int NW = 16, EL = ROUTE_MAX_E / 64;
-  __shared__ double sum[NW][ROUTE_MAX_E];
-  __shared__ int cnt[NW][ROUTE_MAX_E];
-  __shared__ int load[ROUTE_MAX_E];
-  __shared__ double zred[NW], each[NW];
+// The sum of lse^2 and the tokens that count, over all workgroups: valid in thread 0.
+struct BalanceTotals {
+  double z;
+  int64_t n;
+};
+__device__ __forceinline__ BalanceTotals balance_totals(const BalanceParams& p) {
+  constexpr int NW = 16;
+  __shared__ double zred[NW];
   __shared__ int64_t nred[NW];
-  __shared__ int some[NW];
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, E = p.experts, G = p.sequences;
-  int slots = 1;  // sequences at a time
-  while (slots < G && slots < NW) slots *= 2;
-  const int per = NW / slots, share = wave % per, slot = wave / per;
-  for (int e = tid; e < E; e += 1024) load[e] = 0;
+  const int tid = threadIdx.x;
   double z = 0.;
   int64_t n = 0;
-  for (int b = tid; b < G * p.wgs_of; b += 1024) {
+  for (int b = tid; b < p.sequences * p.wgs_of; b += 1024) {
     z += p.zs[b];
     n += p.tokens_of[b];
   }
@@ -182,13 +181,45 @@ __global__ __launch_bounds__(1024) void balance_finish_kernel(BalanceParams p) {
     z += __shfl_xor(z, d);
     n += __shfl_xor(n, d);
   }
-  if (lane == 0) {
-    zred[wave] = z;
-    nred[wave] = n;
+  if ((tid & 63) == 0) {
+    zred[tid >> 6] = z;
+    nred[tid >> 6] = n;
   }
+  __syncthreads();
+  if (tid == 0)
+    for (int w = 1; w < NW; ++w) {
+      z += zred[w];
+      n += nred[w];
+    }
+  return {z, n};
+}
+__device__ __forceinline__ void balance_results(const BalanceParams& p, double balance, int counted, BalanceTotals t) {
+  const double ig = counted ? 1. / counted : 0., in = t.n ? 1. / (double)t.n : 0.;
+  *p.balance = (float)(balance * ig);
+  *p.z = (float)(t.z * in);
+  p.state[0] = (float)ig;
+  p.state[1] = (float)(2. * in);
+}
+
+// The workgroups' sums added up, of BAL_GROUP sequences a workgroup: a sequence is taken by 16 / (sequences, rounded up to a power
+// of two) waves, one at least, that share its workgroups; a lane takes every 64th expert.  16 sequences take 2.6 us: 65536
+// tokens of 64 experts in 1024 sequences 185 us by one workgroup, 41 by several, in 65536 10600 and 214; 8192 tokens in 128 46 and 37.
+__global__ __launch_bounds__(1024) void balance_finish_kernel(BalanceParams p) {
+  constexpr int NW = 16, EL = ROUTE_MAX_E / 64;
+  __shared__ double sum[NW][ROUTE_MAX_E];
+  __shared__ int cnt[NW][ROUTE_MAX_E];
+  __shared__ int load[ROUTE_MAX_E];
+  __shared__ double each[NW];
+  __shared__ int some[NW];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, E = p.experts;
+  const int first = blockIdx.x * BAL_GROUP, G = gridDim.x == 1 ? p.sequences : min(p.sequences, first + BAL_GROUP);
+  int slots = 1;  // sequences at a time
+  while (slots < G - first && slots < NW) slots *= 2;
+  const int per = NW / slots, share = wave % per, slot = wave / per;
+  for (int e = tid; e < E; e += 1024) load[e] = 0;
   double balance = 0.;  // thread 0
   int counted = 0;
-  for (int g0 = 0; g0 < G; g0 += slots) {
+  for (int g0 = first; g0 < G; g0 += slots) {
     const int g = g0 + slot;
     double a[EL];
     int c[EL];
@@ -253,17 +284,51 @@ __global__ __launch_bounds__(1024) void balance_finish_kernel(BalanceParams p) {
       }
   }
   __syncthreads();
-  for (int e = tid; e < E; e += 1024) p.load[e] = load[e];
+  int32_t* const loads = gridDim.x == 1 ? p.load : p.loads + (int64_t)blockIdx.x * E;
+  for (int e = tid; e < E; e += 1024) loads[e] = load[e];
+  if (gridDim.x == 1) {  // uniform
+    const BalanceTotals t = balance_totals(p);
+    if (tid == 0) balance_results(p, balance, counted, t);
+  } else if (tid == 0) {
+    p.balances[blockIdx.x] = balance;
+    p.counted[blockIdx.x] = counted;
+  }
+}
+
+// What the finishing workgroups (at most 1024) have, added up.
+__global__ __launch_bounds__(1024) void balance_join_kernel(BalanceParams p) {
+  constexpr int NW = 16;
+  __shared__ int load[ROUTE_MAX_E];
+  __shared__ double bred[NW];
+  __shared__ int cred[NW];
+  const int tid = threadIdx.x, E = p.experts, groups = (p.sequences + BAL_GROUP - 1) / BAL_GROUP;
+  if (tid < ROUTE_MAX_E) load[tid] = 0;
+  double balance = tid < groups ? p.balances[tid] : 0.;
+  int counted = tid < groups ? p.counted[tid] : 0;
+#pragma unroll
+  for (int d = 32; d; d >>= 1) {
+    balance += __shfl_xor(balance, d);
+    counted += __shfl_xor(counted, d);
+  }
+  if ((tid & 63) == 0) {
+    bred[tid >> 6] = balance;
+    cred[tid >> 6] = counted;
+  }
+  __syncthreads();
+  int k = 0;  // an expert's share of the workgroups, of those that 1024 threads hold at once
+  const int at = tid % E, shares = 1024 / E, share = tid / E;
+  if (share < shares)
+#pragma unroll 8
+    for (int g = share; g < groups; g += shares) k += p.loads[(int64_t)g * E + at];
+  if (share < shares) atomicAdd(&load[at], k);
+  const BalanceTotals t = balance_totals(p);
+  if (tid < E) p.load[tid] = load[tid];  // a barrier behind the last of them
   if (tid == 0) {
     for (int w = 1; w < NW; ++w) {
-      z += zred[w];
-      n += nred[w];
+      balance += bred[w];
+      counted += cred[w];
     }
-    const double ig = counted ? 1. / counted : 0., in = n ? 1. / (double)n : 0.;
-    *p.balance = (float)(balance * ig);
-    *p.z = (float)(z * in);
-    p.state[0] = (float)ig;
-    p.state[1] = (float)(2. * in);
+    balance_results(p, balance, counted, t);
   }
 }
 
@@ -336,6 +401,11 @@ static int64_t balance_wgs(int64_t per, int64_t sequences, int experts) {
   return std::min(most, rounds);
 }
 
+// Workgroups that add up sequences for one more: none where one does it all.
+static int64_t balance_groups(int64_t sequences) {
+  return sequences > BAL_GROUP ? (sequences + BAL_GROUP - 1) / BAL_GROUP : 0;
+}
+
 static int balance_sizes(const std::string& n, int64_t tokens, int64_t sequences, int experts, int top_k) {
   if (tokens < 0 || sequences <= 0 || experts <= 0 || top_k <= 0)
     return fail(STRATA_HIP_EINVAL, n + ": bad tokens, sequences, experts or top_k");
@@ -397,7 +467,8 @@ static bool balance_aligned(const strata_hip_expert_balance_args* a) {
 extern "C" int64_t strata_hip_expert_balance_workspace(int64_t tokens, int64_t sequences, int32_t experts) {
   if (const int rc = strata::balance_sizes("expert_balance_workspace", tokens, sequences, experts, 1)) return rc == STRATA_HIP_EUNSUPPORTED ? -1 : 0;
   if (tokens == 0) return 0;
-  return strata::balance_wgs(tokens / sequences, sequences, experts) * sequences * (12 + 8 * (int64_t)experts);
+  return strata::balance_wgs(tokens / sequences, sequences, experts) * sequences * (12 + 8 * (int64_t)experts) +
+         strata::balance_groups(sequences) * (12 + 4 * (int64_t)experts);
 }
 
 extern "C" int strata_hip_expert_balance(const strata_hip_expert_balance_args* a, void* stream) {
@@ -406,14 +477,18 @@ extern "C" int strata_hip_expert_balance(const strata_hip_expert_balance_args* a
   if (const int rc = balance_params("expert_balance", a, p)) return rc;
   if (!p.balance || !p.z || !p.load) return fail(STRATA_HIP_EINVAL, "expert_balance: null pointer");
   const hipStream_t st = (hipStream_t)stream;
+  const int64_t groups = a->tokens > 0 ? balance_groups(p.sequences) : 0;  // (without tokens all are 0)
   if (a->tokens > 0) {
     if (!p.index || !a->workspace || ((uintptr_t)a->workspace & 7))
       return fail(STRATA_HIP_EINVAL, "expert_balance: index and workspace must be given, the workspace 8-byte aligned");
     p.wgs_of = (int)balance_wgs(p.per, p.sequences, p.experts);
     const int64_t wgs = (int64_t)p.wgs_of * p.sequences;
     p.zs = (double*)a->workspace;
-    p.tokens_of = (int32_t*)(p.zs + wgs);
-    p.sums = (float*)(p.tokens_of + wgs);
+    p.balances = p.zs + wgs;
+    p.tokens_of = (int32_t*)(p.balances + groups);
+    p.counted = p.tokens_of + wgs;
+    p.loads = p.counted + groups;
+    p.sums = (float*)(p.loads + groups * p.experts);
     p.counts = (int32_t*)(p.sums + wgs * p.experts);
     const int rc = balance_width(p.experts, [&](auto lanes) {
       constexpr int L = decltype(lanes)::value, TOK = 256 / L;
@@ -427,8 +502,11 @@ extern "C" int strata_hip_expert_balance(const strata_hip_expert_balance_args* a
     });
     if (rc) return rc;
   }
-  hipLaunchKernelGGL(balance_finish_kernel, dim3(1), dim3(1024), 0, st, p);
-  return check_launch("expert_balance sums");
+  hipLaunchKernelGGL(balance_finish_kernel, dim3((unsigned)std::max<int64_t>(groups, 1)), dim3(1024), 0, st, p);
+  if (const int rc = check_launch("expert_balance sums")) return rc;
+  if (!groups) return STRATA_HIP_OK;
+  hipLaunchKernelGGL(balance_join_kernel, dim3(1), dim3(1024), 0, st, p);
+  return check_launch("expert_balance joined sums");
 }
 
 extern "C" int strata_hip_expert_balance_bwd(const strata_hip_expert_balance_args* a, void* stream) {
