@@ -16,8 +16,8 @@
 // fixed by the sizes.  Loads are integers, so that LDS atomics may add them in any order.
 //
 // Bound by the operations, exponentials of 32 bits (five an element with sigmoid scores), and for few tokens by the three
-// launches: 65536 tokens of 64 experts in fp32 28 us for the sums (0.6 TB/s), 16 to add 512 workgroups' up, 29 for the gradient
-// (1.2 TB/s); 1350 of 24 in bf16 6.5, 5.4 and 4.5.  A call's host path is 17 us, with its backward through autograd 96, so a
+// launches: 65536 tokens of 64 experts in fp32 27 us for the sums (0.6 TB/s), 17 to add 512 workgroups' up, 29 for the gradient
+// (1.2 TB/s); 1350 of 24 in bf16 6.4, 5.8 and 4.2.  A call's host path is 17 us, with its backward through autograd 96, so a
 // training step meets the kernels' time only where it is captured or the GPU lags behind.
 #include <algorithm>
 

@@ -400,10 +400,10 @@ __device__ __forceinline__ void mu_wait() {  // all but the last N copies have l
 // NST stages of MU_K columns (buffer_load ... lds); the fragments of 16 columns are read while those before them
 // multiply, over the stages' borders too, so stage kt + 1 has landed when kt begins.
 // Bound by the matrix instructions and the power that they draw (the clock falls from 2.4 to 1.8 GHz): 48 matrices 960 x 960 to 960 x
-// 3840, P X 312 us (814 TFLOP/s; a library product of 960 x 960 x 3840 by 12 910, of 8192^3 1216), X X^T 178 us (716 of the
-// half that is needed; 256 x 256 tiles on the diagonal and the edge are 42% more, of which 32 x 32 blocks that nobody writes are
-// left out: 209 -> 194 us in a whole step, P X 385 -> 371); 79% of a 256 x 256 tile's cycles in the
-// loop issue them, its start and epilogue are 26% of P X.  128 x 128 tiles wait for L2 (16 KiB a stage of 256 cycles); of two fp16
+// 3840 of two fp16, P X 853 us (896 TFLOP/s of what it multiplies), X X^T 539; of one fp16 P X 312 us (814 TFLOP/s; a library
+// product of 960 x 960 x 3840 by 12 910, of 8192^3 1216), X X^T 178 us (716 of the half that is needed; 256 x 256 tiles on the diagonal
+// and the edge are 42% more, of which 32 x 32 blocks that nobody writes are left out: 209 -> 194 us in a whole step, P X 385 -> 371);
+// 79% of a 256 x 256 tile's cycles in the loop issue them, its start and epilogue are 26% of P X.  128 x 128 tiles wait for L2 (16 KiB a stage of 256 cycles); of two fp16
 // they multiply three times and do not; there P X takes two stages only, so that another tile of the CU multiplies during
 // one's start and epilogue (24 matrices of 640 columns 140 us, with five stages and one tile a CU 163; X X^T with its longer
 // contraction 98 and 87).
@@ -813,9 +813,9 @@ __global__ __launch_bounds__(512, 1) void muon_slim_kernel(MuSlim p) {
 
 // ---- small matrices: the whole step in one workgroup and launch ----
 // X (as two fp16) and A, which P takes the place of, stay in LDS, in the workspace's layout.  Sixteen waves take a 32 x 32
-// block of a product of 128 x 128 each (eight take two: 30 us), eight one of 64 x 64 with half of the contraction.  Bound by
-// latencies and the conversions of the results: 128 x 128 alone 24 us (eighteen launches: 77), of which a step is 8300 cycles with 3
-// x 1024 of matrix instructions, and 16000 go into u, its norm and the result.
+// block of a product of 128 x 128 each (eight take two: 30 us, of one fp16), eight one of 64 x 64 with half of the contraction.  Bound by
+// latencies and the conversions of the results: 128 x 128 alone 49 us, of one fp16 24 (eighteen launches: 77), of which a step is
+// 8300 cycles with 3 x 1024 of matrix instructions, and 16000 go into u, its norm and the result.
 constexpr int MU_SMALL_PER = 32;  // tensors a launch
 struct MuSmall {
   MuTensor t[MU_SMALL_PER];
@@ -1140,7 +1140,7 @@ static MuCall mu_call(const strata_hip_muon_matrix* ts, int64_t count) {
 static int64_t mu_chunks(const strata_hip_muon_matrix& t) { return (t.rows * t.cols + MU_CHUNK - 1) / MU_CHUNK; }
 static int64_t mu_up(int64_t n) { return (n + MU_PAD - 1) / MU_PAD * MU_PAD; }
 
-// The sizes that the kernels' indexes and grids hold: at most 2^23 tiles of 64 x 64 a tensor.
+// The sizes that the kernels' indexes and grids hold: at most 2^22 tiles of 64 x 64 in all.
 static int mu_sizes(const std::string& n, const strata_hip_muon_matrix* ts, int64_t count) {
   int64_t tiles = 0;
   for (int64_t i = 0; i < count; ++i) {
